@@ -129,6 +129,12 @@ _SIGNATURES = {
         "qt_attention_prefill_mma": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
                                      _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_float, _c_int, _c_ptr],
     },
+    "attention_shared": {
+        # q, k_cache, v_cache, out, dtype, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, nq, nkv, d, page_tokens, n_pages,
+        # scale, shared_ranges, own_ranges, part_acc, part_ml, stream
+        "qt_attention_decode_shared": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                                       _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr],
+    },
     "attention_tc": {
         "qt_attention_prefill_tc": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int,
                                     _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_float, _c_int, _c_ptr, _c_ptr],
@@ -172,6 +178,10 @@ _SIGNATURES = {
         "qt_sample": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
         "qt_sample_keyed": [_c_ptr, _c_float, _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_float, _c_ptr],
         "qt_feed_tokens": [_c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr],
+    },
+    "sampling_filtered": {
+        # logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, rows, vocab, stream
+        "qt_sample_filtered": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
     },
 }
 _BOUND: dict[str, ctypes._CFuncPtr] = {}
@@ -1373,6 +1383,83 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
               int(chunk or 0), v_cache.shape[1], int(keep_first), 1 if sink else 0, v_cache.shape[-1], _ptr(sinks), cap, _stream(), launches=launches)
 
 
+# ----------------------------------------------------------------------------- attention over a shared prefix
+@dataclass(frozen=True)
+class SharedPlan:
+    """How ``attention_decode_shared`` cuts its work (``shared_plan`` makes one from the sizes a caller knows on the host).  The same plan serves every
+    call whose sizes do not exceed those it was made for; the lengths themselves are read on the device."""
+
+    n_seqs: int
+    num_heads: int
+    num_kv_heads: int
+    head_dim: int
+    dtype: torch.dtype
+    groups: int
+    most_members: int
+    shared_ranges: int            # ranges that a group's shared keys are cut into
+    own_ranges: int               # ranges that a member's own keys are cut into
+
+    @property
+    def ranges(self) -> int:
+        return self.shared_ranges + self.own_ranges
+
+    @property
+    def acc_elements(self) -> int:
+        """Elements of ``part_acc`` (float)."""
+        return self.n_seqs * self.num_heads * self.ranges * self.head_dim
+
+    @property
+    def ml_elements(self) -> int:
+        """Elements of ``part_ml`` (float)."""
+        return self.n_seqs * self.num_heads * self.ranges * 2
+
+
+def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, groups: int, most_members: int,
+                most_shared: int, most_own: int, sms: int | None = None) -> SharedPlan:
+    """The cut for ``n_seqs`` sequences in ``groups`` groups of at most ``most_members``, a shared length of at most ``most_shared`` tokens and at most
+    ``most_own`` tokens of a member's own.  ``sms``: streaming multiprocessors (default: the current device's)."""
+    if n_seqs < 0 or groups < 1 or not 0 <= most_members <= n_seqs or most_shared < 0 or most_own < 0:
+        raise KernelError(f"shared_plan: {n_seqs} sequences in {groups} groups of at most {most_members}, {most_shared} and {most_own} tokens")
+    if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or head_dim < 1 or dtype not in _CODES:
+        raise KernelError(f"shared_plan: {num_heads} heads over {num_kv_heads} of {head_dim} in {dtype}")
+    shared_ranges = max(1, min(32, -(-most_shared // 128)))
+    own_ranges = max(1, min(8, -(-most_own // 256)))
+    return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges)
+
+
+def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
+                            seq_len: torch.Tensor, members: torch.Tensor, share: torch.Tensor, num_kv_heads: int, page_tokens: int, scale: float,
+                            plan: SharedPlan, part_acc: torch.Tensor, part_ml: torch.Tensor) -> None:
+    """``attention_decode`` for sequences that share prefixes: one query token per sequence, ``seq_len`` counts the keys it sees (none: the result is
+    zero).  ``members`` (int32 [sequences]) lists every sequence once, group by group; ``share`` (int32 [groups, 3]) says of each group where it starts in
+    ``members``, how many members it has and how many leading tokens they share: below that, the keys and values are read through the page list of the
+    group's first member, once for all of them.  A member's page list serves its own tokens from there on, whether or not the shared length ends
+    with a page; no member is shorter than what its group shares, except one without any keys.  Groups that share nothing are groups like any other.
+
+    The keys are cut into ``plan.ranges`` ranges whose partial results pass through ``part_acc`` and ``part_ml`` (float, at least
+    ``plan.acc_elements`` and ``plan.ml_elements``).
+    """
+    n_seqs, num_heads, head_dim = _check_attention(q, k_cache, v_cache, out, block_table, num_kv_heads, page_tokens)
+    if v_cache.shape != k_cache.shape:
+        raise KernelError(f"attention_decode_shared: values {tuple(v_cache.shape)} are not as the keys {tuple(k_cache.shape)}")
+    if head_dim > 256:
+        raise KernelError(f"attention_decode_shared: heads of {head_dim} elements (at most 256)")
+    if block_table.dim() != 2 or block_table.shape[0] != n_seqs or (n_seqs and not block_table.shape[1]):
+        raise KernelError(f"attention_decode_shared: block_table {tuple(block_table.shape)} for {n_seqs} sequences")
+    _need(seq_len, "seq_len", torch.int32, (n_seqs,))
+    _need(members, "members", torch.int32, (n_seqs,))
+    _need(share, "share", torch.int32, (plan.groups, 3))
+    if (plan.n_seqs, plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.dtype) != (n_seqs, num_heads, num_kv_heads, head_dim, q.dtype):
+        raise KernelError(f"attention_decode_shared: the plan is for {plan}, not for q {tuple(q.shape)} {q.dtype} over {num_kv_heads} heads")
+    _need(part_acc, "part_acc", torch.float32)
+    _need(part_ml, "part_ml", torch.float32)
+    if part_acc.numel() < plan.acc_elements or part_ml.numel() < plan.ml_elements:
+        raise KernelError("attention_decode_shared: scratch is too small for this plan")
+    _call("attention_shared", "qt_attention_decode_shared", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q, "q"), _ptr(block_table),
+          block_table.shape[1], _ptr(seq_len), _ptr(members), _ptr(share), n_seqs, plan.groups, num_heads, num_kv_heads, head_dim, page_tokens,
+          k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, _ptr(part_acc), _ptr(part_ml), _stream(), launches=2 if n_seqs else 0)
+
+
 # ----------------------------------------------------------------------------- experts chosen by a table
 def route_top(logits: GemmOut, chosen: torch.Tensor, weights: torch.Tensor, gate: torch.Tensor | None, experts: int, scale: float,
               normalize: bool = True, softmax: bool = False, groups: int = 1, keep_groups: int = 1) -> None:
@@ -1596,6 +1683,29 @@ def sample_keyed(logits: torch.Tensor, temperature: float, seed: int, keys: torc
     seed &= (1 << 64) - 1
     _call("sampling", "qt_sample_keyed", _ptr(logits), float(temperature), seed - (1 << 64) if seed >> 63 else seed, _ptr(keys),
           _ptr(out), rows, logits.shape[1], int(top_k), float(top_p), _stream())
+
+
+def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
+                    uniform: torch.Tensor, out: torch.Tensor, logprob: torch.Tensor | None = None) -> None:
+    """One token per row of float logits [rows, vocab] (rows may lie further apart than they are long), with parameters of the row's own, all on the
+    device: ``temperature`` (0: the lowest id of the largest logit), ``top_k`` (int32; 0: off), ``top_p`` (1: off), ``min_p`` (0: off) and a number
+    ``uniform`` in [0, 1) by which the token is drawn in vocabulary order.  Tokens above which fewer than ``top_k`` logits lie are kept; of these,
+    tokens above which less than ``top_p`` of their mass lies; of these, tokens at least ``min_p`` times as likely as the likeliest.
+    ``out`` (int32) takes the tokens, ``logprob`` (float, optional) the logarithm of the probability with which each was drawn.  NaN counts as -inf;
+    a row that has nothing above -inf gives token 0 with log-probability -inf."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2:
+        raise KernelError("sample_filtered: logits must be a CUDA tensor [rows, vocab] of float32 (there is no host path)")
+    rows, vocab = logits.shape
+    if vocab < 1 or (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        raise KernelError(f"sample_filtered: logits {tuple(logits.shape)} with strides {logits.stride()}")
+    for name, vector in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("uniform", uniform)):
+        _need(vector, name, torch.float32, (rows,))
+    _need(top_k, "top_k", torch.int32, (rows,))
+    _need(out, "out", torch.int32, (rows,))
+    if logprob is not None:
+        _need(logprob, "logprob", torch.float32, (rows,))
+    _call("sampling_filtered", "qt_sample_filtered", _ptr(logits), logits.stride(0) if rows > 1 else vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
+          _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(logprob), rows, vocab, _stream(), launches=1 if rows else 0)
 
 
 _STATUS: dict[int, torch.Tensor] = {}

@@ -1,0 +1,206 @@
+"""Sampling under filters, a row's own parameters and given numbers, against a plain statement in 64 bits."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from qwen_triton_b200.ops import kernels
+from qwen_triton_b200.ops.kernels import KernelError
+
+pytestmark = pytest.mark.gpu
+
+
+def kept_of(x, temperature, k, p, m):
+    """(weights that stay, else 0; y) of one row in 64 bits on the host, from the definition token by token over the distinct logits."""
+    x = torch.where(x.isnan(), float("-inf"), x).double()
+    best = x.max()
+    y = torch.where(x == best, 0.0, x - best) / temperature
+    w = y.exp()
+    values, inverse, counts = x.unique(return_inverse=True, return_counts=True)
+    above = (counts.flip(0).cumsum(0).flip(0) - counts)[inverse]
+    kept = (above < k) if k > 0 else torch.ones_like(x, dtype=torch.bool)
+    mass = torch.zeros_like(values).scatter_add_(0, inverse, torch.where(kept, w, 0.0))
+    above_mass = (mass.flip(0).cumsum(0).flip(0) - mass)[inverse]
+    if p < 1:
+        kept &= above_mass < p * mass.sum()
+    kept &= w >= min(m, 1.0)
+    return torch.where(kept, w, 0.0), y
+
+
+def margins(x, temperature, k, p, m):
+    """How near the nearest token is to the other side of a filter: relative to the row's mass (top_p) and to the weight (min_p)."""
+    w_all, y = kept_of(x, temperature, k, 1.0, 0.0)
+    near = math.inf
+    if p < 1:
+        values, inverse = x.double().unique(return_inverse=True)
+        mass = torch.zeros_like(values).scatter_add_(0, inverse, w_all)
+        above = mass.flip(0).cumsum(0).flip(0) - mass
+        near = float(((above - p * mass.sum()).abs() / mass.sum()).min())
+    if 0 < m < 1:
+        near = min(near, float((w_all[w_all > 0] / m - 1).abs().min()))
+    return near
+
+
+def middle(weights, gen):
+    """(token, number): a token that stays, by its weight, and a number in the middle of its part of the line, where that part is wide enough for a
+    float and the sums' roundings to keep the number inside it."""
+    running = weights.cumsum(0)
+    total = float(running[-1])
+    for _ in range(200):
+        u = float(torch.rand((), generator=gen, dtype=torch.float64))
+        token = int((running > u * total).nonzero()[0])
+        low, high = float(running[token] - weights[token]) / total, float(running[token]) / total
+        if high - low > 2.0 ** -16:
+            return token, (low + high) / 2
+    token = int(weights.argmax())
+    return token, (float(running[token]) - 0.5 * float(weights[token])) / total
+
+
+def run(logits, temperature, top_k, top_p, min_p, uniform, want_logprob=True):
+    rows = logits.shape[0]
+    def vector(values, dtype):
+        return torch.tensor(values, dtype=dtype, device="cuda")
+    out = torch.full((rows,), -5, dtype=torch.int32, device="cuda")
+    logprob = torch.full((rows,), 9.0, device="cuda") if want_logprob else None
+    kernels.sample_filtered(logits, vector(temperature, torch.float32), vector(top_k, torch.int32), vector(top_p, torch.float32),
+                            vector(min_p, torch.float32), vector(uniform, torch.float32), out, logprob)
+    return out.cpu(), None if logprob is None else logprob.cpu()
+
+
+def check(logits, params, seed):
+    """Rows with params[(T, k, p, m)] each: the token of the middle of its part, and its log-probability.  The logarithm's error: y is one subtraction and
+    one division (2^-23 of |y|), the mass a sum whose terms have relative errors of a few 2^-24 times (1 + |y|), the logarithm 2^-22 of itself."""
+    gen = torch.Generator().manual_seed(seed)
+    rows = []
+    for x, (t, k, p, m) in zip(logits.cpu(), params):
+        while margins(x, t, k, p, m) < 1e-5:                  # settled before the kernel sees the row
+            p, m = (p - 1e-3 if p < 1 else p), (m * 1.01 if m else m)
+        weights, y = kept_of(x, t, k, p, m)
+        token, u = middle(weights, gen)
+        rows.append((t, k, p, m, u, token, float(y[token] - weights.sum().log()), float(y[token])))
+    tokens, logprob = run(logits, *[[r[c] for r in rows] for c in range(5)])
+    assert tokens.tolist() == [r[5] for r in rows]
+    for got, (_, _, _, _, _, _, want, y) in zip(logprob.tolist(), rows):
+        assert abs(got - want) <= 2e-6 * (1 + abs(y) + abs(want)), (got, want)
+
+
+PARAMS = [(1.0, 0, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (0.8, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.05), (1.3, 20, 0.95, 0.02), (0.3, 1, 0.5, 0.5), (2.5, 0, 0.999, 0.0),
+          (1.0, 3, 0.7, 0.0), (0.05, 0, 0.9, 0.1), (5.0, 400, 0.99, 0.001), (1.0, 100000, 0.8, 0.0), (1.0, 7, 1.0, 0.9)]
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 199, 503, 1024, 4099, 32000, 50257, 151936, 151937, 262144])
+def test_every_filter_at_many_sizes(vocab):
+    gen = torch.Generator().manual_seed(vocab)
+    logits = 2.5 * torch.randn((len(PARAMS), vocab), generator=gen)
+    logits[:, torch.randint(0, vocab, (min(vocab, 40),), generator=gen)] += 6.0
+    check(logits.cuda(), [(t, min(k, vocab), p, m) for t, k, p, m in PARAMS], vocab)
+
+
+@pytest.mark.parametrize("step", [1.0, 0.25, 2.0 ** -4])
+def test_tokens_that_tie_share_their_fate(step):
+    gen = torch.Generator().manual_seed(int(step * 16))
+    logits = (torch.randn((len(PARAMS), 5000), generator=gen) * 3 / step).round() * step
+    logits[0, 100:200] = -0.0
+    logits[0, 200:300] = 0.0
+    check(logits.cuda(), PARAMS, 1)
+
+
+def test_all_alike_and_nearly_alike():
+    gen = torch.Generator().manual_seed(2)
+    rows = torch.cat([torch.full((3, 40000), 1.5), 3.0 + 1e-4 * torch.rand((4, 40000), generator=gen), torch.full((1, 40000), -3.0e38)])
+    check(rows.cuda(), [(1.0, 0, 1.0, 0.0), (1.0, 5, 0.5, 0.0), (0.5, 0, 0.5, 0.3), (1.0, 0, 0.5, 0.0), (1.0, 1000, 1.0, 0.0), (1.0, 20000, 0.25, 0.0),
+                        (0.01, 0, 0.9, 0.999), (1.0, 0, 1.0, 0.0)], 3)
+
+
+def test_barred_tokens():
+    """Masks of -inf, of the lowest float and of NaN, down to one token that is left."""
+    gen = torch.Generator().manual_seed(4)
+    logits = 2 * torch.randn((len(PARAMS), 20001), generator=gen)
+    for row, mask in enumerate((float("-inf"), torch.finfo(torch.float32).min, float("nan")) * 4):
+        allowed = (1, 2, 30, 3000)[row // 3]
+        barred = torch.randperm(20001, generator=gen)[allowed:]
+        logits[row, barred] = mask
+    check(logits.cuda(), PARAMS, 5)
+
+
+def test_infinities_and_rows_that_leave_nothing():
+    logits = torch.zeros((6, 1000))
+    logits[0] = float("-inf")
+    logits[1] = float("nan")
+    logits[2, 500:] = float("inf")
+    logits[3, 70] = float("inf")
+    logits[4] = float("-inf")
+    logits[5, 3] = float("nan")
+    tokens, logprob = run(logits.cuda(), [1.0, 0.7, 1.0, 0.5, 0.0, 0.0], [0, 5, 0, 0, 0, 0], [1.0, 0.9, 0.9, 1.0, 1.0, 1.0], [0.0] * 6,
+                          [0.5, 0.2, 0.0, 0.99, 0.1, 0.1])
+    assert tokens.tolist() == [0, 0, 500, 70, 0, 0]
+    assert logprob[:2].tolist() == [-math.inf] * 2 and logprob[4] == -math.inf
+    assert abs(float(logprob[2]) + math.log(500)) < 1e-5 and logprob[3] == 0 and logprob[5] == 0
+
+
+def test_greedy_rows_take_the_lowest_id():
+    gen = torch.Generator().manual_seed(6)
+    logits = torch.randn((5, 9999), generator=gen).round()
+    tokens, logprob = run(logits.cuda(), [0.0, 0.0, -1.0, float("nan"), 0.0], [0, 3, 0, 0, 1], [1.0, 0.5, 1.0, 1.0, 0.1], [0.0, 0.1, 0.0, 0.0, 0.9], [0.3] * 5)
+    assert tokens.tolist() == [int((row == row.max()).nonzero()[0]) for row in logits]
+    assert logprob.tolist() == [0.0] * 5
+
+
+def test_numbers_at_the_ends_and_parameters_beyond_theirs():
+    """u = 0 gives the first token that stays, u at and beyond 1 the last; top_p <= 0 leaves the likeliest, min_p > 1 too."""
+    logits = torch.tensor([[1.0, 5.0, 4.9, -3.0, 4.8, 5.0, -40.0]]).repeat(8, 1).cuda()
+    tokens, _ = run(logits, [1.0] * 8, [3, 3, 3, 0, 0, 99, -4, 0], [1.0, 1.0, 1.0, 0.0, -1.0, 1.0, 2.0, 1.0], [0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 7.0],
+                    [0.0, 1.0, 3.0, 0.999, 0.0, 0.0, 0.0, 0.999])
+    assert tokens.tolist() == [1, 5, 5, 5, 1, 0, 0, 5]
+
+
+def test_rows_apart_and_odd_addresses():
+    """A part of wider rows, from an address that no wide load takes."""
+    gen = torch.Generator().manual_seed(7)
+    wide = 2 * torch.randn((len(PARAMS), 12345), generator=gen).cuda()
+    view = wide[:, 3:10000]
+    check(view, PARAMS, 8)
+    check(wide[::2, 1:1002], PARAMS[::2], 9)
+
+
+def test_no_order_of_additions_shows_and_the_stream_is_followed():
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    logits = torch.randn((64, 151936), generator=gen, device="cuda")
+    args = ([0.9] * 64, [0, 50] * 32, [0.95, 1.0, 0.7, 1.0] * 16, [0.0] * 64, [i / 64 for i in range(64)])
+    tokens, logprob = run(logits, *args)
+    again, logprob2 = run(logits, *args)
+    assert torch.equal(tokens, again) and torch.equal(logprob, logprob2)
+    stream = torch.cuda.Stream()
+    late = torch.zeros_like(logits)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(2_000_000)
+        late.copy_(logits)
+        third, _ = run(late, *args, want_logprob=False)
+    assert torch.equal(tokens, third)
+
+
+def test_shares_of_many_numbers():
+    """Over an even grid of numbers each token comes as often as its weight says, to one grid step."""
+    logits = torch.tensor([0.0, 1.0, 2.0, -1.0, 2.0, 0.5]).log_softmax(0)
+    n = 4096
+    tokens, _ = run(logits.repeat(n, 1).cuda(), [1.0] * n, [0] * n, [1.0] * n, [0.0] * n, [(i + 0.5) / n for i in range(n)])
+    counts = torch.bincount(tokens, minlength=6).double()
+    assert bool(((counts - n * logits.double().exp()).abs() <= 1).all())
+
+
+def test_no_rows_and_refusals():
+    empty = torch.empty((0, 50), device="cuda")
+    run(empty, [], [], [], [], [])
+    logits = torch.zeros((3, 50), device="cuda")
+    f, k, out = torch.ones(3, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    good = dict(logits=logits, temperature=f, top_k=k, top_p=f, min_p=f, uniform=f, out=out, logprob=None)
+    for changes, words in ((dict(logits=logits.cpu()), "CUDA"), (dict(logits=logits.bfloat16()), "float32"), (dict(logits=logits[0]), "rows"),
+                           (dict(logits=logits.t()), "strides|shape"), (dict(logits=logits[:1].expand(3, 50)), "strides"),
+                           (dict(logits=torch.zeros((3, 0), device="cuda")), "logits"), (dict(temperature=f[:2]), "temperature"),
+                           (dict(top_k=f), "top_k"), (dict(top_p=f.double()), "top_p"), (dict(min_p=f.cpu()), "min_p"), (dict(uniform=f[::2]), "uniform"),
+                           (dict(out=f), "out"), (dict(logprob=out), "logprob")):
+        with pytest.raises(KernelError, match=words):
+            kernels.sample_filtered(**{**good, **changes})
