@@ -130,10 +130,10 @@ _SIGNATURES = {
                                      _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_float, _c_int, _c_ptr],
     },
     "attention_shared": {
-        # q, k_cache, v_cache, out, dtype, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, nq, nkv, d, page_tokens, n_pages,
-        # scale, shared_ranges, own_ranges, part_acc, part_ml, stream
+        # q, k_cache, v_cache, out, dtype, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, most_members, nq, nkv, d, page_tokens,
+        # n_pages, scale, shared_ranges, own_ranges, on_tc, part_acc, part_ml, status, stream
         "qt_attention_decode_shared": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                                       _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr],
+                                       _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
     },
     "attention_tc": {
         "qt_attention_prefill_tc": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int,
@@ -1414,6 +1414,11 @@ class SharedPlan:
         return self.n_seqs * self.num_heads * self.ranges * 2
 
 
+def _shared_on_tc(dtype: torch.dtype, head_dim: int) -> bool:
+    """Whether the tensor-core kernels take a call (with pages of 64 tokens)."""
+    return dtype == torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
+
+
 def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, groups: int, most_members: int,
                 most_shared: int, most_own: int, sms: int | None = None) -> SharedPlan:
     """The cut for ``n_seqs`` sequences in ``groups`` groups of at most ``most_members``, a shared length of at most ``most_shared`` tokens and at most
@@ -1422,8 +1427,15 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
         raise KernelError(f"shared_plan: {n_seqs} sequences in {groups} groups of at most {most_members}, {most_shared} and {most_own} tokens")
     if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or head_dim < 1 or dtype not in _CODES:
         raise KernelError(f"shared_plan: {num_heads} heads over {num_kv_heads} of {head_dim} in {dtype}")
-    shared_ranges = max(1, min(32, -(-most_shared // 128)))
-    own_ranges = max(1, min(8, -(-most_own // 256)))
+    sms = sms or sm_count()
+    group = num_heads // num_kv_heads
+    if _shared_on_tc(dtype, head_dim):
+        blocks = num_kv_heads * max(1, -(-most_members * group // 128))
+        shared_ranges = max(1, min(32, sms // blocks, -(-most_shared // 128)))
+        own_ranges = max(1, min(8, -(-most_own // 512), 2 * sms // max(1, n_seqs * num_kv_heads)))
+    else:
+        shared_ranges = max(1, min(32, -(-most_shared // 128)))
+        own_ranges = max(1, min(8, -(-most_own // 256)))
     return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges)
 
 
@@ -1455,9 +1467,11 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     _need(part_ml, "part_ml", torch.float32)
     if part_acc.numel() < plan.acc_elements or part_ml.numel() < plan.ml_elements:
         raise KernelError("attention_decode_shared: scratch is too small for this plan")
+    on_tc = _shared_on_tc(q.dtype, head_dim) and page_tokens == 64
     _call("attention_shared", "qt_attention_decode_shared", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q, "q"), _ptr(block_table),
-          block_table.shape[1], _ptr(seq_len), _ptr(members), _ptr(share), n_seqs, plan.groups, num_heads, num_kv_heads, head_dim, page_tokens,
-          k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, _ptr(part_acc), _ptr(part_ml), _stream(), launches=2 if n_seqs else 0)
+          block_table.shape[1], _ptr(seq_len), _ptr(members), _ptr(share), n_seqs, plan.groups, plan.most_members, num_heads, num_kv_heads, head_dim,
+          page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, int(on_tc), _ptr(part_acc), _ptr(part_ml),
+          _ptr(_status_word(q.device)), _stream(), launches=2 if n_seqs else 0)
 
 
 # ----------------------------------------------------------------------------- experts chosen by a table
