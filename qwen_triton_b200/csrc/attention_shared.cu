@@ -32,6 +32,7 @@ struct SharedParams {
     int shared_ranges, own_ranges;
     float* part_acc;                            // [n_seqs, nq, ranges, d]
     float* part_ml;                             // [n_seqs, nq, ranges, 2]
+    int own_warps;                              // warps a block of the own keys' kernel
     int* status;                                // stays 0 unless a wait in a kernel ran out
 };
 
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
 // two-stage cp.async ring of its own, rows behind the last key filled with zeros.  Then the blocks hand their sums to the first one, which joins them with
 // the shared ranges' and writes the result.
 constexpr int OWN_TILE = 32;
-constexpr int OWN_WARPS = 4;
+constexpr int OWN_MAX_WARPS = 4;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -482,18 +483,18 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 }
 
 template <int HD> __host__ __device__ constexpr uint32_t own_tile_bytes() { return OWN_TILE * HD * 2; }
-// Q, the warps' rings (their sums later), then the cluster's inbox in the first block
-template <int HD> constexpr size_t own_smem(int ranges, int rows) {
-    const size_t rings = (size_t)OWN_WARPS * 4 * own_tile_bytes<HD>(), sums = (size_t)OWN_WARPS * 16 * (HD + 2) * 4;
-    return 16 * HD * 2 + (rings > sums ? rings : sums) + (ranges > 1 ? (size_t)ranges * rows * (HD + 2) * 4 : 0);
+// Q; the warps' rings, where their sums go later; the cluster's inbox in the first block; what a row's partial results are multiplied by
+template <int HD> __host__ __device__ constexpr uint32_t own_rings(int warps) { return (uint32_t)warps * 4 * own_tile_bytes<HD>(); }
+template <int HD> constexpr size_t own_smem(int warps, int ranges, int rows) {
+    return 16 * HD * 2 + own_rings<HD>(warps) + (ranges > 1 ? (size_t)ranges * rows * (HD + 4) * 4 : 0) + (size_t)16 * (MAX_RANGES + 8) * 4;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(32 * OWN_WARPS) shared_own_kernel(const SharedParams p) {
+__global__ void __launch_bounds__(32 * OWN_MAX_WARPS) shared_own_kernel(const SharedParams p) {
     constexpr int CHUNKS = HD / 8;                             // 16-byte pieces of a row
     constexpr uint32_t ROW = HD * 2, TILE = own_tile_bytes<HD>();
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, threads = blockDim.x, warps = threads >> 5;
     if (gridDim.x > 1) cluster_arrive_started();
     pdl_launch_dependents();
     const int per = p.nq / p.nkv, heads16 = (per + 15) / 16;
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(32 * OWN_WARPS) shared_own_kernel(const Shared
     const int* table = p.block_table + (size_t)seq * p.max_blocks;
     const int first_tile = min(shared, len) / OWN_TILE;
     const int own_tiles = len > shared ? (len + OWN_TILE - 1) / OWN_TILE - first_tile : 0;
-    const int streams = gridDim.x * OWN_WARPS, stream = blockIdx.x * OWN_WARPS + warp;
+    const int streams = gridDim.x * warps, stream = blockIdx.x * warps + warp;
     const int per_stream = (own_tiles + streams - 1) / streams;
     const int tile_begin = first_tile + stream * per_stream;
     const int n_tiles = max(0, min(per_stream, first_tile + own_tiles - tile_begin));
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(32 * OWN_WARPS) shared_own_kernel(const Shared
     // swizzled rows: 16-byte piece c of row r lies at piece c ^ (r & 7), so that eight rows' pieces are in eight different banks' groups
     auto place = [](uint32_t row, uint32_t c) { return row * ROW + ((c ^ (row & 7u)) << 4); };
     const uint32_t q_s = smem_u32(smem_raw), ring = q_s + 16 * ROW + warp * 4 * TILE;
-    for (int i = tid; i < 16 * CHUNKS; i += 32 * OWN_WARPS) {
+    for (int i = tid; i < 16 * CHUNKS; i += threads) {
         const int r = i / CHUNKS, c = i % CHUNKS;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < rows && c * 8 < p.d) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + ((size_t)seq * p.nq + head0 + r) * p.d + c * 8);
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(32 * OWN_WARPS) shared_own_kernel(const Shared
 
     // the warps' sums through shared memory (the rings are free now)
     float* sums = reinterpret_cast<float*>(smem_raw + 16 * ROW);              // [warps][16][HD]
-    float* sums_ml = sums + OWN_WARPS * 16 * HD;                              // [warps][16][2]
+    float* sums_ml = sums + warps * 16 * HD;                                  // [warps][16][2]
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -629,65 +630,77 @@ __global__ void __launch_bounds__(32 * OWN_WARPS) shared_own_kernel(const Shared
         *reinterpret_cast<float2*>(sums + (warp * 16 + g + 8) * HD + c) = make_float2(o[i][2], o[i][3]);
     }
     __syncthreads();
-    constexpr size_t RINGS = (size_t)OWN_WARPS * 4 * TILE, SUMS = (size_t)OWN_WARPS * 16 * (HD + 2) * 4;
-    float* inbox = reinterpret_cast<float*>(smem_raw + 16 * ROW + (RINGS > SUMS ? RINGS : SUMS));      // [blocks][rows][HD + 2] in the first block
-    const bool several = gridDim.x > 1;
-    if (several) cluster_wait_started();
-    pdl_wait();                                                               // the shared ranges' partial results
-    const Ranges ranges(shared, PAGE, p.shared_ranges);
-    for (int i = tid; i < rows * HD; i += 32 * OWN_WARPS) {
-        const int r = i / HD, c = i % HD;
-        float m_all = -INFINITY, l_all = 0.f, a_all = 0.f;
-#pragma unroll
-        for (int w = 0; w < OWN_WARPS; ++w) m_all = fmaxf(m_all, sums_ml[(w * 16 + r) * 2]);
-#pragma unroll
-        for (int w = 0; w < OWN_WARPS; ++w) {
-            const float f = m_all == -INFINITY ? 0.f : fast_exp2(sums_ml[(w * 16 + r) * 2] - m_all);
-            l_all += sums_ml[(w * 16 + r) * 2 + 1] * f;
-            a_all += sums[(w * 16 + r) * HD + c] * f;
-        }
-        if (several) {
-            float* slot = inbox + ((size_t)blockIdx.x * rows + r) * (HD + 2);
-            cluster_store_float(slot + c, 0, a_all);
+    constexpr int QUADS = HD / 4, SLOT = HD + 4;                              // a row in fours; a row of the inbox: its sums, its maximum and its sum of weights
+    float* inbox = reinterpret_cast<float*>(smem_raw + 16 * ROW + own_rings<HD>(warps));       // [blocks][rows][SLOT] in the first block
+    float* factors = inbox + (gridDim.x > 1 ? gridDim.x * rows * SLOT : 0);   // [16][MAX_RANGES + 8]: by what partial results are multiplied
+    if (gridDim.x > 1) {
+        cluster_wait_started();
+        for (int i = tid; i < rows * QUADS; i += threads) {
+            const int r = i / QUADS, c = i % QUADS * 4;
+            float m_all = -INFINITY, l_all = 0.f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < warps; ++w) m_all = fmaxf(m_all, sums_ml[(w * 16 + r) * 2]);
+            for (int w = 0; w < warps; ++w) {
+                const float f = m_all == -INFINITY ? 0.f : fast_exp2(sums_ml[(w * 16 + r) * 2] - m_all);
+                const float4 v = *reinterpret_cast<const float4*>(sums + (w * 16 + r) * HD + c);
+                l_all += sums_ml[(w * 16 + r) * 2 + 1] * f;
+                a.x += v.x * f; a.y += v.y * f; a.z += v.z * f; a.w += v.w * f;
+            }
+            float* slot = inbox + (size_t)(blockIdx.x * rows + r) * SLOT;
+            cluster_store_float(slot + c, 0, a.x); cluster_store_float(slot + c + 1, 0, a.y);
+            cluster_store_float(slot + c + 2, 0, a.z); cluster_store_float(slot + c + 3, 0, a.w);
             if (c == 0) { cluster_store_float(slot + HD, 0, m_all); cluster_store_float(slot + HD + 1, 0, l_all); }
-        } else if (c < p.d) {
-            const size_t row = (size_t)seq * p.nq + head0 + r, slot = row * (p.shared_ranges + p.own_ranges);
-            float m_own = m_all;
-            for (int k = 0; k < ranges.used; ++k) m_all = fmaxf(m_all, p.part_ml[2 * (slot + k)]);
-            const float f_own = m_own == -INFINITY ? 0.f : fast_exp2(m_own - m_all);
-            l_all *= f_own; a_all *= f_own;
-            for (int k = 0; k < ranges.used; ++k) {
-                const float mk = p.part_ml[2 * (slot + k)], f = mk == -INFINITY ? 0.f : fast_exp2(mk - m_all), a = p.part_acc[(slot + k) * p.d + c];
-                l_all += p.part_ml[2 * (slot + k) + 1] * f;
-                if (f != 0.f) a_all += a * f;
-            }
-            ((__nv_bfloat16*)p.out)[row * p.d + c] = __float2bfloat16_rn(l_all == 0.f ? 0.f : a_all / l_all);
         }
-    }
-    if (several) {
         cluster_barrier();
-        if (blockIdx.x == 0) {
-            for (int i = tid; i < rows * HD; i += 32 * OWN_WARPS) {
-                const int r = i / HD, c = i % HD;
-                if (c >= p.d) continue;
-                const size_t row = (size_t)seq * p.nq + head0 + r, slot = row * (p.shared_ranges + p.own_ranges);
-                float m_all = -INFINITY, l_all = 0.f, a_all = 0.f;
-                for (int b = 0; b < (int)gridDim.x; ++b) m_all = fmaxf(m_all, inbox[((size_t)b * rows + r) * (HD + 2) + HD]);
-                for (int k = 0; k < ranges.used; ++k) m_all = fmaxf(m_all, p.part_ml[2 * (slot + k)]);
-                for (int b = 0; b < (int)gridDim.x; ++b) {
-                    const float* in = inbox + ((size_t)b * rows + r) * (HD + 2);
-                    const float f = in[HD] == -INFINITY ? 0.f : fast_exp2(in[HD] - m_all);
-                    l_all += in[HD + 1] * f;
-                    a_all += in[c] * f;
-                }
-                for (int k = 0; k < ranges.used; ++k) {
-                    const float mk = p.part_ml[2 * (slot + k)], f = mk == -INFINITY ? 0.f : fast_exp2(mk - m_all), a = p.part_acc[(slot + k) * p.d + c];
-                    l_all += p.part_ml[2 * (slot + k) + 1] * f;
-                    if (f != 0.f) a_all += a * f;
-                }
-                ((__nv_bfloat16*)p.out)[row * p.d + c] = __float2bfloat16_rn(l_all == 0.f ? 0.f : a_all / l_all);
-            }
+    }
+    pdl_wait();                                                               // the shared ranges' partial results
+    if (blockIdx.x > 0) return;
+    // What is left in the first block: the own partial results (the cluster's in the inbox, else the warps' sums) and the shared ranges'.
+    const int own = gridDim.x > 1 ? gridDim.x : warps, used = Ranges(shared, PAGE, p.shared_ranges).used, parts = own + used;
+    const int stride = p.shared_ranges + p.own_ranges;
+    auto own_ml = [&](int k, int r) { return gridDim.x > 1 ? inbox + (size_t)(k * rows + r) * SLOT + HD : sums_ml + (k * 16 + r) * 2; };
+    auto own_row = [&](int k, int r) { return gridDim.x > 1 ? inbox + (size_t)(k * rows + r) * SLOT : sums + (k * 16 + r) * HD; };
+    for (int r = warp; r < rows; r += warps) {                                // a warp a row: the maximum over the parts, then every part's factor
+        const float* ml = p.part_ml + ((size_t)seq * p.nq + head0 + r) * stride * 2;
+        float m_all = -INFINITY, l_all = 0.f;
+        float mk[(MAX_RANGES + 8 + 31) / 32], lk[(MAX_RANGES + 8 + 31) / 32];
+#pragma unroll
+        for (int i = 0; i < (MAX_RANGES + 8 + 31) / 32; ++i) {
+            const int k = i * 32 + lane;
+            float2 both = make_float2(-INFINITY, 0.f);
+            if (k < own) { const float* at = own_ml(k, r); both = make_float2(at[0], at[1]); }
+            else if (k < parts) both = *reinterpret_cast<const float2*>(ml + 2 * (k - own));
+            mk[i] = both.x; lk[i] = both.y;
+            m_all = fmaxf(m_all, both.x);
         }
+        m_all = warp_max(m_all);
+#pragma unroll
+        for (int i = 0; i < (MAX_RANGES + 8 + 31) / 32; ++i) {
+            mk[i] = mk[i] == -INFINITY ? 0.f : fast_exp2(mk[i] - m_all);
+            l_all += lk[i] * mk[i];
+        }
+        l_all = warp_sum(l_all);
+        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+#pragma unroll
+        for (int i = 0; i < (MAX_RANGES + 8 + 31) / 32; ++i)
+            if (i * 32 + lane < parts) factors[r * (MAX_RANGES + 8) + i * 32 + lane] = mk[i] * inv;
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * QUADS; i += threads) {
+        const int r = i / QUADS, c = i % QUADS * 4;
+        if (c >= p.d) continue;
+        const size_t row = (size_t)seq * p.nq + head0 + r;
+        const float* f = factors + r * (MAX_RANGES + 8);
+        const float* acc = p.part_acc + row * stride * p.d + c;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float4 v, float by) {                                  // a part without a key for this row may hold anything
+            if (by != 0.f) { a.x += v.x * by; a.y += v.y * by; a.z += v.z * by; a.w += v.w * by; }
+        };
+        for (int k = 0; k < own; ++k) add(*reinterpret_cast<const float4*>(own_row(k, r) + c), f[k]);
+#pragma unroll 8
+        for (int k = 0; k < used; ++k) add(*reinterpret_cast<const float4*>(acc + (size_t)k * p.d), f[own + k]);
+        uint2 packed = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
+        *reinterpret_cast<uint2*>((__nv_bfloat16*)p.out + row * p.d + c) = packed;
     }
 }
 
@@ -710,14 +723,14 @@ int launch_tc(const SharedParams& p, int most_members, cudaStream_t stream) {
     if (rc == QT_OK) rc = cache_map(&map_v, p.v_cache, (uint64_t)p.n_pages * p.nkv * PAGE, p.d);
     if (rc != QT_OK) return rc;
     const int per = p.nq / p.nkv;
-    const size_t smem = (HD / 64) * (HALF_BYTES + 4 * KEY_HALF_BYTES) + 1024 + 192, smem_own = own_smem<HD>(p.own_ranges, per < 16 ? per : 16);
+    const size_t smem = (HD / 64) * (HALF_BYTES + 4 * KEY_HALF_BYTES) + 1024 + 192, smem_own = own_smem<HD>(p.own_warps, p.own_ranges, per < 16 ? per : 16);
     cudaError_t raised = raise_shared<shared_prefix_tc_kernel<HD>>((int)smem);
     if (raised == cudaSuccess) raised = raise_shared<shared_own_kernel<HD>>((int)smem_own);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_shared: cannot raise shared memory: %s", cudaGetErrorString(raised));
     const long long tiles = ((long long)most_members * per + BQ - 1) / BQ, y_own = (long long)p.nkv * ((per + 15) / 16);
     QT_REQUIRE(tiles * p.nkv <= 65535 && y_own <= 65535 && p.n_groups <= 65535 && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
     launch_kernel(shared_prefix_tc_kernel<HD>, dim3(p.shared_ranges, (unsigned)(tiles * p.nkv), p.n_groups), dim3(TC_THREADS), smem, stream, map_k, map_v, p);
-    launch_kernel_cluster(shared_own_kernel<HD>, dim3(p.own_ranges, (unsigned)y_own, p.n_seqs), dim3(32 * OWN_WARPS), smem_own, stream,
+    launch_kernel_cluster(shared_own_kernel<HD>, dim3(p.own_ranges, (unsigned)y_own, p.n_seqs), dim3(32 * p.own_warps), smem_own, stream,
                           (unsigned)p.own_ranges, p);
     QT_CHECK_LAUNCH("attention_shared");
     return QT_OK;
@@ -729,7 +742,7 @@ int launch_tc(const SharedParams& p, int most_members, cudaStream_t stream) {
 extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, const int* block_table,
                                           int max_blocks, const int* seq_len, const int* members, const int* share, int n_seqs, int n_groups,
                                           int most_members, int nq, int nkv, int d, int page_tokens, int n_pages, float scale, int shared_ranges,
-                                          int own_ranges, int on_tc, float* part_acc, float* part_ml, int* status, void* stream) {
+                                          int own_ranges, int own_warps, int on_tc, float* part_acc, float* part_ml, int* status, void* stream) {
     QT_REQUIRE(n_seqs >= 0 && n_groups > 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_shared: bad head counts nq=%d nkv=%d (B=%d, %d groups)", nq, nkv, n_seqs, n_groups);
     QT_REQUIRE(d > 0 && d <= MAX_DIM && page_tokens > 0 && max_blocks > 0 && n_pages > 0, "attention_shared: bad sizes d=%d page=%d", d, page_tokens);
     QT_REQUIRE((long long)max_blocks * page_tokens <= 0x7fffffffll && most_members >= 0 && most_members <= n_seqs, "attention_shared: bad sizes: %d pages a sequence, %d members",
@@ -738,10 +751,10 @@ extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, co
     QT_REQUIRE(scale > 0.f && scale < INFINITY, "attention_shared: a score scale of %g (it must be positive)", (double)scale);
     if (n_seqs == 0) return QT_OK;
     const SharedParams p{q, k_cache, v_cache, out, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, nq, nkv, d, page_tokens, n_pages,
-                         scale, shared_ranges, own_ranges, part_acc, part_ml, status};
+                         scale, shared_ranges, own_ranges, part_acc, part_ml, own_warps, status};
     cudaStream_t s = (cudaStream_t)stream;
     if (on_tc) {
-        QT_REQUIRE(dtype == QT_BF16 && d % 8 == 0 && d <= 128 && page_tokens == PAGE && own_ranges <= 8 && status,
+        QT_REQUIRE(dtype == QT_BF16 && d % 8 == 0 && d <= 128 && page_tokens == PAGE && own_ranges <= 8 && own_warps > 0 && own_warps <= OWN_MAX_WARPS && status,
                    "attention_shared: the tensor-core kernels take bfloat16, heads of up to 128 in steps of 8, pages of 64 (d=%d, pages of %d)", d, page_tokens);
         QT_REQUIRE((long long)n_pages * nkv * PAGE <= 0x7fffffffll, "attention_shared: %d pages of %d heads are beyond a tensor map", n_pages, nkv);
         QT_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)part_acc | (uintptr_t)part_ml) & 15) == 0,
