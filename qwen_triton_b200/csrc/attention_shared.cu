@@ -32,8 +32,8 @@ struct SharedParams {
     int shared_ranges, own_ranges;
     float* part_acc;                            // [n_seqs, nq, ranges, d]
     float* part_ml;                             // [n_seqs, nq, ranges, 2]
-    int own_warps;                              // warps a block of the own keys' kernel
     int* status;                                // stays 0 unless a wait in a kernel ran out
+    int row_tiles, own_tiles, shared_blocks, own_blocks, turn;      // filled in at the launch
 };
 
 // Group g of the call, held within what the member list and the page lists have.
@@ -128,15 +128,15 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
 }
 
 // ----------------------------------------------------------------------------- bfloat16, heads of up to 128 elements, pages of 64
-// Two launches.  The first takes the shared keys of a group on tcgen05: a block has 128 of the rows (member, query head) of a kv head as the M of
-// its products and walks a range of the pages,
+// Two launches.  In the first a block has up to 128 rows (member, query head) of a kv head as the M of products on tcgen05 and walks a range of pages: rows of
+// all members over the group's shared keys, or one member's rows over keys of its own,
 //
 //   S = Q K^T    Q and K in shared memory (K by TMA, 128-byte swizzle), S in tensor memory
 //   P = 2^(S - m) as bfloat16 (the type of the values it is multiplied with), written over its scores in tensor memory
 //   O += P V     P from tensor memory, V as an MN-major operand, O in tensor memory over the whole range
 //
-// one thread a row, so that maxima and sums need no exchange; O is rescaled only where a row's maximum moved by more than 2^8.  The second launch takes
-// every member's own keys on mma.sync (the heads of a kv group are the 16 rows), a range a warp, and joins them with the first one's partial results.
+// one thread a row, so that maxima and sums need no exchange; O is rescaled only where a row's maximum moved by more than 2^8.  A member's own keys give an M of a
+// few rows and cost the tensor cores what 128 would, which is still less than what their keys' way from memory takes.  The second launch joins the ranges.
 constexpr int PAGE = 64;
 constexpr int BQ = 128;
 constexpr int TC_THREADS = 224;      // warp 0: TMA of K, warp 1: MMA and tensor memory, warps 2..5: Q and softmax, warp 6: TMA of V
@@ -144,6 +144,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.f;
 constexpr uint32_t HALF_BYTES = BQ * 128;         // [128 rows][64 columns]
 constexpr uint32_t KEY_HALF_BYTES = PAGE * 128;   // [64 keys][64 columns]
+constexpr int MAX_PARTS = MAX_RANGES;
 
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
@@ -206,8 +207,21 @@ struct Ranges {
     }
 };
 
+// The ranges of a member's own keys, in tiles from the one on in which the shared keys end.
+struct OwnRanges {
+    int tile, tile0, per, used, shared, len;
+    __device__ __forceinline__ OwnRanges(int tile_, int shared_, int len_, int ranges) : tile(tile_), shared(shared_), len(len_) {
+        tile0 = shared / tile;
+        const int tiles = len > shared ? (len + tile - 1) / tile - tile0 : 0;
+        per = (tiles + ranges - 1) / ranges;
+        used = per > 0 ? (tiles + per - 1) / per : 0;
+    }
+    __device__ __forceinline__ int begin(int i) const { return max(shared, (tile0 + i * per) * tile); }
+    __device__ __forceinline__ int end(int i) const { return min(len, (tile0 + (i + 1) * per) * tile); }
+};
+
 template <int HD>
-__global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                          const SharedParams p) {
     constexpr int HALVES = HD / 64;
     constexpr uint32_t Q_BYTES = HALVES * HALF_BYTES;
@@ -240,15 +254,43 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    const Group group = group_at(p, blockIdx.z);
-    const int per = p.nq / p.nkv;
-    const int kvh = blockIdx.y % p.nkv, row0 = blockIdx.y / p.nkv * BQ;
-    const int rows = min(BQ, group.count * per - row0);
-    const Ranges ranges(group.shared, PAGE, p.shared_ranges);
-    const int tile_begin = (int)blockIdx.x * ranges.per;
-    const int n_tiles = min(ranges.per, (group.shared + PAGE - 1) / PAGE - tile_begin);
-    if (rows <= 0 || n_tiles <= 0) return;                    // uniform for the block, before tensor memory is taken
-    const int* table = p.block_table + (size_t)member_at(p, group.first) * p.max_blocks;
+    const int per = p.nq / p.nkv, stride = p.shared_ranges + p.own_ranges;
+    // Blocks of shared keys and blocks of own keys take turns by as many as there are multiprocessors, so that each of these has one of either kind: the
+    // first are bound by the tensor cores and the exponentials, the second by memory.
+    const int turns = min(p.shared_blocks, p.own_blocks) / p.turn;
+    int index = blockIdx.x;
+    bool of_group;
+    if (index < 2 * turns * p.turn) {
+        of_group = (index / p.turn & 1) == 0;
+        index = index / p.turn / 2 * p.turn + index % p.turn;
+    } else {
+        index -= turns * p.turn;
+        of_group = index < p.shared_blocks;
+        if (!of_group) index -= p.shared_blocks - turns * p.turn;
+    }
+    // What this block has: `rows` rows from row0 on, of a group (member by member) or of one member, the keys [begin, end) of a page list.  Neighbours in
+    // the grid share keys: the row tiles of a kv head and range.
+    const int tiles_here = of_group ? p.row_tiles : p.own_tiles, ranges_here = of_group ? p.shared_ranges : p.own_ranges;
+    const int row0 = index % tiles_here * BQ, kvh = index / tiles_here % p.nkv, at = index / tiles_here / p.nkv / ranges_here;
+    int range = index / tiles_here / p.nkv % ranges_here, rows, begin, end, first;
+    if (of_group) {
+        const Group group = group_at(p, at);
+        const Ranges ranges(group.shared, PAGE, p.shared_ranges);
+        rows = min(BQ, group.count * per - row0);
+        begin = range * ranges.per * PAGE;
+        end = min(group.shared, begin + ranges.per * PAGE);
+        first = group.first;
+    } else {
+        const OwnRanges own(PAGE, group_of(p, at).shared, max(0, min(p.seq_len[member_at(p, at)], p.max_blocks * PAGE)), p.own_ranges);
+        rows = min(BQ, per - row0);
+        begin = own.begin(range);
+        end = own.end(range);
+        first = at;
+        range += p.shared_ranges;
+    }
+    const int tile_begin = begin / PAGE, n_tiles = (end + PAGE - 1) / PAGE - tile_begin;
+    if (rows <= 0 || begin >= end) return;                    // uniform for the block, before tensor memory is taken
+    const int* table = p.block_table + (size_t)member_at(p, first) * p.max_blocks;
     auto row_of_tile = [&](int j) { return (page_at(p, table, tile_begin + j) * p.nkv + kvh) * PAGE; };
 
     if (warp == 1) {
@@ -274,30 +316,12 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
             }
         }
     } else if (warp == 6) {
-        for (int j = 0; j < n_tiles; ++j) {
-            const int s = j & 1, row = row_of_tile(j);
-            const int visible = min(PAGE, group.shared - (tile_begin + j) * PAGE);
-            bool ok = true;
-            if (lane == 0) ok = mbar_wait(v_empty + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u, status, 1);
-            if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
-            if (visible == PAGE) {
-                if (lane == 0) {
-                    mbar_expect_tx(v_full + 8 * s, KV_BYTES);
-                    for (int h = 0; h < HALVES; ++h) tma_load_2d(v_s + s * KV_BYTES + h * KEY_HALF_BYTES, &map_v, v_full + 8 * s, h * 64, row);
-                }
-            } else {
-                // the page in which the shared tokens end: what lies behind them has weight zero and may be anything, infinities and NaN among
-                // them, so zeros take its place
-                const __nv_bfloat16* src = (const __nv_bfloat16*)p.v_cache + (size_t)row * p.d;
-                for (int i = lane; i < PAGE * HD / 8; i += 32) {
-                    const int key = i / (HD / 8), c = i % (HD / 8);
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (key < visible && c * 8 < p.d) v = *reinterpret_cast<const uint4*>(src + (size_t)key * p.d + c * 8);
-                    store_shared16(v_s + s * KV_BYTES + (c >> 3) * KEY_HALF_BYTES + key * 128 + (((c & 7) ^ (key & 7)) << 4), v);
-                }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(v_full + 8 * s);
+        if (lane == 0) {
+            for (int j = 0; j < n_tiles; ++j) {
+                const int s = j & 1, row = row_of_tile(j);
+                if (!mbar_wait(v_empty + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u, status, 1)) break;
+                mbar_expect_tx(v_full + 8 * s, KV_BYTES);
+                for (int h = 0; h < HALVES; ++h) tma_load_2d(v_s + s * KV_BYTES + h * KEY_HALF_BYTES, &map_v, v_full + 8 * s, h * 64, row);
             }
         }
     } else if (warp == 1) {
@@ -341,9 +365,9 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
         const int r = quarter * 32 + lane;                     // this thread's row = its tensor-memory lane
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
         const bool live = r < rows, idle = quarter * 32 >= rows;    // an idle warp's rows of P are whatever is there, and go nowhere
-        const int at = row0 + (live ? r : 0);
-        const int seq = member_at(p, group.first + at / per), head = kvh * per + at % per;
-        const int limit = live ? min(group.shared, p.seq_len[seq]) : 0;      // keys this row sees
+        const int mine = row0 + (live ? r : 0);
+        const int seq = member_at(p, of_group ? first + mine / per : first), head = kvh * per + (of_group ? mine % per : mine);
+        const int limit = live ? min(end, p.seq_len[seq]) : 0;               // the row sees the keys below this
         const float scale2 = p.scale * LOG2E;
         {
             const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + ((size_t)seq * p.nq + head) * p.d);
@@ -362,6 +386,20 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
             const int s = j & 1;
             ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * s, (uint32_t)(j >> 1) & 1u, status, 3));      // the warp is together from here on
             if (!ok) break;
+            const int pos0 = (tile_begin + j) * PAGE;
+            if (pos0 < begin || pos0 + PAGE > end) {
+                // A page in which the keys begin or end: what lies outside has weight zero and may be anything, infinities and NaN among them, so
+                // zeros take its values' place, a quarter of the page a warp, before the product may read it.
+                ok = __all_sync(0xffffffffu, mbar_wait(v_full + 8 * s, (uint32_t)(j >> 1) & 1u, status, 3));
+                if (!ok) break;
+                for (int i = lane; i < PAGE / 4 * (HD / 8); i += 32) {
+                    const int key = quarter * (PAGE / 4) + i / (HD / 8), c = i % (HD / 8);
+                    if (pos0 + key < begin || pos0 + key >= end)
+                        store_shared16(v_s + s * KV_BYTES + (c >> 3) * KEY_HALF_BYTES + key * 128 + (((c & 7) ^ (key & 7)) << 4), make_uint4(0, 0, 0, 0));
+                }
+                fence_async_shared();
+                __syncwarp();
+            }
             if (idle) {
                 if (lane == 0) mbar_arrive(p_full + 8 * s);
                 continue;
@@ -372,13 +410,12 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
             tmem_load32_start(s_addr, v[0]);
             tmem_load32_start(s_addr + 32, v[1]);
             tmem_wait_ld();
-            const int seen = limit - (tile_begin + j) * PAGE;  // keys of this tile that the row sees
-            if (seen < PAGE) {
+            if (limit - pos0 < PAGE || pos0 < begin) {
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
-                        if (q * 32 + c >= seen) v[q][c] = 0xff800000u;
+                        if (q * 32 + c >= limit - pos0 || q * 32 + c < begin - pos0) v[q][c] = 0xff800000u;
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -432,7 +469,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_full + 8 * ((n_tiles - 1) & 1), (uint32_t)((n_tiles - 1) >> 1) & 1u, status, 3));
         if (ok && !idle) {
             tc_fence_after();
-            const size_t slot = ((size_t)seq * p.nq + head) * (p.shared_ranges + p.own_ranges) + blockIdx.x;
+            const size_t slot = ((size_t)seq * p.nq + head) * stride + range;
             float* dst = p.part_acc + slot * p.d;
 #pragma unroll 1
             for (int c0 = 0; c0 < HD; c0 += 32) {
@@ -461,11 +498,69 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_prefix_tc_kernel(const _
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
 }
 
-// A member's own keys: the blocks of (16 query heads of a kv head, member) are a cluster along x, every warp of theirs walks tiles of 32 keys through a
-// two-stage cp.async ring of its own, rows behind the last key filled with zeros.  Then the blocks hand their sums to the first one, which joins them with
-// the shared ranges' and writes the result.
-constexpr int OWN_TILE = 32;
-constexpr int OWN_MAX_WARPS = 4;
+// What rows' partial results are multiplied by: row r of `rows` has `parts` of them, ml(r, k) their maximum and sum; a warp a row.
+template <typename ML>
+__device__ __forceinline__ void part_factors(float* factors, int rows, int parts, int warp, int warps, int lane, ML ml) {
+    constexpr int TURNS = (MAX_PARTS + 31) / 32;
+    for (int r = warp; r < rows; r += warps) {
+        float m_all = -INFINITY, l_all = 0.f, mk[TURNS], lk[TURNS];
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const int k = i * 32 + lane;
+            const float2 both = k < parts ? ml(r, k) : make_float2(-INFINITY, 0.f);
+            mk[i] = both.x; lk[i] = both.y;
+            m_all = fmaxf(m_all, both.x);
+        }
+        m_all = warp_max(m_all);
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            mk[i] = mk[i] == -INFINITY ? 0.f : fast_exp2(mk[i] - m_all);
+            l_all += lk[i] * mk[i];
+        }
+        l_all = warp_sum(l_all);
+        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;    // a row without a key is zero
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i)
+            if (i * 32 + lane < parts) factors[r * MAX_PARTS + i * 32 + lane] = mk[i] * inv;
+    }
+}
+__device__ __forceinline__ void add_part(float4& a, float4 v, float by) {      // a part without a key for the row may hold anything
+    if (by != 0.f) { a.x += v.x * by; a.y += v.y * by; a.z += v.z * by; a.w += v.w * by; }
+}
+
+// Joins the partial results of up to 16 query heads of a member's kv head.
+constexpr int JOIN_THREADS = 128;
+
+__global__ void __launch_bounds__(JOIN_THREADS) shared_join_parts_kernel(const SharedParams p) {
+    pdl_launch_dependents();
+    __shared__ float factors[16 * MAX_PARTS];
+    const int tid = threadIdx.x, per = p.nq / p.nkv, heads16 = (per + 15) / 16, stride = p.shared_ranges + p.own_ranges;
+    const int h0 = blockIdx.x % heads16 * 16, rows = min(16, per - h0), head0 = blockIdx.x / heads16 * per + h0;
+    pdl_wait();
+    const int seq = member_at(p, blockIdx.y), shared = group_of(p, blockIdx.y).shared;
+    const int of_group = Ranges(shared, PAGE, p.shared_ranges).used;
+    const int parts = of_group + OwnRanges(PAGE, shared, max(0, min(p.seq_len[seq], p.max_blocks * PAGE)), p.own_ranges).used;
+    const size_t row0 = (size_t)seq * p.nq + head0;
+    auto slot_of = [&](int k) { return k < of_group ? k : p.shared_ranges + k - of_group; };
+    part_factors(factors, rows, parts, tid >> 5, JOIN_THREADS / 32, tid & 31,
+                 [&](int r, int k) { return *reinterpret_cast<const float2*>(p.part_ml + 2 * ((row0 + r) * stride + slot_of(k))); });
+    __syncthreads();
+    const int quads = p.d / 4;
+    for (int i = tid; i < rows * quads; i += JOIN_THREADS) {
+        const int r = i / quads, c = i % quads * 4;
+        const float* acc = p.part_acc + (row0 + r) * stride * p.d + c;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int k = 0; k < parts; ++k) add_part(a, *reinterpret_cast<const float4*>(acc + (size_t)slot_of(k) * p.d), factors[r * MAX_PARTS + k]);
+        *reinterpret_cast<uint2*>((__nv_bfloat16*)p.out + (row0 + r) * p.d + c) = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
+    }
+}
+
+// One warp walks keys on mma.sync, the up to 16 query heads of a kv head as the rows, 16 keys at a time through a ring of four
+// stages of its own (cp.async, three tiles ahead), so that nothing in the loop waits for another warp.  Keys outside [begin, end) are zeros in shared memory:
+// their weight is zero, and what lies there may be anything, infinities and NaN among them.
+constexpr int WALK_TILE = 16;
+constexpr int WALK_STAGES = 4;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -482,17 +577,132 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int HD> __host__ __device__ constexpr uint32_t own_tile_bytes() { return OWN_TILE * HD * 2; }
-// Q; the warps' rings, where their sums go later; the cluster's inbox in the first block; what a row's partial results are multiplied by
-template <int HD> __host__ __device__ constexpr uint32_t own_rings(int warps) { return (uint32_t)warps * 4 * own_tile_bytes<HD>(); }
-template <int HD> constexpr size_t own_smem(int warps, int ranges, int rows) {
-    return 16 * HD * 2 + own_rings<HD>(warps) + (ranges > 1 ? (size_t)ranges * rows * (HD + 4) * 4 : 0) + (size_t)16 * (MAX_RANGES + 8) * 4;
+template <int HD> constexpr uint32_t WALK_BYTES = WALK_STAGES * 2 * WALK_TILE * HD * 2;      // a warp's ring
+
+// What a warp has of its rows g and g + 8 (lane = 4 g + t): maximum (base 2), this lane's share of the sum, columns 8 i + 2 t and the next.
+template <int HD> struct Walked { float m[2], l[2], o[HD / 8][4]; };
+
+// `heads` query heads from head0 on; `first`: the page list for positions below `shared`, `mine`: from there on.
+template <int HD>
+__device__ __forceinline__ void walk_keys(const SharedParams& p, Walked<HD>& w, int seq, int kvh, int head0, int heads, const int* first, const int* mine,
+                                          int shared, int begin, int end, uint32_t ring, int lane) {
+    constexpr int CHUNKS = HD / 8;                             // 16-byte pieces of a row
+    constexpr uint32_t ROW = HD * 2, TILE = WALK_TILE * ROW;
+    const int g = lane >> 2, t = lane & 3, mi = lane >> 3;
+    // swizzled rows: piece c of row r lies at piece c ^ (r & 7), so that the pieces that eight lanes of an ldmatrix name are in different banks
+    auto place = [](uint32_t row, uint32_t c) { return row * ROW + ((c ^ (row & 7u)) << 4); };
+    const int tile0 = begin / WALK_TILE, n_tiles = end > begin ? (end + WALK_TILE - 1) / WALK_TILE - tile0 : 0;
+    // page numbers of 32 pages at a time, one a lane: a look into the page list in front of every tile would put a round trip on its path
+    int pages_from = -1, page_first = 0, page_mine = 0;
+    auto issue = [&](int j) {
+        if (j < n_tiles) {
+            const int pos0 = (tile0 + j) * WALK_TILE, index = pos0 / PAGE;
+            if (pages_from < 0 || index >= pages_from + 32) {
+                pages_from = index;
+                const int at = min(index + lane, p.max_blocks - 1);
+                page_first = at * PAGE < shared ? page_at(p, first, at) : 0;
+                page_mine = (at + 1) * PAGE > shared ? page_at(p, mine, at) : 0;
+            }
+            const int of_first = __shfl_sync(0xffffffffu, page_first, index - pages_from), of_mine = __shfl_sync(0xffffffffu, page_mine, index - pages_from);
+            const uint32_t dst = ring + (uint32_t)(j % WALK_STAGES) * 2 * TILE;
+#pragma unroll
+            for (int i = 0; i < WALK_TILE * CHUNKS / 32; ++i) {
+                const int piece = i * 32 + lane, r = piece / CHUNKS, c = piece % CHUNKS, pos = pos0 + r;
+                const bool take = pos >= begin && pos < end && c * 8 < p.d;
+                const size_t from = take ? (((size_t)(pos < shared ? of_first : of_mine) * p.nkv + kvh) * PAGE + pos % PAGE) * p.d + c * 8 : 0;
+                cp_async16(dst + place(r, c), (const __nv_bfloat16*)p.k_cache + from, take);
+                cp_async16(dst + TILE + place(r, c), (const __nv_bfloat16*)p.v_cache + from, take);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int j = 0; j < WALK_STAGES - 1; ++j) issue(j);
+    uint32_t qf[HD / 16][4];                                   // rows g and g + 8, columns 16 ks + 2 t, + 8: as the product takes them
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = g + (e & 1) * 8, c = ks * 16 + (e >> 1) * 8 + 2 * t;
+            qf[ks][e] = r < heads && c < p.d ? *reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)p.q + ((size_t)seq * p.nq + head0 + r) * p.d + c) : 0u;
+        }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) { w.m[r] = -INFINITY; w.l[r] = 0.f; }
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) w.o[i][0] = w.o[i][1] = w.o[i][2] = w.o[i][3] = 0.f;
+    const float scale2 = p.scale * LOG2E;
+    for (int j = 0; j < n_tiles; ++j) {
+        issue(j + WALK_STAGES - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(WALK_STAGES - 1) : "memory");
+        __syncwarp();
+        const uint32_t k_s = ring + (uint32_t)(j % WALK_STAGES) * 2 * TILE, v_s = k_s + TILE;
+        const int pos0 = (tile0 + j) * WALK_TILE;
+        float s[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+            uint32_t b[4];
+            ldmatrix_x4(b, k_s + place((mi >> 1) * 8 + (lane & 7), ks * 2 + (mi & 1)));
+            mma_bf16(s[0], qf[ks], b[0], b[1]);
+            mma_bf16(s[1], qf[ks], b[2], b[3]);
+        }
+        if (pos0 < begin || pos0 + WALK_TILE > end) {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int pos = pos0 + nt * 8 + 2 * t + (e & 1);
+                    if (pos < begin || pos >= end) s[nt][e] = -INFINITY;
+                }
+        }
+        float alpha[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(w.m[r], mx * scale2), m_use = m_new == -INFINITY ? 0.f : m_new;
+            alpha[r] = fast_exp2(w.m[r] - m_use);
+            w.m[r] = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 2 * r; e < 2 * r + 2; ++e) {
+                    s[nt][e] = fast_exp2(fmaf(s[nt][e], scale2, -m_use));
+                    sum += s[nt][e];
+                }
+            w.l[r] = w.l[r] * alpha[r] + sum;
+        }
+        const uint32_t pa[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
+#pragma unroll
+        for (int n2 = 0; n2 < HD / 16; ++n2) {
+#pragma unroll
+            for (int i = 2 * n2; i < 2 * n2 + 2; ++i) { w.o[i][0] *= alpha[0]; w.o[i][1] *= alpha[0]; w.o[i][2] *= alpha[1]; w.o[i][3] *= alpha[1]; }
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, v_s + place((mi & 1) * 8 + (lane & 7), n2 * 2 + (mi >> 1)));
+            mma_bf16(w.o[2 * n2], pa, b[0], b[1]);
+            mma_bf16(w.o[2 * n2 + 1], pa, b[2], b[3]);
+        }
+        __syncwarp();                                          // the stage may be overwritten by the next issue
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 1);
+        w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 2);
+    }
+}
+
+// Everything in one launch, where so little is shared that a second launch costs more than reading it again (out of the L2 cache): the blocks of (16 query
+// heads of a kv head, member) are a cluster along x whose warps each walk a range of all of the member's keys; the first block joins the ranges.
+constexpr int DIRECT_MAX_WARPS = 6;
+
+template <int HD> constexpr size_t direct_smem(int warps, int ranges, int rows) {
+    return (size_t)warps * WALK_BYTES<HD> + (ranges > 1 ? (size_t)ranges * rows * (HD + 4) * 4 : 0) + 16 * MAX_PARTS * 4;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(32 * OWN_MAX_WARPS) shared_own_kernel(const SharedParams p) {
-    constexpr int CHUNKS = HD / 8;                             // 16-byte pieces of a row
-    constexpr uint32_t ROW = HD * 2, TILE = own_tile_bytes<HD>();
+__global__ void __launch_bounds__(32 * DIRECT_MAX_WARPS) shared_direct_kernel(const SharedParams p) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, threads = blockDim.x, warps = threads >> 5;
     if (gridDim.x > 1) cluster_arrive_started();
@@ -500,151 +710,44 @@ __global__ void __launch_bounds__(32 * OWN_MAX_WARPS) shared_own_kernel(const Sh
     const int per = p.nq / p.nkv, heads16 = (per + 15) / 16;
     const int kvh = blockIdx.y / heads16, h0 = blockIdx.y % heads16 * 16;
     const int rows = min(16, per - h0), head0 = kvh * per + h0;
-    const int seq = member_at(p, blockIdx.z), shared = group_of(p, blockIdx.z).shared;
+    pdl_wait();
+    const int seq = member_at(p, blockIdx.z);
+    const Group group = group_of(p, blockIdx.z);
     const int len = max(0, min(p.seq_len[seq], p.max_blocks * PAGE));
-    const int* table = p.block_table + (size_t)seq * p.max_blocks;
-    const int first_tile = min(shared, len) / OWN_TILE;
-    const int own_tiles = len > shared ? (len + OWN_TILE - 1) / OWN_TILE - first_tile : 0;
-    const int streams = gridDim.x * warps, stream = blockIdx.x * warps + warp;
-    const int per_stream = (own_tiles + streams - 1) / streams;
-    const int tile_begin = first_tile + stream * per_stream;
-    const int n_tiles = max(0, min(per_stream, first_tile + own_tiles - tile_begin));
-
-    // swizzled rows: 16-byte piece c of row r lies at piece c ^ (r & 7), so that eight rows' pieces are in eight different banks' groups
-    auto place = [](uint32_t row, uint32_t c) { return row * ROW + ((c ^ (row & 7u)) << 4); };
-    const uint32_t q_s = smem_u32(smem_raw), ring = q_s + 16 * ROW + warp * 4 * TILE;
-    for (int i = tid; i < 16 * CHUNKS; i += threads) {
-        const int r = i / CHUNKS, c = i % CHUNKS;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows && c * 8 < p.d) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + ((size_t)seq * p.nq + head0 + r) * p.d + c * 8);
-        store_shared16(q_s + place(r, c), v);
-    }
-    auto issue = [&](int j) {
-        if (j < n_tiles) {
-            const int tile = tile_begin + j, pos0 = tile * OWN_TILE;
-            const int page = page_at(p, table, pos0 / PAGE);
-            const size_t off = (((size_t)page * p.nkv + kvh) * PAGE + pos0 % PAGE) * p.d;
-            const __nv_bfloat16 *k = (const __nv_bfloat16*)p.k_cache + off, *v = (const __nv_bfloat16*)p.v_cache + off;
-            const uint32_t dst = ring + (uint32_t)(j & 1) * 2 * TILE;
-#pragma unroll
-            for (int i = 0; i < OWN_TILE * CHUNKS / 32; ++i) {
-                const int piece = i * 32 + lane, r = piece / CHUNKS, c = piece % CHUNKS;
-                const bool take = pos0 + r < len && c * 8 < p.d;
-                const size_t from = take ? (size_t)r * p.d + c * 8 : 0;
-                cp_async16(dst + place(r, c), k + from, take);
-                cp_async16(dst + TILE + place(r, c), v + from, take);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    issue(0);
-    __syncthreads();
-    uint32_t qf[HD / 16][4];
-#pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) ldmatrix_x4(qf[ks], q_s + place((lane & 7) + ((lane >> 3) & 1) * 8, ks * 2 + (lane >> 4)));
-
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[HD / 8][4] = {};
-    const float scale2 = p.scale * LOG2E;
-    const int mi = lane >> 3;
-    for (int j = 0; j < n_tiles; ++j) {
-        issue(j + 1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncwarp();
-        const uint32_t k_s = ring + (uint32_t)(j & 1) * 2 * TILE, v_s = k_s + TILE;
-        const int pos0 = (tile_begin + j) * OWN_TILE;
-        float s[4][4] = {};
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t b[4];
-                ldmatrix_x4(b, k_s + place(half * 16 + (mi >> 1) * 8 + (lane & 7), ks * 2 + (mi & 1)));
-                mma_bf16(s[2 * half], qf[ks], b[0], b[1]);
-                mma_bf16(s[2 * half + 1], qf[ks], b[2], b[3]);
-            }
-        if (pos0 < shared || pos0 + OWN_TILE > len) {
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int pos = pos0 + nt * 8 + 2 * t + (e & 1);
-                    if (pos < shared || pos >= len) s[nt][e] = -INFINITY;
-                }
-        }
-        float alpha[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float mx = fmaxf(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])),
-                             fmaxf(fmaxf(s[2][2 * r], s[2][2 * r + 1]), fmaxf(s[3][2 * r], s[3][2 * r + 1])));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m[r], mx * scale2), m_use = m_new == -INFINITY ? 0.f : m_new;
-            alpha[r] = fast_exp2(m[r] - m_use);
-            m[r] = m_new;
-            float sum = 0.f;
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-                for (int e = 2 * r; e < 2 * r + 2; ++e) {
-                    s[nt][e] = fast_exp2(fmaf(s[nt][e], scale2, -m_use));
-                    sum += s[nt][e];
-                }
-            l[r] = l[r] * alpha[r] + sum;                      // this thread's share of the row's sum
-        }
-        uint32_t pa[2][4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            pa[half][0] = pack_bf16(s[2 * half][0], s[2 * half][1]); pa[half][1] = pack_bf16(s[2 * half][2], s[2 * half][3]);
-            pa[half][2] = pack_bf16(s[2 * half + 1][0], s[2 * half + 1][1]); pa[half][3] = pack_bf16(s[2 * half + 1][2], s[2 * half + 1][3]);
-        }
-#pragma unroll
-        for (int n2 = 0; n2 < HD / 16; ++n2) {
-#pragma unroll
-            for (int i = 2 * n2; i < 2 * n2 + 2; ++i) { o[i][0] *= alpha[0]; o[i][1] *= alpha[0]; o[i][2] *= alpha[1]; o[i][3] *= alpha[1]; }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t b[4];
-                ldmatrix_x4_trans(b, v_s + place(half * 16 + (mi & 1) * 8 + (lane & 7), n2 * 2 + (mi >> 1)));
-                mma_bf16(o[2 * n2], pa[half], b[0], b[1]);
-                mma_bf16(o[2 * n2 + 1], pa[half], b[2], b[3]);
-            }
-        }
-        __syncwarp();                                          // the stage may be overwritten by the next issue
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const OwnRanges all(WALK_TILE, 0, len, gridDim.x * warps);
+    const int range = blockIdx.x * warps + warp;
+    Walked<HD> w;
+    walk_keys<HD>(p, w, seq, kvh, head0, rows, p.block_table + (size_t)member_at(p, group.first) * p.max_blocks, p.block_table + (size_t)seq * p.max_blocks,
+                  group.shared, all.begin(range), all.end(range), smem_u32(smem_raw) + warp * WALK_BYTES<HD>, lane);
     __syncthreads();
 
-    // the warps' sums through shared memory (the rings are free now)
-    float* sums = reinterpret_cast<float*>(smem_raw + 16 * ROW);              // [warps][16][HD]
-    float* sums_ml = sums + warps * 16 * HD;                                  // [warps][16][2]
+    // the warps' sums through shared memory (the rings are free now), the blocks' through the first one's inbox
+    constexpr int QUADS = HD / 4, SLOT = HD + 4;                              // a row in fours; with its maximum and its sum of weights
+    float* sums = reinterpret_cast<float*>(smem_raw);                         // [warps][rows][SLOT]
+    float* inbox = reinterpret_cast<float*>(smem_raw + warps * WALK_BYTES<HD>);                // [blocks][rows][SLOT] in the first block
+    float* factors = inbox + (gridDim.x > 1 ? gridDim.x * rows * SLOT : 0);   // [16][MAX_PARTS]
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (t == 0) { sums_ml[(warp * 16 + g + 8 * r) * 2] = m[r]; sums_ml[(warp * 16 + g + 8 * r) * 2 + 1] = l[r]; }
-    }
+        const int row = g + 8 * r;
+        if (row >= rows) continue;
+        float* slot = sums + (warp * rows + row) * SLOT;
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
-        const int c = i * 8 + 2 * t;
-        *reinterpret_cast<float2*>(sums + (warp * 16 + g) * HD + c) = make_float2(o[i][0], o[i][1]);
-        *reinterpret_cast<float2*>(sums + (warp * 16 + g + 8) * HD + c) = make_float2(o[i][2], o[i][3]);
+        for (int i = 0; i < HD / 8; ++i) *reinterpret_cast<float2*>(slot + i * 8 + 2 * t) = make_float2(w.o[i][2 * r], w.o[i][2 * r + 1]);
+        if (t == 0) *reinterpret_cast<float2*>(slot + HD) = make_float2(w.m[r], w.l[r]);
     }
     __syncthreads();
-    constexpr int QUADS = HD / 4, SLOT = HD + 4;                              // a row in fours; a row of the inbox: its sums, its maximum and its sum of weights
-    float* inbox = reinterpret_cast<float*>(smem_raw + 16 * ROW + own_rings<HD>(warps));       // [blocks][rows][SLOT] in the first block
-    float* factors = inbox + (gridDim.x > 1 ? gridDim.x * rows * SLOT : 0);   // [16][MAX_RANGES + 8]: by what partial results are multiplied
     if (gridDim.x > 1) {
         cluster_wait_started();
         for (int i = tid; i < rows * QUADS; i += threads) {
             const int r = i / QUADS, c = i % QUADS * 4;
             float m_all = -INFINITY, l_all = 0.f;
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = 0; w < warps; ++w) m_all = fmaxf(m_all, sums_ml[(w * 16 + r) * 2]);
-            for (int w = 0; w < warps; ++w) {
-                const float f = m_all == -INFINITY ? 0.f : fast_exp2(sums_ml[(w * 16 + r) * 2] - m_all);
-                const float4 v = *reinterpret_cast<const float4*>(sums + (w * 16 + r) * HD + c);
-                l_all += sums_ml[(w * 16 + r) * 2 + 1] * f;
-                a.x += v.x * f; a.y += v.y * f; a.z += v.z * f; a.w += v.w * f;
+            for (int k = 0; k < warps; ++k) m_all = fmaxf(m_all, sums[(k * rows + r) * SLOT + HD]);
+            for (int k = 0; k < warps; ++k) {
+                const float* slot = sums + (k * rows + r) * SLOT;
+                const float f = m_all == -INFINITY ? 0.f : fast_exp2(slot[HD] - m_all);
+                l_all += slot[HD + 1] * f;
+                add_part(a, *reinterpret_cast<const float4*>(slot + c), f);
             }
             float* slot = inbox + (size_t)(blockIdx.x * rows + r) * SLOT;
             cluster_store_float(slot + c, 0, a.x); cluster_store_float(slot + c + 1, 0, a.y);
@@ -652,55 +755,18 @@ __global__ void __launch_bounds__(32 * OWN_MAX_WARPS) shared_own_kernel(const Sh
             if (c == 0) { cluster_store_float(slot + HD, 0, m_all); cluster_store_float(slot + HD + 1, 0, l_all); }
         }
         cluster_barrier();
+        if (blockIdx.x > 0) return;
     }
-    pdl_wait();                                                               // the shared ranges' partial results
-    if (blockIdx.x > 0) return;
-    // What is left in the first block: the own partial results (the cluster's in the inbox, else the warps' sums) and the shared ranges'.
-    const int own = gridDim.x > 1 ? gridDim.x : warps, used = Ranges(shared, PAGE, p.shared_ranges).used, parts = own + used;
-    const int stride = p.shared_ranges + p.own_ranges;
-    auto own_ml = [&](int k, int r) { return gridDim.x > 1 ? inbox + (size_t)(k * rows + r) * SLOT + HD : sums_ml + (k * 16 + r) * 2; };
-    auto own_row = [&](int k, int r) { return gridDim.x > 1 ? inbox + (size_t)(k * rows + r) * SLOT : sums + (k * 16 + r) * HD; };
-    for (int r = warp; r < rows; r += warps) {                                // a warp a row: the maximum over the parts, then every part's factor
-        const float* ml = p.part_ml + ((size_t)seq * p.nq + head0 + r) * stride * 2;
-        float m_all = -INFINITY, l_all = 0.f;
-        float mk[(MAX_RANGES + 8 + 31) / 32], lk[(MAX_RANGES + 8 + 31) / 32];
-#pragma unroll
-        for (int i = 0; i < (MAX_RANGES + 8 + 31) / 32; ++i) {
-            const int k = i * 32 + lane;
-            float2 both = make_float2(-INFINITY, 0.f);
-            if (k < own) { const float* at = own_ml(k, r); both = make_float2(at[0], at[1]); }
-            else if (k < parts) both = *reinterpret_cast<const float2*>(ml + 2 * (k - own));
-            mk[i] = both.x; lk[i] = both.y;
-            m_all = fmaxf(m_all, both.x);
-        }
-        m_all = warp_max(m_all);
-#pragma unroll
-        for (int i = 0; i < (MAX_RANGES + 8 + 31) / 32; ++i) {
-            mk[i] = mk[i] == -INFINITY ? 0.f : fast_exp2(mk[i] - m_all);
-            l_all += lk[i] * mk[i];
-        }
-        l_all = warp_sum(l_all);
-        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-#pragma unroll
-        for (int i = 0; i < (MAX_RANGES + 8 + 31) / 32; ++i)
-            if (i * 32 + lane < parts) factors[r * (MAX_RANGES + 8) + i * 32 + lane] = mk[i] * inv;
-    }
+    const float* from = gridDim.x > 1 ? inbox : sums;
+    const int parts = gridDim.x > 1 ? gridDim.x : warps;
+    part_factors(factors, rows, parts, warp, warps, lane, [&](int r, int k) { return *reinterpret_cast<const float2*>(from + (size_t)(k * rows + r) * SLOT + HD); });
     __syncthreads();
     for (int i = tid; i < rows * QUADS; i += threads) {
         const int r = i / QUADS, c = i % QUADS * 4;
         if (c >= p.d) continue;
-        const size_t row = (size_t)seq * p.nq + head0 + r;
-        const float* f = factors + r * (MAX_RANGES + 8);
-        const float* acc = p.part_acc + row * stride * p.d + c;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](float4 v, float by) {                                  // a part without a key for this row may hold anything
-            if (by != 0.f) { a.x += v.x * by; a.y += v.y * by; a.z += v.z * by; a.w += v.w * by; }
-        };
-        for (int k = 0; k < own; ++k) add(*reinterpret_cast<const float4*>(own_row(k, r) + c), f[k]);
-#pragma unroll 8
-        for (int k = 0; k < used; ++k) add(*reinterpret_cast<const float4*>(acc + (size_t)k * p.d), f[own + k]);
-        uint2 packed = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
-        *reinterpret_cast<uint2*>((__nv_bfloat16*)p.out + row * p.d + c) = packed;
+        for (int k = 0; k < parts; ++k) add_part(a, *reinterpret_cast<const float4*>(from + (size_t)(k * rows + r) * SLOT + c), factors[r * MAX_PARTS + k]);
+        *reinterpret_cast<uint2*>((__nv_bfloat16*)p.out + ((size_t)seq * p.nq + head0 + r) * p.d + c) = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
     }
 }
 
@@ -717,50 +783,70 @@ int cache_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t d) {
 }
 
 template <int HD>
-int launch_tc(const SharedParams& p, int most_members, cudaStream_t stream) {
+int launch_parts(SharedParams p, int most_members, cudaStream_t stream) {
     CUtensorMap map_k, map_v;
     int rc = cache_map(&map_k, p.k_cache, (uint64_t)p.n_pages * p.nkv * PAGE, p.d);
     if (rc == QT_OK) rc = cache_map(&map_v, p.v_cache, (uint64_t)p.n_pages * p.nkv * PAGE, p.d);
     if (rc != QT_OK) return rc;
-    const int per = p.nq / p.nkv;
-    const size_t smem = (HD / 64) * (HALF_BYTES + 4 * KEY_HALF_BYTES) + 1024 + 192, smem_own = own_smem<HD>(p.own_warps, p.own_ranges, per < 16 ? per : 16);
-    cudaError_t raised = raise_shared<shared_prefix_tc_kernel<HD>>((int)smem);
-    if (raised == cudaSuccess) raised = raise_shared<shared_own_kernel<HD>>((int)smem_own);
+    const size_t smem = (HD / 64) * (HALF_BYTES + 4 * KEY_HALF_BYTES) + 1024 + 192;
+    const cudaError_t raised = raise_shared<shared_parts_kernel<HD>>((int)smem);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_shared: cannot raise shared memory: %s", cudaGetErrorString(raised));
-    const long long tiles = ((long long)most_members * per + BQ - 1) / BQ, y_own = (long long)p.nkv * ((per + 15) / 16);
-    QT_REQUIRE(tiles * p.nkv <= 65535 && y_own <= 65535 && p.n_groups <= 65535 && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
-    launch_kernel(shared_prefix_tc_kernel<HD>, dim3(p.shared_ranges, (unsigned)(tiles * p.nkv), p.n_groups), dim3(TC_THREADS), smem, stream, map_k, map_v, p);
-    launch_kernel_cluster(shared_own_kernel<HD>, dim3(p.own_ranges, (unsigned)y_own, p.n_seqs), dim3(32 * p.own_warps), smem_own, stream,
-                          (unsigned)p.own_ranges, p);
+    const int per = p.nq / p.nkv;
+    const long long tiles = ((long long)most_members * per + BQ - 1) / BQ, own_tiles = (per + BQ - 1) / BQ, heads = (long long)p.nkv * ((per + 15) / 16);
+    const long long shared = tiles * p.nkv * p.shared_ranges * p.n_groups, own = own_tiles * p.nkv * p.own_ranges * p.n_seqs;
+    QT_REQUIRE(shared + own <= 0x3fffffffll && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
+    p.row_tiles = (int)tiles; p.own_tiles = (int)own_tiles; p.shared_blocks = (int)shared; p.own_blocks = (int)own; p.turn = sm_count();
+    launch_kernel(shared_parts_kernel<HD>, dim3((unsigned)(shared + own)), dim3(TC_THREADS), smem, stream, map_k, map_v, p);
+    launch_kernel(shared_join_parts_kernel, dim3((unsigned)heads, p.n_seqs), dim3(JOIN_THREADS), 0, stream, p);
+    QT_CHECK_LAUNCH("attention_shared");
+    return QT_OK;
+}
+
+template <int HD>
+int launch_direct(const SharedParams& p, int warps, cudaStream_t stream) {
+    const int per = p.nq / p.nkv;
+    const size_t smem = direct_smem<HD>(warps, p.own_ranges, per < 16 ? per : 16);
+    QT_REQUIRE(smem <= 227 * 1024, "attention_shared: %d blocks of %d warps want %zu bytes of shared memory a block", p.own_ranges, warps, smem);
+    const cudaError_t raised = raise_shared<shared_direct_kernel<HD>>((int)smem);
+    if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_shared: cannot raise shared memory: %s", cudaGetErrorString(raised));
+    const long long heads = (long long)p.nkv * ((per + 15) / 16);
+    QT_REQUIRE(heads <= 65535 && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
+    launch_kernel_cluster(shared_direct_kernel<HD>, dim3(p.own_ranges, (unsigned)heads, p.n_seqs), dim3(32 * warps), smem, stream, (unsigned)p.own_ranges, p);
     QT_CHECK_LAUNCH("attention_shared");
     return QT_OK;
 }
 
 }  // namespace
 
-// on_tc: bfloat16, d % 8 == 0 and at most 128, pages of 64, own_ranges at most 8.
+// on_tc: bfloat16, d % 8 == 0 and at most 128, pages of 64.  With shared_ranges = 0 (on_tc) one launch walks all of a member's keys, by own_ranges <= 8
+// blocks of direct_warps warps a member and kv head.
 extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, const int* block_table,
                                           int max_blocks, const int* seq_len, const int* members, const int* share, int n_seqs, int n_groups,
                                           int most_members, int nq, int nkv, int d, int page_tokens, int n_pages, float scale, int shared_ranges,
-                                          int own_ranges, int own_warps, int on_tc, float* part_acc, float* part_ml, int* status, void* stream) {
+                                          int own_ranges, int direct_warps, int on_tc, float* part_acc, float* part_ml, int* status, void* stream) {
     QT_REQUIRE(n_seqs >= 0 && n_groups > 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_shared: bad head counts nq=%d nkv=%d (B=%d, %d groups)", nq, nkv, n_seqs, n_groups);
     QT_REQUIRE(d > 0 && d <= MAX_DIM && page_tokens > 0 && max_blocks > 0 && n_pages > 0, "attention_shared: bad sizes d=%d page=%d", d, page_tokens);
     QT_REQUIRE((long long)max_blocks * page_tokens <= 0x7fffffffll && most_members >= 0 && most_members <= n_seqs, "attention_shared: bad sizes: %d pages a sequence, %d members",
                max_blocks, most_members);
-    QT_REQUIRE(shared_ranges > 0 && own_ranges > 0 && shared_ranges + own_ranges <= MAX_RANGES, "attention_shared: %d and %d ranges", shared_ranges, own_ranges);
+    QT_REQUIRE(shared_ranges >= 0 && own_ranges > 0 && shared_ranges + own_ranges <= MAX_RANGES, "attention_shared: %d and %d ranges", shared_ranges, own_ranges);
     QT_REQUIRE(scale > 0.f && scale < INFINITY, "attention_shared: a score scale of %g (it must be positive)", (double)scale);
     if (n_seqs == 0) return QT_OK;
     const SharedParams p{q, k_cache, v_cache, out, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, nq, nkv, d, page_tokens, n_pages,
-                         scale, shared_ranges, own_ranges, part_acc, part_ml, own_warps, status};
+                         scale, shared_ranges, own_ranges, part_acc, part_ml, status, 0, 0, 0, 0, 0};
     cudaStream_t s = (cudaStream_t)stream;
     if (on_tc) {
-        QT_REQUIRE(dtype == QT_BF16 && d % 8 == 0 && d <= 128 && page_tokens == PAGE && own_ranges <= 8 && own_warps > 0 && own_warps <= OWN_MAX_WARPS && status,
+        QT_REQUIRE(dtype == QT_BF16 && d % 8 == 0 && d <= 128 && page_tokens == PAGE && status,
                    "attention_shared: the tensor-core kernels take bfloat16, heads of up to 128 in steps of 8, pages of 64 (d=%d, pages of %d)", d, page_tokens);
         QT_REQUIRE((long long)n_pages * nkv * PAGE <= 0x7fffffffll, "attention_shared: %d pages of %d heads are beyond a tensor map", n_pages, nkv);
         QT_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)part_acc | (uintptr_t)part_ml) & 15) == 0,
                    "attention_shared: operands must be 16-byte aligned");
-        return d <= 64 ? launch_tc<64>(p, most_members, s) : launch_tc<128>(p, most_members, s);
+        if (shared_ranges == 0) {
+            QT_REQUIRE(own_ranges <= 8 && direct_warps > 0 && direct_warps <= DIRECT_MAX_WARPS, "attention_shared: %d blocks of %d warps", own_ranges, direct_warps);
+            return d <= 64 ? launch_direct<64>(p, direct_warps, s) : launch_direct<128>(p, direct_warps, s);
+        }
+        return d <= 64 ? launch_parts<64>(p, most_members, s) : launch_parts<128>(p, most_members, s);
     }
+    QT_REQUIRE(shared_ranges > 0, "attention_shared: %d ranges of shared keys", shared_ranges);
     const long long items = (long long)n_seqs * nq * (shared_ranges + own_ranges);
     QT_REQUIRE(items / 4 < 0x7fffffffll, "attention_shared: too many rows for one launch");
     return QT_DISPATCH_DTYPE(dtype, "attention_shared", {

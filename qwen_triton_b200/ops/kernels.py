@@ -131,7 +131,7 @@ _SIGNATURES = {
     },
     "attention_shared": {
         # q, k_cache, v_cache, out, dtype, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, most_members, nq, nkv, d, page_tokens,
-        # n_pages, scale, shared_ranges, own_ranges, own_warps, on_tc, part_acc, part_ml, status, stream
+        # n_pages, scale, shared_ranges, own_ranges, direct_warps, on_tc, part_acc, part_ml, status, stream
         "qt_attention_decode_shared": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
                                        _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
     },
@@ -1398,7 +1398,7 @@ class SharedPlan:
     most_members: int
     shared_ranges: int            # ranges that a group's shared keys are cut into
     own_ranges: int               # ranges that a member's own keys are cut into
-    own_warps: int = 4            # warps that walk a range of a member's own keys
+    direct_warps: int = 4         # with shared_ranges 0: one launch walks all keys of every member, by own_ranges blocks of this many warps
 
     @property
     def ranges(self) -> int:
@@ -1434,12 +1434,11 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
         blocks = num_kv_heads * max(1, -(-most_members * group // 128))
         shared_ranges = max(1, min(32, 2 * sms // blocks, -(-most_shared // 128)))
         pairs = max(1, n_seqs * num_kv_heads * -(-group // 16))
-        own_warps = 2 if pairs >= sms else 4
-        own_ranges = max(1, min(8, -(-most_own // 512), 2 * sms // pairs))
+        own_ranges = max(1, min(16, -(-most_own // 128), max(-(-most_own // 1024), sms // pairs)))
     else:
         shared_ranges = max(1, min(32, -(-most_shared // 128)))
-        own_ranges, own_warps = max(1, min(8, -(-most_own // 256))), 4
-    return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges, own_warps)
+        own_ranges = max(1, min(8, -(-most_own // 256)))
+    return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges)
 
 
 def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
@@ -1473,8 +1472,8 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     on_tc = _shared_on_tc(q.dtype, head_dim) and page_tokens == 64
     _call("attention_shared", "qt_attention_decode_shared", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q, "q"), _ptr(block_table),
           block_table.shape[1], _ptr(seq_len), _ptr(members), _ptr(share), n_seqs, plan.groups, plan.most_members, num_heads, num_kv_heads, head_dim,
-          page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, plan.own_warps, int(on_tc), _ptr(part_acc), _ptr(part_ml),
-          _ptr(_status_word(q.device)), _stream(), launches=2 if n_seqs else 0)
+          page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, plan.direct_warps, int(on_tc), _ptr(part_acc), _ptr(part_ml),
+          _ptr(_status_word(q.device)), _stream(), launches=(2 if plan.shared_ranges else 1) if n_seqs else 0)
 
 
 # ----------------------------------------------------------------------------- experts chosen by a table

@@ -149,6 +149,13 @@ def test_every_cut_gives_the_result(shared_ranges, own_ranges, dtype):
     case.check(case.run(dataclasses.replace(case.plan, shared_ranges=shared_ranges, own_ranges=own_ranges)))
 
 
+@pytest.mark.parametrize("own_ranges,direct_warps", [(1, 1), (1, 4), (2, 3), (3, 6), (8, 2), (8, 4)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (6, 3, 48), (40, 2, 128), (5, 5, 80)])
+def test_one_launch_over_all_keys_gives_the_result(own_ranges, direct_warps, heads, kv_heads, dim):
+    case = Case([(777, [1, 300, 64]), (0, [90, None]), (130, [2, 2]), (9, [0, 1])], heads, kv_heads, dim, seed=7)
+    case.check(case.run(dataclasses.replace(case.plan, shared_ranges=0, own_ranges=own_ranges, direct_warps=direct_warps)))
+
+
 def test_scores_far_apart_and_one_key_far_above():
     """Running maxima that move by more than any rescaling step, upwards and downwards."""
     case = Case([(640, [100, 3])], 4, 2, 64, seed=8)
@@ -159,6 +166,28 @@ def test_scores_far_apart_and_one_key_far_above():
         case.k[case.table[0, 5], :, 10 + i] *= 20
     # members share pages, so what is equal stays equal; the copies of partly shared pages do not arise at 640 = 10 pages
     case.check(case.run())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("direct", [False, True])
+def test_shared_positions_are_read_through_the_first_members_list_only(dtype, direct):
+    """The other members' lists name pages of anything below the shared length, and what their own page holds below it counts for nothing."""
+    case = Case([(200, [40, 3, 100]), (64, [1, 70])], 8, 2, 64, dtype, seed=12)
+    want = case.run().clone()
+    case.check(want)
+    barred = case.k.shape[0] - 1
+    plan = dataclasses.replace(case.plan, shared_ranges=0, own_ranges=2, direct_warps=3) if direct and dtype == torch.bfloat16 else case.plan
+    truth = case.table.clone(), case.k.clone(), case.v.clone()
+    for first, count, shared in case.share.tolist():
+        for i in case.members[first + 1:first + count]:
+            if shared % PAGE:
+                page = int(case.table[i, shared // PAGE])
+                case.k[page, :, :shared % PAGE] = float("nan")
+                case.v[page, :, :shared % PAGE] = float("nan")
+            case.table[i, :shared // PAGE] = barred
+    out = case.run(plan)
+    case.table, case.k, case.v = truth
+    case.check(out)
 
 
 def test_the_same_call_gives_the_same_bits_and_follows_its_stream():
@@ -231,7 +260,12 @@ def test_refusals():
             (dict(plan=dataclasses.replace(case.plan, num_heads=8)), "plan")):
         with pytest.raises(KernelError, match=words):
             case.run(**changes)
-    for changes in (dict(shared_ranges=0), dict(own_ranges=0), dict(shared_ranges=1 << 20)):
+    for changes in (dict(shared_ranges=-1), dict(own_ranges=0), dict(shared_ranges=1 << 20), dict(shared_ranges=0, own_ranges=9), dict(shared_ranges=0, direct_warps=7),
+                    dict(shared_ranges=0, direct_warps=0)):
         with pytest.raises(KernelError):
             plan = dataclasses.replace(case.plan, **changes)
             case.run(plan, part_acc=torch.empty(max(plan.acc_elements, 1), device="cuda"), part_ml=torch.empty(max(plan.ml_elements, 1), device="cuda"))
+    wide = Case([(70, [1, 5])], 40, 2, 128)                   # more shared memory than a block has
+    with pytest.raises(KernelError, match="shared memory"):
+        wide.run(dataclasses.replace(wide.plan, shared_ranges=0, own_ranges=8, direct_warps=6))
+    wide.check(wide.run())                                    # and nothing of that stays behind
