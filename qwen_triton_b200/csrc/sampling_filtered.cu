@@ -11,6 +11,20 @@
 // of the largest: w has 24 bits, so a weight above 2^-16 loses nothing and a smaller one at most 2^-41, and no order of additions shows.
 // T <= 0 takes the lowest id of the largest logit (log-probability 0).  NaN counts as -inf; a row without anything above -inf gives id 0 with
 // log-probability -inf.
+//
+// A row is shared by a cluster of up to eight blocks, each with a part of the ids in shared memory, so that it comes from memory once.  What survives the filters
+// is a small head of the row as a rule, and is found without a look at the rest:
+//
+//   * the largest logit of every thread goes into 256 bins by its distance below the row's; where the bins' running count reaches top_k (or their
+//     mass p times the row's mass) lies a bound that at least so many tokens reach, and seldom many more;
+//   * the tokens above the bound go to the first block in vocabulary order (min_p gives a bound by itself); that block sorts their keys, finds the thresholds
+//     on the running count and mass, and draws.
+//
+// Only the row's mass for top_p without top_k takes an exponential a token, an approximate one (its error, 2^-22, is that of a sum in float).  A row whose head
+// does not fit the list finds its thresholds by bins of all of its tokens, three times by a factor of 256, and then by bisection; such a row, and one without
+// filters, draws over all blocks.
+//
+// Measured behind a cold cache: one row of 151,936 MEASURED_1, 64 rows MEASURED_64, 256 rows (156 MB) MEASURED_256.
 #include "common.cuh"
 
 #include <math.h>
@@ -19,143 +33,524 @@ using namespace qt;
 
 namespace {
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 512;
+constexpr int WARPS = THREADS / 32;
+constexpr int MAX_BLOCKS = 8;
+constexpr int BINS = 256;
+constexpr int LIST = 2048;             // tokens that the first block takes; a block of b hands over LIST / b at most
+constexpr int PER_THREAD = LIST / THREADS;
+constexpr float BINS_PER_NAT = 8.f;
+constexpr float LOG2E = 1.4426950408889634f;
 typedef unsigned long long u64;
-
-// Floats as unsigned integers of the same order; the two zeros share a key, NaN is -inf.
-__device__ __forceinline__ unsigned int ordered_key(float x) {
-    if (isnan(x)) x = -INFINITY;
-    unsigned int bits = __float_as_uint(x);
-    if (bits == 0x80000000u) bits = 0u;
-    return (bits & 0x80000000u) ? ~bits : (bits | 0x80000000u);
-}
-
-__device__ __forceinline__ float depth_of(float x, float mx, float t) { return (x == mx ? 0.f : (isnan(x) ? -INFINITY : x - mx)) / t; }
-__device__ __forceinline__ u64 units_of(float w) { return (u64)__float2ll_rn(w * 1099511627776.f); }
-
-__device__ u64 block_total(u64 v, u64* scratch) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[threadIdx.x & 31];
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
-}
 
 struct Rows {
     const float* logits; long long row_stride;
     const float* temperature; const int* top_k; const float* top_p; const float* min_p; const float* uniform;
     int* token; float* logprob;
-    int vocab;
+    int vocab, blocks, turns, cached;  // blocks a row; turns of a warp over its ids, 128 a turn; whether they are kept in shared memory
 };
 
-__global__ void __launch_bounds__(THREADS) sample_filtered_kernel(const Rows r) {
-    pdl_launch_dependents();
-    pdl_wait();
-    __shared__ u64 scratch[32];
-    __shared__ u64 warp_mass[32];
-    __shared__ float best[32];
-    const int at = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const float* row = r.logits + at * r.row_stride;
-    const float t = r.temperature[at];
-    float mx = -INFINITY;
-    for (int i = threadIdx.x; i < r.vocab; i += THREADS) mx = fmaxf(mx, row[i]);
-    mx = warp_max(mx);
-    if (lane == 0) best[warp] = mx;
-    __syncthreads();
-    mx = warp_max(best[lane]);
-    if (!(t > 0.f) || mx == -INFINITY) {
-        unsigned int first = 0x7fffffffu;
-        for (int i = threadIdx.x; i < r.vocab; i += THREADS)
-            if (row[i] == mx) { first = i; break; }
-        first = __reduce_min_sync(0xffffffffu, first);
-        if (lane == 0) scratch[warp] = first;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            u64 token = scratch[0];
-            for (int w = 1; w < 32; ++w) token = scratch[w] < token ? scratch[w] : token;
-            r.token[at] = mx == -INFINITY ? 0 : (int)token;
-            if (r.logprob) r.logprob[at] = mx == -INFINITY ? -INFINITY : 0.f;
-        }
-        return;
+// Floats as unsigned integers of the same order (no NaN comes here); the two zeros share a key.
+__device__ __forceinline__ unsigned int ordered_key(float x) {
+    unsigned int bits = __float_as_uint(x);
+    if (bits == 0x80000000u) bits = 0u;
+    return (bits & 0x80000000u) ? ~bits : (bits | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(unsigned int key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
+
+__device__ __forceinline__ float below(float x, float mx) { return x == mx ? 0.f : x - mx; }      // two equal infinities too
+// w in units of 2^-40, rounded to nearest even: two 20-bit steps, each exact in float.
+__device__ __forceinline__ u64 units_of(float w) {
+    const float high = w * 1048576.f;
+    const unsigned int whole = (unsigned int)high;
+    return ((u64)whole << 20) + __float2uint_rn((high - (float)whole) * 1048576.f);
+}
+
+__device__ __forceinline__ u64 warp_total(u64 v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+__device__ __forceinline__ u64 warp_prefix(u64 v, int lane) {                                     // inclusive
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const u64 other = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= off) v += other;
     }
-    unsigned int floor_key = 0;
-    const int k = r.top_k[at];
-    if (k > 0 && k < r.vocab) {                              // the lowest threshold above which fewer than k logits lie
-        unsigned int low = 0, high = ordered_key(mx);
+    return v;
+}
+
+__device__ __forceinline__ void remote_store(const u64* local, uint32_t rank, u64 value) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote), "l"(value) : "memory");
+}
+__device__ __forceinline__ unsigned int remote_load(const unsigned int* local, uint32_t rank) {
+    uint32_t remote;
+    unsigned int value;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(value) : "r"(remote) : "memory");
+    return value;
+}
+
+struct Shared {
+    u64 slots[2][MAX_BLOCKS][2];                 // two numbers of every block, by turns
+    u64 scratch[WARPS][2];
+    u64 per_warp[WARPS];
+    unsigned int bins[2][3][BINS];               // count, mass low, mass high, by turns
+    unsigned int bin_found;
+    u64 above;
+    int answer;
+};
+
+struct Row {
+    const Rows& r;
+    Shared& sh;
+    const float* row;
+    float4* kept;                                // this block's ids in shared memory
+    int rank, blocks, warp, lane, shift, quads, turn;
+    float mx, t;
+
+    // ids in fours from the 16-byte boundary at or before the row's start on; a place outside the row is -inf
+    __device__ __forceinline__ int quad_at(int i) const { return ((rank * WARPS + warp) * r.turns + i) * 32 + lane; }
+    __device__ __forceinline__ float4 load(int i) const {
+        const int q = quad_at(i), id = 4 * q - shift;
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (q < quads) {
+            if (id >= 0 && id + 4 <= r.vocab) {
+                v = *reinterpret_cast<const float4*>(row + id);
+            } else {
+                if (id >= 0 && id < r.vocab) v.x = row[id];
+                if (id + 1 >= 0 && id + 1 < r.vocab) v.y = row[id + 1];
+                if (id + 2 >= 0 && id + 2 < r.vocab) v.z = row[id + 2];
+                if (id + 3 >= 0 && id + 3 < r.vocab) v.w = row[id + 3];
+            }
+        }
+        return v;
+    }
+    static __device__ __forceinline__ float4 without_nan(float4 v) {
+        v.x = isnan(v.x) ? -INFINITY : v.x; v.y = isnan(v.y) ? -INFINITY : v.y;
+        v.z = isnan(v.z) ? -INFINITY : v.z; v.w = isnan(v.w) ? -INFINITY : v.w;
+        return v;
+    }
+    __device__ __forceinline__ float4 quad(int i) const { return r.cached ? kept[(warp * r.turns + i) * 32 + lane] : without_nan(load(i)); }
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        for (int i = 0; i < r.turns; ++i) {
+            const float4 v = quad(i);
+            f(v.x); f(v.y); f(v.z); f(v.w);
+        }
+    }
+
+    // the first read of the row: five turns' loads in flight, kept where they fit; this thread's largest
+    __device__ __forceinline__ float fetch() const {
+        float best = -INFINITY;
+        for (int i0 = 0; i0 < r.turns; i0 += 5) {
+            float4 v[5];
+#pragma unroll
+            for (int j = 0; j < 5; ++j) v[j] = i0 + j < r.turns ? load(i0 + j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll
+            for (int j = 0; j < 5; ++j) {
+                const float4 c = without_nan(v[j]);
+                best = fmaxf(best, fmaxf(fmaxf(c.x, c.y), fmaxf(c.z, c.w)));
+                if (r.cached && i0 + j < r.turns) kept[(warp * r.turns + i0 + j) * 32 + lane] = c;
+            }
+        }
+        return best;
+    }
+
+    __device__ __forceinline__ void barrier() const { if (blocks > 1) cluster_barrier(); else __syncthreads(); }
+    // Every block's two numbers (all of its first threads have them), seen by all: sh.slots[returned][block].
+    __device__ __forceinline__ int exchange(u64 a, u64 b) {
+        const int at = turn;
+        turn ^= 1;
+        if (threadIdx.x < blocks) {
+            if (blocks > 1) { remote_store(&sh.slots[at][rank][0], threadIdx.x, a); remote_store(&sh.slots[at][rank][1], threadIdx.x, b); }
+            else { sh.slots[at][0][0] = a; sh.slots[at][0][1] = b; }
+        }
+        barrier();
+        return at;
+    }
+    // Sums over the row of what every thread brings.
+    __device__ __forceinline__ u64 row_total(u64 v) {
+        v = warp_total(v);
+        __syncthreads();
+        if (lane == 0) sh.scratch[warp][0] = v;
+        __syncthreads();
+        v = warp_total(lane < WARPS ? sh.scratch[lane][0] : 0);
+        const int at = exchange(v, 0);
+        u64 all = 0;
+        for (int k = 0; k < blocks; ++k) all += sh.slots[at][k][0];
+        return all;
+    }
+    // The least and the largest.
+    __device__ __forceinline__ void row_ends(unsigned int& least, unsigned int& most) {
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        __syncthreads();
+        if (lane == 0) { sh.scratch[warp][0] = least; sh.scratch[warp][1] = most; }
+        __syncthreads();
+        least = __reduce_min_sync(0xffffffffu, lane < WARPS ? (unsigned int)sh.scratch[lane][0] : 0xffffffffu);
+        most = __reduce_max_sync(0xffffffffu, lane < WARPS ? (unsigned int)sh.scratch[lane][1] : 0u);
+        const int at = exchange(least, most);
+        for (int k = 0; k < blocks; ++k) {
+            least = min(least, (unsigned int)sh.slots[at][k][0]);
+            most = max(most, (unsigned int)sh.slots[at][k][1]);
+        }
+    }
+
+    __device__ __forceinline__ float depth(float x) const { return below(x, mx) / t; }
+    __device__ __forceinline__ u64 mass(float x) const { return units_of(expf(depth(x))); }
+
+    __device__ __forceinline__ void clear_bins(int at) const {
+        for (int i = threadIdx.x; i < 3 * BINS; i += THREADS) (&sh.bins[at][0][0])[i] = 0;
+    }
+    __device__ __forceinline__ void add_to_bin(int at, int bin, bool by_mass, u64 m) const {
+        if (!by_mass) { atomicAdd(&sh.bins[at][0][bin], 1u); return; }
+        const unsigned int low = (unsigned int)m, before = atomicAdd(&sh.bins[at][1][bin], low);
+        const unsigned int high = (unsigned int)(m >> 32) + (before > 0xffffffffu - low ? 1u : 0u);
+        if (high) atomicAdd(&sh.bins[at][2][bin], high);
+    }
+    // After a barrier behind the last addition: the first bin at which the running number over all blocks, started from `above`, reaches `wanted`; above: the
+    // number in front of it.  BINS where none does.
+    __device__ __forceinline__ int find_bin(int at, bool by_mass, double wanted, u64& above) {
+        if (threadIdx.x == 0) { sh.bin_found = BINS; sh.above = above; }
+        u64 n = 0, upto = 0;
+        if (threadIdx.x < BINS) {                             // a thread a bin, all blocks' loads in flight together
+            unsigned int low[MAX_BLOCKS], high[MAX_BLOCKS];
+#pragma unroll
+            for (int k = 0; k < MAX_BLOCKS; ++k) {
+                low[k] = k >= blocks ? 0 : blocks > 1 ? remote_load(&sh.bins[at][by_mass ? 1 : 0][threadIdx.x], k) : sh.bins[at][by_mass ? 1 : 0][threadIdx.x];
+                high[k] = k >= blocks || !by_mass ? 0 : blocks > 1 ? remote_load(&sh.bins[at][2][threadIdx.x], k) : sh.bins[at][2][threadIdx.x];
+            }
+#pragma unroll
+            for (int k = 0; k < MAX_BLOCKS; ++k) n += ((u64)high[k] << 32) + low[k];
+            upto = warp_prefix(n, lane);
+        }
+        __syncthreads();
+        if (threadIdx.x < BINS && lane == 31) sh.per_warp[warp] = upto;
+        __syncthreads();
+        if (threadIdx.x < BINS) {
+            for (int i = 0; i < warp; ++i) upto += sh.per_warp[i];
+            upto += above;
+            if ((double)upto >= wanted && ((threadIdx.x == 0) || (double)(upto - n) < wanted)) { sh.bin_found = threadIdx.x; sh.above = upto - n; }
+        }
+        __syncthreads();
+        above = sh.above;
+        return sh.bin_found;
+    }
+
+    // The lowest threshold above which (strictly) less than `wanted` of the tokens with a key of at least floor_key lies, their number or their mass.
+    __device__ unsigned int threshold(bool by_mass, double wanted, unsigned int floor_key) {
+        u64 above = 0;
+        int prefix = 0, level = 0;
+        float scale = BINS_PER_NAT / t;
+        auto place = [&](float x) {                           // of a token at this level; none: negative
+            if (ordered_key(x) < floor_key) return -1;
+            const float at = -below(x, mx) * scale;
+            const int index = at < 1073741824.f ? (int)at : 1073741824;
+            if (level == 0) return min(index, BINS - 1);
+            return index >> 8 == prefix ? index & (BINS - 1) : -1;
+        };
+        for (;;) {
+            clear_bins(level & 1);
+            __syncthreads();
+            each([&](float x) {
+                const int bin = place(x);
+                if (bin >= 0) add_to_bin(level & 1, bin, by_mass, by_mass ? mass(x) : 0);
+            });
+            barrier();
+            const int bin = find_bin(level & 1, by_mass, wanted, above);
+            if (bin == BINS) return floor_key;                // all of them are less than is wanted
+            if (level == 2 || (level == 0 && (bin == BINS - 1 || !(scale * 65536.f < INFINITY)))) { prefix = level ? (prefix << 8) + bin : bin; break; }
+            prefix = level ? (prefix << 8) + bin : bin;
+            ++level;
+            scale *= 256.f;
+        }
+        const bool last = level == 0;
+        auto inside = [&](float x) {
+            if (ordered_key(x) < floor_key) return false;
+            const float at = -below(x, mx) * scale;
+            const int index = at < 1073741824.f ? (int)at : 1073741824;
+            return (last ? min(index, BINS - 1) : index) == prefix;
+        };
+        unsigned int low = 0xffffffffu, high = 0;
+        each([&](float x) { if (inside(x)) { low = min(low, ordered_key(x)); high = max(high, ordered_key(x)); } });
+        row_ends(low, high);
         while (low < high) {
             const unsigned int mid = low + (high - low) / 2;
             u64 n = 0;
-            for (int i = threadIdx.x; i < r.vocab; i += THREADS) n += ordered_key(row[i]) > mid;
-            if (block_total(n, scratch) < (u64)k) high = mid; else low = mid + 1;
+            each([&](float x) { if (ordered_key(x) > mid && inside(x)) n += by_mass ? mass(x) : 1; });
+            if ((double)(above + row_total(n)) < wanted) high = mid; else low = mid + 1;
         }
-        floor_key = low;
+        barrier();                                            // the bins' readers are done
+        return low;
     }
-    auto mass_above = [&](unsigned int key, bool with) {
-        u64 m = 0;
-        for (int i = threadIdx.x; i < r.vocab; i += THREADS) {
-            const float x = row[i];
-            const unsigned int mine = ordered_key(x);
-            if (mine > key || (with && mine == key)) m += units_of(expf(depth_of(x, mx, t)));
-        }
-        return block_total(m, scratch);
-    };
-    const float p = r.top_p[at];
-    if (p < 1.f) {                                           // the lowest threshold above which less than p of the mass lies
-        const double target = (double)p * (double)mass_above(floor_key, true);
-        unsigned int low = floor_key, high = ordered_key(mx);
-        while (low < high) {
-            const unsigned int mid = low + (high - low) / 2;
-            if ((double)mass_above(mid, false) < target) high = mid; else low = mid + 1;
-        }
-        floor_key = low;
+
+    __device__ __forceinline__ u64 target_of(u64 total, float uniform) const {
+        const double wanted = floor((double)uniform * (double)total);
+        const u64 target = wanted > 0. ? (u64)wanted : 0;
+        return target < total ? target : total - 1;           // a number of 1 and more: the last token that stays
     }
-    const float least = fminf(r.min_p[at], 1.f);
-    const int chunk = ((r.vocab + 31) / 32 + 31) & ~31;      // ids a warp, in vocabulary order
-    const int begin = min(r.vocab, warp * chunk), end = min(r.vocab, begin + chunk);
-    auto mass_at = [&](int i) -> u64 {
-        if (i >= end) return 0;
-        const float x = row[i];
-        if (ordered_key(x) < floor_key) return 0;
-        const float w = expf(depth_of(x, mx, t));
-        return w < least ? 0 : units_of(w);
-    };
-    u64 mine = 0;
-    for (int i = begin + lane; i < end; i += 32) mine += mass_at(i);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
-    if (lane == 0) warp_mass[warp] = mine;
-    __syncthreads();
-    u64 total = 0, before = 0;
-    for (int w = 0; w < 32; ++w) { if (w == warp) before = total; total += warp_mass[w]; }
-    const double wanted = floor((double)r.uniform[at] * (double)total);
-    u64 target = wanted > 0. ? (u64)wanted : 0;
-    if (target >= total) target = total - 1;                 // a number of 1 and more: the last token that stays
-    if (before <= target && target < before + warp_mass[warp]) {
+    __device__ __forceinline__ void answer(int at, int token, float x, u64 total) const {
+        r.token[at] = token;
+        if (r.logprob) r.logprob[at] = depth(x) - logf((float)total * (1.f / 1099511627776.f));
+    }
+
+    // Draws among the tokens with a key of at least floor_key and a weight of at least `least`, over all blocks.
+    __device__ void draw(int at, unsigned int floor_key, float least) {
+        auto stays = [&](float x) -> u64 {
+            if (ordered_key(x) < floor_key) return 0;
+            const float w = expf(depth(x));
+            return w < least ? 0 : units_of(w);
+        };
+        u64 mine = 0;
+        each([&](float x) { mine += stays(x); });
+        mine = warp_total(mine);
+        __syncthreads();
+        if (lane == 0) sh.per_warp[warp] = mine;
+        __syncthreads();
+        u64 block = 0, before = 0;
+        for (int w = 0; w < WARPS; ++w) { if (w == warp) before = block; block += sh.per_warp[w]; }
+        const int slot = exchange(block, 0);
+        u64 total = 0;
+        for (int k = 0; k < blocks; ++k) { if (k == rank) before += total; total += sh.slots[slot][k][0]; }
+        const u64 target = target_of(total, r.uniform[at]);
+        if (!(before <= target && target < before + mine)) return;
         u64 running = before;
-        for (int i0 = begin; i0 < end; i0 += 32) {
-            const u64 m = mass_at(i0 + lane);
-            u64 prefix = m;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const u64 other = __shfl_up_sync(0xffffffffu, prefix, off);
-                if (lane >= off) prefix += other;
-            }
-            const unsigned int beyond = __ballot_sync(0xffffffffu, running + prefix > target);
+        for (int i = 0; i < r.turns; ++i) {
+            const float4 v = quad(i);
+            const u64 m[4] = {stays(v.x), stays(v.y), stays(v.z), stays(v.w)};
+            const u64 own = m[0] + m[1] + m[2] + m[3], upto = running + warp_prefix(own, lane);
+            const unsigned int beyond = __ballot_sync(0xffffffffu, upto > target);
             if (beyond) {
-                const int token = i0 + __ffs(beyond) - 1;
-                if (lane == 0) {
-                    r.token[at] = token;
-                    if (r.logprob) r.logprob[at] = depth_of(row[token], mx, t) - logf((float)total * (1.f / 1099511627776.f));
+                if (lane == __ffs(beyond) - 1) {
+                    u64 sum = upto - own;
+                    int e = 0;
+                    while (e < 3 && sum + m[e] <= target) sum += m[e++];
+                    answer(at, 4 * quad_at(i) - shift + e, e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w, total);
                 }
                 return;
             }
-            running += __shfl_sync(0xffffffffu, prefix, 31);
+            running = __shfl_sync(0xffffffffu, upto, 31);
         }
     }
+};
+
+// Inclusive prefix sums of PER_THREAD numbers a thread over the block; returns the whole.
+__device__ __forceinline__ u64 block_prefix(u64 (&v)[PER_THREAD], u64* per_warp, int warp, int lane) {
+#pragma unroll
+    for (int j = 1; j < PER_THREAD; ++j) v[j] += v[j - 1];
+    const u64 own = v[PER_THREAD - 1], upto = warp_prefix(own, lane);
+    __syncthreads();
+    if (lane == 31) per_warp[warp] = upto;
+    __syncthreads();
+    u64 base = upto - own, all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) { if (w < warp) base += per_warp[w]; all += per_warp[w]; }
+#pragma unroll
+    for (int j = 0; j < PER_THREAD; ++j) v[j] += base;
+    return all;
+}
+
+// n <= LIST keys, largest first (bitonic, the next power of two filled up with zeros).
+__device__ void sort_down(unsigned int* keys, int n) {
+    int size = 32;
+    while (size < n) size *= 2;
+    for (int i = n + threadIdx.x; i < size; i += THREADS) keys[i] = 0;
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < size / 2; i += THREADS) {
+                const int a = 2 * i - (i & (j - 1)), b = a + j;                  // the pair of this step
+                const unsigned int x = keys[a], y = keys[b];
+                if ((a & k) == 0 ? x < y : x > y) { keys[a] = y; keys[b] = x; }
+            }
+        }
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows r) {
+    pdl_launch_dependents();
+    if (r.blocks > 1) cluster_arrive_started();
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ Shared sh;
+    // the first block's: tokens above the bound as (key, id), by block and in vocabulary order; behind them the blocks' parts of the row, where the keys are sorted later
+    u64* list = reinterpret_cast<u64*>(smem);
+    float4* kept = reinterpret_cast<float4*>(smem + LIST * sizeof(u64));
+    const int blocks = r.blocks, rank = blockIdx.x % blocks, at = blockIdx.x / blocks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    const float* row = r.logits + at * r.row_stride;
+    const int shift = (int)(((uintptr_t)row >> 2) & 3);
+    Row w{r, sh, row, kept, rank, blocks, warp, lane, shift, (r.vocab + shift + 3) / 4, 0, -INFINITY, r.temperature[at]};
+    w.clear_bins(0);
+    const float own_best = w.fetch();
+    if (blocks > 1) cluster_wait_started();
+    {
+        unsigned int low = 0, high = ordered_key(own_best);
+        w.row_ends(low, high);
+        w.mx = of_key(high);
+    }
+    const float mx = w.mx, t = w.t;
+    if (!(t > 0.f) || mx == -INFINITY) {                       // the lowest id of the largest logit
+        unsigned int first = 0xffffffffu, unused = 0;
+        for (int i = 0; i < r.turns; ++i) {
+            const float4 v = w.quad(i);
+            const unsigned int id = 4 * w.quad_at(i) - shift;
+            if (first == 0xffffffffu) first = v.x == mx ? id : v.y == mx ? id + 1 : v.z == mx ? id + 2 : v.w == mx ? id + 3 : first;
+        }
+        w.row_ends(first, unused);
+        if (rank == 0 && threadIdx.x == 0) {
+            r.token[at] = mx == -INFINITY ? 0 : (int)first;
+            if (r.logprob) r.logprob[at] = mx == -INFINITY ? -INFINITY : 0.f;
+        }
+        w.barrier();
+        return;
+    }
+    const int k = r.top_k[at];
+    const float p = r.top_p[at], m = r.min_p[at], least = m > 0.f ? fminf(m, 1.f) : 0.f;
+    const bool by_count = k > 0 && k < r.vocab, by_mass = p < 1.f, by_weight = least > 0.f;
+    if (!by_count && !by_mass && !by_weight) {
+        w.draw(at, 0u, 0.f);
+        w.barrier();
+        return;
+    }
+    const float per_nat = LOG2E / t;
+    const bool whole = blocks == 1 && r.vocab <= LIST;         // the list takes the row as it is
+    bool fits = mx < INFINITY && per_nat < INFINITY && t < 1e30f;
+    float bound = -INFINITY;
+    double row_mass = 0.;                                      // for top_p alone, in units
+    if (fits && !whole) {
+        if (by_weight && !by_count) bound = mx + t * logf(least);
+        if (by_count || by_mass) {
+            const bool counting = by_count;
+            if (own_best > -INFINITY) w.add_to_bin(0, min((int)(-w.depth(own_best) * BINS_PER_NAT), BINS - 1), !counting, counting ? 0 : w.mass(own_best));
+            float sum = 0.f;
+            if (!counting) {
+                w.each([&](float x) {
+                    float e;
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x - mx) * per_nat));
+                    sum += e;
+                });
+                sum = warp_sum(sum);
+                if (lane == 0) sh.scratch[warp][1] = __float_as_uint(sum);
+                __syncthreads();
+                sum = warp_sum(lane < WARPS ? __uint_as_float((unsigned int)sh.scratch[lane][1]) : 0.f);
+            }
+            const int slot = w.exchange(__float_as_uint(sum), 0);
+            for (int b = 0; b < blocks; ++b) row_mass += (double)__uint_as_float((unsigned int)sh.slots[slot][b][0]);
+            row_mass *= 1099511627776.;
+            u64 above = 0;
+            const int bin = w.find_bin(0, !counting, counting ? (double)k : (double)p * row_mass, above);
+            // every token of the bins up to this one lies above the bound; the last bin has no end
+            if (bin < BINS - 1) bound = fmaxf(bound, mx - t * (float)(bin + 1) * (1.f / BINS_PER_NAT));
+        }
+        bound -= 1e-5f * (fabsf(mx) + fabsf(mx - bound));      // what the bound's and the bins' roundings are
+    }
+    if (fits) {
+        auto above = [&](float x) { return x > -INFINITY && !(x < bound); };
+        int n = 0;
+        w.each([&](float x) { n += above(x); });
+        n = __reduce_add_sync(0xffffffffu, n);
+        __syncthreads();
+        if (lane == 0) sh.per_warp[warp] = n;
+        __syncthreads();
+        int from = 0, mine = 0;
+        for (int i = 0; i < WARPS; ++i) { if (i < warp) from += (int)sh.per_warp[i]; mine += (int)sh.per_warp[i]; }
+        const int room = LIST / blocks;
+        if (mine <= room && n > 0) {
+            for (int i = 0; i < r.turns; ++i) {
+                const float4 v = w.quad(i);
+                const bool hit[4] = {above(v.x), above(v.y), above(v.z), above(v.w)};
+                const int own = hit[0] + hit[1] + hit[2] + hit[3];
+                if (!__any_sync(0xffffffffu, own)) continue;
+                const int upto = (int)warp_prefix(own, lane);
+                int slot = rank * room + from + upto - own;
+                const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (hit[e]) {
+                        const u64 entry = ((u64)ordered_key(x[e]) << 32) | (unsigned int)(4 * w.quad_at(i) - shift + e);
+                        if (blocks > 1) remote_store(list + slot, 0, entry); else list[slot] = entry;
+                        ++slot;
+                    }
+                from += __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        const int slot = w.exchange(mine, 0);
+        for (int b = 0; b < blocks; ++b) fits = fits && (int)sh.slots[slot][b][0] <= room;
+        if (fits) {
+            if (rank > 0) return;
+            // the first block alone: PER_THREAD neighbours of the list a thread
+            int count = 0;
+            for (int b = 0; b < blocks; ++b) count += (int)sh.slots[slot][b][0];
+            u64 entry[PER_THREAD];
+            unsigned int* keys = reinterpret_cast<unsigned int*>(kept);
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; ++j) {
+                int i = threadIdx.x * PER_THREAD + j, b = 0;
+                entry[j] = 0;
+                if (i >= count) continue;
+                const int to = i;
+                while (i >= (int)sh.slots[slot][b][0]) i -= (int)sh.slots[slot][b++][0];
+                entry[j] = list[b * room + i];
+                keys[to] = (unsigned int)(entry[j] >> 32);
+            }
+            unsigned int floor_key = 0;
+            if (by_count || by_mass) {
+                sort_down(keys, count);
+                if (by_count && k <= count) floor_key = keys[k - 1];
+                if (by_mass) {
+                    u64 upto[PER_THREAD], own[PER_THREAD];
+#pragma unroll
+                    for (int j = 0; j < PER_THREAD; ++j) {
+                        const int i = threadIdx.x * PER_THREAD + j;
+                        upto[j] = own[j] = i < count && keys[i] >= floor_key ? w.mass(of_key(keys[i])) : 0;
+                    }
+                    const u64 in_list = block_prefix(upto, sh.per_warp, warp, lane);
+                    const double wanted = (double)p * (by_count || whole ? (double)in_list : row_mass);
+                    // the last place in front of which less than that lies; the likeliest token stays whatever p is
+                    int last = 0;
+#pragma unroll
+                    for (int j = 0; j < PER_THREAD; ++j) {
+                        const int i = threadIdx.x * PER_THREAD + j;
+                        if (i < count && keys[i] >= floor_key && (double)(upto[j] - own[j]) < wanted) last = i;
+                    }
+                    last = __reduce_max_sync(0xffffffffu, last);
+                    if (lane == 0) sh.scratch[warp][0] = last;
+                    __syncthreads();
+                    last = __reduce_max_sync(0xffffffffu, lane < WARPS ? (int)sh.scratch[lane][0] : 0);
+                    floor_key = max(floor_key, keys[last]);
+                }
+            }
+            u64 upto[PER_THREAD], own[PER_THREAD];
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; ++j) {
+                const unsigned int key = (unsigned int)(entry[j] >> 32);
+                own[j] = 0;
+                if (threadIdx.x * PER_THREAD + j < count && key >= floor_key) {
+                    const float weight = expf(w.depth(of_key(key)));
+                    own[j] = weight < least ? 0 : units_of(weight);
+                }
+                upto[j] = own[j];
+            }
+            const u64 total = block_prefix(upto, sh.per_warp, warp, lane);
+            const u64 target = w.target_of(total, r.uniform[at]);
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; ++j)
+                if (upto[j] > target && upto[j] - own[j] <= target) w.answer(at, (int)(unsigned int)entry[j], of_key((unsigned int)(entry[j] >> 32)), total);
+            return;
+        }
+    }
+    unsigned int floor_key = 0;
+    if (by_count) floor_key = w.threshold(false, (double)k, 0u);
+    if (by_mass) {
+        u64 all = 0;
+        w.each([&](float x) { if (ordered_key(x) >= floor_key) all += w.mass(x); });
+        const double wanted = (double)p * (double)w.row_total(all);
+        floor_key = wanted > 0. ? w.threshold(true, wanted, floor_key) : ordered_key(mx);
+    }
+    w.draw(at, floor_key, least);
+    w.barrier();
 }
 
 }  // namespace
@@ -164,10 +559,23 @@ __global__ void __launch_bounds__(THREADS) sample_filtered_kernel(const Rows r) 
 // logprob float [rows] or null.
 extern "C" int qt_sample_filtered(const float* logits, long long row_stride, const float* temperature, const int* top_k, const float* top_p,
                                   const float* min_p, const float* uniform, int* token, float* logprob, int rows, int vocab, void* stream) {
-    QT_REQUIRE(rows >= 0 && vocab > 0 && (rows <= 1 || row_stride >= vocab), "sample_filtered: bad sizes rows=%d vocab=%d stride=%lld", rows, vocab, row_stride);
+    QT_REQUIRE(rows >= 0 && vocab > 0 && vocab <= 0x3fffffff && (rows <= 1 || row_stride >= vocab), "sample_filtered: bad sizes rows=%d vocab=%d stride=%lld",
+               rows, vocab, row_stride);
     if (rows == 0) return QT_OK;
-    const Rows r{logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, vocab};
-    launch_kernel(sample_filtered_kernel, dim3(rows), dim3(THREADS), 0, (cudaStream_t)stream, r);
+    QT_REQUIRE(rows <= 0x7fffffff / MAX_BLOCKS, "sample_filtered: %d rows are more than one launch takes", rows);
+    // so many blocks a row that two of them fit an SM, and more where rows are few, down to 4,096 ids a block
+    int blocks = 1;
+    while (blocks < MAX_BLOCKS && (vocab / blocks > 20480 || (vocab / blocks > 8192 && (long long)rows * blocks < sm_count()))) blocks *= 2;
+    const int quads = (vocab + 3 + 3) / 4, turns = (quads + blocks * THREADS - 1) / (blocks * THREADS);
+    size_t part = (size_t)turns * THREADS * sizeof(float4);
+    const int cached = part <= 200 * 1024;                     // a longer part is read again
+    if (!cached) part = 0;
+    if (part < LIST * sizeof(unsigned int)) part = LIST * sizeof(unsigned int);
+    const size_t smem = LIST * sizeof(u64) + part;
+    const cudaError_t raised = raise_shared<sample_filtered_kernel>((int)smem);
+    if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "sample_filtered: cannot raise shared memory: %s", cudaGetErrorString(raised));
+    const Rows r{logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, vocab, blocks, turns, cached};
+    launch_kernel_cluster(sample_filtered_kernel, dim3((unsigned)(rows * blocks)), dim3(THREADS), smem, (cudaStream_t)stream, (unsigned)blocks, r);
     QT_CHECK_LAUNCH("sample_filtered");
     return QT_OK;
 }

@@ -29,18 +29,19 @@ def kept_of(x, temperature, k, p, m):
     return torch.where(kept, w, 0.0), y
 
 
-def margins(x, temperature, k, p, m):
-    """How near the nearest token is to the other side of a filter: relative to the row's mass (top_p) and to the weight (min_p)."""
-    w_all, y = kept_of(x, temperature, k, 1.0, 0.0)
-    near = math.inf
+def settled(x, temperature, k, p, m):
+    """(p, m) moved to where no rounding decides: p into the middle of the two running masses around it, m between two weights."""
+    w, _ = kept_of(x, temperature, k, 1.0, 0.0)
     if p < 1:
         values, inverse = x.double().unique(return_inverse=True)
-        mass = torch.zeros_like(values).scatter_add_(0, inverse, w_all)
-        above = mass.flip(0).cumsum(0).flip(0) - mass
-        near = float(((above - p * mass.sum()).abs() / mass.sum()).min())
+        mass = torch.zeros_like(values).scatter_add_(0, inverse, w).flip(0).cumsum(0) / w.sum()
+        i = int((mass < p).sum())
+        p = (float(mass[i - 1] if i else 0.0) + float(mass[min(i, len(mass) - 1)])) / 2
     if 0 < m < 1:
-        near = min(near, float((w_all[w_all > 0] / m - 1).abs().min()))
-    return near
+        ordered = w[w > 0].unique()
+        i = int((ordered < m).sum())
+        m = (float(ordered[i - 1] if i else 0.0) + float(ordered[min(i, len(ordered) - 1)])) / 2
+    return p, m
 
 
 def middle(weights, gen):
@@ -75,8 +76,7 @@ def check(logits, params, seed):
     gen = torch.Generator().manual_seed(seed)
     rows = []
     for x, (t, k, p, m) in zip(logits.cpu(), params):
-        while margins(x, t, k, p, m) < 1e-5:                  # settled before the kernel sees the row
-            p, m = (p - 1e-3 if p < 1 else p), (m * 1.01 if m else m)
+        p, m = settled(x, t, k, p, m)
         weights, y = kept_of(x, t, k, p, m)
         token, u = middle(weights, gen)
         rows.append((t, k, p, m, u, token, float(y[token] - weights.sum().log()), float(y[token])))
@@ -90,7 +90,7 @@ PARAMS = [(1.0, 0, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (0.8, 0, 0.9, 0.0), (1.0, 0, 
           (1.0, 3, 0.7, 0.0), (0.05, 0, 0.9, 0.1), (5.0, 400, 0.99, 0.001), (1.0, 100000, 0.8, 0.0), (1.0, 7, 1.0, 0.9)]
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 199, 503, 1024, 4099, 32000, 50257, 151936, 151937, 262144])
+@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 199, 503, 1024, 4099, 32000, 50257, 151936, 151937, 262144, 500001])
 def test_every_filter_at_many_sizes(vocab):
     gen = torch.Generator().manual_seed(vocab)
     logits = 2.5 * torch.randn((len(PARAMS), vocab), generator=gen)
@@ -163,6 +163,27 @@ def test_rows_apart_and_odd_addresses():
     view = wide[:, 3:10000]
     check(view, PARAMS, 8)
     check(wide[::2, 1:1002], PARAMS[::2], 9)
+
+
+@pytest.mark.parametrize("vocab", [6000, 151936])
+def test_heads_that_fit_no_list(vocab):
+    """Flat rows: what stays is a large part of the vocabulary, by count, by mass and by both."""
+    gen = torch.Generator().manual_seed(vocab)
+    params = [(1.0, vocab // 2, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.0, vocab // 3, 0.9, 0.0), (3.0, 0, 0.99, 0.02), (0.9, vocab - 1, 0.5, 0.0), (1.0, 5000, 0.99, 0.0),
+              (2.0, 2500, 1.0, 0.0), (1e-3, 3000, 0.999, 0.0), (1e4, 0, 0.3, 0.0), (1.0, 0, 1.0, 1e-4), (1.0, 3000, 1.0, 1e-9), (50.0, 0, 0.5, 0.9)]
+    logits = torch.randn((len(params), vocab), generator=gen)
+    logits[::2] = (logits[::2] * 8).round() / 8               # hundreds of tokens to a value
+    check(logits.cuda(), params, vocab)
+
+
+def test_tokens_that_stand_out_side_by_side():
+    """More of them in one block's part of the row than a part of the list holds, and all of them in one thread's."""
+    logits = torch.randn((4, 151936), generator=torch.Generator().manual_seed(12)) - 20
+    logits[0, 1000:1700] += 25
+    logits[1, 40000:40004] += 25
+    logits[2, 151900:] += 30
+    logits[3, :300] += 25
+    check(logits.cuda(), [(1.0, 500, 1.0, 0.0), (1.0, 3, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (0.8, 299, 0.95, 0.001)], 13)
 
 
 def test_no_order_of_additions_shows_and_the_stream_is_followed():
