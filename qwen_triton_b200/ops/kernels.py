@@ -1701,14 +1701,6 @@ def sample_keyed(logits: torch.Tensor, temperature: float, seed: int, keys: torc
           _ptr(out), rows, logits.shape[1], int(top_k), float(top_p), _stream())
 
 
-def _filtered_launches(rows: int, vocab: int) -> int:
-    """Launches of qt_sample_filtered (its rule): a second one for the rows that a list does not settle, where a row has few blocks for its ids."""
-    blocks, sms = 1, sm_count()
-    while blocks < 8 and rows * blocks * 2 <= 2 * sms and vocab // blocks > 8192:
-        blocks *= 2
-    return 1 if vocab // blocks <= 20480 else 2
-
-
 def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
                     uniform: torch.Tensor, out: torch.Tensor, logprob: torch.Tensor | None = None) -> None:
     """One token per row of float logits [rows, vocab] (rows may lie further apart than they are long), with parameters of the row's own, all on the
@@ -1729,7 +1721,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     if logprob is not None:
         _need(logprob, "logprob", torch.float32, (rows,))
     _call("sampling_filtered", "qt_sample_filtered", _ptr(logits), logits.stride(0) if rows > 1 else vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
-          _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(logprob), rows, vocab, _stream(), launches=_filtered_launches(rows, vocab) if rows else 0)
+          _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(logprob), rows, vocab, _stream(), launches=1 if rows else 0)
 
 
 _STATUS: dict[int, torch.Tensor] = {}
