@@ -6,6 +6,10 @@ Pages are ``page_tokens`` positions long.  A group that keeps all keys takes pag
 grows; a group that keeps a window of them takes at most ``ring_pages`` and reuses them as a ring.
 Slots and pages go back to their free lists when the sequence ends and are handed out again.
 
+A sequence may start with the leading whole pages of another one (``alloc(prefix_of, tokens)``): such a page is held by
+several slots, nobody writes to it any more (a sequence writes at its length and beyond), and it goes back to the free list when the
+last of them ends.  Groups that keep a window reuse their pages and cannot be shared.
+
 No device memory is touched here, so the invariants (no slot or page lost, held twice or freed
 twice) can be checked without a GPU.  The reference keeps one length for the whole batch and grows
 its tensors by reallocation (qwen_triton/modules/cache.py:21-65).
@@ -35,6 +39,7 @@ class GroupGeometry:
 class _Slot:
     length: int = 0
     pages: list[list[int]] = field(default_factory=list)   # per group
+    shared: int = 0                                        # leading pages taken from another slot
 
 
 class CacheBook:
@@ -48,21 +53,50 @@ class CacheBook:
         self._free_slots = list(range(num_slots - 1, -1, -1))         # pop() hands out the lowest number first
         self._free_pages = [list(range(g.num_pages - 1, -1, -1)) for g in self.groups]
         self._live: dict[int, _Slot] = {}
+        self._holders: list[dict[int, int]] = [{} for _ in self.groups]   # pages held by more than one slot, and by how many
+        self._sharers = 0                                                 # live slots that started with another one's pages
 
     # ------------------------------------------------------------------ slots
-    def alloc(self) -> int:
+    def alloc(self, prefix_of: int | None = None, tokens: int = 0) -> int:
+        """A slot for a new sequence, empty, or with the first ``tokens`` (whole pages) of the sequence in ``prefix_of``."""
+        source = None
+        if prefix_of is not None:
+            source = self._entry(prefix_of)
+            if tokens <= 0 or tokens % self.page_tokens or tokens > source.length:
+                raise CacheError(f"slot {prefix_of}: {tokens} of its {source.length} tokens are not whole pages of {self.page_tokens}")
+            if any(g.ring_pages for g in self.groups):
+                raise CacheError("pages of a windowed cache group are used again and cannot be shared")
         if not self._free_slots:
             raise CacheFull(f"all {self.num_slots} sequence slots are in use")
         slot = self._free_slots.pop()
-        self._live[slot] = _Slot(0, [[] for _ in self.groups])
+        entry = self._live[slot] = _Slot(0, [[] for _ in self.groups])
+        if source is not None:
+            entry.length, entry.shared = tokens, tokens // self.page_tokens
+            self._sharers += 1
+            for held, holders, pages in zip(source.pages, self._holders, entry.pages):
+                pages.extend(held[:entry.shared])
+                for page in pages:
+                    holders[page] = holders.get(page, 1) + 1
         return slot
 
     def free(self, slot: int) -> None:
         entry = self._live.pop(slot, None)
         if entry is None:
             raise CacheError(f"slot {slot} is not in use (freed twice, or never allocated)")
+        self._sharers -= entry.shared > 0
         for group, pages in enumerate(entry.pages):
-            self._free_pages[group].extend(reversed(pages))
+            holders = self._holders[group]
+            if not holders:
+                self._free_pages[group].extend(reversed(pages))
+                continue
+            for page in reversed(pages):
+                count = holders.get(page, 1)
+                if count == 1:
+                    self._free_pages[group].append(page)
+                elif count == 2:
+                    del holders[page]
+                else:
+                    holders[page] = count - 1
         self._free_slots.append(slot)
 
     def is_live(self, slot: int) -> bool:
@@ -115,6 +149,40 @@ class CacheBook:
     def pages(self, slot: int, group: int) -> list[int]:
         return self._entry(slot).pages[group]
 
+    def shared_groups(self, slots: list[int]) -> list[tuple[list[int], int]]:
+        """Which of ``slots`` share leading tokens: (places in ``slots``, tokens that all of them hold on the same pages) for every group of two and more, and
+        one group of the rest with 0 tokens, if there is a rest.  Empty where none do."""
+        if not self._sharers or not self.groups:
+            return []
+        by_page: dict[int, list[int]] = {}
+        alone: list[int] = []
+        for place, slot in enumerate(slots):
+            pages = self._entry(slot).pages[0]
+            if pages:
+                by_page.setdefault(pages[0], []).append(place)
+            else:
+                alone.append(place)
+        groups = []
+        for places in by_page.values():
+            if len(places) == 1:
+                alone += places
+                continue
+            # A page that two sequences both hold at a place has the same pages in front of it in both.  The pages taken from another sequence are
+            # common to all as a rule (not where that sequence is not among these); what is, lies below that.
+            entries = [self._entry(slots[p]) for p in places]
+            high = common = min(entry.shared for entry in entries if entry.shared)
+            low, first = 1, entries[0].pages[0]
+            while low <= high:
+                if all(len(entry.pages[0]) >= common and entry.pages[0][common - 1] == first[common - 1] for entry in entries):
+                    low = common + 1
+                else:
+                    high = common - 1
+                common = (low + high + 1) // 2 if low <= high else high
+            groups.append((places, common * self.page_tokens))
+        if groups and alone:
+            groups.append((alone, 0))
+        return groups
+
     def free_pages(self, group: int) -> int:
         return len(self._free_pages[group])
 
@@ -128,7 +196,12 @@ class CacheBook:
         if sorted(slots) != list(range(self.num_slots)):
             raise CacheError(f"slot accounting is broken: {sorted(slots)}")
         for group, geometry in enumerate(self.groups):
-            held = [p for entry in self._live.values() for p in entry.pages[group]]
-            everything = self._free_pages[group] + held
+            held: dict[int, int] = {}
+            for entry in self._live.values():
+                for page in entry.pages[group]:
+                    held[page] = held.get(page, 0) + 1
+            if {page: n for page, n in held.items() if n > 1} != self._holders[group]:
+                raise CacheError(f"page accounting of group {group} is broken: pages held more than once")
+            everything = self._free_pages[group] + list(held)
             if sorted(everything) != list(range(geometry.num_pages)):
                 raise CacheError(f"page accounting of group {group} is broken")

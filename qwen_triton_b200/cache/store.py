@@ -16,7 +16,7 @@ import torch
 
 from ..ops import kernels
 from ..parts.base import KVRequest, StateRequest
-from .book import CacheBook, GroupGeometry
+from .book import CacheBook, CacheError, GroupGeometry
 
 
 @dataclass
@@ -141,8 +141,15 @@ class SequenceCache:
         return views[0] if count is None else tuple(views)
 
     # ------------------------------------------------------------------ slots
-    def alloc(self) -> int:
-        slot = self.book.alloc()
+    @property
+    def can_share(self) -> bool:
+        """Whether a sequence may start with another one's pages: everything that is kept per sequence is in pages that keep every position."""
+        return bool(self.groups) and not self.has_window and not self._state_of
+
+    def alloc(self, prefix_of: int | None = None, tokens: int = 0) -> int:
+        if prefix_of is not None and not self.can_share:
+            raise CacheError("this model keeps more per sequence than pages of all its positions: no sequence can start with another one's")
+        slot = self.book.alloc(prefix_of, tokens)
         if self._row_table is not None:
             with torch.cuda.device(self.device):
                 kernels.zero_rows(*self._row_table, slot)

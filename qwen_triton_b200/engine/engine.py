@@ -27,7 +27,7 @@ from ..ops import kernels
 from ..parts.base import Runtime, Workspace
 from ..weights import open_checkpoint, random_source
 from .model import CausalLM, expected_tensors
-from .step import StepContext, StepEntry, plan_passes
+from .step import StepContext, StepEntry, plan_passes, shared_shape
 
 _DTYPES = {
     "bf16": torch.bfloat16, "bfloat16": torch.bfloat16, "fp32": torch.float32, "float32": torch.float32,
@@ -159,9 +159,19 @@ class Engine:
         return self.cache.num_slots
 
     # ------------------------------------------------------------------ sequences
-    def new_sequence(self) -> int:
-        """Take a slot for a sequence that starts at position 0."""
-        return self.cache.alloc()
+    @property
+    def can_share(self) -> bool:
+        """Whether a sequence may start with another one's cached tokens."""
+        return self.cache.can_share
+
+    def new_sequence(self, prefix_of: int | None = None, tokens: int | None = None) -> int:
+        """Take a slot for a sequence that starts at position 0, or with the first ``tokens`` (whole pages; default: all of its whole pages) of the sequence in
+        ``prefix_of``, whose keys and values it then shares.  Sequences that share their first pages are read together in one-token steps."""
+        if prefix_of is None:
+            return self.cache.alloc()
+        if tokens is None:
+            tokens = self.length(prefix_of) // self.page_tokens * self.page_tokens
+        return self.cache.alloc(prefix_of, tokens)
 
     def release(self, slot: int) -> None:
         """Give back the slot and every page the sequence holds."""
@@ -357,9 +367,16 @@ class Engine:
             tables.append(table)
         context = -(-(max(past) + 1) // 1024) * 1024
         pad = padded - count
-        prepared = self._ctx.prepare_decode(slots + [cache.dummy_slot] * pad, past + [0] * pad, tables)
+        groups, shape = book.shared_groups(slots), None
+        if groups:
+            if pad:                                              # padded rows: one token of their own
+                if groups[-1][1]:
+                    groups.append(([], 0))
+                groups[-1][0].extend(range(count, padded))
+            shape = shared_shape(groups, [p + 1 for p in past] + [1] * pad)
+        prepared = self._ctx.prepare_decode(slots + [cache.dummy_slot] * pad, past + [0] * pad, tables, groups, shape)
         return PlannedDecode(slots=tuple(slots), lengths=tuple(p + 1 for p in past), count=count, padded=padded,
-                             key=(padded, tuple(widths), context), context=context, prepared=prepared)
+                             key=(padded, tuple(widths), context, shape), context=context, prepared=prepared)
 
     def _run_planned(self, plan: "PlannedDecode", tokens: list[int], chosen: torch.Tensor | None = None) -> torch.Tensor:
         cache, count, padded = self.cache, plan.count, plan.padded

@@ -24,6 +24,7 @@ from .step import StepEntry
 class GenerationResult:
     tokens: list[int] = field(default_factory=list)
     finish_reason: str = ""      # "stop", "length" or "max_seq_len"
+    logprobs: list[float] = field(default_factory=list)      # of each token, where the request's sampling asks for them
 
 
 def pages_for(tokens: int, page_tokens: int) -> int:
@@ -31,9 +32,10 @@ def pages_for(tokens: int, page_tokens: int) -> int:
 
 
 def plan_batches(prompt_lengths: Sequence[int], max_new_tokens: int, *, page_tokens: int, total_pages: int,
-                 num_slots: int, max_seq_len: int, max_batch_size: int | None = None) -> list[list[int]]:
+                 num_slots: int, max_seq_len: int, max_batch_size: int | None = None, shared_tokens: int = 0) -> list[list[int]]:
     """Group request indices, in order, into batches whose sequences all fit the cache at their
-    final length (prompt + new tokens, capped by ``max_seq_len``, rounded up to whole pages)."""
+    final length (prompt + new tokens, capped by ``max_seq_len``, rounded up to whole pages).  The first ``shared_tokens`` (whole pages) of all prompts are
+    held once a batch."""
     limit = min(num_slots, max_batch_size or num_slots)
     if limit <= 0:
         raise ValueError("a batch needs room for at least one sequence")
@@ -48,11 +50,12 @@ def plan_batches(prompt_lengths: Sequence[int], max_new_tokens: int, *, page_tok
         need = pages_for(min(length + max_new_tokens, max_seq_len), page_tokens)
         if need > total_pages:
             raise ValueError(f"request {index} needs {need} cache pages, the cache has {total_pages}")
-        if current and (len(current) >= limit or used + need > total_pages):
+        own = need - shared_tokens // page_tokens if current else need
+        if current and (len(current) >= limit or used + own > total_pages):
             batches.append(current)
-            current, used = [], 0
+            current, used, own = [], 0, need
         current.append(index)
-        used += need
+        used += own
     if current:
         batches.append(current)
     return batches
@@ -71,6 +74,17 @@ def finish_reason(token: int, produced: int, total_length: int, *, stop_ids: fro
     return ""
 
 
+def common_prefix(prompts: Sequence[Sequence[int]], page_tokens: int) -> int:
+    """Tokens, in whole pages, with which all prompts start, at least one token of each left over."""
+    if len(prompts) < 2:
+        return 0
+    first, shortest = list(prompts[0]), min(len(p) for p in prompts)
+    n = 0
+    while n < shortest - 1 and all(p[n] == first[n] for p in prompts):
+        n += 1
+    return n // page_tokens * page_tokens
+
+
 class BatchRun:
     """One batch of requests that start together: ``start()`` runs every prompt in one step and
     samples each request's first token; every ``advance()`` then feeds the last tokens back, one per
@@ -78,8 +92,12 @@ class BatchRun:
     A request that ends gives its slot back at once."""
 
     def __init__(self, engine, sampler, prompts: Sequence[Sequence[int]], results: list[GenerationResult],
-                 indices: Sequence[int], *, max_new_tokens: int, sampling: SamplingParams, stop: frozenset[int]) -> None:
+                 indices: Sequence[int], *, max_new_tokens: int, sampling: "SamplingParams | Sequence[SamplingParams]", stop: frozenset[int],
+                 shared_tokens: int = 0) -> None:
+        """``sampling``: for all requests, or one for each prompt.  The first ``shared_tokens`` (whole pages) of the batch's prompts are the same: they run once,
+        in the first request's sequence, and the others start with its pages."""
         self.engine, self.sampler = engine, sampler
+        self.shared_tokens = shared_tokens
         self.prompts, self.results = prompts, results
         self.max_new_tokens, self.sampling, self.stop = max_new_tokens, sampling, stop
         self.active = list(indices)
@@ -94,9 +112,20 @@ class BatchRun:
         return not self.active
 
     def start(self) -> list[int]:
-        self.slot_of = {index: self.engine.new_sequence() for index in self.active}
-        self._entries = [StepEntry(self.slot_of[i], list(self.prompts[i]), [len(self.prompts[i]) - 1]) for i in self.active]
+        skip = self.shared_tokens if len(self.active) > 1 else 0
+        if skip:
+            first = self.active[0]
+            self.slot_of = {first: self.engine.new_sequence()}
+            self.engine.step([StepEntry(self.slot_of[first], list(self.prompts[first][:skip]), [])])
+            for index in self.active[1:]:
+                self.slot_of[index] = self.engine.new_sequence(prefix_of=self.slot_of[first], tokens=skip)
+        else:
+            self.slot_of = {index: self.engine.new_sequence() for index in self.active}
+        self._entries = [StepEntry(self.slot_of[i], list(self.prompts[i][skip:]), [len(self.prompts[i]) - skip - 1]) for i in self.active]
         return self._run()
+
+    def _params(self, order: list[int]):
+        return self.sampling if isinstance(self.sampling, SamplingParams) else [self.sampling[i] for i in order]
 
     def advance(self) -> list[int]:
         return self._run()
@@ -136,7 +165,7 @@ class BatchRun:
         planner = getattr(engine, "plan_decode", None)
         plan, expected = None, None
         if launch is not None and planner is not None:
-            pending = launch(logits, self.sampling, order, steps)
+            pending = launch(logits, self._params(order), order, steps)
             expected = [i for i in order if i in alive and not self._ends_whatever_it_emits(i)]
             if expected:
                 plan = planner([self.slot_of[i] for i in expected])
@@ -146,17 +175,20 @@ class BatchRun:
                 self._ahead = (engine.run_planned(plan, [row_of[i] for i in expected], chosen=chosen), list(expected))
                 plan = None
             tokens = pending.tokens()
+            logprobs = getattr(pending, "logprobs", lambda: None)()
         else:
-            tokens = self.sampler.sample(logits, self.sampling, order, steps)
+            tokens, logprobs = self.sampler.sample(logits, self._params(order), order, steps), None
         engine.check_kernels(wait=False)                 # the tokens are on the host: their step has finished
         still: list[int] = []
         emitted: list[int] = []
-        for index, token in zip(order, tokens):
+        for row, (index, token) in enumerate(zip(order, tokens)):
             if index not in alive:                       # ended by a stop token while this step was already queued
                 continue
             emitted.append(int(token))
             result = self.results[index]
             result.tokens.append(int(token))
+            if logprobs is not None and (self.sampling if isinstance(self.sampling, SamplingParams) else self.sampling[index]).logprobs:
+                result.logprobs.append(logprobs[row])
             reason = finish_reason(int(token), len(result.tokens), len(self.prompts[index]) + len(result.tokens),
                                    stop_ids=self.stop, max_new_tokens=self.max_new_tokens,
                                    max_seq_len=self.engine.max_seq_len)
@@ -190,15 +222,20 @@ def stop_set(engine, stop_token_ids: Sequence[int] | None, ignore_eos: bool) -> 
 
 
 def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 16,
-             sampling: SamplingParams | None = None, stop_token_ids: Sequence[int] | None = None,
-             ignore_eos: bool = False, max_batch_size: int | None = None, sampler=None) -> list[GenerationResult]:
-    """Generate for every prompt; returns one result per prompt, in order.
+             sampling: "SamplingParams | Sequence[SamplingParams] | None" = None, stop_token_ids: Sequence[int] | None = None,
+             ignore_eos: bool = False, max_batch_size: int | None = None, sampler=None, share_prefix: bool = False) -> list[GenerationResult]:
+    """Generate for every prompt; returns one result per prompt, in order.  ``sampling``: for all requests, or one for each.  ``share_prefix``: what all prompts
+    start with, in whole pages, runs once a batch and is held once (where the engine says ``can_share``); results are the same up to rounding.
 
     ``engine`` offers ``new_sequence()``, ``release(slot)``, ``step(entries) -> logits``,
     ``eos_token_ids``, ``max_seq_len``, ``page_tokens``, ``total_pages`` and ``num_slots``;
     ``sampler.sample(logits, params, requests, steps)`` returns one token id per row.
     """
-    sampling = sampling or SamplingParams()
+    sampling = sampling if sampling is not None else SamplingParams()
+    if not isinstance(sampling, SamplingParams):
+        sampling = list(sampling)
+        if len(sampling) != len(prompts):
+            raise ValueError(f"{len(sampling)} sampling parameters for {len(prompts)} prompts")
     if sampler is None:
         from ..sampling import Sampler
         sampler = Sampler(engine.device)
@@ -208,12 +245,13 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
         for result in results:
             result.finish_reason = "length"
         return results
+    shared = common_prefix(prompts, engine.page_tokens) if share_prefix and getattr(engine, "can_share", False) else 0
     batches = plan_batches([len(p) for p in prompts], max_new_tokens, page_tokens=engine.page_tokens,
                            total_pages=engine.total_pages, num_slots=engine.num_slots,
-                           max_seq_len=engine.max_seq_len, max_batch_size=max_batch_size)
+                           max_seq_len=engine.max_seq_len, max_batch_size=max_batch_size, shared_tokens=shared)
     for batch in batches:
         run = BatchRun(engine, sampler, prompts, results, batch, max_new_tokens=max_new_tokens, sampling=sampling,
-                       stop=stop)
+                       stop=stop, shared_tokens=shared)
         try:
             run.start()
             while not run.done:

@@ -49,6 +49,30 @@ def plan_passes(lengths: list[int], max_tokens: int, chunk_limit: int | None) ->
     return passes
 
 
+@dataclass(frozen=True)
+class SharedPrefixes:
+    """Sequences of a one-token pass that hold the same leading pages, as ``kernels.attention_decode_shared`` takes them.  ``groups``, ``most_members``,
+    ``most_shared`` and ``most_own`` are the sizes its plan is made for: limits of what the arrays hold, rounded up so that few shapes arise."""
+
+    members: torch.Tensor       # int32 [sequences]
+    share: torch.Tensor         # int32 [groups, 3]
+    groups: int
+    most_members: int
+    most_shared: int
+    most_own: int
+
+
+def shared_shape(groups: list[tuple[list[int], int]], lengths: list[int]) -> tuple[int, int, int, int]:
+    """(groups, members, shared tokens, own tokens) at most, rounded up: groups and members to powers of two, shared tokens to 1,024, own ones to a power of
+    two from 64 on."""
+    def power(n: int, least: int = 1) -> int:
+        while least < n:
+            least *= 2
+        return least
+    own = max(lengths[p] - shared for places, shared in groups for p in places)
+    return (power(len(groups)), power(max(len(places) for places, _ in groups)), -(-max(shared for _, shared in groups) // 1024) * 1024, power(own, 64))
+
+
 class StepContext:
     """Device-side description of one pass."""
 
@@ -63,6 +87,7 @@ class StepContext:
         self.token_ids = self.token_seq = self.token_pos = None
         self.seq_start = self.seq_past = self.seq_len = self.slots = self.want_rows = None
         self.order = None          # [sequences, 2]: number and length, the longest first (planned one-token passes)
+        self.shared: SharedPrefixes | None = None      # which sequences share leading pages (planned one-token passes)
         self._tables: dict[int, torch.Tensor] = {}
         self._decode_plans: dict[tuple, "_DecodePlan"] = {}
 
@@ -71,7 +96,7 @@ class StepContext:
 
     @staticmethod
     def meta_size(max_tokens: int, max_seqs: int, table_widths: list[int]) -> int:
-        return 4 * max_tokens + 7 * max_seqs + 8 + max_seqs * sum(table_widths) + 64
+        return 4 * max_tokens + 12 * max_seqs + 8 + max_seqs * sum(table_widths) + 64
 
     def fill(self, slots: list[int], tokens: list[list[int]], past: list[int], want_rows: list[int],
              tables: list[np.ndarray], max_context: int | None = None) -> None:
@@ -108,7 +133,7 @@ class StepContext:
         (self.token_ids, self.token_seq, self.token_pos, self.seq_start, self.seq_past, self.seq_len,
          self.slots, self.want_rows) = views[:8]
         self._tables = {g: views[8 + g].view(n_seqs, tables[g].shape[1]) for g in range(len(tables))}
-        self.order = None
+        self.order = self.shared = None
         self.n_tokens, self.n_seqs, self.n_want = n_tokens, n_seqs, len(want_rows)
         self.max_q_len = max(q_lens) if q_lens else 0
         self.max_context = max_context if max_context is not None else (int(seq_len.max()) if n_seqs else 0)
@@ -116,22 +141,31 @@ class StepContext:
         self.from_start = not past_arr.any()
 
     # ------------------------------------------------------------------ one token per sequence
-    def prepare_decode(self, slots: list[int], past: list[int], tables: list[np.ndarray]):
+    def prepare_decode(self, slots: list[int], past: list[int], tables: list[np.ndarray], groups=(), shape=None):
         """The part of ``fill`` for a pass of one token per sequence (every row wanted) that does not need the
         tokens: the same layout at the same addresses, written into pinned buffers that are kept (a small ring,
         each guarded by an event, so that a caller who runs ahead of the device cannot overwrite a copy that has
-        not happened yet) with the parts that never change filled in once.  Returns what ``commit_decode`` takes."""
+        not happened yet) with the parts that never change filled in once.  Returns what ``commit_decode`` takes.  ``groups``: the places that share leading
+        tokens (``CacheBook.shared_groups``), with their ``shared_shape``."""
         n = len(slots)
-        key = (n, tuple(t.shape[1] for t in tables))
+        key = (n, tuple(t.shape[1] for t in tables), shape)
         plan = self._decode_plans.get(key)
         if plan is None:
-            plan = self._decode_plans[key] = _DecodePlan(self._meta, n, key[1])
+            plan = self._decode_plans[key] = _DecodePlan(self._meta, n, key[1], shape)
         host, array, event = plan.next_buffer()
         array[2 * n:3 * n] = past
         array[plan.at_past:plan.at_past + n] = past
         np.add(array[plan.at_past:plan.at_past + n], 1, out=array[plan.at_len:plan.at_len + n])
         if plan.order is not None:
             longest_first(array[plan.at_len:plan.at_len + n], array[plan.at_order:plan.at_order + 2 * n].reshape(n, 2))
+        if shape is not None:
+            share = array[plan.at_share:plan.at_share + 3 * shape[0]].reshape(shape[0], 3)
+            share[:] = 0                                             # groups beyond the present ones have no members
+            at = 0
+            for row, (places, tokens) in enumerate(groups):
+                share[row] = (at, len(places), tokens)
+                array[plan.at_members + at:plan.at_members + at + len(places)] = places
+                at += len(places)
         array[plan.at_slots:plan.at_slots + n] = slots
         for offset, table in zip(plan.at_tables, tables):
             array[offset:offset + table.size] = table.reshape(-1)
@@ -153,7 +187,7 @@ class StepContext:
         self.meta_bytes = 4 * plan.total
         (self.token_ids, self.token_seq, self.token_pos, self.seq_start, self.seq_past, self.seq_len,
          self.slots, self.want_rows) = plan.views[:8]
-        self._tables, self.order = plan.tables, plan.order
+        self._tables, self.order, self.shared = plan.tables, plan.order, plan.shared
         self.n_tokens = self.n_seqs = self.n_want = n
         self.max_q_len = 1
         self.max_context = max_context
@@ -176,20 +210,23 @@ class _DecodePlan:
 
     RING = 4
 
-    def __init__(self, meta: torch.Tensor, n: int, widths: tuple[int, ...]) -> None:
+    def __init__(self, meta: torch.Tensor, n: int, widths: tuple[int, ...], shape: tuple[int, int, int, int] | None = None) -> None:
         self.n = n
         sizes = [n, n, n, n + 1, n, n, n, n] + [n * w for w in widths]
         offsets = np.concatenate(([0], np.cumsum(sizes))).tolist()
         self.at_order = -(-offsets[-1] // 2) * 2                      # read eight bytes at a time
         ordered = n >= ORDERED_FROM
-        self.total = self.at_order + (2 * n if ordered else 0)
+        self.at_members = self.at_order + (2 * n if ordered else 0)
+        self.at_share = self.at_members + (n if shape else 0)
+        self.total = self.at_share + (3 * shape[0] if shape else 0)
         if self.total > meta.numel():
             raise ValueError(f"step metadata of {self.total} words exceeds the buffer of {meta.numel()}")
         self.at_past, self.at_len, self.at_slots = offsets[4], offsets[5], offsets[6]
         self.at_tables = offsets[8:8 + len(widths)]
         self.views = [meta[offsets[i]:offsets[i + 1]] for i in range(len(sizes))]
         self.tables = {g: self.views[8 + g].view(n, w) for g, w in enumerate(widths)}
-        self.order = meta[self.at_order:self.total].view(n, 2) if ordered else None
+        self.order = meta[self.at_order:self.at_members].view(n, 2) if ordered else None
+        self.shared = SharedPrefixes(meta[self.at_members:self.at_share], meta[self.at_share:self.total].view(shape[0], 3), *shape) if shape else None
         self.buffers = []
         for _ in range(self.RING):
             host = torch.zeros(self.total, dtype=torch.int32, pin_memory=True)

@@ -1421,11 +1421,14 @@ def _shared_on_tc(dtype: torch.dtype, head_dim: int) -> bool:
 
 
 def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, groups: int, most_members: int,
-                most_shared: int, most_own: int, sms: int | None = None) -> SharedPlan:
+                most_shared: int, most_own: int, sms: int | None = None, most_ranges: int = 64) -> SharedPlan:
     """The cut for ``n_seqs`` sequences in ``groups`` groups of at most ``most_members``, a shared length of at most ``most_shared`` tokens and at most
-    ``most_own`` tokens of a member's own.  ``sms``: streaming multiprocessors (default: the current device's)."""
+    ``most_own`` tokens of a member's own.  ``sms``: streaming multiprocessors (default: the current device's); ``most_ranges``: of a row, 2 to 64 (scratch is
+    by ranges)."""
     if n_seqs < 0 or groups < 1 or not 0 <= most_members <= n_seqs or most_shared < 0 or most_own < 0:
         raise KernelError(f"shared_plan: {n_seqs} sequences in {groups} groups of at most {most_members}, {most_shared} and {most_own} tokens")
+    if not 2 <= most_ranges <= 64:
+        raise KernelError(f"shared_plan: {most_ranges} ranges")
     if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or head_dim < 1 or dtype not in _CODES:
         raise KernelError(f"shared_plan: {num_heads} heads over {num_kv_heads} of {head_dim} in {dtype}")
     sms = sms or sm_count()
@@ -1438,7 +1441,14 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
     else:
         shared_ranges = max(1, min(32, -(-most_shared // 128)))
         own_ranges = max(1, min(8, -(-most_own // 256)))
+    own_ranges = min(own_ranges, max(1, most_ranges - shared_ranges), most_ranges - 1)
+    shared_ranges = min(shared_ranges, most_ranges - own_ranges)
     return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges)
+
+
+def sharing_pays(n_seqs: int, most_members: int, most_shared: int) -> bool:
+    """Whether one-token steps are faster by ``attention_decode_shared`` than by ``attention_decode``."""
+    return (most_members - 1) * most_shared >= 4096
 
 
 def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,

@@ -339,6 +339,19 @@ class Attention:
         enough = max(fills) - 0.13
         return next(splits for splits, fill in enumerate(fills, start=1) if fill >= enough), 1
 
+    def _shared_plan(self, ctx, cache) -> "kernels.SharedPlan | None":
+        """The plan for sequences that share leading pages, or None where ``attention_decode`` takes them: attention with anything beyond a scale, more rows than
+        the scratch holds ranges of, or too little shared for it to pay."""
+        shared = ctx.shared
+        if (self.window or self.penalised or self.chunk or self.keep_first or self.sink or self.softcap is not None or self.dv != self.d
+                or self.v_heads != self.nkv or cache.ring_tokens or self.scale <= 0 or ctx.n_seqs * 2 > _MAX_SPLIT_PAIRS):
+            return None
+        if not kernels.sharing_pays(ctx.n_seqs, shared.most_members, shared.most_shared):
+            return None
+        return kernels.shared_plan(ctx.n_seqs, num_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.d, dtype=self.runtime.dtype, groups=shared.groups,
+                                   most_members=min(shared.most_members, ctx.n_seqs), most_shared=shared.most_shared, most_own=shared.most_own,
+                                   sms=self.runtime.sm_count, most_ranges=min(64, _MAX_SPLIT_PAIRS // ctx.n_seqs))
+
     def forward(self, x, ctx, cache):
         tokens = x.shape[0]
         ws = self.runtime.workspace
@@ -369,7 +382,13 @@ class Attention:
                 v_heads=self.v_heads if self.own_values else None, v_head_dim=self.dv if self.own_values else None,
                 unit_norm=self.norm_mode == "unit", row_inv=ws.view("attn.row_inv", tokens, 2) if self.norm_mode == "whole" else None,
                 extra_cols=self.gate_cols)
-        if ctx.is_decode:
+        plan = self._shared_plan(ctx, cache) if ctx.is_decode and getattr(ctx, "shared", None) is not None else None
+        if plan is not None:
+            shared = ctx.shared
+            kernels.attention_decode_shared(q, cache.k, cache.v, out, table, ctx.seq_len, shared.members, shared.share, self.nkv, cache.page_tokens, self.scale,
+                                            plan, ws.view("attn.part_acc", _MAX_SPLIT_PAIRS * self.nq * self.dv),
+                                            ws.view("attn.part_ml", _MAX_SPLIT_PAIRS * self.nq * 2))
+        elif ctx.is_decode:
             n_splits, warps = self._splits(ctx, cache)
             kernels.attention_decode(q, cache.k, cache.v, out, table, ctx.seq_len, self.nkv, cache.page_tokens,
                                      cache.ring_tokens, self.window, self.scale, n_splits,

@@ -11,7 +11,7 @@ Added: a model without a folder (``--preset NAME --random-weights``), prompts as
 (``--prompt-ids 1,2,3``, repeatable: a batch of unequal prompts) or random (``--random-prompts 5,9,17``),
 ``--temperature``, ``--seed`` (the seed of everything the run draws: sampling, random weights, random
 prompts; ``--sampling-seed`` and ``--weights-seed`` set one of them apart), ``--stop-ids``,
-``--ignore-eos``, ``--max-tokens`` (cache size), ``--max-seq-len``, ``--max-batch-size``.
+``--ignore-eos``, ``--min-p``, ``--samples`` (continuations of every prompt, ranked), ``--max-tokens`` (cache size), ``--max-seq-len``, ``--max-batch-size``.
 """
 from __future__ import annotations
 
@@ -35,6 +35,8 @@ def _parse_args(argv=None) -> argparse.Namespace:
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--top-k", type=int, default=0, help="with --temperature: draw from the k most likely tokens only")
     parser.add_argument("--top-p", type=float, default=1.0, help="with --temperature: draw from the most likely tokens that sum to this share")
+    parser.add_argument("--min-p", type=float, default=0.0, help="with --temperature: draw from tokens at least this many times as likely as the likeliest")
+    parser.add_argument("--samples", type=int, default=1, help="continuations of every prompt, the likeliest first (they share the prompt's cache pages)")
     parser.add_argument("--seed", type=int, default=0, help="seed of everything the run draws")
     parser.add_argument("--sampling-seed", type=int, default=None, help="seed of temperature sampling (default: --seed)")
     parser.add_argument("--weights-seed", type=int, default=None, help="seed of --random-weights (default: --seed)")
@@ -104,16 +106,24 @@ def main(argv=None) -> None:
 
     outputs = model.forward(prompts[0], logits_to_keep=1)
     next_token = outputs.logits[:, -1].argmax(dim=-1)
-    results = model.generate(prompts, max_new_tokens=args.max_new_tokens, temperature=args.temperature,
-                             seed=sampling_seed, stop_token_ids=_ids(args.stop_ids, "--stop-ids"),
-                             ignore_eos=args.ignore_eos, max_batch_size=args.max_batch_size, top_k=args.top_k, top_p=args.top_p)
+    if args.samples > 1:
+        several = [model.continuations(prompt, args.samples, max_new_tokens=args.max_new_tokens, temperature=args.temperature, seed=sampling_seed,
+                                       stop_token_ids=_ids(args.stop_ids, "--stop-ids"), ignore_eos=args.ignore_eos, top_k=args.top_k,
+                                       top_p=args.top_p, min_p=args.min_p) for prompt in prompts]
+        prompts = [prompt for prompt in prompts for _ in range(args.samples)]
+        results = [result for of_prompt in several for result in of_prompt]
+    else:
+        results = model.generate(prompts, max_new_tokens=args.max_new_tokens, temperature=args.temperature,
+                                 seed=sampling_seed, stop_token_ids=_ids(args.stop_ids, "--stop-ids"),
+                                 ignore_eos=args.ignore_eos, max_batch_size=args.max_batch_size, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
     print(f"backend={args.backend}")
     print(f"next_token={next_token.tolist()}")
     for prompt, result in zip(prompts, results):
         if tokenizer is not None:
             print(tokenizer.decode(prompt + result.tokens))
         else:
-            print(f"generated={result.tokens} finish={result.finish_reason}")
+            mean = f" mean_logprob={sum(result.logprobs) / max(1, len(result.logprobs)):.4f}" if result.logprobs else ""
+            print(f"generated={result.tokens} finish={result.finish_reason}{mean}")
 
     if args.compare_ref:
         kept = outputs.logits.float().cpu()

@@ -1,0 +1,197 @@
+"""Pages held by several sequences: the book's accounting, which sequences share, and the generation loop's use of it (no GPU)."""
+import random
+
+import numpy as np
+import pytest
+
+from qwen_triton_b200.cache import CacheBook, CacheError, CacheFull, GroupGeometry, SequenceCache
+from qwen_triton_b200.engine.generate import common_prefix, generate, plan_batches
+from qwen_triton_b200.engine.step import shared_shape
+from qwen_triton_b200.parts.base import KVRequest, StateRequest
+from qwen_triton_b200.sampling import SamplingParams, uniform_for
+from qwen_triton_b200.sampling.sampler import uniforms_for
+from test_generate_loop import ArgmaxSampler, ScriptedEngine
+
+
+def make_book(slots=8, pages=20, groups=1):
+    return CacheBook(slots, 64, [GroupGeometry(pages) for _ in range(groups)], 4096)
+
+
+def test_a_sequence_starts_with_another_ones_pages():
+    book = make_book(groups=2)
+    a = book.alloc()
+    book.extend(a, 200)
+    b = book.alloc(a, 128)
+    assert book.length(b) == 128
+    for group in range(2):
+        assert book.pages(b, group) == book.pages(a, group)[:2] and book.free_pages(group) == 16
+    book.extend(b, 130)                                    # its own page behind the shared ones
+    assert book.pages(b, 0)[2] != book.pages(a, 0)[2]
+    book.check()
+    book.free(a)                                           # the shared pages stay with b
+    assert book.free_pages(0) == 17
+    book.check()
+    book.free(b)
+    assert book.free_pages(0) == book.free_pages(1) == 20
+    book.check()
+
+
+def test_what_cannot_be_shared():
+    book = make_book(slots=2)
+    a = book.alloc()
+    book.extend(a, 100)
+    for tokens in (0, -64, 63, 100, 128):
+        with pytest.raises(CacheError, match="whole pages"):
+            book.alloc(a, tokens)
+    with pytest.raises(CacheError, match="not in use"):
+        book.alloc(1, 64)
+    book.alloc(a, 64)
+    with pytest.raises(CacheFull):
+        book.alloc(a, 64)
+    windowed = CacheBook(4, 64, [GroupGeometry(8), GroupGeometry(8, 2)], 4096)
+    slot = windowed.alloc()
+    windowed.extend(slot, 64)
+    with pytest.raises(CacheError, match="windowed"):
+        windowed.alloc(slot, 64)
+    windowed.check()
+    common = dict(max_tokens=512, max_seq_len=512, dtype=None, device=None, allocate=False)
+    import torch
+    common["dtype"] = torch.float32
+    assert SequenceCache([KVRequest(2, 16)], [None], **common).can_share
+    assert not SequenceCache([KVRequest(2, 16, 64)], [None], **common).can_share
+
+
+def test_random_lives_of_sharing_sequences():
+    rng = random.Random(5)
+    book = make_book(slots=12, pages=60, groups=2)
+    for _ in range(2000):
+        live = book.live_slots()
+        what = rng.random()
+        try:
+            if what < 0.25 or not live:
+                book.alloc()
+            elif what < 0.5:
+                source = rng.choice(live)
+                whole = book.length(source) // 64
+                if whole:
+                    book.alloc(source, 64 * rng.randint(1, whole))
+            elif what < 0.8:
+                slot = rng.choice(live)
+                book.extend(slot, book.length(slot) + rng.randint(0, 150))
+            else:
+                book.free(rng.choice(live))
+        except CacheFull:
+            book.free(rng.choice(book.live_slots()))
+        book.check()
+        live = book.live_slots()
+        rng.shuffle(live)
+        groups = book.shared_groups(live)
+        if groups:
+            assert sorted(place for places, _ in groups for place in places) == list(range(len(live)))
+        for places, tokens in groups:
+            pages = [tuple(book.pages(live[p], 0)[:tokens // 64]) for p in places]
+            assert len(set(pages)) == 1 if tokens else True
+            assert tokens == 0 or (len(places) > 1 and all(book.length(live[p]) >= tokens for p in places))
+    for slot in book.live_slots():
+        book.free(slot)
+    assert book.shared_groups([]) == [] and book.free_pages(0) == 60
+    book.check()
+
+
+def test_groups_of_sequences_that_share():
+    book = make_book()
+    a, other = book.alloc(), book.alloc()
+    book.extend(a, 200)
+    book.extend(other, 70)
+    assert book.shared_groups([a, other]) == []
+    b, c = book.alloc(a, 192), book.alloc(a, 64)
+    assert book.shared_groups([b, other, a]) == [([0, 2], 192), ([1], 0)]
+    assert book.shared_groups([c, b]) == [([0, 1], 64)]
+    assert book.shared_groups([b, other]) == []             # alone, each of them
+    book.free(a)
+    assert book.shared_groups([c, b]) == [([0, 1], 64)]
+
+
+def test_shapes_are_rounded_up():
+    assert shared_shape([([0, 2, 3], 192), ([1], 0)], [200, 90, 260, 193]) == (2, 4, 1024, 128)
+    assert shared_shape([([0, 1], 1024)], [1025, 1030]) == (1, 2, 1024, 64)
+    assert shared_shape([([0, 1], 1088)], [1100, 1200]) == (1, 2, 2048, 128)
+
+
+def test_the_prefix_of_all_prompts():
+    long = list(range(300))
+    assert common_prefix([long, long[:200] + [7], long], 64) == 192
+    assert common_prefix([long[:128], long], 64) == 64       # a token of each is left over
+    assert common_prefix([long[:129], long], 64) == 128
+    assert common_prefix([long], 64) == 0 and common_prefix([[1] + long, long], 64) == 0
+
+
+def test_batches_hold_what_is_shared_once():
+    lengths = [300] * 6
+    assert plan_batches(lengths, 20, page_tokens=64, total_pages=12, num_slots=8, max_seq_len=4096) == [[0, 1], [2, 3], [4, 5]]
+    assert plan_batches(lengths, 20, page_tokens=64, total_pages=12, num_slots=8, max_seq_len=4096, shared_tokens=256) == [[0, 1, 2, 3, 4, 5]]
+    assert plan_batches(lengths, 20, page_tokens=64, total_pages=7, num_slots=8, max_seq_len=4096, shared_tokens=256) == [[0, 1, 2], [3, 4, 5]]
+
+
+class SharingEngine(ScriptedEngine):
+    """Counts what each sequence holds; a shared start is taken from a sequence that holds it."""
+
+    can_share = True
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.shared: list[tuple[int, int, int]] = []
+
+    def new_sequence(self, prefix_of=None, tokens=None):
+        slot = super().new_sequence()
+        if prefix_of is not None:
+            assert tokens % self.page_tokens == 0 and 0 < tokens <= self.lengths[prefix_of]
+            self.lengths[slot] = tokens
+            self.shared.append((slot, prefix_of, tokens))
+        return slot
+
+    def step(self, entries):
+        if len(entries) == 1 and not entries[0].want:
+            self.steps.append([(entries[0].slot, len(entries[0].tokens))])
+            self.lengths[entries[0].slot] += len(entries[0].tokens)
+            return None
+        return super().step(entries)
+
+
+def test_generation_runs_the_shared_prefix_once():
+    prompts = [[1, 2, 3, 4, 5, 6, 7, 8, 9, 10 + i] for i in range(3)]
+    plain = generate(ScriptedEngine(total_pages=30, vocab=90), prompts, max_new_tokens=3, sampler=ArgmaxSampler())
+    engine = SharingEngine(total_pages=30, vocab=90)
+    shared = generate(engine, prompts, max_new_tokens=3, sampler=ArgmaxSampler(), share_prefix=True)
+    assert [r.tokens for r in shared] == [r.tokens for r in plain]
+    assert engine.steps[0] == [(0, 8)] and engine.steps[1] == [(0, 2), (1, 2), (2, 2)]
+    assert engine.shared == [(1, 0, 8), (2, 0, 8)] and not engine.lengths
+    engine = SharingEngine(total_pages=30, vocab=90)          # not asked for, nothing shared
+    generate(engine, prompts, max_new_tokens=3, sampler=ArgmaxSampler())
+    assert engine.steps[0] == [(0, 10), (1, 10), (2, 10)] and not engine.shared
+
+
+def test_parameters_of_each_request():
+    class Sampler:
+        def __init__(self):
+            self.seen = []
+
+        def sample(self, logits, params, requests, steps):
+            self.seen.append((params, list(requests)))
+            return logits.argmax(dim=-1).tolist()
+
+    params = [SamplingParams(temperature=0.5, seed=i, min_p=0.1) for i in range(3)]
+    sampler = Sampler()
+    generate(ScriptedEngine(), [[46], [10], [20]], max_new_tokens=4, sampling=params, sampler=sampler)
+    assert sampler.seen[0] == (params, [0, 1, 2]) and sampler.seen[-1] == (params[1:], [1, 2])      # the first ends early
+    with pytest.raises(ValueError, match="sampling parameters"):
+        generate(ScriptedEngine(), [[1], [2]], sampling=params, sampler=sampler)
+    with pytest.raises(ValueError, match="min_p"):
+        SamplingParams(min_p=1.5)
+
+
+def test_uniform_numbers_of_many_rows():
+    rng = random.Random(1)
+    rows = [(rng.getrandbits(64), rng.randrange(1 << 20), rng.randrange(1 << 16)) for _ in range(200)] + [(0, 0, 0), ((1 << 64) - 1, 5, 7)]
+    got = uniforms_for(np.array([r[0] for r in rows], dtype=np.uint64), np.array([r[1] for r in rows]), np.array([r[2] for r in rows]))
+    assert got.dtype == np.float32 and got.tolist() == [uniform_for(*r) for r in rows]
