@@ -186,6 +186,25 @@ __device__ __forceinline__ void store_shared16(uint32_t addr, uint4 v) {
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// The products as a whole warp meets them: all lanes go through the same instructions, so that descriptors stay in the registers that a warp has in common, and one
+// lane's are carried out.  Issued by a lane that runs alone, a product takes about 100 cycles to leave, 12 of them a tile: MEASURED_ISSUE.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    return elected;
+}
+__device__ __forceinline__ void mma_one(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void mma_one_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void commit_one(uint32_t bar, uint32_t one) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one) : "memory");
+}
+
 // MN-major operand stored as [64-element MN blocks][K rows][64 elements], 128-byte swizzle (V: [key][dim]).
 __device__ __forceinline__ uint64_t operand_desc_mn(uint32_t saddr, uint32_t mn_block_bytes) {
     uint64_t d = 0;
@@ -325,40 +344,39 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint64_t q_desc0 = operand_desc(q_s), k_desc0 = operand_desc(k_s), v_desc0 = operand_desc_mn(v_s, KEY_HALF_BYTES);
-            bool ok = mbar_wait(q_full, 0, status, 2);
-            auto issue_qk = [&](int i) {
-                const int s = i & 1;
-                if (!mbar_wait(k_full + 8 * s, (uint32_t)(i >> 1) & 1u, status, 2)) return false;
-                // this buffer held P of tile i - 2, whose P V was issued before this; the tensor pipe runs its instructions in order
-                tc_fence_after();
-                const uint64_t k_desc = k_desc0 + (uint64_t)(s * (KV_BYTES >> 4));
+        const uint64_t q_desc0 = operand_desc(q_s), k_desc0 = operand_desc(k_s), v_desc0 = operand_desc_mn(v_s, KEY_HALF_BYTES);
+        const uint32_t one = elect_one();
+        auto wait = [&](uint32_t bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase, status, 2)) != 0; };
+        auto issue_qk = [&](int i) {
+            const int s = i & 1;
+            if (!wait(k_full + 8 * s, (uint32_t)(i >> 1) & 1u)) return false;
+            // this buffer held P of tile i - 2, whose P V was issued before this; the tensor pipe runs its instructions in order
+            tc_fence_after();
+            const uint64_t k_desc = k_desc0 + (uint64_t)(s * (KV_BYTES >> 4));
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    const uint32_t in_half = (uint32_t)(ks & 3) * 32u;
-                    umma_bf16(tmem_base + s * PAGE, q_desc0 + (uint64_t)(((uint32_t)(ks >> 2) * HALF_BYTES + in_half) >> 4),
-                              k_desc + (uint64_t)(((uint32_t)(ks >> 2) * KEY_HALF_BYTES + in_half) >> 4), IDESC_QK, ks > 0 ? 1u : 0u);
-                }
-                umma_commit(s_full + 8 * s);
-                umma_commit(k_empty + 8 * s);
-                return true;
-            };
-            if (ok) ok = issue_qk(0);
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                if (j + 1 < n_tiles) { ok = issue_qk(j + 1); if (!ok) break; }
-                const int s = j & 1;
-                const uint32_t phase = (uint32_t)(j >> 1) & 1u;
-                if (!mbar_wait(p_full + 8 * s, phase, status, 2) || !mbar_wait(v_full + 8 * s, phase, status, 2)) break;
-                tc_fence_after();
-                const uint64_t v_desc = v_desc0 + (uint64_t)(s * (KV_BYTES >> 4));
-#pragma unroll
-                for (int ks = 0; ks < PAGE / 16; ++ks)
-                    umma_bf16_a_tmem(tmem_base + O_COL, tmem_base + s * PAGE + (uint32_t)(ks * 8), v_desc + (uint64_t)(((uint32_t)ks * (16 * 128)) >> 4),
-                                     IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-                umma_commit(pv_full + 8 * s);
-                umma_commit(v_empty + 8 * s);
+            for (int ks = 0; ks < HD / 16; ++ks) {
+                const uint32_t in_half = (uint32_t)(ks & 3) * 32u;
+                mma_one(tmem_base + s * PAGE, q_desc0 + (uint64_t)(((uint32_t)(ks >> 2) * HALF_BYTES + in_half) >> 4),
+                        k_desc + (uint64_t)(((uint32_t)(ks >> 2) * KEY_HALF_BYTES + in_half) >> 4), IDESC_QK, ks > 0 ? 1u : 0u, one);
             }
+            commit_one(s_full + 8 * s, one);
+            commit_one(k_empty + 8 * s, one);
+            return true;
+        };
+        bool ok = wait(q_full, 0) && issue_qk(0);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+            if (j + 1 < n_tiles) { ok = issue_qk(j + 1); if (!ok) break; }
+            const int s = j & 1;
+            const uint32_t phase = (uint32_t)(j >> 1) & 1u;
+            if (!wait(p_full + 8 * s, phase) || !wait(v_full + 8 * s, phase)) break;
+            tc_fence_after();
+            const uint64_t v_desc = v_desc0 + (uint64_t)(s * (KV_BYTES >> 4));
+#pragma unroll
+            for (int ks = 0; ks < PAGE / 16; ++ks)
+                mma_one_a_tmem(tmem_base + O_COL, tmem_base + s * PAGE + (uint32_t)(ks * 8), v_desc + (uint64_t)(((uint32_t)ks * (16 * 128)) >> 4), IDESC_PV,
+                               (j > 0 || ks > 0) ? 1u : 0u, one);
+            commit_one(pv_full + 8 * s, one);
+            commit_one(v_empty + 8 * s, one);
         }
     } else {
         const int quarter = warp & 3;
