@@ -8,6 +8,7 @@ split-K partial sums that the consumer adds up in float.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -1398,33 +1399,54 @@ class SharedPlan:
     most_members: int
     shared_ranges: int            # ranges that a group's shared keys are cut into
     own_ranges: int               # ranges that a member's own keys are cut into
+    page_tokens: int = 64
     direct_warps: int = 4         # with shared_ranges 0: one launch walks all keys of every member, by own_ranges blocks of this many warps
 
     @property
     def ranges(self) -> int:
         return self.shared_ranges + self.own_ranges
 
-    @property
+    @functools.cached_property
     def acc_elements(self) -> int:
         """Elements of ``part_acc`` (float)."""
         return self.n_seqs * self.num_heads * self.ranges * self.head_dim
 
-    @property
+    @functools.cached_property
     def ml_elements(self) -> int:
         """Elements of ``part_ml`` (float)."""
         return self.n_seqs * self.num_heads * self.ranges * 2
 
+    @functools.cached_property
+    def q_shape(self) -> tuple[int, int, int]:
+        return self.n_seqs, self.num_heads, self.head_dim
 
-def _shared_on_tc(dtype: torch.dtype, head_dim: int) -> bool:
-    """Whether the tensor-core kernels take a call (with pages of 64 tokens)."""
-    return dtype == torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128
+    @functools.cached_property
+    def page_shape(self) -> tuple[int, int, int]:
+        return self.num_kv_heads, self.page_tokens, self.head_dim
+
+    @functools.cached_property
+    def share_shape(self) -> tuple[int, int]:
+        return self.groups, 3
+
+    @functools.cached_property
+    def on_tc(self) -> int:
+        """1 where the tensor-core kernels take the call."""
+        return int(_shared_on_tc(self.dtype, self.head_dim, self.page_tokens))
+
+
+DIRECT_BYTES = 48 << 20       # keys and values that one launch reads over all members (out of the L2 cache where they are shared)
+
+
+def _shared_on_tc(dtype: torch.dtype, head_dim: int, page_tokens: int) -> bool:
+    """Whether the tensor-core kernels take a call."""
+    return dtype == torch.bfloat16 and head_dim % 8 == 0 and head_dim <= 128 and page_tokens == 64
 
 
 def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, groups: int, most_members: int,
-                most_shared: int, most_own: int, sms: int | None = None, most_ranges: int = 64) -> SharedPlan:
+                most_shared: int, most_own: int, sms: int | None = None, most_ranges: int = 64, page_tokens: int = 64) -> SharedPlan:
     """The cut for ``n_seqs`` sequences in ``groups`` groups of at most ``most_members``, a shared length of at most ``most_shared`` tokens and at most
     ``most_own`` tokens of a member's own.  ``sms``: streaming multiprocessors (default: the current device's); ``most_ranges``: of a row, 2 to 64 (scratch is
-    by ranges)."""
+    by ranges); ``page_tokens``: of the cache."""
     if n_seqs < 0 or groups < 1 or not 0 <= most_members <= n_seqs or most_shared < 0 or most_own < 0:
         raise KernelError(f"shared_plan: {n_seqs} sequences in {groups} groups of at most {most_members}, {most_shared} and {most_own} tokens")
     if not 2 <= most_ranges <= 64:
@@ -1433,22 +1455,53 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
         raise KernelError(f"shared_plan: {num_heads} heads over {num_kv_heads} of {head_dim} in {dtype}")
     sms = sms or sm_count()
     group = num_heads // num_kv_heads
-    if _shared_on_tc(dtype, head_dim):
-        blocks = num_kv_heads * max(1, -(-most_members * group // 128))
-        shared_ranges = max(1, min(32, 2 * sms // blocks, -(-most_shared // 128)))
+    if _shared_on_tc(dtype, head_dim, page_tokens):
         pairs = max(1, n_seqs * num_kv_heads * -(-group // 16))
-        own_ranges = max(1, min(16, -(-most_own // 128), max(-(-most_own // 1024), sms // pairs)))
+        most_len = most_shared + most_own
+        if n_seqs * num_kv_heads * most_len * 4 * head_dim <= DIRECT_BYTES:
+            # All of a (member, kv head)'s keys by a cluster of blocks: as many as leave one block an SM (three with heads of 64, whose rings are small), and
+            # as many warps as have 32 keys each.  Two launches instead cost about 5 us more; from here on reading the shared keys once saves more than that.
+            blocks = 1
+            while blocks < 4 and pairs * blocks * 2 <= sms * (3 if head_dim <= 64 else 1) and most_len > 128 * blocks:
+                blocks *= 2
+            warps = max(1, min(2 if pairs > sms else 4, -(-most_len // (32 * blocks))))
+            return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, 0, blocks, page_tokens, warps)
+        # A block takes about 0.70 us a tile of 64 keys alone on its SM and 1.22 us beside another; a range more costs about 0.4 us, in partial results and
+        # in what it takes from the blocks of own keys.
+        rows, tiles = num_kv_heads * groups * max(1, -(-most_members * group // 128)), -(-most_shared // 64)
+        shared_ranges = min(range(1, 33), key=lambda r: (-(-tiles // r) * (0.70 if rows * r <= sms else 1.22 * -(-rows * r // (2 * sms))) + 0.4 * r, r))
+        own_ranges = max(1, min(16, -(-most_own // 64 // max(8, -(-tiles // shared_ranges)))))
     else:
         shared_ranges = max(1, min(32, -(-most_shared // 128)))
         own_ranges = max(1, min(8, -(-most_own // 256)))
     own_ranges = min(own_ranges, max(1, most_ranges - shared_ranges), most_ranges - 1)
     shared_ranges = min(shared_ranges, most_ranges - own_ranges)
-    return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges)
+    return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges, page_tokens)
 
 
 def sharing_pays(n_seqs: int, most_members: int, most_shared: int) -> bool:
     """Whether one-token steps are faster by ``attention_decode_shared`` than by ``attention_decode``."""
     return (most_members - 1) * most_shared >= 4096
+
+
+def _check_shared(q, k_cache, v_cache, out, block_table, seq_len, members, share, num_kv_heads, page_tokens, plan, part_acc, part_ml) -> None:
+    """Raises what is wrong with a call of ``attention_decode_shared``."""
+    n_seqs, num_heads, head_dim = _check_attention(q, k_cache, v_cache, out, block_table, num_kv_heads, page_tokens)
+    if v_cache.shape != k_cache.shape:
+        raise KernelError(f"attention_decode_shared: values {tuple(v_cache.shape)} are not as the keys {tuple(k_cache.shape)}")
+    if head_dim > 256:
+        raise KernelError(f"attention_decode_shared: heads of {head_dim} elements (at most 256)")
+    if block_table.dim() != 2 or block_table.shape[0] != n_seqs or (n_seqs and not block_table.shape[1]):
+        raise KernelError(f"attention_decode_shared: block_table {tuple(block_table.shape)} for {n_seqs} sequences")
+    _need(seq_len, "seq_len", torch.int32, (n_seqs,))
+    _need(members, "members", torch.int32, (n_seqs,))
+    _need(share, "share", torch.int32, (plan.groups, 3))
+    if (plan.n_seqs, plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.dtype, plan.page_tokens) != (n_seqs, num_heads, num_kv_heads, head_dim, q.dtype, page_tokens):
+        raise KernelError(f"attention_decode_shared: the plan is for {plan}, not for q {tuple(q.shape)} {q.dtype} over {num_kv_heads} heads and pages of {page_tokens}")
+    _need(part_acc, "part_acc", torch.float32)
+    _need(part_ml, "part_ml", torch.float32)
+    if part_acc.numel() < plan.acc_elements or part_ml.numel() < plan.ml_elements:
+        raise KernelError("attention_decode_shared: scratch is too small for this plan")
 
 
 def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
@@ -1463,26 +1516,19 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     The keys are cut into ``plan.ranges`` ranges whose partial results pass through ``part_acc`` and ``part_ml`` (float, at least
     ``plan.acc_elements`` and ``plan.ml_elements``).
     """
-    n_seqs, num_heads, head_dim = _check_attention(q, k_cache, v_cache, out, block_table, num_kv_heads, page_tokens)
-    if v_cache.shape != k_cache.shape:
-        raise KernelError(f"attention_decode_shared: values {tuple(v_cache.shape)} are not as the keys {tuple(k_cache.shape)}")
-    if head_dim > 256:
-        raise KernelError(f"attention_decode_shared: heads of {head_dim} elements (at most 256)")
-    if block_table.dim() != 2 or block_table.shape[0] != n_seqs or (n_seqs and not block_table.shape[1]):
-        raise KernelError(f"attention_decode_shared: block_table {tuple(block_table.shape)} for {n_seqs} sequences")
-    _need(seq_len, "seq_len", torch.int32, (n_seqs,))
-    _need(members, "members", torch.int32, (n_seqs,))
-    _need(share, "share", torch.int32, (plan.groups, 3))
-    if (plan.n_seqs, plan.num_heads, plan.num_kv_heads, plan.head_dim, plan.dtype) != (n_seqs, num_heads, num_kv_heads, head_dim, q.dtype):
-        raise KernelError(f"attention_decode_shared: the plan is for {plan}, not for q {tuple(q.shape)} {q.dtype} over {num_kv_heads} heads")
-    _need(part_acc, "part_acc", torch.float32)
-    _need(part_ml, "part_ml", torch.float32)
-    if part_acc.numel() < plan.acc_elements or part_ml.numel() < plan.ml_elements:
-        raise KernelError("attention_decode_shared: scratch is too small for this plan")
-    on_tc = _shared_on_tc(q.dtype, head_dim) and page_tokens == 64
+    shape = plan.q_shape
+    # one expression for a call that is in order: the host's part of a short step is its time
+    if not (q.shape == shape == out.shape and k_cache.shape == v_cache.shape and k_cache.shape[1:] == plan.page_shape and q.dtype is plan.dtype is k_cache.dtype
+            and plan.dtype is v_cache.dtype is out.dtype and block_table.dim() == 2 and block_table.shape[0] == shape[0] and block_table.shape[1] > 0
+            and seq_len.shape == members.shape == shape[:1] and share.shape == plan.share_shape and num_kv_heads == plan.num_kv_heads and page_tokens == plan.page_tokens
+            and block_table.dtype is seq_len.dtype is members.dtype is share.dtype is torch.int32 and part_acc.dtype is part_ml.dtype is torch.float32
+            and part_acc.numel() >= plan.acc_elements and part_ml.numel() >= plan.ml_elements and shape[2] <= 256
+            and all(t.is_cuda and t.is_contiguous() for t in (q, k_cache, v_cache, out, block_table, seq_len, members, share, part_acc, part_ml))):
+        _check_shared(q, k_cache, v_cache, out, block_table, seq_len, members, share, num_kv_heads, page_tokens, plan, part_acc, part_ml)
+    n_seqs, num_heads, head_dim = shape
     _call("attention_shared", "qt_attention_decode_shared", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q, "q"), _ptr(block_table),
           block_table.shape[1], _ptr(seq_len), _ptr(members), _ptr(share), n_seqs, plan.groups, plan.most_members, num_heads, num_kv_heads, head_dim,
-          page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, plan.direct_warps, int(on_tc), _ptr(part_acc), _ptr(part_ml),
+          page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, plan.direct_warps, plan.on_tc, _ptr(part_acc), _ptr(part_ml),
           _ptr(_status_word(q.device)), _stream(), launches=(2 if plan.shared_ranges else 1) if n_seqs else 0)
 
 
@@ -1711,14 +1757,8 @@ def sample_keyed(logits: torch.Tensor, temperature: float, seed: int, keys: torc
           _ptr(out), rows, logits.shape[1], int(top_k), float(top_p), _stream())
 
 
-def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
-                    uniform: torch.Tensor, out: torch.Tensor, logprob: torch.Tensor | None = None) -> None:
-    """One token per row of float logits [rows, vocab] (rows may lie further apart than they are long), with parameters of the row's own, all on the
-    device: ``temperature`` (0: the lowest id of the largest logit), ``top_k`` (int32; 0: off), ``top_p`` (1: off), ``min_p`` (0: off) and a number
-    ``uniform`` in [0, 1) by which the token is drawn in vocabulary order.  Tokens above which fewer than ``top_k`` logits lie are kept; of these,
-    tokens above which less than ``top_p`` of their mass lies; of these, tokens at least ``min_p`` times as likely as the likeliest.
-    ``out`` (int32) takes the tokens, ``logprob`` (float, optional) the logarithm of the probability with which each was drawn.  NaN counts as -inf;
-    a row that has nothing above -inf gives token 0 with log-probability -inf."""
+def _check_filtered(logits, temperature, top_k, top_p, min_p, uniform, out, logprob) -> None:
+    """Raises what is wrong with a call of ``sample_filtered``."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2:
         raise KernelError("sample_filtered: logits must be a CUDA tensor [rows, vocab] of float32 (there is no host path)")
     rows, vocab = logits.shape
@@ -1730,6 +1770,23 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     _need(out, "out", torch.int32, (rows,))
     if logprob is not None:
         _need(logprob, "logprob", torch.float32, (rows,))
+
+
+def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
+                    uniform: torch.Tensor, out: torch.Tensor, logprob: torch.Tensor | None = None) -> None:
+    """One token per row of float logits [rows, vocab] (rows may lie further apart than they are long), with parameters of the row's own, all on the
+    device: ``temperature`` (0: the lowest id of the largest logit), ``top_k`` (int32; 0: off), ``top_p`` (1: off), ``min_p`` (0: off) and a number
+    ``uniform`` in [0, 1) by which the token is drawn in vocabulary order.  Tokens above which fewer than ``top_k`` logits lie are kept; of these,
+    tokens above which less than ``top_p`` of their mass lies; of these, tokens at least ``min_p`` times as likely as the likeliest.
+    ``out`` (int32) takes the tokens, ``logprob`` (float, optional) the logarithm of the probability with which each was drawn.  NaN counts as -inf;
+    a row that has nothing above -inf gives token 0 with log-probability -inf."""
+    if logits.dim() != 2 or not (logits.stride(1) == 1 and logits.shape[1] > 0 and logits.stride(0) >= logits.shape[1] and logits.is_cuda and
+            logits.dtype is temperature.dtype is top_p.dtype is min_p.dtype is uniform.dtype is torch.float32 and top_k.dtype is out.dtype is torch.int32
+            and logits.shape[:1] == temperature.shape == top_k.shape == top_p.shape == min_p.shape == uniform.shape == out.shape
+            and (logprob is None or (logprob.shape == out.shape and logprob.dtype is torch.float32 and logprob.is_cuda and logprob.is_contiguous()))
+            and all(t.is_cuda and t.is_contiguous() for t in (temperature, top_k, top_p, min_p, uniform, out))):
+        _check_filtered(logits, temperature, top_k, top_p, min_p, uniform, out, logprob)
+    rows, vocab = logits.shape
     _call("sampling_filtered", "qt_sample_filtered", _ptr(logits), logits.stride(0) if rows > 1 else vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
           _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(logprob), rows, vocab, _stream(), launches=1 if rows else 0)
 

@@ -350,7 +350,7 @@ class Attention:
             return None
         return kernels.shared_plan(ctx.n_seqs, num_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.d, dtype=self.runtime.dtype, groups=shared.groups,
                                    most_members=min(shared.most_members, ctx.n_seqs), most_shared=shared.most_shared, most_own=shared.most_own,
-                                   sms=self.runtime.sm_count, most_ranges=min(64, _MAX_SPLIT_PAIRS // ctx.n_seqs))
+                                   sms=self.runtime.sm_count, most_ranges=min(64, _MAX_SPLIT_PAIRS // ctx.n_seqs), page_tokens=cache.page_tokens)
 
     def forward(self, x, ctx, cache):
         tokens = x.shape[0]

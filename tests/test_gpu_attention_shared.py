@@ -65,7 +65,7 @@ class Case:
         self.scale = dim ** -0.5
         own = [o or 0 for _, group in groups for o in group]
         self.plan = kernels.shared_plan(batch, num_heads=heads, num_kv_heads=kv_heads, head_dim=dim, dtype=dtype, groups=len(groups),
-                                        most_members=max(len(o) for _, o in groups), most_shared=max(s for s, _ in groups), most_own=max(own))
+                                        most_members=max(len(o) for _, o in groups), most_shared=max(s for s, _ in groups), most_own=max(own), page_tokens=page)
 
     def run(self, plan=None, **changes):
         plan = plan or self.plan
@@ -255,6 +255,7 @@ def test_refusals():
             (dict(share=case.share[:, :2].contiguous()), "shape"),
             (dict(num_kv_heads=4), "cache shape"),
             (dict(page_tokens=32), "cache shape"),
+            (dict(plan=dataclasses.replace(case.plan, page_tokens=16)), "plan"),
             (dict(part_acc=torch.empty(3, device="cuda")), "scratch"),
             (dict(part_ml=torch.empty(3, device="cuda")), "scratch"),
             (dict(plan=dataclasses.replace(case.plan, num_heads=8)), "plan")):
