@@ -33,7 +33,7 @@ struct SharedParams {
     float* part_acc;                            // [n_seqs, nq, ranges, d]
     float* part_ml;                             // [n_seqs, nq, ranges, 2]
     int* status;                                // stays 0 unless a wait in a kernel ran out
-    int row_tiles, own_tiles, shared_blocks, own_blocks, turn;      // filled in at the launch
+    int row_tiles, own_tiles, shared_items, own_items, turn;        // filled in at the launch
 };
 
 // Group g of the call, held within what the member list and the page lists have.
@@ -57,52 +57,204 @@ __device__ __forceinline__ Group group_of(const SharedParams& p, int at) {
 __device__ __forceinline__ int member_at(const SharedParams& p, int at) { return min(max(p.members[at], 0), p.n_seqs - 1); }
 __device__ __forceinline__ int page_at(const SharedParams& p, const int* table, int index) { return min(max(table[index], 0), p.n_pages - 1); }
 
-// A warp takes a row (member, query head) and one of its key ranges.
-template <typename T>
-__global__ void __launch_bounds__(128) shared_simple_kernel(const SharedParams p) {
+// Ranges of a group's shared tiles: `per` tiles each but the last; ranges from `used` on hold nothing and leave no partial result.
+struct Ranges {
+    int per, used;
+    __device__ __forceinline__ Ranges(int tokens, int tile, int ranges) {
+        const int tiles = (tokens + tile - 1) / tile;
+        per = (tiles + ranges - 1) / ranges;
+        used = per > 0 ? (tiles + per - 1) / per : 0;
+    }
+};
+
+// The ranges of a member's own keys, in tiles from the one on in which the shared keys end.
+struct OwnRanges {
+    int tile, tile0, per, used, shared, len;
+    __device__ __forceinline__ OwnRanges(int tile_, int shared_, int len_, int ranges) : tile(tile_), shared(shared_), len(len_) {
+        tile0 = shared / tile;
+        const int tiles = len > shared ? (len + tile - 1) / tile - tile0 : 0;
+        per = (tiles + ranges - 1) / ranges;
+        used = per > 0 ? (tiles + per - 1) / per : 0;
+    }
+    __device__ __forceinline__ int begin(int i) const { return max(shared, (tile0 + i * per) * tile); }
+    __device__ __forceinline__ int end(int i) const { return min(len, (tile0 + (i + 1) * per) * tile); }
+};
+
+// ----------------------------------------------------------------------------- any element type, heads of up to 256 elements, any page size
+// A block has up to 32 rows (member, query head) of a kv head, of all members over a range of the group's shared keys or of one member over a range of its own,
+// and walks the range 32 keys at a time through shared memory, as floats, the next tile's loads under way meanwhile.  Eight lanes have a row, a sixteenth or
+// more of the dims each; where there are fewer rows, several groups of lanes share one's keys, each with a maximum, a sum and sums of its own, which meet at the
+// end.  Five sequences of 900 shared and 60 own keys in float, 16 heads over 8 of 128: MEASURED_F32 (a warp a row and range, a key at a time, 78 us).
+constexpr int ANY_TILE = 32;
+constexpr int ANY_THREADS = 256;
+constexpr int ANY_ROWS = ANY_THREADS / 8;
+
+template <typename T> __device__ __forceinline__ float4 load4(const T* p);
+template <> __device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+inline size_t any_smem(int dims) { return (size_t)2 * ANY_TILE * (dims + 4) * sizeof(float); }
+
+// FOURS: fours of dims a lane has, d <= 32 FOURS
+template <typename T, int FOURS>
+__global__ void __launch_bounds__(ANY_THREADS) shared_any_kernel(const SharedParams p) {
     pdl_launch_dependents();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + warp;
-    const int ranges = p.shared_ranges + p.own_ranges;
-    if (item >= (long long)p.n_seqs * p.nq * ranges) return;
-    const int range = (int)(item % ranges);
-    const int head = (int)(item / ranges % p.nq), at = (int)(item / ranges / p.nq);
-    const Group group = group_of(p, at);
-    const int seq = member_at(p, at);
-    const int len = max(0, min(p.seq_len[seq], p.max_blocks * p.page));
-    const int shared = min(group.shared, len);
-    const int kvh = head / (p.nq / p.nkv);
-    const bool of_group = range < p.shared_ranges;
-    const int* table = p.block_table + (size_t)(of_group ? member_at(p, group.first) : seq) * p.max_blocks;
-    const int from = of_group ? 0 : shared, count = of_group ? shared : len - shared;
-    const int n = of_group ? p.shared_ranges : p.own_ranges, i = of_group ? range : range - p.shared_ranges;
-    const int per = (count + n - 1) / n;
-    const int begin = from + min(count, i * per), end = from + min(count, (i + 1) * per);
-    const T* q = (const T*)p.q + ((size_t)seq * p.nq + head) * p.d;
-    float qv[MAX_DIM / 32], acc[MAX_DIM / 32];
-#pragma unroll
-    for (int c = 0; c < MAX_DIM / 32; ++c) { qv[c] = c * 32 + lane < p.d ? to_float(q[c * 32 + lane]) * p.scale : 0.f; acc[c] = 0.f; }
-    float m = -INFINITY, l = 0.f;
-    for (int j = begin; j < end; ++j) {
-        const int page = page_at(p, table, j / p.page);
-        const size_t off = (((size_t)page * p.nkv + kvh) * p.page + j % p.page) * p.d;
-        float s = 0.f;
-#pragma unroll
-        for (int c = 0; c < MAX_DIM / 32; ++c)
-            if (c * 32 + lane < p.d) s += qv[c] * to_float(((const T*)p.k_cache)[off + c * 32 + lane]);
-        s = warp_sum(s);
-        const float m_new = fmaxf(m, s), alpha = m == -INFINITY ? 0.f : expf(m - m_new), w = s == -INFINITY ? 0.f : expf(s - m_new);
-        l = l * alpha + w;
-#pragma unroll
-        for (int c = 0; c < MAX_DIM / 32; ++c)
-            if (c * 32 + lane < p.d) acc[c] = acc[c] * alpha + w * to_float(((const T*)p.v_cache)[off + c * 32 + lane]);
-        m = m_new;
+    extern __shared__ __align__(16) float any_tile[];
+    constexpr int DIMS = 32 * FOURS, PITCH = DIMS + 4;
+    float* k_s = any_tile;                                     // [ANY_TILE][PITCH]
+    float* v_s = any_tile + ANY_TILE * PITCH;
+    const int per = p.nq / p.nkv, ranges_all = p.shared_ranges + p.own_ranges;
+    int index = blockIdx.x;
+    const bool of_group = index < p.shared_items;
+    if (!of_group) index -= p.shared_items;
+    const int tiles = of_group ? p.row_tiles : p.own_tiles, n_ranges = of_group ? p.shared_ranges : p.own_ranges;
+    const int row0 = index % tiles * ANY_ROWS, kvh = index / tiles % p.nkv, at = index / tiles / p.nkv / n_ranges;
+    int range = index / tiles / p.nkv % n_ranges, rows, begin, end, first;
+    if (of_group) {
+        const Group group = group_at(p, at);
+        const Ranges cut(group.shared, ANY_TILE, n_ranges);
+        rows = min(ANY_ROWS, group.count * per - row0);
+        begin = range * cut.per * ANY_TILE;
+        end = min(group.shared, begin + cut.per * ANY_TILE);
+        first = group.first;
+    } else {
+        const OwnRanges cut(ANY_TILE, group_of(p, at).shared, max(0, min(p.seq_len[member_at(p, at)], p.max_blocks * p.page)), n_ranges);
+        rows = min(ANY_ROWS, per - row0);
+        begin = cut.begin(range);
+        end = cut.end(range);
+        first = at;
+        range += p.shared_ranges;
     }
-    const size_t slot = ((size_t)seq * p.nq + head) * ranges + range;
-    for (int c = 0; c < MAX_DIM / 32; ++c)
-        if (c * 32 + lane < p.d) p.part_acc[slot * p.d + c * 32 + lane] = acc[c];
-    if (lane == 0) { p.part_ml[2 * slot] = m; p.part_ml[2 * slot + 1] = l; }
+    if (rows <= 0 || begin >= end) return;
+    const int* table = p.block_table + (size_t)member_at(p, first) * p.max_blocks;
+    int width = 1;                                             // rows, rounded up to a power of two: groups of lanes g, g + width, ... have row g
+    while (width < rows) width *= 2;
+    const int group = threadIdx.x >> 3, lane = threadIdx.x & 7, share = group / width, shares = ANY_ROWS / width, row = group % width;
+    const bool live = row < rows;
+    const int place = row0 + (live ? row : 0);
+    const int seq = member_at(p, of_group ? first + place / per : first), head = kvh * per + (of_group ? place % per : place);
+    const int limit = live ? min(end, p.seq_len[seq]) : 0;
+    // fours of a row start on boundaries of theirs
+    const bool wide = p.d % 4 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache) & (4 * sizeof(T) - 1)) == 0;
+    auto four = [&](const void* base, size_t row_at, int c) {  // dims c to c + 3 of a row, zeros beyond its end
+        const T* at_row = (const T*)base + row_at;
+        if (wide && c < p.d) return load4<T>(at_row + c);
+        return make_float4(c < p.d ? to_float(at_row[c]) : 0.f, c + 1 < p.d ? to_float(at_row[c + 1]) : 0.f, c + 2 < p.d ? to_float(at_row[c + 2]) : 0.f,
+                           c + 3 < p.d ? to_float(at_row[c + 3]) : 0.f);
+    };
+    float4 q[FOURS], o[FOURS];
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) {
+        q[i] = four(p.q, ((size_t)seq * p.nq + head) * p.d, 4 * (lane + 8 * i));
+        q[i].x *= p.scale; q[i].y *= p.scale; q[i].z *= p.scale; q[i].w *= p.scale;
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float m = -INFINITY, l = 0.f;
+    // a thread brings FOURS fours of keys and of values: key threadIdx.x / 8, the dims that it also computes with
+    const int my_key = threadIdx.x >> 3;
+    float4 next_k[FOURS], next_v[FOURS];
+    auto fetch = [&](int pos0) {
+        const int pos = pos0 + my_key;
+        const bool take = pos >= begin && pos < end;           // whatever else lies there counts for nothing
+        const size_t at_row = take ? (((size_t)page_at(p, table, pos / p.page) * p.nkv + kvh) * p.page + pos % p.page) * p.d : 0;
+#pragma unroll
+        for (int i = 0; i < FOURS; ++i) {
+            next_k[i] = take ? four(p.k_cache, at_row, 4 * (lane + 8 * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            next_v[i] = take ? four(p.v_cache, at_row, 4 * (lane + 8 * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    const int tile0 = begin / ANY_TILE * ANY_TILE;
+    fetch(tile0);
+    for (int pos0 = tile0; pos0 < end; pos0 += ANY_TILE) {
+        __syncthreads();                                       // the tile before has been read
+#pragma unroll
+        for (int i = 0; i < FOURS; ++i) {
+            *reinterpret_cast<float4*>(k_s + my_key * PITCH + 4 * (lane + 8 * i)) = next_k[i];
+            *reinterpret_cast<float4*>(v_s + my_key * PITCH + 4 * (lane + 8 * i)) = next_v[i];
+        }
+        __syncthreads();
+        if (pos0 + ANY_TILE < end) fetch(pos0 + ANY_TILE);
+        for (int j0 = share; j0 < ANY_TILE; j0 += 4 * shares) {
+            float s[4];
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = j0 + u * shares;
+                s[u] = 0.f;
+                if (j < ANY_TILE) {
+#pragma unroll
+                    for (int i = 0; i < FOURS; ++i) {
+                        const float4 k = *reinterpret_cast<const float4*>(k_s + j * PITCH + 4 * (lane + 8 * i));
+                        s[u] = fmaf(q[i].x, k.x, fmaf(q[i].y, k.y, fmaf(q[i].z, k.z, fmaf(q[i].w, k.w, s[u]))));
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int off = 1; off < 8; off <<= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], off);
+                const int pos = pos0 + j0 + u * shares;
+                if (j0 + u * shares >= ANY_TILE || pos < begin || pos >= limit) s[u] = -INFINITY;
+                top = fmaxf(top, s[u]);
+            }
+            const float at_top = top == -INFINITY ? 0.f : top;
+            if (top > m) {
+                const float alpha = expf(m - at_top);
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < FOURS; ++i) { o[i].x *= alpha; o[i].y *= alpha; o[i].z *= alpha; o[i].w *= alpha; }
+                m = top;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = j0 + u * shares;
+                const float w = expf(s[u] - at_top);           // 0 of -inf
+                l += w;
+                if (j < ANY_TILE) {
+#pragma unroll
+                    for (int i = 0; i < FOURS; ++i) {
+                        const float4 v = *reinterpret_cast<const float4*>(v_s + j * PITCH + 4 * (lane + 8 * i));
+                        o[i].x = fmaf(w, v.x, o[i].x); o[i].y = fmaf(w, v.y, o[i].y); o[i].z = fmaf(w, v.z, o[i].z); o[i].w = fmaf(w, v.w, o[i].w);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    float* meet = any_tile;                                    // [ANY_ROWS][PITCH]: sums, then maximum and sum of weights behind them
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) *reinterpret_cast<float4*>(meet + group * PITCH + 4 * (lane + 8 * i)) = o[i];
+    if (lane == 0) { meet[group * PITCH + DIMS] = m; meet[group * PITCH + DIMS + 1] = l; }
+    __syncthreads();
+    if (!live || share > 0) return;
+    float top = -INFINITY, total = 0.f;
+    for (int i = 0; i < shares; ++i) top = fmaxf(top, meet[(row + i * width) * PITCH + DIMS]);
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < shares; ++i) {
+        const float* part = meet + (row + i * width) * PITCH;
+        const float f = part[DIMS] == -INFINITY ? 0.f : expf(part[DIMS] - top);
+        total += part[DIMS + 1] * f;
+#pragma unroll
+        for (int c = 0; c < FOURS; ++c) {
+            const float4 v = *reinterpret_cast<const float4*>(part + 4 * (lane + 8 * c));
+            o[c].x = fmaf(v.x, f, o[c].x); o[c].y = fmaf(v.y, f, o[c].y); o[c].z = fmaf(v.z, f, o[c].z); o[c].w = fmaf(v.w, f, o[c].w);
+        }
+    }
+    const size_t slot = ((size_t)seq * p.nq + head) * ranges_all + range;
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) {
+        const float x[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (4 * (lane + 8 * i) + e < p.d) p.part_acc[slot * p.d + 4 * (lane + 8 * i) + e] = x[e];
+    }
+    if (lane == 0) { p.part_ml[2 * slot] = top; p.part_ml[2 * slot + 1] = total; }
 }
 
 // A block joins the ranges of a row; a row without a key is zero.
@@ -110,18 +262,21 @@ template <typename T>
 __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) {
     pdl_launch_dependents();
     pdl_wait();
-    const size_t row = blockIdx.x;
-    const int ranges = p.shared_ranges + p.own_ranges;
-    const float* ml = p.part_ml + row * ranges * 2;
+    const int head = blockIdx.x % p.nq, at = blockIdx.x / p.nq, seq = member_at(p, at), shared = group_of(p, at).shared;
+    const int of_group = Ranges(shared, ANY_TILE, p.shared_ranges).used;
+    const int parts = of_group + OwnRanges(ANY_TILE, shared, max(0, min(p.seq_len[seq], p.max_blocks * p.page)), p.own_ranges).used;
+    const size_t row = (size_t)seq * p.nq + head, slot0 = row * (p.shared_ranges + p.own_ranges);
+    auto slot_of = [&](int k) { return slot0 + (k < of_group ? k : p.shared_ranges + k - of_group); };
     float m = -INFINITY;
-    for (int s = 0; s < ranges; ++s) m = fmaxf(m, ml[2 * s]);
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[2 * slot_of(k)]);
     for (int c = threadIdx.x; c < p.d; c += blockDim.x) {
         float a = 0.f, l = 0.f;
-        for (int s = 0; s < ranges; ++s) {
-            if (ml[2 * s] == -INFINITY) continue;
-            const float f = expf(ml[2 * s] - m);
-            l += ml[2 * s + 1] * f;
-            a += p.part_acc[(row * ranges + s) * p.d + c] * f;
+        for (int k = 0; k < parts; ++k) {
+            const float mk = p.part_ml[2 * slot_of(k)], lk = p.part_ml[2 * slot_of(k) + 1];
+            if (mk == -INFINITY && lk == 0.f) continue;
+            const float f = expf(mk - m);
+            l += lk * f;
+            a += p.part_acc[slot_of(k) * p.d + c] * f;
         }
         ((T*)p.out)[row * p.d + c] = from_float<T>(l == 0.f ? 0.f : a / l);
     }
@@ -216,29 +371,6 @@ __device__ __forceinline__ uint64_t operand_desc_mn(uint32_t saddr, uint32_t mn_
     return d;
 }
 
-// Ranges of a group's shared pages: `per` pages each but the last; ranges from `used` on hold nothing and leave no partial result.
-struct Ranges {
-    int per, used;
-    __device__ __forceinline__ Ranges(int tokens, int tile, int ranges) {
-        const int tiles = (tokens + tile - 1) / tile;
-        per = (tiles + ranges - 1) / ranges;
-        used = per > 0 ? (tiles + per - 1) / per : 0;
-    }
-};
-
-// The ranges of a member's own keys, in tiles from the one on in which the shared keys end.
-struct OwnRanges {
-    int tile, tile0, per, used, shared, len;
-    __device__ __forceinline__ OwnRanges(int tile_, int shared_, int len_, int ranges) : tile(tile_), shared(shared_), len(len_) {
-        tile0 = shared / tile;
-        const int tiles = len > shared ? (len + tile - 1) / tile - tile0 : 0;
-        per = (tiles + ranges - 1) / ranges;
-        used = per > 0 ? (tiles + per - 1) / per : 0;
-    }
-    __device__ __forceinline__ int begin(int i) const { return max(shared, (tile0 + i * per) * tile); }
-    __device__ __forceinline__ int end(int i) const { return min(len, (tile0 + (i + 1) * per) * tile); }
-};
-
 template <int HD>
 __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                          const SharedParams p) {
@@ -276,7 +408,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
     const int per = p.nq / p.nkv, stride = p.shared_ranges + p.own_ranges;
     // Blocks of shared keys and blocks of own keys take turns by as many as there are multiprocessors, so that each of these has one of either kind: the
     // first are bound by the tensor cores and the exponentials, the second by memory.
-    const int turns = min(p.shared_blocks, p.own_blocks) / p.turn;
+    const int turns = min(p.shared_items, p.own_items) / p.turn;
     int index = blockIdx.x;
     bool of_group;
     if (index < 2 * turns * p.turn) {
@@ -284,8 +416,8 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
         index = index / p.turn / 2 * p.turn + index % p.turn;
     } else {
         index -= turns * p.turn;
-        of_group = index < p.shared_blocks;
-        if (!of_group) index -= p.shared_blocks - turns * p.turn;
+        of_group = index < p.shared_items;
+        if (!of_group) index -= p.shared_items - turns * p.turn;
     }
     // What this block has: `rows` rows from row0 on, of a group (member by member) or of one member, the keys [begin, end) of a page list.  Neighbours in
     // the grid share keys: the row tiles of a kv head and range.
@@ -800,6 +932,22 @@ int cache_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t d) {
     return QT_OK;
 }
 
+template <typename T, int FOURS>
+int launch_any(SharedParams p, int most_members, cudaStream_t stream) {
+    const size_t smem = any_smem(32 * FOURS);
+    const cudaError_t raised = raise_shared<shared_any_kernel<T, FOURS>>((int)smem);
+    if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_shared: cannot raise shared memory: %s", cudaGetErrorString(raised));
+    const int per = p.nq / p.nkv;
+    const long long tiles = ((long long)most_members * per + ANY_ROWS - 1) / ANY_ROWS, own_tiles = (per + ANY_ROWS - 1) / ANY_ROWS;
+    const long long shared = tiles * p.nkv * p.shared_ranges * p.n_groups, own = own_tiles * p.nkv * p.own_ranges * p.n_seqs;
+    QT_REQUIRE(shared + own <= 0x3fffffffll && (long long)p.n_seqs * p.nq <= 0x7fffffffll, "attention_shared: too many rows for one launch");
+    p.row_tiles = (int)tiles; p.own_tiles = (int)own_tiles; p.shared_items = (int)shared; p.own_items = (int)own;
+    launch_kernel(shared_any_kernel<T, FOURS>, dim3((unsigned)(shared + own)), dim3(ANY_THREADS), smem, stream, p);
+    launch_kernel(shared_join_kernel<T>, dim3((unsigned)(p.n_seqs * p.nq)), dim3(128), 0, stream, p);
+    QT_CHECK_LAUNCH("attention_shared");
+    return QT_OK;
+}
+
 template <int HD>
 int launch_parts(SharedParams p, int most_members, cudaStream_t stream) {
     CUtensorMap map_k, map_v;
@@ -813,7 +961,7 @@ int launch_parts(SharedParams p, int most_members, cudaStream_t stream) {
     const long long tiles = ((long long)most_members * per + BQ - 1) / BQ, own_tiles = (per + BQ - 1) / BQ, heads = (long long)p.nkv * ((per + 15) / 16);
     const long long shared = tiles * p.nkv * p.shared_ranges * p.n_groups, own = own_tiles * p.nkv * p.own_ranges * p.n_seqs;
     QT_REQUIRE(shared + own <= 0x3fffffffll && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
-    p.row_tiles = (int)tiles; p.own_tiles = (int)own_tiles; p.shared_blocks = (int)shared; p.own_blocks = (int)own; p.turn = sm_count();
+    p.row_tiles = (int)tiles; p.own_tiles = (int)own_tiles; p.shared_items = (int)shared; p.own_items = (int)own; p.turn = sm_count();
     launch_kernel(shared_parts_kernel<HD>, dim3((unsigned)(shared + own)), dim3(TC_THREADS), smem, stream, map_k, map_v, p);
     launch_kernel(shared_join_parts_kernel, dim3((unsigned)heads, p.n_seqs), dim3(JOIN_THREADS), 0, stream, p);
     QT_CHECK_LAUNCH("attention_shared");
@@ -865,13 +1013,10 @@ extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, co
         return d <= 64 ? launch_parts<64>(p, most_members, s) : launch_parts<128>(p, most_members, s);
     }
     QT_REQUIRE(shared_ranges > 0, "attention_shared: %d ranges of shared keys", shared_ranges);
-    const long long items = (long long)n_seqs * nq * (shared_ranges + own_ranges);
-    QT_REQUIRE(items / 4 < 0x7fffffffll, "attention_shared: too many rows for one launch");
     return QT_DISPATCH_DTYPE(dtype, "attention_shared", {
-        launch_kernel(shared_simple_kernel<T>, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, s, p);
-        launch_kernel(shared_join_kernel<T>, dim3((unsigned)(n_seqs * nq)), dim3(128), 0, s, p);
-        QT_CHECK_LAUNCH("attention_shared");
-        return QT_OK;
+        if (d <= 64) return launch_any<T, 2>(p, most_members, s);
+        if (d <= 128) return launch_any<T, 4>(p, most_members, s);
+        return launch_any<T, 8>(p, most_members, s);
     });
 }
 

@@ -1472,8 +1472,9 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
         shared_ranges = min(range(1, 33), key=lambda r: (-(-tiles // r) * (0.70 if rows * r <= sms else 1.22 * -(-rows * r // (2 * sms))) + 0.4 * r, r))
         own_ranges = max(1, min(16, -(-most_own // 64 // max(8, -(-tiles // shared_ranges)))))
     else:
-        shared_ranges = max(1, min(32, -(-most_shared // 128)))
-        own_ranges = max(1, min(8, -(-most_own // 256)))
+        # blocks of 32 rows, about three an SM, ranges of at least 64 keys
+        shared_ranges = max(1, min(32, -(-most_shared // 64), 3 * sms // (num_kv_heads * groups * max(1, -(-most_members * group // 32)))))
+        own_ranges = max(1, min(16, -(-most_own // 64), max(-(-most_own // 512), 3 * sms // max(1, n_seqs * num_kv_heads * -(-group // 32)))))
     own_ranges = min(own_ranges, max(1, most_ranges - shared_ranges), most_ranges - 1)
     shared_ranges = min(shared_ranges, most_ranges - own_ranges)
     return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges, page_tokens)
