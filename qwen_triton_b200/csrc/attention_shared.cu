@@ -257,31 +257,6 @@ __global__ void __launch_bounds__(ANY_THREADS) shared_any_kernel(const SharedPar
     if (lane == 0) { p.part_ml[2 * slot] = top; p.part_ml[2 * slot + 1] = total; }
 }
 
-// A block joins the ranges of a row; a row without a key is zero.
-template <typename T>
-__global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int head = blockIdx.x % p.nq, at = blockIdx.x / p.nq, seq = member_at(p, at), shared = group_of(p, at).shared;
-    const int of_group = Ranges(shared, ANY_TILE, p.shared_ranges).used;
-    const int parts = of_group + OwnRanges(ANY_TILE, shared, max(0, min(p.seq_len[seq], p.max_blocks * p.page)), p.own_ranges).used;
-    const size_t row = (size_t)seq * p.nq + head, slot0 = row * (p.shared_ranges + p.own_ranges);
-    auto slot_of = [&](int k) { return slot0 + (k < of_group ? k : p.shared_ranges + k - of_group); };
-    float m = -INFINITY;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[2 * slot_of(k)]);
-    for (int c = threadIdx.x; c < p.d; c += blockDim.x) {
-        float a = 0.f, l = 0.f;
-        for (int k = 0; k < parts; ++k) {
-            const float mk = p.part_ml[2 * slot_of(k)], lk = p.part_ml[2 * slot_of(k) + 1];
-            if (mk == -INFINITY && lk == 0.f) continue;
-            const float f = expf(mk - m);
-            l += lk * f;
-            a += p.part_acc[slot_of(k) * p.d + c] * f;
-        }
-        ((T*)p.out)[row * p.d + c] = from_float<T>(l == 0.f ? 0.f : a / l);
-    }
-}
-
 // ----------------------------------------------------------------------------- bfloat16, heads of up to 128 elements, pages of 64
 // Two launches.  In the first a block has up to 128 rows (member, query head) of a kv head as the M of products on tcgen05 and walks a range of pages: rows of
 // all members over the group's shared keys, or one member's rows over keys of its own,
@@ -649,7 +624,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
 }
 
 // What rows' partial results are multiplied by: row r of `rows` has `parts` of them, ml(r, k) their maximum and sum; a warp a row.
-template <typename ML>
+template <bool BASE2, typename ML>
 __device__ __forceinline__ void part_factors(float* factors, int rows, int parts, int warp, int warps, int lane, ML ml) {
     constexpr int TURNS = (MAX_PARTS + 31) / 32;
     for (int r = warp; r < rows; r += warps) {
@@ -664,7 +639,7 @@ __device__ __forceinline__ void part_factors(float* factors, int rows, int parts
         m_all = warp_max(m_all);
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
-            mk[i] = mk[i] == -INFINITY ? 0.f : fast_exp2(mk[i] - m_all);
+            mk[i] = mk[i] == -INFINITY ? 0.f : BASE2 ? fast_exp2(mk[i] - m_all) : expf(mk[i] - m_all);
             l_all += lk[i] * mk[i];
         }
         l_all = warp_sum(l_all);
@@ -678,23 +653,37 @@ __device__ __forceinline__ void add_part(float4& a, float4 v, float by) {      /
     if (by != 0.f) { a.x += v.x * by; a.y += v.y * by; a.z += v.z * by; a.w += v.w * by; }
 }
 
-// Joins the partial results of up to 16 query heads of a member's kv head.
+// Joins the partial results of up to 16 query heads of a member's kv head.  TILE: what ranges are cut in; BASE2: maxima are base 2, and the exponential may be
+// approximate.
 constexpr int JOIN_THREADS = 128;
 
-__global__ void __launch_bounds__(JOIN_THREADS) shared_join_parts_kernel(const SharedParams p) {
+template <typename T, int TILE, bool BASE2>
+__global__ void __launch_bounds__(JOIN_THREADS) shared_join_kernel(const SharedParams p) {
     pdl_launch_dependents();
     __shared__ float factors[16 * MAX_PARTS];
     const int tid = threadIdx.x, per = p.nq / p.nkv, heads16 = (per + 15) / 16, stride = p.shared_ranges + p.own_ranges;
     const int h0 = blockIdx.x % heads16 * 16, rows = min(16, per - h0), head0 = blockIdx.x / heads16 * per + h0;
     pdl_wait();
     const int seq = member_at(p, blockIdx.y), shared = group_of(p, blockIdx.y).shared;
-    const int of_group = Ranges(shared, PAGE, p.shared_ranges).used;
-    const int parts = of_group + OwnRanges(PAGE, shared, max(0, min(p.seq_len[seq], p.max_blocks * PAGE)), p.own_ranges).used;
+    const int of_group = Ranges(shared, TILE, p.shared_ranges).used;
+    const int parts = of_group + OwnRanges(TILE, shared, max(0, min(p.seq_len[seq], p.max_blocks * p.page)), p.own_ranges).used;
     const size_t row0 = (size_t)seq * p.nq + head0;
     auto slot_of = [&](int k) { return k < of_group ? k : p.shared_ranges + k - of_group; };
-    part_factors(factors, rows, parts, tid >> 5, JOIN_THREADS / 32, tid & 31,
-                 [&](int r, int k) { return *reinterpret_cast<const float2*>(p.part_ml + 2 * ((row0 + r) * stride + slot_of(k))); });
+    part_factors<BASE2>(factors, rows, parts, tid >> 5, JOIN_THREADS / 32, tid & 31,
+                        [&](int r, int k) { return *reinterpret_cast<const float2*>(p.part_ml + 2 * ((row0 + r) * stride + slot_of(k))); });
     __syncthreads();
+    if (p.d % 4) {                                             // rows that are not whole fours
+        for (int i = tid; i < rows * p.d; i += JOIN_THREADS) {
+            const int r = i / p.d, c = i % p.d;
+            float a = 0.f;
+            for (int k = 0; k < parts; ++k) {
+                const float f = factors[r * MAX_PARTS + k];
+                if (f != 0.f) a += p.part_acc[((row0 + r) * stride + slot_of(k)) * p.d + c] * f;
+            }
+            ((T*)p.out)[(row0 + r) * p.d + c] = from_float<T>(a);
+        }
+        return;
+    }
     const int quads = p.d / 4;
     for (int i = tid; i < rows * quads; i += JOIN_THREADS) {
         const int r = i / quads, c = i % quads * 4;
@@ -702,7 +691,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) shared_join_parts_kernel(const S
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
         for (int k = 0; k < parts; ++k) add_part(a, *reinterpret_cast<const float4*>(acc + (size_t)slot_of(k) * p.d), factors[r * MAX_PARTS + k]);
-        *reinterpret_cast<uint2*>((__nv_bfloat16*)p.out + (row0 + r) * p.d + c) = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
+        T* to = (T*)p.out + (row0 + r) * p.d + c;
+        to[0] = from_float<T>(a.x); to[1] = from_float<T>(a.y); to[2] = from_float<T>(a.z); to[3] = from_float<T>(a.w);
     }
 }
 
@@ -909,7 +899,7 @@ __global__ void __launch_bounds__(32 * DIRECT_MAX_WARPS) shared_direct_kernel(co
     }
     const float* from = gridDim.x > 1 ? inbox : sums;
     const int parts = gridDim.x > 1 ? gridDim.x : warps;
-    part_factors(factors, rows, parts, warp, warps, lane, [&](int r, int k) { return *reinterpret_cast<const float2*>(from + (size_t)(k * rows + r) * SLOT + HD); });
+    part_factors<true>(factors, rows, parts, warp, warps, lane, [&](int r, int k) { return *reinterpret_cast<const float2*>(from + (size_t)(k * rows + r) * SLOT + HD); });
     __syncthreads();
     for (int i = tid; i < rows * QUADS; i += threads) {
         const int r = i / QUADS, c = i % QUADS * 4;
@@ -940,10 +930,12 @@ int launch_any(SharedParams p, int most_members, cudaStream_t stream) {
     const int per = p.nq / p.nkv;
     const long long tiles = ((long long)most_members * per + ANY_ROWS - 1) / ANY_ROWS, own_tiles = (per + ANY_ROWS - 1) / ANY_ROWS;
     const long long shared = tiles * p.nkv * p.shared_ranges * p.n_groups, own = own_tiles * p.nkv * p.own_ranges * p.n_seqs;
-    QT_REQUIRE(shared + own <= 0x3fffffffll && (long long)p.n_seqs * p.nq <= 0x7fffffffll, "attention_shared: too many rows for one launch");
+    QT_REQUIRE(shared + own <= 0x3fffffffll, "attention_shared: too many rows for one launch");
     p.row_tiles = (int)tiles; p.own_tiles = (int)own_tiles; p.shared_items = (int)shared; p.own_items = (int)own;
     launch_kernel(shared_any_kernel<T, FOURS>, dim3((unsigned)(shared + own)), dim3(ANY_THREADS), smem, stream, p);
-    launch_kernel(shared_join_kernel<T>, dim3((unsigned)(p.n_seqs * p.nq)), dim3(128), 0, stream, p);
+    const long long heads = (long long)p.nkv * ((per + 15) / 16);
+    QT_REQUIRE(heads <= 0x7fffffffll && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
+    launch_kernel(shared_join_kernel<T, ANY_TILE, false>, dim3((unsigned)heads, p.n_seqs), dim3(JOIN_THREADS), 0, stream, p);
     QT_CHECK_LAUNCH("attention_shared");
     return QT_OK;
 }
@@ -963,7 +955,7 @@ int launch_parts(SharedParams p, int most_members, cudaStream_t stream) {
     QT_REQUIRE(shared + own <= 0x3fffffffll && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
     p.row_tiles = (int)tiles; p.own_tiles = (int)own_tiles; p.shared_items = (int)shared; p.own_items = (int)own; p.turn = sm_count();
     launch_kernel(shared_parts_kernel<HD>, dim3((unsigned)(shared + own)), dim3(TC_THREADS), smem, stream, map_k, map_v, p);
-    launch_kernel(shared_join_parts_kernel, dim3((unsigned)heads, p.n_seqs), dim3(JOIN_THREADS), 0, stream, p);
+    launch_kernel(shared_join_kernel<__nv_bfloat16, PAGE, true>, dim3((unsigned)heads, p.n_seqs), dim3(JOIN_THREADS), 0, stream, p);
     QT_CHECK_LAUNCH("attention_shared");
     return QT_OK;
 }
@@ -999,13 +991,13 @@ extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, co
     if (n_seqs == 0) return QT_OK;
     const SharedParams p{q, k_cache, v_cache, out, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, nq, nkv, d, page_tokens, n_pages,
                          scale, shared_ranges, own_ranges, part_acc, part_ml, status, 0, 0, 0, 0, 0};
+    QT_REQUIRE((((uintptr_t)part_acc | (uintptr_t)part_ml) & 15) == 0, "attention_shared: scratch must be 16-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
     if (on_tc) {
         QT_REQUIRE(dtype == QT_BF16 && d % 8 == 0 && d <= 128 && page_tokens == PAGE && status,
                    "attention_shared: the tensor-core kernels take bfloat16, heads of up to 128 in steps of 8, pages of 64 (d=%d, pages of %d)", d, page_tokens);
         QT_REQUIRE((long long)n_pages * nkv * PAGE <= 0x7fffffffll, "attention_shared: %d pages of %d heads are beyond a tensor map", n_pages, nkv);
-        QT_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)part_acc | (uintptr_t)part_ml) & 15) == 0,
-                   "attention_shared: operands must be 16-byte aligned");
+        QT_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) == 0, "attention_shared: operands must be 16-byte aligned");
         if (shared_ranges == 0) {
             QT_REQUIRE(own_ranges <= 8 && direct_warps > 0 && direct_warps <= DIRECT_MAX_WARPS, "attention_shared: %d blocks of %d warps", own_ranges, direct_warps);
             return d <= 64 ? launch_direct<64>(p, direct_warps, s) : launch_direct<128>(p, direct_warps, s);

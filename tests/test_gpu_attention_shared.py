@@ -137,6 +137,17 @@ def test_long_prefix_and_long_own_keys():
     case.check(case.run())
 
 
+def test_float32_from_odd_addresses():
+    """Operands that start between the boundaries of wide loads."""
+    case = Case([(70, [1, 20, 90]), (0, [5])], 4, 2, 64, torch.float32, seed=3)
+    def moved(tensor):
+        place = torch.empty(tensor.numel() + 1, dtype=tensor.dtype, device="cuda")[1:].view(tensor.shape)
+        return place.copy_(tensor)
+    out = moved(torch.zeros_like(case.q))
+    case.run(q=moved(case.q), k_cache=moved(case.k), v_cache=moved(case.v), out=out)
+    case.check(out)
+
+
 def test_sequences_without_keys():
     case = Case([(100, [5, None, 7]), (0, [None]), (64, [None, None])], 8, 2, 64, seed=6)
     case.check(case.run())
@@ -266,6 +277,8 @@ def test_refusals():
         with pytest.raises(KernelError):
             plan = dataclasses.replace(case.plan, **changes)
             case.run(plan, part_acc=torch.empty(max(plan.acc_elements, 1), device="cuda"), part_ml=torch.empty(max(plan.ml_elements, 1), device="cuda"))
+    with pytest.raises(KernelError, match="aligned"):
+        case.run(part_acc=torch.empty(case.plan.acc_elements + 1, device="cuda")[1:])
     wide = Case([(70, [1, 5])], 40, 2, 128)                   # more shared memory than a block has
     with pytest.raises(KernelError, match="shared memory"):
         wide.run(dataclasses.replace(wide.plan, shared_ranges=0, own_ranges=8, direct_warps=6))
