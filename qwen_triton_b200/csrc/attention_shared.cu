@@ -102,8 +102,8 @@ inline size_t any_smem(int dims) { return (size_t)2 * ANY_TILE * (dims + 4) * si
 // FOURS: fours of dims a lane has, d <= 32 FOURS
 template <typename T, int FOURS>
 __global__ void __launch_bounds__(ANY_THREADS) shared_any_kernel(const SharedParams p) {
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     extern __shared__ __align__(16) float any_tile[];
     constexpr int DIMS = 32 * FOURS, PITCH = DIMS + 4;
     float* k_s = any_tile;                                     // [ANY_TILE][PITCH]
@@ -361,8 +361,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
     const uint32_t base = (raw + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw);
     const uint32_t q_s = base, k_s = q_s + Q_BYTES, v_s = k_s + 2 * KV_BYTES, bars = v_s + 2 * KV_BYTES;
-    const uint32_t q_full = bars, k_full = bars + 8, k_empty = bars + 24, v_full = bars + 40, v_empty = bars + 56;
-    const uint32_t s_full = bars + 72, p_full = bars + 88, pv_full = bars + 104;
+    const uint32_t q_full = bars, k_full = bars + 8, v_full = bars + 24, s_full = bars + 40, p_full = bars + 56, pv_full = bars + 72;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bars - base) + 128);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int* status = p.status;
@@ -372,8 +371,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
         prefetch_tensor_map(&map_v);
         mbar_init(q_full, 4);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_full + 8 * i, 1); mbar_init(v_empty + 8 * i, 1);
+            mbar_init(k_full + 8 * i, 1); mbar_init(v_full + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4);
             mbar_init(pv_full + 8 * i, 1);
         }
@@ -436,7 +434,8 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
         if (lane == 0) {
             for (int j = 0; j < n_tiles; ++j) {
                 const int s = j & 1, row = row_of_tile(j);
-                if (!mbar_wait(k_empty + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u, status, 1)) break;
+                // the stage's last product has been formed: its scores were there
+                if (!mbar_wait(s_full + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u, status, 1)) break;
                 mbar_expect_tx(k_full + 8 * s, KV_BYTES);
                 for (int h = 0; h < HALVES; ++h) tma_load_2d(k_s + s * KV_BYTES + h * KEY_HALF_BYTES, &map_k, k_full + 8 * s, h * 64, row);
             }
@@ -445,7 +444,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
         if (lane == 0) {
             for (int j = 0; j < n_tiles; ++j) {
                 const int s = j & 1, row = row_of_tile(j);
-                if (!mbar_wait(v_empty + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u, status, 1)) break;
+                if (!mbar_wait(pv_full + 8 * s, ((uint32_t)(j >> 1) & 1u) ^ 1u, status, 1)) break;
                 mbar_expect_tx(v_full + 8 * s, KV_BYTES);
                 for (int h = 0; h < HALVES; ++h) tma_load_2d(v_s + s * KV_BYTES + h * KEY_HALF_BYTES, &map_v, v_full + 8 * s, h * 64, row);
             }
@@ -467,7 +466,6 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
                         k_desc + (uint64_t)(((uint32_t)(ks >> 2) * KEY_HALF_BYTES + in_half) >> 4), IDESC_QK, ks > 0 ? 1u : 0u, one);
             }
             commit_one(s_full + 8 * s, one);
-            commit_one(k_empty + 8 * s, one);
             return true;
         };
         bool ok = wait(q_full, 0) && issue_qk(0);
@@ -483,7 +481,6 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
                 mma_one_a_tmem(tmem_base + O_COL, tmem_base + s * PAGE + (uint32_t)(ks * 8), v_desc + (uint64_t)(((uint32_t)ks * (16 * 128)) >> 4), IDESC_PV,
                                (j > 0 || ks > 0) ? 1u : 0u, one);
             commit_one(pv_full + 8 * s, one);
-            commit_one(v_empty + 8 * s, one);
         }
     } else {
         const int quarter = warp & 3;
@@ -505,7 +502,8 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        float m_run = -INFINITY, l_run = 0.f;                  // the maximum this row scales by (base 2) and its sum
+        float m_run = -INFINITY;                               // the maximum this row scales by (base 2)
+        uint64_t sum2[2] = {0ull, 0ull};                       // its sum, in two pairs
         bool ok = true;
         for (int j = 0; j < n_tiles; ++j) {
             const int s = j & 1;
@@ -567,7 +565,11 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
                 }
                 tmem_wait_st();
             }
-            uint64_t sum2[2] = {0ull, 0ull};
+            if (__any_sync(0xffffffffu, moves)) {
+                const uint64_t alpha2 = pair_f32(alpha, alpha);
+                sum2[0] = fma2(sum2[0], alpha2, 0ull);
+                sum2[1] = fma2(sum2[1], alpha2, 0ull);
+            }
             const uint64_t scale22 = pair_f32(scale2, scale2), neg_m2 = pair_f32(-m_use, -m_use);
             uint32_t packed[32];
 #pragma unroll
@@ -585,10 +587,6 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + 8 * s);
-            float sum[4];
-            unpair_f32(sum2[0], sum[0], sum[2]);
-            unpair_f32(sum2[1], sum[1], sum[3]);
-            l_run = l_run * alpha + (sum[0] + sum[1]) + (sum[2] + sum[3]);
             m_run = m_new;
         }
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_full + 8 * ((n_tiles - 1) & 1), (uint32_t)((n_tiles - 1) >> 1) & 1u, status, 3));
@@ -609,7 +607,10 @@ __global__ void __launch_bounds__(TC_THREADS, 2) shared_parts_kernel(const __gri
                         }
                 }
             }
-            if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(m_run, l_run);
+            float sum[4];
+            unpair_f32(sum2[0], sum[0], sum[2]);
+            unpair_f32(sum2[1], sum[1], sum[3]);
+            if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(m_run, (sum[0] + sum[1]) + (sum[2] + sum[3]));
         }
     }
     __syncwarp();
@@ -663,10 +664,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) shared_join_kernel(const SharedP
     __shared__ float factors[16 * MAX_PARTS];
     const int tid = threadIdx.x, per = p.nq / p.nkv, heads16 = (per + 15) / 16, stride = p.shared_ranges + p.own_ranges;
     const int h0 = blockIdx.x % heads16 * 16, rows = min(16, per - h0), head0 = blockIdx.x / heads16 * per + h0;
-    pdl_wait();
+    // The kernel before this one lets it start once each of its blocks is past its own wait: what kernels before that one wrote (lists and lengths) is there.
     const int seq = member_at(p, blockIdx.y), shared = group_of(p, blockIdx.y).shared;
     const int of_group = Ranges(shared, TILE, p.shared_ranges).used;
     const int parts = of_group + OwnRanges(TILE, shared, max(0, min(p.seq_len[seq], p.max_blocks * p.page)), p.own_ranges).used;
+    pdl_wait();                                                // the partial results
     const size_t row0 = (size_t)seq * p.nq + head0;
     auto slot_of = [&](int k) { return k < of_group ? k : p.shared_ranges + k - of_group; };
     part_factors<BASE2>(factors, rows, parts, tid >> 5, JOIN_THREADS / 32, tid & 31,

@@ -1466,10 +1466,17 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
                 blocks *= 2
             warps = max(1, min(2 if pairs > sms else 4, -(-most_len // (32 * blocks))))
             return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, 0, blocks, page_tokens, warps)
-        # A block takes about 0.70 us a tile of 64 keys alone on its SM and 1.22 us beside another; a range more costs about 0.4 us, in partial results and
-        # in what it takes from the blocks of own keys.
         rows, tiles = num_kv_heads * groups * max(1, -(-most_members * group // 128)), -(-most_shared // 64)
-        shared_ranges = min(range(1, 33), key=lambda r: (-(-tiles // r) * (0.70 if rows * r <= sms else 1.22 * -(-rows * r // (2 * sms))) + 0.4 * r, r))
+        own_us = n_seqs * num_kv_heads * -(-group // 128) * (0.9 * -(-most_own // 64) * 0.75 + 5.0)
+
+        def microseconds(ranges: int) -> float:
+            # Two blocks an SM.  A block takes about 4 us, and a tile of 64 keys 0.7 us where few blocks run, 1.2 us beside another; a block of own keys 5 us and
+            # 0.9 us a tile (members have three quarters of the longest's, say).  The slowest block or all of them over their places, and 0.4 us a range for its
+            # partial results.
+            each = -(-tiles // ranges) * (0.7 if rows * ranges + n_seqs * num_kv_heads <= sms else 1.2) + 4.0
+            return max(each, (rows * ranges * each + own_us) / (2 * sms)) + 0.4 * ranges
+
+        shared_ranges = min(range(1, 33), key=lambda r: (microseconds(r), r))
         own_ranges = max(1, min(16, -(-most_own // 64 // max(8, -(-tiles // shared_ranges)))))
     else:
         # blocks of 32 rows, about three an SM, ranges of at least 64 keys
