@@ -63,14 +63,15 @@ class SharedPrefixes:
 
 
 def shared_shape(groups: list[tuple[list[int], int]], lengths: list[int]) -> tuple[int, int, int, int]:
-    """(groups, members, shared tokens, own tokens) at most, rounded up: groups and members to powers of two, shared tokens to 1,024, own ones to a power of
-    two from 64 on."""
+    """(groups, members, shared tokens, own tokens) at most, rounded up: groups and members to powers of two, shared tokens to a power of two from 64 to
+    1,024 and to multiples of that beyond, own ones to a power of two from 64 on."""
     def power(n: int, least: int = 1) -> int:
         while least < n:
             least *= 2
         return least
     own = max(lengths[p] - shared for places, shared in groups for p in places)
-    return (power(len(groups)), power(max(len(places) for places, _ in groups)), -(-max(shared for _, shared in groups) // 1024) * 1024, power(own, 64))
+    most = max(shared for _, shared in groups)
+    return (power(len(groups)), power(max(len(places) for places, _ in groups)), power(most, 64) if most <= 1024 else -(-most // 1024) * 1024, power(own, 64))
 
 
 class StepContext:

@@ -1487,9 +1487,14 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
     return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges, page_tokens)
 
 
-def sharing_pays(n_seqs: int, most_members: int, most_shared: int) -> bool:
-    """Whether one-token steps are faster by ``attention_decode_shared`` than by ``attention_decode``."""
-    return (most_members - 1) * most_shared >= 4096
+SHARING_PAYS = 56 << 20       # keys and values, in bfloat16's bytes, that are not read again
+
+
+def sharing_pays(most_members: int, most_shared: int, num_kv_heads: int, head_dim: int) -> bool:
+    """Whether a one-token step is faster by ``attention_decode_shared`` than by ``attention_decode``: by what the other members would read again.  32 heads over 8
+    of 128, microseconds, one / the other: 16 sequences of 512 shared and 64 own tokens 9.5 / 12.7, of 1,024 14.1 / 13.2, of 4,096 39 / 17; 8 of 1,024 11.5 / 12.2,
+    of 2,048 15.8 / 12.8, of 16,384 71 / 29; 2 of 4,096 12.1 / 18.2, of 16,384 29 / 26; 64 of 16,384 480 / 39."""
+    return (most_members - 1) * most_shared * num_kv_heads * head_dim * 4 >= SHARING_PAYS
 
 
 def _check_shared(q, k_cache, v_cache, out, block_table, seq_len, members, share, num_kv_heads, page_tokens, plan, part_acc, part_ml) -> None:
@@ -1531,13 +1536,15 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             and seq_len.shape == members.shape == shape[:1] and share.shape == plan.share_shape and num_kv_heads == plan.num_kv_heads and page_tokens == plan.page_tokens
             and block_table.dtype is seq_len.dtype is members.dtype is share.dtype is torch.int32 and part_acc.dtype is part_ml.dtype is torch.float32
             and part_acc.numel() >= plan.acc_elements and part_ml.numel() >= plan.ml_elements and shape[2] <= 256
-            and all(t.is_cuda and t.is_contiguous() for t in (q, k_cache, v_cache, out, block_table, seq_len, members, share, part_acc, part_ml))):
+            and q.is_cuda and k_cache.is_cuda and v_cache.is_cuda and out.is_cuda and block_table.is_cuda and seq_len.is_cuda and members.is_cuda and share.is_cuda
+            and part_acc.is_cuda and part_ml.is_cuda and q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous() and out.is_contiguous()
+            and block_table.is_contiguous() and seq_len.is_contiguous() and members.is_contiguous() and share.is_contiguous() and part_acc.is_contiguous()
+            and part_ml.is_contiguous()):
         _check_shared(q, k_cache, v_cache, out, block_table, seq_len, members, share, num_kv_heads, page_tokens, plan, part_acc, part_ml)
-    n_seqs, num_heads, head_dim = shape
-    _call("attention_shared", "qt_attention_decode_shared", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q, "q"), _ptr(block_table),
-          block_table.shape[1], _ptr(seq_len), _ptr(members), _ptr(share), n_seqs, plan.groups, plan.most_members, num_heads, num_kv_heads, head_dim,
-          page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, plan.direct_warps, plan.on_tc, _ptr(part_acc), _ptr(part_ml),
-          _ptr(_status_word(q.device)), _stream(), launches=(2 if plan.shared_ranges else 1) if n_seqs else 0)
+    _call("attention_shared", "qt_attention_decode_shared", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _CODES[plan.dtype],
+          block_table.data_ptr(), block_table.shape[1], seq_len.data_ptr(), members.data_ptr(), share.data_ptr(), shape[0], plan.groups, plan.most_members, shape[1],
+          num_kv_heads, shape[2], page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, plan.direct_warps, plan.on_tc, part_acc.data_ptr(),
+          part_ml.data_ptr(), _status_word(q.device).data_ptr(), _stream(), launches=(2 if plan.shared_ranges else 1) if shape[0] else 0)
 
 
 # ----------------------------------------------------------------------------- experts chosen by a table
@@ -1792,7 +1799,8 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
             logits.dtype is temperature.dtype is top_p.dtype is min_p.dtype is uniform.dtype is torch.float32 and top_k.dtype is out.dtype is torch.int32
             and logits.shape[:1] == temperature.shape == top_k.shape == top_p.shape == min_p.shape == uniform.shape == out.shape
             and (logprob is None or (logprob.shape == out.shape and logprob.dtype is torch.float32 and logprob.is_cuda and logprob.is_contiguous()))
-            and all(t.is_cuda and t.is_contiguous() for t in (temperature, top_k, top_p, min_p, uniform, out))):
+            and temperature.is_cuda and top_k.is_cuda and top_p.is_cuda and min_p.is_cuda and uniform.is_cuda and out.is_cuda and temperature.is_contiguous()
+            and top_k.is_contiguous() and top_p.is_contiguous() and min_p.is_contiguous() and uniform.is_contiguous() and out.is_contiguous()):
         _check_filtered(logits, temperature, top_k, top_p, min_p, uniform, out, logprob)
     rows, vocab = logits.shape
     _call("sampling_filtered", "qt_sample_filtered", _ptr(logits), logits.stride(0) if rows > 1 else vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),

@@ -346,7 +346,7 @@ class Attention:
         if (self.window or self.penalised or self.chunk or self.keep_first or self.sink or self.softcap is not None or self.dv != self.d
                 or self.v_heads != self.nkv or cache.ring_tokens or self.scale <= 0 or ctx.n_seqs * 2 > _MAX_SPLIT_PAIRS):
             return None
-        if not kernels.sharing_pays(ctx.n_seqs, shared.most_members, shared.most_shared):
+        if not kernels.sharing_pays(min(shared.most_members, ctx.n_seqs), shared.most_shared, self.nkv, self.d):
             return None
         return kernels.shared_plan(ctx.n_seqs, num_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.d, dtype=self.runtime.dtype, groups=shared.groups,
                                    most_members=min(shared.most_members, ctx.n_seqs), most_shared=shared.most_shared, most_own=shared.most_own,

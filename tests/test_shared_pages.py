@@ -113,7 +113,7 @@ def test_groups_of_sequences_that_share():
 
 
 def test_shapes_are_rounded_up():
-    assert shared_shape([([0, 2, 3], 192), ([1], 0)], [200, 90, 260, 193]) == (2, 4, 1024, 128)
+    assert shared_shape([([0, 2, 3], 192), ([1], 0)], [200, 90, 260, 193]) == (2, 4, 256, 128)
     assert shared_shape([([0, 1], 1024)], [1025, 1030]) == (1, 2, 1024, 64)
     assert shared_shape([([0, 1], 1088)], [1100, 1200]) == (1, 2, 2048, 128)
 
