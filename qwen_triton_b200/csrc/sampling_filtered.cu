@@ -12,19 +12,24 @@
 // T <= 0 takes the lowest id of the largest logit (log-probability 0).  NaN counts as -inf; a row without anything above -inf gives id 0 with
 // log-probability -inf.
 //
-// A row is shared by a cluster of up to eight blocks, each with a part of the ids in shared memory, so that it comes from memory once.  What survives the filters
-// is a small head of the row as a rule, and is found without a look at the rest:
+// A row is shared by a cluster of up to eight blocks.  What survives the filters is a small head of the row as a rule, and is found in one pass over the row:
 //
-//   * the largest logit of every thread goes into 256 bins by its distance below the row's; where the bins' running count reaches top_k (or their
-//     mass p times the row's mass) lies a bound that at least so many tokens reach, and seldom many more;
-//   * the tokens above the bound go to the first block in vocabulary order (min_p gives a bound by itself); that block sorts their keys, finds the thresholds
-//     on the running count and mass, and draws.
+//   * every thread notes the largest logit of each few of its turns.  These go into 256 bins by their distance below the row's largest; where the bins' running
+//     count reaches top_k (or their mass p times the row's mass) lies a bound that at least so many tokens reach, and seldom many more;
+//   * only where a noted logit lies above the bound (min_p gives one by itself) the tokens behind it are read again, and those above the bound go to the first
+//     block in vocabulary order; that block sorts their keys, finds the thresholds on the running count and mass, and draws.
 //
-// Only the row's mass for top_p without top_k takes an exponential a token, an approximate one (its error, 2^-22, is that of a sum in float).  A row whose head
-// does not fit the list finds its thresholds by bins of all of its tokens, each 256 times narrower than the one before, until what is in the bin of the threshold
-// fits the list (three times; what is still alike then is bisected).  Such a row, and one without filters, draws over all blocks.
+// Only the row's mass for top_p without top_k takes an exponential a token, an approximate one, in the same pass.  A row whose head does not fit the list, or whose
+// threshold lies within that mass's error, finds its thresholds by bins of all of its tokens, each 256 times narrower than the one before, until what is in the bin
+// of the threshold fits the list (three times; what is still alike then is bisected).  Such a row, and one without filters, draws over all blocks.  These read the
+// row again for every pass, out of the L2 cache where it is still there.
 //
-// Measured behind a cold cache: one row of 151,936 MEASURED_1, 64 rows MEASURED_64, 256 rows (156 MB) MEASURED_256.
+// The first pass goes at the memory's rate where every row is read at once, by few blocks a row if rows are many; passes with exponentials want many blocks a row.  So rows
+// that need those are then marked and left to a second launch.
+//
+// Measured behind a cold cache: one row of 151,936 14.6 us, 64 rows 37 to 51, 256 rows (156 MB, 24 us of copying) 122 to 136, by what the rows ask for; with every row on
+// eight blocks that kept it in shared memory (37 rows at a time) 14.8, 49 to 78 and 131 to 170.  A row of 256 is read in 30 us; the rest is the head: what it runs is
+// short and serial (bins 5 us, tokens read again 4 to 17, sort and draw 8 to 12), so that its instructions' way into the SM counts, and loops stay loops.
 #include "common.cuh"
 
 #include <math.h>
@@ -38,16 +43,25 @@ constexpr int WARPS = THREADS / 32;
 constexpr int MAX_BLOCKS = 8;
 constexpr int BINS = 256;
 constexpr int LIST = 2048;             // tokens that the first block takes; a block of b hands over LIST / b at most
-constexpr int PER_THREAD = LIST / THREADS;
 constexpr float BINS_PER_NAT = 8.f;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr int TURNS = 5;               // turns whose loads are in flight together in the first pass; a noted logit is the largest of so many, or of a multiple
+constexpr int WAITING = 32 * (TURNS + 1);
+constexpr int FEW = 256;               // keys that are sorted rather than sent through narrower bins
+constexpr int MARK = -1, TAKEN = -2;   // in place of a token: the row is left to the second launch; a cluster of that launch has it
+constexpr int MAX_NOTES = 16;          // noted logits of a thread
+constexpr double LOG2E = 1.4426950408889634;
+// Bound of the relative error of a row's mass from the first pass: 2^-22 of an exponential, half a unit of the difference in it (2^-24 of the distance below the
+// largest, in bits log2(vocabulary) at most on the average that weights give), 2^-24 for each of seven additions and a scaling.
+constexpr double MASS_ERROR = 1. / 524288.;
 typedef unsigned long long u64;
 
 struct Rows {
     const float* logits; long long row_stride;
     const float* temperature; const int* top_k; const float* top_p; const float* min_p; const float* uniform;
     int* token; float* logprob;
-    int vocab, blocks, turns, cached;  // blocks a row; turns of a warp over its ids, 128 a turn; whether they are kept in shared memory
+    int rows, vocab, blocks, turns, span;      // blocks a row; turns of a warp over its ids, 128 a turn; turns a noted logit
+    int cached;                        // whether a block keeps its ids in shared memory for further passes
+    int mark;                          // whether rows that need more passes get MARK for a token
 };
 
 // Floats as unsigned integers of the same order (no NaN comes here); the two zeros share a key.
@@ -58,14 +72,31 @@ __device__ __forceinline__ unsigned int ordered_key(float x) {
 }
 __device__ __forceinline__ float of_key(unsigned int key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
 
+// The number of a key, -inf for that of no number.
+__device__ __forceinline__ float least_of(unsigned int key) { return key == 0 ? -INFINITY : of_key(key); }
 __device__ __forceinline__ float below(float x, float mx) { return x == mx ? 0.f : x - mx; }      // two equal infinities too
-__device__ __forceinline__ float depth_of(float x, float mx, float t) { return below(x, mx) / t; }
-__device__ __forceinline__ float weight_of(float x, float mx, float t) { return expf(below(x, mx) / t); }
-// w in units of 2^-40, rounded to nearest even: two 20-bit steps, each exact in float.
+
+// e^((x - mx) / t) without a branch, so that several can be under way.  The quotient is that of a division, by Markstein's method (a product with the rounded
+// reciprocal, and a correction by the exact remainder): t and the numerator are scaled to t in [1, 2), and what is 200 t below the largest weighs nothing.
+struct Weigh {
+    float mx, scale, t, inverse, lowest;
+    __device__ __forceinline__ Weigh(float mx, float temperature) : mx(mx) {
+        const int exponent = (int)(__float_as_uint(temperature) >> 23) - 127;
+        scale = __uint_as_float((unsigned int)(127 - min(max(exponent, -127), 126)) << 23);
+        t = temperature * scale;
+        inverse = 1.f / t;
+        lowest = -200.f * t;
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float d = fmaxf(below(x, mx) * scale, lowest), q = d * inverse;
+        return expf(fmaf(fmaf(-q, t, d), inverse, q));
+    }
+};
+// w in units of 2^-40, rounded to nearest even: the whole units of 2^-20, then what is left, each by adding a number whose last place is one.
 __device__ __forceinline__ u64 units_of(float w) {
-    const float high = w * 1048576.f;
-    const unsigned int whole = (unsigned int)high;
-    return ((u64)whole << 20) + __float2uint_rn((high - (float)whole) * 1048576.f);
+    const float high = w * 1048576.f, sum = high + 8388608.f;
+    const float low = (high - (sum - 8388608.f)) * 1048576.f + 12582912.f;
+    return ((u64)(__float_as_uint(sum) - 0x4b000000u) << 20) + (long long)(int)(__float_as_uint(low) - 0x4b400000u);
 }
 
 __device__ __forceinline__ u64 warp_total(u64 v) {
@@ -127,23 +158,8 @@ __device__ __noinline__ u64 warps_before(u64 mine, u64* per_warp, int warp, int 
     for (int w = 0; w < WARPS; ++w) { const u64 n = per_warp[w]; if (w < warp) base += n; all += n; }
     return base;
 }
-// Inclusive prefix sums over the block of the numbers i = j THREADS + thread, of which there are n; returns the whole.
-__device__ __forceinline__ u64 block_prefix(u64 (&v)[PER_THREAD], int n, u64* per_warp, int warp, int lane) {
-    u64 base = 0;
-#pragma unroll
-    for (int j = 0; j < PER_THREAD; ++j) {
-        if (j * THREADS >= n) break;
-        const u64 upto = warp_prefix(v[j], lane);
-        u64 all;
-        const u64 before = warps_before(upto, per_warp, warp, lane, all);
-        v[j] = base + before + upto;
-        base += all;
-    }
-    return base;
-}
-
 // n <= LIST keys, largest first (bitonic, the next power of two filled up with zeros).
-__device__ void sort_down(unsigned int* keys, int n) {
+__device__ __noinline__ void sort_down(unsigned int* keys, int n) {
     int size = 32;
     while (size < n) size *= 2;
     for (int i = n + threadIdx.x; i < size; i += THREADS) keys[i] = 0;
@@ -159,20 +175,35 @@ __device__ void sort_down(unsigned int* keys, int n) {
     __syncthreads();
 }
 
-// Of sorted keys of at least floor_key, the last in front of which less than `wanted` lies, what lies above all of them included; the first if there is none.
-__device__ __forceinline__ int last_below(const u64 (&upto)[PER_THREAD], const u64 (&own)[PER_THREAD], const unsigned int* sorted, int n, unsigned int floor_key, u64 above,
-                                          double wanted, u64* per_warp, int warp, int lane) {
+// Of n sorted keys, the last of at least floor_key in front of which less than `wanted` lies (their number or their mass, `above` included; `share` of what all of
+// them have where it is positive); the first if there is none.  Beside it in bit 32, whether a key, or the list's end, begins within `error` of that.
+// One copy of this and of the sort: a block waits for instructions that it runs once.
+__device__ __noinline__ u64 cut(const unsigned int* keys, u64* before, u64* per_warp, int n, bool by_mass, unsigned int floor_key, u64 above, double wanted, double share,
+                                double error, Weigh weigh) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    u64 total = above;
+#pragma unroll 1
+    for (int j = 0; j < n; j += THREADS) {
+        const int i = j + threadIdx.x;
+        const u64 own = i >= n || keys[i] < floor_key ? 0 : by_mass ? units_of(weigh(of_key(keys[i]))) : 1, upto = warp_prefix(own, lane);
+        u64 all;
+        const u64 base = warps_before(upto, per_warp, warp, lane, all);
+        if (i < n) before[i] = total + base + upto - own;
+        total += all;
+    }
+    if (share > 0.) wanted = share * (double)total;
+    bool doubt = fabs((double)total - wanted) <= error;
     int last = 0;
-#pragma unroll
-    for (int j = 0; j < PER_THREAD; ++j) {
-        const int i = j * THREADS + threadIdx.x;
-        if (i < n && sorted[i] >= floor_key && (double)(above + upto[j] - own[j]) < wanted) last = i;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const double lies = (double)before[i];
+        if (keys[i] >= floor_key && lies < wanted) last = i;
+        doubt |= i > 0 && fabs(lies - wanted) <= error;
     }
     last = __reduce_max_sync(0xffffffffu, last);
-    __syncthreads();
+    doubt = __syncthreads_or(doubt);
     if (lane == 0) per_warp[warp] = last;
     __syncthreads();
-    return __reduce_max_sync(0xffffffffu, lane < WARPS ? (int)per_warp[lane] : 0);
+    return (u64)doubt << 32 | keys[__reduce_max_sync(0xffffffffu, lane < WARPS ? (int)per_warp[lane] : 0)];
 }
 
 __device__ __forceinline__ u64 target_of(u64 total, float uniform) {
@@ -185,20 +216,37 @@ __device__ __forceinline__ void give_answer(const Rows& r, int at, int token, fl
     if (r.logprob) r.logprob[at] = depth - logf((float)total * (1.f / 1099511627776.f));
 }
 // Adds a token to its bin of [count, mass low, mass high][BINS].
-__device__ __forceinline__ void add_to_bins(unsigned int (*bins)[BINS], int bin, bool by_mass, u64 m) {
-    atomicAdd(&bins[0][bin], 1u);
+__device__ __forceinline__ void add_to_bins(unsigned int (*bins)[BINS], int bin, bool by_mass, u64 m, bool count = true) {
+    if (count) atomicAdd(&bins[0][bin], 1u);
     if (!by_mass) return;
     const unsigned int low = (unsigned int)m, before = atomicAdd(&bins[1][bin], low);
     const unsigned int high = (unsigned int)(m >> 32) + (before > 0xffffffffu - low ? 1u : 0u);
     if (high) atomicAdd(&bins[2][bin], high);
 }
 
+// Above 1e30 the weights of finite logits are alike; NaN stays.
+__device__ __forceinline__ float temperature_of(const Rows& r, int at) { const float t = r.temperature[at]; return t > 1e30f ? 1e30f : t; }
+
+struct Filters {
+    int k;
+    float p, least;
+    bool by_count, by_mass, by_weight;
+    __device__ __forceinline__ Filters(const Rows& r, int at) : k(r.top_k[at]), p(r.top_p[at]) {
+        const float m = r.min_p[at];
+        least = m > 0.f ? fminf(m, 1.f) : 0.f;
+        by_count = k > 0 && k < r.vocab, by_mass = p < 1.f, by_weight = least > 0.f;
+    }
+};
+
 struct Row {
     const Rows& r;
     Shared& sh;
     const float* row;
-    float4* kept;                                // this block's ids in shared memory
-    unsigned int* keys;                          // the first block's: LIST of them, to be sorted
+    float4* kept;                                // this block's ids, where they are kept
+    float* notes;                                // [note][thread]; null: not wanted
+    unsigned int* waiting;                       // [WAITING] of a warp: quads to be read again, in vocabulary order
+    unsigned int* keys;                          // [LIST], the first block's, to be sorted
+    u64* before;                                 // [LIST], the first block's: what lies before each
     int rank, blocks, warp, lane, shift, quads, turn;
     float mx, t;
 
@@ -220,39 +268,92 @@ struct Row {
         }
         return v;
     }
-    static __device__ __forceinline__ float4 without_nan(float4 v) {
-        v.x = isnan(v.x) ? -INFINITY : v.x; v.y = isnan(v.y) ? -INFINITY : v.y;
-        v.z = isnan(v.z) ? -INFINITY : v.z; v.w = isnan(v.w) ? -INFINITY : v.w;
-        return v;
-    }
+    static __device__ __forceinline__ float without_nan(float x) { return fmaxf(x, -INFINITY); }
+    static __device__ __forceinline__ float4 without_nan(float4 v) { return make_float4(without_nan(v.x), without_nan(v.y), without_nan(v.z), without_nan(v.w)); }
     // quad number q of this block, whichever thread has read it
     __device__ __forceinline__ float4 any_quad(int q) const { return r.cached ? kept[q] : without_nan(load_quad(rank * WARPS * r.turns * 32 + q)); }
-    __device__ __forceinline__ float4 quad(int i) const { return r.cached ? kept[(warp * r.turns + i) * 32 + lane] : without_nan(load(i)); }
-    // The loop stays a loop: with an exponential and a division for every number, a pass that is unrolled is tens of kilobytes of instructions that run once or
-    // twice, and a block waits for those.
-    template <typename F> __device__ __forceinline__ void each_turn(F f) const {
-#pragma unroll 1
-        for (int i = 0; i < r.turns; ++i) f(i, quad(i));
-    }
+    struct Four { float x[4]; };
+    // Another pass over this thread's logits.  The loop stays a loop: with an exponential and a division for every number, a pass that is unrolled is tens of
+    // kilobytes of instructions that run once or twice, and a block waits for those.
     template <typename F> __device__ __forceinline__ void each(F f) const {
-        each_turn([&](int, float4 v) { f(v.x); f(v.y); f(v.z); f(v.w); });
+#pragma unroll 1
+        for (int i = 0; i < r.turns; ++i) {
+            const float4 v = any_quad((warp * r.turns + i) * 32 + lane);
+            f({v.x, v.y, v.z, v.w});
+        }
     }
 
-    // the first read of the row: five turns' loads in flight, kept where they fit; this thread's largest
-    __device__ __forceinline__ float fetch() const {
+    // The first pass: notes the largest logit of each `span` turns and returns this thread's.  With SUM, sum becomes the mass of this thread's logits in units of
+    // that of its largest: one exponential a token against the largest so far, and the sum scaled where that grows.
+    template <bool SUM> __device__ __forceinline__ float fetch(double& sum) const {
         float best = -INFINITY;
-        for (int i0 = 0; i0 < r.turns; i0 += 5) {
-            float4 v[5];
+        sum = 0.;
+        const float per_nat = (float)(LOG2E / t), rest = (float)(LOG2E / t - per_nat), lowest = -200.f * t;       // e^-200: nothing
+        for (int note = 0, i0 = 0; i0 < r.turns; ++note) {
+            float top = -INFINITY;
+            for (const int end = min(i0 + r.span, r.turns); i0 < end; i0 += TURNS) {
+                float4 v[TURNS];
 #pragma unroll
-            for (int j = 0; j < 5; ++j) v[j] = i0 + j < r.turns ? load(i0 + j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                for (int j = 0; j < TURNS; ++j) v[j] = i0 + j < end ? load(i0 + j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                float most = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 5; ++j) {
-                const float4 c = without_nan(v[j]);
-                best = fmaxf(best, fmaxf(fmaxf(c.x, c.y), fmaxf(c.z, c.w)));
-                if (r.cached && i0 + j < r.turns) kept[(warp * r.turns + i0 + j) * 32 + lane] = c;
+                for (int j = 0; j < TURNS; ++j) most = fmaxf(most, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+                top = fmaxf(top, most);
+                if (r.cached) {
+#pragma unroll
+                    for (int j = 0; j < TURNS; ++j) if (i0 + j < end) kept[(warp * r.turns + i0 + j) * 32 + lane] = without_nan(v[j]);
+                }
+                if (SUM) {
+                    if (most > best) { sum = best > -INFINITY ? sum * expf((best - most) / t) : 0.; best = most; }
+                    if (best > -INFINITY) {
+                        auto of = [&](float x) {
+                            const float d = fmaxf(x - best, lowest);          // NaN too
+                            float e;
+                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, per_nat, d * rest)));
+                            return e;
+                        };
+                        float part = 0.f;
+#pragma unroll
+                        for (int j = 0; j < TURNS; ++j) part += (of(v[j].x) + of(v[j].y)) + (of(v[j].z) + of(v[j].w));
+                        sum += part;
+                    }
+                }
             }
+            best = fmaxf(best, top);
+            if (notes) notes[note * THREADS + threadIdx.x] = top;
         }
         return best;
+    }
+    // Calls f(quad of the block, logits) for the quads behind this warp's notes that `hit` takes, in vocabulary order, up to 32 of them in a call (lanes
+    // without one: logits of -inf); ends where f returns false.
+    template <typename H, typename F> __device__ __forceinline__ void again(H hit, F f) const {
+        int have = 0;
+        auto take = [&](int from, int n) {
+            const int q = lane < n ? (int)waiting[from + lane] : 0;
+            return f(q, lane < n ? any_quad(q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY));
+        };
+        for (int note = 0; note * r.span < r.turns; ++note) {
+            const unsigned int lanes = __ballot_sync(0xffffffffu, hit(notes[note * THREADS + threadIdx.x]));
+            if (lanes == 0) continue;
+            const int all = __popc(lanes), end = min((note + 1) * r.span, r.turns);
+            const bool mine = lanes >> lane & 1;
+            for (int i = note * r.span; i < end; i += TURNS) {
+                int to = have + __popc(lanes & ((1u << lane) - 1));
+#pragma unroll
+                for (int j = 0; j < TURNS; ++j, to += all) if (mine && i + j < end) waiting[to] = (unsigned int)(warp * r.turns + i + j) * 32 + lane;
+                have += all * min(TURNS, end - i);
+                __syncwarp();
+                int from = 0;
+                for (; have - from >= 32; from += 32) if (!take(from, 32)) return;
+                if (from == 0) continue;
+                const unsigned int rest = from + lane < have ? waiting[from + lane] : 0;
+                __syncwarp();
+                have -= from;
+                if (lane < have) waiting[lane] = rest;
+                __syncwarp();
+            }
+        }
+        if (have > 0) take(0, have);
     }
 
     __device__ __forceinline__ void barrier() const { if (blocks > 1) cluster_barrier(); else __syncthreads(); }
@@ -295,8 +396,8 @@ struct Row {
         }
     }
 
-    __device__ __forceinline__ float depth(float x) const { return depth_of(x, mx, t); }
-    __device__ __forceinline__ u64 mass(float x) const { return units_of(weight_of(x, mx, t)); }
+    __device__ __forceinline__ float depth(float x) const { return below(x, mx) / t; }
+    __device__ __forceinline__ Weigh weigh() const { return Weigh(mx, t); }
 
     __device__ __forceinline__ void clear_bins(int at) const {
         for (int i = threadIdx.x; i < 3 * BINS; i += THREADS) (&sh.bins[at][0][0])[i] = 0;
@@ -343,8 +444,10 @@ struct Row {
     // `share` is wanted where it is positive.
     __device__ unsigned int threshold(bool by_mass, double wanted, double share, unsigned int floor_key) {
         u64 above = 0;
-        int prefix = 0, level = 0;
+        int prefix = 0, level = 0, tokens = 0;
         float scale = BINS_PER_NAT / t;
+        const float floor_x = least_of(floor_key);
+        const Weigh weight = weigh();
         auto index_of = [&](float x) {
             const float at = -below(x, mx) * scale;
             const int index = at < 1073741824.f ? (int)at : 1073741824;
@@ -353,48 +456,50 @@ struct Row {
         for (;; ++level, scale *= 256.f) {                    // a power of two: a place is that of the level before and eight bits more
             clear_bins(level & 1);
             __syncthreads();
-            each([&](float x) {
-                if (ordered_key(x) < floor_key) return;
-                const int index = index_of(x);
-                if (level == 0 || index >> 8 == prefix) add_to_bins(sh.bins[level & 1], index & (BINS - 1), by_mass, by_mass ? mass(x) : 0);
+            each([&](const Four& v) {
+                int index[4];
+                bool in[4];
+                u64 m[4] = {};
+                for (int e = 0; e < 4; ++e) {
+                    index[e] = index_of(v.x[e]);
+                    in[e] = v.x[e] >= floor_x && (level == 0 || index[e] >> 8 == prefix);
+                }
+                if (by_mass && __any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3]))
+                    for (int e = 0; e < 4; ++e) m[e] = units_of(weight(v.x[e]));
+                for (int e = 0; e < 4; ++e) if (in[e]) add_to_bins(sh.bins[level & 1], index[e] & (BINS - 1), by_mass, m[e], !by_mass || level > 0);
             });
             barrier();
             const int bin = find_bin(level & 1, by_mass, wanted, level == 0 ? share : 0., above);
             if (bin == BINS) { barrier(); return floor_key; } // all of them are less than is wanted
             prefix = (prefix << 8) + bin;
             // the last bin of the first level has no lower end
-            if (sh.bin_tokens <= LIST || level == 2 || (level == 0 && bin == BINS - 1) || !(scale * 65536.f < INFINITY)) break;
+            tokens = by_mass && level == 0 ? LIST + 1 : (int)sh.bin_tokens;        // masses alone at first: no row comes here for a few tokens
+            if (tokens <= FEW || level == 2 || (level == 0 && bin == BINS - 1) || !(scale * 65536.f < INFINITY)) break;
         }
-        auto inside = [&](float x) { return ordered_key(x) >= floor_key && index_of(x) == prefix; };
+        auto inside = [&](float x) { return x >= floor_x && index_of(x) == prefix; };
         unsigned int found;
-        if (sh.bin_tokens <= LIST) {                          // the bin's keys to the first block, in any order: they are sorted there
+        if (tokens <= LIST) {                                 // the bin's keys to the first block, in any order: they are sorted there
             if (threadIdx.x == 0) sh.taken = 0;
-            const int tokens = sh.bin_tokens;
             barrier();
-            each([&](float x) { if (inside(x)) remote_store(keys + remote_add(&sh.taken, 0), 0, ordered_key(x)); });
+            each([&](const Four& v) { for (int e = 0; e < 4; ++e) if (inside(v.x[e])) remote_store(keys + remote_add(&sh.taken, 0), 0, ordered_key(v.x[e])); });
             barrier();
             found = 0;
             if (rank == 0) {
                 sort_down(keys, tokens);
-                u64 upto[PER_THREAD], own[PER_THREAD];
-#pragma unroll
-                for (int j = 0; j < PER_THREAD; ++j) {
-                    const int i = j * THREADS + threadIdx.x;
-                    upto[j] = own[j] = i >= tokens ? 0 : by_mass ? mass(of_key(keys[i])) : 1;
-                }
-                block_prefix(upto, tokens, sh.per_warp, warp, lane);
-                found = keys[last_below(upto, own, keys, tokens, 0u, above, wanted, sh.per_warp, warp, lane)];
+                found = (unsigned int)cut(keys, before, sh.per_warp, tokens, by_mass, 0u, above, wanted, 0., 0., weigh());
             }
             const int slot = exchange(found, 0);
             found = (unsigned int)sh.slots[slot][0][0];
         } else {
             unsigned int low = 0xffffffffu, high = 0;
-            each([&](float x) { if (inside(x)) { low = min(low, ordered_key(x)); high = max(high, ordered_key(x)); } });
+            each([&](const Four& v) {
+                for (int e = 0; e < 4; ++e) if (inside(v.x[e])) { low = min(low, ordered_key(v.x[e])); high = max(high, ordered_key(v.x[e])); }
+            });
             row_ends(low, high);
             while (low < high) {
                 const unsigned int mid = low + (high - low) / 2;
                 u64 n = 0;
-                each([&](float x) { if (ordered_key(x) > mid && inside(x)) n += by_mass ? mass(x) : 1; });
+                each([&](const Four& v) { for (int e = 0; e < 4; ++e) if (ordered_key(v.x[e]) > mid && inside(v.x[e])) n += by_mass ? units_of(weight(v.x[e])) : 1; });
                 if ((double)(above + row_total(n)) < wanted) high = mid; else low = mid + 1;
             }
             found = low;
@@ -403,15 +508,32 @@ struct Row {
         return max(found, floor_key);
     }
 
+    // The answer of a row without a number above -inf.
+    __device__ __forceinline__ void give_nothing(int at) const {
+        if (rank != 0 || threadIdx.x != 0) return;
+        r.token[at] = 0;
+        if (r.logprob) r.logprob[at] = -INFINITY;
+    }
+    // Thresholds and token by passes over the whole row.
+    __device__ __forceinline__ void by_passes(int at, const Filters& f) {
+        unsigned int floor_key = 0;
+        if (f.by_count) floor_key = threshold(false, (double)f.k, 0., 0u);
+        if (f.by_mass) floor_key = f.p > 0.f ? threshold(true, 0., (double)f.p, floor_key) : ordered_key(mx);
+        draw(at, floor_key, f.least);
+        barrier();
+    }
+
     // Draws among the tokens with a key of at least floor_key and a weight of at least `least`, over all blocks.
     __device__ void draw(int at, unsigned int floor_key, float least) {
+        const float floor_x = least_of(floor_key);
+        const Weigh weight = weigh();
         auto stays = [&](float x) -> u64 {
-            if (ordered_key(x) < floor_key) return 0;
-            const float w = weight_of(x, mx, t);
-            return w < least ? 0 : units_of(w);
+            const float w = weight(x);
+            const u64 m = units_of(w);
+            return x >= floor_x && w >= least ? m : 0;
         };
         u64 mine = 0;
-        each([&](float x) { mine += stays(x); });
+        each([&](const Four& v) { mine += (stays(v.x[0]) + stays(v.x[1])) + (stays(v.x[2]) + stays(v.x[3])); });
         mine = warp_total(mine);
         __syncthreads();
         if (lane == 0) sh.per_warp[warp] = mine;
@@ -439,85 +561,102 @@ struct Row {
             if (sum <= target && target < sum + own) {
                 int e = 0;
                 while (e < 3 && sum + m[e] <= target) sum += m[e++];
-                give_answer(r, at, id + e, depth_of(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w, mx, t), total);
+                give_answer(r, at, id + e, depth(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w), total);
             }
             running += all;
         }
     }
 };
 
+// Shared memory of the first launch in front of what is kept: list and found, what waits, and the larger of places with notes and keys with what lies before them.
+__host__ __device__ __forceinline__ size_t head_bytes(const Rows& r) {
+    const size_t noting = LIST * sizeof(unsigned short) + (size_t)((r.turns + r.span - 1) / r.span) * THREADS * sizeof(float);
+    const size_t sorting = LIST * (sizeof(unsigned int) + sizeof(u64));
+    return 2 * LIST * sizeof(u64) + WARPS * WAITING * sizeof(unsigned int) + (noting > sorting ? noting : sorting);
+}
+
 __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows r) {
     pdl_launch_dependents();
     if (r.blocks > 1) cluster_arrive_started();
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Shared sh;
-    // the first block's: tokens above the bound as (key, id), by block and in vocabulary order; behind them the blocks' parts of the row, where the keys are sorted later
-    u64* list = reinterpret_cast<u64*>(smem);
-    float4* kept = reinterpret_cast<float4*>(smem + LIST * sizeof(u64));
+    u64* list = reinterpret_cast<u64*>(smem);                  // the first block's: tokens above the bound as (key, id), by block and in vocabulary order
+    u64* found = list + LIST;                                  // this block's, as its warps find them, and their places among their warp's
+    unsigned int* waiting = reinterpret_cast<unsigned int*>(found + LIST);
+    unsigned short* place = reinterpret_cast<unsigned short*>(waiting + WARPS * WAITING);
+    float* notes = reinterpret_cast<float*>(place + LIST);
+    unsigned int* keys = reinterpret_cast<unsigned int*>(waiting + WARPS * WAITING);       // later, where places and notes were
+    u64* before = reinterpret_cast<u64*>(keys + LIST);
+    float4* kept = reinterpret_cast<float4*>(smem + head_bytes(r));
     const int blocks = r.blocks, rank = blockIdx.x % blocks, at = blockIdx.x / blocks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     const float* row = r.logits + at * r.row_stride;
     const int shift = (int)(((uintptr_t)row >> 2) & 3);
-    Row w{r, sh, row, kept, reinterpret_cast<unsigned int*>(list), rank, blocks, warp, lane, shift, (r.vocab + shift + 3) / 4, 0, -INFINITY, r.temperature[at]};
+    Row w{r, sh, row, kept, notes, waiting + warp * WAITING, keys, before, rank, blocks, warp, lane, shift, (r.vocab + shift + 3) / 4, 0, -INFINITY, temperature_of(r, at)};
     w.clear_bins(0);
-    const float own_best = w.fetch();
+    const float t = w.t;
+    const Filters f(r, at);
+    const bool filtered = f.by_count || f.by_mass || f.by_weight;
+    if (r.mark && !filtered && t > 0.f) {                      // the same for all blocks of the row
+        if (rank == 0 && threadIdx.x == 0) r.token[at] = MARK;
+        if (blocks > 1) cluster_wait_started();
+        return;
+    }
+    const bool whole = blocks == 1 && r.vocab <= LIST;         // the list takes the row as it is
+    const bool counting = f.by_count, summing = f.by_mass && !f.by_count && !whole && t > 0.f;
+    if (threadIdx.x == 0) sh.taken = 0;
+    double sum;
+    const float own_best = summing ? w.fetch<true>(sum) : w.fetch<false>(sum);
     if (blocks > 1) cluster_wait_started();
     {
         unsigned int low = 0, high = ordered_key(own_best);
         w.row_ends(low, high);
         w.mx = of_key(high);
     }
-    const float mx = w.mx, t = w.t;
+    const float mx = w.mx;
     if (!(t > 0.f) || mx == -INFINITY) {                       // the lowest id of the largest logit
         unsigned int first = 0xffffffffu, unused = 0;
-        for (int i = 0; i < r.turns; ++i) {
-            const float4 v = w.quad(i);
-            const unsigned int id = 4 * w.quad_at(i) - shift;
-            if (first == 0xffffffffu) first = v.x == mx ? id : v.y == mx ? id + 1 : v.z == mx ? id + 2 : v.w == mx ? id + 3 : first;
-        }
+        if (mx > -INFINITY)
+            w.again([&](float x) { return x == mx; }, [&](int q, float4 v) {
+                const unsigned int id = 4 * (rank * WARPS * r.turns * 32 + q) - shift;
+                first = v.x == mx ? id : v.y == mx ? id + 1 : v.z == mx ? id + 2 : v.w == mx ? id + 3 : first;
+                return !__any_sync(0xffffffffu, first != 0xffffffffu);
+            });
         w.row_ends(first, unused);
-        if (rank == 0 && threadIdx.x == 0) {
-            r.token[at] = mx == -INFINITY ? 0 : (int)first;
-            if (r.logprob) r.logprob[at] = mx == -INFINITY ? -INFINITY : 0.f;
+        if (mx == -INFINITY) {
+            w.give_nothing(at);
+        } else if (rank == 0 && threadIdx.x == 0) {
+            r.token[at] = (int)first;
+            if (r.logprob) r.logprob[at] = 0.f;
         }
         w.barrier();
         return;
     }
-    const int k = r.top_k[at];
-    const float p = r.top_p[at], m = r.min_p[at], least = m > 0.f ? fminf(m, 1.f) : 0.f;
-    const bool by_count = k > 0 && k < r.vocab, by_mass = p < 1.f, by_weight = least > 0.f;
-    if (!by_count && !by_mass && !by_weight) {
-        w.draw(at, 0u, 0.f);
-        w.barrier();
-        return;
-    }
-    const float per_nat = LOG2E / t;
-    const bool whole = blocks == 1 && r.vocab <= LIST;         // the list takes the row as it is
-    bool fits = mx < INFINITY && per_nat < INFINITY && t < 1e30f;
+    bool fits = filtered && mx < INFINITY && t > 1e-30f;
     float bound = -INFINITY;
     double row_mass = 0.;                                      // for top_p alone, in units
     if (fits && !whole) {
-        if (by_weight && !by_count) bound = mx + t * logf(least);
-        if (by_count || by_mass) {
-            const bool counting = by_count;
-            if (own_best > -INFINITY) add_to_bins(sh.bins[0], min((int)(-w.depth(own_best) * BINS_PER_NAT), BINS - 1), !counting, counting ? 0 : w.mass(own_best));
-            float sum = 0.f;
-            if (!counting) {
-                w.each([&](float x) {
-                    float e;
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x - mx) * per_nat));
-                    sum += e;
-                });
-                sum = warp_sum(sum);
-                if (lane == 0) sh.scratch[warp][1] = __float_as_uint(sum);
-                __syncthreads();
-                sum = warp_sum(lane < WARPS ? __uint_as_float((unsigned int)sh.scratch[lane][1]) : 0.f);
+        if (f.by_weight && !f.by_count) bound = mx + t * logf(f.least);
+        if (f.by_count || f.by_mass) {
+            const Weigh weight = w.weigh();
+            for (int note = 0; note * r.span < r.turns; ++note) {
+                const float x = notes[note * THREADS + threadIdx.x];
+                if (x > -INFINITY) add_to_bins(sh.bins[0], min((int)(-w.depth(x) * BINS_PER_NAT), BINS - 1), !counting, counting ? 0 : units_of(weight(x)));
             }
-            const int slot = w.exchange(__float_as_uint(sum), 0);
-            for (int b = 0; b < blocks; ++b) row_mass += (double)__uint_as_float((unsigned int)sh.slots[slot][b][0]);
+            if (summing) {
+                sum = own_best > -INFINITY ? sum * weight(own_best) : 0.;
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                if (lane == 0) sh.scratch[warp][1] = (u64)__double_as_longlong(sum);
+                __syncthreads();
+                sum = 0.;
+                for (int i = 0; i < WARPS; ++i) sum += __longlong_as_double((long long)sh.scratch[i][1]);
+            }
+            const int slot = w.exchange((u64)__double_as_longlong(sum), 0);
+            for (int b = 0; b < blocks; ++b) row_mass += __longlong_as_double((long long)sh.slots[slot][b][0]);
             row_mass *= 1099511627776.;
             u64 above = 0;
-            double wanted = counting ? (double)k : (double)p * row_mass;
+            double wanted = counting ? (double)f.k : (double)f.p * row_mass;
             const int bin = w.find_bin(0, !counting, wanted, 0., above);
             // every token of the bins up to this one lies above the bound; the last bin has no end
             if (bin < BINS - 1) bound = fmaxf(bound, mx - t * (float)(bin + 1) * (1.f / BINS_PER_NAT));
@@ -526,93 +665,153 @@ __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows 
     }
     if (fits) {
         auto above = [&](float x) { return x > -INFINITY && !(x < bound); };
-        int n = 0;
-        w.each([&](float x) { n += above(x); });
-        n = __reduce_add_sync(0xffffffffu, n);
-        __syncthreads();
-        if (lane == 0) sh.per_warp[warp] = n;
-        __syncthreads();
-        int from = 0, mine = 0;
-        for (int i = 0; i < WARPS; ++i) { if (i < warp) from += (int)sh.per_warp[i]; mine += (int)sh.per_warp[i]; }
-        const int room = LIST / blocks;
-        if (mine <= room && n > 0) {
-            w.each_turn([&](int i, float4 v) {
-                const bool hit[4] = {above(v.x), above(v.y), above(v.z), above(v.w)};
-                const int own = hit[0] + hit[1] + hit[2] + hit[3];
-                if (!__any_sync(0xffffffffu, own)) return;
-                const int upto = (int)warp_prefix(own, lane);
-                int slot = rank * room + from + upto - own;
-                const float x[4] = {v.x, v.y, v.z, v.w};
+        // a long list takes one block longer than the second launch does
+        const int room = (r.mark ? LIST / 2 : LIST) / blocks;
+        int in_warp = 0;
+        w.again(above, [&](int q, float4 v) {
+            const int own = above(v.x) + above(v.y) + above(v.z) + above(v.w);
+            int upto = own;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (hit[e]) {
-                        const u64 entry = ((u64)ordered_key(x[e]) << 32) | (unsigned int)(4 * w.quad_at(i) - shift + e);
-                        if (blocks > 1) remote_store(list + slot, 0, entry); else list[slot] = entry;
-                        ++slot;
-                    }
-                from += __shfl_sync(0xffffffffu, upto, 31);
-            });
-        }
+            for (int off = 1; off < 32; off <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, upto, off);
+                if (lane >= off) upto += other;
+            }
+            const int all = __shfl_sync(0xffffffffu, upto, 31);
+            int slot = 0;
+            if (lane == 0) slot = (int)atomicAdd(&sh.taken, (unsigned int)all);
+            slot = __shfl_sync(0xffffffffu, slot, 0);
+            if (slot + all > room) return false;               // the list has no room for this row: sh.taken says so
+            slot += upto - own;
+            int of_warp = in_warp + upto - own;
+            in_warp += all;
+            auto put = [&](float x, int e) {
+                if (!above(x)) return;
+                found[slot] = ((u64)ordered_key(x) << 32) | (unsigned int)(4 * (rank * WARPS * r.turns * 32 + q) - shift + e);
+                place[slot++] = (unsigned short)of_warp++;
+            };
+            put(v.x, 0); put(v.y, 1); put(v.z, 2); put(v.w, 3);
+            return true;
+        });
+        __syncthreads();
+        if (lane == 0) sh.per_warp[warp] = in_warp;
+        __syncthreads();
+        const int mine = (int)sh.taken;
+        if (mine <= room)
+            for (int i = threadIdx.x; i < mine; i += THREADS) {
+                const int of = (((int)(unsigned int)found[i] + shift) / 4) / (r.turns * 32) - rank * WARPS;
+                int to = rank * room + place[i];
+                for (int b = 0; b < of; ++b) to += (int)sh.per_warp[b];
+                if (blocks > 1) remote_store(list + to, 0, found[i]); else list[to] = found[i];
+            }
         const int slot = w.exchange(mine, 0);
         for (int b = 0; b < blocks; ++b) fits = fits && (int)sh.slots[slot][b][0] <= room;
-        if (fits) {
-            if (rank > 0) return;
+        if (fits && rank > 0) {
+            if (!summing || sh.slots[w.exchange(0, 0)][0][0]) return;
+        } else if (fits) {
             // the first block alone: places j THREADS + thread of the list a thread
             int count = 0;
             for (int b = 0; b < blocks; ++b) count += (int)sh.slots[slot][b][0];
-            u64 entry[PER_THREAD] = {};
-            unsigned int* keys = reinterpret_cast<unsigned int*>(kept);
-#pragma unroll
-            for (int j = 0; j < PER_THREAD; ++j) {
-                int i = j * THREADS + threadIdx.x, b = 0;
-                if (i >= count) break;
-                const int to = i;
+#pragma unroll 1
+            for (int to = threadIdx.x; to < count; to += THREADS) {
+                int i = to, b = 0;
                 while (i >= (int)sh.slots[slot][b][0]) i -= (int)sh.slots[slot][b++][0];
-                entry[j] = list[b * room + i];
-                keys[to] = (unsigned int)(entry[j] >> 32);
+                const u64 entry = list[b * room + i];
+                found[to] = entry;                             // what was there is in the list
+                keys[to] = (unsigned int)(entry >> 32);
             }
             unsigned int floor_key = 0;
-            if (by_count || by_mass) {
-                sort_down(keys, count);
-                if (by_count && k <= count) floor_key = keys[k - 1];
-                if (by_mass) {
-                    u64 upto[PER_THREAD], own[PER_THREAD];
-#pragma unroll
-                    for (int j = 0; j < PER_THREAD; ++j) {
-                        const int i = j * THREADS + threadIdx.x;
-                        upto[j] = own[j] = i < count && keys[i] >= floor_key ? w.mass(of_key(keys[i])) : 0;
+            if (f.by_count || f.by_mass) sort_down(keys, count);
+            if (f.by_count && f.k <= count) floor_key = keys[f.k - 1];
+            if (f.by_mass) {
+                // the likeliest token stays whatever p is
+                const double wanted = (double)f.p * row_mass;
+                const u64 last = f.p > 0.f ? cut(keys, before, sh.per_warp, count, true, floor_key, 0, wanted, summing ? 0. : (double)f.p, wanted * MASS_ERROR, w.weigh()) : keys[0];
+                floor_key = max(floor_key, (unsigned int)last);
+                if (summing) {
+                    fits = last >> 32 == 0;
+                    w.exchange(fits, 0);
+                }
+            }
+            if (fits) {
+                u64 total = 0;
+                const Weigh weigh = w.weigh();
+#pragma unroll 1
+                for (int j = 0; j < count; j += THREADS) {
+                    const int i = j + threadIdx.x;
+                    u64 own = 0, all;
+                    if (i < count && (unsigned int)(found[i] >> 32) >= floor_key) {
+                        const float weight = weigh(of_key((unsigned int)(found[i] >> 32)));
+                        own = weight < f.least ? 0 : units_of(weight);
                     }
-                    const u64 in_list = block_prefix(upto, count, sh.per_warp, warp, lane);
-                    const double wanted = (double)p * (by_count || whole ? (double)in_list : row_mass);
-                    // the likeliest token stays whatever p is
-                    floor_key = max(floor_key, keys[last_below(upto, own, keys, count, floor_key, 0, wanted, sh.per_warp, warp, lane)]);
+                    const u64 upto = warp_prefix(own, lane), base = warps_before(upto, sh.per_warp, warp, lane, all);
+                    if (i < count) before[i] = total + base + upto - own;
+                    total += all;
                 }
+                __syncthreads();
+                const u64 target = target_of(total, r.uniform[at]);
+#pragma unroll 1
+                for (int i = threadIdx.x; i < count; i += THREADS)
+                    if (before[i] <= target && target < (i + 1 < count ? before[i + 1] : total))
+                        give_answer(r, at, (int)(unsigned int)found[i], w.depth(of_key((unsigned int)(found[i] >> 32))), total);
+                return;
             }
-            u64 upto[PER_THREAD], own[PER_THREAD];
-#pragma unroll
-            for (int j = 0; j < PER_THREAD; ++j) {
-                const unsigned int key = (unsigned int)(entry[j] >> 32);
-                own[j] = 0;
-                if (j * THREADS + threadIdx.x < count && key >= floor_key) {
-                    const float weight = expf(w.depth(of_key(key)));
-                    own[j] = weight < least ? 0 : units_of(weight);
-                }
-                upto[j] = own[j];
-            }
-            const u64 total = block_prefix(upto, count, sh.per_warp, warp, lane);
-            const u64 target = target_of(total, r.uniform[at]);
-#pragma unroll
-            for (int j = 0; j < PER_THREAD; ++j)
-                if (own[j] > 0 && upto[j] > target && upto[j] - own[j] <= target)
-                    give_answer(r, at, (int)(unsigned int)entry[j], w.depth(of_key((unsigned int)(entry[j] >> 32))), total);
-            return;
         }
     }
-    unsigned int floor_key = 0;
-    if (by_count) floor_key = w.threshold(false, (double)k, 0., 0u);
-    if (by_mass) floor_key = p > 0.f ? w.threshold(true, 0., (double)p, floor_key) : ordered_key(mx);
-    w.draw(at, floor_key, least);
-    w.barrier();
+    if (r.mark) {
+        if (rank == 0 && threadIdx.x == 0) r.token[at] = MARK;
+        return;
+    }
+    w.by_passes(at, f);
+}
+
+// The rows that the launch before has marked, each by the cluster that comes to it first.
+__global__ void __launch_bounds__(THREADS, 2) sample_marked_kernel(const Rows r) {
+    pdl_launch_dependents();
+    if (r.blocks > 1) cluster_arrive_started();
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ Shared sh;
+    const int blocks = r.blocks, rank = blockIdx.x % blocks, cluster = blockIdx.x / blocks, clusters = gridDim.x / blocks, warp = threadIdx.x >> 5,
+              lane = threadIdx.x & 31;
+    if (blocks > 1) cluster_wait_started();
+    pdl_wait();
+    unsigned int* keys = reinterpret_cast<unsigned int*>(smem);
+    u64* before = reinterpret_cast<u64*>(keys + LIST);
+    float4* kept = reinterpret_cast<float4*>(before + LIST);
+    const int start = (int)((long long)r.rows * cluster / clusters);
+    int seen = 0;                                              // rows from start on that are known to be no longer there to take
+    for (;;) {
+        Row w{r, sh, nullptr, kept, nullptr, nullptr, keys, before, rank, blocks, warp, lane, 0, 0, 0, -INFINITY, 1.f};
+        int taken = -1;
+        if (rank == 0 && warp == 0)
+            while (taken < 0 && seen < r.rows) {
+                const int i = seen + lane, at = i < r.rows - start ? start + i : start + i - r.rows;
+                unsigned int marked = __ballot_sync(0xffffffffu, i < r.rows && *(volatile int*)(r.token + at) == MARK);
+                while (taken < 0 && marked) {
+                    const int first = __ffs(marked) - 1;
+                    marked &= marked - 1;
+                    int was = 0;
+                    if (lane == first) was = atomicCAS(r.token + at, MARK, TAKEN);
+                    if (__shfl_sync(0xffffffffu, was, first) == MARK) taken = __shfl_sync(0xffffffffu, at, first);
+                }
+                if (taken < 0) seen += 32;
+            }
+        // from the first warp of the first block to all
+        if (rank == 0) {
+            if (threadIdx.x == 0) sh.above = (u64)(unsigned int)taken;
+            __syncthreads();
+        }
+        const int at = (int)(unsigned int)sh.slots[w.exchange(rank == 0 ? sh.above : 0, 0)][0][0];
+        if (at < 0) break;
+        w.row = r.logits + at * r.row_stride;
+        w.shift = (int)(((uintptr_t)w.row >> 2) & 3);
+        w.quads = (r.vocab + w.shift + 3) / 4;
+        w.t = temperature_of(r, at);
+        double unused;
+        unsigned int low = 0, high = ordered_key(w.fetch<false>(unused));
+        w.row_ends(low, high);
+        w.mx = of_key(high);
+        if (w.mx == -INFINITY) { w.give_nothing(at); w.barrier(); } else { w.by_passes(at, Filters(r, at)); }
+    }
 }
 
 }  // namespace
@@ -625,19 +824,39 @@ extern "C" int qt_sample_filtered(const float* logits, long long row_stride, con
                rows, vocab, row_stride);
     if (rows == 0) return QT_OK;
     QT_REQUIRE(rows <= 0x7fffffff / MAX_BLOCKS, "sample_filtered: %d rows are more than one launch takes", rows);
-    // so many blocks a row that two of them fit an SM, and more where rows are few, down to 4,096 ids a block
-    int blocks = 1;
-    while (blocks < MAX_BLOCKS && (vocab / blocks > 20480 || (vocab / blocks > 8192 && (long long)rows * blocks < sm_count()))) blocks *= 2;
-    const int quads = (vocab + 3 + 3) / 4, turns = (quads + blocks * THREADS - 1) / (blocks * THREADS);
-    size_t part = (size_t)turns * THREADS * sizeof(float4);
-    const int cached = part <= 200 * 1024;                     // a longer part is read again
-    if (!cached) part = 0;
-    if (part < LIST * sizeof(unsigned int)) part = LIST * sizeof(unsigned int);
-    const size_t smem = LIST * sizeof(u64) + part;
-    const cudaError_t raised = raise_shared<sample_filtered_kernel>((int)smem);
+    // down to 4,096 ids a block, and as many blocks a row as are resident at a time with two an SM
+    const int resident = 2 * sm_count();
+    int most = 1;
+    while (most < MAX_BLOCKS && vocab / most > 8192) most *= 2;
+    int blocks = most;
+    while (blocks > 1 && (long long)rows * blocks > resident) blocks /= 2;
+    auto rows_of = [&](int blocks) {
+        const int quads = (vocab + 3 + 3) / 4, turns = (quads + blocks * THREADS - 1) / (blocks * THREADS);
+        const int span = TURNS * ((turns + TURNS * MAX_NOTES - 1) / (TURNS * MAX_NOTES));
+        return Rows{logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, rows, vocab, blocks, turns, span, 0, 0};
+    };
+    auto part_of = [&](const Rows& r) { return (size_t)r.turns * THREADS * sizeof(float4); };
+    constexpr size_t ONE = 219 * 1024, TWO = 106 * 1024;        // of an SM's shared memory for one block and for each of two, the static part taken off
+    Rows r = rows_of(blocks);
+    // 64 rows by four blocks each take 37 to 51 us where the rows that need more passes stay with them and 40 to 91 where these are left to the second launch; 256 rows
+    // by one block each take 122 to 136 with it and 244 without
+    r.mark = blocks < most && blocks < 4;
+    size_t smem = head_bytes(r);
+    r.cached = !r.mark && smem + part_of(r) <= ((long long)rows * blocks > sm_count() ? TWO : ONE);
+    if (r.cached) smem += part_of(r);
+    cudaError_t raised = raise_shared<sample_filtered_kernel>((int)smem);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "sample_filtered: cannot raise shared memory: %s", cudaGetErrorString(raised));
-    const Rows r{logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, vocab, blocks, turns, cached};
     launch_kernel_cluster(sample_filtered_kernel, dim3((unsigned)(rows * blocks)), dim3(THREADS), smem, (cudaStream_t)stream, (unsigned)blocks, r);
+    if (r.mark) {
+        const int clusters = resident / most < rows ? resident / most : rows;
+        Rows marked = rows_of(most);
+        smem = LIST * (sizeof(unsigned int) + sizeof(u64));
+        marked.cached = smem + part_of(marked) <= ONE;
+        if (marked.cached) smem += part_of(marked);
+        raised = raise_shared<sample_marked_kernel>((int)smem);
+        if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "sample_filtered: cannot raise shared memory: %s", cudaGetErrorString(raised));
+        launch_kernel_cluster(sample_marked_kernel, dim3((unsigned)(clusters * most)), dim3(THREADS), smem, (cudaStream_t)stream, (unsigned)most, marked);
+    }
     QT_CHECK_LAUNCH("sample_filtered");
     return QT_OK;
 }

@@ -186,6 +186,48 @@ def test_tokens_that_stand_out_side_by_side():
     check(logits.cuda(), [(1.0, 500, 1.0, 0.0), (1.0, 3, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (0.8, 299, 0.95, 0.001)], 13)
 
 
+@pytest.mark.parametrize("rows, vocab", [(90, 40001), (330, 20003), (75, 151936), (40, 70000), (700, 8300)])
+def test_more_rows_than_fit_at_a_time(rows, vocab):
+    """Few blocks a row, rows that are left to a second launch: without filters, with wide heads, and none of these side by side with rows of every kind."""
+    gen = torch.Generator().manual_seed(rows)
+    logits = 2.0 * torch.randn((rows, vocab + 3), generator=gen)[:, 3:]
+    logits[:, torch.randint(0, vocab, (30,), generator=gen)] += 7.0
+    logits[1::5, ::3] = float("-inf")
+    logits[2::5, 1::4] = float("nan")
+    kinds = PARAMS + [(1.0, 0, 0.97, 0.0), (1.5, 0, 0.6, 1e-4), (2.0, 3000, 1.0, 0.0), (1.0, 900, 0.95, 0.0), (1e-6, 0, 1.0, 0.0)]
+    params = [kinds[i % len(kinds)] for i in range(rows)]
+    whole = torch.empty((rows, vocab + 3), device="cuda")
+    whole[:, 3:] = logits.cuda()
+    check(whole[:, 3:], params, rows + 1)
+    nothing = torch.full((rows, vocab), float("-inf"), device="cuda")
+    tokens, logprob = run(nothing, *[[p[c] for p in params] for c in range(4)], [0.5] * rows)
+    assert tokens.tolist() == [0] * rows and logprob.tolist() == [-math.inf] * rows
+
+
+@pytest.mark.parametrize("rows", [12, 156])
+def test_shares_that_end_beside_a_token(rows):
+    """top_p a millionth more or less than what lies before a token.  The weights' errors are 2^-23 and less of each, of both signs; what stays beside ten tokens that stand out is
+    2e-5 of the mass: a millionth decides."""
+    gen = torch.Generator().manual_seed(rows)
+    vocab = 30000
+    logits = torch.randn((rows, vocab), generator=gen).clamp(max=2.0)
+    params, wanted = [], []
+    for row in range(rows):
+        heads = torch.randperm(vocab, generator=gen)[:10]
+        logits[row, heads] = 22.0 + torch.rand((10,), generator=gen)
+        w, _ = kept_of(logits[row], 1.0, 0, 1.0, 0.0)
+        share = w[w > 0.1].sort(descending=True).values.cumsum(0) / w.sum()
+        p = torch.tensor(float(share[1 + row % 8]) + (1e-6 if row % 2 else -1e-6)).item()
+        weights, y = kept_of(logits[row], 1.0, 0, p, 0.0)
+        token, u = middle(weights, gen)
+        params.append((1.0, 0, p, 0.0, u))
+        wanted.append((token, float(y[token] - weights.sum().log())))
+    tokens, logprob = run(logits.cuda(), *[[p[c] for p in params] for c in range(5)])
+    assert tokens.tolist() == [w[0] for w in wanted]
+    for got, (_, want) in zip(logprob.tolist(), wanted):
+        assert abs(got - want) <= 2e-6 * (3 + abs(want)), (got, want)
+
+
 def test_no_order_of_additions_shows_and_the_stream_is_followed():
     gen = torch.Generator(device="cuda").manual_seed(8)
     logits = torch.randn((64, 151936), generator=gen, device="cuda")
