@@ -84,7 +84,7 @@ struct OwnRanges {
 // A block has up to 32 rows (member, query head) of a kv head, of all members over a range of the group's shared keys or of one member over a range of its own,
 // and walks the range 32 keys at a time through shared memory, as floats, the next tile's loads under way meanwhile.  Eight lanes have a row, a sixteenth or
 // more of the dims each; where there are fewer rows, several groups of lanes share one's keys, each with a maximum, a sum and sums of its own, which meet at the
-// end.  Five sequences of 900 shared and 60 own keys in float, 16 heads over 8 of 128: MEASURED_F32 (a warp a row and range, a key at a time, 78 us).
+// end.  Five sequences of 900 shared and 60 own keys in float, 16 heads over 8 of 128: 22 us (a warp a row and range, a key at a time, 78 us).
 constexpr int ANY_TILE = 32;
 constexpr int ANY_THREADS = 256;
 constexpr int ANY_ROWS = ANY_THREADS / 8;
@@ -267,6 +267,10 @@ __global__ void __launch_bounds__(ANY_THREADS) shared_any_kernel(const SharedPar
 //
 // one thread a row, so that maxima and sums need no exchange; O is rescaled only where a row's maximum moved by more than 2^8.  A member's own keys give an M of a
 // few rows and cost the tensor cores what 128 would, which is still less than what their keys' way from memory takes.  The second launch joins the ranges.
+//
+// Bound by the chain of a tile (scores, their 64 exponentials a row, P, O) where rows are many, and by memory where own keys are.  Measured, 32 heads over 8 of 128:
+// eight sequences of 2,048 shared and 130 own keys 12.5 us, 48 of three prompts of up to 5,000 and 700 37 us, 64 of 16,384 and 512 50 us (146 MB and 18 GFLOP: 2.9 TB/s); 128
+// sequences of 64 heads, 32,000 and 600 keys, 168 to 196 us by the clock that the power limit leaves (136 GFLOP: 0.8 to 0.7 PFLOP/s).
 constexpr int PAGE = 64;
 constexpr int BQ = 128;
 constexpr int TC_THREADS = 224;      // warp 0: TMA of K, warp 1: MMA and tensor memory, warps 2..5: Q and softmax, warp 6: TMA of V
@@ -317,7 +321,8 @@ __device__ __forceinline__ void store_shared16(uint32_t addr, uint4 v) {
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // The products as a whole warp meets them: all lanes go through the same instructions, so that descriptors stay in the registers that a warp has in common, and one
-// lane's are carried out.  Issued by a lane that runs alone, a product takes about 100 cycles to leave, 12 of them a tile: MEASURED_ISSUE.
+// lane's are carried out.  Issued by a lane that runs alone, a product takes about 100 cycles to leave, 12 of them a tile: a tile of a
+// block that is alone on its SM took 0.82 us so and takes 0.68.
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t elected;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
@@ -836,7 +841,8 @@ __device__ __forceinline__ void walk_keys(const SharedParams& p, Walked<HD>& w, 
 }
 
 // Everything in one launch, where so little is shared that a second launch costs more than reading it again (out of the L2 cache): the blocks of (16 query
-// heads of a kv head, member) are a cluster along x whose warps each walk a range of all of the member's keys; the first block joins the ranges.
+// heads of a kv head, member) are a cluster along x whose warps each walk a range of all of the member's keys; the first block joins the ranges.  Bound by latency:
+// two sequences of 199 shared and 40 own keys, 16 heads over 8, 5.2 us (about 5 us more in two launches); 20 of 1,500 and 90, 5 heads of 64, 10 us.
 constexpr int DIRECT_MAX_WARPS = 6;
 
 template <int HD> constexpr size_t direct_smem(int warps, int ranges, int rows) {
