@@ -269,8 +269,8 @@ __global__ void __launch_bounds__(ANY_THREADS) shared_any_kernel(const SharedPar
 // few rows and cost the tensor cores what 128 would, which is still less than what their keys' way from memory takes.  The second launch joins the ranges.
 //
 // Bound by the chain of a tile (scores, their 64 exponentials a row, P, O) where rows are many, and by memory where own keys are.  Measured, 32 heads over 8 of 128:
-// eight sequences of 2,048 shared and 130 own keys 12.5 us, 48 of three prompts of up to 5,000 and 700 37 us, 64 of 16,384 and 512 50 us (146 MB and 18 GFLOP: 2.9 TB/s); 128
-// sequences of 64 heads, 32,000 and 600 keys, 168 to 196 us by the clock that the power limit leaves (136 GFLOP: 0.8 to 0.7 PFLOP/s).
+// eight sequences of 2,048 shared and 130 own keys 12.5 us, 48 of three prompts of up to 5,000 and 700 36 us, 64 of 16,384 and 512 46 us (146 MB and 18 GFLOP: 3.2 TB/s); 128
+// sequences of 64 heads, 32,000 and 600 keys, 168 to 198 us by the clock that the power limit leaves (136 GFLOP: 0.8 to 0.7 PFLOP/s).
 constexpr int PAGE = 64;
 constexpr int BQ = 128;
 constexpr int TC_THREADS = 224;      // warp 0: TMA of K, warp 1: MMA and tensor memory, warps 2..5: Q and softmax, warp 6: TMA of V
