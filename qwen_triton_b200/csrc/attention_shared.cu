@@ -984,12 +984,26 @@ int launch_direct(const SharedParams& p, int warps, cudaStream_t stream) {
 
 }  // namespace
 
+// A call's arguments as one structure, which its caller lays out field by field.
+struct SharedCall {
+    const void *q, *k_cache, *v_cache;
+    void* out;
+    const int *block_table, *seq_len, *members, *share;
+    float *part_acc, *part_ml;
+    int* status;
+    void* stream;
+    double scale;
+    int dtype, n_seqs, n_groups, most_members, nq, nkv, d, page_tokens, shared_ranges, own_ranges, direct_warps, on_tc, max_blocks, n_pages;
+};
+static_assert(sizeof(SharedCall) == 13 * 8 + 14 * 4, "12 addresses, a number of 64 bits and 14 of 32, without gaps");
+
 // on_tc: bfloat16, d % 8 == 0 and at most 128, pages of 64.  With shared_ranges = 0 (on_tc) one launch walks all of a member's keys, by own_ranges <= 8
 // blocks of direct_warps warps a member and kv head.
-extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, const int* block_table,
-                                          int max_blocks, const int* seq_len, const int* members, const int* share, int n_seqs, int n_groups,
-                                          int most_members, int nq, int nkv, int d, int page_tokens, int n_pages, float scale, int shared_ranges,
-                                          int own_ranges, int direct_warps, int on_tc, float* part_acc, float* part_ml, int* status, void* stream) {
+extern "C" int qt_attention_decode_shared(const SharedCall* call) {
+    const SharedCall& c = *call;
+    const int n_seqs = c.n_seqs, n_groups = c.n_groups, most_members = c.most_members, nq = c.nq, nkv = c.nkv, d = c.d, page_tokens = c.page_tokens, n_pages = c.n_pages,
+              max_blocks = c.max_blocks, shared_ranges = c.shared_ranges, own_ranges = c.own_ranges, direct_warps = c.direct_warps;
+    const float scale = (float)c.scale;
     QT_REQUIRE(n_seqs >= 0 && n_groups > 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "attention_shared: bad head counts nq=%d nkv=%d (B=%d, %d groups)", nq, nkv, n_seqs, n_groups);
     QT_REQUIRE(d > 0 && d <= MAX_DIM && page_tokens > 0 && max_blocks > 0 && n_pages > 0, "attention_shared: bad sizes d=%d page=%d", d, page_tokens);
     QT_REQUIRE((long long)max_blocks * page_tokens <= 0x7fffffffll && most_members >= 0 && most_members <= n_seqs, "attention_shared: bad sizes: %d pages a sequence, %d members",
@@ -997,15 +1011,15 @@ extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, co
     QT_REQUIRE(shared_ranges >= 0 && own_ranges > 0 && shared_ranges + own_ranges <= MAX_RANGES, "attention_shared: %d and %d ranges", shared_ranges, own_ranges);
     QT_REQUIRE(scale > 0.f && scale < INFINITY, "attention_shared: a score scale of %g (it must be positive)", (double)scale);
     if (n_seqs == 0) return QT_OK;
-    const SharedParams p{q, k_cache, v_cache, out, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, nq, nkv, d, page_tokens, n_pages,
-                         scale, shared_ranges, own_ranges, part_acc, part_ml, status, 0, 0, 0, 0, 0};
-    QT_REQUIRE((((uintptr_t)part_acc | (uintptr_t)part_ml) & 15) == 0, "attention_shared: scratch must be 16-byte aligned");
-    cudaStream_t s = (cudaStream_t)stream;
-    if (on_tc) {
-        QT_REQUIRE(dtype == QT_BF16 && d % 8 == 0 && d <= 128 && page_tokens == PAGE && status,
+    const SharedParams p{c.q, c.k_cache, c.v_cache, c.out, c.block_table, max_blocks, c.seq_len, c.members, c.share, n_seqs, n_groups, nq, nkv, d, page_tokens, n_pages,
+                         scale, shared_ranges, own_ranges, c.part_acc, c.part_ml, c.status, 0, 0, 0, 0, 0};
+    QT_REQUIRE((((uintptr_t)c.part_acc | (uintptr_t)c.part_ml) & 15) == 0, "attention_shared: scratch must be 16-byte aligned");
+    cudaStream_t s = (cudaStream_t)c.stream;
+    if (c.on_tc) {
+        QT_REQUIRE(c.dtype == QT_BF16 && d % 8 == 0 && d <= 128 && page_tokens == PAGE && c.status,
                    "attention_shared: the tensor-core kernels take bfloat16, heads of up to 128 in steps of 8, pages of 64 (d=%d, pages of %d)", d, page_tokens);
         QT_REQUIRE((long long)n_pages * nkv * PAGE <= 0x7fffffffll, "attention_shared: %d pages of %d heads are beyond a tensor map", n_pages, nkv);
-        QT_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) == 0, "attention_shared: operands must be 16-byte aligned");
+        QT_REQUIRE((((uintptr_t)c.q | (uintptr_t)c.k_cache | (uintptr_t)c.v_cache | (uintptr_t)c.out) & 15) == 0, "attention_shared: operands must be 16-byte aligned");
         if (shared_ranges == 0) {
             QT_REQUIRE(own_ranges <= 8 && direct_warps > 0 && direct_warps <= DIRECT_MAX_WARPS, "attention_shared: %d blocks of %d warps", own_ranges, direct_warps);
             return d <= 64 ? launch_direct<64>(p, direct_warps, s) : launch_direct<128>(p, direct_warps, s);
@@ -1013,7 +1027,7 @@ extern "C" int qt_attention_decode_shared(const void* q, const void* k_cache, co
         return d <= 64 ? launch_parts<64>(p, most_members, s) : launch_parts<128>(p, most_members, s);
     }
     QT_REQUIRE(shared_ranges > 0, "attention_shared: %d ranges of shared keys", shared_ranges);
-    return QT_DISPATCH_DTYPE(dtype, "attention_shared", {
+    return QT_DISPATCH_DTYPE(c.dtype, "attention_shared", {
         if (d <= 64) return launch_any<T, 2>(p, most_members, s);
         if (d <= 128) return launch_any<T, 4>(p, most_members, s);
         return launch_any<T, 8>(p, most_members, s);

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -131,10 +132,7 @@ _SIGNATURES = {
                                      _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_float, _c_int, _c_ptr],
     },
     "attention_shared": {
-        # q, k_cache, v_cache, out, dtype, block_table, max_blocks, seq_len, members, share, n_seqs, n_groups, most_members, nq, nkv, d, page_tokens,
-        # n_pages, scale, shared_ranges, own_ranges, direct_warps, on_tc, part_acc, part_ml, status, stream
-        "qt_attention_decode_shared": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                                       _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
+        "qt_attention_decode_shared": [ctypes.c_char_p],      # a SharedCall (_SHARED_CALL)
     },
     "attention_tc": {
         "qt_attention_prefill_tc": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int,
@@ -1429,10 +1427,19 @@ class SharedPlan:
         return self.groups, 3
 
     @functools.cached_property
-    def on_tc(self) -> int:
-        """1 where the tensor-core kernels take the call."""
-        return int(_shared_on_tc(self.dtype, self.head_dim, self.page_tokens))
+    def numbers(self) -> tuple[int, ...]:
+        """The numbers of a call that the plan has, in the order of the library's structure."""
+        return (_CODES[self.dtype], self.n_seqs, self.groups, self.most_members, self.num_heads, self.num_kv_heads, self.head_dim, self.page_tokens,
+                self.shared_ranges, self.own_ranges, self.direct_warps, int(_shared_on_tc(self.dtype, self.head_dim, self.page_tokens)))
 
+    @functools.cached_property
+    def launches(self) -> int:
+        return (2 if self.shared_ranges else 1) if self.n_seqs else 0
+
+
+# q, k_cache, v_cache, out, block_table, seq_len, members, share, part_acc, part_ml, status, stream, scale, the plan's numbers, max_blocks, n_pages: ctypes takes
+# 3 us for as many arguments and 0.6 for a structure of them, of 10 that the smallest call took.
+_SHARED_CALL = struct.Struct("@12Pd14i")
 
 DIRECT_BYTES = 48 << 20       # keys and values that one launch reads over all members (out of the L2 cache where they are shared)
 
@@ -1553,10 +1560,10 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             and block_table.is_contiguous() and seq_len.is_contiguous() and members.is_contiguous() and share.is_contiguous() and part_acc.is_contiguous()
             and part_ml.is_contiguous()):
         _check_shared(q, k_cache, v_cache, out, block_table, seq_len, members, share, num_kv_heads, page_tokens, plan, part_acc, part_ml)
-    _call("attention_shared", "qt_attention_decode_shared", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _CODES[plan.dtype],
-          block_table.data_ptr(), block_table.shape[1], seq_len.data_ptr(), members.data_ptr(), share.data_ptr(), shape[0], plan.groups, plan.most_members, shape[1],
-          num_kv_heads, shape[2], page_tokens, k_cache.shape[0], float(scale), plan.shared_ranges, plan.own_ranges, plan.direct_warps, plan.on_tc, part_acc.data_ptr(),
-          part_ml.data_ptr(), _status_word(q.device).data_ptr(), _stream(), launches=(2 if plan.shared_ranges else 1) if shape[0] else 0)
+    _call("attention_shared", "qt_attention_decode_shared",
+          _SHARED_CALL.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_len.data_ptr(), members.data_ptr(),
+                            share.data_ptr(), part_acc.data_ptr(), part_ml.data_ptr(), _status_word(q.device).data_ptr(), _stream(), scale, *plan.numbers,
+                            block_table.shape[1], k_cache.shape[0]), launches=plan.launches)
 
 
 # ----------------------------------------------------------------------------- experts chosen by a table
