@@ -764,7 +764,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows 
     w.by_passes(at, f);
 }
 
-// The rows that the launch before has marked, each by the cluster that comes to it first.
+// The rows that the launch before has marked, each by the cluster that comes to it first; a block looks for them 512 rows at a time (4,096 rows of 20,000,
+// every 97th marked: 259 us; a warp 32 at a time 306).
 __global__ void __launch_bounds__(THREADS, 2) sample_marked_kernel(const Rows r) {
     pdl_launch_dependents();
     if (r.blocks > 1) cluster_arrive_started();
@@ -782,25 +783,22 @@ __global__ void __launch_bounds__(THREADS, 2) sample_marked_kernel(const Rows r)
     for (;;) {
         Row w{r, sh, nullptr, kept, nullptr, nullptr, keys, before, rank, blocks, warp, lane, 0, 0, 0, -INFINITY, 1.f};
         int taken = -1;
-        if (rank == 0 && warp == 0)
+        if (rank == 0)
             while (taken < 0 && seen < r.rows) {
-                const int i = seen + lane, at = i < r.rows - start ? start + i : start + i - r.rows;
-                unsigned int marked = __ballot_sync(0xffffffffu, i < r.rows && *(volatile int*)(r.token + at) == MARK);
-                while (taken < 0 && marked) {
-                    const int first = __ffs(marked) - 1;
-                    marked &= marked - 1;
-                    int was = 0;
-                    if (lane == first) was = atomicCAS(r.token + at, MARK, TAKEN);
-                    if (__shfl_sync(0xffffffffu, was, first) == MARK) taken = __shfl_sync(0xffffffffu, at, first);
-                }
-                if (taken < 0) seen += 32;
+                const int i = seen + (int)threadIdx.x, at = i < r.rows - start ? start + i : start + i - r.rows;
+                const bool marked = i < r.rows && *(volatile int*)(r.token + at) == MARK;
+                if (threadIdx.x == 0) sh.bin_found = 0xffffffffu;
+                __syncthreads();
+                if (marked) atomicMin(&sh.bin_found, (unsigned int)i);
+                __syncthreads();
+                const unsigned int first = sh.bin_found;
+                if (first == 0xffffffffu) { seen += THREADS; __syncthreads(); continue; }
+                if (i == (int)first) sh.above = (u64)(unsigned int)(atomicCAS(r.token + at, MARK, TAKEN) == MARK ? at : -1);
+                __syncthreads();
+                taken = (int)(unsigned int)sh.above;
             }
-        // from the first warp of the first block to all
-        if (rank == 0) {
-            if (threadIdx.x == 0) sh.above = (u64)(unsigned int)taken;
-            __syncthreads();
-        }
-        const int at = (int)(unsigned int)sh.slots[w.exchange(rank == 0 ? sh.above : 0, 0)][0][0];
+        // from the first block to all
+        const int at = (int)(unsigned int)sh.slots[w.exchange((u64)(unsigned int)taken, 0)][0][0];
         if (at < 0) break;
         w.row = r.logits + at * r.row_stride;
         w.shift = (int)(((uintptr_t)w.row >> 2) & 3);
