@@ -20,15 +20,15 @@
 //     block in vocabulary order; that block sorts their keys, finds the thresholds on the running count and mass, and draws.
 //
 // Only the row's mass for top_p without top_k takes an exponential a token, an approximate one, in the same pass.  A row whose head does not fit the list, or whose
-// threshold lies within that mass's error, finds its thresholds by bins of all of its tokens, each 256 times narrower than the one before, until what is in the bin
-// of the threshold fits the list (three times; what is still alike then is bisected).  Such a row, and one without filters, draws over all blocks.  These read the
-// row again for every pass, out of the L2 cache where it is still there.
+// threshold lies within that mass's error, finds its thresholds by bins of all of its tokens, each 256 times narrower than the one before, until the bin of the
+// threshold has few tokens, which are sorted (three times; a bin that is still longer than the list is bisected).  Such a row, and one without filters, draws over all
+// blocks.  For these passes a block keeps its ids in shared memory where they fit, and reads them again otherwise.
 //
 // The first pass goes at the memory's rate where every row is read at once, by few blocks a row if rows are many; passes with exponentials want many blocks a row.  So rows
 // that need those are then marked and left to a second launch.
 //
-// Measured behind a cold cache: one row of 151,936 14.6 us, 64 rows 37 to 51, 256 rows (156 MB, 24 us of copying) 122 to 136, by what the rows ask for; with every row on
-// eight blocks that kept it in shared memory (37 rows at a time) 14.8, 49 to 78 and 131 to 170.  A row of 256 is read in 30 us; the rest is the head: what it runs is
+// Measured behind a cold cache: one row of 151,936 14.6 us, 64 rows 37 to 51, 256 rows (156 MB, 24 us of copying) 121 to 130, by what the rows ask for; with every row on
+// eight blocks that kept it in shared memory (37 rows at a time) 15.8, 49 to 78 and 131 to 170.  A row of 256 is read in 30 us; the rest is the head: what it runs is
 // short and serial (bins 5 us, tokens read again 4 to 17, sort and draw 8 to 12), so that its instructions' way into the SM counts, and loops stay loops.
 #include "common.cuh"
 
@@ -837,7 +837,7 @@ extern "C" int qt_sample_filtered(const float* logits, long long row_stride, con
     constexpr size_t ONE = 219 * 1024, TWO = 106 * 1024;        // of an SM's shared memory for one block and for each of two, the static part taken off
     Rows r = rows_of(blocks);
     // 64 rows by four blocks each take 37 to 51 us where the rows that need more passes stay with them and 40 to 91 where these are left to the second launch; 256 rows
-    // by one block each take 122 to 136 with it and 244 without
+    // by one block each take 121 to 130 with it and 244 without
     r.mark = blocks < most && blocks < 4;
     size_t smem = head_bytes(r);
     r.cached = !r.mark && smem + part_of(r) <= ((long long)rows * blocks > sm_count() ? TWO : ONE);
