@@ -8,7 +8,8 @@
 //           y - log(mass)
 //
 // So tokens that tie share their fate, and every filter is a threshold on the logit.  A mass is a sum of whole numbers, w in units of 2^-40
-// of the largest: w has 24 bits, so a weight above 2^-16 loses nothing and a smaller one at most 2^-41, and no order of additions shows.
+// of the largest: w has 24 bits, so a weight above 2^-16 loses nothing and a smaller one at most 2^-41, and no order of additions shows.  A row of 2^24 equal
+// logits would sum to 2^64, which 64 bits do not hold: a call of more than 2^23 is refused.
 // T <= 0 takes the lowest id of the largest logit (log-probability 0).  NaN counts as -inf; a row without anything above -inf gives id 0 with
 // log-probability -inf.
 //
@@ -49,6 +50,7 @@ constexpr int WAITING = 32 * (TURNS + 1);
 constexpr int FEW = 256;               // keys that are sorted rather than sent through narrower bins
 constexpr int MARK = -1, TAKEN = -2;   // in place of a token: the row is left to the second launch; a cluster of that launch has it
 constexpr int MAX_NOTES = 16;          // noted logits of a thread
+constexpr int MAX_VOCAB = 1 << 23;     // whose masses fit 64 bits, whatever the row
 constexpr double LOG2E = 1.4426950408889634;
 // Bound of the relative error of a row's mass from the first pass: 2^-22 of an exponential, half a unit of the difference in it (2^-24 of the distance below the
 // largest, in bits log2(vocabulary) at most on the average that weights give), 2^-24 for each of seven additions and a scaling.
@@ -818,8 +820,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_marked_kernel(const Rows r)
 // logprob float [rows] or null.
 extern "C" int qt_sample_filtered(const float* logits, long long row_stride, const float* temperature, const int* top_k, const float* top_p,
                                   const float* min_p, const float* uniform, int* token, float* logprob, int rows, int vocab, void* stream) {
-    QT_REQUIRE(rows >= 0 && vocab > 0 && vocab <= 0x3fffffff && (rows <= 1 || row_stride >= vocab), "sample_filtered: bad sizes rows=%d vocab=%d stride=%lld",
+    QT_REQUIRE(rows >= 0 && vocab > 0 && (rows <= 1 || row_stride >= vocab), "sample_filtered: bad sizes rows=%d vocab=%d stride=%lld",
                rows, vocab, row_stride);
+    QT_REQUIRE(vocab <= MAX_VOCAB, "sample_filtered: a vocabulary of %d tokens is beyond the %d whose masses fit 64 bits", vocab, MAX_VOCAB);
     if (rows == 0) return QT_OK;
     QT_REQUIRE(rows <= 0x7fffffff / MAX_BLOCKS, "sample_filtered: %d rows are more than one launch takes", rows);
     // down to 4,096 ids a block, and as many blocks a row as are resident at a time with two an SM

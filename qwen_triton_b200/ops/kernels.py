@@ -1813,7 +1813,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     ``uniform`` in [0, 1) by which the token is drawn in vocabulary order.  Tokens above which fewer than ``top_k`` logits lie are kept; of these,
     tokens above which less than ``top_p`` of their mass lies; of these, tokens at least ``min_p`` times as likely as the likeliest.
     ``out`` (int32) takes the tokens, ``logprob`` (float, optional) the logarithm of the probability with which each was drawn.  NaN counts as -inf;
-    a row that has nothing above -inf gives token 0 with log-probability -inf."""
+    a row that has nothing above -inf gives token 0 with log-probability -inf.  A vocabulary has at most 2^23 tokens."""
     if logits.dim() != 2 or not (logits.stride(1) == 1 and logits.shape[1] > 0 and logits.stride(0) >= logits.shape[1] and logits.is_cuda and
             logits.dtype is temperature.dtype is top_p.dtype is min_p.dtype is uniform.dtype is torch.float32 and top_k.dtype is out.dtype is torch.int32
             and logits.shape[:1] == temperature.shape == top_k.shape == top_p.shape == min_p.shape == uniform.shape == out.shape

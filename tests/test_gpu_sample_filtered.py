@@ -267,3 +267,16 @@ def test_no_rows_and_refusals():
                            (dict(out=f), "out"), (dict(logprob=out), "logprob")):
         with pytest.raises(KernelError, match=words):
             kernels.sample_filtered(**{**good, **changes})
+
+
+def test_the_largest_vocabulary_and_one_beyond():
+    """2^23 equal logits weigh 2^63 units of 2^-40; a row of 2^24 would not fit 64 bits, so no more than the first are taken."""
+    vocab = 1 << 23
+    logits = torch.zeros((1, vocab + 1), device="cuda")
+    for filters in ((0, 1.0, 0.0), (5, 0.5, 0.3)):            # ties share their fate: every token stays
+        for u in (0.0, 0.25, 0.8125, 1.0):
+            tokens, logprob = run(logits[:, :vocab], [1.0], [filters[0]], [filters[1]], [filters[2]], [u])
+            assert tokens.tolist() == [min(int(u * vocab), vocab - 1)]
+            assert abs(float(logprob[0]) + math.log(vocab)) <= 2e-6 * (1 + math.log(vocab))
+    with pytest.raises(KernelError, match="vocabulary"):
+        run(logits, [1.0], [0], [1.0], [0.0], [0.5])
