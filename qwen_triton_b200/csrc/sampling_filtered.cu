@@ -52,9 +52,6 @@ constexpr int MARK = -1, TAKEN = -2;   // in place of a token: the row is left t
 constexpr int MAX_NOTES = 16;          // noted logits of a thread
 constexpr int MAX_VOCAB = 1 << 23;     // whose masses fit 64 bits, whatever the row
 constexpr double LOG2E = 1.4426950408889634;
-// Bound of the relative error of a row's mass from the first pass: 2^-22 of an exponential, half a unit of the difference in it (2^-24 of the distance below the
-// largest, in bits log2(vocabulary) at most on the average that weights give), 2^-24 for each of seven additions and a scaling.
-constexpr double MASS_ERROR = 1. / 524288.;
 typedef unsigned long long u64;
 
 struct Rows {
@@ -64,7 +61,19 @@ struct Rows {
     int rows, vocab, blocks, turns, span;      // blocks a row; turns of a warp over its ids, 128 a turn; turns a noted logit
     int cached;                        // whether a block keeps its ids in shared memory for further passes
     int mark;                          // whether rows that need more passes get MARK for a token
+    double mass_error;
 };
+
+// How far, relative to it, a row's mass from the first pass may lie from the sum of units that decides.
+//
+//   first pass   2^-22 of each exponential; 2^-24 for each of seven additions of floats; a thread's sum is scaled once more for each time its largest logit grew,
+//                TURNS turns at a time, and once at the end, 2^-22 of an expf each (of all floats from -87 to 0, 2.6 2^-24 at most)
+//   units        2^-22 of an expf, and half a unit, 2^-41, of every token
+//   exponents    in both, a difference and a quotient or product are rounded, 2^-24 of the exponent each; steps on a thread's way to the largest logit add up to
+//                the token's distance y from it.  On the average that the weights give, y is their entropy less the logarithm of their sum, at most ln(vocabulary)
+inline double mass_error(int vocab, int turns) {
+    return (4. + (turns + TURNS - 1) / TURNS + log((double)vocab) + vocab / 524288.) / 4194304.;
+}
 
 // Floats as unsigned integers of the same order (no NaN comes here); the two zeros share a key.
 __device__ __forceinline__ unsigned int ordered_key(float x) {
@@ -727,7 +736,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows 
             if (f.by_mass) {
                 // the likeliest token stays whatever p is
                 const double wanted = (double)f.p * row_mass;
-                const u64 last = f.p > 0.f ? cut(keys, before, sh.per_warp, count, true, floor_key, 0, wanted, summing ? 0. : (double)f.p, wanted * MASS_ERROR, w.weigh()) : keys[0];
+                const u64 last = f.p > 0.f ? cut(keys, before, sh.per_warp, count, true, floor_key, 0, wanted, summing ? 0. : (double)f.p, wanted * r.mass_error, w.weigh()) : keys[0];
                 floor_key = max(floor_key, (unsigned int)last);
                 if (summing) {
                     fits = last >> 32 == 0;
@@ -834,7 +843,7 @@ extern "C" int qt_sample_filtered(const float* logits, long long row_stride, con
     auto rows_of = [&](int blocks) {
         const int quads = (vocab + 3 + 3) / 4, turns = (quads + blocks * THREADS - 1) / (blocks * THREADS);
         const int span = TURNS * ((turns + TURNS * MAX_NOTES - 1) / (TURNS * MAX_NOTES));
-        return Rows{logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, rows, vocab, blocks, turns, span, 0, 0};
+        return Rows{logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, rows, vocab, blocks, turns, span, 0, 0, mass_error(vocab, turns)};
     };
     auto part_of = [&](const Rows& r) { return (size_t)r.turns * THREADS * sizeof(float4); };
     constexpr size_t ONE = 219 * 1024, TWO = 106 * 1024;        // of an SM's shared memory for one block and for each of two, the static part taken off

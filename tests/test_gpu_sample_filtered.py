@@ -280,3 +280,38 @@ def test_the_largest_vocabulary_and_one_beyond():
             assert abs(float(logprob[0]) + math.log(vocab)) <= 2e-6 * (1 + math.log(vocab))
     with pytest.raises(KernelError, match="vocabulary"):
         run(logits, [1.0], [0], [1.0], [0.0], [0.5])
+
+
+def test_a_share_that_the_tail_of_a_large_vocabulary_decides():
+    """Masses are sums of whole units of 2^-40.  2^23 - 2 tokens of 1.55 units count as two each, 3.4e-6 of the mass more than their weights: with those, what lies
+    before the second token is p of the mass and 6e-7 more, with the weights 2.5e-6 less.  However the row is walked (top_k, which leaves every token
+    here, takes another way), the units decide."""
+    vocab = 1 << 23
+    logits = torch.full((1, vocab), math.log(1.55) - 40 * math.log(2))
+    first, second = 1000, vocab - 77
+    logits[0, first], logits[0, second] = 0.0, math.log(0.1)
+    p = 1 / ((1.1 + (vocab - 2) * 1.55 * 2.0 ** -40) * (1 + 2.5e-6))
+    assert p * (1.1 + (vocab - 2) * 2 * 2.0 ** -40) > 1 + 5e-7
+    for k in (0, vocab - 1):
+        tokens, logprob = run(logits.cuda(), [1.0], [k], [p], [0.0], [0.97])
+        assert tokens.tolist() == [second]
+        assert abs(float(logprob[0]) - math.log(0.1 / 1.1)) < 1e-5
+
+
+def test_shares_that_end_beside_a_token_of_a_large_vocabulary():
+    """As above, over two million tokens whose units' roundings cancel: a millionth more or less decides."""
+    gen = torch.Generator().manual_seed(21)
+    vocab = 1 << 21
+    for row in range(4):
+        logits = torch.randn((1, vocab), generator=gen).clamp(max=2.0)
+        heads = torch.randperm(vocab, generator=gen)[:10]
+        logits[0, heads] = 26.0 + torch.rand((10,), generator=gen)
+        w, _ = kept_of(logits[0], 1.0, 0, 1.0, 0.0)
+        share = w[w > 0.1].sort(descending=True).values.cumsum(0) / w.sum()
+        p = torch.tensor(float(share[1 + 2 * row]) + (1e-6 if row % 2 else -1e-6)).item()
+        weights, y = kept_of(logits[0], 1.0, 0, p, 0.0)
+        token, u = middle(weights, gen)
+        tokens, logprob = run(logits.cuda(), [1.0], [0], [p], [0.0], [u])
+        want = float(y[token] - weights.sum().log())
+        assert tokens.tolist() == [token]
+        assert abs(float(logprob[0]) - want) <= 2e-6 * (3 + abs(want))
