@@ -823,7 +823,25 @@ __global__ void __launch_bounds__(THREADS, 2) sample_marked_kernel(const Rows r)
     }
 }
 
+// How a call is cut.
+struct Cut {
+    int resident, most, blocks;        // blocks at a time; blocks a row at most, and as many as it takes
+    bool mark;                         // whether rows that need more passes are left to a second launch
+    Cut(int rows, int vocab) : resident(2 * sm_count()), most(1) {
+        // down to 4,096 ids a block, and as many blocks a row as are resident at a time with two an SM
+        while (most < MAX_BLOCKS && vocab / most > 8192) most *= 2;
+        blocks = most;
+        while (blocks > 1 && (long long)rows * blocks > resident) blocks /= 2;
+        // 64 rows by four blocks each take 37 to 51 us where the rows that need more passes stay with them and 40 to 91 where these are left to the second launch; 256
+        // rows by one block each take 121 to 130 with it and 244 without
+        mark = blocks < most && blocks < 4;
+    }
+};
+
 }  // namespace
+
+// The launches that a call of qt_sample_filtered makes.
+extern "C" int qt_sample_filtered_launches(int rows, int vocab) { return rows > 0 ? (Cut(rows, vocab).mark ? 2 : 1) : 0; }
 
 // logits [rows, vocab] float with rows `row_stride` elements apart; temperature, top_p, min_p, uniform float [rows], top_k int [rows]; token int [rows],
 // logprob float [rows] or null.
@@ -834,12 +852,8 @@ extern "C" int qt_sample_filtered(const float* logits, long long row_stride, con
     QT_REQUIRE(vocab <= MAX_VOCAB, "sample_filtered: a vocabulary of %d tokens is beyond the %d whose masses fit 64 bits", vocab, MAX_VOCAB);
     if (rows == 0) return QT_OK;
     QT_REQUIRE(rows <= 0x7fffffff / MAX_BLOCKS, "sample_filtered: %d rows are more than one launch takes", rows);
-    // down to 4,096 ids a block, and as many blocks a row as are resident at a time with two an SM
-    const int resident = 2 * sm_count();
-    int most = 1;
-    while (most < MAX_BLOCKS && vocab / most > 8192) most *= 2;
-    int blocks = most;
-    while (blocks > 1 && (long long)rows * blocks > resident) blocks /= 2;
+    const Cut of(rows, vocab);
+    const int resident = of.resident, most = of.most;
     auto rows_of = [&](int blocks) {
         const int quads = (vocab + 3 + 3) / 4, turns = (quads + blocks * THREADS - 1) / (blocks * THREADS);
         const int span = TURNS * ((turns + TURNS * MAX_NOTES - 1) / (TURNS * MAX_NOTES));
@@ -847,10 +861,9 @@ extern "C" int qt_sample_filtered(const float* logits, long long row_stride, con
     };
     auto part_of = [&](const Rows& r) { return (size_t)r.turns * THREADS * sizeof(float4); };
     constexpr size_t ONE = 219 * 1024, TWO = 106 * 1024;        // of an SM's shared memory for one block and for each of two, the static part taken off
+    const int blocks = of.blocks;
     Rows r = rows_of(blocks);
-    // 64 rows by four blocks each take 37 to 51 us where the rows that need more passes stay with them and 40 to 91 where these are left to the second launch; 256 rows
-    // by one block each take 121 to 130 with it and 244 without
-    r.mark = blocks < most && blocks < 4;
+    r.mark = of.mark;
     size_t smem = head_bytes(r);
     r.cached = !r.mark && smem + part_of(r) <= ((long long)rows * blocks > sm_count() ? TWO : ONE);
     if (r.cached) smem += part_of(r);

@@ -181,6 +181,7 @@ _SIGNATURES = {
     "sampling_filtered": {
         # logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, rows, vocab, stream
         "qt_sample_filtered": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+        "qt_sample_filtered_launches": [_c_int, _c_int],
     },
 }
 _BOUND: dict[str, ctypes._CFuncPtr] = {}
@@ -1806,6 +1807,11 @@ def _check_filtered(logits, temperature, top_k, top_p, min_p, uniform, out, logp
         _need(logprob, "logprob", torch.float32, (rows,))
 
 
+@functools.lru_cache(maxsize=1024)
+def _filtered_launches(rows: int, vocab: int) -> int:
+    return _fn("sampling_filtered", "qt_sample_filtered_launches")(rows, vocab)
+
+
 def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
                     uniform: torch.Tensor, out: torch.Tensor, logprob: torch.Tensor | None = None) -> None:
     """One token per row of float logits [rows, vocab] (rows may lie further apart than they are long), with parameters of the row's own, all on the
@@ -1823,7 +1829,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
         _check_filtered(logits, temperature, top_k, top_p, min_p, uniform, out, logprob)
     rows, vocab = logits.shape
     _call("sampling_filtered", "qt_sample_filtered", _ptr(logits), logits.stride(0) if rows > 1 else vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
-          _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(logprob), rows, vocab, _stream(), launches=1 if rows else 0)
+          _ptr(min_p), _ptr(uniform), _ptr(out), _ptr(logprob), rows, vocab, _stream(), launches=_filtered_launches(rows, vocab))
 
 
 _STATUS: dict[int, torch.Tensor] = {}
