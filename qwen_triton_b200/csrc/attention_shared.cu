@@ -938,11 +938,10 @@ int launch_any(SharedParams p, int most_members, cudaStream_t stream) {
     const int per = p.nq / p.nkv;
     const long long tiles = ((long long)most_members * per + ANY_ROWS - 1) / ANY_ROWS, own_tiles = (per + ANY_ROWS - 1) / ANY_ROWS;
     const long long shared = tiles * p.nkv * p.shared_ranges * p.n_groups, own = own_tiles * p.nkv * p.own_ranges * p.n_seqs;
-    QT_REQUIRE(shared + own <= 0x3fffffffll, "attention_shared: too many rows for one launch");
+    const long long heads = (long long)p.nkv * ((per + 15) / 16);
+    QT_REQUIRE(shared + own <= 0x3fffffffll && heads <= 0x7fffffffll && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
     p.row_tiles = (int)tiles; p.own_tiles = (int)own_tiles; p.shared_items = (int)shared; p.own_items = (int)own;
     launch_kernel(shared_any_kernel<T, FOURS>, dim3((unsigned)(shared + own)), dim3(ANY_THREADS), smem, stream, p);
-    const long long heads = (long long)p.nkv * ((per + 15) / 16);
-    QT_REQUIRE(heads <= 0x7fffffffll && p.n_seqs <= 65535, "attention_shared: too many rows for one launch");
     launch_kernel(shared_join_kernel<T, ANY_TILE, false>, dim3((unsigned)heads, p.n_seqs), dim3(JOIN_THREADS), 0, stream, p);
     QT_CHECK_LAUNCH("attention_shared");
     return QT_OK;

@@ -283,3 +283,19 @@ def test_refusals():
     with pytest.raises(KernelError, match="shared memory"):
         wide.run(dataclasses.replace(wide.plan, shared_ranges=0, own_ranges=8, direct_warps=6))
     wide.check(wide.run())                                    # and nothing of that stays behind
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_refused_call_launches_nothing(dtype):
+    """More sequences than the second launch takes: the first has not run either."""
+    n = 65536
+    plan = kernels.shared_plan(n, num_heads=1, num_kv_heads=1, head_dim=8, dtype=dtype, groups=1, most_members=2, most_shared=64, most_own=1)
+    plan = dataclasses.replace(plan, shared_ranges=1, own_ranges=1)
+    q, cache = torch.zeros((n, 1, 8), dtype=dtype, device="cuda"), torch.zeros((2, 1, 64, 8), dtype=dtype, device="cuda")
+    table, lengths = torch.zeros((n, 2), dtype=torch.int32, device="cuda"), torch.full((n,), 65, dtype=torch.int32, device="cuda")
+    members, share = torch.arange(n, dtype=torch.int32, device="cuda"), torch.tensor([[0, 2, 64]], dtype=torch.int32, device="cuda")
+    acc, ml, out = torch.full((plan.acc_elements,), 7.0, device="cuda"), torch.full((plan.ml_elements,), 7.0, device="cuda"), torch.full_like(q, 7.0)
+    with pytest.raises(KernelError, match="too many"):
+        kernels.attention_decode_shared(q, cache, cache, out, table, lengths, members, share, 1, 64, 0.5, plan, acc, ml)
+    torch.cuda.synchronize()
+    assert all(bool((x == 7).all()) for x in (acc, ml, out))
