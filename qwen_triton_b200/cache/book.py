@@ -55,6 +55,7 @@ class CacheBook:
         self._live: dict[int, _Slot] = {}
         self._holders: list[dict[int, int]] = [{} for _ in self.groups]   # pages held by more than one slot, and by how many
         self._sharers = 0                                                 # live slots that started with another one's pages
+        self._grouped: tuple[tuple[int, ...], list] | None = None         # slots of the last ``shared_groups`` and its result, until a slot comes or goes
 
     # ------------------------------------------------------------------ slots
     def alloc(self, prefix_of: int | None = None, tokens: int = 0) -> int:
@@ -69,6 +70,7 @@ class CacheBook:
         if not self._free_slots:
             raise CacheFull(f"all {self.num_slots} sequence slots are in use")
         slot = self._free_slots.pop()
+        self._grouped = None
         entry = self._live[slot] = _Slot(0, [[] for _ in self.groups])
         if source is not None:
             entry.length, entry.shared = tokens, tokens // self.page_tokens
@@ -83,6 +85,7 @@ class CacheBook:
         entry = self._live.pop(slot, None)
         if entry is None:
             raise CacheError(f"slot {slot} is not in use (freed twice, or never allocated)")
+        self._grouped = None
         self._sharers -= entry.shared > 0
         for group, pages in enumerate(entry.pages):
             holders = self._holders[group]
@@ -151,37 +154,93 @@ class CacheBook:
 
     def shared_groups(self, slots: list[int]) -> list[tuple[list[int], int]]:
         """Which of ``slots`` share leading tokens: (places in ``slots``, tokens that all of them hold on the same pages) for every group of two and more, and
-        one group of the rest with 0 tokens, if there is a rest.  Empty where none do."""
+        one group of the rest with 0 tokens, if there is a rest.  Empty where none do.  Where prefixes of prefixes are shared there are several ways to group
+        sequences; the one with the most tokens that members hold beside another one, sum of (members - 1) * tokens, is taken."""
         if not self._sharers or not self.groups:
             return []
-        by_page: dict[int, list[int]] = {}
-        alone: list[int] = []
-        for place, slot in enumerate(slots):
-            pages = self._entry(slot).pages[0]
-            if pages:
-                by_page.setdefault(pages[0], []).append(place)
-            else:
-                alone.append(place)
-        groups = []
-        for places in by_page.values():
-            if len(places) == 1:
-                alone += places
-                continue
-            # A page that two sequences both hold at a place has the same pages in front of it in both.  The pages taken from another sequence are
-            # common to all as a rule (not where that sequence is not among these); what is, lies below that.
-            entries = [self._entry(slots[p]) for p in places]
-            high = common = min(entry.shared for entry in entries if entry.shared)
-            low, first = 1, entries[0].pages[0]
-            while low <= high:
-                if all(len(entry.pages[0]) >= common and entry.pages[0][common - 1] == first[common - 1] for entry in entries):
-                    low = common + 1
+        # pages that a sequence adds as it grows are its own, so that step after step of the same sequences has the same groups
+        if self._grouped is None or self._grouped[0] != tuple(slots):
+            self._grouped = tuple(slots), self._find_groups(slots)
+        return [(list(places), tokens) for places, tokens in self._grouped[1]]
+
+    def _find_groups(self, slots: list[int]) -> list[tuple[list[int], int]]:
+        entries = [self._entry(slot) for slot in slots]
+        pages = [entry.pages[0] for entry in entries]
+        # A tree: a node's places agree on the pages in front of its depth and go apart there, into places by themselves and branches, which are nodes again.
+        # A page that two sequences both hold at a place has the same pages in front of it in both.
+        nodes: list[tuple[int, list[int], list[int], tuple[int, ...]]] = []       # (depth, places by themselves, branches, depths of the nodes above)
+        work = [(-1, list(range(len(slots))))]
+        while work:
+            parent, places = work.pop()
+            depth, above = 0, ()
+            if parent >= 0:
+                depth, above = self._common_pages(entries, places, nodes[parent][0] + 1), (*nodes[parent][3], nodes[parent][0])
+                nodes[parent][2].append(len(nodes))
+            branches: dict[int, list[int]] = {}
+            alone = []
+            for place in places:
+                if len(pages[place]) > depth:
+                    branches.setdefault(pages[place][depth], []).append(place)
                 else:
-                    high = common - 1
-                common = (low + high + 1) // 2 if low <= high else high
-            groups.append((places, common * self.page_tokens))
-        if groups and alone:
-            groups.append((alone, 0))
-        return groups
+                    alone.append(place)
+            for branch in branches.values():
+                if len(branch) == 1:
+                    alone += branch
+                else:
+                    work.append((len(nodes), branch))
+            nodes.append((depth, alone, [], above))
+        # From the leaves on: what a node's places are worth where each may join a group of an upper node's depth, and whether the node has a group of its own
+        # then, which reads its pages once itself.
+        worth: list[dict[int, tuple[int, bool]]] = [{} for _ in nodes]
+        for node in reversed(range(len(nodes))):
+            depth, alone, branches, above = nodes[node]
+
+            def joined(to: int) -> int:
+                return len(alone) * to + sum(worth[branch][to][0] for branch in branches)
+            own = joined(depth) - depth
+            for upper in above or (0,):
+                without = joined(upper)
+                worth[node][upper] = (max(own, without), own > without)
+        members: dict[int, list[int]] = {}
+        work = [(0, -1)]                                          # a node, and the node whose group its places join (-1: none)
+        while work:
+            node, group = work.pop()
+            depth, alone, branches, above = nodes[node]
+            if worth[node][nodes[group][0] if group >= 0 else 0][1]:
+                group = node
+            members.setdefault(group, []).extend(alone)
+            work += [(branch, group) for branch in branches]
+        groups = sorted((sorted(places), nodes[node][0] * self.page_tokens) for node, places in members.items() if node >= 0)
+        if not groups:
+            return []
+        rest = sorted(members.get(-1, ()))
+        return groups + [(rest, 0)] if rest else groups
+
+    @staticmethod
+    def _common_pages(entries: list[_Slot], places: list[int], low: int) -> int:
+        """Leading pages that the sequences at ``places`` all hold, of which the first ``low`` are known to be."""
+        lists = [entries[place].pages[0] for place in places]
+        first, high = lists[0], min(len(pages) for pages in lists)
+
+        def agree(n: int) -> bool:
+            page = first[n - 1]
+            return all(pages[n - 1] == page for pages in lists)
+
+        # what they took from another sequence is common to them all as a rule, and no more
+        guess = min(high, max(low, min((entries[place].shared for place in places if entries[place].shared), default=low)))
+        if not agree(guess):
+            high = guess - 1
+        elif guess == high or not agree(guess + 1):
+            return guess
+        else:
+            low = guess + 1
+        while low < high:
+            middle = (low + high + 1) // 2
+            if agree(middle):
+                low = middle
+            else:
+                high = middle - 1
+        return low
 
     def free_pages(self, group: int) -> int:
         return len(self._free_pages[group])

@@ -195,3 +195,97 @@ def test_uniform_numbers_of_many_rows():
     rows = [(rng.getrandbits(64), rng.randrange(1 << 20), rng.randrange(1 << 16)) for _ in range(200)] + [(0, 0, 0), ((1 << 64) - 1, 5, 7)]
     got = uniforms_for(np.array([r[0] for r in rows], dtype=np.uint64), np.array([r[1] for r in rows]), np.array([r[2] for r in rows]))
     assert got.dtype == np.float32 and got.tolist() == [uniform_for(*r) for r in rows]
+
+
+def worth_of(groups):
+    return sum((len(places) - 1) * tokens for places, tokens in groups if tokens)
+
+
+def test_prefixes_of_prefixes():
+    """A short start that all hold beside long ones that some hold: each sequence is grouped where more is shared."""
+    book = make_book(slots=24, pages=400)
+    deep = book.alloc()
+    book.extend(deep, 3000)
+    drafts = [book.alloc(deep, 2560) for _ in range(4)]
+    assert book.shared_groups([deep, *drafts]) == [([0, 1, 2, 3, 4], 2560)]
+    shallow = book.alloc(deep, 64)                          # one more, that took a page only: the others stay together
+    assert book.shared_groups([deep, shallow, *drafts]) == [([0, 2, 3, 4, 5], 2560), ([1], 0)]
+    also = book.alloc(deep, 64)
+    assert book.shared_groups([also, deep, shallow, *drafts]) == [([0, 2], 64), ([1, 3, 4, 5, 6], 2560)]
+    assert book.shared_groups([deep, shallow]) == [([0, 1], 64)]
+
+
+def test_a_continuation_of_one_of_two_users_behind_a_system_prompt():
+    book = make_book(slots=8, pages=200)
+    system = book.alloc()
+    book.extend(system, 128)
+    users = [book.alloc(system, 128) for _ in range(2)]
+    for user in users:
+        book.extend(user, 2600)
+    continued = [book.alloc(user, 2560) for user in users]
+    assert book.shared_groups([users[0], continued[0]]) == [([0, 1], 2560)]
+    assert book.shared_groups([*users, *continued]) == [([0, 2], 2560), ([1, 3], 2560)]
+    book.free(users[0])
+    assert book.shared_groups([continued[0], users[1], continued[1], system]) == [([0, 3], 128), ([1, 2], 2560)]
+
+
+def test_groups_follow_slots_that_come_and_go():
+    """The same numbers of slots may be other sequences, and what a caller does to a result is its own."""
+    book = make_book(slots=3, pages=60)
+    a = book.alloc()
+    book.extend(a, 200)
+    b, c = book.alloc(a, 192), book.alloc(a, 64)
+    first = book.shared_groups([a, b, c])
+    assert first == [([0, 1], 192), ([2], 0)]
+    first[-1][0].append(7)
+    book.extend(c, 500)
+    assert book.shared_groups([a, b, c]) == [([0, 1], 192), ([2], 0)]
+    book.free(b)
+    book.free(c)
+    assert (book.alloc(), book.alloc(a, 128)) == (c, b)
+    book.extend(c, 100)
+    assert book.shared_groups([a, b, c]) == [([0, 1], 128), ([2], 0)]
+    with pytest.raises(CacheError, match="not in use"):
+        book.free(c)
+        book.shared_groups([a, b, c])
+
+
+def partitions(items):
+    if not items:
+        yield []
+        return
+    first, rest = items[0], items[1:]
+    for partition in partitions(rest):
+        yield [[first], *partition]
+        for i in range(len(partition)):
+            yield [*partition[:i], [first, *partition[i]], *partition[i + 1:]]
+
+
+def test_the_grouping_is_the_best_one():
+    """Random families of up to seven sequences against every way to part them."""
+    rng = random.Random(9)
+    for _ in range(150):
+        book = make_book(slots=8, pages=200)
+        for _ in range(rng.randint(2, 7)):
+            live = [s for s in book.live_slots() if book.length(s) >= 64]
+            if live and rng.random() < 0.85:
+                source = rng.choice(live)
+                slot = book.alloc(source, 64 * rng.randint(1, book.length(source) // 64))
+            else:
+                slot = book.alloc()
+            book.extend(slot, book.length(slot) + rng.randint(0, 400))
+        slots = book.live_slots()
+        rng.shuffle(slots)
+        pages = [book.pages(s, 0) for s in slots]
+
+        def common(places):
+            n = 0
+            while all(len(pages[p]) > n and pages[p][n] == pages[places[0]][n] for p in places):
+                n += 1
+            return 64 * n
+        groups = book.shared_groups(slots)
+        for places, tokens in groups:
+            assert tokens in (0, common(places))
+        most = max(worth_of([(places, common(places)) for places in partition]) for partition in partitions(list(range(len(slots)))))
+        assert worth_of(groups) == most
+        assert not groups or sorted(p for places, _ in groups for p in places) == list(range(len(slots)))
