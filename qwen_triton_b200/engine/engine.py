@@ -27,7 +27,7 @@ from ..ops import kernels
 from ..parts.base import Runtime, Workspace
 from ..weights import open_checkpoint, random_source
 from .model import CausalLM, expected_tensors
-from .step import StepContext, StepEntry, plan_passes, shared_shape
+from .step import StepContext, StepEntry, plan_passes, shared_shape, tokens_not_again
 
 _DTYPES = {
     "bf16": torch.bfloat16, "bfloat16": torch.bfloat16, "fp32": torch.float32, "float32": torch.float32,
@@ -368,15 +368,20 @@ class Engine:
         context = -(-(max(past) + 1) // 1024) * 1024
         pad = padded - count
         groups, shape = book.shared_groups(slots), None
+        # a shape of groups only where some layer takes it: every shape is a graph of its own
+        pays = tuple(kind for kind in sorted(self.runtime.options.get("shared_attention", ()))
+                     if kernels.sharing_pays(tokens_not_again(groups), *kind, self.dtype, self.page_tokens)) if groups else ()
+        if not pays:
+            groups = []
         if groups:
             if pad:                                              # padded rows: one token of their own
                 if groups[-1][1]:
                     groups.append(([], 0))
                 groups[-1][0].extend(range(count, padded))
             shape = shared_shape(groups, [p + 1 for p in past] + [1] * pad)
-        prepared = self._ctx.prepare_decode(slots + [cache.dummy_slot] * pad, past + [0] * pad, tables, groups, shape)
+        prepared = self._ctx.prepare_decode(slots + [cache.dummy_slot] * pad, past + [0] * pad, tables, groups, shape, pays)
         return PlannedDecode(slots=tuple(slots), lengths=tuple(p + 1 for p in past), count=count, padded=padded,
-                             key=(padded, tuple(widths), context, shape), context=context, prepared=prepared)
+                             key=(padded, tuple(widths), context, shape, pays), context=context, prepared=prepared)
 
     def _run_planned(self, plan: "PlannedDecode", tokens: list[int], chosen: torch.Tensor | None = None) -> torch.Tensor:
         cache, count, padded = self.cache, plan.count, plan.padded

@@ -52,7 +52,8 @@ def plan_passes(lengths: list[int], max_tokens: int, chunk_limit: int | None) ->
 @dataclass(frozen=True)
 class SharedPrefixes:
     """Sequences of a one-token pass that hold the same leading pages, as ``kernels.attention_decode_shared`` takes them.  ``groups``, ``most_members``,
-    ``most_shared`` and ``most_own`` are the sizes its plan is made for: limits of what the arrays hold, rounded up so that few shapes arise."""
+    ``most_shared`` and ``most_own`` are the sizes its plan is made for: limits of what the arrays hold, rounded up so that few shapes arise.  ``pays``: the
+    kinds of attention, (query heads, kv heads, elements of a head), that take it for this pass."""
 
     members: torch.Tensor       # int32 [sequences]
     share: torch.Tensor         # int32 [groups, 3]
@@ -60,18 +61,24 @@ class SharedPrefixes:
     most_members: int
     most_shared: int
     most_own: int
+    pays: tuple[tuple[int, int, int], ...]
 
 
 def shared_shape(groups: list[tuple[list[int], int]], lengths: list[int]) -> tuple[int, int, int, int]:
-    """(groups, members, shared tokens, own tokens) at most, rounded up: groups and members to powers of two, shared tokens to a power of two from 64 to
-    1,024 and to multiples of that beyond, own ones to a power of two from 64 on."""
+    """(groups, members of one that shares, shared tokens, own tokens) at most, rounded up: groups and members to powers of two, shared tokens to a power of two
+    from 64 to 1,024 and to multiples of that beyond, own ones to a power of two from 64 on."""
     def power(n: int, least: int = 1) -> int:
         while least < n:
             least *= 2
         return least
     own = max(lengths[p] - shared for places, shared in groups for p in places)
     most = max(shared for _, shared in groups)
-    return (power(len(groups)), power(max(len(places) for places, _ in groups)), power(most, 64) if most <= 1024 else -(-most // 1024) * 1024, power(own, 64))
+    return (power(len(groups)), power(max((len(places) for places, shared in groups if shared), default=0)), power(most, 64) if most <= 1024 else -(-most // 1024) * 1024, power(own, 64))
+
+
+def tokens_not_again(groups: list[tuple[list[int], int]]) -> int:
+    """Tokens whose keys and values are not read again where each group's shared ones are read once."""
+    return sum((len(places) - 1) * shared for places, shared in groups if places)
 
 
 class StepContext:
@@ -142,17 +149,17 @@ class StepContext:
         self.from_start = not past_arr.any()
 
     # ------------------------------------------------------------------ one token per sequence
-    def prepare_decode(self, slots: list[int], past: list[int], tables: list[np.ndarray], groups=(), shape=None):
+    def prepare_decode(self, slots: list[int], past: list[int], tables: list[np.ndarray], groups=(), shape=None, pays=()):
         """The part of ``fill`` for a pass of one token per sequence (every row wanted) that does not need the
         tokens: the same layout at the same addresses, written into pinned buffers that are kept (a small ring,
         each guarded by an event, so that a caller who runs ahead of the device cannot overwrite a copy that has
         not happened yet) with the parts that never change filled in once.  Returns what ``commit_decode`` takes.  ``groups``: the places that share leading
-        tokens (``CacheBook.shared_groups``), with their ``shared_shape``."""
+        tokens (``CacheBook.shared_groups``), with their ``shared_shape`` and the kinds of attention that read them together."""
         n = len(slots)
-        key = (n, tuple(t.shape[1] for t in tables), shape)
+        key = (n, tuple(t.shape[1] for t in tables), shape, pays)
         plan = self._decode_plans.get(key)
         if plan is None:
-            plan = self._decode_plans[key] = _DecodePlan(self._meta, n, key[1], shape)
+            plan = self._decode_plans[key] = _DecodePlan(self._meta, n, key[1], shape, pays)
         host, array, event = plan.next_buffer()
         array[2 * n:3 * n] = past
         array[plan.at_past:plan.at_past + n] = past
@@ -211,7 +218,7 @@ class _DecodePlan:
 
     RING = 4
 
-    def __init__(self, meta: torch.Tensor, n: int, widths: tuple[int, ...], shape: tuple[int, int, int, int] | None = None) -> None:
+    def __init__(self, meta: torch.Tensor, n: int, widths: tuple[int, ...], shape: tuple[int, int, int, int] | None = None, pays=()) -> None:
         self.n = n
         sizes = [n, n, n, n + 1, n, n, n, n] + [n * w for w in widths]
         offsets = np.concatenate(([0], np.cumsum(sizes))).tolist()
@@ -227,7 +234,7 @@ class _DecodePlan:
         self.views = [meta[offsets[i]:offsets[i + 1]] for i in range(len(sizes))]
         self.tables = {g: self.views[8 + g].view(n, w) for g, w in enumerate(widths)}
         self.order = meta[self.at_order:self.at_members].view(n, 2) if ordered else None
-        self.shared = SharedPrefixes(meta[self.at_members:self.at_share], meta[self.at_share:self.total].view(shape[0], 3), *shape) if shape else None
+        self.shared = SharedPrefixes(meta[self.at_members:self.at_share], meta[self.at_share:self.total].view(shape[0], 3), *shape, pays) if shape else None
         self.buffers = []
         for _ in range(self.RING):
             host = torch.zeros(self.total, dtype=torch.int32, pin_memory=True)

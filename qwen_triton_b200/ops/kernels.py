@@ -1452,8 +1452,8 @@ def _shared_on_tc(dtype: torch.dtype, head_dim: int, page_tokens: int) -> bool:
 
 def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, groups: int, most_members: int,
                 most_shared: int, most_own: int, sms: int | None = None, most_ranges: int = 64, page_tokens: int = 64) -> SharedPlan:
-    """The cut for ``n_seqs`` sequences in ``groups`` groups of at most ``most_members``, a shared length of at most ``most_shared`` tokens and at most
-    ``most_own`` tokens of a member's own.  ``sms``: streaming multiprocessors (default: the current device's); ``most_ranges``: of a row, 2 to 64 (scratch is
+    """The cut for ``n_seqs`` sequences in ``groups`` groups, those that share of at most ``most_members``, a shared length of at most ``most_shared`` tokens and
+    at most ``most_own`` tokens of a member's own.  ``sms``: streaming multiprocessors (default: the current device's); ``most_ranges``: of a row, 2 to 64 (scratch is
     by ranges); ``page_tokens``: of the cache."""
     if n_seqs < 0 or groups < 1 or not 0 <= most_members <= n_seqs or most_shared < 0 or most_own < 0:
         raise KernelError(f"shared_plan: {n_seqs} sequences in {groups} groups of at most {most_members}, {most_shared} and {most_own} tokens")
@@ -1507,14 +1507,24 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
     return SharedPlan(n_seqs, num_heads, num_kv_heads, head_dim, dtype, groups, most_members, shared_ranges, own_ranges, page_tokens)
 
 
-SHARING_PAYS = 56 << 20       # keys and values, in bfloat16's bytes, that are not read again
+SHARING_PAYS = 50 << 20       # bytes of keys and values that are not read again: on the tensor cores
+SHARING_PAYS_MORE = 6 << 20   # and as many more for each query head of a kv head beyond four
+SHARING_PAYS_FLOAT = 1 << 20  # in float32
 
 
-def sharing_pays(most_members: int, most_shared: int, num_kv_heads: int, head_dim: int) -> bool:
-    """Whether a one-token step is faster by ``attention_decode_shared`` than by ``attention_decode``: by what the other members would read again.  32 heads over 8
-    of 128, microseconds, one / the other: 16 sequences of 512 shared and 64 own tokens 9.5 / 12.7, of 1,024 14.1 / 13.2, of 4,096 39 / 17; 8 of 1,024 11.5 / 12.2,
-    of 2,048 15.8 / 12.8, of 16,384 71 / 29; 2 of 4,096 12.1 / 18.2, of 16,384 29 / 26; 64 of 16,384 480 / 39."""
-    return (most_members - 1) * most_shared * num_kv_heads * head_dim * 4 >= SHARING_PAYS
+def sharing_pays(not_again: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, page_tokens: int = 64) -> bool:
+    """Whether a one-token step is faster by ``attention_decode_shared`` than by ``attention_decode``.  ``not_again``: tokens whose keys and values are not read
+    again, the sum over the groups of (members - 1) times shared.
+
+    Tensor cores, one / the other form's microseconds behind a cold cache (32 heads over 8 of 128): 2 sequences of 4,096 shared tokens 14 / 17, 8 of 1,024
+    13 / 13, of 2,048 18 / 14, 64 of 16,384 483 / 42; 8 that share 4,096 beside 56 of 6,000 243 / 255, 32 beside 32 of 3,000 135 / 100.  16 heads over one of
+    128, whose join has few blocks: 16 of 8,192 28 / 36, 64 of 4,096 34 / 31.  Over 271 batches of 17 head shapes what it takes is 1.8 % slower than the
+    faster one on the average.  Float32 heads up to 128: faster at all of 32 batches, 1.02 to 2.7 times, from 1 MB on.  Other sizes on the FMA pipe: slower at
+    27 of 40, up to 2.3 times, and left to ``attention_decode``."""
+    saved = not_again * num_kv_heads * head_dim * 2 * dtype.itemsize
+    if _shared_on_tc(dtype, head_dim, page_tokens):
+        return saved >= SHARING_PAYS + max(0, num_heads // num_kv_heads - 4) * SHARING_PAYS_MORE
+    return dtype == torch.float32 and head_dim <= 128 and saved >= SHARING_PAYS_FLOAT
 
 
 def _check_shared(q, k_cache, v_cache, out, block_table, seq_len, members, share, num_kv_heads, page_tokens, plan, part_acc, part_ml) -> None:

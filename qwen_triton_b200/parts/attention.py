@@ -166,6 +166,11 @@ class Attention:
         self.side_name = "attn.values." + str(params.get("v_blend_key", "first"))
         if self.v_blend is not None:
             ws.declare(self.side_name, runtime.max_step_tokens * self.nkv * self.dv, torch.float32)
+        # whether a one-token step may read what sequences share once; the engine asks about every kind that does
+        self.takes_shared = not (self.window or self.penalised or self.chunk or self.keep_first or self.sink or self.softcap is not None or self.dv != self.d
+                                 or self.v_heads != self.nkv or self.scale <= 0)
+        if self.takes_shared:
+            runtime.options.setdefault("shared_attention", set()).add((self.nq, self.nkv, self.d))
         # few tokens: the projection takes rows whose norm factor is still to be applied (``ScaledRows``)
         self.takes_scaled_rows = self.qkv.fused_capable and not self.own_values
 
@@ -343,10 +348,7 @@ class Attention:
         """The plan for sequences that share leading pages, or None where ``attention_decode`` takes them: attention with anything beyond a scale, more rows than
         the scratch holds ranges of, or too little shared for it to pay."""
         shared = ctx.shared
-        if (self.window or self.penalised or self.chunk or self.keep_first or self.sink or self.softcap is not None or self.dv != self.d
-                or self.v_heads != self.nkv or cache.ring_tokens or self.scale <= 0 or ctx.n_seqs * 2 > _MAX_SPLIT_PAIRS):
-            return None
-        if not kernels.sharing_pays(min(shared.most_members, ctx.n_seqs), shared.most_shared, self.nkv, self.d):
+        if not self.takes_shared or (self.nq, self.nkv, self.d) not in shared.pays or cache.ring_tokens or ctx.n_seqs * 2 > _MAX_SPLIT_PAIRS:
             return None
         return kernels.shared_plan(ctx.n_seqs, num_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.d, dtype=self.runtime.dtype, groups=shared.groups,
                                    most_members=min(shared.most_members, ctx.n_seqs), most_shared=shared.most_shared, most_own=shared.most_own,

@@ -1,0 +1,91 @@
+"""One-token steps over shared pages as the engine runs them: launched, captured and replayed, by the form that a step takes for itself."""
+from __future__ import annotations
+
+import dataclasses
+
+import pytest
+import torch
+
+from gpu_util import assert_close, make_engine, plain_logits, random_tokens
+from qwen_triton_b200 import Engine, StepEntry, load_preset
+from qwen_triton_b200.ops import kernels
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def plans(monkeypatch):
+    """The plans of the shared calls that steps make."""
+    seen = []
+    real = kernels.attention_decode_shared
+    monkeypatch.setattr(kernels, "attention_decode_shared", lambda *args: (seen.append(args[11]), real(*args))[1])
+    return seen
+
+
+@pytest.mark.parametrize("preset", ("tiny-a", "tiny-b", "tiny-d"))
+def test_two_launches_in_a_captured_step(preset, plans, monkeypatch):
+    """bfloat16 on the tensor cores, small sizes made to take the form of large ones: two groups and one sequence in seven rows, padded to eight."""
+    monkeypatch.setattr(kernels, "sharing_pays", lambda *args: True)
+    monkeypatch.setattr(kernels, "DIRECT_BYTES", 0)
+    engine = make_engine(preset, "bf16", max_tokens=4096)
+    prompts = [random_tokens(preset, 300, 1), random_tokens(preset, 70, 2), random_tokens(preset, 33, 3)]
+    first = [engine.new_sequence() for _ in prompts]
+    engine.step([StepEntry(s, p, []) for s, p in zip(first, prompts)])
+    history = {s: list(p) for s, p in zip(first, prompts)}
+    for source, tokens in ((0, 256), (0, 256), (0, 192), (1, 64)):
+        history[engine.new_sequence(first[source], tokens)] = prompts[source][:tokens]
+    order = [first[1], *[s for s in history if s not in first], first[0], first[2]]
+    assert len(order) == 7
+    for step in range(5):
+        tokens = [random_tokens(preset, 1, 100 * step + i)[0] for i in range(len(order))]
+        logits = engine.step([StepEntry(s, [t], [0]) for s, t in zip(order, tokens)]).cpu()
+        for row, (slot, token) in enumerate(zip(order, tokens)):
+            history[slot].append(token)
+            assert_close(logits[row:row + 1], plain_logits(preset, "bf16", history[slot])[-1:], "bf16", f"{preset} step {step} row {row}")
+    assert plans and all(plan.shared_ranges > 0 for plan in plans)
+    assert engine.graph_replays >= 3
+    engine.check_kernels()
+
+
+def steps_of(engine, shared, members, alone, steps=4):
+    """Logits of ``steps`` steps of ``members`` sequences that took ``shared`` tokens of the first, and of ``alone`` more by themselves."""
+    preset = "tiny-d"
+    first = engine.new_sequence()
+    engine.step([StepEntry(first, random_tokens(preset, shared + 5, 1), [])])
+    slots = [first] + [engine.new_sequence(first, shared) for _ in range(members - 1)]
+    apart = [engine.new_sequence() for _ in range(alone)]
+    if apart:
+        engine.step([StepEntry(s, random_tokens(preset, 90 + i, 2 + i), []) for i, s in enumerate(apart)])
+    out = []
+    for step in range(steps):
+        entries = [StepEntry(s, [random_tokens(preset, 1, 1000 * step + i)[0]], [0]) for i, s in enumerate(slots + apart)]
+        out.append(engine.step(entries).cpu())
+    shape = engine._plan_decode(slots + apart, True).key[3]
+    for slot in slots + apart:
+        engine.release(slot)
+    engine.check_kernels()
+    return out, shape
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, dim, shared, members, alone", [
+    ("bf16", 5, 5, 64, 1920, 32, 0), ("bf16", 5, 5, 64, 1920, 30, 6), ("bf16", 8, 4, 128, 1856, 16, 3), ("fp32", 5, 5, 64, 1920, 32, 3), ("fp32", 4, 2, 128, 512, 3, 2)])
+def test_a_step_shares_of_itself_where_it_pays(dtype, heads, kv_heads, dim, shared, members, alone, plans, monkeypatch):
+    """The rule as it is: the step takes the shared form in two launches, and gives what it gives without."""
+    config = dataclasses.replace(load_preset("tiny-d"), num_attention_heads=heads, num_key_value_heads=kv_heads, head_dim=dim)
+    engine = Engine.from_config(config, seed=4, dtype=dtype, max_tokens=8192)
+    got, shape = steps_of(engine, shared, members, alone)
+    assert shape is not None and plans and all(plan.shared_ranges > 0 and plan.head_dim == dim for plan in plans)
+    count = len(plans)
+    monkeypatch.setattr(kernels, "sharing_pays", lambda *args: False)
+    want, shape = steps_of(engine, shared, members, alone)
+    assert shape is None and len(plans) == count
+    for step, (a, b) in enumerate(zip(got, want)):
+        assert_close(a, b, dtype, f"step {step}")
+
+
+@pytest.mark.parametrize("shared, members, alone", [(64, 2, 14), (1920, 2, 30), (1920, 8, 56)])
+def test_a_step_that_shares_little_is_a_step_like_any_other(shared, members, alone, plans):
+    """No shared call, and no shape of groups under which a graph of its own would be kept."""
+    engine = make_engine("tiny-d", "bf16", max_tokens=16384)
+    _, shape = steps_of(engine, shared, members, alone, steps=2)
+    assert shape is None and not plans

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from qwen_triton_b200.engine.step import shared_shape, tokens_not_again
 from qwen_triton_b200.ops import kernels
 from qwen_triton_b200.ops.kernels import KernelError
 
@@ -38,3 +39,41 @@ def test_there_is_no_host_path():
     with pytest.raises(KernelError, match="host"):
         f = torch.zeros(1)
         kernels.sample_filtered(torch.zeros((1, 5)), f, one, f, f, f, one)
+
+
+def pays(groups, heads=32, kv_heads=8, dim=128, dtype=torch.bfloat16, page=64):
+    return kernels.sharing_pays(tokens_not_again(groups), heads, kv_heads, dim, dtype, page)
+
+
+def test_what_is_not_read_again_decides():
+    """Of each group by itself, whatever else is in the batch: 50 MB of keys and values, 4,096 bytes a token at these sizes."""
+    def rest(first, count):
+        return list(range(first, first + count)), 0
+    assert tokens_not_again([([0, 2, 3], 192), ([1], 0)]) == 384
+    assert tokens_not_again([(list(range(8)), 2048), ([8, 9], 64), rest(10, 6)]) == 7 * 2048 + 64
+    assert tokens_not_again([([0, 1], 640), ([], 0)]) == 640
+    assert not pays([([0, 1], 64), rest(2, 254)])               # 256 KB
+    assert not pays([([0, 1], 512), rest(2, 62)])
+    assert not pays([([0, 1], 4096), rest(2, 60)])              # 16 MB
+    assert not pays([([0, 1], 64)] * 32 + [rest(64, 192)])
+    assert pays([([0, 1], 16384)]) and pays([([0, 1], 16384), rest(2, 254)])
+    assert pays([(list(range(8)), 2048)]) and not pays([(list(range(8)), 1024)])
+    assert pays([(list(range(4 * g, 4 * g + 4)), 1100) for g in range(4)])     # 13,200 tokens over four groups
+    assert not pays([(list(range(17)), 4096)], heads=16, kv_heads=1)           # 32 MB; sixteen heads to a kv head want 122
+    assert pays([(list(range(64)), 4096)], heads=16, kv_heads=1)
+
+
+def test_the_kernel_that_would_run_decides():
+    many = [(list(range(64)), 16384)]
+    assert pays(many) and pays(many, heads=5, kv_heads=5, dim=64) and pays(many, heads=6, kv_heads=3, dim=40)
+    for sizes in (dict(dim=256), dict(dim=160), dict(dim=20), dict(page=16), dict(dim=256, dtype=torch.float32)):
+        assert not pays(many, **sizes)
+    few = [([0, 1], 256)]                                       # 2 MB of float32
+    assert pays(few, dtype=torch.float32) and pays(few, dtype=torch.float32, page=16) and not pays(few)
+    assert not pays([([0, 1], 64)], dtype=torch.float32)
+
+
+def test_shapes_leave_out_what_shares_nothing():
+    """The most members are of a group that shares, so that sequences beside it do not widen the plan."""
+    lengths = [5000] * 2 + [300] * 62
+    assert shared_shape([([0, 1], 4096), (list(range(2, 64)), 0)], lengths) == (2, 2, 4096, 1024)
