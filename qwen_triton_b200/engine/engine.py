@@ -20,7 +20,7 @@ from typing import Sequence
 import numpy as np
 import torch
 
-from ..cache import SequenceCache
+from ..cache import CacheError, SequenceCache
 from ..config import load_config
 from ..config.spec import ModelSpec
 from ..ops import kernels
@@ -107,6 +107,7 @@ class Engine:
         self._graphs: OrderedDict[tuple, object] = OrderedDict()
         self.max_graphs = max(1, int(max_graphs))
         self._graph_logits: torch.Tensor | None = None
+        self._planned: set[int] = set()          # sequences whose last position is planned and has not run
         self._status_host = torch.zeros(4, dtype=torch.int32, pin_memory=True)
         self._status_event: torch.cuda.Event | None = None
         self.max_graph_batch = max_graph_batch
@@ -166,16 +167,21 @@ class Engine:
 
     def new_sequence(self, prefix_of: int | None = None, tokens: int | None = None) -> int:
         """Take a slot for a sequence that starts at position 0, or with the first ``tokens`` (whole pages; default: all of its whole pages) of the sequence in
-        ``prefix_of``, whose keys and values it then shares.  Sequences that share their first pages are read together in one-token steps."""
+        ``prefix_of``, whose keys and values it then shares.  Sequences that share their first pages are read together in one-token steps.  A position that is
+        planned (``plan_decode``) and has not run yet has no keys and values to share."""
         if prefix_of is None:
             return self.cache.alloc()
+        length = self.length(prefix_of) - (prefix_of in self._planned)
         if tokens is None:
-            tokens = self.length(prefix_of) // self.page_tokens * self.page_tokens
+            tokens = length // self.page_tokens * self.page_tokens
+        elif tokens > length:
+            raise CacheError(f"slot {prefix_of}: {tokens} tokens of which {length} have run")
         return self.cache.alloc(prefix_of, tokens)
 
     def release(self, slot: int) -> None:
         """Give back the slot and every page the sequence holds."""
         self.cache.free(slot)
+        self._planned.discard(slot)
 
     def length(self, slot: int) -> int:
         return self.cache.book.length(slot)
@@ -353,6 +359,7 @@ class Engine:
             past = [book.length(s) for s in slots]
             for slot, before in zip(slots, past):
                 book.extend(slot, before + 1)
+            self._planned.update(slots)
         else:
             past = [book.length(s) - 1 for s in slots]
         widths, tables = [], []
@@ -386,6 +393,7 @@ class Engine:
     def _run_planned(self, plan: "PlannedDecode", tokens: list[int], chosen: torch.Tensor | None = None) -> torch.Tensor:
         cache, count, padded = self.cache, plan.count, plan.padded
         fill = -1 if chosen is not None else 0                  # padded rows: token 0 either way
+        self._planned.difference_update(plan.slots)
         self._ctx.commit_decode(plan.prepared, tokens + [fill] * (padded - count), plan.context, chosen, self.spec.vocab_size)
         self.last_meta_bytes = self._ctx.meta_bytes
         key = plan.key

@@ -8,6 +8,7 @@ import torch
 
 from gpu_util import assert_close, make_engine, plain_logits, random_tokens
 from qwen_triton_b200 import Engine, StepEntry, load_preset
+from qwen_triton_b200.cache import CacheError
 from qwen_triton_b200.ops import kernels
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +90,35 @@ def test_a_step_that_shares_little_is_a_step_like_any_other(shared, members, alo
     engine = make_engine("tiny-d", "bf16", max_tokens=16384)
     _, shape = steps_of(engine, shared, members, alone, steps=2)
     assert shape is None and not plans
+
+
+def test_a_position_that_is_planned_and_has_not_run_is_not_shared():
+    """Its keys and values are not there yet."""
+    engine = make_engine("tiny-d", "fp32")
+    prompt = random_tokens("tiny-d", 127, 5)
+    slot = engine.new_sequence()
+    engine.step([StepEntry(slot, prompt, [])])
+    plan = engine.plan_decode([slot])
+    assert engine.length(slot) == 128
+    with pytest.raises(CacheError, match="127 have run"):
+        engine.new_sequence(slot, 128)
+    early = engine.new_sequence(slot)
+    assert engine.length(early) == 64
+    plan = engine.plan_decode([slot], extend=False)               # planned again: still not run
+    with pytest.raises(CacheError, match="127 have run"):
+        engine.new_sequence(slot, 128)
+    token = random_tokens("tiny-d", 1, 6)
+    engine.run_planned(plan, token)
+    late = engine.new_sequence(slot)
+    assert engine.length(late) == 128
+    logits = engine.step([StepEntry(early, prompt[64:100], [35]), StepEntry(late, [7, 9], [1])])
+    assert_close(logits[:1], plain_logits("tiny-d", "fp32", prompt[:100])[-1:], "fp32", "taken before the step")
+    assert_close(logits[1:], plain_logits("tiny-d", "fp32", prompt + token + [7, 9])[-1:], "fp32", "taken behind it")
+    for s in (slot, early, late):
+        engine.release(s)
+    engine.plan_decode([again := engine.new_sequence()])
+    engine.release(again)                                         # a slot's next sequence has nothing of a plan that never ran
+    slot = engine.new_sequence()
+    engine.step([StepEntry(slot, prompt[:64], [])])
+    assert engine.length(engine.new_sequence(slot)) == 64
+    engine.cache.book.check()
