@@ -99,8 +99,12 @@ class BatchRun:
         self.engine, self.sampler = engine, sampler
         self.shared_tokens = shared_tokens
         self.prompts, self.results = prompts, results
-        self.max_new_tokens, self.sampling, self.stop = max_new_tokens, sampling, stop
         self.active = list(indices)
+        if not isinstance(sampling, SamplingParams):
+            of_batch = [sampling[i] for i in self.active]
+            if of_batch and all(p == of_batch[0] for p in of_batch):
+                sampling = of_batch[0]
+        self.max_new_tokens, self.sampling, self.stop = max_new_tokens, sampling, stop
         self.slot_of: dict[int, int] = {}
         self._entries: list[StepEntry] = []
         self._plan = None           # the next one-token step, prepared while the device ran the last one

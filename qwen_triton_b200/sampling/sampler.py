@@ -159,7 +159,8 @@ class Sampler:
 
     def launch(self, logits: torch.Tensor, params: "SamplingParams | list[SamplingParams]", requests: list[int], steps: list[int]) -> PendingTokens:
         """Start the choice and the copy of the ids to pinned host memory; the caller may do other work before
-        it asks the returned object for the tokens.  ``params``: for all rows, or one for each."""
+        it asks the returned object for the tokens.  ``params``: for all rows, or one for each; rows with their own are chosen by the kernel for filters
+        even where they are alike, so that no row's choice depends on which others are still there."""
         rows = logits.shape[0]
         if rows != len(requests) or rows != len(steps):
             raise ValueError("one request index and one step number per logits row")
@@ -167,9 +168,9 @@ class Sampler:
             params = list(params)
             if len(params) != rows:
                 raise ValueError(f"{len(params)} sampling parameters for {rows} rows")
-            if any(p != params[0] for p in params) or (params and (params[0].min_p > 0 or params[0].logprobs)):
+            if params:
                 return self._launch_filtered(logits, params, requests, steps)
-            params = params[0] if params else SamplingParams()
+            params = SamplingParams()
         if params.min_p > 0 or params.logprobs:
             return self._launch_filtered(logits, [params] * rows, requests, steps)
         out = torch.empty(rows, dtype=torch.int32, device=self.device)

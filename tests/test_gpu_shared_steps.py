@@ -122,3 +122,24 @@ def test_a_position_that_is_planned_and_has_not_run_is_not_shared():
     engine.step([StepEntry(slot, prompt[:64], [])])
     assert engine.length(engine.new_sequence(slot)) == 64
     engine.cache.book.check()
+
+
+def test_a_batch_keeps_its_kernel_while_requests_end(monkeypatch):
+    """Rows with parameters of their own go through one kernel, also when those that are left are alike."""
+    from qwen_triton_b200 import SamplingParams
+    from qwen_triton_b200.sampling.sampler import Sampler
+    calls = []
+    for name in ("argmax", "sample_keyed", "sample_filtered"):
+        real = getattr(kernels, name)
+        monkeypatch.setattr(kernels, name, lambda *args, _name=name, _real=real: (calls.append(_name), _real(*args))[1])
+    logits = torch.randn((3, 500), generator=torch.Generator().manual_seed(1)).cuda()
+    sampler = Sampler(torch.device("cuda:0"))
+    alike, other = SamplingParams(temperature=0.8, top_p=0.9), SamplingParams()
+    sampler.sample(logits, [alike, other, alike], [0, 1, 2], [0] * 3)
+    sampler.sample(logits[:2], [alike, alike], [0, 2], [1] * 2)
+    sampler.sample(logits[:1], [other], [1], [1])
+    assert calls == ["sample_filtered"] * 3
+    sampler.sample(logits, alike, [0, 1, 2], [0] * 3)               # one for all rows: as without a list
+    sampler.sample(logits, other, [0, 1, 2], [0] * 3)
+    assert calls[3:] == ["sample_keyed", "argmax"]
+    assert sampler.sample(logits[:0], [], [], []) == []

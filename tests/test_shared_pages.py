@@ -289,3 +289,22 @@ def test_the_grouping_is_the_best_one():
         most = max(worth_of([(places, common(places)) for places in partition]) for partition in partitions(list(range(len(slots)))))
         assert worth_of(groups) == most
         assert not groups or sorted(p for places, _ in groups for p in places) == list(range(len(slots)))
+
+
+def test_requests_that_are_alike_are_one_kind():
+    """A list of equal parameters is the same call as one for all; a list that differs stays a list to the end."""
+    class Sampler:
+        def __init__(self):
+            self.seen = []
+
+        def sample(self, logits, params, requests, steps):
+            self.seen.append(params)
+            return logits.argmax(dim=-1).tolist()
+
+    one = SamplingParams(temperature=0.5, seed=3)
+    sampler = Sampler()
+    generate(ScriptedEngine(), [[1], [2], [3]], max_new_tokens=2, sampling=[SamplingParams(temperature=0.5, seed=3) for _ in range(3)], sampler=sampler)
+    assert sampler.seen and all(params == one for params in sampler.seen)
+    sampler = Sampler()
+    generate(ScriptedEngine(), [[46], [10], [20]], max_new_tokens=4, sampling=[SamplingParams(), one, one], sampler=sampler)
+    assert sampler.seen[0] == [SamplingParams(), one, one] and sampler.seen[-1] == [one, one]      # the first ends early
