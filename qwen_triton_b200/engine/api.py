@@ -111,13 +111,15 @@ class QwenB200ForCausalLM:
     @torch.no_grad()
     def continuations(self, prompt: Sequence[int], n: int, max_new_tokens: int = 16, temperature: float = 1.0, seed: int = 0,
                       stop_token_ids: Sequence[int] | None = None, ignore_eos: bool = False, top_k: int = 0, top_p: float = 1.0,
-                      min_p: float = 0.0) -> list[GenerationResult]:
-        """``n`` continuations of one prompt, the likeliest first (by the mean log-probability of their tokens as they were drawn).  The prompt's whole pages run
-        and are held once, and every step reads them once for all continuations, where the model's cache is pages of all positions."""
+                      min_p: float = 0.0, max_batch_size: int | None = None) -> list[GenerationResult]:
+        """``n`` continuations of one prompt, the likeliest first: by the mean log-probability with which their tokens were drawn, that is under the temperature and
+        the filters of the call (where these leave one token, every mean is 0).  The prompt's whole pages run and are held once a batch, where the model's
+        cache is pages of all positions, and steps read them once for all continuations where that is faster."""
         if n < 1:
             raise ValueError(f"{n} continuations")
         results = self.generate([list(prompt)] * n, max_new_tokens=max_new_tokens, temperature=temperature, seed=seed, stop_token_ids=stop_token_ids,
-                                ignore_eos=ignore_eos, top_k=top_k, top_p=top_p, min_p=min_p, logprobs=True, share_prefix=True)
+                                ignore_eos=ignore_eos, max_batch_size=max_batch_size, top_k=top_k, top_p=top_p, min_p=min_p, logprobs=True,
+                                share_prefix=True)
         return sorted(results, key=lambda r: -sum(r.logprobs) / max(1, len(r.logprobs)))
 
     def start_batch(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 16, temperature: float = 0.0,

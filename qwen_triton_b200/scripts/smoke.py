@@ -109,7 +109,7 @@ def main(argv=None) -> None:
     if args.samples > 1:
         several = [model.continuations(prompt, args.samples, max_new_tokens=args.max_new_tokens, temperature=args.temperature, seed=sampling_seed,
                                        stop_token_ids=_ids(args.stop_ids, "--stop-ids"), ignore_eos=args.ignore_eos, top_k=args.top_k,
-                                       top_p=args.top_p, min_p=args.min_p) for prompt in prompts]
+                                       top_p=args.top_p, min_p=args.min_p, max_batch_size=args.max_batch_size) for prompt in prompts]
         prompts = [prompt for prompt in prompts for _ in range(args.samples)]
         results = [result for of_prompt in several for result in of_prompt]
     else:

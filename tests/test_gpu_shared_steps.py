@@ -143,3 +143,16 @@ def test_a_batch_keeps_its_kernel_while_requests_end(monkeypatch):
     sampler.sample(logits, other, [0, 1, 2], [0] * 3)
     assert calls[3:] == ["sample_keyed", "argmax"]
     assert sampler.sample(logits[:0], [], [], []) == []
+
+
+def test_the_command_keeps_its_batch_size(monkeypatch, capsys):
+    import importlib
+    loop = importlib.import_module("qwen_triton_b200.engine.generate")
+    from qwen_triton_b200.scripts import smoke
+    batches = []
+    real = loop.BatchRun
+    monkeypatch.setattr(loop, "BatchRun", lambda *args, **kw: (batches.append(list(args[4])), real(*args, **kw))[1])
+    smoke.main(["--preset", "tiny-b", "--random-weights", "--random-prompts", "150", "--samples", "5", "--max-batch-size", "2", "--temperature", "0.8",
+                "--max-new-tokens", "3", "--ignore-eos"])
+    assert batches == [[0, 1], [2, 3], [4]]
+    assert sum(line.startswith("generated=") for line in capsys.readouterr().out.splitlines()) == 5
