@@ -9,7 +9,7 @@ accepted and has no effect: every kernel failure raises here.
 
 Added: a model without a folder (``--preset NAME --random-weights``), prompts as token ids
 (``--prompt-ids 1,2,3``, repeatable: a batch of unequal prompts) or random (``--random-prompts 5,9,17``),
-``--temperature``, ``--seed`` (the seed of everything the run draws: sampling, random weights, random
+``--temperature`` (0, or 1 with ``--samples``), ``--seed`` (the seed of everything the run draws: sampling, random weights, random
 prompts; ``--sampling-seed`` and ``--weights-seed`` set one of them apart), ``--stop-ids``,
 ``--ignore-eos``, ``--min-p``, ``--samples`` (continuations of every prompt, ranked), ``--max-tokens`` (cache size), ``--max-seq-len``, ``--max-batch-size``.
 """
@@ -32,11 +32,11 @@ def _parse_args(argv=None) -> argparse.Namespace:
                         help="comma-separated token ids; repeat for a batch of unequal prompts")
     parser.add_argument("--random-prompts", default=None, help="comma-separated lengths of prompts of uniform random token ids")
     parser.add_argument("--max-new-tokens", type=int, default=8)
-    parser.add_argument("--temperature", type=float, default=0.0)
+    parser.add_argument("--temperature", type=float, default=None, help="default: 0, the likeliest token; 1 with --samples")
     parser.add_argument("--top-k", type=int, default=0, help="with --temperature: draw from the k most likely tokens only")
     parser.add_argument("--top-p", type=float, default=1.0, help="with --temperature: draw from the most likely tokens that sum to this share")
     parser.add_argument("--min-p", type=float, default=0.0, help="with --temperature: draw from tokens at least this many times as likely as the likeliest")
-    parser.add_argument("--samples", type=int, default=1, help="continuations of every prompt, the likeliest first (they share the prompt's cache pages)")
+    parser.add_argument("--samples", type=int, default=1, help="continuations of every prompt, the likeliest first (they share the prompt's cache pages, and are drawn)")
     parser.add_argument("--seed", type=int, default=0, help="seed of everything the run draws")
     parser.add_argument("--sampling-seed", type=int, default=None, help="seed of temperature sampling (default: --seed)")
     parser.add_argument("--weights-seed", type=int, default=None, help="seed of --random-weights (default: --seed)")
@@ -81,6 +81,7 @@ def main(argv=None) -> None:
         options["max_seq_len"] = args.max_seq_len
     weights_seed = args.seed if args.weights_seed is None else args.weights_seed
     sampling_seed = args.seed if args.sampling_seed is None else args.sampling_seed
+    temperature = args.temperature if args.temperature is not None else 1.0 if args.samples > 1 else 0.0    # several of the likeliest would be one
 
     def build(dtype: str):
         """The model in ``dtype``; with random weights, always the values a bfloat16 folder of --dtype would hold."""
@@ -107,13 +108,13 @@ def main(argv=None) -> None:
     outputs = model.forward(prompts[0], logits_to_keep=1)
     next_token = outputs.logits[:, -1].argmax(dim=-1)
     if args.samples > 1:
-        several = [model.continuations(prompt, args.samples, max_new_tokens=args.max_new_tokens, temperature=args.temperature, seed=sampling_seed,
+        several = [model.continuations(prompt, args.samples, max_new_tokens=args.max_new_tokens, temperature=temperature, seed=sampling_seed,
                                        stop_token_ids=_ids(args.stop_ids, "--stop-ids"), ignore_eos=args.ignore_eos, top_k=args.top_k,
                                        top_p=args.top_p, min_p=args.min_p, max_batch_size=args.max_batch_size) for prompt in prompts]
         prompts = [prompt for prompt in prompts for _ in range(args.samples)]
         results = [result for of_prompt in several for result in of_prompt]
     else:
-        results = model.generate(prompts, max_new_tokens=args.max_new_tokens, temperature=args.temperature,
+        results = model.generate(prompts, max_new_tokens=args.max_new_tokens, temperature=temperature,
                                  seed=sampling_seed, stop_token_ids=_ids(args.stop_ids, "--stop-ids"),
                                  ignore_eos=args.ignore_eos, max_batch_size=args.max_batch_size, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
     print(f"backend={args.backend}")

@@ -156,3 +156,12 @@ def test_the_command_keeps_its_batch_size(monkeypatch, capsys):
                 "--max-new-tokens", "3", "--ignore-eos"])
     assert batches == [[0, 1], [2, 3], [4]]
     assert sum(line.startswith("generated=") for line in capsys.readouterr().out.splitlines()) == 5
+
+
+@pytest.mark.parametrize("asked, different", [([], True), (["--temperature", "0"], False)])
+def test_the_command_draws_its_samples(asked, different, capsys):
+    """Without a temperature, several samples are drawn at 1; none of them at 0."""
+    from qwen_triton_b200.scripts import smoke
+    smoke.main(["--preset", "tiny-b", "--random-weights", "--random-prompts", "90", "--samples", "4", "--max-new-tokens", "6", "--ignore-eos", *asked])
+    lines = {line.split(" finish")[0] for line in capsys.readouterr().out.splitlines() if line.startswith("generated=")}
+    assert len(lines) == (4 if different else 1)
