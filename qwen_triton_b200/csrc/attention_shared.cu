@@ -841,8 +841,9 @@ __device__ __forceinline__ void walk_keys(const SharedParams& p, Walked<HD>& w, 
 }
 
 // Everything in one launch, where so little is shared that a second launch costs more than reading it again (out of the L2 cache): the blocks of (16 query
-// heads of a kv head, member) are a cluster along x whose warps each walk a range of all of the member's keys; the first block joins the ranges.  Bound by latency:
-// two sequences of 199 shared and 40 own keys, 16 heads over 8, 5.2 us (about 5 us more in two launches); 20 of 1,500 and 90, 5 heads of 64, 10 us.
+// heads of a kv head, member) are a cluster along x whose warps each walk a range of all of the member's keys; the first block joins the ranges.  Its callers are those
+// of the operator alone: steps of the engine share reading from sizes on that are beyond this form.  Bound by latency: two sequences of 199 shared and 40 own keys, 16
+// heads over 8, 5.2 us (about 5 us more in two launches); 20 of 1,500 and 90, 5 heads of 64, 10 us.
 constexpr int DIRECT_MAX_WARPS = 6;
 
 template <int HD> constexpr size_t direct_smem(int warps, int ranges, int rows) {

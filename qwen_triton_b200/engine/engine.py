@@ -167,8 +167,8 @@ class Engine:
 
     def new_sequence(self, prefix_of: int | None = None, tokens: int | None = None) -> int:
         """Take a slot for a sequence that starts at position 0, or with the first ``tokens`` (whole pages; default: all of its whole pages) of the sequence in
-        ``prefix_of``, whose keys and values it then shares.  Sequences that share their first pages are read together in one-token steps.  A position that is
-        planned (``plan_decode``) and has not run yet has no keys and values to share."""
+        ``prefix_of``, whose keys and values it then shares.  Captured one-token steps read sequences that share their first pages together where that is faster
+        (``kernels.sharing_pays``).  A position that is planned (``plan_decode``) and has not run yet has no keys and values to share."""
         if prefix_of is None:
             return self.cache.alloc()
         length = self.length(prefix_of) - (prefix_of in self._planned)

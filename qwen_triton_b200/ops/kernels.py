@@ -1468,7 +1468,8 @@ def shared_plan(n_seqs: int, *, num_heads: int, num_kv_heads: int, head_dim: int
         most_len = most_shared + most_own
         if n_seqs * num_kv_heads * most_len * 4 * head_dim <= DIRECT_BYTES:
             # All of a (member, kv head)'s keys by a cluster of blocks: as many as leave one block an SM (three with heads of 64, whose rings are small), and
-            # as many warps as have 32 keys each.  Two launches instead cost about 5 us more; from here on reading the shared keys once saves more than that.
+            # as many warps as have 32 keys each.  Behind a cold cache, 32 heads over 8 of 128, one launch / two: 2 sequences of 512 shared and 64 own tokens 8.1 / 10.8 us,
+            # 32 of 256 12.8 / 15.9, 16 of 512 11.6 / 13.7, 2 of 2,048 12.6 / 14.0, 2 of 4,096 18.9 / 17.2.
             blocks = 1
             while blocks < 4 and pairs * blocks * 2 <= sms * (3 if head_dim <= 64 else 1) and most_len > 128 * blocks:
                 blocks *= 2
