@@ -20,10 +20,10 @@
 //   * only where a noted logit lies above the bound (min_p gives one by itself) the tokens behind it are read again, and those above the bound go to the first
 //     block in vocabulary order; that block sorts their keys, finds the thresholds on the running count and mass, and draws.
 //
-// Only the row's mass for top_p without top_k takes an exponential a token, an approximate one, in the same pass.  A row whose head does not fit the list, or whose
-// threshold lies within that mass's error, finds its thresholds by bins of all of its tokens, each 256 times narrower than the one before, until the bin of the
-// threshold has few tokens, which are sorted (three times; a bin that is still longer than the list is bisected).  Such a row, and one without filters, draws over all
-// blocks.  For these passes a block keeps its ids in shared memory where they fit, and reads them again otherwise.
+// Only the row's mass for top_p without top_k takes an exponential a token, an approximate one, in the same pass.  Where the threshold lies within that mass's error
+// the mass is formed again, in units.  A row whose head does not fit the list finds its thresholds by bins of all of its tokens, each 256 times narrower than the one
+// before, until the bin of the threshold has few tokens, which are sorted (three times; a bin that is still longer than the list is bisected).  Such a row, and one
+// without filters, draws over all blocks.  For these passes a block keeps its ids in shared memory where they fit, and reads them again otherwise.
 //
 // The first pass goes at the memory's rate where every row is read at once, by few blocks a row if rows are many; passes with exponentials want many blocks a row.  So rows
 // that need those are then marked and left to a second launch.
@@ -187,7 +187,8 @@ __device__ __noinline__ void sort_down(unsigned int* keys, int n) {
 }
 
 // Of n sorted keys, the last of at least floor_key in front of which less than `wanted` lies (their number or their mass, `above` included; `share` of what all of
-// them have where it is positive); the first if there is none.  Beside it in bit 32, whether a key, or the list's end, begins within `error` of that.
+// them have where it is positive); the first if there is none.  Beside it in bit 32, whether a key, or the list's end, begins within `error` of that; error < 0: whether
+// the list ends in front of it.
 // One copy of this and of the sort: a block waits for instructions that it runs once.
 __device__ __noinline__ u64 cut(const unsigned int* keys, u64* before, u64* per_warp, int n, bool by_mass, unsigned int floor_key, u64 above, double wanted, double share,
                                 double error, Weigh weigh) {
@@ -203,7 +204,7 @@ __device__ __noinline__ u64 cut(const unsigned int* keys, u64* before, u64* per_
         total += all;
     }
     if (share > 0.) wanted = share * (double)total;
-    bool doubt = fabs((double)total - wanted) <= error;
+    bool doubt = error < 0. ? (double)total < wanted : fabs((double)total - wanted) <= error;
     int last = 0;
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const double lies = (double)before[i];
@@ -534,6 +535,13 @@ struct Row {
         barrier();
     }
 
+    // The row's mass in units.
+    __device__ __forceinline__ u64 mass() {
+        const Weigh weight = weigh();
+        u64 mine = 0;
+        each([&](const Four& v) { for (int e = 0; e < 4; ++e) mine += units_of(weight(v.x[e])); });
+        return row_total(mine);
+    }
     // Draws among the tokens with a key of at least floor_key and a weight of at least `least`, over all blocks.
     __device__ void draw(int at, unsigned int floor_key, float least) {
         const float floor_x = least_of(floor_key);
@@ -586,7 +594,9 @@ __host__ __device__ __forceinline__ size_t head_bytes(const Rows& r) {
     return 2 * LIST * sizeof(u64) + WARPS * WAITING * sizeof(unsigned int) + (noting > sorting ? noting : sorting);
 }
 
-__global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows r) {
+// WHOLE: the list takes every row as it is, so that nothing is bound or summed beforehand.  A kernel of its own, since instructions that run once are waited for: 100
+// rows of 503 tokens 14.1 us, by the kernel for all rows 16.1.
+template <bool WHOLE> __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows r) {
     pdl_launch_dependents();
     if (r.blocks > 1) cluster_arrive_started();
     extern __shared__ __align__(16) unsigned char smem[];
@@ -613,8 +623,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows 
         if (blocks > 1) cluster_wait_started();
         return;
     }
-    const bool whole = blocks == 1 && r.vocab <= LIST;         // the list takes the row as it is
-    const bool counting = f.by_count, summing = f.by_mass && !f.by_count && !whole && t > 0.f;
+    const bool counting = f.by_count, summing = !WHOLE && f.by_mass && !f.by_count && t > 0.f;
     if (threadIdx.x == 0) sh.taken = 0;
     double sum;
     const float own_best = summing ? w.fetch<true>(sum) : w.fetch<false>(sum);
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows 
     bool fits = filtered && mx < INFINITY && t > 1e-30f;
     float bound = -INFINITY;
     double row_mass = 0.;                                      // for top_p alone, in units
-    if (fits && !whole) {
+    if (fits && !WHOLE) {
         if (f.by_weight && !f.by_count) bound = mx + t * logf(f.least);
         if (f.by_count || f.by_mass) {
             const Weigh weight = w.weigh();
@@ -718,6 +727,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows 
         for (int b = 0; b < blocks; ++b) fits = fits && (int)sh.slots[slot][b][0] <= room;
         if (fits && rank > 0) {
             if (!summing || sh.slots[w.exchange(0, 0)][0][0]) return;
+            if (!r.mark) {
+                w.mass();
+                if (sh.slots[w.exchange(0, 0)][0][0]) return;
+            }
         } else if (fits) {
             // the first block alone: places j THREADS + thread of the list a thread
             int count = 0;
@@ -741,6 +754,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_filtered_kernel(const Rows 
                 if (summing) {
                     fits = last >> 32 == 0;
                     w.exchange(fits, 0);
+                    // in doubt, which the row's mass in units settles where the list reaches so far (64 rows of 151,936, one or more in doubt: 48 to 60 us, 60 to 119 by
+                    // bins of all tokens)
+                    if (!fits && !r.mark) {
+                        const u64 settled = cut(keys, before, sh.per_warp, count, true, 0u, 0, (double)f.p * (double)w.mass(), 0., -1., w.weigh());
+                        floor_key = (unsigned int)settled;
+                        fits = settled >> 32 == 0;
+                        w.exchange(fits, 0);
+                    }
                 }
             }
             if (fits) {
@@ -867,9 +888,11 @@ extern "C" int qt_sample_filtered(const float* logits, long long row_stride, con
     size_t smem = head_bytes(r);
     r.cached = !r.mark && smem + part_of(r) <= ((long long)rows * blocks > sm_count() ? TWO : ONE);
     if (r.cached) smem += part_of(r);
-    cudaError_t raised = raise_shared<sample_filtered_kernel>((int)smem);
+    const bool whole = blocks == 1 && vocab <= LIST;
+    cudaError_t raised = whole ? raise_shared<sample_filtered_kernel<true>>((int)smem) : raise_shared<sample_filtered_kernel<false>>((int)smem);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "sample_filtered: cannot raise shared memory: %s", cudaGetErrorString(raised));
-    launch_kernel_cluster(sample_filtered_kernel, dim3((unsigned)(rows * blocks)), dim3(THREADS), smem, (cudaStream_t)stream, (unsigned)blocks, r);
+    launch_kernel_cluster(whole ? sample_filtered_kernel<true> : sample_filtered_kernel<false>, dim3((unsigned)(rows * blocks)), dim3(THREADS), smem, (cudaStream_t)stream,
+                          (unsigned)blocks, r);
     if (r.mark) {
         const int clusters = resident / most < rows ? resident / most : rows;
         Rows marked = rows_of(most);
