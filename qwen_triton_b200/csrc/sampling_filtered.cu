@@ -681,7 +681,8 @@ template <bool WHOLE> __global__ void __launch_bounds__(THREADS, 2) sample_filte
             // every token of the bins up to this one lies above the bound; the last bin has no end
             if (bin < BINS - 1) bound = fmaxf(bound, mx - t * (float)(bin + 1) * (1.f / BINS_PER_NAT));
         }
-        bound -= 1e-5f * (fabsf(mx) + fabsf(mx - bound));      // what the bound's and the bins' roundings are
+        // what the bound's and the bins' roundings are, and those of a weight at min_p, 4e-7 of it (at a high temperature many logits lie so near)
+        bound -= 1e-5f * (fabsf(mx) + fabsf(mx - bound)) + 1e-6f * t;
     }
     if (fits) {
         auto above = [&](float x) { return x > -INFINITY && !(x < bound); };

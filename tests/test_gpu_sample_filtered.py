@@ -315,3 +315,15 @@ def test_shares_that_end_beside_a_token_of_a_large_vocabulary():
         want = float(y[token] - weights.sum().log())
         assert tokens.tolist() == [token]
         assert abs(float(logprob[0]) - want) <= 2e-6 * (3 + abs(want))
+
+
+@pytest.mark.parametrize("vocab", [600, 5000, 40000])
+def test_weights_that_round_to_the_least_stay_whichever_way_the_row_goes(vocab):
+    """At a temperature of 10,000 a logit 1e-4 below the largest weighs 1 - 1e-8, which is 1 in 32 bits: min_p = 1 keeps both, and a top_k that leaves every token
+    (which makes the row go another way) changes nothing."""
+    logits = torch.full((1, vocab), -30.0)
+    logits[0, 7], logits[0, vocab // 2] = 0.03, 0.03 - 1e-4
+    for u, token in ((0.2, 7), (0.8, vocab // 2)):
+        for k in (0, vocab - 1):
+            tokens, logprob = run(logits.cuda(), [1e4], [k], [1.0], [1.0], [u])
+            assert tokens.tolist() == [token] and abs(float(logprob[0]) + math.log(2)) < 1e-6
