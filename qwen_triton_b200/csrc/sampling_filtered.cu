@@ -28,7 +28,7 @@
 // The first pass goes at the memory's rate where every row is read at once, by few blocks a row if rows are many; passes with exponentials want many blocks a row.  So rows
 // that need those are then marked and left to a second launch.
 //
-// Measured behind a cold cache: one row of 151,936 14.6 us, 64 rows 37 to 51, 256 rows (156 MB, 24 us of copying) 121 to 130, by what the rows ask for; with every row on
+// Measured behind a cold cache: one row of 151,936 14.5 us, 64 rows 31 to 59, 256 rows (156 MB, 24 us of copying) 113 to 139, by what the rows ask for; with every row on
 // eight blocks that kept it in shared memory (37 rows at a time) 15.8, 49 to 78 and 131 to 170.  A row of 256 is read in 30 us; the rest is the head: what it runs is
 // short and serial (bins 5 us, tokens read again 4 to 17, sort and draw 8 to 12), so that its instructions' way into the SM counts, and loops stay loops.
 #include "common.cuh"
@@ -854,8 +854,8 @@ struct Cut {
         while (most < MAX_BLOCKS && vocab / most > 8192) most *= 2;
         blocks = most;
         while (blocks > 1 && (long long)rows * blocks > resident) blocks /= 2;
-        // 64 rows by four blocks each take 37 to 51 us where the rows that need more passes stay with them and 40 to 91 where these are left to the second launch; 256
-        // rows by one block each take 121 to 130 with it and 244 without
+        // 64 rows by four blocks each take 31 to 59 us where the rows that need more passes stay with them and 40 to 91 where these are left to the second launch; 256
+        // rows by one block each take 113 to 139 with it and 244 without
         mark = blocks < most && blocks < 4;
     }
 };
