@@ -14,7 +14,7 @@ import torch
 from ..config import config_from_dict, load_config
 from ..sampling import Sampler, SamplingParams
 from .engine import Engine, parse_dtype
-from .generate import BatchRun, GenerationResult, generate, stop_set
+from .generate import BatchRun, GenerationResult, generate, shared_start, stop_set
 from .step import StepEntry
 
 
@@ -124,14 +124,15 @@ class QwenB200ForCausalLM:
 
     def start_batch(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 16, temperature: float = 0.0,
                     seed: int = 0, stop_token_ids: Sequence[int] | None = None, ignore_eos: bool = False,
-                    top_k: int = 0, top_p: float = 1.0) -> BatchRun:
+                    top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, logprobs: bool = False, share_prefix: bool = False) -> BatchRun:
         """Step-by-step generation of one batch: ``run.start()`` runs the prompts and returns each request's
         first token, every ``run.advance()`` one more token per request still going; ``run.results`` collects
-        them and ``run.close()`` gives the cache back.  ``generate`` is this, looped over batches."""
+        them and ``run.close()`` gives the cache back.  ``generate`` is this, looped over batches, and has the same options."""
         results = [GenerationResult() for _ in prompts]
         return BatchRun(self.engine, self.sampler, prompts, results, range(len(prompts)), max_new_tokens=max_new_tokens,
-                        sampling=SamplingParams(temperature=temperature, seed=seed, top_k=top_k, top_p=top_p),
-                        stop=stop_set(self.engine, stop_token_ids, ignore_eos))
+                        sampling=SamplingParams(temperature=temperature, seed=seed, top_k=top_k, top_p=top_p, min_p=min_p, logprobs=logprobs),
+                        stop=stop_set(self.engine, stop_token_ids, ignore_eos),
+                        shared_tokens=shared_start(self.engine, prompts) if share_prefix else 0)
 
     @torch.no_grad()
     def greedy_generate(self, input_ids, attention_mask=None, max_new_tokens: int = 16) -> torch.LongTensor:

@@ -85,6 +85,11 @@ def common_prefix(prompts: Sequence[Sequence[int]], page_tokens: int) -> int:
     return n // page_tokens * page_tokens
 
 
+def shared_start(engine, prompts: Sequence[Sequence[int]]) -> int:
+    """Tokens of ``prompts`` that their sequences can hold together: their common whole pages where the engine says ``can_share``."""
+    return common_prefix(prompts, engine.page_tokens) if getattr(engine, "can_share", False) else 0
+
+
 class BatchRun:
     """One batch of requests that start together: ``start()`` runs every prompt in one step and
     samples each request's first token; every ``advance()`` then feeds the last tokens back, one per
@@ -249,7 +254,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
         for result in results:
             result.finish_reason = "length"
         return results
-    shared = common_prefix(prompts, engine.page_tokens) if share_prefix and getattr(engine, "can_share", False) else 0
+    shared = shared_start(engine, prompts) if share_prefix else 0
     batches = plan_batches([len(p) for p in prompts], max_new_tokens, page_tokens=engine.page_tokens,
                            total_pages=engine.total_pages, num_slots=engine.num_slots,
                            max_seq_len=engine.max_seq_len, max_batch_size=max_batch_size, shared_tokens=shared)

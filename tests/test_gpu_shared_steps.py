@@ -165,3 +165,24 @@ def test_the_command_draws_its_samples(asked, different, capsys):
     smoke.main(["--preset", "tiny-b", "--random-weights", "--random-prompts", "90", "--samples", "4", "--max-new-tokens", "6", "--ignore-eos", *asked])
     lines = {line.split(" finish")[0] for line in capsys.readouterr().out.splitlines() if line.startswith("generated=")}
     assert len(lines) == (4 if different else 1)
+
+
+def test_a_batch_step_by_step_has_the_options_of_generate():
+    from gpu_util import model_folder
+    from qwen_triton_b200 import QwenB200ForCausalLM
+    model = QwenB200ForCausalLM.from_pretrained_hf(model_folder("tiny-b", "fp32"), dtype="fp32", max_tokens=4096)
+    start = random_tokens("tiny-b", 150, 7)
+    prompts = [start + random_tokens("tiny-b", 3 + i, 8 + i) for i in range(3)]
+    options = dict(max_new_tokens=5, temperature=0.9, seed=3, min_p=0.02, logprobs=True, share_prefix=True, ignore_eos=True)
+    want = model.generate(prompts, **options)
+    run = model.start_batch(prompts, **options)
+    try:
+        run.start()
+        first = model.engine.cache.book.pages(run.slot_of[0], 0)[:2]
+        assert all(model.engine.cache.book.pages(run.slot_of[i], 0)[:2] == first for i in (1, 2))
+        while not run.done:
+            run.advance()
+    finally:
+        run.close()
+    assert [r.tokens for r in run.results] == [r.tokens for r in want]
+    assert [r.logprobs for r in run.results] == [r.logprobs for r in want] and all(len(r.logprobs) == 5 for r in want)
