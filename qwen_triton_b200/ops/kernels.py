@@ -140,6 +140,27 @@ _SIGNATURES = {
         "qt_attention_prefill_rows": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr,
                                       _c_int, _c_ll, _c_int, _c_int, _c_int, _c_ptr, _c_ptr],
     },
+    "gemm_fp8": {
+        # x, dtype, values, scales, rows, k, stream
+        "qt_quantise_rows": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+        "qt_quantise_weight": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+        # x8, x_scale, w8, w_scale, out, dtype, rows, n, k, status, stream
+        "qt_gemm_fp8": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr],
+    },
+    "cache8": {
+        # qkv, in_dtype, n_splits, split_stride, q_out, out_dtype, k, v, k_scale, v_scale, seq_start, seq_past, n_seqs, max_q_len, block_table, max_blocks, n_pages,
+        # q_weight, k_weight, eps, cos_sin, rotary_dim, max_pos, interleaved, nq, nkv, d, stream
+        "qt_qkv_write_cache8": [_c_ptr, _c_int, _c_int, _c_ll, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+                                _c_ptr, _c_ptr, _c_float, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
+    },
+    "attention_cache8": {
+        # q, dtype, k, v, k_scale, v_scale, out, block_table, max_blocks, n_pages, seq_len, n_seqs, nq, nkv, d, scale, ranges, range_pages, part_acc, part_ml, stream
+        "qt_attention_decode_cache8": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float,
+                                       _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr],
+        # q, dtype, k, v, k_scale, v_scale, out, block_table, max_blocks, n_pages, seq_start, seq_past, n_seqs, max_q_len, nq, nkv, d, scale, stream
+        "qt_attention_prefill_cache8": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+                                        _c_int, _c_float, _c_ptr],
+    },
     "gemm_f32": {
         "qt_gemm_f32": [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr],
     },
@@ -1576,6 +1597,275 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
           _SHARED_CALL.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_len.data_ptr(), members.data_ptr(),
                             share.data_ptr(), part_acc.data_ptr(), part_ml.data_ptr(), _status_word(q.device).data_ptr(), _stream(), scale, *plan.numbers,
                             block_table.shape[1], k_cache.shape[0]), launches=plan.launches)
+
+
+# ----------------------------------------------------------------------------- weights and rows in 8 bits
+FP8_GROUP = 128            # columns (and rows of a weight) that share a scale
+E4M3 = torch.float8_e4m3fn
+
+
+@dataclass(frozen=True)
+class Fp8Weight:
+    """A weight [N, K] of 8-bit numbers: ``values`` (e4m3) times ``scales`` [ceil(N / 128), ceil(K / 128)] (float), one for each block of 128 x 128.
+    ``quantise_weight_fp8`` makes one; a checkpoint's values and scales of that form are taken as they are."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        _need(self.values, "values", E4M3)
+        if self.values.dim() != 2 or self.values.numel() == 0:
+            raise KernelError(f"Fp8Weight: values {tuple(self.values.shape)} are not [N, K]")
+        n, k = self.values.shape
+        _need(self.scales, "scales", torch.float32, (-(-n // FP8_GROUP), -(-k // FP8_GROUP)))
+        if self.scales.device != self.values.device:
+            raise KernelError(f"Fp8Weight: values on {self.values.device}, scales on {self.scales.device}")
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+
+@dataclass(frozen=True)
+class Fp8Rows:
+    """Rows [M, K] in 8 bits: ``values`` (e4m3) times ``scales`` [ceil(K / 128), M] (float), one for each row and 128 columns (``quantise_rows_fp8``)."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        _need(self.values, "values", E4M3)
+        if self.values.dim() != 2 or self.values.shape[1] == 0:
+            raise KernelError(f"Fp8Rows: values {tuple(self.values.shape)} are not [M, K]")
+        m, k = self.values.shape
+        _need(self.scales, "scales", torch.float32, (-(-k // FP8_GROUP), m))
+        if self.scales.device != self.values.device:
+            raise KernelError(f"Fp8Rows: values on {self.values.device}, scales on {self.scales.device}")
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+
+def fp8_rows(rows: int, columns: int, device) -> Fp8Rows:
+    """Room for ``rows`` rows in 8 bits (contents undefined): what ``quantise_rows_fp8`` fills and ``gemm_fp8`` takes as scratch."""
+    return Fp8Rows(torch.empty((rows, columns), dtype=E4M3, device=device),
+                   torch.empty((-(-columns // FP8_GROUP), rows), dtype=torch.float32, device=device))
+
+
+def _same_device(name: str, *tensors: torch.Tensor) -> None:
+    """All on the current device, whose current stream the kernels are launched on."""
+    device = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+    for tensor in tensors:
+        if tensor.get_device() != device:
+            raise KernelError(f"{name}: a tensor on {tensor.device}, the current device is cuda:{device}")
+
+
+def quantise_rows_fp8(x: torch.Tensor, rows: Fp8Rows) -> None:
+    """rows = x [M, K] (bfloat16 or float32) in 8 bits: of each row and 128 columns the scale is s = max(amax / 448, 2^-100) and the values are x / s (in
+    float) rounded to e4m3.  A row with a number that is not finite has NaN in its place."""
+    _need(x, "x", shape=rows.shape)
+    _same_device("quantise_rows_fp8", x, rows.values)
+    _call("gemm_fp8", "qt_quantise_rows", _ptr(x), _code(x, "x"), _ptr(rows.values), _ptr(rows.scales), *x.shape, _stream())
+
+
+def quantise_weight_fp8(weight: torch.Tensor) -> Fp8Weight:
+    """``weight`` [N, K] (bfloat16 or float32) in 8 bits, as ``quantise_rows_fp8`` does it but with one scale for each block of 128 x 128."""
+    _need(weight, "weight")
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise KernelError(f"quantise_weight_fp8: weight {tuple(weight.shape)} is not [N, K]")
+    _same_device("quantise_weight_fp8", weight)
+    code = _code(weight, "weight")
+    n, k = weight.shape
+    out = Fp8Weight(torch.empty((n, k), dtype=E4M3, device=weight.device),
+                    torch.empty((-(-n // FP8_GROUP), -(-k // FP8_GROUP)), dtype=torch.float32, device=weight.device))
+    _call("gemm_fp8", "qt_quantise_weight", _ptr(weight), code, _ptr(out.values), _ptr(out.scales), n, k, _stream())
+    return out
+
+
+def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None = None) -> None:
+    """out [M, N] (bfloat16 or float32) = x [M, K] W^T with both operands in 8 bits and their scales on the sums of each 128 columns, in float, rounded once.
+
+    ``x`` is ``Fp8Rows``, or bfloat16 or float32 rows that are brought to 8 bits first (``quantise_rows_fp8``), through ``scratch`` (``fp8_rows(M, K)``, or
+    larger in M: its leading rows serve)."""
+    n, k = weight.shape
+    m = x.shape[0]
+    _need(out, "out", shape=(m, n))
+    launches = 1
+    if not isinstance(x, Fp8Rows):
+        if scratch is None or scratch.shape[1] != k or scratch.shape[0] < m:
+            raise KernelError(f"gemm_fp8: scratch for {m} x {k} rows in 8 bits is required, got {None if scratch is None else tuple(scratch.shape)}")
+        if scratch.shape[0] > m:
+            groups = scratch.scales.shape[0]
+            scratch = Fp8Rows(scratch.values[:m], scratch.scales.view(-1)[:groups * m].view(groups, m))
+        quantise_rows_fp8(x, scratch)
+        x = scratch
+    if x.shape[1] != k:
+        raise KernelError(f"gemm_fp8: rows {tuple(x.shape)} for a weight {tuple(weight.shape)}")
+    _same_device("gemm_fp8", x.values, weight.values, out)
+    _call("gemm_fp8", "qt_gemm_fp8", _ptr(x.values), _ptr(x.scales), _ptr(weight.values), _ptr(weight.scales), _ptr(out), _code(out, "out"), m, n, k,
+          _ptr(_status_word(out.device)), _stream(), launches=launches)
+
+
+# ----------------------------------------------------------------------------- a cache of keys and values in 8 bits
+@dataclass(frozen=True)
+class Cache8:
+    """Keys and values in 8 bits: ``k`` and ``v`` [pages, kv_heads, 64, d] (e4m3, d a multiple of 16 up to 256) times ``k_scale`` and ``v_scale`` [pages, kv_heads]
+    (float): a scale for each block of a page's 64 tokens and a head.  ``qkv_write_cache8`` leaves powers of two between 2^-40 and 2^40 there; attention takes
+    any positive number of that range."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    def __post_init__(self) -> None:
+        _need(self.k, "k", E4M3)
+        if self.k.dim() != 4 or self.k.numel() == 0 or self.k.shape[2] != 64 or self.k.shape[3] % 16 or self.k.shape[3] > 256:
+            raise KernelError(f"Cache8: keys {tuple(self.k.shape)} are not [pages, kv_heads, 64, a multiple of 16 up to 256]")
+        _need(self.v, "v", E4M3, self.k.shape)
+        _need(self.k_scale, "k_scale", torch.float32, self.k.shape[:2])
+        _need(self.v_scale, "v_scale", torch.float32, self.k.shape[:2])
+        if not self.k.device == self.v.device == self.k_scale.device == self.v_scale.device:
+            raise KernelError("Cache8: keys, values and scales are on different devices")
+
+    @property
+    def pages(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def head_dim(self) -> int:
+        return self.k.shape[3]
+
+
+def cache8(pages: int, kv_heads: int, head_dim: int, device) -> Cache8:
+    """An empty cache in 8 bits (zeros under the smallest scale)."""
+    shape = (pages, kv_heads, 64, head_dim)
+    return Cache8(*(torch.zeros(shape, dtype=torch.uint8, device=device).view(E4M3) for _ in range(2)),
+                  *(torch.full(shape[:2], 2.0 ** -40, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def qkv_write_cache8(qkv: GemmOut, q_out: torch.Tensor, cache: Cache8, seq_start: torch.Tensor, seq_past: torch.Tensor, block_table: torch.Tensor, max_q_len: int,
+                     q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float, cos_sin: torch.Tensor | None, interleaved: bool = False) -> None:
+    """``qk_norm_rope_write`` into a cache in 8 bits: per-head RMS norm of q and k (where weights are given) and rotation (where a table is), q to ``q_out``
+    [T, nq, d], k and v of the step's tokens to the pages of their sequences.
+
+    ``qkv`` [*, T, (nq + 2 nkv) d]; sequence i has the tokens from ``seq_start[i]`` (int32 [sequences + 1]) on, at most ``max_q_len``, and ``seq_past[i]``
+    earlier ones in the pages that row i of ``block_table`` (int32) lists; no two sequences write the same page.
+
+    The scale of a page and head is 2^e with the smallest e between -40 and 40 whose 448-fold reaches every finite number there; values are rounded to e4m3
+    once, and beyond 448 * 2^40 end there.  e starts with the write of a page's first place and then only grows: what the page's earlier places hold is then brought
+    under the larger scale (exact but for numbers below 2^-6 of it).  Infinities are held as NaN.  Places behind a sequence's last token stay as they were."""
+    tokens, num_heads, head_dim = q_out.shape
+    n_seqs = seq_past.shape[0]
+    _need(q_out, "q_out", shape=(tokens, num_heads, cache.head_dim))
+    if qkv.rows != tokens or qkv.cols != (num_heads + 2 * cache.kv_heads) * head_dim:
+        raise KernelError(f"qkv_write_cache8: a projection {tuple(qkv.tensor.shape)} for {tokens} tokens of {num_heads} + 2 * {cache.kv_heads} heads of {head_dim}")
+    _need(seq_past, "seq_past", torch.int32, (n_seqs,))
+    _need(seq_start, "seq_start", torch.int32, (n_seqs + 1,))
+    _need(block_table, "block_table", torch.int32, (n_seqs, block_table.shape[-1]))
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _need(w, name, torch.float32, (head_dim,))
+    rotary_dim, max_pos = 0, 0
+    if cos_sin is not None:
+        _need(cos_sin, "cos_sin", torch.float32)
+        max_pos, rotary_dim = cos_sin.shape
+    if not qkv.tensor.is_cuda:
+        raise KernelError("qkv must be a CUDA tensor (there is no host path)")
+    if max_q_len < 0 or max_q_len > tokens:
+        raise KernelError(f"qkv_write_cache8: max_q_len={max_q_len} of {tokens} tokens")
+    _same_device("qkv_write_cache8", qkv.tensor, q_out, cache.k, seq_start, seq_past, block_table)
+    _call("cache8", "qt_qkv_write_cache8", _ptr(qkv.tensor), _code(qkv.tensor, "qkv"), qkv.n_splits, qkv.split_stride, _ptr(q_out), _code(q_out, "q_out"), _ptr(cache.k),
+          _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(seq_start), _ptr(seq_past), n_seqs, int(max_q_len), _ptr(block_table), block_table.shape[1],
+          cache.pages, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos_sin), rotary_dim, max_pos, 1 if interleaved else 0, num_heads, cache.kv_heads, head_dim,
+          _stream())
+
+
+@dataclass(frozen=True)
+class Decode8Plan:
+    """How ``attention_decode_cache8`` cuts the keys of its sequences (``decode8_plan``): ``ranges`` ranges of ``range_pages`` pages, the last one taking
+    whatever is left.  Any plan gives the result of every call with its sizes."""
+
+    q_shape: tuple[int, int, int]
+    num_kv_heads: int
+    dtype: torch.dtype
+    ranges: int
+    range_pages: int
+
+    @property
+    def acc_elements(self) -> int:
+        return self.q_shape[0] * self.q_shape[1] * self.ranges * self.q_shape[2] if self.ranges > 1 else 0
+
+    @property
+    def ml_elements(self) -> int:
+        return self.q_shape[0] * self.q_shape[1] * self.ranges * 2 if self.ranges > 1 else 0
+
+
+def decode8_plan(batch: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, max_context: int, sms: int = 148) -> Decode8Plan:
+    """A plan for ``batch`` sequences of up to ``max_context`` keys (a longer one is right too, but slower)."""
+    if batch < 0 or num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or head_dim <= 0 or max_context < 0 or dtype not in _CODES:
+        raise KernelError(f"decode8_plan: {batch} sequences of {num_heads} heads over {num_kv_heads} of {head_dim}, {dtype}, {max_context} keys")
+    pages = max(1, -(-max_context // 64))
+    walks = max(1, batch * num_kv_heads * -(-(num_heads // num_kv_heads) // 8))
+    ranges = max(1, min(4 * sms // walks, -(-pages // 4), 64))
+    range_pages = -(-pages // ranges)
+    return Decode8Plan((batch, num_heads, head_dim), num_kv_heads, dtype, -(-pages // range_pages), range_pages)
+
+
+def _check_cache8(name: str, q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, n_seqs: int) -> None:
+    _need(q, "q")
+    _code(q, "q")
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.kv_heads or q.shape[1] == 0:
+        raise KernelError(f"{name}: queries {tuple(q.shape)} for {cache.kv_heads} kv heads of {cache.head_dim}")
+    _need(out, "out", q.dtype, q.shape)
+    _need(block_table, "block_table", torch.int32)
+    if block_table.dim() != 2 or block_table.shape[0] != n_seqs or block_table.shape[1] == 0:
+        raise KernelError(f"{name}: a block table {tuple(block_table.shape)} for {n_seqs} sequences")
+    _same_device(name, q, cache.k, out, block_table)
+
+
+def attention_decode_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor, scale: float, plan: Decode8Plan,
+                            part_acc: torch.Tensor | None = None, part_ml: torch.Tensor | None = None) -> None:
+    """``attention_decode`` over a cache in 8 bits: one query token per sequence, q and out [sequences, nq, d] (bfloat16 or float32); ``seq_len`` counts the keys
+    it sees (none: the result is zero).  Where the plan cuts the keys into ranges their partial results pass through ``part_acc`` and ``part_ml`` (float, at least
+    ``plan.acc_elements`` and ``plan.ml_elements``).  What lies behind a sequence's last key is not looked at."""
+    _check_cache8("attention_decode_cache8", q, cache, out, block_table, q.shape[0])
+    _need(seq_len, "seq_len", torch.int32, q.shape[:1])
+    if tuple(q.shape) != plan.q_shape or q.dtype != plan.dtype or cache.kv_heads != plan.num_kv_heads:
+        raise KernelError(f"attention_decode_cache8: a plan for {plan.q_shape} over {plan.num_kv_heads} kv heads, {plan.dtype}; queries {tuple(q.shape)} over {cache.kv_heads}, {q.dtype}")
+    if plan.ranges > 1:
+        for name, part, need in (("part_acc", part_acc, plan.acc_elements), ("part_ml", part_ml, plan.ml_elements)):
+            if part is None:
+                raise KernelError(f"attention_decode_cache8: {name} is required for {plan.ranges} ranges")
+            _need(part, name, torch.float32)
+            if part.numel() < need:
+                raise KernelError(f"attention_decode_cache8: {name} holds {part.numel()} of {need} elements")
+        _same_device("attention_decode_cache8", part_acc, part_ml)
+    _same_device("attention_decode_cache8", seq_len)
+    _call("attention_cache8", "qt_attention_decode_cache8", _ptr(q), _code(q, "q"), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(out),
+          _ptr(block_table), block_table.shape[1], cache.pages, _ptr(seq_len), q.shape[0], q.shape[1], cache.kv_heads, cache.head_dim, float(scale), plan.ranges,
+          plan.range_pages, _ptr(part_acc), _ptr(part_ml), _stream(), launches=2 if plan.ranges > 1 else 1)
+
+
+def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_start: torch.Tensor, seq_past: torch.Tensor,
+                             max_q_len: int, scale: float) -> None:
+    """``attention_prefill`` over a cache in 8 bits: packed queries [T, nq, d], sequence i's from ``seq_start[i]`` on (at most ``max_q_len``), behind ``seq_past[i]`` earlier
+    tokens; the cache already holds this step's keys; a query sees the keys up to its own."""
+    n_seqs = seq_past.shape[0]
+    _check_cache8("attention_prefill_cache8", q, cache, out, block_table, n_seqs)
+    _need(seq_past, "seq_past", torch.int32, (n_seqs,))
+    _need(seq_start, "seq_start", torch.int32, (n_seqs + 1,))
+    if max_q_len < 0 or max_q_len > q.shape[0]:
+        raise KernelError(f"attention_prefill_cache8: max_q_len={max_q_len} of {q.shape[0]} tokens")
+    _same_device("attention_prefill_cache8", seq_start, seq_past)
+    _call("attention_cache8", "qt_attention_prefill_cache8", _ptr(q), _code(q, "q"), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(out),
+          _ptr(block_table), block_table.shape[1], cache.pages, _ptr(seq_start), _ptr(seq_past), n_seqs, int(max_q_len), q.shape[1], cache.kv_heads, cache.head_dim,
+          float(scale), _stream())
 
 
 # ----------------------------------------------------------------------------- experts chosen by a table

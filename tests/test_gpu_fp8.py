@@ -1,0 +1,183 @@
+"""The product of rows and a weight in 8 bits with a scale for each block of 128, and what brings both to 8 bits, against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import plain_8bit as plain
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+
+
+def _rows(m, k, dtype, seed, outliers=True):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((m, k), generator=gen)
+    if outliers:
+        x *= torch.where(torch.rand(k, generator=gen) < 0.02, 30.0, 1.0)
+    return x.to(dtype)
+
+
+def _weight(n, k, seed):
+    """Values and scales as a checkpoint may hold them: scales that are no powers of two, a block of zeros, the largest numbers."""
+    gen = torch.Generator().manual_seed(seed)
+    values = (torch.randn((n, k), generator=gen) * 100).clamp(-448, 448).to(E4M3)
+    scales = 1e-3 * torch.rand((-(-n // 128), -(-k // 128)), generator=gen) + 1e-5
+    values.view(torch.uint8)[:min(n, 128), :min(k, 128)] = 0 if min(scales.shape) > 1 else values.view(torch.uint8)[:min(n, 128), :min(k, 128)]
+    return values, scales
+
+
+def _check_product(m, n, k, dtype, out_dtype=None, seed=0):
+    from qwen_triton_b200.ops import kernels
+    x, (values, scales) = _rows(m, k, dtype, seed), _weight(n, k, seed + 1)
+    out = torch.full((m, n), math.nan, dtype=out_dtype or dtype, device="cuda")
+    weight = kernels.Fp8Weight(values.cuda(), scales.cuda())
+    kernels.gemm_fp8(x.cuda(), weight, out, kernels.fp8_rows(m, k, "cuda"))
+    want, bound = plain.product(*plain.quantise_rows(x), values.double(), scales)
+    bound = bound + want.abs() * torch.finfo(out.dtype).eps / 2 * (1 + 2 ** -8)
+    off = (out.double().cpu() - want).abs()
+    assert bool((off <= bound).all()), f"{float((off / bound.clamp(min=1e-300)).max())} of the bound"
+    kernels.check_status()
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 9, 16, 17, 31, 33, 64, 65, 100, 128, 129, 200, 256, 257, 400])
+@pytest.mark.parametrize("n,k", [(128, 128), (384, 512), (1000, 2832), (130, 272), (72, 1040)])
+def test_product(m, n, k):
+    _check_product(m, n, k, torch.bfloat16, seed=m)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 3, 7), (40, 129, 129), (3, 257, 100), (70, 65, 1000), (1, 127, 16), (300, 1, 48), (4, 24, 131)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_product_of_odd_sizes(m, n, k, dtype):
+    _check_product(m, n, k, dtype)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1024, 2048), (8, 512, 12288), (333, 640, 4096), (77, 1000, 2832), (600, 768, 1024)])
+def test_product_in_float32(m, n, k):
+    _check_product(m, n, k, torch.float32)
+    _check_product(m, n, k, torch.bfloat16, torch.float32)
+    _check_product(m, n, k, torch.float32, torch.bfloat16)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (8, 6144, 4096), (700, 5120, 1024), (2048, 2560, 512)])
+def test_product_of_many_tiles(m, n, k):
+    _check_product(m, n, k, torch.bfloat16)
+
+
+def test_the_same_rows_give_the_same_bits():
+    """Alone and twice, in 8 bits already or not: sums are in one order."""
+    from qwen_triton_b200.ops import kernels
+    for m in (4, 48, 300):
+        x, (values, scales) = _rows(m, 1152, torch.bfloat16, 3).cuda(), _weight(1024, 1152, 4)
+        weight = kernels.Fp8Weight(values.cuda(), scales.cuda())
+        rows = kernels.fp8_rows(m, 1152, "cuda")
+        outs = [torch.empty((m, 1024), dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+        kernels.gemm_fp8(x, weight, outs[0], rows)
+        kernels.gemm_fp8(x, weight, outs[1], kernels.fp8_rows(m + 7, 1152, "cuda"))
+        kernels.gemm_fp8(rows, weight, outs[2])
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_rows_and_sums_at_the_ends_of_the_range():
+    """Rows of zeros, of the smallest and largest numbers, with an infinity or a NaN: such a row is NaN, the others are as without it."""
+    from qwen_triton_b200.ops import kernels
+    x = _rows(7, 512, torch.float32, 5)
+    x[0] = 0
+    x[1] *= 1e-38
+    x[2] *= 1e30
+    x[3, 200] = math.inf
+    x[4, 300] = math.nan
+    x[5, 100] = -math.inf
+    values, scales = _weight(256, 512, 6)
+    weight = kernels.Fp8Weight(values.cuda(), scales.cuda())
+    out = torch.empty((7, 256), device="cuda")
+    kernels.gemm_fp8(x.cuda(), weight, out, kernels.fp8_rows(7, 512, "cuda"))
+    out = out.double().cpu()
+    assert bool((out[0] == 0).all())
+    for row in (3, 4):
+        assert bool(out[row].isnan().all())
+    assert bool(out[5].isnan().any())          # the weight's block of zeros times NaN is NaN as well
+    want, bound = plain.product(*plain.quantise_rows(x), values.double(), scales)
+    for row in (1, 2, 6):
+        assert bool(((out[row] - want[row]).abs() <= bound[row] + want[row].abs() * 2.0 ** -24 + 2.0 ** -149).all())
+
+
+@pytest.mark.parametrize("m,k", [(1, 128), (3, 1), (5, 130), (9, 1000), (130, 256), (2, 25600)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_in_8_bits(m, k, dtype):
+    from qwen_triton_b200.ops import kernels
+    x = _rows(m, k, dtype, k)
+    rows = kernels.fp8_rows(m, k, "cuda")
+    kernels.quantise_rows_fp8(x.cuda(), rows)
+    values, scales = plain.quantise_rows(x)
+    assert torch.equal(rows.scales.cpu(), scales)
+    assert torch.equal(rows.values.double().cpu(), values)
+
+
+@pytest.mark.parametrize("n,k", [(128, 128), (1, 1), (130, 257), (384, 1024)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_weight_in_8_bits(n, k, dtype):
+    from qwen_triton_b200.ops import kernels
+    w = _rows(n, k, dtype, n + k) * 0.02
+    weight = kernels.quantise_weight_fp8(w.cuda())
+    values, scales = plain.quantise_weight(w)
+    assert torch.equal(weight.scales.cpu(), scales)
+    assert torch.equal(weight.values.double().cpu(), values)
+
+
+def test_captured_and_on_another_stream():
+    from qwen_triton_b200.ops import kernels
+    values, scales = _weight(512, 1024, 8)
+    weight = kernels.Fp8Weight(values.cuda(), scales.cuda())
+    x, out, rows = torch.zeros((24, 1024), dtype=torch.bfloat16, device="cuda"), torch.empty((24, 512), dtype=torch.bfloat16, device="cuda"), kernels.fp8_rows(24, 1024, "cuda")
+    kernels.gemm_fp8(x, weight, out, rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kernels.gemm_fp8(x, weight, out, rows)
+    stream = torch.cuda.Stream()
+    for seed in (1, 2):
+        given = _rows(24, 1024, torch.bfloat16, seed)
+        x.copy_(given)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        stream.synchronize()
+        want, bound = plain.product(*plain.quantise_rows(given), values.double(), scales)
+        assert bool(((out.double().cpu() - want).abs() <= bound + want.abs() * 2.0 ** -8).all())
+        with torch.cuda.stream(stream):
+            second = torch.empty_like(out)
+            kernels.gemm_fp8(x, weight, second, kernels.fp8_rows(24, 1024, "cuda"))
+        stream.synchronize()
+        assert torch.equal(second, out)
+
+
+def test_refusals():
+    from qwen_triton_b200.ops import kernels
+    Error = kernels.KernelError
+    values, scales = (t.cuda() for t in _weight(256, 384, 9))
+    weight = kernels.Fp8Weight(values, scales)
+    with pytest.raises(Error, match="values"):
+        kernels.Fp8Weight(values.float(), scales)
+    with pytest.raises(Error, match="scales"):
+        kernels.Fp8Weight(values, scales[:, :2])
+    with pytest.raises(Error, match="contiguous"):
+        kernels.Fp8Weight(values[:, :128], scales[:, :1].contiguous())
+    x, out = torch.zeros((4, 384), device="cuda"), torch.empty((4, 256), device="cuda")
+    rows = kernels.fp8_rows(4, 384, "cuda")
+    with pytest.raises(Error, match="scratch"):
+        kernels.gemm_fp8(x, weight, out)
+    with pytest.raises(Error, match="scratch"):
+        kernels.gemm_fp8(x, weight, out, kernels.fp8_rows(3, 384, "cuda"))
+    with pytest.raises(Error, match="out"):
+        kernels.gemm_fp8(x, weight, out[:, :100].contiguous(), rows)
+    with pytest.raises(Error, match="neither"):
+        kernels.gemm_fp8(x, weight, out.half(), rows)
+    with pytest.raises(Error, match="neither"):
+        kernels.gemm_fp8(x.half(), weight, out, rows)
+    with pytest.raises(Error, match="rows"):
+        kernels.gemm_fp8(kernels.fp8_rows(4, 128, "cuda"), weight, out)
+    with pytest.raises(Error, match="CUDA"):
+        kernels.gemm_fp8(x.cpu(), weight, out, rows)
+    none = torch.empty((0, 256), device="cuda")
+    kernels.gemm_fp8(x[:0], weight, none, rows)                # nothing to do
