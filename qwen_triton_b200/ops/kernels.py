@@ -144,8 +144,8 @@ _SIGNATURES = {
         # x, dtype, values, scales, rows, k, stream
         "qt_quantise_rows": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
         "qt_quantise_weight": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
-        # x8, x_scale, w8, w_scale, out, dtype, rows, n, k, status, stream
-        "qt_gemm_fp8": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr],
+        # x8, x_scale, w8, w_scale, out, dtype, rows, n, k, form, splits, status, stream
+        "qt_gemm_fp8": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr],
     },
     "cache8": {
         # qkv, in_dtype, n_splits, split_stride, q_out, out_dtype, k, v, k_scale, v_scale, seq_start, seq_past, n_seqs, max_q_len, block_table, max_blocks, n_pages,
@@ -1662,8 +1662,8 @@ def _same_device(name: str, *tensors: torch.Tensor) -> None:
 
 
 def quantise_rows_fp8(x: torch.Tensor, rows: Fp8Rows) -> None:
-    """rows = x [M, K] (bfloat16 or float32) in 8 bits: of each row and 128 columns the scale is s = max(amax / 448, 2^-100) and the values are x / s (in
-    float) rounded to e4m3.  A row with a number that is not finite has NaN in its place."""
+    """rows = x [M, K] (bfloat16 or float32) in 8 bits: of each row and 128 columns the scale is s = max(amax r, 2^-100), r the float next to
+    1 / 448, and the values are x / s (in float) rounded to e4m3.  A row with a number that is not finite has NaN in its place."""
     _need(x, "x", shape=rows.shape)
     _same_device("quantise_rows_fp8", x, rows.values)
     _call("gemm_fp8", "qt_quantise_rows", _ptr(x), _code(x, "x"), _ptr(rows.values), _ptr(rows.scales), *x.shape, _stream())
@@ -1683,15 +1683,30 @@ def quantise_weight_fp8(weight: torch.Tensor) -> Fp8Weight:
     return out
 
 
-def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None = None) -> None:
+@functools.lru_cache(maxsize=4096)
+def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
+    """(form, ranges of K) of the product of ``m`` rows and a weight [n, k]: form 0 takes any sizes, 16 to 128 few rows in tiles of so many, 256 many rows."""
+    if k % 16:
+        return 0, 1
+    if m > 128:
+        return 256, 1
+    tile = next(t for t in (16, 32, 64, 128) if m <= t)
+    groups, tiles = -(-k // FP8_GROUP), -(-n // 128)
+    splits = max(1, min(8, groups // 2, 2 * sms // tiles))
+    return tile, splits
+
+
+def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None = None, plan: tuple[int, int] | None = None) -> None:
     """out [M, N] (bfloat16 or float32) = x [M, K] W^T with both operands in 8 bits and their scales on the sums of each 128 columns, in float, rounded once.
 
     ``x`` is ``Fp8Rows``, or bfloat16 or float32 rows that are brought to 8 bits first (``quantise_rows_fp8``), through ``scratch`` (``fp8_rows(M, K)``, or
-    larger in M: its leading rows serve)."""
+    larger in M: its leading rows serve).  ``plan``: ``fp8_plan``'s, or another one of its kind."""
     n, k = weight.shape
     m = x.shape[0]
     _need(out, "out", shape=(m, n))
-    launches = 1
+    form, splits = plan or fp8_plan(m, n, k)
+    if form not in (0, 16, 32, 64, 128, 256) or not 1 <= splits <= 8:
+        raise KernelError(f"gemm_fp8: a plan {plan}")
     if not isinstance(x, Fp8Rows):
         if scratch is None or scratch.shape[1] != k or scratch.shape[0] < m:
             raise KernelError(f"gemm_fp8: scratch for {m} x {k} rows in 8 bits is required, got {None if scratch is None else tuple(scratch.shape)}")
@@ -1704,7 +1719,7 @@ def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, 
         raise KernelError(f"gemm_fp8: rows {tuple(x.shape)} for a weight {tuple(weight.shape)}")
     _same_device("gemm_fp8", x.values, weight.values, out)
     _call("gemm_fp8", "qt_gemm_fp8", _ptr(x.values), _ptr(x.scales), _ptr(weight.values), _ptr(weight.scales), _ptr(out), _code(out, "out"), m, n, k,
-          _ptr(_status_word(out.device)), _stream(), launches=launches)
+          form, splits, _ptr(_status_word(out.device)), _stream())
 
 
 # ----------------------------------------------------------------------------- a cache of keys and values in 8 bits

@@ -6,6 +6,7 @@ import math
 import torch
 
 TOP, GROUP, PAGE = 448.0, 128, 64
+PER_TOP = torch.tensor(1 / TOP, dtype=torch.float32)          # what the largest number is multiplied by for a scale
 
 
 def as_e4m3(x: torch.Tensor) -> torch.Tensor:
@@ -18,14 +19,14 @@ def as_e4m3(x: torch.Tensor) -> torch.Tensor:
 
 
 def quantise_rows(x: torch.Tensor):
-    """(values float64 [M, K], scales float32 [groups, M]): division and scale in float32, as they are defined."""
+    """(values float64 [M, K], scales float32 [groups, M]): the scale and the division in float32, as they are defined."""
     m, k = x.shape
     x = x.float().cpu()
     groups = -(-k // GROUP)
     values, scales = torch.empty((m, k), dtype=torch.float64), torch.empty((groups, m))
     for g in range(groups):
         piece = x[:, g * GROUP:(g + 1) * GROUP]
-        scales[g] = (piece.nan_to_num(0.0, math.inf, -math.inf).abs().amax(1) / TOP).clamp(min=2.0 ** -100)
+        scales[g] = (piece.nan_to_num(0.0, math.inf, -math.inf).abs().amax(1) * PER_TOP).clamp(min=2.0 ** -100)
         values[:, g * GROUP:(g + 1) * GROUP] = as_e4m3(piece / scales[g][:, None])
     return values, scales
 
@@ -38,7 +39,7 @@ def quantise_weight(w: torch.Tensor):
     for i in range(scales.shape[0]):
         for g in range(scales.shape[1]):
             at = (slice(i * GROUP, (i + 1) * GROUP), slice(g * GROUP, (g + 1) * GROUP))
-            scales[i, g] = (w[at].abs().amax() / TOP).clamp(min=2.0 ** -100)
+            scales[i, g] = (w[at].abs().amax() * PER_TOP).clamp(min=2.0 ** -100)
             values[at] = as_e4m3(w[at] / scales[i, g])
     return values, scales
 

@@ -27,12 +27,12 @@ def _weight(n, k, seed):
     return values, scales
 
 
-def _check_product(m, n, k, dtype, out_dtype=None, seed=0):
+def _check_product(m, n, k, dtype, out_dtype=None, seed=0, plan=None):
     from qwen_triton_b200.ops import kernels
     x, (values, scales) = _rows(m, k, dtype, seed), _weight(n, k, seed + 1)
     out = torch.full((m, n), math.nan, dtype=out_dtype or dtype, device="cuda")
     weight = kernels.Fp8Weight(values.cuda(), scales.cuda())
-    kernels.gemm_fp8(x.cuda(), weight, out, kernels.fp8_rows(m, k, "cuda"))
+    kernels.gemm_fp8(x.cuda(), weight, out, kernels.fp8_rows(m, k, "cuda"), plan)
     want, bound = plain.product(*plain.quantise_rows(x), values.double(), scales)
     bound = bound + want.abs() * torch.finfo(out.dtype).eps / 2 * (1 + 2 ** -8)
     off = (out.double().cpu() - want).abs()
@@ -62,6 +62,14 @@ def test_product_in_float32(m, n, k):
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (8, 6144, 4096), (700, 5120, 1024), (2048, 2560, 512)])
 def test_product_of_many_tiles(m, n, k):
     _check_product(m, n, k, torch.bfloat16)
+
+
+@pytest.mark.parametrize("form,splits", [(0, 1), (256, 1)] + [(form, splits) for form in (16, 32, 64, 128) for splits in (1, 2, 3, 5, 7, 8)])
+@pytest.mark.parametrize("m,n,k", [(1, 130, 1040), (150, 300, 1040), (33, 256, 400), (129, 512, 112)])
+def test_product_by_every_plan(form, splits, m, n, k):
+    """Any plan gives the result, more ranges than K has blocks among them."""
+    _check_product(m, n, k, torch.bfloat16, torch.float32, plan=(form, splits))
+    _check_product(m, n, k, torch.bfloat16, plan=(form, splits))
 
 
 def test_the_same_rows_give_the_same_bits():
@@ -179,5 +187,8 @@ def test_refusals():
         kernels.gemm_fp8(kernels.fp8_rows(4, 128, "cuda"), weight, out)
     with pytest.raises(Error, match="CUDA"):
         kernels.gemm_fp8(x.cpu(), weight, out, rows)
+    for plan in ((48, 1), (16, 0), (16, 9)):
+        with pytest.raises(Error, match="plan"):
+            kernels.gemm_fp8(x, weight, out, rows, plan)
     none = torch.empty((0, 256), device="cuda")
     kernels.gemm_fp8(x[:0], weight, none, rows)                # nothing to do
