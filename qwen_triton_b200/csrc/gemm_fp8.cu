@@ -18,27 +18,48 @@ namespace {
 constexpr float LEAST_SCALE = 0x1p-100f, PER_TOP = 1.f / TOP;
 
 // ----------------------------------------------------------------------------- rows in 8 bits
-// A warp a row and 128 columns, four columns a lane.  Scales as [group, row].
+// Four neighbouring columns a lane.  WIDE: rows begin where four elements do.
+template <typename T> __device__ __forceinline__ void load4(float (&v)[4], const T* row, int c0, int k, bool wide) {
+    if (wide && c0 + 4 <= k) {
+        if constexpr (sizeof(T) == 2) {
+            const uint2 two = *reinterpret_cast<const uint2*>(row + c0);
+            const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two.y));
+            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+        } else {
+            const float4 f = *reinterpret_cast<const float4*>(row + c0);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = c0 + i < k ? to_float(row[c0 + i]) : 0.f;
+    }
+}
+// A warp's 128 columns in 8 bits, four a lane, and their scale.
+__device__ __forceinline__ uint32_t quantise4(const float (&v)[4], float& scale) {
+    const float largest = warp_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+    scale = fmaxf(__fmul_rn(largest, PER_TOP), LEAST_SCALE);
+    return pack4(__fdiv_rn(v[0], scale), __fdiv_rn(v[1], scale), __fdiv_rn(v[2], scale), __fdiv_rn(v[3], scale));
+}
+// A warp a row and 128 columns.  Scales as [group, row].
 template <typename T>
-__global__ void __launch_bounds__(256) quantise_rows_kernel(const T* x, uint8_t* values, float* scales, int rows, int k, int groups) {
+__global__ void __launch_bounds__(256) quantise_rows_kernel(const T* x, uint8_t* values, float* scales, int rows, int k, int groups, int wide) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (unit >= (long long)rows * groups) return;
     const int m = (int)(unit / groups), g = (int)(unit % groups), c0 = g * GROUP + lane * 4;
-    const T* row = x + (size_t)m * k;
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c0 + i < k ? to_float(row[c0 + i]) : 0.f;
-    const float largest = warp_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
-    const float scale = fmaxf(__fmul_rn(largest, PER_TOP), LEAST_SCALE);
+    float v[4], scale;
+    load4(v, x + (size_t)m * k, c0, k, wide);
+    const uint32_t four = quantise4(v, scale);
     if (lane == 0) scales[(size_t)g * rows + m] = scale;
+    uint8_t* to = values + (size_t)m * k + c0;
+    if (wide && c0 + 4 <= k) {
+        *reinterpret_cast<uint32_t*>(to) = four;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-        const uint32_t two = pack2(__fdiv_rn(v[i], scale), __fdiv_rn(v[i + 1], scale));
-        if (c0 + i < k) values[(size_t)m * k + c0 + i] = (uint8_t)two;
-        if (c0 + i + 1 < k) values[(size_t)m * k + c0 + i + 1] = (uint8_t)(two >> 8);
+        for (int i = 0; i < 4; ++i)
+            if (c0 + i < k) to[i] = (uint8_t)(four >> (8 * i));
     }
 }
 
@@ -109,13 +130,22 @@ __global__ void __launch_bounds__(256) gemm_fp8_any_kernel(const uint8_t* x8, co
 constexpr int BM = 128;                                     // the instruction's M
 constexpr uint32_t A_BYTES = BM * GROUP;
 
-__device__ __forceinline__ void umma_fp8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+// A whole warp goes through the same instructions, so that descriptors stay in the registers that a warp has in common, and one lane's products are carried out:
+// issued by a lane that runs alone, a product takes about 100 cycles to leave and a commit 180, more than the tensor cores need for it.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    return elected;
 }
+__device__ __forceinline__ void umma_fp8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+// Arrives at the barrier once the products issued so far are complete.
+__device__ __forceinline__ void commit_one(uint32_t bar, uint32_t one) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one) : "memory");
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code)); }
 __device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int c_inner, int c_outer) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c_inner), "r"(c_outer) : "memory");
 }
@@ -152,58 +182,83 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 struct GemmParams {
+    const void* x; int x_wide;                              // FUSED: the rows as they are, and whether they begin where four elements do
     const float* x_scale; const float* w_scale; void* out;
-    int rows, n, groups;
+    int rows, n, k, groups;
     int groups_per_split;
-    int wide;                                               // rows of the output begin at 32-byte boundaries
+    int wide;                                               // rows of the output begin at boundaries of 32 bytes (2) or of four numbers (1)
     int* status;
 };
 
 // Few rows.  The weight's rows are the instruction's M (a tile is one row of scale blocks), BX rows of x its N; a cluster's blocks take a range of K each and add
-// their sums through distributed shared memory in the order of their ranks.  192 threads: warp 0 copies, warp 1 issues, warps 2 to 5 add up, a weight row a thread.
-constexpr int FEW_THREADS = 192, PREFETCH = 16;
-template <int BX> struct Few {
-    static constexpr uint32_t STAGE_BYTES = A_BYTES + BX * GROUP;
-    static constexpr int PARK = BM + 1;                     // floats from one column of parked sums to the next
-    static size_t smem(int stages) { return (size_t)stages * STAGE_BYTES + 2 * BX * 4 + 8 * (2 * stages + 4) + 16 + 1024; }
+// their sums through distributed shared memory in the order of their ranks.  Warp 0 copies, warp 1 issues, the others add up, a weight row and CW rows of x a
+// thread.  Four accumulators: from the last product of a group to the slot's next one (a commit, two waits, the read) it takes about 1,000 cycles, and a group's
+// products 300.
+// XT: the type of rows that the summing warps bring to 8 bits themselves, straight into shared memory, ahead of their sums (few of them, in up to FUSED_GROUPS groups a
+// block: saves the launch); uint8_t: rows in 8 bits already.
+constexpr int PREFETCH = 16;                                // weight tiles asked into the L2 cache ahead of the wait
+constexpr int CHUNK = 16;                                   // groups whose scales are in shared memory at a time, twice
+constexpr int FEW_SLOTS = 4, FUSED_GROUPS = 2 * CHUNK;
+template <int BX, typename XT> struct Few {
+    static constexpr bool FUSED = sizeof(XT) > 1;
+    static constexpr int SUM_WARPS = BX >= 64 ? 8 : 4, CW = BX * 4 / SUM_WARPS, THREADS = 64 + 32 * SUM_WARPS;
+    static constexpr uint32_t X_BYTES = BX * GROUP, STAGE_BYTES = A_BYTES + (FUSED ? 0 : X_BYTES), SCALE_BYTES = 2 * CHUNK * BX * 4;
+    // ring, FUSED: the rows in 8 bits, scales, barriers, the address in tensor memory
+    static size_t smem(int stages, int groups) {
+        return (size_t)stages * STAGE_BYTES + (FUSED ? groups * X_BYTES : 0) + SCALE_BYTES + 8 * (2 * stages + 2 * FEW_SLOTS + (FUSED ? groups : 0)) + 16 + 1024;
+    }
 };
 
-template <int BX, typename TO>
-__global__ void __launch_bounds__(FEW_THREADS) gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GemmParams p,
-                                                                   int stages) {
-    constexpr uint32_t STAGE_BYTES = Few<BX>::STAGE_BYTES, TMEM_COLS = 2 * BX < 32 ? 32 : 2 * BX, IDESC = FP8_IDESC<BX>;
-    constexpr int PARK = Few<BX>::PARK;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    uint8_t* smem = smem_raw + (base - raw);
-    const uint32_t scales_at = stages * STAGE_BYTES, bars = base + scales_at + 2 * BX * 4;
-    const uint32_t full0 = bars, empty0 = bars + 8 * stages, acc_full = empty0 + 8 * stages, acc_empty = acc_full + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (acc_empty + 16 - base));
-    float* column_scale = reinterpret_cast<float*>(smem + scales_at);                       // [2][BX]
+template <typename TO> __device__ __forceinline__ void store4(TO* at, const float (&y)[4], int there, bool wide) {
+    if (wide && there >= 4) {
+        if constexpr (sizeof(TO) == 2) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
+            *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+            *reinterpret_cast<float4*>(at) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < there) at[i] = from_float<TO>(y[i]);
+    }
+}
 
+template <int BX, typename XT, typename TO>
+__global__ void __launch_bounds__(Few<BX, XT>::THREADS) gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                                            const GemmParams p, int stages) {
+    using F = Few<BX, XT>;
+    constexpr bool FUSED = F::FUSED;
+    constexpr uint32_t STAGE_BYTES = F::STAGE_BYTES, TMEM_COLS = FEW_SLOTS * BX, IDESC = FP8_IDESC<BX>;
+    constexpr int CW = F::CW, SUM_THREADS = 32 * F::SUM_WARPS;
+    extern __shared__ uint8_t smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x, splits = gridDim.x, w0 = blockIdx.y * BM, x0 = blockIdx.z * BX;
     const int g_begin = split * p.groups_per_split, count = min(p.groups, g_begin + p.groups_per_split) - g_begin;      // >= 1: the host cuts so
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - raw);
+    const uint32_t rows_at = stages * STAGE_BYTES, scales_at = rows_at + (FUSED ? p.groups_per_split * F::X_BYTES : 0), bars = base + scales_at + F::SCALE_BYTES;
+    const uint32_t full0 = bars, empty0 = bars + 8 * stages, acc_full = empty0 + 8 * stages, acc_empty = acc_full + 8 * FEW_SLOTS, x_full = acc_empty + 8 * FEW_SLOTS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (x_full + (FUSED ? 8 * p.groups_per_split : 0) - base));
+    float* scales = reinterpret_cast<float*>(smem + scales_at);                             // [2][CHUNK][BX]
     int* status = p.status;
     if (threadIdx.x == 0) {
         prefetch_tensor_map(&map_w);
-        prefetch_tensor_map(&map_x);
+        if (!FUSED) prefetch_tensor_map(&map_x);
         for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4); }
+        for (int s = 0; s < FEW_SLOTS; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, F::SUM_WARPS); }
+        if (FUSED)
+            for (int i = 0; i < count; ++i) mbar_init(x_full + 8 * i, p.rows);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
-    pdl_launch_dependents();                                // not before the columns are this block's: a dependent's block must not take them first and wait
-    float acc[BX];
-#pragma unroll
-    for (int c = 0; c < BX; ++c) acc[c] = 0.f;
+    // The address in tensor memory, for the issuing and the summing warps.  Columns are taken once the kernels before this one are done (their blocks never wait for
+    // columns that this one holds), and dependents are let in once this block has its own.
+    auto columns = [&]() {
+        asm volatile("bar.sync 2, %0;" ::"n"(SUM_THREADS + 32) : "memory");
+        tc_fence_after();
+        return *(volatile uint32_t*)tmem_slot;
+    };
 
     if (warp == 0) {
         if (lane == 0) {
@@ -216,72 +271,129 @@ __global__ void __launch_bounds__(FEW_THREADS) gemm_fp8_few_kernel(const __grid_
                 mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
                 const uint32_t dst = base + s * STAGE_BYTES;
                 tma_load_2d(dst, &map_w, full0 + 8 * s, (g_begin + i) * GROUP, w0);
-                tma_load_2d(dst + A_BYTES, &map_x, full0 + 8 * s, (g_begin + i) * GROUP, x0);
+                if (!FUSED) tma_load_2d(dst + A_BYTES, &map_x, full0 + 8 * s, (g_begin + i) * GROUP, x0);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint64_t a_desc0 = operand_desc(base), b_desc0 = operand_desc(base + A_BYTES);
-            for (int i = 0; i < count; ++i) {
-                const int s = i % stages, b = i & 1;
-                if (i >= 2 && !mbar_wait(acc_empty + 8 * b, (uint32_t)(i / 2 - 1) & 1u, status, 2)) break;
-                if (!mbar_wait(full0 + 8 * s, (uint32_t)(i / stages) & 1u, status, 2)) break;
-                tc_fence_after();
-                const uint64_t step = (uint64_t)(s * (STAGE_BYTES >> 4));
+        pdl_wait();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        const uint32_t tmem_base = columns();
+        pdl_launch_dependents();
+        const uint64_t a_desc0 = operand_desc(base), b_desc0 = operand_desc(base + (FUSED ? rows_at : A_BYTES));
+        const uint32_t one = elect_one();
+        int s = 0;
+        uint32_t phase = 0;
+        for (int i = 0; i < count; ++i) {
+            const int b = i % FEW_SLOTS;
+            if (i >= FEW_SLOTS && !wait_warp(acc_empty + 8 * b, (uint32_t)(i / FEW_SLOTS - 1) & 1u, status, 2)) break;
+            if (FUSED && !wait_warp(x_full + 8 * i, 0, status, 2)) break;
+            if (!wait_warp(full0 + 8 * s, phase, status, 2)) break;
+            tc_fence_after();
+            const uint64_t a_desc = a_desc0 + (uint64_t)(s * (STAGE_BYTES >> 4)), b_desc = b_desc0 + (uint64_t)(FUSED ? i * (F::X_BYTES >> 4) : s * (STAGE_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < GROUP / 32; ++k) umma_fp8(tmem_base + b * BX, a_desc0 + step + 2 * k, b_desc0 + step + 2 * k, IDESC, k > 0 ? 1u : 0u);
-                umma_commit(empty0 + 8 * s);
-                umma_commit(acc_full + 8 * b);
-            }
+            for (int k = 0; k < GROUP / 32; ++k) umma_fp8(tmem_base + b * BX, a_desc + 2 * k, b_desc + 2 * k, IDESC, k > 0 ? 1u : 0u, one);
+            commit_one(acc_full + 8 * b, one);
+            commit_one(empty0 + 8 * s, one);
+            if (++s == stages) { s = 0; phase ^= 1u; }
         }
     } else {
-        const int quarter = warp & 3, column = (warp - 2) * 32 + lane;
-        pdl_wait();                                         // the rows' scales come from the kernel before; the output may still be read by one
-        const float* w_scale = p.w_scale + (size_t)blockIdx.y * p.groups;
-        auto scale_of = [&](int g) { return column < BX && x0 + column < p.rows ? p.x_scale[(size_t)g * p.rows + x0 + column] * w_scale[g] : 0.f; };
-        float mine = scale_of(g_begin);
+        const int quarter = warp & 3, part = (warp - 2) >> 2, row = quarter * 32 + lane, thread = threadIdx.x - 64;
+        constexpr int PER = CHUNK * BX / SUM_THREADS;       // scales of a chunk that a thread fetches
+        pdl_wait();                                         // the rows come from the kernel before; the output may still be read by one
+        const uint32_t tmem_base = columns();
+        const float* w_scale = p.w_scale + (size_t)blockIdx.y * p.groups + g_begin;
+        float fetched[PER];
+        auto fetch = [&](int i0) {
+            const float* x_scale = p.x_scale + (size_t)g_begin * p.rows + x0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int e = thread + j * SUM_THREADS, i = i0 + e / BX, c = e % BX;
+                fetched[j] = i < count && x0 + c < p.rows ? x_scale[(size_t)i * p.rows + c] * w_scale[i] : 0.f;
+            }
+        };
+        if constexpr (FUSED) {
+            // units of a group and row, four at a time in flight; as the swizzle of 128 bytes has them: 16-byte pieces of a row, their number xor the row's
+            const XT* x = (const XT*)p.x;
+            const int units = count * p.rows;
+            for (int u0 = warp - 2; u0 < units; u0 += 4 * F::SUM_WARPS) {
+                float v[4][4], by[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int u = u0 + j * F::SUM_WARPS, i = u / p.rows, m = u % p.rows;
+                    if (u < units) {
+                        load4(v[j], x + (size_t)m * p.k, (g_begin + i) * GROUP + lane * 4, p.k, p.x_wide);
+                        by[j] = w_scale[i];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int u = u0 + j * F::SUM_WARPS, i = u / p.rows, m = u % p.rows;
+                    if (u >= units) break;
+                    float scale;
+                    const uint32_t four = quantise4(v[j], scale);
+                    *reinterpret_cast<uint32_t*>(smem + rows_at + i * F::X_BYTES + m * GROUP + (((lane >> 2) ^ (m & 7)) << 4) + ((lane & 3) << 2)) = four;
+                    if (lane == 0) scales[i * BX + m] = scale * by[j];
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the products read it
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(x_full + 8 * i);
+                }
+            }
+        } else {
+            fetch(0);
+        }
+        uint64_t acc[CW / 2];
+#pragma unroll
+        for (int c = 0; c < CW / 2; ++c) acc[c] = 0ull;
         bool ok = true;                                     // a wait that gave up ends the work, not the way through the barriers
+        if (FUSED) asm volatile("bar.sync 1, %0;" ::"n"(SUM_THREADS) : "memory");           // every scale is there
         for (int i = 0; i < count; ++i) {
-            const int b = i & 1;
-            float* scale = column_scale + b * BX;
-            if (column < BX) scale[column] = mine;
-            if (i + 1 < count) mine = scale_of(g_begin + i + 1);
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            ok = ok && mbar_wait(acc_full + 8 * b, (uint32_t)(i / 2) & 1u, status, 3);
+            const int b = i % FEW_SLOTS;
+            float* chunk = scales + ((i / CHUNK) & 1) * (CHUNK * BX);
+            if (!FUSED && i % CHUNK == 0) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) chunk[thread + j * SUM_THREADS] = fetched[j];
+                if (i + CHUNK < count) fetch(i + CHUNK);
+                asm volatile("bar.sync 1, %0;" ::"n"(SUM_THREADS) : "memory");
+            }
+            ok = ok && mbar_wait(acc_full + 8 * b, (uint32_t)(i / FEW_SLOTS) & 1u, status, 3);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) continue;
             tc_fence_after();
-            const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * BX);
+            const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * BX + part * CW);
+            uint32_t v[CW / 16][16];
 #pragma unroll
-            for (int c0 = 0; c0 < BX; c0 += 16) {
-                uint32_t v[16];
-                tmem_load16(at + (uint32_t)c0, v);
-                if (c0 + 16 == BX) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty + 8 * b);
-                }
+            for (int c = 0; c < CW / 16; ++c) tmem_load16_start(at + 16 * c, v[c]);
+            const float* by = chunk + (i % CHUNK) * BX + part * CW;
+            tmem_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty + 8 * b);
 #pragma unroll
-                for (int c = 0; c < 16; c += 4) {
-                    const float4 by = *reinterpret_cast<const float4*>(scale + c0 + c);
-                    acc[c0 + c] = fmaf(__uint_as_float(v[c]), by.x, acc[c0 + c]);
-                    acc[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), by.y, acc[c0 + c + 1]);
-                    acc[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), by.z, acc[c0 + c + 2]);
-                    acc[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), by.w, acc[c0 + c + 3]);
-                }
+            for (int c = 0; c < CW; c += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(by + c);
+                acc[c / 2] = fma2(pair_u32(v[c / 16][c % 16], v[c / 16][c % 16 + 1]), pair_f32(f.x, f.y), acc[c / 2]);
+                acc[c / 2 + 1] = fma2(pair_u32(v[c / 16][c % 16 + 2], v[c / 16][c % 16 + 3]), pair_f32(f.z, f.w), acc[c / 2 + 1]);
             }
         }
-        const int row = quarter * 32 + lane;
         if (splits == 1) {
             if (w0 + row < p.n) {
 #pragma unroll
-                for (int c = 0; c < BX; ++c)
-                    if (x0 + c < p.rows) ((TO*)p.out)[(size_t)(x0 + c) * p.n + w0 + row] = from_float<TO>(acc[c]);
+                for (int c = 0; c < CW; ++c) {
+                    const float2 y = unpair(acc[c / 2]);
+                    const int m = x0 + part * CW + c;
+                    if (m < p.rows) ((TO*)p.out)[(size_t)m * p.n + w0 + row] = from_float<TO>((c & 1) ? y.y : y.x);
+                }
             }
         } else {
-            float* park = reinterpret_cast<float*>(smem);   // over the ring: every product that read it is complete
+            float* park = reinterpret_cast<float*>(smem);   // [BX][BM] over the ring: every product that read it is complete
+            // (after a wait that gave up, copies may still land there; the result is invalid then)
 #pragma unroll
-            for (int c = 0; c < BX; ++c) park[c * PARK + row] = acc[c];
+            for (int c = 0; c < CW; ++c) {
+                const float2 y = unpair(acc[c / 2]);
+                park[(part * CW + c) * BM + row] = (c & 1) ? y.y : y.x;
+            }
         }
     }
     tc_fence_before();
@@ -290,30 +402,37 @@ __global__ void __launch_bounds__(FEW_THREADS) gemm_fp8_few_kernel(const __grid_
         const unsigned long long t0 = global_timer();
         while (global_timer() - t0 < 2000000ull) __nanosleep(1000);
     }
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*(volatile uint32_t*)tmem_slot), "r"(TMEM_COLS) : "memory");
     if (splits > 1) {
         cluster_sync_all();
-        // the block of rank r finishes columns r, r + splits, ...: the ranks' sums one after the other
-        const uint32_t park = base;
-        for (int i = threadIdx.x; i < (BX / splits + 1) * BM; i += FEW_THREADS) {
-            const int c = (i >> 7) * splits + split, row = i & (BM - 1);
+        // the block of rank r finishes columns r, r + splits, ..., four weight rows a thread: the ranks' sums one after the other
+        for (int i = threadIdx.x;; i += F::THREADS) {
+            const int c = (i >> 5) * splits + split, row = (i & 31) * 4;
             if (c >= BX || x0 + c >= p.rows) break;
-            float sum = 0.f;
-            for (int r = 0; r < splits; ++r) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(park + (uint32_t)(c * PARK + row) * 4, r)) : "memory");
-                sum += v;
-            }
-            if (w0 + row < p.n) ((TO*)p.out)[(size_t)(x0 + c) * p.n + w0 + row] = from_float<TO>(sum);
+            float v[8][4];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < splits)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[r][0]), "=f"(v[r][1]), "=f"(v[r][2]), "=f"(v[r][3])
+                                 : "r"(map_to_cta(base + (uint32_t)(c * BM + row) * 4, r)) : "memory");
+            float sum[4] = {};
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] += r < splits ? v[r][j] : 0.f;
+            if (w0 + row < p.n) store4((TO*)p.out + (size_t)(x0 + c) * p.n + w0 + row, sum, p.n - w0 - row, p.wide != 0);
         }
         cluster_sync_all();                                 // nobody leaves while its sums are read
     }
 }
 
-// Many rows.  128 rows of x are the instruction's M, 256 weight rows its N; eight warps add up, a row of x and 128 weight rows (one scale block) a thread.  One block
-// an SM walks tiles; 320 threads: warp 0 copies, warp 1 issues, warps 2 to 9 add up and store.
-constexpr int BN = 256, MANY_THREADS = 320, MANY_STAGES = 4;
-constexpr uint32_t B_BYTES = BN * GROUP, MANY_STAGE_BYTES = A_BYTES + B_BYTES;
+// Many rows.  128 rows of x are the instruction's M, 256 weight rows its N; eight warps add up, a row of x and 128 weight rows (of one scale block) a thread.  One
+// block an SM walks tiles.  320 threads: warp 0 copies, warp 1 issues, warps 2 to 9 add up and store.  SPLIT: a cluster a tile, whose blocks take a range of K each and
+// add their sums through distributed shared memory, as for few rows.
+constexpr int BN = 256, PARK_ROW = BN + 4;                  // floats from a row of parked sums to the next: 16 bytes of eight neighbouring rows are all the banks
+constexpr int MANY_THREADS = 320, MANY_STAGES = 4, MANY_SLOTS = 512 / BN, MANY_CW = BN / 2;
+constexpr uint32_t MANY_STAGE_BYTES = A_BYTES + BN * GROUP;
+constexpr size_t MANY_SMEM = (size_t)MANY_STAGES * MANY_STAGE_BYTES + 8 * (2 * MANY_STAGES + 2 * MANY_SLOTS) + 16 + 1024;
 constexpr int RASTER = 8;
 
 __device__ __forceinline__ void tile_of(int t, int w_tiles, int x_tiles, int& w, int& x) {     // groups of RASTER weight tiles, in a group rows of tiles
@@ -322,25 +441,29 @@ __device__ __forceinline__ void tile_of(int t, int w_tiles, int x_tiles, int& w,
     x = r / width;
 }
 
-template <typename TO>
+template <bool SPLIT, typename TO>
 __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GemmParams p) {
-    constexpr uint32_t IDESC = FP8_IDESC<BN>, TMEM_COLS = 2 * BN;
+    constexpr int STAGES = MANY_STAGES, SLOTS = MANY_SLOTS, CW = MANY_CW;
+    constexpr uint32_t IDESC = FP8_IDESC<BN>, TMEM_COLS = 512, STAGE_BYTES = MANY_STAGE_BYTES;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw);
-    const uint32_t bars = base + MANY_STAGES * MANY_STAGE_BYTES;
-    const uint32_t full0 = bars, empty0 = bars + 8 * MANY_STAGES, acc_full = empty0 + 8 * MANY_STAGES, acc_empty = acc_full + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (acc_empty + 16 - base));
+    const uint32_t bars = base + STAGES * STAGE_BYTES;
+    const uint32_t full0 = bars, empty0 = bars + 8 * STAGES, acc_full = empty0 + 8 * STAGES, acc_empty = acc_full + 8 * SLOTS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (acc_empty + 8 * SLOTS - base));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int w_tiles = (p.n + BN - 1) / BN, x_tiles = (p.rows + BM - 1) / BM, tiles = w_tiles * x_tiles;
+    const int splits = SPLIT ? gridDim.x : 1, split = SPLIT ? blockIdx.x : 0, first = SPLIT ? blockIdx.y : blockIdx.x, step = SPLIT ? gridDim.y : gridDim.x;
+    const int g_begin = split * p.groups_per_split, count = min(p.groups, g_begin + p.groups_per_split) - g_begin;
     int* status = p.status;
     if (threadIdx.x == 0) {
         prefetch_tensor_map(&map_w);
         prefetch_tensor_map(&map_x);
-        for (int s = 0; s < MANY_STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 8); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    pdl_wait();                                             // ahead of the columns: see the kernel for few rows
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -349,67 +472,74 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    pdl_launch_dependents();                                // not before the columns are this block's: a dependent's block must not take them first and wait
+    pdl_launch_dependents();
     if (warp == 0) {
         if (lane == 0) {
-            pdl_wait();
             int s = 0;
             uint32_t phase = 1;
             bool ok = true;
-            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            for (int tile = first; tile < tiles && ok; tile += step) {
                 int w, x;
                 tile_of(tile, w_tiles, x_tiles, w, x);
-                for (int g = 0; g < p.groups; ++g) {
+                                for (int g = 0; g < count; ++g) {
                     ok = mbar_wait(empty0 + 8 * s, phase, status, 1);
                     if (!ok) break;
-                    mbar_expect_tx(full0 + 8 * s, MANY_STAGE_BYTES);
-                    const uint32_t dst = base + s * MANY_STAGE_BYTES;
-                    tma_load_2d(dst, &map_x, full0 + 8 * s, g * GROUP, x * BM);
-                    tma_load_2d(dst + A_BYTES, &map_w, full0 + 8 * s, g * GROUP, w * BN);
-                    if (++s == MANY_STAGES) { s = 0; phase ^= 1u; }
+                    mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
+                    const uint32_t dst = base + s * STAGE_BYTES;
+                    tma_load_2d(dst, &map_x, full0 + 8 * s, (g_begin + g) * GROUP, x * BM);
+                    tma_load_2d(dst + A_BYTES, &map_w, full0 + 8 * s, (g_begin + g) * GROUP, w * BN);
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint64_t a_desc0 = operand_desc(base), b_desc0 = operand_desc(base + A_BYTES);
-            int s = 0, b = 0;
-            uint32_t phase = 0, acc_phase = 1;
-            bool ok = true;
-            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x)
-                for (int g = 0; g < p.groups; ++g) {
-                    ok = mbar_wait(acc_empty + 8 * b, acc_phase, status, 2) && mbar_wait(full0 + 8 * s, phase, status, 2);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t step = (uint64_t)(s * (MANY_STAGE_BYTES >> 4));
+        const uint64_t a_desc0 = operand_desc(base), b_desc0 = operand_desc(base + A_BYTES);
+        const uint32_t one = elect_one();
+        int s = 0, b = 0;
+        uint32_t phase = 0, acc_phase = 1;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step)
+            for (int g = 0; g < count; ++g) {
+                ok = wait_warp(full0 + 8 * s, phase, status, 2) && wait_warp(acc_empty + 8 * b, acc_phase, status, 2);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t at = (uint64_t)(s * (STAGE_BYTES >> 4));
 #pragma unroll
-                    for (int k = 0; k < GROUP / 32; ++k) umma_fp8(tmem_base + b * BN, a_desc0 + step + 2 * k, b_desc0 + step + 2 * k, IDESC, k > 0 ? 1u : 0u);
-                    umma_commit(empty0 + 8 * s);
-                    umma_commit(acc_full + 8 * b);
-                    if (++s == MANY_STAGES) { s = 0; phase ^= 1u; }
-                    if ((b ^= 1) == 0) acc_phase ^= 1u;
-                }
-        }
+                for (int k = 0; k < GROUP / 32; ++k) umma_fp8(tmem_base + b * BN, a_desc0 + at + 2 * k, b_desc0 + at + 2 * k, IDESC, k > 0 ? 1u : 0u, one);
+                commit_one(acc_full + 8 * b, one);
+                commit_one(empty0 + 8 * s, one);
+                if (++s == STAGES) { s = 0; phase ^= 1u; }
+                if (++b == SLOTS) { b = 0; acc_phase ^= 1u; }
+            }
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
-        pdl_wait();
-        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+        const int quarter = warp & 3, part = (warp - 2) >> 2, row = quarter * 32 + lane;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * CW);
         int b = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        for (int tile = first; tile < tiles && ok; tile += step) {
             int w, x;
             tile_of(tile, w_tiles, x_tiles, w, x);
-            const int m = x * BM + row, n0 = w * BN + half * 128;
-            const float* x_scale = p.x_scale + min(m, p.rows - 1);
-            const float* w_scale = p.w_scale + (size_t)min(n0 / GROUP, (p.n - 1) / GROUP) * p.groups;
-            uint64_t acc[64];
+            const int m = x * BM + row, n0 = w * BN + part * CW;
+            const float* x_scale = p.x_scale + (size_t)g_begin * p.rows + min(m, p.rows - 1);
+            const float* w_scale = p.w_scale + (size_t)min(n0 / GROUP, (p.n - 1) / GROUP) * p.groups + g_begin;
+            uint64_t acc[CW / 2];
 #pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] = 0ull;
-            float by = x_scale[0] * w_scale[0];
-            for (int g = 0; g < p.groups; ++g) {
-                const float now = by;
-                if (g + 1 < p.groups) by = x_scale[(size_t)(g + 1) * p.rows] * w_scale[g + 1];
+            for (int c = 0; c < CW / 2; ++c) acc[c] = 0ull;
+            // scales four groups at a time, the next four on their way: a group is shorter than their way from the L2 cache
+            float by[4], next[4];
+            auto fetch = [&](int g0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) next[i] = x_scale[(size_t)min(g0 + i, count - 1) * p.rows] * w_scale[min(g0 + i, count - 1)];
+            };
+            fetch(0);
+            for (int g = 0; g < count; ++g) {
+                if ((g & 3) == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) by[i] = next[i];
+                    if (g + 4 < count) fetch(g + 4);
+                }
+                const float now = (g & 2) ? (g & 1) ? by[3] : by[2] : (g & 1) ? by[1] : by[0];
                 ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, acc_phase, status, 3));
                 if (!ok) break;
                 tc_fence_after();
@@ -418,23 +548,33 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
                 uint32_t v[2][16];
                 tmem_load16_start(at, v[0]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < CW / 16; ++i) {
                     tmem_wait_ld();
-                    if (i < 7) tmem_load16_start(at + 16 * (i + 1), v[(i + 1) & 1]);
+                    if (i + 1 < CW / 16) {
+                        tmem_load16_start(at + 16 * (i + 1), v[(i + 1) & 1]);
+                    } else {                                // everything is read: the slot may take other sums
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_empty + 8 * b);
+                    }
 #pragma unroll
                     for (int c = 0; c < 8; ++c) acc[8 * i + c] = fma2(pair_u32(v[i & 1][2 * c], v[i & 1][2 * c + 1]), by2, acc[8 * i + c]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + 8 * b);
-                if ((b ^= 1) == 0) acc_phase ^= 1u;
+                if (++b == SLOTS) { b = 0; acc_phase ^= 1u; }
             }
             TO* dst = (TO*)p.out + (size_t)m * p.n + n0;
-            if (!ok || m >= p.rows) {
-            } else if (p.wide && n0 + 128 <= p.n) {
+            if (SPLIT) {
+                float* park = reinterpret_cast<float*>(smem) + row * PARK_ROW + part * CW;      // over the ring: every product that read it is complete
+#pragma unroll
+                for (int c = 0; c < CW / 2; c += 2) {
+                    const float2 lo = unpair(acc[c]), hi = unpair(acc[c + 1]);
+                    *reinterpret_cast<float4*>(park + 2 * c) = make_float4(lo.x, lo.y, hi.x, hi.y);
+                }
+            } else if (!ok || m >= p.rows) {
+            } else if (p.wide == 2 && n0 + CW <= p.n) {
                 constexpr int PER = 32 / sizeof(TO);       // numbers in 32 bytes
 #pragma unroll
-                for (int c = 0; c < 128; c += PER) {
+                for (int c = 0; c < CW; c += PER) {
                     uint32_t word[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -452,7 +592,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < 64; ++c) {
+                for (int c = 0; c < CW / 2; ++c) {
                     const float2 y = unpair(acc[c]);
                     if (n0 + 2 * c < p.n) dst[2 * c] = from_float<TO>(y.x);
                     if (n0 + 2 * c + 1 < p.n) dst[2 * c + 1] = from_float<TO>(y.y);
@@ -468,6 +608,33 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
         while (global_timer() - t0 < 2000000ull) __nanosleep(1000);
     }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    if (SPLIT) {
+        cluster_sync_all();
+        // the block of rank r finishes rows r, r + splits, ..., a warp a row, four neighbouring numbers a lane at a time
+        int w, x;
+        tile_of(first, w_tiles, x_tiles, w, x);
+        for (int i = warp; i * splits + split < BM; i += MANY_THREADS / 32) {
+            const int r = i * splits + split, m = x * BM + r;
+            if (m >= p.rows) break;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int c = half * 128 + lane * 4;
+                float v[8][4];
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < splits)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[q][0]), "=f"(v[q][1]), "=f"(v[q][2]), "=f"(v[q][3])
+                                     : "r"(map_to_cta(base + (uint32_t)(r * PARK_ROW + c) * 4, q)) : "memory");
+                float sum[4] = {};
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[j] += q < splits ? v[q][j] : 0.f;
+                if (w * BN + c < p.n) store4((TO*)p.out + (size_t)m * p.n + w * BN + c, sum, p.n - w * BN - c, p.wide != 0);
+            }
+        }
+        cluster_sync_all();                                 // nobody leaves while its sums are read
+    }
 }
 
 // ----------------------------------------------------------------------------- host side
@@ -483,56 +650,81 @@ int byte_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t k, uint3
     return QT_OK;
 }
 
-template <int BX, typename TO>
-int launch_few(const void* x8, const void* w8, GemmParams p, int k, int splits, cudaStream_t stream) {
+template <int BX, typename XT, typename TO>
+int launch_few(const void* x8, const void* w8, GemmParams p, int splits, cudaStream_t stream) {
+    using F = Few<BX, XT>;
     CUtensorMap map_w, map_x;
-    int rc = byte_map(&map_w, w8, p.n, k, BM);
+    int rc = byte_map(&map_w, w8, p.n, p.k, BM);
     if (rc) return rc;
-    rc = byte_map(&map_x, x8, p.rows, k, BX);
+    if (F::FUSED) map_x = map_w;                            // not used
+    else rc = byte_map(&map_x, x8, p.rows, p.k, BX);
     if (rc) return rc;
     p.groups_per_split = (p.groups + splits - 1) / splits;
     splits = (p.groups + p.groups_per_split - 1) / p.groups_per_split;
-    int stages = std::min(BX <= 32 ? 4 : 5, p.groups_per_split);
-    const int park = splits > 1 ? (int)((BX * Few<BX>::PARK * 4 + Few<BX>::STAGE_BYTES - 1) / Few<BX>::STAGE_BYTES) : 1;
+    QT_REQUIRE(splits >= 1 && splits <= 8 && (!F::FUSED || (p.groups_per_split <= FUSED_GROUPS && p.rows <= BX)), "gemm_fp8: %d ranges of %d groups", splits, p.groups_per_split);
+    int stages = std::min(4, p.groups_per_split);
+    const int park = splits > 1 ? (int)((BX * BM * 4 + F::STAGE_BYTES - 1) / F::STAGE_BYTES) : 1;
     stages = std::max(std::max(stages, park), 2);
-    const cudaError_t raised = raise_shared<gemm_fp8_few_kernel<BX, TO>>(227 * 1024);
+    const cudaError_t raised = raise_shared<gemm_fp8_few_kernel<BX, XT, TO>>(227 * 1024);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "gemm_fp8: cannot raise shared memory: %s", cudaGetErrorString(raised));
-    launch_kernel_cluster(gemm_fp8_few_kernel<BX, TO>, dim3(splits, (p.n + BM - 1) / BM, (p.rows + BX - 1) / BX), dim3(FEW_THREADS), Few<BX>::smem(stages), stream, splits, map_w,
-                          map_x, p, stages);
+    launch_kernel_cluster(gemm_fp8_few_kernel<BX, XT, TO>, dim3(splits, (p.n + BM - 1) / BM, (p.rows + BX - 1) / BX), dim3(F::THREADS), F::smem(stages, p.groups_per_split), stream,
+                          splits, map_w, map_x, p, stages);
     QT_CHECK_LAUNCH("gemm_fp8 few");
     return QT_OK;
 }
 
-template <typename TO> int launch_many(const void* x8, const void* w8, const GemmParams& p, int k, cudaStream_t stream) {
+template <typename TO> int launch_many(const void* x8, const void* w8, GemmParams p, int splits, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
-    int rc = byte_map(&map_w, w8, p.n, k, BN);
+    int rc = byte_map(&map_w, w8, p.n, p.k, BN);
     if (rc) return rc;
-    rc = byte_map(&map_x, x8, p.rows, k, BM);
+    rc = byte_map(&map_x, x8, p.rows, p.k, BM);
     if (rc) return rc;
-    const cudaError_t raised = raise_shared<gemm_fp8_many_kernel<TO>>(227 * 1024);
+    cudaError_t raised = raise_shared<gemm_fp8_many_kernel<false, TO>>(227 * 1024);
+    if (raised == cudaSuccess) raised = raise_shared<gemm_fp8_many_kernel<true, TO>>(227 * 1024);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "gemm_fp8: cannot raise shared memory: %s", cudaGetErrorString(raised));
     const long long tiles = (long long)((p.n + BN - 1) / BN) * ((p.rows + BM - 1) / BM);
     QT_REQUIRE(tiles <= 0x7fffffff / RASTER, "gemm_fp8: %d x %d outputs are too many", p.rows, p.n);
-    launch_kernel(gemm_fp8_many_kernel<TO>, dim3((unsigned)std::min<long long>(tiles, sm_count())), dim3(MANY_THREADS),
-                  (size_t)MANY_STAGES * MANY_STAGE_BYTES + 8 * (2 * MANY_STAGES + 4) + 16 + 1024, stream, map_w, map_x, p);
+    p.groups_per_split = (p.groups + splits - 1) / splits;
+    splits = (p.groups + p.groups_per_split - 1) / p.groups_per_split;
+    if (splits > 1) {
+        QT_REQUIRE(splits <= 8 && tiles <= 65535, "gemm_fp8: %d ranges of K for %lld tiles", splits, tiles);
+        launch_kernel_cluster(gemm_fp8_many_kernel<true, TO>, dim3(splits, (unsigned)tiles), dim3(MANY_THREADS), MANY_SMEM, stream, splits, map_w, map_x, p);
+    } else {
+        launch_kernel(gemm_fp8_many_kernel<false, TO>, dim3((unsigned)std::min<long long>(tiles, sm_count())), dim3(MANY_THREADS), MANY_SMEM, stream, map_w, map_x, p);
+    }
     QT_CHECK_LAUNCH("gemm_fp8 many");
     return QT_OK;
 }
 
+int quantise_rows(const void* x, int dtype, void* values, float* scales, int rows, int k, cudaStream_t stream) {
+    const int groups = (k + GROUP - 1) / GROUP;
+    const long long blocks = ((long long)rows * groups + 7) / 8;
+    QT_REQUIRE(blocks <= 0x7fffffff, "quantise_rows: %d x %d is too large", rows, k);
+    const int wide = k % 4 == 0 && (((uintptr_t)x & 15) | ((uintptr_t)values & 3)) == 0;
+    return QT_DISPATCH_DTYPE(dtype, "quantise_rows", {
+        launch_kernel(quantise_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x, (uint8_t*)values, scales, rows, k, groups, wide);
+        QT_CHECK_LAUNCH("quantise_rows");
+        return QT_OK;
+    });
+}
+
+template <typename XT, typename TO> int launch_fused(const GemmParams& p, const void* w8, int splits, cudaStream_t stream) {
+    return launch_few<16, XT, TO>(nullptr, w8, p, splits, stream);
+}
+
 }  // namespace
+
+// The arguments of qt_gemm_fp8 as one structure: rows in 8 bits (x8, x_scale), which are made from x first where it is given.
+struct Fp8Call {
+    const void* x; void* x8; float* x_scale; const void* w8; const float* w_scale; void* out; int* status; void* stream;
+    int x_dtype, out_dtype, rows, n, k, form, splits, fused;
+};
+static_assert(sizeof(Fp8Call) == 8 * 8 + 8 * 4, "8 addresses and 8 numbers of 32 bits, without gaps");
 
 // x [rows, k] -> values [rows, k] e4m3, scales [ceil(k / 128), rows].
 extern "C" int qt_quantise_rows(const void* x, int dtype, void* values, float* scales, int rows, int k, void* stream) {
     QT_REQUIRE(rows >= 0 && k > 0, "quantise_rows: bad sizes %d x %d", rows, k);
-    if (rows == 0) return QT_OK;
-    const int groups = (k + GROUP - 1) / GROUP;
-    const long long blocks = ((long long)rows * groups + 7) / 8;
-    QT_REQUIRE(blocks <= 0x7fffffff, "quantise_rows: %d x %d is too large", rows, k);
-    return QT_DISPATCH_DTYPE(dtype, "quantise_rows", {
-        launch_kernel(quantise_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const T*)x, (uint8_t*)values, scales, rows, k, groups);
-        QT_CHECK_LAUNCH("quantise_rows");
-        return QT_OK;
-    });
+    return rows == 0 ? QT_OK : quantise_rows(x, dtype, values, scales, rows, k, (cudaStream_t)stream);
 }
 
 // w [n, k] -> values [n, k] e4m3, scales [ceil(n / 128), ceil(k / 128)].
@@ -546,26 +738,38 @@ extern "C" int qt_quantise_weight(const void* w, int dtype, void* values, float*
     });
 }
 
-// x8 [rows, k], x_scale [groups, rows], w8 [n, k], w_scale [ceil(n / 128), groups], out [rows, n].  `form`: -1 chooses; 0 any sizes; 16, 32, 64, 128: few rows in
-// tiles of so many, with `splits` ranges of K; 256: many rows.
-extern "C" int qt_gemm_fp8(const void* x8, const float* x_scale, const void* w8, const float* w_scale, void* out, int dtype, int rows, int n, int k, int form, int splits,
-                           int* status, void* stream) {
-    QT_REQUIRE(rows >= 0 && n > 0 && k > 0 && (rows + 63) / 64 <= 65535, "gemm_fp8: bad sizes M=%d N=%d K=%d", rows, n, k);
-    QT_REQUIRE(status != nullptr, "gemm_fp8: a status word is required");
-    if (rows == 0) return QT_OK;
-    const int size = dtype == QT_F32 ? 4 : 2;
-    GemmParams p{x_scale, w_scale, out, rows, n, (k + GROUP - 1) / GROUP, 0, (uintptr_t)out % 32 == 0 && (size_t)n * size % 32 == 0, status};
-    cudaStream_t s = (cudaStream_t)stream;
-    const bool aligned = k % 16 == 0 && (((uintptr_t)x8 | (uintptr_t)w8) & 15) == 0;
-    if (!aligned) form = 0;
-    return QT_DISPATCH_DTYPE(dtype, "gemm_fp8", {
-        if (form == 16) return launch_few<16, T>(x8, w8, p, k, splits, s);
-        if (form == 32) return launch_few<32, T>(x8, w8, p, k, splits, s);
-        if (form == 64) return launch_few<64, T>(x8, w8, p, k, splits, s);
-        if (form == 128) return launch_few<128, T>(x8, w8, p, k, splits, s);
-        if (form == 256) return launch_many<T>(x8, w8, p, k, s);
-        launch_kernel(gemm_fp8_any_kernel<T>, dim3((n + 63) / 64, (rows + 63) / 64), dim3(256), 0, s, (const uint8_t*)x8, x_scale, (const uint8_t*)w8, w_scale, (T*)out, rows, n,
-                      k, p.groups);
+// x [rows, k] or null, x8 [rows, k], x_scale [groups, rows], w8 [n, k], w_scale [ceil(n / 128), groups], out [rows, n].  `form`: 0 any sizes; 16, 32, 64: few rows in
+// tiles of so many, 256: many rows, with `splits` ranges of K.  `fused` (form 16, at most 16 rows and 32 groups a range): x is brought to 8 bits on the way, and x8
+// and x_scale stay as they are.
+extern "C" int qt_gemm_fp8(const Fp8Call* call) {
+    const Fp8Call& c = *call;
+    QT_REQUIRE(c.rows >= 0 && c.n > 0 && c.k > 0 && (c.rows + 63) / 64 <= 65535 && (c.n + BM - 1) / BM <= 65535, "gemm_fp8: bad sizes M=%d N=%d K=%d", c.rows, c.n, c.k);
+    if (c.rows == 0) return QT_OK;
+    QT_REQUIRE(c.status != nullptr && (c.x || !c.fused), "gemm_fp8: a status word is required");
+    const int size = c.out_dtype == QT_F32 ? 4 : 2;
+    cudaStream_t s = (cudaStream_t)c.stream;
+    const GemmParams p{c.x, c.k % 4 == 0 && (uintptr_t)c.x % 16 == 0, c.x_scale, c.w_scale, c.out, c.rows, c.n, c.k, (c.k + GROUP - 1) / GROUP, 0,
+                       (uintptr_t)c.out % 32 == 0 && (size_t)c.n * size % 32 == 0 ? 2 : (uintptr_t)c.out % 16 == 0 && c.n % 4 == 0 ? 1 : 0, c.status};
+    const bool aligned = c.k % 16 == 0 && (((uintptr_t)c.x8 | (uintptr_t)c.w8) & 15) == 0;
+    const int form = aligned ? c.form : 0;
+    if (c.fused && form == 16) {
+        if (c.x_dtype == QT_F32 && c.out_dtype == QT_F32) return launch_fused<float, float>(p, c.w8, c.splits, s);
+        if (c.x_dtype == QT_F32 && c.out_dtype == QT_BF16) return launch_fused<float, __nv_bfloat16>(p, c.w8, c.splits, s);
+        if (c.x_dtype == QT_BF16 && c.out_dtype == QT_F32) return launch_fused<__nv_bfloat16, float>(p, c.w8, c.splits, s);
+        if (c.x_dtype == QT_BF16 && c.out_dtype == QT_BF16) return launch_fused<__nv_bfloat16, __nv_bfloat16>(p, c.w8, c.splits, s);
+        QT_FAIL(QT_ERR_ARG, "gemm_fp8: unknown element types %d, %d", c.x_dtype, c.out_dtype);
+    }
+    if (c.x) {
+        const int rc = quantise_rows(c.x, c.x_dtype, c.x8, c.x_scale, c.rows, c.k, s);
+        if (rc) return rc;
+    }
+    return QT_DISPATCH_DTYPE(c.out_dtype, "gemm_fp8", {
+        if (form == 16) return launch_few<16, uint8_t, T>(c.x8, c.w8, p, c.splits, s);
+        if (form == 32) return launch_few<32, uint8_t, T>(c.x8, c.w8, p, c.splits, s);
+        if (form == 64) return launch_few<64, uint8_t, T>(c.x8, c.w8, p, c.splits, s);
+        if (form == 256) return launch_many<T>(c.x8, c.w8, p, c.splits, s);
+        launch_kernel(gemm_fp8_any_kernel<T>, dim3((c.n + 63) / 64, (c.rows + 63) / 64), dim3(256), 0, s, (const uint8_t*)c.x8, c.x_scale, (const uint8_t*)c.w8, c.w_scale, (T*)c.out,
+                      c.rows, c.n, c.k, p.groups);
         QT_CHECK_LAUNCH("gemm_fp8");
         return QT_OK;
     });

@@ -144,8 +144,7 @@ _SIGNATURES = {
         # x, dtype, values, scales, rows, k, stream
         "qt_quantise_rows": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
         "qt_quantise_weight": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
-        # x8, x_scale, w8, w_scale, out, dtype, rows, n, k, form, splits, status, stream
-        "qt_gemm_fp8": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr],
+        "qt_gemm_fp8": [ctypes.c_char_p],                     # an Fp8Call (_FP8_CALL)
     },
     "cache8": {
         # qkv, in_dtype, n_splits, split_stride, q_out, out_dtype, k, v, k_scale, v_scale, seq_start, seq_past, n_seqs, max_q_len, block_table, max_blocks, n_pages,
@@ -1683,43 +1682,85 @@ def quantise_weight_fp8(weight: torch.Tensor) -> Fp8Weight:
     return out
 
 
+FP8_FORMS = (0, 16, 32, 64, 256)
+FP8_FUSED_UNITS = 16       # most rows times groups a block that a product brings to 8 bits on the way, four warps at it (one row of 1024 x 2048: 4.4 us in the place of 4.9;
+                           # 16 rows in ranges of 4 groups, 64 units: 16 us in the place of 8)
+
+
 @functools.lru_cache(maxsize=4096)
 def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
-    """(form, ranges of K) of the product of ``m`` rows and a weight [n, k]: form 0 takes any sizes, 16 to 128 few rows in tiles of so many, 256 many rows."""
+    """(form, ranges of K) of the product of ``m`` rows and a weight [n, k]: form 0 takes any sizes, 16 to 64 few rows in tiles of so many, 256 many rows.
+
+    Up to 64 rows read the weight once, in ranges that give up to 256 blocks (8 rows of 6144 x 4096 in 4 / 5 / 6 / 8 ranges: 9.6 / 9.4 / 12.3 / 11.8 us; of 4096 x 12288
+    in 4 / 8: 16.3 / 14.2).  Beyond, the smaller of two times in us, fitted to 30 shapes of 100 to 768 rows: tiles of 64 rows, two blocks an SM, 0.37 to 0.5 a group of
+    K; of 128 x 256, one block an SM, 0.45 to 0.62, which the L2 cache's 12 TB/s to all SMs bounds.  Clusters of ranges over more than 130 SMs do not fit at once
+    (333 rows of 4096 x 12288 in 1 / 2 / 3 ranges: 58 / 39 / 51 us)."""
+    groups, blocks_n = -(-k // FP8_GROUP), -(-n // 128)
     if k % 16:
         return 0, 1
-    if m > 128:
-        return 256, 1
-    tile = next(t for t in (16, 32, 64, 128) if m <= t)
-    groups, tiles = -(-k // FP8_GROUP), -(-n // 128)
-    splits = max(1, min(8, groups // 2, 2 * sms // tiles))
-    return tile, splits
+    if m <= 64:
+        return next(t for t in (16, 32, 64) if m <= t), max(1, min(8, groups // 2, 256 * sms // 148 // blocks_n))
+    best = None
+    for form, tiles in ((64, blocks_n * -(-m // 64)), (256, -(-n // 256) * -(-m // 128))):
+        for splits in range(1, 6 if form == 64 else 7):
+            blocks, per_split = tiles * splits, -(-groups // splits)
+            if splits > 1 and (blocks > (256 if form == 64 else 130) * sms // 148 or per_split < 2):
+                break
+            if form == 64:
+                cost = 6 + 0.4 * (splits - 1) + per_split * (0.37 if blocks <= sms else 0.5 * -(-blocks // (2 * sms)))
+            else:
+                cost = 8 + 3 * (splits > 1) + per_split * -(-blocks // sms) * (0.45 + 0.17 * min(1.0, blocks / sms))
+            if best is None or cost < best[0]:
+                best = (cost, form, splits)
+    return best[1:]
+
+
+# x, x8, x_scale, w8, w_scale, out, status, stream, x_dtype, out_dtype, rows, n, k, form, splits, fused: a structure costs the host less than as many arguments
+_FP8_CALL = struct.Struct("@8P8i")
 
 
 def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None = None, plan: tuple[int, int] | None = None) -> None:
     """out [M, N] (bfloat16 or float32) = x [M, K] W^T with both operands in 8 bits and their scales on the sums of each 128 columns, in float, rounded once.
 
     ``x`` is ``Fp8Rows``, or bfloat16 or float32 rows that are brought to 8 bits first (``quantise_rows_fp8``), through ``scratch`` (``fp8_rows(M, K)``, or
-    larger in M: its leading rows serve).  ``plan``: ``fp8_plan``'s, or another one of its kind."""
+    larger in M: its leading rows serve; its contents afterwards are undefined).  ``plan``: ``fp8_plan``'s, or another one of its kind."""
+    given = type(x) is Fp8Rows
+    w = weight.values
+    n, k = w.shape
+    rows = x if given else scratch
+    values = x.values if given else x
+    m, device = values.shape[0], _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+    # one expression for a call that is in order: the host's part of a short product is its time
+    if not (values.dim() == 2 and values.shape[1] == k and out.shape == (m, n) and out.is_contiguous() and out.dtype in _CODES and rows is not None
+            and rows.values.shape[1] == k and rows.values.shape[0] >= m and (given or (x.dtype in _CODES and x.is_contiguous()))
+            and values.get_device() == out.get_device() == w.get_device() == rows.values.get_device() == device):
+        _check_gemm_fp8(x, weight, out, scratch, given)
+    form, splits = plan or fp8_plan(m, n, k)
+    if form not in FP8_FORMS or not 1 <= splits <= 8:
+        raise KernelError(f"gemm_fp8: a plan {plan}")
+    fused = not given and form == 16 and k % 16 == 0 and m * -(-(-(-k // FP8_GROUP)) // splits) <= FP8_FUSED_UNITS
+    _call("gemm_fp8", "qt_gemm_fp8",
+          _FP8_CALL.pack(0 if given else x.data_ptr(), rows.values.data_ptr(), rows.scales.data_ptr(), w.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
+                         _status_word(out.device).data_ptr(), _stream(), 0 if given else _CODES[x.dtype], _CODES[out.dtype], m, n, k, form, splits, fused),
+          launches=1 if given or fused else 2)
+
+
+def _check_gemm_fp8(x, weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None, given: bool) -> None:
+    """The refusal of a call that is not in order."""
     n, k = weight.shape
     m = x.shape[0]
-    _need(out, "out", shape=(m, n))
-    form, splits = plan or fp8_plan(m, n, k)
-    if form not in (0, 16, 32, 64, 128, 256) or not 1 <= splits <= 8:
-        raise KernelError(f"gemm_fp8: a plan {plan}")
-    if not isinstance(x, Fp8Rows):
+    if given:
+        if x.shape[1] != k:
+            raise KernelError(f"gemm_fp8: rows {tuple(x.shape)} for a weight {tuple(weight.shape)}")
+    else:
+        _need(x, "x", shape=(m, k))
+        _code(x, "x")
         if scratch is None or scratch.shape[1] != k or scratch.shape[0] < m:
             raise KernelError(f"gemm_fp8: scratch for {m} x {k} rows in 8 bits is required, got {None if scratch is None else tuple(scratch.shape)}")
-        if scratch.shape[0] > m:
-            groups = scratch.scales.shape[0]
-            scratch = Fp8Rows(scratch.values[:m], scratch.scales.view(-1)[:groups * m].view(groups, m))
-        quantise_rows_fp8(x, scratch)
-        x = scratch
-    if x.shape[1] != k:
-        raise KernelError(f"gemm_fp8: rows {tuple(x.shape)} for a weight {tuple(weight.shape)}")
-    _same_device("gemm_fp8", x.values, weight.values, out)
-    _call("gemm_fp8", "qt_gemm_fp8", _ptr(x.values), _ptr(x.scales), _ptr(weight.values), _ptr(weight.scales), _ptr(out), _code(out, "out"), m, n, k,
-          form, splits, _ptr(_status_word(out.device)), _stream())
+    _need(out, "out", shape=(m, n))
+    _code(out, "out")
+    _same_device("gemm_fp8", x.values if given else x, weight.values, out, *(() if scratch is None else (scratch.values,)))
+    raise KernelError("gemm_fp8: this call is not in order")
 
 
 # ----------------------------------------------------------------------------- a cache of keys and values in 8 bits

@@ -64,7 +64,7 @@ def test_product_of_many_tiles(m, n, k):
     _check_product(m, n, k, torch.bfloat16)
 
 
-@pytest.mark.parametrize("form,splits", [(0, 1), (256, 1)] + [(form, splits) for form in (16, 32, 64, 128) for splits in (1, 2, 3, 5, 7, 8)])
+@pytest.mark.parametrize("form,splits", [(0, 1)] + [(form, splits) for form in (16, 32, 64, 256) for splits in (1, 2, 3, 5, 7, 8)])
 @pytest.mark.parametrize("m,n,k", [(1, 130, 1040), (150, 300, 1040), (33, 256, 400), (129, 512, 112)])
 def test_product_by_every_plan(form, splits, m, n, k):
     """Any plan gives the result, more ranges than K has blocks among them."""
@@ -75,15 +75,32 @@ def test_product_by_every_plan(form, splits, m, n, k):
 def test_the_same_rows_give_the_same_bits():
     """Alone and twice, in 8 bits already or not: sums are in one order."""
     from qwen_triton_b200.ops import kernels
-    for m in (4, 48, 300):
+    for m, plan in ((48, None), (300, None), (4, (32, 2)), (20, (16, 3))):
         x, (values, scales) = _rows(m, 1152, torch.bfloat16, 3).cuda(), _weight(1024, 1152, 4)
         weight = kernels.Fp8Weight(values.cuda(), scales.cuda())
         rows = kernels.fp8_rows(m, 1152, "cuda")
         outs = [torch.empty((m, 1024), dtype=torch.bfloat16, device="cuda") for _ in range(3)]
-        kernels.gemm_fp8(x, weight, outs[0], rows)
-        kernels.gemm_fp8(x, weight, outs[1], kernels.fp8_rows(m + 7, 1152, "cuda"))
-        kernels.gemm_fp8(rows, weight, outs[2])
+        kernels.gemm_fp8(x, weight, outs[0], rows, plan)
+        kernels.gemm_fp8(x, weight, outs[1], kernels.fp8_rows(m + 7, 1152, "cuda"), plan)
+        kernels.quantise_rows_fp8(x, rows)
+        kernels.gemm_fp8(rows, weight, outs[2], plan=plan)
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (3, 130, 2832), (5, 384, 2992), (16, 128, 1040)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_come_in_8_bits_give_the_same_bits(m, n, k, dtype):
+    """Whether a product brings its rows to 8 bits on the way or finds them so, its sums are the same."""
+    from qwen_triton_b200.ops import kernels
+    x, (values, scales) = _rows(m, k, dtype, 3).cuda(), _weight(n, k, 4)
+    weight = kernels.Fp8Weight(values.cuda(), scales.cuda())
+    rows = kernels.fp8_rows(m, k, "cuda")
+    kernels.quantise_rows_fp8(x, rows)
+    for splits in (1, 2, 8):
+        outs = [torch.empty((m, n), dtype=dtype, device="cuda") for _ in range(2)]
+        kernels.gemm_fp8(x, weight, outs[0], kernels.fp8_rows(m, k, "cuda"), (16, splits))
+        kernels.gemm_fp8(rows, weight, outs[1], plan=(16, splits))
+        assert torch.equal(*outs)
 
 
 def test_rows_and_sums_at_the_ends_of_the_range():
