@@ -2,13 +2,17 @@
 //
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j,     k_j = s_k[page of j] k8_j,     v_j = s_v[page of j] v8_j
 //
-// A block takes eight rows (query token, head of a kv head's group) and a range of pages; each of its warps walks pages of its own, 32 keys at a time, straight
-// from memory into the registers of mma.sync: which keys and elements a lane's share of a fragment is, is free as long as both operands agree, so a lane
-// loads 16 neighbouring bytes.  S^T = K q^T and O^T += V^T P^T have keys and values as the operand with 16 rows and the eight query rows as the other.
+// A block takes eight rows (query token, head of a kv head's group) and a range of pages; each of its warps walks portions of 32 keys of its own (16 for heads
+// beyond 128) through a ring of its own in shared memory, which it fills with cp.async: no warp waits for another before the end.  S^T = K q^T and O^T += V^T P^T on
+// mma.sync have keys and values as the operand with 16 rows and the eight query rows as the other.  Which keys and elements a lane's share of a fragment is, is free as
+// long as both operands agree, so a lane reads 16 neighbouring bytes; the 16-byte pieces of a row lie where the row's number xored with theirs says, so that the lanes
+// that read together meet all banks.
 //
 // Every e4m3 number is a half.  Queries are brought to halves with a power of two for each row (its largest element lies in [2^14, 2^15), so no digit
 // of it is lost but below 2^-38 of that); FLOAT queries are two halves, and so is P then.  A weight is p_j s_v[j] relative to the largest such: the running
 // maximum is that of the score plus log2 s_v, so that halves hold the weights whatever scales the pages have; the sum of the p_j takes the scale back out.
+//
+// Ranges of a sequence join in the cluster that they form (up to eight), or through memory and a second launch.
 #include "fp8.cuh"
 
 #include <math.h>
@@ -21,6 +25,7 @@ namespace {
 constexpr int PAGE = 64;
 constexpr int WARPS = 4;
 constexpr int ROWS = 8;                                    // query rows of a block
+constexpr int MAX_CLUSTER = 8, MAX_RANGES = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.f;                        // a row's maximum moves when the true one is more than 2^8 above it
 
@@ -54,6 +59,16 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes on their way to shared memory; zeros where `there` is false
+__device__ __forceinline__ void copy16(void* to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <int WORDS> __device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* at) {
     if constexpr (WORDS == 4) {
         const uint4 x = *reinterpret_cast<const uint4*>(at);
@@ -65,19 +80,36 @@ template <int WORDS> __device__ __forceinline__ void load_words(uint32_t* w, con
 }
 
 // D: the head size rounded up to 64, 128 or 256; what lies between d and D is zero.
-template <int D, typename T>
-__global__ void __launch_bounds__(32 * WARPS) attention_cache8_kernel(const Params p) {
+template <int D> struct Ring {
+    static constexpr int SUBS = D > 128 ? 1 : 2, KEYS = 16 * SUBS, PER_PAGE = PAGE / KEYS;      // 16 keys each, at a time
+    static constexpr int STAGES = 3, PIECES = D / 16;                  // 16-byte pieces of a row
+    static constexpr int HALF = KEYS * D, STAGE = 2 * HALF + 16;       // keys, values, their scales
+    static constexpr size_t SMEM = (size_t)WARPS * STAGES * STAGE;
+    static_assert(SMEM >= (size_t)WARPS * ROWS * (D + 2) * 4 + ROWS * (D + 2) * 4, "the warps' results and the block's lie over the rings");
+    // where piece c of row r lies
+    __device__ static int at(int r, int c) { return r * D + ((D == 64 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 4); }
+};
+
+// JOIN: how ranges meet.  ALONE: there is one; CLUSTER: the blocks of a cluster along x; MEMORY: parts for the second launch.
+constexpr int ALONE = 0, CLUSTER = 1, MEMORY = 2;
+
+template <int D, int JOIN, typename T>
+__global__ void __launch_bounds__(32 * WARPS, 2) attention_cache8_kernel(const Params p) {
+    using R = Ring<D>;
     constexpr bool FLOAT = sizeof(T) == 4;
-    constexpr int CHUNKS = D / 64, STEPS = D / 16;         // 64 elements of a key among four lanes; 16 an instruction
-    constexpr int SUBS = D > 128 ? 1 : 2;                  // 16 keys each, at a time
-    constexpr int KEYS = 16 * SUBS, PER_PAGE = PAGE / KEYS;
+    constexpr int STEPS = D / 16, SUBS = R::SUBS, KEYS = R::KEYS, PER_PAGE = R::PER_PAGE, STAGES = R::STAGES;
+    constexpr int KPIECES = D / 64;                        // of a key row, a lane's pieces: KPIECES t + c (of 64 elements: t)
     constexpr int VBYTES = D / 8;                          // of a value row, a lane's neighbouring elements
-    constexpr int VPIECE = VBYTES < 16 ? VBYTES : 16, VPIECES = VBYTES / VPIECE;
-    extern __shared__ float shared[];                      // [WARPS][ROWS][D], then [WARPS][ROWS][2]
+    extern __shared__ __align__(128) uint8_t shared[];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int seq = blockIdx.z, kvh = blockIdx.y % p.nkv, group = p.nq / p.nkv;
-    const int tile = p.seq_start ? blockIdx.x : blockIdx.y / p.nkv, range = p.seq_start ? 0 : blockIdx.x;
+    const int tile = p.seq_start ? blockIdx.x : blockIdx.y / p.nkv, range = JOIN == ALONE ? 0 : blockIdx.x;
+    uint8_t* ring = shared + warp * STAGES * R::STAGE;
+    if (p.d < D) {                                         // what no copy reaches
+        for (int i = lane; i < STAGES * R::STAGE / 16; i += 32) *reinterpret_cast<uint4*>(ring + 16 * i) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+    }
     pdl_wait();
     const int capacity = p.max_blocks * PAGE;
     int token0 = seq, tokens = 1, past;
@@ -89,29 +121,78 @@ __global__ void __launch_bounds__(32 * WARPS) attention_cache8_kernel(const Para
         past = min(p.seq_len[seq], capacity) - 1;
     }
     const int row0 = tile * ROWS, rows = tokens * group;
-    if (row0 >= rows) return;
+    if (row0 >= rows) return;                              // prompts only: the same for a whole cluster
     const int last_row = min(row0 + ROWS, rows) - 1;
     const int end = min(past + last_row / group + 1, capacity);          // keys that any row sees
     const int page_begin = range * p.range_pages, pages = (end + PAGE - 1) / PAGE;
     const int page_end = range == p.ranges - 1 ? pages : min(pages, page_begin + p.range_pages);        // the last range takes what is left
-    if (page_begin >= page_end && range > 0) return;       // the join knows from the length
+    if (JOIN == MEMORY && page_begin >= page_end && range > 0) return;   // the join knows from the length
 
-    // queries: row g of the block, elements 64 c + 16 t + 4 j .. + 3 for instruction 4 c + j
+    const int* table = p.block_table + (size_t)seq * p.max_blocks;
+    const int begin = page_begin * PER_PAGE + warp, stop = (min(end, page_end * PAGE) + KEYS - 1) / KEYS;      // portions; the warp's are begin, begin + WARPS, ...
+    auto page_number = [&](int u) { return u < stop ? min(max(table[u / PER_PAGE], 0), p.n_pages - 1) : 0; };
+    // portion u on its way to stage s
+    auto fetch = [&](int u, int s, int page) {
+        uint8_t* to = ring + s * R::STAGE;
+        if (u < stop) {
+            const size_t block = (size_t)page * p.nkv + kvh;
+            const int key = u % PER_PAGE * KEYS, there = end - u * KEYS;
+            const uint8_t* k = p.k + (block * PAGE + key) * p.d;
+            const uint8_t* v = p.v + (block * PAGE + key) * p.d;
+            const int pieces = p.d >> 4;
+            if (p.d == D) {
+#pragma unroll
+                for (int i = lane; i < KEYS * R::PIECES; i += 32) {
+                    const int r = i / R::PIECES, c = i % R::PIECES;
+                    copy16(to + R::at(r, c), k + 16 * i, true);
+                    copy16(to + R::HALF + R::at(r, c), v + 16 * i, r < there);
+                }
+            } else {
+                for (int i = lane; i < KEYS * pieces; i += 32) {
+                    const int r = i / pieces, c = i % pieces;
+                    copy16(to + R::at(r, c), k + 16 * i, true);
+                    copy16(to + R::HALF + R::at(r, c), v + 16 * i, r < there);
+                }
+            }
+            if (lane < 2) copy4(to + 2 * R::HALF + 4 * lane, (lane ? p.v_scale : p.k_scale) + block);
+        }
+        copies_end();
+    };
+    int page = page_number(begin + (STAGES - 1) * WARPS);  // of the next portion to fetch
+    {
+        int first[STAGES - 1];
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) first[s] = page_number(begin + s * WARPS);
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) fetch(begin + s * WARPS, s, first[s]);
+    }
+
+    // queries: row g of the block; of key rows, lane t has the elements from 16 KPIECES t on (instruction 4 c + j: 4 of them from 16 c + 4 j on)
     uint32_t qh[STEPS][2], ql[FLOAT ? STEPS : 1][2];
     float factor;
     {
         const int row = row0 + g;
-        const bool there = row <= last_row;
+        const bool here = row <= last_row;
         const T* q = (const T*)p.q + ((size_t)(token0 + row / group) * p.nq + kvh * group + row % group) * p.d;
         float x[STEPS][4], most = 0.f;
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = (s >> 2) * 64 + 16 * t + 4 * (s & 3);
-                x[s][i] = there && at < p.d ? to_float(q[at + i]) : 0.f;
-                most = fmaxf(most, fabsf(x[s][i]));
+        for (int s = 0; s < STEPS; ++s) {
+            const int at = 16 * KPIECES * t + 4 * s;
+            if (here && at < p.d) {
+                if constexpr (FLOAT) {
+                    const float4 f = *reinterpret_cast<const float4*>(q + at);
+                    x[s][0] = f.x; x[s][1] = f.y; x[s][2] = f.z; x[s][3] = f.w;
+                } else {
+                    const uint2 f = *reinterpret_cast<const uint2*>(q + at);
+                    const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&f.x)), hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&f.y));
+                    x[s][0] = lo.x; x[s][1] = lo.y; x[s][2] = hi.x; x[s][3] = hi.y;
+                }
+            } else {
+                x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[s][i]));
+        }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         // 2^-shift brings the largest to [2^14, 2^15); none for rows of zeros or with infinities
@@ -139,143 +220,124 @@ __global__ void __launch_bounds__(32 * WARPS) attention_cache8_kernel(const Para
     const int limit1 = row0 + 2 * t + 1 <= last_row ? past + (row0 + 2 * t + 1) / group + 1 : 0;
     const int least = past + row0 / group + 1;             // keys below are seen by every row that is there
 
-    const int* table = p.block_table + (size_t)seq * p.max_blocks;
-    auto page_number = [&](int at) { return at < page_end ? min(max(table[at], 0), p.n_pages - 1) : 0; };
     float acc[STEPS][4] = {};
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    uint32_t kw[SUBS][2][STEPS], vw[SUBS][4][VBYTES / 4];
-    auto load_keys = [&](int page, int key) {              // 16 u + g and + 8, from place `key` of the page
-        const uint8_t* at = p.k + (((size_t)page * p.nkv + kvh) * PAGE + key) * p.d;
+    int s_at = 0;
+    for (int u = begin; u < stop; u += WARPS) {
+        // the stage that the portion before this one left is the next to fill
+        fetch(u + (STAGES - 1) * WARPS, s_at == 0 ? STAGES - 1 : s_at - 1, page);
+        page = page_number(u + STAGES * WARPS);
+        copies_wait<STAGES - 1>();
+        __syncwarp();
+        const uint8_t* stage = ring + s_at * R::STAGE;
+        s_at = s_at == STAGES - 1 ? 0 : s_at + 1;
+        const float2 scales = *reinterpret_cast<const float2*>(stage + 2 * R::HALF);
+        const float f0 = factor0 * scales.x, f1 = factor1 * scales.x, lift = log2f(scales.y), out_of = 1.f / scales.y;
+        const int key0 = u * KEYS;
+        float s[SUBS][4];
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u)
+        for (int v = 0; v < SUBS; ++v) {
+            float c[2][4] = {};                            // two chains of half as many dependent instructions
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < KPIECES; ++i) {
+                uint32_t a[4], b[4];
+                load_words<4>(a, stage + R::at(16 * v + g, KPIECES * t + i));
+                load_words<4>(b, stage + R::at(16 * v + 8 + g, KPIECES * t + i));
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c) {
-                    const int byte = 64 * c + 16 * t;
-                    if (byte < p.d) load_words<4>(&kw[u][h][4 * c], at + (size_t)(16 * u + 8 * h + g) * p.d + byte);
-                    else
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) kw[u][h][4 * c + j] = 0;
-                }
-    };
-    auto load_values = [&](int page, int key, int there) {  // keys 16 u + 2 t, + 1, + 8, + 9; those behind the last are zero
-        const uint8_t* at = p.v + (((size_t)page * p.nkv + kvh) * PAGE + key) * p.d;
-#pragma unroll
-        for (int u = 0; u < SUBS; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-                for (int c = 0; c < VPIECES; ++c) {
-                    const int byte = g * VBYTES + c * VPIECE;
-                    uint32_t* w = &vw[u][i][c * VPIECE / 4];
-                    if (byte < p.d && r < there) load_words<VPIECE / 4>(w, at + (size_t)r * p.d + byte);
-                    else
-#pragma unroll
-                        for (int j = 0; j < VPIECE / 4; ++j) w[j] = 0;
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t a0 = halves(a[j]), a1 = halves(b[j]), a2 = halves(a[j] >> 16), a3 = halves(b[j] >> 16);
+                    mma(c[j & 1], a0, a1, a2, a3, qh[4 * i + j][0], qh[4 * i + j][1]);
+                    if (FLOAT) mma(c[j & 1], a0, a1, a2, a3, ql[FLOAT ? 4 * i + j : 0][0], ql[FLOAT ? 4 * i + j : 0][1]);
                 }
             }
-    };
-
-    int page_at = page_begin + warp;
-    int page = page_number(page_at), next_page = page_number(page_at + WARPS);
-    if (page_at < page_end) load_keys(page, 0);
-    for (; page_at < page_end; page_at += WARPS) {
-        const float ks = p.k_scale[(size_t)page * p.nkv + kvh], vs = p.v_scale[(size_t)page * p.nkv + kvh];
-        const int after_next = page_number(page_at + 2 * WARPS);
-        const float f0 = factor0 * ks, f1 = factor1 * ks, lift = log2f(vs), out_of = 1.f / vs;
+            s[v][0] = fmaf(c[0][0] + c[1][0], f0, lift); s[v][1] = fmaf(c[0][1] + c[1][1], f1, lift);
+            s[v][2] = fmaf(c[0][2] + c[1][2], f0, lift); s[v][3] = fmaf(c[0][3] + c[1][3], f1, lift);
+        }
+        if (key0 + KEYS > least || last_row < row0 + ROWS - 1) {
 #pragma unroll
-        for (int part = 0; part < PER_PAGE; ++part) {
-            const int key0 = page_at * PAGE + part * KEYS;
-            load_values(page, part * KEYS, end - key0);
-            float s[SUBS][4];
+            for (int v = 0; v < SUBS; ++v)
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) {
-                float c[4] = {};
+                for (int i = 0; i < 4; ++i)
+                    if (key0 + 16 * v + g + 8 * (i >> 1) >= ((i & 1) ? limit1 : limit0)) s[v][i] = -INFINITY;
+        }
+        float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) {
-                    const uint32_t a = kw[u][0][i], b = kw[u][1][i];
-                    const uint32_t a0 = halves(a), a1 = halves(b), a2 = halves(a >> 16), a3 = halves(b >> 16);
-                    mma(c, a0, a1, a2, a3, qh[i][0], qh[i][1]);
-                    if (FLOAT) mma(c, a0, a1, a2, a3, ql[FLOAT ? i : 0][0], ql[FLOAT ? i : 0][1]);
-                }
-                s[u][0] = fmaf(c[0], f0, lift); s[u][1] = fmaf(c[1], f1, lift);
-                s[u][2] = fmaf(c[2], f0, lift); s[u][3] = fmaf(c[3], f1, lift);
+        for (int v = 0; v < SUBS; ++v) {
+            top0 = fmaxf(top0, fmaxf(s[v][0], s[v][2]));
+            top1 = fmaxf(top1, fmaxf(s[v][1], s[v][3]));
+        }
+        if (__any_sync(0xffffffffu, top0 > m0 + RESCALE_STEP || top1 > m1 + RESCALE_STEP)) {
+#pragma unroll
+            for (int off = 4; off < 32; off *= 2) {
+                top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, off));
+                top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, off));
             }
-            if (part + 1 < PER_PAGE) load_keys(page, (part + 1) * KEYS);
-            else if (page_at + WARPS < page_end) load_keys(next_page, 0);
-            if (key0 + KEYS > least || last_row < row0 + ROWS - 1) {
+            const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1);
+            const float a0 = n0 == -INFINITY ? 1.f : fast_exp2(m0 - n0), a1 = n1 == -INFINITY ? 1.f : fast_exp2(m1 - n1);
+            l0 *= a0; l1 *= a1;
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u)
+            for (int i = 0; i < STEPS; ++i) { acc[i][0] *= a0; acc[i][1] *= a1; acc[i][2] *= a0; acc[i][3] *= a1; }
+            m0 = n0; m1 = n1;
+        }
+        const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (key0 + 16 * u + g + 8 * (i >> 1) >= ((i & 1) ? limit1 : limit0)) s[u][i] = -INFINITY;
+        for (int v = 0; v < SUBS; ++v) {
+            const float w0 = fast_exp2(s[v][0] - u0), w1 = fast_exp2(s[v][1] - u1), w2 = fast_exp2(s[v][2] - u0), w3 = fast_exp2(s[v][3] - u1);
+            l0 = fmaf(w0 + w2, out_of, l0);
+            l1 = fmaf(w1 + w3, out_of, l1);
+            const uint32_t h0 = pack_half(w0, w1), h1 = pack_half(w2, w3);
+            const uint32_t b0 = transposed(h0), b1 = transposed(h1);
+            uint32_t r0 = 0, r1 = 0;
+            if (FLOAT) {
+                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h0)), y = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                r0 = transposed(pack_half(w0 - x.x, w1 - x.y));
+                r1 = transposed(pack_half(w2 - y.x, w3 - y.y));
             }
-            float top0 = -INFINITY, top1 = -INFINITY;
+            const uint8_t* values = stage + R::HALF;
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) {
-                top0 = fmaxf(top0, fmaxf(s[u][0], s[u][2]));
-                top1 = fmaxf(top1, fmaxf(s[u][1], s[u][3]));
-            }
-            if (__any_sync(0xffffffffu, top0 > m0 + RESCALE_STEP || top1 > m1 + RESCALE_STEP)) {
+            for (int c = 0; c < (VBYTES + 15) / 16; ++c) {
+                constexpr int WORDS = VBYTES < 16 ? VBYTES / 4 : 4;
+                uint32_t vw[4][WORDS];                     // keys 16 v + 2 t, + 1, + 8, + 9
 #pragma unroll
-                for (int off = 4; off < 32; off *= 2) {
-                    top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, off));
-                    top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, off));
-                }
-                const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1);
-                const float a0 = n0 == -INFINITY ? 1.f : fast_exp2(m0 - n0), a1 = n1 == -INFINITY ? 1.f : fast_exp2(m1 - n1);
-                l0 *= a0; l1 *= a1;
-#pragma unroll
-                for (int i = 0; i < STEPS; ++i) { acc[i][0] *= a0; acc[i][1] *= a1; acc[i][2] *= a0; acc[i][3] *= a1; }
-                m0 = n0; m1 = n1;
-            }
-            const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
-#pragma unroll
-            for (int u = 0; u < SUBS; ++u) {
-                const float w0 = fast_exp2(s[u][0] - u0), w1 = fast_exp2(s[u][1] - u1), w2 = fast_exp2(s[u][2] - u0), w3 = fast_exp2(s[u][3] - u1);
-                l0 = fmaf(w0 + w2, out_of, l0);
-                l1 = fmaf(w1 + w3, out_of, l1);
-                const uint32_t h0 = pack_half(w0, w1), h1 = pack_half(w2, w3);
-                const uint32_t b0 = transposed(h0), b1 = transposed(h1);
-                uint32_t r0 = 0, r1 = 0;
-                if (FLOAT) {
-                    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h0)), y = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                    r0 = transposed(pack_half(w0 - x.x, w1 - x.y));
-                    r1 = transposed(pack_half(w2 - y.x, w3 - y.y));
+                for (int i = 0; i < 4; ++i) {
+                    const int byte = g * VBYTES + 16 * c;
+                    load_words<WORDS>(vw[i], values + R::at(16 * v + 2 * t + (i & 1) + 8 * (i >> 1), byte >> 4) + (byte & 15));
                 }
 #pragma unroll
-                for (int w = 0; w < VBYTES / 4; ++w) {
+                for (int w = 0; w < WORDS; ++w) {
                     // bytes of neighbouring keys side by side: an element's two keys are one half2
-                    const uint32_t a01 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x5140), a23 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x7362);
-                    const uint32_t b01 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x5140), b23 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x7362);
+                    const uint32_t a01 = __byte_perm(vw[0][w], vw[1][w], 0x5140), a23 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+                    const uint32_t b01 = __byte_perm(vw[2][w], vw[3][w], 0x5140), b23 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
                     const uint32_t x0 = halves(a01), x1 = halves(a01 >> 16), x2 = halves(b01), x3 = halves(b01 >> 16);
                     const uint32_t y0 = halves(a23), y1 = halves(a23 >> 16), y2 = halves(b23), y3 = halves(b23 >> 16);
-                    mma(acc[2 * w], x0, x1, x2, x3, b0, b1);
-                    mma(acc[2 * w + 1], y0, y1, y2, y3, b0, b1);
+                    mma(acc[8 * c + 2 * w], x0, x1, x2, x3, b0, b1);
+                    mma(acc[8 * c + 2 * w + 1], y0, y1, y2, y3, b0, b1);
                     if (FLOAT) {
-                        mma(acc[2 * w], x0, x1, x2, x3, r0, r1);
-                        mma(acc[2 * w + 1], y0, y1, y2, y3, r0, r1);
+                        mma(acc[8 * c + 2 * w], x0, x1, x2, x3, r0, r1);
+                        mma(acc[8 * c + 2 * w + 1], y0, y1, y2, y3, r0, r1);
                     }
                 }
             }
         }
-        page = next_page;
-        next_page = after_next;
+        __syncwarp();                                      // the stage may be filled again
     }
-    // the warps' results, then the block's
+    // the warps' results, then the block's, over the rings
+    copies_wait<0>();
+    __syncthreads();
 #pragma unroll
     for (int off = 4; off < 32; off *= 2) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, off);
         l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
-    float* sums = shared + WARPS * ROWS * D;
+    float* parts = reinterpret_cast<float*>(shared);       // [WARPS][ROWS][D]
+    float* sums = parts + WARPS * ROWS * D;                // [WARPS][ROWS][2]
+    float* block_part = sums + WARPS * ROWS * 2;           // CLUSTER: [ROWS][D], [ROWS][2]
+    float* block_sums = block_part + ROWS * D;
     if (g == 0) {
         sums[(warp * ROWS + 2 * t) * 2] = m0; sums[(warp * ROWS + 2 * t) * 2 + 1] = l0;
         sums[(warp * ROWS + 2 * t + 1) * 2] = m1; sums[(warp * ROWS + 2 * t + 1) * 2 + 1] = l1;
     }
-    float* own = shared + warp * ROWS * D + g * VBYTES;
+    float* own = parts + warp * ROWS * D + g * VBYTES;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {                      // elements 2 i and 2 i + 1 of the lane's
         *reinterpret_cast<float2*>(own + (2 * t) * D + 2 * i) = make_float2(acc[i][0], acc[i][2]);
@@ -291,60 +353,108 @@ __global__ void __launch_bounds__(32 * WARPS) attention_cache8_kernel(const Para
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             const float mw = sums[(w * ROWS + r) * 2];
-            const float by = mw == -INFINITY ? 0.f : fast_exp2(mw - m);
             // a warp without keys has nothing; one whose sums are NaN hands that on
-            l = fmaf(sums[(w * ROWS + r) * 2 + 1], mw == -INFINITY ? 1.f : by, l);
-            a = fmaf(shared[(w * ROWS + r) * D + c], mw == -INFINITY ? 1.f : by, a);
+            const float by = mw == -INFINITY ? 1.f : fast_exp2(mw - m);
+            l = fmaf(sums[(w * ROWS + r) * 2 + 1], by, l);
+            a = fmaf(parts[(w * ROWS + r) * D + c], by, a);
         }
         const int head = kvh * group + row % group;
-        if (p.ranges == 1) {
+        if (JOIN == ALONE) {
             ((T*)p.out)[((size_t)(token0 + row / group) * p.nq + head) * p.d + c] = from_float<T>(l == 0.f ? 0.f : a / l);
-        } else {
+        } else if (JOIN == MEMORY) {
             const size_t part = ((size_t)seq * p.nq + head) * p.ranges + range;
             p.part_acc[part * p.d + c] = a;
             if (c == 0) { p.part_ml[part * 2] = m; p.part_ml[part * 2 + 1] = l; }
+        } else {
+            block_part[r * D + c] = a;
+            if (c == 0) { block_sums[2 * r] = m; block_sums[2 * r + 1] = l; }
         }
+    }
+    if (JOIN == CLUSTER) {
+        cluster_barrier();
+        const int ranks = gridDim.x, live = last_row - row0 + 1;
+        const uint32_t part0 = shared_address(block_part), sums0 = shared_address(block_sums);
+        auto remote = [](uint32_t at, int rank) {
+            uint32_t there;
+            float v;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+            return v;
+        };
+        for (int i = range * 32 * WARPS + threadIdx.x; i < live * p.d; i += ranks * 32 * WARPS) {
+            const int r = i / p.d, c = i % p.d;
+            float mr[MAX_CLUSTER], lr[MAX_CLUSTER], ar[MAX_CLUSTER], m = -INFINITY, l = 0.f, a = 0.f;
+#pragma unroll
+            for (int k = 0; k < MAX_CLUSTER; ++k)
+                if (k < ranks) {
+                    mr[k] = remote(sums0 + 8 * r, k);
+                    lr[k] = remote(sums0 + 8 * r + 4, k);
+                    ar[k] = remote(part0 + 4 * (r * D + c), k);
+                }
+#pragma unroll
+            for (int k = 0; k < MAX_CLUSTER; ++k)
+                if (k < ranks) m = fmaxf(m, mr[k]);
+#pragma unroll
+            for (int k = 0; k < MAX_CLUSTER; ++k)
+                if (k < ranks) {
+                    const float by = mr[k] == -INFINITY ? 1.f : fast_exp2(mr[k] - m);
+                    l = fmaf(lr[k], by, l);
+                    a = fmaf(ar[k], by, a);
+                }
+            const int row = row0 + r;
+            ((T*)p.out)[((size_t)(token0 + row / group) * p.nq + kvh * group + row % group) * p.d + c] = from_float<T>(l == 0.f ? 0.f : a / l);
+        }
+        cluster_barrier();                                 // nobody leaves while its part is read
     }
 }
 
 // The ranges of a (sequence, head): sum of l and acc, each at its distance from the largest maximum.
 template <typename T>
 __global__ void __launch_bounds__(128) join_cache8_kernel(const Params p) {
+    __shared__ float by[MAX_RANGES];
     pdl_launch_dependents();
     pdl_wait();
-    const int head = blockIdx.x, seq = blockIdx.y;
+    const int head = blockIdx.x, seq = blockIdx.y, lane = threadIdx.x & 31;
     const int pages = (min(p.seq_len[seq], p.max_blocks * PAGE) + PAGE - 1) / PAGE;
     const int used = min(max(1, (pages + p.range_pages - 1) / p.range_pages), p.ranges);
     const size_t first = ((size_t)seq * p.nq + head) * p.ranges;
-    const float* ml = p.part_ml + first * 2;
-    float m = -INFINITY, l = 0.f;
-    for (int r = 0; r < used; ++r) m = fmaxf(m, ml[2 * r]);
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + first;
+    // every warp the same
+    const float2 a = lane < used ? ml[lane] : make_float2(-INFINITY, 0.f), b = lane + 32 < used ? ml[lane + 32] : make_float2(-INFINITY, 0.f);
+    const float m = warp_max(fmaxf(a.x, b.x));
+    const float fa = a.x == -INFINITY ? 1.f : fast_exp2(a.x - m), fb = b.x == -INFINITY ? 1.f : fast_exp2(b.x - m);
+    const float l = warp_sum(fmaf(a.y, fa, b.y * fb));
+    if (threadIdx.x < 32) { by[lane] = fa; by[lane + 32] = fb; }
+    __syncthreads();
     for (int c = threadIdx.x; c < p.d; c += 128) {
-        float a = 0.f;
-        l = 0.f;
-        for (int r = 0; r < used; ++r) {
-            const float by = ml[2 * r] == -INFINITY ? 1.f : fast_exp2(ml[2 * r] - m);
-            l = fmaf(ml[2 * r + 1], by, l);
-            a = fmaf(p.part_acc[(first + r) * p.d + c], by, a);
-        }
-        ((T*)p.out)[((size_t)seq * p.nq + head) * p.d + c] = from_float<T>(l == 0.f ? 0.f : a / l);
+        float sum = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < used; ++r) sum = fmaf(p.part_acc[(first + r) * p.d + c], by[r], sum);
+        ((T*)p.out)[((size_t)seq * p.nq + head) * p.d + c] = from_float<T>(l == 0.f ? 0.f : sum / l);
     }
 }
 
-template <int D, typename T> int launch(const Params& p, dim3 grid, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)(WARPS * ROWS * D + WARPS * ROWS * 2) * 4;
-    launch_kernel(attention_cache8_kernel<D, T>, grid, dim3(32 * WARPS), smem, stream, p);
+template <int D, int JOIN, typename T> int launch(const Params& p, dim3 grid, cudaStream_t stream) {
+    const cudaError_t raised = raise_shared<attention_cache8_kernel<D, JOIN, T>>((int)Ring<D>::SMEM);
+    if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8: cannot raise shared memory: %s", cudaGetErrorString(raised));
+    if (JOIN == CLUSTER) launch_kernel_cluster(attention_cache8_kernel<D, JOIN, T>, grid, dim3(32 * WARPS), Ring<D>::SMEM, stream, grid.x, p);
+    else launch_kernel(attention_cache8_kernel<D, JOIN, T>, grid, dim3(32 * WARPS), Ring<D>::SMEM, stream, p);
     QT_CHECK_LAUNCH("attention_cache8");
-    if (p.ranges > 1) {
+    if (JOIN == MEMORY) {
         launch_kernel(join_cache8_kernel<T>, dim3(p.nq, grid.z), dim3(128), 0, stream, p);
         QT_CHECK_LAUNCH("attention_cache8 join");
     }
     return QT_OK;
 }
+template <int D, typename T> int launch_join(const Params& p, dim3 grid, cudaStream_t stream) {
+    if (p.ranges == 1) return launch<D, ALONE, T>(p, grid, stream);
+    if (p.ranges <= MAX_CLUSTER) return launch<D, CLUSTER, T>(p, grid, stream);
+    return launch<D, MEMORY, T>(p, grid, stream);
+}
 template <typename T> int launch_size(const Params& p, dim3 grid, cudaStream_t stream) {
-    if (p.d <= 64) return launch<64, T>(p, grid, stream);
-    if (p.d <= 128) return launch<128, T>(p, grid, stream);
-    return launch<256, T>(p, grid, stream);
+    if (p.d <= 64) return launch_join<64, T>(p, grid, stream);
+    if (p.d <= 128) return launch_join<128, T>(p, grid, stream);
+    return launch_join<256, T>(p, grid, stream);
 }
 
 int check(const char* name, int dtype, int nq, int nkv, int d, int max_blocks, int n_pages, const void* q, const void* k, const void* v, const void* out) {
@@ -357,7 +467,7 @@ int check(const char* name, int dtype, int nq, int nkv, int d, int max_blocks, i
 
 }  // namespace
 
-// One query a sequence: q and out [n_seqs, nq, d], seq_len [n_seqs] keys each (none: zeros).  With `ranges` > 1, part_acc holds n_seqs nq ranges d floats and part_ml
+// One query a sequence: q and out [n_seqs, nq, d], seq_len [n_seqs] keys each (none: zeros).  With `ranges` > 8, part_acc holds n_seqs nq ranges d floats and part_ml
 // n_seqs nq ranges 2.  A block walks range_pages pages of its
 // sequence, the last range whatever is left.
 extern "C" int qt_attention_decode_cache8(const void* q, int dtype, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out, const int* block_table,
@@ -368,7 +478,8 @@ extern "C" int qt_attention_decode_cache8(const void* q, int dtype, const void* 
     if (rc) return rc;
     const int tiles = (nq / nkv + ROWS - 1) / ROWS;
     QT_REQUIRE(n_seqs > 0 && n_seqs <= 65535 && (long long)nkv * tiles <= 65535, "attention_decode_cache8: %d sequences of %d heads", n_seqs, nq);
-    QT_REQUIRE(ranges >= 1 && range_pages >= 1 && (ranges == 1 || (part_acc && part_ml)), "attention_decode_cache8: %d ranges of %d pages", ranges, range_pages);
+    QT_REQUIRE(ranges >= 1 && ranges <= MAX_RANGES && range_pages >= 1 && (ranges <= MAX_CLUSTER || (part_acc && part_ml && (uintptr_t)part_ml % 8 == 0)),
+               "attention_decode_cache8: %d ranges of %d pages", ranges, range_pages);
     Params p{q, out, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, max_blocks, n_pages, nullptr, nullptr, seq_len, nq, nkv, d, scale, ranges,
              range_pages, part_acc, part_ml};
     const dim3 grid(ranges, nkv * tiles, n_seqs);

@@ -1842,6 +1842,9 @@ def qkv_write_cache8(qkv: GemmOut, q_out: torch.Tensor, cache: Cache8, seq_start
           _stream())
 
 
+_CLUSTER_RANGES, _MOST_RANGES = 8, 64         # ranges that join in a cluster, and through memory
+
+
 @dataclass(frozen=True)
 class Decode8Plan:
     """How ``attention_decode_cache8`` cuts the keys of its sequences (``decode8_plan``): ``ranges`` ranges of ``range_pages`` pages, the last one taking
@@ -1855,11 +1858,11 @@ class Decode8Plan:
 
     @property
     def acc_elements(self) -> int:
-        return self.q_shape[0] * self.q_shape[1] * self.ranges * self.q_shape[2] if self.ranges > 1 else 0
+        return self.q_shape[0] * self.q_shape[1] * self.ranges * self.q_shape[2] if self.ranges > _CLUSTER_RANGES else 0
 
     @property
     def ml_elements(self) -> int:
-        return self.q_shape[0] * self.q_shape[1] * self.ranges * 2 if self.ranges > 1 else 0
+        return self.q_shape[0] * self.q_shape[1] * self.ranges * 2 if self.ranges > _CLUSTER_RANGES else 0
 
 
 def decode8_plan(batch: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, max_context: int, sms: int = 148) -> Decode8Plan:
@@ -1888,13 +1891,15 @@ def _check_cache8(name: str, q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
 def attention_decode_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor, scale: float, plan: Decode8Plan,
                             part_acc: torch.Tensor | None = None, part_ml: torch.Tensor | None = None) -> None:
     """``attention_decode`` over a cache in 8 bits: one query token per sequence, q and out [sequences, nq, d] (bfloat16 or float32); ``seq_len`` counts the keys
-    it sees (none: the result is zero).  Where the plan cuts the keys into ranges their partial results pass through ``part_acc`` and ``part_ml`` (float, at least
+    it sees (none: the result is zero).  Where the plan cuts the keys into more than eight ranges their partial results pass through ``part_acc`` and ``part_ml`` (float, at least
     ``plan.acc_elements`` and ``plan.ml_elements``).  What lies behind a sequence's last key is not looked at."""
     _check_cache8("attention_decode_cache8", q, cache, out, block_table, q.shape[0])
     _need(seq_len, "seq_len", torch.int32, q.shape[:1])
     if tuple(q.shape) != plan.q_shape or q.dtype != plan.dtype or cache.kv_heads != plan.num_kv_heads:
         raise KernelError(f"attention_decode_cache8: a plan for {plan.q_shape} over {plan.num_kv_heads} kv heads, {plan.dtype}; queries {tuple(q.shape)} over {cache.kv_heads}, {q.dtype}")
-    if plan.ranges > 1:
+    if not 1 <= plan.ranges <= _MOST_RANGES or plan.range_pages < 1:
+        raise KernelError(f"attention_decode_cache8: {plan.ranges} ranges of {plan.range_pages} pages")
+    if plan.ranges > _CLUSTER_RANGES:
         for name, part, need in (("part_acc", part_acc, plan.acc_elements), ("part_ml", part_ml, plan.ml_elements)):
             if part is None:
                 raise KernelError(f"attention_decode_cache8: {name} is required for {plan.ranges} ranges")
@@ -1905,7 +1910,7 @@ def attention_decode_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, b
     _same_device("attention_decode_cache8", seq_len)
     _call("attention_cache8", "qt_attention_decode_cache8", _ptr(q), _code(q, "q"), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(out),
           _ptr(block_table), block_table.shape[1], cache.pages, _ptr(seq_len), q.shape[0], q.shape[1], cache.kv_heads, cache.head_dim, float(scale), plan.ranges,
-          plan.range_pages, _ptr(part_acc), _ptr(part_ml), _stream(), launches=2 if plan.ranges > 1 else 1)
+          plan.range_pages, _ptr(part_acc), _ptr(part_ml), _stream(), launches=2 if plan.ranges > _CLUSTER_RANGES else 1)
 
 
 def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_start: torch.Tensor, seq_past: torch.Tensor,

@@ -118,7 +118,7 @@ def test_what_lies_behind_the_last_key_is_not_looked_at():
             t[2] = t[5] = math.nan
         q = torch.randn((3, 4, 64), generator=torch.Generator().manual_seed(2)).to(dtype)
         want, bound = plain.attention(q, *_held(cache), table, [1] * 3, [n - 1 for n in lengths], 0.125, DIGITS[dtype])
-        for ranges in ((1, 9), (2, 1), (3, 1)):
+        for ranges in ((1, 9), (2, 1), (3, 1), (12, 1)):
             plan = kernels.Decode8Plan((3, 4, 64), 2, dtype, *ranges)
             out = torch.full_like(q, math.nan, device="cuda")
             scratch = [torch.full((n,), math.nan, device="cuda") for n in (plan.acc_elements, plan.ml_elements)]
@@ -135,7 +135,7 @@ def test_a_nan_that_is_seen_is_handed_on():
     cache.k.view(torch.uint8)[1, 0, 5, 3] = 0x7f
     q = torch.ones((2, 1, 64), dtype=BF16, device="cuda")
     out = torch.empty_like(q)
-    for ranges in ((1, 9), (2, 1)):
+    for ranges in ((1, 9), (2, 1), (9, 1)):
         plan = kernels.Decode8Plan((2, 1, 64), 1, BF16, *ranges)
         scratch = [torch.empty(n, device="cuda") for n in (plan.acc_elements, plan.ml_elements)]
         kernels.attention_decode_cache8(q, cache, out, _ints([[0, 1], [2, 0]]), _ints([100, 64]), 0.1, plan, *scratch)
@@ -430,7 +430,7 @@ def test_refusals():
         kernels.Cache8(cache.k.view(torch.uint8), cache.v, cache.k_scale, cache.v_scale)
     q = torch.zeros((2, 4, 64), dtype=BF16, device="cuda")
     out, table, lens = torch.empty_like(q), _ints([[0, 1], [2, 3]]), _ints([100, 3])
-    plan = kernels.Decode8Plan((2, 4, 64), 2, BF16, 2, 1)
+    plan = kernels.Decode8Plan((2, 4, 64), 2, BF16, 9, 1)
     acc, ml = (torch.empty(n, device="cuda") for n in (plan.acc_elements, plan.ml_elements))
     decode = kernels.attention_decode_cache8
     decode(q, cache, out, table, lens, 0.1, plan, acc, ml)
@@ -438,6 +438,8 @@ def test_refusals():
         decode(q, cache, out, table, lens, 0.1, plan)
     with pytest.raises(Error, match="part_ml"):
         decode(q, cache, out, table, lens, 0.1, plan, acc, ml[:-1])
+    with pytest.raises(Error, match="65 ranges"):
+        decode(q, cache, out, table, lens, 0.1, kernels.Decode8Plan((2, 4, 64), 2, BF16, 65, 1), acc, ml)
     with pytest.raises(Error, match="plan"):
         decode(q[:1], cache, out[:1], table[:1], lens[:1], 0.1, plan, acc, ml)
     with pytest.raises(Error, match="out must"):
