@@ -38,6 +38,7 @@ struct Params {
     int nq, nkv, d;
     float scale;
     int ranges, range_pages;                               // a block walks range_pages pages of its sequence
+    int clusters;                                          // ranges join in clusters (up to eight), else through memory
     float* part_acc; float* part_ml;
 };
 
@@ -82,7 +83,7 @@ template <int WORDS> __device__ __forceinline__ void load_words(uint32_t* w, con
 // D: the head size rounded up to 64, 128 or 256; what lies between d and D is zero.
 template <int D> struct Ring {
     static constexpr int SUBS = D > 128 ? 1 : 2, KEYS = 16 * SUBS, PER_PAGE = PAGE / KEYS;      // 16 keys each, at a time
-    static constexpr int STAGES = 3, PIECES = D / 16;                  // 16-byte pieces of a row
+    static constexpr int STAGES = 2, PIECES = D / 16;                  // 16-byte pieces of a row
     static constexpr int HALF = KEYS * D, STAGE = 2 * HALF + 16;       // keys, values, their scales
     static constexpr size_t SMEM = (size_t)WARPS * STAGES * STAGE;
     static_assert(SMEM >= (size_t)WARPS * ROWS * (D + 2) * 4 + ROWS * (D + 2) * 4, "the warps' results and the block's lie over the rings");
@@ -94,7 +95,7 @@ template <int D> struct Ring {
 constexpr int ALONE = 0, CLUSTER = 1, MEMORY = 2;
 
 template <int D, int JOIN, typename T>
-__global__ void __launch_bounds__(32 * WARPS, 2) attention_cache8_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3) attention_cache8_kernel(const Params p) {
     using R = Ring<D>;
     constexpr bool FLOAT = sizeof(T) == 4;
     constexpr int STEPS = D / 16, SUBS = R::SUBS, KEYS = R::KEYS, PER_PAGE = R::PER_PAGE, STAGES = R::STAGES;
@@ -111,6 +112,12 @@ __global__ void __launch_bounds__(32 * WARPS, 2) attention_cache8_kernel(const P
         __syncwarp();
     }
     pdl_wait();
+    const int* table = p.block_table + (size_t)seq * p.max_blocks;
+    const int page_begin = range * p.range_pages, begin = page_begin * PER_PAGE + warp;
+    // the first pages are asked for together with the lengths that say whether they are needed
+    int first[STAGES];
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) first[s] = table[min((begin + s * WARPS) / PER_PAGE, p.max_blocks - 1)];
     const int capacity = p.max_blocks * PAGE;
     int token0 = seq, tokens = 1, past;
     if (p.seq_start) {
@@ -124,12 +131,11 @@ __global__ void __launch_bounds__(32 * WARPS, 2) attention_cache8_kernel(const P
     if (row0 >= rows) return;                              // prompts only: the same for a whole cluster
     const int last_row = min(row0 + ROWS, rows) - 1;
     const int end = min(past + last_row / group + 1, capacity);          // keys that any row sees
-    const int page_begin = range * p.range_pages, pages = (end + PAGE - 1) / PAGE;
+    const int pages = (end + PAGE - 1) / PAGE;
     const int page_end = range == p.ranges - 1 ? pages : min(pages, page_begin + p.range_pages);        // the last range takes what is left
     if (JOIN == MEMORY && page_begin >= page_end && range > 0) return;   // the join knows from the length
 
-    const int* table = p.block_table + (size_t)seq * p.max_blocks;
-    const int begin = page_begin * PER_PAGE + warp, stop = (min(end, page_end * PAGE) + KEYS - 1) / KEYS;      // portions; the warp's are begin, begin + WARPS, ...
+    const int stop = (min(end, page_end * PAGE) + KEYS - 1) / KEYS;      // portions; the warp's are begin, begin + WARPS, ...
     auto page_number = [&](int u) { return u < stop ? min(max(table[u / PER_PAGE], 0), p.n_pages - 1) : 0; };
     // portion u on its way to stage s
     auto fetch = [&](int u, int s, int page) {
@@ -158,14 +164,9 @@ __global__ void __launch_bounds__(32 * WARPS, 2) attention_cache8_kernel(const P
         }
         copies_end();
     };
-    int page = page_number(begin + (STAGES - 1) * WARPS);  // of the next portion to fetch
-    {
-        int first[STAGES - 1];
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) first[s] = page_number(begin + s * WARPS);
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) fetch(begin + s * WARPS, s, first[s]);
-    }
+    for (int s = 0; s < STAGES - 1; ++s) fetch(begin + s * WARPS, s, min(max(first[s], 0), p.n_pages - 1));
+    int page = min(max(first[STAGES - 1], 0), p.n_pages - 1);      // of the next portion to fetch
 
     // queries: row g of the block; of key rows, lane t has the elements from 16 KPIECES t on (instruction 4 c + j: 4 of them from 16 c + 4 j on)
     uint32_t qh[STEPS][2], ql[FLOAT ? STEPS : 1][2];
@@ -408,13 +409,16 @@ __global__ void __launch_bounds__(32 * WARPS, 2) attention_cache8_kernel(const P
     }
 }
 
-// The ranges of a (sequence, head): sum of l and acc, each at its distance from the largest maximum.
-template <typename T>
-__global__ void __launch_bounds__(128) join_cache8_kernel(const Params p) {
-    __shared__ float by[MAX_RANGES];
+// The ranges of a (sequence, head): sum of l and acc, each at its distance from the largest maximum.  GROUPS of threads (four for more than 16 ranges) take every
+// GROUPS-th range, so that sixteen parts are on their way at a time (32 ranges of one sequence of 8,192: 11.5 us with four groups, 12.3 with one; but 4 ranges of 128
+// sequences of 4,096, whose blocks are many: 191 and 180).
+constexpr int JOIN_WIDTH = 128;
+template <int GROUPS, typename T>
+__global__ void __launch_bounds__(GROUPS * JOIN_WIDTH) join_cache8_kernel(const Params p) {
+    __shared__ float by[MAX_RANGES], parts[GROUPS][JOIN_WIDTH];
     pdl_launch_dependents();
     pdl_wait();
-    const int head = blockIdx.x, seq = blockIdx.y, lane = threadIdx.x & 31;
+    const int head = blockIdx.x, seq = blockIdx.y, lane = threadIdx.x & 31, member = threadIdx.x % JOIN_WIDTH, of = threadIdx.x / JOIN_WIDTH;
     const int pages = (min(p.seq_len[seq], p.max_blocks * PAGE) + PAGE - 1) / PAGE;
     const int used = min(max(1, (pages + p.range_pages - 1) / p.range_pages), p.ranges);
     const size_t first = ((size_t)seq * p.nq + head) * p.ranges;
@@ -426,11 +430,24 @@ __global__ void __launch_bounds__(128) join_cache8_kernel(const Params p) {
     const float l = warp_sum(fmaf(a.y, fa, b.y * fb));
     if (threadIdx.x < 32) { by[lane] = fa; by[lane + 32] = fb; }
     __syncthreads();
-    for (int c = threadIdx.x; c < p.d; c += 128) {
+    for (int c0 = 0; c0 < p.d; c0 += JOIN_WIDTH) {         // the same for every thread
+        const int c = c0 + member;
         float sum = 0.f;
+        if (c < p.d) {
 #pragma unroll 4
-        for (int r = 0; r < used; ++r) sum = fmaf(p.part_acc[(first + r) * p.d + c], by[r], sum);
-        ((T*)p.out)[((size_t)seq * p.nq + head) * p.d + c] = from_float<T>(l == 0.f ? 0.f : sum / l);
+            for (int r = of; r < used; r += GROUPS) sum = fmaf(p.part_acc[(first + r) * p.d + c], by[r], sum);
+        }
+        if (GROUPS > 1) {
+            parts[of][member] = sum;
+            __syncthreads();
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) sum += parts[i][member];
+        }
+        if (of == 0 && c < p.d) {
+            ((T*)p.out)[((size_t)seq * p.nq + head) * p.d + c] = from_float<T>(l == 0.f ? 0.f : sum / l);
+        }
+        __syncthreads();
     }
 }
 
@@ -441,14 +458,15 @@ template <int D, int JOIN, typename T> int launch(const Params& p, dim3 grid, cu
     else launch_kernel(attention_cache8_kernel<D, JOIN, T>, grid, dim3(32 * WARPS), Ring<D>::SMEM, stream, p);
     QT_CHECK_LAUNCH("attention_cache8");
     if (JOIN == MEMORY) {
-        launch_kernel(join_cache8_kernel<T>, dim3(p.nq, grid.z), dim3(128), 0, stream, p);
+        if (p.ranges > 16) launch_kernel(join_cache8_kernel<4, T>, dim3(p.nq, grid.z), dim3(4 * JOIN_WIDTH), 0, stream, p);
+        else launch_kernel(join_cache8_kernel<1, T>, dim3(p.nq, grid.z), dim3(JOIN_WIDTH), 0, stream, p);
         QT_CHECK_LAUNCH("attention_cache8 join");
     }
     return QT_OK;
 }
 template <int D, typename T> int launch_join(const Params& p, dim3 grid, cudaStream_t stream) {
     if (p.ranges == 1) return launch<D, ALONE, T>(p, grid, stream);
-    if (p.ranges <= MAX_CLUSTER) return launch<D, CLUSTER, T>(p, grid, stream);
+    if (p.clusters) return launch<D, CLUSTER, T>(p, grid, stream);
     return launch<D, MEMORY, T>(p, grid, stream);
 }
 template <typename T> int launch_size(const Params& p, dim3 grid, cudaStream_t stream) {
@@ -467,38 +485,51 @@ int check(const char* name, int dtype, int nq, int nkv, int d, int max_blocks, i
 
 }  // namespace
 
-// One query a sequence: q and out [n_seqs, nq, d], seq_len [n_seqs] keys each (none: zeros).  With `ranges` > 8, part_acc holds n_seqs nq ranges d floats and part_ml
-// n_seqs nq ranges 2.  A block walks range_pages pages of its
+// The arguments of the two calls below as one structure.
+struct Cache8Call {
+    const void *q, *k, *v;
+    const float *k_scale, *v_scale;
+    void* out;
+    const int *block_table, *seq_start, *seq_past, *seq_len;
+    float *part_acc, *part_ml;
+    int* status;
+    void* stream;
+    double scale;
+    int dtype, max_blocks, n_pages, n_seqs, n_tokens, max_q_len, nq, nkv, d, ranges, range_pages, clusters;
+};
+static_assert(sizeof(Cache8Call) == 15 * 8 + 12 * 4, "14 addresses, a number of 64 bits and 12 of 32, without gaps");
+
+// One query a sequence: q and out [n_seqs, nq, d], seq_len [n_seqs] keys each (none: zeros).  Ranges join in clusters of blocks (at most eight,
+// with `clusters`) or through memory: part_acc holds n_seqs nq ranges d floats and part_ml n_seqs nq ranges 2.  A block walks range_pages pages of its
 // sequence, the last range whatever is left.
-extern "C" int qt_attention_decode_cache8(const void* q, int dtype, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out, const int* block_table,
-                                          int max_blocks, int n_pages, const int* seq_len, int n_seqs, int nq, int nkv, int d, float scale, int ranges, int range_pages,
-                                          float* part_acc, float* part_ml, void* stream) {
-    if (n_seqs == 0) return QT_OK;
-    const int rc = check("attention_decode_cache8", dtype, nq, nkv, d, max_blocks, n_pages, q, k, v, out);
+extern "C" int qt_attention_decode_cache8(const Cache8Call* call) {
+    const Cache8Call& c = *call;
+    if (c.n_seqs == 0) return QT_OK;
+    const int rc = check("attention_decode_cache8", c.dtype, c.nq, c.nkv, c.d, c.max_blocks, c.n_pages, c.q, c.k, c.v, c.out);
     if (rc) return rc;
-    const int tiles = (nq / nkv + ROWS - 1) / ROWS;
-    QT_REQUIRE(n_seqs > 0 && n_seqs <= 65535 && (long long)nkv * tiles <= 65535, "attention_decode_cache8: %d sequences of %d heads", n_seqs, nq);
-    QT_REQUIRE(ranges >= 1 && ranges <= MAX_RANGES && range_pages >= 1 && (ranges <= MAX_CLUSTER || (part_acc && part_ml && (uintptr_t)part_ml % 8 == 0)),
-               "attention_decode_cache8: %d ranges of %d pages", ranges, range_pages);
-    Params p{q, out, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, max_blocks, n_pages, nullptr, nullptr, seq_len, nq, nkv, d, scale, ranges,
-             range_pages, part_acc, part_ml};
-    const dim3 grid(ranges, nkv * tiles, n_seqs);
-    return dtype == QT_F32 ? launch_size<float>(p, grid, (cudaStream_t)stream) : launch_size<__nv_bfloat16>(p, grid, (cudaStream_t)stream);
+    const int tiles = (c.nq / c.nkv + ROWS - 1) / ROWS;
+    QT_REQUIRE(c.n_seqs > 0 && c.n_seqs <= 65535 && (long long)c.nkv * tiles <= 65535, "attention_decode_cache8: %d sequences of %d heads", c.n_seqs, c.nq);
+    const int clusters = c.clusters && c.ranges <= MAX_CLUSTER;
+    QT_REQUIRE(c.ranges >= 1 && c.ranges <= MAX_RANGES && c.range_pages >= 1 && (c.ranges == 1 || clusters || (c.part_acc && c.part_ml && (uintptr_t)c.part_ml % 8 == 0)),
+               "attention_decode_cache8: %d ranges of %d pages", c.ranges, c.range_pages);
+    const Params p{c.q, c.out, (const uint8_t*)c.k, (const uint8_t*)c.v, c.k_scale, c.v_scale, c.block_table, c.max_blocks, c.n_pages, nullptr, nullptr, c.seq_len, c.nq, c.nkv, c.d,
+                   (float)c.scale, c.ranges, c.range_pages, clusters, c.part_acc, c.part_ml};
+    const dim3 grid(c.ranges, c.nkv * tiles, c.n_seqs);
+    return c.dtype == QT_F32 ? launch_size<float>(p, grid, (cudaStream_t)c.stream) : launch_size<__nv_bfloat16>(p, grid, (cudaStream_t)c.stream);
 }
 
 // Packed queries [n_tokens, nq, d] of sequences whose keys, this call's own among them, are in the cache; causal.
-extern "C" int qt_attention_prefill_cache8(const void* q, int dtype, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out, const int* block_table,
-                                           int max_blocks, int n_pages, const int* seq_start, const int* seq_past, int n_seqs, int max_q_len, int nq, int nkv, int d,
-                                           float scale, void* stream) {
-    if (n_seqs == 0 || max_q_len == 0) return QT_OK;
-    const int rc = check("attention_prefill_cache8", dtype, nq, nkv, d, max_blocks, n_pages, q, k, v, out);
+extern "C" int qt_attention_prefill_cache8(const Cache8Call* call) {
+    const Cache8Call& c = *call;
+    if (c.n_seqs == 0 || c.max_q_len == 0) return QT_OK;
+    const int rc = check("attention_prefill_cache8", c.dtype, c.nq, c.nkv, c.d, c.max_blocks, c.n_pages, c.q, c.k, c.v, c.out);
     if (rc) return rc;
-    QT_REQUIRE(n_seqs > 0 && n_seqs <= 65535 && nkv <= 65535 && max_q_len > 0 && (long long)max_q_len * (nq / nkv) <= 0x7fffffff - ROWS,
-               "attention_prefill_cache8: %d sequences of up to %d tokens", n_seqs, max_q_len);
-    Params p{q, out, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, max_blocks, n_pages, seq_start, seq_past, nullptr, nq, nkv, d, scale, 1,
-             0x7fffffff / PAGE, nullptr, nullptr};
-    const dim3 grid((unsigned)((max_q_len * (nq / nkv) + ROWS - 1) / ROWS), nkv, n_seqs);
-    return dtype == QT_F32 ? launch_size<float>(p, grid, (cudaStream_t)stream) : launch_size<__nv_bfloat16>(p, grid, (cudaStream_t)stream);
+    QT_REQUIRE(c.n_seqs > 0 && c.n_seqs <= 65535 && c.nkv <= 65535 && c.max_q_len > 0 && (long long)c.max_q_len * (c.nq / c.nkv) <= 0x7fffffff - ROWS,
+               "attention_prefill_cache8: %d sequences of up to %d tokens", c.n_seqs, c.max_q_len);
+    const Params p{c.q, c.out, (const uint8_t*)c.k, (const uint8_t*)c.v, c.k_scale, c.v_scale, c.block_table, c.max_blocks, c.n_pages, c.seq_start, c.seq_past, nullptr, c.nq, c.nkv, c.d,
+                   (float)c.scale, 1, 0x7fffffff / PAGE, 0, nullptr, nullptr};
+    const dim3 grid((unsigned)((c.max_q_len * (c.nq / c.nkv) + ROWS - 1) / ROWS), c.nkv, c.n_seqs);
+    return c.dtype == QT_F32 ? launch_size<float>(p, grid, (cudaStream_t)c.stream) : launch_size<__nv_bfloat16>(p, grid, (cudaStream_t)c.stream);
 }
 
 QT_DEFINE_LAST_ERROR(attention_cache8)

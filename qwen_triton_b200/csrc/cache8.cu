@@ -12,145 +12,290 @@ using namespace qt_fp8;
 
 namespace {
 
-constexpr int PAGE = 64;
-constexpr int THREADS = 256;
+constexpr int PAGE = 64, THREADS = 256, WARPS = THREADS / 32;
 
 struct WriteParams {
     const void* qkv; int n_splits; size_t split_stride;
+    int wide;                                              // eight elements of the projection begin where 16 bytes do
     void* q_out;
     uint8_t* k; uint8_t* v; float* k_scale; float* v_scale;
-    const int* seq_start; const int* seq_past; const int* block_table; int max_blocks, n_pages;
+    const int* seq_start; const int* seq_past; const int* block_table; int n_seqs, max_blocks, n_pages;
     const float* q_weight; const float* k_weight; float eps;
     const float* cos_sin; int rotary_dim, max_pos, interleaved;
     int nq, nkv, d;
 };
 
-// A row's factor of the norm: 1 over its root mean square.
-template <typename TI>
-__device__ __forceinline__ float row_factor(const WriteParams& p, size_t at, int lane) {
-    const TI* x = (const TI*)p.qkv + at;
-    float sum = 0.f;
-    for (int i = lane; i < p.d; i += 32) {
-        const float v = load_sum(x, (size_t)i, p.n_splits, p.split_stride);
-        sum = fmaf(v, v, sum);
+__device__ __forceinline__ void load8(float (&v)[8], const float* at, bool wide) {
+    if (wide) {
+        const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = at[i];
     }
-    return rsqrtf(warp_sum(sum) / (float)p.d + p.eps);
+}
+__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16* at, bool wide) {
+    if (wide) {
+        const uint4 a = *reinterpret_cast<const uint4*>(at);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_float(at[i]);
+    }
+}
+__device__ __forceinline__ void store8(float* at, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* at, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Element i of a row, normed and rotated.
-template <typename TI>
-__device__ __forceinline__ float treated(const WriteParams& p, size_t at, int i, float factor, const float* weight, const float* angles) {
-    const TI* x = (const TI*)p.qkv + at;
-    auto element = [&](int j) {
-        const float v = load_sum(x, (size_t)j, p.n_splits, p.split_stride);
-        return weight ? v * factor * weight[j] : v;
-    };
-    const float own = element(i);
-    if (angles == nullptr || i >= p.rotary_dim) return own;
-    const int half = p.rotary_dim / 2;
-    const int pair = p.interleaved ? i >> 1 : i % half;
-    const bool first = p.interleaved ? (i & 1) == 0 : i < half;
-    const float other = element(p.interleaved ? i ^ 1 : first ? i + half : i - half);
-    const float c = angles[pair], s = angles[half + pair];
-    return first ? own * c - other * s : own * c + other * s;
-}
-
-// grid: (2 nkv + nq heads, pages that a sequence's tokens touch, sequences); a warp a token.
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(THREADS) qkv_write_cache8_kernel(const WriteParams p) {
-    extern __shared__ float rows[];                        // [64][d] of keys or values
-    __shared__ float most[THREADS / 32];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int seq = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int start = p.seq_start[seq], count = p.seq_start[seq + 1] - start, past = p.seq_past[seq];
-    if (count <= 0) return;
-    const int page_at = past / PAGE + blockIdx.y;
-    const int low = max(past, page_at * PAGE), high = min(past + count, (page_at + 1) * PAGE);
-    if (low >= high) return;
-    const int head = blockIdx.x, width = (p.nq + 2 * p.nkv) * p.d;
-    const bool query = head >= 2 * p.nkv, value = !query && head >= p.nkv;
-    const int column = query ? (head - 2 * p.nkv) * p.d : (p.nq + head) * p.d;         // values lie behind the keys
-    const float* weight = query ? p.q_weight : value ? nullptr : p.k_weight;
-    if (!query && page_at >= p.max_blocks) return;
-    float largest = 0.f;
-    for (int pos = low + warp; pos < high; pos += THREADS / 32) {
-        const int token = start + pos - past;
-        const size_t at = (size_t)token * width + column;
-        const float factor = weight ? row_factor<TI>(p, at, lane) : 1.f;
-        const float* angles = value || p.cos_sin == nullptr ? nullptr : p.cos_sin + (size_t)min(pos, p.max_pos - 1) * p.rotary_dim;
-        for (int i = lane; i < p.d; i += 32) {
-            const float y = treated<TI>(p, at, i, factor, weight, angles);
-            if (query) {
-                ((TO*)p.q_out)[((size_t)token * p.nq + head - 2 * p.nkv) * p.d + i] = from_float<TO>(y);
-            } else {
-                const float held = nan_if_infinite(y);
-                rows[(pos - page_at * PAGE) * p.d + i] = held;
-                largest = fmaxf(largest, fabsf(held));     // of the finite ones: fmaxf passes over NaN
-            }
+// A row of L lanes, eight neighbouring elements a lane (the lanes from d / 8 on have none): normed where there is a weight, rotated where there are angles.
+// Every lane of the warp calls, rows of a warp may be treated differently, and the exchanges are all lanes' together; `there` says whether this lane has elements.
+template <int L, typename TI>
+__device__ __forceinline__ void treated_row(float (&x)[8], const WriteParams& p, size_t at, int position, const float* weight, bool rotate, bool there) {
+    const int e = (threadIdx.x & (L - 1)) * 8;             // the lane's first element
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (there) {
+        load8(x, (const TI*)p.qkv + at + e, p.wide);
+        for (int s = 1; s < p.n_splits; ++s) {
+            float more[8];
+            load8(more, (const TI*)p.qkv + at + e + s * p.split_stride, p.wide);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] += more[i];
         }
     }
-    if (query) return;
+    if (p.q_weight || p.k_weight) {                        // the same for all lanes, as what follows it
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+        for (int off = L / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const float factor = rsqrtf(sum / (float)p.d + p.eps);
+        if (there && weight) {
+            float w[8];
+            load8(w, weight + e, true);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * factor * w[i];
+        }
+    }
+    if (p.rotary_dim == 0) return;
+    const int half = p.rotary_dim / 2;
+    const float* angles = p.cos_sin + (size_t)min(position, p.max_pos - 1) * p.rotary_dim;
+    if (p.interleaved) {
+        if (there && rotate) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+                if (e + i < p.rotary_dim) {
+                    const float c = angles[(e + i) / 2], s = angles[half + (e + i) / 2], a = x[i], b = x[i + 1];
+                    x[i] = a * c - b * s;
+                    x[i + 1] = b * c + a * s;
+                }
+        }
+    } else {
+        // the other halves of the pairs are half / 8 lanes away
+        const bool first = e < half, turned = e < p.rotary_dim;
+        const int lane = threadIdx.x & 31, from = turned ? lane + (first ? half / 8 : -half / 8) : lane;
+        float other[8], c[8], s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], from);
+        if (there && rotate && turned) {
+            load8(c, angles + (first ? e : e - half), true);
+            load8(s, angles + half + (first ? e : e - half), true);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = first ? x[i] * c[i] - other[i] * s[i] : x[i] * c[i] + other[i] * s[i];
+        }
+    }
+}
+// Infinities as NaN, and the largest finite size: fmaxf passes over NaN.
+__device__ __forceinline__ float hold(float (&x)[8]) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x[i] = nan_if_infinite(x[i]);
+        most = fmaxf(most, fabsf(x[i]));
+    }
+    return most;
+}
+__device__ __forceinline__ uint2 pack8(const float (&x)[8], float by) {
+    return make_uint2(pack4(x[0] * by, x[1] * by, x[2] * by, x[3] * by), pack4(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
+}
+// Eight held numbers under a larger scale.
+__device__ __forceinline__ uint2 smaller8(uint2 w, float by) {
+    const float2 a = floats(w.x), b = floats(w.x >> 16), c = floats(w.y), d = floats(w.y >> 16);
+    return make_uint2(pack4(a.x * by, a.y * by, b.x * by, b.y * by), pack4(c.x * by, c.y * by, d.x * by, d.y * by));
+}
+struct Head { bool query, value; int index; size_t column; };
+__device__ __forceinline__ Head head_of(const WriteParams& p, int h) {     // keys, values, queries
+    Head r;
+    r.query = h >= 2 * p.nkv;
+    r.value = !r.query && h >= p.nkv;
+    r.index = r.query ? h - 2 * p.nkv : r.value ? h - p.nkv : h;
+    r.column = (size_t)(r.query ? r.index : p.nq + h) * p.d;               // values lie behind the keys
+    return r;
+}
+
+// grid: (2 nkv + nq heads, pages that a sequence's tokens touch, sequences).  A row of L lanes a token; what is to be held stays in registers between
+// the page's largest number and the write.
+template <int L, typename TI, typename TO>
+__global__ void __launch_bounds__(THREADS) write_pages_kernel(const WriteParams p) {
+    constexpr int ROWS = THREADS / L, ITERS = (PAGE + ROWS - 1) / ROWS;
+    __shared__ float most[WARPS];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int seq = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = (threadIdx.x & (L - 1)) * 8;
+    const int start = p.seq_start[seq], count = p.seq_start[seq + 1] - start, past = p.seq_past[seq];
+    const int page_at = past / PAGE + blockIdx.y, low = max(past, page_at * PAGE), high = min(past + count, (page_at + 1) * PAGE);
+    if (low >= high) return;
+    const Head head = head_of(p, blockIdx.x);
+    if (!head.query && page_at >= p.max_blocks) return;
+    const float* weight = head.query ? p.q_weight : head.value ? nullptr : p.k_weight;
+    const size_t width = (size_t)(p.nq + 2 * p.nkv) * p.d;
+    float x[ITERS][8], largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int pos = low + i * ROWS + threadIdx.x / L;
+        if (low + i * ROWS >= high) break;                 // the same for the block
+        const bool there = pos < high && e < p.d;
+        const int token = start + min(pos, high - 1) - past;
+        treated_row<L, TI>(x[i], p, token * width + head.column, pos, weight, !head.value, there);
+        if (head.query) {
+            if (there) store8((TO*)p.q_out + ((size_t)token * p.nq + head.index) * p.d + e, x[i]);
+        } else {
+            largest = fmaxf(largest, hold(x[i]));          // lanes without elements hold zeros
+        }
+    }
+    if (head.query) return;
     largest = warp_max(largest);
     if (lane == 0) most[warp] = largest;
     __syncthreads();
-    largest = warp_max(most[lane & (THREADS / 32 - 1)]);
-    const int kvh = value ? head - p.nkv : head;
+    largest = warp_max(most[lane & (WARPS - 1)]);
     const int page = min(max(p.block_table[(size_t)seq * p.max_blocks + page_at], 0), p.n_pages - 1);
-    float* scales = (value ? p.v_scale : p.k_scale) + (size_t)page * p.nkv + kvh;
-    uint8_t* block = (value ? p.v : p.k) + ((size_t)page * p.nkv + kvh) * PAGE * p.d;
-    const int first = low - page_at * PAGE, last = high - page_at * PAGE;
+    float* scales = (head.value ? p.v_scale : p.k_scale) + (size_t)page * p.nkv + head.index;
+    uint8_t* block = (head.value ? p.v : p.k) + ((size_t)page * p.nkv + head.index) * PAGE * p.d;
+    const int first = low - page_at * PAGE;
     const float was = first ? *scales : 0.f;
     const int power = first ? max(power_over(was), power_for(largest)) : power_for(largest);
     const float scale = power_of_two(power), inverse = power_of_two(-power);
     __syncthreads();                                       // everybody has read the scale
     if (threadIdx.x == 0) *scales = scale;
     if (first && scale != was) {                           // what the page holds, under the larger scale
-        const float smaller = was * inverse;
-        uint32_t* words = (uint32_t*)block;
-        for (int i = threadIdx.x; i < first * p.d / 4; i += THREADS) {
-            const float2 a = floats(words[i]), b = floats(words[i] >> 16);
-            words[i] = pack4(a.x * smaller, a.y * smaller, b.x * smaller, b.y * smaller);
+        uint2* words = reinterpret_cast<uint2*>(block);
+        for (int i = threadIdx.x; i < first * p.d / 8; i += THREADS) words[i] = smaller8(words[i], was * inverse);
+    }
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int pos = low + i * ROWS + threadIdx.x / L;
+        if (pos < high && e < p.d) *reinterpret_cast<uint2*>(block + (size_t)(pos - page_at * PAGE) * p.d + e) = pack8(x[i], inverse);
+    }
+}
+
+// One token a sequence at most: a row of L lanes a (sequence, head).
+template <int L, typename TI, typename TO>
+__global__ void __launch_bounds__(THREADS) write_tokens_kernel(const WriteParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int heads = p.nq + 2 * p.nkv, e = (threadIdx.x & (L - 1)) * 8;
+    const long long row = (long long)blockIdx.x * (THREADS / L) + threadIdx.x / L;
+    const int seq = (int)min(row / heads, (long long)p.n_seqs - 1);
+    const Head head = head_of(p, (int)(row % heads));
+    const int token = p.seq_start[seq], pos = p.seq_past[seq], page_at = pos / PAGE;
+    const bool live = row < (long long)p.n_seqs * heads && p.seq_start[seq + 1] > token && (head.query || page_at < p.max_blocks), there = live && e < p.d;
+    float x[8];
+    treated_row<L, TI>(x, p, (size_t)token * heads * p.d + head.column, pos, head.query ? p.q_weight : head.value ? nullptr : p.k_weight, !head.value, there);
+    if (head.query && there) store8((TO*)p.q_out + ((size_t)token * p.nq + head.index) * p.d + e, x);
+    float largest = head.query ? 0.f : hold(x);
+#pragma unroll
+    for (int off = L / 2; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
+    const int page = live && !head.query ? min(max(p.block_table[(size_t)seq * p.max_blocks + page_at], 0), p.n_pages - 1) : 0;
+    float* scales = (head.value ? p.v_scale : p.k_scale) + (size_t)page * p.nkv + head.index;
+    uint8_t* block = (head.value ? p.v : p.k) + ((size_t)page * p.nkv + head.index) * PAGE * p.d;
+    const int first = pos % PAGE;
+    const bool writes = live && !head.query;
+    const float was = writes && first ? *scales : 0.f;
+    __syncwarp();                                          // every lane of the row has read the scale
+    if (!writes || e >= p.d) return;
+    const int power = first ? max(power_over(was), power_for(largest)) : power_for(largest);
+    const float scale = power_of_two(power), inverse = power_of_two(-power);
+    if (e == 0) *scales = scale;
+    if (first && scale != was)                             // what the page holds, under the larger scale
+        for (int i = 0; i < first; ++i) {
+            uint2* words = reinterpret_cast<uint2*>(block + (size_t)i * p.d + e);
+            *words = smaller8(*words, was * inverse);
         }
+    *reinterpret_cast<uint2*>(block + (size_t)first * p.d + e) = pack8(x, inverse);
+}
+
+template <int L, typename TI, typename TO> int launch(const WriteParams& p, int max_q_len, cudaStream_t stream) {
+    const int heads = p.nq + 2 * p.nkv;
+    if (max_q_len == 1) {
+        const long long blocks = ((long long)p.n_seqs * heads + THREADS / L - 1) / (THREADS / L);
+        QT_REQUIRE(blocks <= 0x7fffffff, "qkv_write_cache8: %d sequences of %d heads", p.n_seqs, heads);
+        launch_kernel(write_tokens_kernel<L, TI, TO>, dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
+    } else {
+        const int pages = (max_q_len - 1 + PAGE - 1) / PAGE + 1;
+        QT_REQUIRE(pages <= 65535 && p.n_seqs <= 65535, "qkv_write_cache8: %d sequences of up to %d tokens", p.n_seqs, max_q_len);
+        launch_kernel(write_pages_kernel<L, TI, TO>, dim3(heads, pages, p.n_seqs), dim3(THREADS), 0, stream, p);
     }
-    uint32_t* words = (uint32_t*)(block + (size_t)first * p.d);
-    const float* from = rows + first * p.d;
-    for (int i = threadIdx.x; i < (last - first) * p.d / 4; i += THREADS) {
-        const float4 y = *reinterpret_cast<const float4*>(from + 4 * i);
-        words[i] = pack4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
-    }
+    QT_CHECK_LAUNCH("qkv_write_cache8");
+    return QT_OK;
+}
+template <typename TI, typename TO> int launch_size(const WriteParams& p, int max_q_len, cudaStream_t stream) {
+    if (p.d <= 32) return launch<4, TI, TO>(p, max_q_len, stream);
+    if (p.d <= 64) return launch<8, TI, TO>(p, max_q_len, stream);
+    if (p.d <= 128) return launch<16, TI, TO>(p, max_q_len, stream);
+    return launch<32, TI, TO>(p, max_q_len, stream);
 }
 
 }  // namespace
 
-extern "C" int qt_qkv_write_cache8(const void* qkv, int in_dtype, int n_splits, long long split_stride, void* q_out, int out_dtype, void* k, void* v, float* k_scale,
-                                   float* v_scale, const int* seq_start, const int* seq_past, int n_seqs, int max_q_len, const int* block_table, int max_blocks, int n_pages,
-                                   const float* q_weight, const float* k_weight, float eps, const float* cos_sin, int rotary_dim, int max_pos, int interleaved, int nq,
-                                   int nkv, int d, void* stream) {
+// The arguments of the call below as one structure.
+struct WriteCall {
+    const void* qkv;
+    long long split_stride;
+    void *q_out, *k, *v;
+    float *k_scale, *v_scale;
+    const int *seq_start, *seq_past, *block_table;
+    const float *q_weight, *k_weight, *cos_sin;
+    void* stream;
+    double eps;
+    int in_dtype, out_dtype, n_splits, n_seqs, max_q_len, max_blocks, n_pages, rotary_dim, max_pos, interleaved, nq, nkv, d, unused;
+};
+static_assert(sizeof(WriteCall) == 15 * 8 + 14 * 4, "15 numbers of 64 bits and 14 of 32, without gaps");
+
+extern "C" int qt_qkv_write_cache8(const WriteCall* call) {
+    const WriteCall& c = *call;
+    const int n_seqs = c.n_seqs, max_q_len = c.max_q_len, nq = c.nq, nkv = c.nkv, d = c.d, rotary_dim = c.rotary_dim;
     if (n_seqs == 0 || max_q_len == 0) return QT_OK;
-    QT_REQUIRE(n_seqs > 0 && n_seqs <= 65535 && max_q_len > 0 && nq > 0 && nkv > 0 && n_pages > 0 && max_blocks > 0 && n_splits >= 1, "qkv_write_cache8: bad sizes");
+    QT_REQUIRE(n_seqs > 0 && max_q_len > 0 && nq > 0 && nkv > 0 && c.n_pages > 0 && c.max_blocks > 0 && c.n_splits >= 1, "qkv_write_cache8: bad sizes");
     QT_REQUIRE(d > 0 && d <= 256 && d % 16 == 0, "qkv_write_cache8: head_dim=%d is not a multiple of 16 up to 256", d);
-    QT_REQUIRE(rotary_dim >= 0 && rotary_dim <= d && rotary_dim % 2 == 0 && (rotary_dim == 0 || (cos_sin && max_pos > 0)), "qkv_write_cache8: rotary_dim=%d of %d", rotary_dim, d);
-    const int pages = (max_q_len - 1 + PAGE - 1) / PAGE + 1;
-    QT_REQUIRE(pages <= 65535, "qkv_write_cache8: %d tokens of a sequence are too many", max_q_len);
-    WriteParams p{qkv, n_splits, (size_t)split_stride, q_out, (uint8_t*)k, (uint8_t*)v, k_scale, v_scale, seq_start, seq_past, block_table, max_blocks, n_pages, q_weight,
-                  k_weight, eps, rotary_dim ? cos_sin : nullptr, rotary_dim, max_pos, interleaved, nq, nkv, d};
-    const dim3 grid(2 * nkv + nq, pages, n_seqs);
-    const size_t smem = (size_t)PAGE * d * 4;
-#define QT_WRITE(TI, TO)                                                                                                                                     \
-    do {                                                                                                                                                     \
-        const cudaError_t raised = raise_shared<qkv_write_cache8_kernel<TI, TO>>(PAGE * 256 * 4);                                                             \
-        if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "qkv_write_cache8: cannot raise shared memory: %s", cudaGetErrorString(raised));                    \
-        launch_kernel(qkv_write_cache8_kernel<TI, TO>, grid, dim3(THREADS), smem, (cudaStream_t)stream, p);                                                   \
-        QT_CHECK_LAUNCH("qkv_write_cache8");                                                                                                                  \
-        return QT_OK;                                                                                                                                         \
-    } while (0)
-    if (in_dtype == QT_F32 && out_dtype == QT_F32) QT_WRITE(float, float);
-    if (in_dtype == QT_F32 && out_dtype == QT_BF16) QT_WRITE(float, __nv_bfloat16);
-    if (in_dtype == QT_BF16 && out_dtype == QT_BF16) QT_WRITE(__nv_bfloat16, __nv_bfloat16);
-    if (in_dtype == QT_BF16 && out_dtype == QT_F32) QT_WRITE(__nv_bfloat16, float);
-#undef QT_WRITE
-    QT_FAIL(QT_ERR_ARG, "qkv_write_cache8: unknown element types %d, %d", in_dtype, out_dtype);
+    QT_REQUIRE(rotary_dim >= 0 && rotary_dim <= d && rotary_dim % (c.interleaved ? 2 : 16) == 0 && (rotary_dim == 0 || (c.cos_sin && c.max_pos > 0)),
+               "qkv_write_cache8: rotary_dim=%d of %d (of pairs that are not neighbours a multiple of 16)", rotary_dim, d);
+    QT_REQUIRE((((uintptr_t)c.q_out | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.q_weight | (uintptr_t)c.k_weight | (uintptr_t)c.cos_sin) & 15) == 0,
+               "qkv_write_cache8: operands must be 16-byte aligned");
+    const int size = c.in_dtype == QT_F32 ? 4 : 2;
+    const WriteParams p{c.qkv, c.n_splits, (size_t)c.split_stride, (uintptr_t)c.qkv % 16 == 0 && c.split_stride * size % 16 == 0, c.q_out, (uint8_t*)c.k, (uint8_t*)c.v, c.k_scale,
+                        c.v_scale, c.seq_start, c.seq_past, c.block_table, n_seqs, c.max_blocks, c.n_pages, c.q_weight, c.k_weight, (float)c.eps, rotary_dim ? c.cos_sin : nullptr,
+                        rotary_dim, c.max_pos, c.interleaved, nq, nkv, d};
+    cudaStream_t s = (cudaStream_t)c.stream;
+    if (c.in_dtype == QT_F32 && c.out_dtype == QT_F32) return launch_size<float, float>(p, max_q_len, s);
+    if (c.in_dtype == QT_F32 && c.out_dtype == QT_BF16) return launch_size<float, __nv_bfloat16>(p, max_q_len, s);
+    if (c.in_dtype == QT_BF16 && c.out_dtype == QT_BF16) return launch_size<__nv_bfloat16, __nv_bfloat16>(p, max_q_len, s);
+    if (c.in_dtype == QT_BF16 && c.out_dtype == QT_F32) return launch_size<__nv_bfloat16, float>(p, max_q_len, s);
+    QT_FAIL(QT_ERR_ARG, "qkv_write_cache8: unknown element types %d, %d", c.in_dtype, c.out_dtype);
 }
 
 QT_DEFINE_LAST_ERROR(cache8)

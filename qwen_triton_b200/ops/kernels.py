@@ -147,18 +147,11 @@ _SIGNATURES = {
         "qt_gemm_fp8": [ctypes.c_char_p],                     # an Fp8Call (_FP8_CALL)
     },
     "cache8": {
-        # qkv, in_dtype, n_splits, split_stride, q_out, out_dtype, k, v, k_scale, v_scale, seq_start, seq_past, n_seqs, max_q_len, block_table, max_blocks, n_pages,
-        # q_weight, k_weight, eps, cos_sin, rotary_dim, max_pos, interleaved, nq, nkv, d, stream
-        "qt_qkv_write_cache8": [_c_ptr, _c_int, _c_int, _c_ll, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
-                                _c_ptr, _c_ptr, _c_float, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
+        "qt_qkv_write_cache8": [ctypes.c_char_p],             # a WriteCall (_WRITE8_CALL)
     },
     "attention_cache8": {
-        # q, dtype, k, v, k_scale, v_scale, out, block_table, max_blocks, n_pages, seq_len, n_seqs, nq, nkv, d, scale, ranges, range_pages, part_acc, part_ml, stream
-        "qt_attention_decode_cache8": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float,
-                                       _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr],
-        # q, dtype, k, v, k_scale, v_scale, out, block_table, max_blocks, n_pages, seq_start, seq_past, n_seqs, max_q_len, nq, nkv, d, scale, stream
-        "qt_attention_prefill_cache8": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int,
-                                        _c_int, _c_float, _c_ptr],
+        "qt_attention_decode_cache8": [ctypes.c_char_p],      # a Cache8Call (_CACHE8_CALL)
+        "qt_attention_prefill_cache8": [ctypes.c_char_p],
     },
     "gemm_f32": {
         "qt_gemm_f32": [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr],
@@ -1652,9 +1645,13 @@ def fp8_rows(rows: int, columns: int, device) -> Fp8Rows:
                    torch.empty((-(-columns // FP8_GROUP), rows), dtype=torch.float32, device=device))
 
 
+def _current_device() -> int:
+    return _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+
+
 def _same_device(name: str, *tensors: torch.Tensor) -> None:
     """All on the current device, whose current stream the kernels are launched on."""
-    device = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+    device = _current_device()
     for tensor in tensors:
         if tensor.get_device() != device:
             raise KernelError(f"{name}: a tensor on {tensor.device}, the current device is cuda:{device}")
@@ -1729,7 +1726,7 @@ def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, 
     n, k = w.shape
     rows = x if given else scratch
     values = x.values if given else x
-    m, device = values.shape[0], _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+    m, device = values.shape[0], _current_device()
     # one expression for a call that is in order: the host's part of a short product is its time
     if not (values.dim() == 2 and values.shape[1] == k and out.shape == (m, n) and out.is_contiguous() and out.dtype in _CODES and rows is not None
             and rows.values.shape[1] == k and rows.values.shape[0] >= m and (given or (x.dtype in _CODES and x.is_contiguous()))
@@ -1808,7 +1805,7 @@ def cache8(pages: int, kv_heads: int, head_dim: int, device) -> Cache8:
 def qkv_write_cache8(qkv: GemmOut, q_out: torch.Tensor, cache: Cache8, seq_start: torch.Tensor, seq_past: torch.Tensor, block_table: torch.Tensor, max_q_len: int,
                      q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float, cos_sin: torch.Tensor | None, interleaved: bool = False) -> None:
     """``qk_norm_rope_write`` into a cache in 8 bits: per-head RMS norm of q and k (where weights are given) and rotation (where a table is), q to ``q_out``
-    [T, nq, d], k and v of the step's tokens to the pages of their sequences.
+    [T, nq, d], k and v of the step's tokens to the pages of their sequences.  Of pairs that are not neighbours the table has a multiple of 16 columns.
 
     ``qkv`` [*, T, (nq + 2 nkv) d]; sequence i has the tokens from ``seq_start[i]`` (int32 [sequences + 1]) on, at most ``max_q_len``, and ``seq_past[i]``
     earlier ones in the pages that row i of ``block_table`` (int32) lists; no two sequences write the same page.
@@ -1816,30 +1813,58 @@ def qkv_write_cache8(qkv: GemmOut, q_out: torch.Tensor, cache: Cache8, seq_start
     The scale of a page and head is 2^e with the smallest e between -40 and 40 whose 448-fold reaches every finite number there; values are rounded to e4m3
     once, and beyond 448 * 2^40 end there.  e starts with the write of a page's first place and then only grows: what the page's earlier places hold is then brought
     under the larger scale (exact but for numbers below 2^-6 of it).  Infinities are held as NaN.  Places behind a sequence's last token stay as they were."""
+    proj, device = qkv.tensor, _current_device()
+    n_seqs, tokens = seq_past.shape[0], proj.shape[1]
+    num_heads = q_out.shape[1]
+    k = cache.k
+    _, kv_heads, _, head_dim = k.shape
+    # one expression for a call that is in order: the host's part of a short step is its time
+    if not (q_out.shape == (tokens, num_heads, head_dim) and proj.shape[2] == (num_heads + 2 * kv_heads) * head_dim and proj.dtype in _CODES and q_out.dtype in _CODES
+            and q_out.is_contiguous() and seq_start.shape == (n_seqs + 1,) and seq_past.dim() == 1 and block_table.dim() == 2 and block_table.shape[0] == n_seqs
+            and block_table.shape[1] > 0 and block_table.dtype is seq_start.dtype is seq_past.dtype is torch.int32
+            and (q_weight is None or (q_weight.shape == (head_dim,) and q_weight.dtype is torch.float32 and q_weight.get_device() == device and q_weight.is_contiguous()))
+            and (k_weight is None or (k_weight.shape == (head_dim,) and k_weight.dtype is torch.float32 and k_weight.get_device() == device and k_weight.is_contiguous()))
+            and (cos_sin is None or (cos_sin.dim() == 2 and cos_sin.dtype is torch.float32 and cos_sin.get_device() == device and cos_sin.is_contiguous()))
+            and block_table.is_contiguous() and seq_start.is_contiguous() and seq_past.is_contiguous() and 0 <= max_q_len <= tokens
+            and proj.get_device() == q_out.get_device() == k.get_device() == seq_start.get_device() == seq_past.get_device() == block_table.get_device() == device):
+        _check_write_cache8(qkv, q_out, cache, seq_start, seq_past, block_table, max_q_len, q_weight, k_weight, cos_sin)
+    _call("cache8", "qt_qkv_write_cache8",
+          _WRITE8_CALL.pack(proj.data_ptr(), qkv.split_stride, q_out.data_ptr(), k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+                            seq_start.data_ptr(), seq_past.data_ptr(), block_table.data_ptr(), _ptr(q_weight) or 0, _ptr(k_weight) or 0, _ptr(cos_sin) or 0, _stream(), eps,
+                            _CODES[proj.dtype], _CODES[q_out.dtype], proj.shape[0], n_seqs, max_q_len, block_table.shape[1], k.shape[0],
+                            0 if cos_sin is None else cos_sin.shape[1], 0 if cos_sin is None else cos_sin.shape[0], interleaved, num_heads, kv_heads, head_dim, 0))
+
+
+# qkv, split_stride, q_out, k, v, k_scale, v_scale, seq_start, seq_past, block_table, q_weight, k_weight, cos_sin, stream, eps, in_dtype, out_dtype, n_splits, n_seqs,
+# max_q_len, max_blocks, n_pages, rotary_dim, max_pos, interleaved, nq, nkv, d, unused: a structure costs the host less than as many arguments
+_WRITE8_CALL = struct.Struct("@Pq12Pd14i")
+
+
+def _check_write_cache8(qkv, q_out, cache, seq_start, seq_past, block_table, max_q_len, q_weight, k_weight, cos_sin) -> None:
+    """The refusal of a call that is not in order."""
     tokens, num_heads, head_dim = q_out.shape
     n_seqs = seq_past.shape[0]
     _need(q_out, "q_out", shape=(tokens, num_heads, cache.head_dim))
+    _code(q_out, "q_out")
+    _code(qkv.tensor, "qkv")
     if qkv.rows != tokens or qkv.cols != (num_heads + 2 * cache.kv_heads) * head_dim:
         raise KernelError(f"qkv_write_cache8: a projection {tuple(qkv.tensor.shape)} for {tokens} tokens of {num_heads} + 2 * {cache.kv_heads} heads of {head_dim}")
     _need(seq_past, "seq_past", torch.int32, (n_seqs,))
     _need(seq_start, "seq_start", torch.int32, (n_seqs + 1,))
-    _need(block_table, "block_table", torch.int32, (n_seqs, block_table.shape[-1]))
+    _need(block_table, "block_table", torch.int32, (n_seqs, max(1, block_table.shape[-1])))
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None:
             _need(w, name, torch.float32, (head_dim,))
-    rotary_dim, max_pos = 0, 0
+            _same_device("qkv_write_cache8", w)
     if cos_sin is not None:
         _need(cos_sin, "cos_sin", torch.float32)
-        max_pos, rotary_dim = cos_sin.shape
+        _same_device("qkv_write_cache8", cos_sin)
     if not qkv.tensor.is_cuda:
         raise KernelError("qkv must be a CUDA tensor (there is no host path)")
     if max_q_len < 0 or max_q_len > tokens:
         raise KernelError(f"qkv_write_cache8: max_q_len={max_q_len} of {tokens} tokens")
     _same_device("qkv_write_cache8", qkv.tensor, q_out, cache.k, seq_start, seq_past, block_table)
-    _call("cache8", "qt_qkv_write_cache8", _ptr(qkv.tensor), _code(qkv.tensor, "qkv"), qkv.n_splits, qkv.split_stride, _ptr(q_out), _code(q_out, "q_out"), _ptr(cache.k),
-          _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(seq_start), _ptr(seq_past), n_seqs, int(max_q_len), _ptr(block_table), block_table.shape[1],
-          cache.pages, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos_sin), rotary_dim, max_pos, 1 if interleaved else 0, num_heads, cache.kv_heads, head_dim,
-          _stream())
+    raise KernelError("qkv_write_cache8: this call is not in order")
 
 
 _CLUSTER_RANGES, _MOST_RANGES = 8, 64         # ranges that join in a cluster, and through memory
@@ -1848,21 +1873,26 @@ _CLUSTER_RANGES, _MOST_RANGES = 8, 64         # ranges that join in a cluster, a
 @dataclass(frozen=True)
 class Decode8Plan:
     """How ``attention_decode_cache8`` cuts the keys of its sequences (``decode8_plan``): ``ranges`` ranges of ``range_pages`` pages, the last one taking
-    whatever is left.  Any plan gives the result of every call with its sizes."""
+    whatever is left, that join in clusters of blocks (at most eight) or through memory and a second launch.  Any plan gives the result of every call with its sizes."""
 
     q_shape: tuple[int, int, int]
     num_kv_heads: int
     dtype: torch.dtype
     ranges: int
     range_pages: int
+    clusters: bool = True
+
+    @property
+    def through_memory(self) -> bool:
+        return self.ranges > 1 and not (self.clusters and self.ranges <= _CLUSTER_RANGES)
 
     @property
     def acc_elements(self) -> int:
-        return self.q_shape[0] * self.q_shape[1] * self.ranges * self.q_shape[2] if self.ranges > _CLUSTER_RANGES else 0
+        return self.q_shape[0] * self.q_shape[1] * self.ranges * self.q_shape[2] if self.through_memory else 0
 
     @property
     def ml_elements(self) -> int:
-        return self.q_shape[0] * self.q_shape[1] * self.ranges * 2 if self.ranges > _CLUSTER_RANGES else 0
+        return self.q_shape[0] * self.q_shape[1] * self.ranges * 2 if self.through_memory else 0
 
 
 def decode8_plan(batch: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, max_context: int, sms: int = 148) -> Decode8Plan:
@@ -1871,9 +1901,22 @@ def decode8_plan(batch: int, *, num_heads: int, num_kv_heads: int, head_dim: int
         raise KernelError(f"decode8_plan: {batch} sequences of {num_heads} heads over {num_kv_heads} of {head_dim}, {dtype}, {max_context} keys")
     pages = max(1, -(-max_context // 64))
     walks = max(1, batch * num_kv_heads * -(-(num_heads // num_kv_heads) // 8))
-    ranges = max(1, min(4 * sms // walks, -(-pages // 4), 64))
+    # blocks that are resident at once
+    slots = sms * (2 if head_dim > 128 or (dtype == torch.float32 and head_dim > 64) else 3 if head_dim > 64 or dtype == torch.float32 else 4)
+    clusters = True
+    if walks >= 128 and pages >= 48:
+        # many sequences, seldom of one length: equal portions, so that the longest does not keep a cluster's other blocks (48 of 3,000 to 12,000: 130 us, uncut 153)
+        ranges, clusters = min(_MOST_RANGES, -(-pages // 16)), False
+    else:
+        # as many blocks as are resident; at least two pages each, and eight where so many ranges join through memory
+        ranges = max(1, min(slots // walks, -(-pages // 2) if pages > 4 else 1, max(_CLUSTER_RANGES, pages // 8), _MOST_RANGES))
     range_pages = -(-pages // ranges)
-    return Decode8Plan((batch, num_heads, head_dim), num_kv_heads, dtype, -(-pages // range_pages), range_pages)
+    return Decode8Plan((batch, num_heads, head_dim), num_kv_heads, dtype, -(-pages // range_pages), range_pages, clusters)
+
+
+# q, k, v, k_scale, v_scale, out, block_table, seq_start, seq_past, seq_len, part_acc, part_ml, status, stream, scale, dtype, max_blocks, n_pages, n_seqs, n_tokens, max_q_len,
+# nq, nkv, d, ranges, range_pages, clusters: a structure costs the host less than as many arguments
+_CACHE8_CALL = struct.Struct("@14Pd12i")
 
 
 def _check_cache8(name: str, q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, n_seqs: int) -> None:
@@ -1891,15 +1934,36 @@ def _check_cache8(name: str, q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
 def attention_decode_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor, scale: float, plan: Decode8Plan,
                             part_acc: torch.Tensor | None = None, part_ml: torch.Tensor | None = None) -> None:
     """``attention_decode`` over a cache in 8 bits: one query token per sequence, q and out [sequences, nq, d] (bfloat16 or float32); ``seq_len`` counts the keys
-    it sees (none: the result is zero).  Where the plan cuts the keys into more than eight ranges their partial results pass through ``part_acc`` and ``part_ml`` (float, at least
+    it sees (none: the result is zero).  Where the plan's ranges join through memory their partial results pass through ``part_acc`` and ``part_ml`` (float, at least
     ``plan.acc_elements`` and ``plan.ml_elements``).  What lies behind a sequence's last key is not looked at."""
+    k, device = cache.k, _current_device()
+    shape, through_memory = plan.q_shape, plan.through_memory
+    # one expression for a call that is in order: the host's part of a short step is its time
+    if not (q.shape == shape == out.shape and q.dtype is plan.dtype is out.dtype and k.shape[1] == plan.num_kv_heads and k.shape[3] == shape[2] and shape[1] % k.shape[1] == 0
+            and block_table.dim() == 2 and block_table.shape[0] == shape[0] and block_table.shape[1] > 0 and seq_len.shape == shape[:1]
+            and block_table.dtype is seq_len.dtype is torch.int32 and 1 <= plan.ranges <= _MOST_RANGES and plan.range_pages >= 1
+            and q.is_contiguous() and out.is_contiguous() and block_table.is_contiguous() and seq_len.is_contiguous()
+            and q.get_device() == out.get_device() == k.get_device() == block_table.get_device() == seq_len.get_device() == device
+            and (not through_memory or (part_acc is not None and part_ml is not None and part_acc.dtype is part_ml.dtype is torch.float32 and part_acc.is_contiguous()
+                                        and part_ml.is_contiguous() and part_acc.numel() >= plan.acc_elements and part_ml.numel() >= plan.ml_elements
+                                        and part_acc.get_device() == part_ml.get_device() == device))):
+        _check_decode_cache8(q, cache, out, block_table, seq_len, plan, part_acc, part_ml)
+    _call("attention_cache8", "qt_attention_decode_cache8",
+          _CACHE8_CALL.pack(q.data_ptr(), k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(), 0, 0,
+                            seq_len.data_ptr(), part_acc.data_ptr() if through_memory else 0, part_ml.data_ptr() if through_memory else 0, 0, _stream(), scale,
+                            _CODES[q.dtype], block_table.shape[1], k.shape[0], shape[0], shape[0], 1, shape[1], k.shape[1], shape[2], plan.ranges, plan.range_pages, plan.clusters),
+          launches=2 if through_memory else 1)
+
+
+def _check_decode_cache8(q, cache, out, block_table, seq_len, plan, part_acc, part_ml) -> None:
+    """The refusal of a call that is not in order."""
     _check_cache8("attention_decode_cache8", q, cache, out, block_table, q.shape[0])
     _need(seq_len, "seq_len", torch.int32, q.shape[:1])
-    if tuple(q.shape) != plan.q_shape or q.dtype != plan.dtype or cache.kv_heads != plan.num_kv_heads:
+    if tuple(q.shape) != tuple(plan.q_shape) or q.dtype != plan.dtype or cache.kv_heads != plan.num_kv_heads:
         raise KernelError(f"attention_decode_cache8: a plan for {plan.q_shape} over {plan.num_kv_heads} kv heads, {plan.dtype}; queries {tuple(q.shape)} over {cache.kv_heads}, {q.dtype}")
     if not 1 <= plan.ranges <= _MOST_RANGES or plan.range_pages < 1:
         raise KernelError(f"attention_decode_cache8: {plan.ranges} ranges of {plan.range_pages} pages")
-    if plan.ranges > _CLUSTER_RANGES:
+    if plan.through_memory:
         for name, part, need in (("part_acc", part_acc, plan.acc_elements), ("part_ml", part_ml, plan.ml_elements)):
             if part is None:
                 raise KernelError(f"attention_decode_cache8: {name} is required for {plan.ranges} ranges")
@@ -1908,9 +1972,7 @@ def attention_decode_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, b
                 raise KernelError(f"attention_decode_cache8: {name} holds {part.numel()} of {need} elements")
         _same_device("attention_decode_cache8", part_acc, part_ml)
     _same_device("attention_decode_cache8", seq_len)
-    _call("attention_cache8", "qt_attention_decode_cache8", _ptr(q), _code(q, "q"), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(out),
-          _ptr(block_table), block_table.shape[1], cache.pages, _ptr(seq_len), q.shape[0], q.shape[1], cache.kv_heads, cache.head_dim, float(scale), plan.ranges,
-          plan.range_pages, _ptr(part_acc), _ptr(part_ml), _stream(), launches=2 if plan.ranges > _CLUSTER_RANGES else 1)
+    raise KernelError("attention_decode_cache8: this call is not in order")
 
 
 def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_start: torch.Tensor, seq_past: torch.Tensor,
@@ -1924,9 +1986,10 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     if max_q_len < 0 or max_q_len > q.shape[0]:
         raise KernelError(f"attention_prefill_cache8: max_q_len={max_q_len} of {q.shape[0]} tokens")
     _same_device("attention_prefill_cache8", seq_start, seq_past)
-    _call("attention_cache8", "qt_attention_prefill_cache8", _ptr(q), _code(q, "q"), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(out),
-          _ptr(block_table), block_table.shape[1], cache.pages, _ptr(seq_start), _ptr(seq_past), n_seqs, int(max_q_len), q.shape[1], cache.kv_heads, cache.head_dim,
-          float(scale), _stream())
+    _call("attention_cache8", "qt_attention_prefill_cache8",
+          _CACHE8_CALL.pack(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(),
+                            seq_start.data_ptr(), seq_past.data_ptr(), 0, 0, 0, _status_word(q.device).data_ptr(), _stream(), scale, _CODES[q.dtype], block_table.shape[1],
+                            cache.pages, n_seqs, q.shape[0], max_q_len, q.shape[1], cache.kv_heads, cache.head_dim, 1, 1, 0))
 
 
 # ----------------------------------------------------------------------------- experts chosen by a table

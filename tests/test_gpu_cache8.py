@@ -82,7 +82,7 @@ def test_decode_lengths(length):
     _decode([length, 3], 4, 4, 64, F32, seed=length)
 
 
-@pytest.mark.parametrize("ranges", [(1, 1000), (1, 1), (2, 6), (4, 3), (7, 2), (13, 1), (3, 1), (64, 5), (9, 2), (16, 1)])
+@pytest.mark.parametrize("ranges", [(1, 1000), (1, 1), (2, 6), (4, 3), (7, 2), (13, 1), (3, 1), (64, 5), (9, 2), (16, 1), (2, 6, False), (7, 2, False), (5, 1, False)])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_decode_in_ranges(ranges, dtype):
     """Any cut gives the result: ranges that are empty, a last one that takes many pages, sequences without keys."""
