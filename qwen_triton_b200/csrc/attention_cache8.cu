@@ -13,6 +13,7 @@
 // maximum is that of the score plus log2 s_v, so that halves hold the weights whatever scales the pages have; the sum of the p_j takes the scale back out.
 //
 // Ranges of a sequence join in the cluster that they form (up to eight), or through memory and a second launch.
+#include "cache8_call.h"
 #include "fp8.cuh"
 
 #include <math.h>
@@ -484,20 +485,6 @@ int check(const char* name, int dtype, int nq, int nkv, int d, int max_blocks, i
 }
 
 }  // namespace
-
-// The arguments of the two calls below as one structure.
-struct Cache8Call {
-    const void *q, *k, *v;
-    const float *k_scale, *v_scale;
-    void* out;
-    const int *block_table, *seq_start, *seq_past, *seq_len;
-    float *part_acc, *part_ml;
-    int* status;
-    void* stream;
-    double scale;
-    int dtype, max_blocks, n_pages, n_seqs, n_tokens, max_q_len, nq, nkv, d, ranges, range_pages, clusters;
-};
-static_assert(sizeof(Cache8Call) == 15 * 8 + 12 * 4, "14 addresses, a number of 64 bits and 12 of 32, without gaps");
 
 // One query a sequence: q and out [n_seqs, nq, d], seq_len [n_seqs] keys each (none: zeros).  Ranges join in clusters of blocks (at most eight,
 // with `clusters`) or through memory: part_acc holds n_seqs nq ranges d floats and part_ml n_seqs nq ranges 2.  A block walks range_pages pages of its

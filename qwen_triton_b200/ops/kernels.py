@@ -153,6 +153,9 @@ _SIGNATURES = {
         "qt_attention_decode_cache8": [ctypes.c_char_p],      # a Cache8Call (_CACHE8_CALL)
         "qt_attention_prefill_cache8": [ctypes.c_char_p],
     },
+    "attention_cache8_tc": {
+        "qt_attention_prefill_cache8_tc": [ctypes.c_char_p],  # a Cache8Call
+    },
     "gemm_f32": {
         "qt_gemm_f32": [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr],
     },
@@ -1976,9 +1979,37 @@ def _check_decode_cache8(q, cache, out, block_table, seq_len, plan, part_acc, pa
 
 
 def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_start: torch.Tensor, seq_past: torch.Tensor,
-                             max_q_len: int, scale: float) -> None:
+                             max_q_len: int, scale: float, impl: str | None = None) -> None:
     """``attention_prefill`` over a cache in 8 bits: packed queries [T, nq, d], sequence i's from ``seq_start[i]`` on (at most ``max_q_len``), behind ``seq_past[i]`` earlier
-    tokens; the cache already holds this step's keys; a query sees the keys up to its own."""
+    tokens; the cache already holds this step's keys; a query sees the keys up to its own.
+
+    ``impl``: "tc" (tcgen05: bfloat16 heads of 64 or 128 under a positive scale; the default for those and more than 64 rows a kv head) or "mma" (any call).  A value
+    that is not a number makes the results of the queries that see it NaN, and on "tc" and "mma" may make those of earlier queries of the call that read its
+    page."""
+    n_seqs, device, k = seq_past.shape[0], _current_device(), cache.k
+    # one expression for a call that is in order
+    if not (q.dim() == 3 and q.shape == out.shape and q.dtype is out.dtype and q.dtype in _CODES and q.shape[2] == k.shape[3] and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0
+            and block_table.dim() == 2 and block_table.shape[0] == n_seqs and block_table.shape[1] > 0 and seq_past.dim() == 1 and seq_start.shape == (n_seqs + 1,)
+            and block_table.dtype is seq_start.dtype is seq_past.dtype is torch.int32 and 0 <= max_q_len <= q.shape[0]
+            and q.is_contiguous() and out.is_contiguous() and block_table.is_contiguous() and seq_start.is_contiguous() and seq_past.is_contiguous()
+            and q.get_device() == out.get_device() == k.get_device() == block_table.get_device() == seq_start.get_device() == seq_past.get_device() == device):
+        _check_prefill_cache8(q, cache, out, block_table, seq_start, seq_past, max_q_len)
+    on_tc = q.dtype is torch.bfloat16 and k.shape[3] in (64, 128) and scale > 0
+    if impl not in (None, "tc", "mma") or (impl == "tc" and not on_tc):
+        raise KernelError(f"attention_prefill_cache8: impl={impl!r} for {q.dtype}, heads of {k.shape[3]}, a scale of {scale}")
+    if impl == "mma" or (impl is None and max_q_len * (q.shape[1] // k.shape[1]) <= _MMA_ROWS):
+        on_tc = False
+    _call(*(("attention_cache8_tc", "qt_attention_prefill_cache8_tc") if on_tc else ("attention_cache8", "qt_attention_prefill_cache8")),
+          _CACHE8_CALL.pack(q.data_ptr(), k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(),
+                            seq_start.data_ptr(), seq_past.data_ptr(), 0, 0, 0, _status_word(q.device).data_ptr(), _stream(), scale, _CODES[q.dtype], block_table.shape[1],
+                            k.shape[0], n_seqs, q.shape[0], max_q_len, q.shape[1], k.shape[1], k.shape[3], 1, 1, 0))
+
+
+_MMA_ROWS = 64             # query rows a kv head (tokens times its group) up to which mma.sync, eight rows a block, takes prompts
+
+
+def _check_prefill_cache8(q, cache, out, block_table, seq_start, seq_past, max_q_len) -> None:
+    """The refusal of a call that is not in order."""
     n_seqs = seq_past.shape[0]
     _check_cache8("attention_prefill_cache8", q, cache, out, block_table, n_seqs)
     _need(seq_past, "seq_past", torch.int32, (n_seqs,))
@@ -1986,10 +2017,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     if max_q_len < 0 or max_q_len > q.shape[0]:
         raise KernelError(f"attention_prefill_cache8: max_q_len={max_q_len} of {q.shape[0]} tokens")
     _same_device("attention_prefill_cache8", seq_start, seq_past)
-    _call("attention_cache8", "qt_attention_prefill_cache8",
-          _CACHE8_CALL.pack(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(),
-                            seq_start.data_ptr(), seq_past.data_ptr(), 0, 0, 0, _status_word(q.device).data_ptr(), _stream(), scale, _CODES[q.dtype], block_table.shape[1],
-                            cache.pages, n_seqs, q.shape[0], max_q_len, q.shape[1], cache.kv_heads, cache.head_dim, 1, 1, 0))
+    raise KernelError("attention_prefill_cache8: this call is not in order")
 
 
 # ----------------------------------------------------------------------------- experts chosen by a table

@@ -96,11 +96,13 @@ def write(values, scales, rows, table, start, past):
                 scales[page, h] = scale
 
 
-def attention(q, k, v, table, counts, past, scale, half_digits: int):
+def attention(q, k, v, table, counts, past, scale, half_digits: int, split: bool = False):
     """(out, bound) for packed queries [tokens, heads, d] over held keys and values [pages, kv_heads, 64, d] (float64, scales within): ``counts`` queries of
     each sequence behind ``past`` earlier tokens.  The bound: a score's sum of d products off by 2^-23 of their sizes' sum each, its scaling and exponential by
     2^-21 of the score and 2^-21; a weight is rounded to ``half_digits`` binary digits; sums over the keys off by 2^-23 an addition, of which a block's
-    order has at most 200 for a range of keys in turn and the joins, the others within an instruction."""
+    order has at most 200 for a range of keys in turn and the joins, the others within an instruction.  ``split``: queries are the sum of two e4m3 numbers, the
+    largest of a row between 2^7 and 2^8.  The nearest one leaves at most 2^-4 of an element, four binary digits of the eight of a bfloat16 number, which the second
+    holds down to its last place, 2^-9: off by at most 2^-10, 2^-17 of the row's largest."""
     q = q.double().cpu()
     heads, group = q.shape[1], q.shape[1] // k.shape[1]
     out, bound = torch.zeros_like(q), torch.zeros_like(q)
@@ -114,6 +116,8 @@ def attention(q, k, v, table, counts, past, scale, half_digits: int):
                 rows = q[at:at + n, h]
                 s = rows @ keys.T * scale
                 off = (rows.abs() @ keys.abs().T * abs(scale)) * (keys.shape[1] + 4) * 2.0 ** -23 + s.abs() * 2.0 ** -21 + 2.0 ** -21
+                if split:
+                    off = off + rows.abs().amax(1, keepdim=True) * keys.abs().sum(1)[None, :] * abs(scale) * 2.0 ** -17
                 hidden = torch.arange(total)[None, :] > past[i] + torch.arange(n)[:, None]
                 p = torch.softmax(s.masked_fill(hidden, -math.inf), dim=1)
                 off = off.masked_fill(hidden, 0.0).amax(1, keepdim=True)

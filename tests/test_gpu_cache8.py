@@ -125,8 +125,9 @@ def test_what_lies_behind_the_last_key_is_not_looked_at():
             kernels.attention_decode_cache8(q.cuda(), cache, out, table.cuda(), _ints(lengths), 0.125, plan, *scratch)
             _close(out, want, bound)
         out = torch.full_like(q, math.nan, device="cuda")
-        kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints([0, 1, 2, 3]), _ints([n - 1 for n in lengths]), 1, 0.125)
-        _close(out, want, bound)
+        for impl in ("tc", "mma") if dtype == BF16 else ("mma",):
+            kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints([0, 1, 2, 3]), _ints([n - 1 for n in lengths]), 1, 0.125, impl)
+            _close(out, *plain.attention(q, *_held(cache), table, [1] * 3, [n - 1 for n in lengths], 0.125, DIGITS[dtype], impl == "tc"))
 
 
 def test_a_nan_that_is_seen_is_handed_on():
@@ -142,19 +143,20 @@ def test_a_nan_that_is_seen_is_handed_on():
         assert bool(out[0].isnan().all()) and bool(out[1].isfinite().all())
 
 
-def _prompt(counts, past, heads, kv_heads, dim, dtype, seed=0, scale=None, spread=3):
+def _prompt(counts, past, heads, kv_heads, dim, dtype, seed=0, scale=None, spread=3, impl=None):
     from qwen_triton_b200.ops import kernels
     pages_of = [-(-(n + p) // PAGE) for n, p in zip(counts, past)]
     pages = sum(pages_of) + 1
     cache = _filled(pages, kv_heads, dim, seed, spread)
     table = _table(pages_of, pages, seed)
     q = torch.randn((sum(counts), heads, dim), generator=torch.Generator().manual_seed(seed + 1)).to(dtype)
-    out = torch.full_like(q, math.nan, device="cuda")
     scale = dim ** -0.5 if scale is None else scale
     starts = [sum(counts[:i]) for i in range(len(counts) + 1)]
-    kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints(starts), _ints(past), max(counts), scale)
-    want, bound = plain.attention(q, *_held(cache), table, counts, past, scale, DIGITS[dtype])
-    _close(out, want, bound)
+    want = {}
+    for form in (impl,) if impl else ("tc", "mma") if dtype == BF16 and dim in (64, 128) and scale > 0 else ("mma",):
+        out = torch.full_like(q, math.nan, device="cuda")
+        kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints(starts), _ints(past), max(counts), scale, form)
+        _close(out, *plain.attention(q, *_held(cache), table, counts, past, scale, DIGITS[dtype], form == "tc"))
     kernels.check_status()
 
 
@@ -181,6 +183,33 @@ def test_prompts_of_many_sequences():
 def test_prompt_with_scales_far_apart(heads, kv_heads, dim):
     _prompt([150, 70], [300, 0], heads, kv_heads, dim, BF16, spread=30, scale=1e-3)
     _prompt([150, 70], [300, 0], heads, kv_heads, dim, BF16, spread=4, scale=2.0)
+    _prompt([150, 70], [300, 0], heads, kv_heads, dim, BF16, scale=-0.1)
+    _prompt([150, 70], [300, 0], heads, kv_heads, dim, BF16, scale=0.0)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_queries_of_all_sizes(dim):
+    """Rows of zeros, of the smallest and the largest numbers, elements far below the row's largest; a row with an infinity is NaN, the others are as without it."""
+    from qwen_triton_b200.ops import kernels
+    counts, past = [90], [70]
+    cache, table = _filled(4, 1, dim, 3), torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    gen = torch.Generator().manual_seed(9)
+    q = torch.randn((90, 2, dim), generator=gen) * torch.exp2(torch.randint(-14, 1, (90, 2, dim), generator=gen).float())
+    q[3] = 0
+    q[5] *= 2.0 ** -100
+    q[7] *= 2.0 ** 10
+    q = q.to(BF16)
+    want = {impl: plain.attention(q, *_held(cache), table, counts, past, dim ** -0.5, DIGITS[BF16], impl == "tc") for impl in ("tc", "mma")}
+    q[11, 1, 5] = math.inf
+    for impl in ("tc", "mma"):
+        out = torch.full_like(q, math.nan, device="cuda")
+        kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints([0, 90]), _ints(past), 90, dim ** -0.5, impl)
+        assert bool(out[11, 1].isnan().all())
+        out[11, 1] = 0
+        for part in want[impl]:
+            part[11, 1] = 0
+        _close(out, *want[impl])
+    kernels.check_status()
 
 
 # ----------------------------------------------------------------------------- the write
@@ -348,7 +377,7 @@ def test_a_prompt_and_steps_behind_it(dtype):
         return rows
 
     def check(out, counts, q):
-        want, bound = plain.attention(q.cpu(), *_held(cache), table.cpu(), counts, past, dim ** -0.5, DIGITS[dtype])
+        want, bound = plain.attention(q.cpu(), *_held(cache), table.cpu(), counts, past, dim ** -0.5, DIGITS[dtype], dtype == BF16)
         _close(out, want, bound)
         # without 8 bits: a key's numbers are off by 2^-4 of themselves at most, a value's too
         at = 0
@@ -459,6 +488,11 @@ def test_refusals():
         prefill(q, cache, out, table, _ints([0, 1, 2]), _ints([0, 0]), 3, 0.1)
     with pytest.raises(Error, match="seq_start"):
         prefill(q, cache, out, table, _ints([0, 1]), _ints([0, 0]), 1, 0.1)
+    for impl, scale in (("other", 0.1), ("tc", -0.1)):
+        with pytest.raises(Error, match="impl"):
+            prefill(q, cache, out, table, _ints([0, 1, 2]), _ints([0, 0]), 1, scale, impl)
+    with pytest.raises(Error, match="impl"):
+        prefill(q.float(), cache, out.float(), table, _ints([0, 1, 2]), _ints([0, 0]), 1, 0.1, "tc")
     qkv = kernels.GemmOut(torch.zeros((1, 2, 512), dtype=BF16, device="cuda"))
     write = kernels.qkv_write_cache8
     write(qkv, q, cache, _ints([0, 1, 2]), _ints([0, 0]), table, 1, None, None, 0.0, None)
