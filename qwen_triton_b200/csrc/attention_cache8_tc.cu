@@ -11,11 +11,14 @@
 // A weight is p_j s_v[j] relative to the largest such, as in attention_cache8.cu: the maximum is that of the score plus log2 s_v, and the row's sum takes the scale out.
 //
 // A block takes 256 rows (query token, head of a kv head's group; a token's heads are neighbours) as two tiles of 128 and walks the keys page by page.  S of a
-// page is double buffered, P lies over the scores it came from, O stays in tensor memory and is scaled only where a row's maximum runs 2^8 ahead of the one it is
-// scaled by.  512 threads: warp 0 copies (TMA tiles of keys, bulk copies of values), warp 1 issues, warps 4 to 7 convert values, warps 8 to 11 and 12 to 15 are the
+// page is double buffered, P lies over the scores it came from, O stays in tensor memory and is scaled only where a row's maximum runs 2^14 ahead of the one it is
+// scaled by (halves end at 2^16; at 2^8, 2 % slower).  512 threads: warp 0 copies (TMA tiles of keys, bulk copies of values), warp 1 issues, warps 4 to 7 convert values, warps 8 to 11 and 12 to 15 are the
 // softmax of the two tiles, with most of the registers: 88 + 88 + 168 + 168 = 4 * 128.  Every mbarrier wait is bounded and reports through a status word.
 //
-// prompt of 4,096 tokens behind 8,192, 32 heads over 8 of 128: the figures stand in the table of the design document's section on 8-bit operators.
+// What bounds it: the products of scores with a page's 64 keys, whose time is their queries' way from shared memory (66 cycles for 128 x 64 x 32, of which the
+// tensor cores need 32), 1,650 cycles of the 1,900 that a page takes for 256 rows.  Two pages at a time would halve it, but tensor memory then holds one sum
+// per row and the two threads of a row walk in step: 739 us in the place of 712 for 4,096 tokens behind 8,192, 32 heads over 8 of 128 (965 TFLOP/s; the same over a
+// 16-bit cache, attention_tc.cu, 734).
 #include "cache8_call.h"
 #include "fp8.cuh"
 #include "tc_common.cuh"
@@ -32,7 +35,7 @@ constexpr int PAGE = 64;
 constexpr int BQ = 128, TILES = 2;                         // rows of a tile = the instruction's M; tiles of a block
 constexpr int THREADS = 512;
 constexpr int K_STAGES = 3, RAW_STAGES = 3, V_STAGES = 3;
-constexpr float RESCALE_STEP = 8.f, LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_STEP = 14.f, LOG2E = 1.4426950408889634f;
 
 struct TcParams {
     const __nv_bfloat16* q; __nv_bfloat16* out;
