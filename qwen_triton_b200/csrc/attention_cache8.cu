@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int seq = blockIdx.z, kvh = blockIdx.y % p.nkv, group = p.nq / p.nkv;
-    const int tile = p.seq_start ? blockIdx.x : blockIdx.y / p.nkv, range = JOIN == ALONE ? 0 : blockIdx.x;
+    const int tile = p.seq_start ? blockIdx.x / p.ranges : blockIdx.y / p.nkv, range = JOIN == ALONE ? 0 : p.seq_start ? blockIdx.x % p.ranges : blockIdx.x;
     uint8_t* ring = shared + warp * STAGES * R::STAGE;
     if (p.d < D) {                                         // what no copy reaches
         for (int i = lane; i < STAGES * R::STAGE / 16; i += 32) *reinterpret_cast<uint4*>(ring + 16 * i) = make_uint4(0, 0, 0, 0);
@@ -114,7 +114,10 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
     }
     pdl_wait();
     const int* table = p.block_table + (size_t)seq * p.max_blocks;
-    const int page_begin = range * p.range_pages, begin = page_begin * PER_PAGE + warp;
+    int range_pages = p.range_pages;
+    if (JOIN == CLUSTER && p.seq_start)                    // prompts: equal ranges of what the tile's last row sees
+        range_pages = max(1, (p.seq_past[seq] + (min((tile + 1) * ROWS, (p.seq_start[seq + 1] - p.seq_start[seq]) * group) - 1) / group + PAGE) / PAGE + p.ranges - 1) / p.ranges;
+    const int page_begin = range * range_pages, begin = page_begin * PER_PAGE + warp;
     // the first pages are asked for together with the lengths that say whether they are needed
     int first[STAGES];
 #pragma unroll
@@ -129,11 +132,11 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
         past = min(p.seq_len[seq], capacity) - 1;
     }
     const int row0 = tile * ROWS, rows = tokens * group;
-    if (row0 >= rows) return;                              // prompts only: the same for a whole cluster
+    if (row0 >= rows) return;                              // prompts only, and the same for a whole cluster
     const int last_row = min(row0 + ROWS, rows) - 1;
     const int end = min(past + last_row / group + 1, capacity);          // keys that any row sees
     const int pages = (end + PAGE - 1) / PAGE;
-    const int page_end = range == p.ranges - 1 ? pages : min(pages, page_begin + p.range_pages);        // the last range takes what is left
+    const int page_end = range == p.ranges - 1 ? pages : min(pages, page_begin + range_pages);        // the last range takes what is left
     if (JOIN == MEMORY && page_begin >= page_end && range > 0) return;   // the join knows from the length
 
     const int stop = (min(end, page_end * PAGE) + KEYS - 1) / KEYS;      // portions; the warp's are begin, begin + WARPS, ...
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
     }
     if (JOIN == CLUSTER) {
         cluster_barrier();
-        const int ranks = gridDim.x, live = last_row - row0 + 1;
+        const int ranks = p.ranges, live = last_row - row0 + 1;
         const uint32_t part0 = shared_address(block_part), sums0 = shared_address(block_sums);
         auto remote = [](uint32_t at, int rank) {
             uint32_t there;
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(GROUPS * JOIN_WIDTH) join_cache8_kernel(const 
 template <int D, int JOIN, typename T> int launch(const Params& p, dim3 grid, cudaStream_t stream) {
     const cudaError_t raised = raise_shared<attention_cache8_kernel<D, JOIN, T>>((int)Ring<D>::SMEM);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8: cannot raise shared memory: %s", cudaGetErrorString(raised));
-    if (JOIN == CLUSTER) launch_kernel_cluster(attention_cache8_kernel<D, JOIN, T>, grid, dim3(32 * WARPS), Ring<D>::SMEM, stream, grid.x, p);
+    if (JOIN == CLUSTER) launch_kernel_cluster(attention_cache8_kernel<D, JOIN, T>, grid, dim3(32 * WARPS), Ring<D>::SMEM, stream, (unsigned)p.ranges, p);
     else launch_kernel(attention_cache8_kernel<D, JOIN, T>, grid, dim3(32 * WARPS), Ring<D>::SMEM, stream, p);
     QT_CHECK_LAUNCH("attention_cache8");
     if (JOIN == MEMORY) {
@@ -505,7 +508,8 @@ extern "C" int qt_attention_decode_cache8(const Cache8Call* call) {
     return c.dtype == QT_F32 ? launch_size<float>(p, grid, (cudaStream_t)c.stream) : launch_size<__nv_bfloat16>(p, grid, (cudaStream_t)c.stream);
 }
 
-// Packed queries [n_tokens, nq, d] of sequences whose keys, this call's own among them, are in the cache; causal.
+// Packed queries [n_tokens, nq, d] of sequences whose keys, this call's own among them, are in the cache; causal.  A tile's keys are walked by a cluster of `ranges`
+// blocks.
 extern "C" int qt_attention_prefill_cache8(const Cache8Call* call) {
     const Cache8Call& c = *call;
     if (c.n_seqs == 0 || c.max_q_len == 0) return QT_OK;
@@ -514,8 +518,10 @@ extern "C" int qt_attention_prefill_cache8(const Cache8Call* call) {
     QT_REQUIRE(c.n_seqs > 0 && c.n_seqs <= 65535 && c.nkv <= 65535 && c.max_q_len > 0 && (long long)c.max_q_len * (c.nq / c.nkv) <= 0x7fffffff - ROWS,
                "attention_prefill_cache8: %d sequences of up to %d tokens", c.n_seqs, c.max_q_len);
     const Params p{c.q, c.out, (const uint8_t*)c.k, (const uint8_t*)c.v, c.k_scale, c.v_scale, c.block_table, c.max_blocks, c.n_pages, c.seq_start, c.seq_past, nullptr, c.nq, c.nkv, c.d,
-                   (float)c.scale, 1, 0x7fffffff / PAGE, 0, nullptr, nullptr};
-    const dim3 grid((unsigned)((c.max_q_len * (c.nq / c.nkv) + ROWS - 1) / ROWS), c.nkv, c.n_seqs);
+                   (float)c.scale, c.ranges, 0x7fffffff / PAGE, c.ranges > 1, nullptr, nullptr};
+    const long long blocks = (((long long)c.max_q_len * (c.nq / c.nkv) + ROWS - 1) / ROWS) * c.ranges;
+    QT_REQUIRE(c.ranges >= 1 && c.ranges <= MAX_CLUSTER && blocks <= 0x7fffffff, "attention_prefill_cache8: %d ranges", c.ranges);
+    const dim3 grid((unsigned)blocks, c.nkv, c.n_seqs);
     return c.dtype == QT_F32 ? launch_size<float>(p, grid, (cudaStream_t)c.stream) : launch_size<__nv_bfloat16>(p, grid, (cudaStream_t)c.stream);
 }
 

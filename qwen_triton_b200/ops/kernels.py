@@ -1979,11 +1979,12 @@ def _check_decode_cache8(q, cache, out, block_table, seq_len, plan, part_acc, pa
 
 
 def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_start: torch.Tensor, seq_past: torch.Tensor,
-                             max_q_len: int, scale: float, impl: str | None = None) -> None:
+                             max_q_len: int, scale: float, impl: str | None = None, ranges: int | None = None) -> None:
     """``attention_prefill`` over a cache in 8 bits: packed queries [T, nq, d], sequence i's from ``seq_start[i]`` on (at most ``max_q_len``), behind ``seq_past[i]`` earlier
     tokens; the cache already holds this step's keys; a query sees the keys up to its own.
 
-    ``impl``: "tc" (tcgen05: bfloat16 heads of 64 or 128 under a positive scale; the default for those and more than 64 rows a kv head) or "mma" (any call).  A value
+    ``impl``: "tc" (tcgen05: bfloat16 heads of 64 or 128 under a positive scale; the default for those, but for few rows) or "mma" (any call; a
+    tile of eight rows by a cluster of ``ranges`` blocks, up to eight).  A value
     that is not a number makes the results of the queries that see it NaN, and on "tc" and "mma" may make those of earlier queries of the call that read its
     page."""
     n_seqs, device, k = seq_past.shape[0], _current_device(), cache.k
@@ -1997,15 +1998,23 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     on_tc = q.dtype is torch.bfloat16 and k.shape[3] in (64, 128) and scale > 0
     if impl not in (None, "tc", "mma") or (impl == "tc" and not on_tc):
         raise KernelError(f"attention_prefill_cache8: impl={impl!r} for {q.dtype}, heads of {k.shape[3]}, a scale of {scale}")
-    if impl == "mma" or (impl is None and max_q_len * (q.shape[1] // k.shape[1]) <= _MMA_ROWS):
+    walks = -(-max_q_len * (q.shape[1] // k.shape[1]) // 8) * k.shape[1] * n_seqs         # tiles of eight rows
+    if impl == "mma" or (impl is None and walks <= _MMA_WALKS[k.shape[3] == 64]):
         on_tc = False
+    if ranges is None:
+        # as many blocks as are resident
+        ranges = 1 if on_tc else max(1, min(_CLUSTER_RANGES, 2 * 148 // max(1, walks)))
+    elif on_tc or not 1 <= ranges <= _CLUSTER_RANGES:
+        raise KernelError(f"attention_prefill_cache8: {ranges} ranges")
     _call(*(("attention_cache8_tc", "qt_attention_prefill_cache8_tc") if on_tc else ("attention_cache8", "qt_attention_prefill_cache8")),
           _CACHE8_CALL.pack(q.data_ptr(), k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(),
                             seq_start.data_ptr(), seq_past.data_ptr(), 0, 0, 0, _status_word(q.device).data_ptr(), _stream(), scale, _CODES[q.dtype], block_table.shape[1],
-                            k.shape[0], n_seqs, q.shape[0], max_q_len, q.shape[1], k.shape[1], k.shape[3], 1, 1, 0))
+                            k.shape[0], n_seqs, q.shape[0], max_q_len, q.shape[1], k.shape[1], k.shape[3], ranges, 1, 0))
 
 
-_MMA_ROWS = 64             # query rows a kv head (tokens times its group) up to which mma.sync, eight rows a block, takes prompts
+# Tiles of eight query rows (of heads of 128, and of 64) up to which mma.sync takes prompts: their blocks are many, where 256 rows a block would leave most SMs idle
+# (32 heads over 8 of 128 behind 8,000 tokens, mma.sync / tcgen05: 8 tokens 22 / 112 us, 64 108 / 144, 128 154 / 147; behind 500: 15 / 20, 24 / 22).
+_MMA_WALKS = (444, 1184)
 
 
 def _check_prefill_cache8(q, cache, out, block_table, seq_start, seq_past, max_q_len) -> None:

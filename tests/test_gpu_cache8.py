@@ -143,7 +143,7 @@ def test_a_nan_that_is_seen_is_handed_on():
         assert bool(out[0].isnan().all()) and bool(out[1].isfinite().all())
 
 
-def _prompt(counts, past, heads, kv_heads, dim, dtype, seed=0, scale=None, spread=3, impl=None):
+def _prompt(counts, past, heads, kv_heads, dim, dtype, seed=0, scale=None, spread=3, impl=None, ranges=None):
     from qwen_triton_b200.ops import kernels
     pages_of = [-(-(n + p) // PAGE) for n, p in zip(counts, past)]
     pages = sum(pages_of) + 1
@@ -155,7 +155,7 @@ def _prompt(counts, past, heads, kv_heads, dim, dtype, seed=0, scale=None, sprea
     want = {}
     for form in (impl,) if impl else ("tc", "mma") if dtype == BF16 and dim in (64, 128) and scale > 0 else ("mma",):
         out = torch.full_like(q, math.nan, device="cuda")
-        kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints(starts), _ints(past), max(counts), scale, form)
+        kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints(starts), _ints(past), max(counts), scale, form, ranges if form == "mma" else None)
         _close(out, *plain.attention(q, *_held(cache), table, counts, past, scale, DIGITS[dtype], form == "tc"))
     kernels.check_status()
 
@@ -177,6 +177,14 @@ def test_prompts_of_many_sequences():
     _prompt([1, 130, 0, 64, 257, 12, 300], [0, 5, 64, 0, 700, 129, 0], 8, 2, 128, BF16)
     _prompt([1, 130, 0, 64, 257, 12, 300], [0, 5, 64, 0, 700, 129, 0], 6, 2, 64, BF16)
     _prompt([1, 130, 0, 64], [0, 5, 64, 0], 6, 2, 64, F32)
+
+
+@pytest.mark.parametrize("ranges", [1, 2, 3, 7, 8])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_prompts_in_ranges(ranges, dtype):
+    """A tile's keys by clusters of every size, more blocks than pages among them, sequences without tokens."""
+    _prompt([3, 20, 0, 1, 70], [0, 700, 64, 5, 63], 8, 2, 128, dtype, impl="mma", ranges=ranges)
+    _prompt([3, 20, 0, 1, 70], [0, 700, 64, 5, 63], 3, 1, 48, dtype, impl="mma", ranges=ranges)
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 2, 64), (4, 2, 48)])
@@ -491,6 +499,9 @@ def test_refusals():
     for impl, scale in (("other", 0.1), ("tc", -0.1)):
         with pytest.raises(Error, match="impl"):
             prefill(q, cache, out, table, _ints([0, 1, 2]), _ints([0, 0]), 1, scale, impl)
+    for impl, ranges in (("mma", 9), ("mma", 0), ("tc", 2)):
+        with pytest.raises(Error, match="ranges"):
+            prefill(q, cache, out, table, _ints([0, 1, 2]), _ints([0, 0]), 1, 0.1, impl, ranges)
     with pytest.raises(Error, match="impl"):
         prefill(q.float(), cache, out.float(), table, _ints([0, 1, 2]), _ints([0, 0]), 1, 0.1, "tc")
     qkv = kernels.GemmOut(torch.zeros((1, 2, 512), dtype=BF16, device="cuda"))
