@@ -29,6 +29,7 @@ class CacheView:
     page_tokens: int = 0
     ring_tokens: int = 0              # 0: position p sits at element p; else at p % ring_tokens
     writable: bool = True             # False: this call reads an entry that another call writes
+    eight: kernels.Cache8 | None = None  # the same in 8 bits with its scales, where that is how it is kept
     state: torch.Tensor | None = None  # [num_slots + 1, *shape]; the last row belongs to no sequence (padded rows of a fixed-shape step)
 
 
@@ -39,6 +40,7 @@ class _Group:
     ring_tokens: int
     k: torch.Tensor | None = None
     v: torch.Tensor | None = None
+    eight: list[kernels.Cache8] | None = None     # of each entry
 
 
 def round_up(value: int, multiple: int) -> int:
@@ -103,6 +105,11 @@ class SequenceCache:
         if allocate:
             for group in self.groups:
                 request = group.request
+                if request.eight:
+                    if page_tokens != 64 or group.ring_tokens:
+                        raise CacheError("a cache in 8 bits keeps every key, in pages of 64 tokens")
+                    group.eight = [kernels.cache8(total_pages + 1, request.kv_heads, request.head_dim, device) for _ in group.owners]
+                    continue
                 shape = (len(group.owners), total_pages + 1, request.kv_heads, page_tokens)
                 group.k = torch.zeros((*shape, request.head_dim), dtype=dtype, device=device)
                 if request.shared_values:
@@ -135,6 +142,9 @@ class SequenceCache:
                 view.ring_tokens = group.ring_tokens
                 if group.k is not None:
                     view.k, view.v = group.k[entry], group.v[entry]
+                elif group.eight is not None:
+                    view.eight = group.eight[entry]
+                    view.k, view.v = view.eight.k, view.eight.v
             if key in self._state_of:
                 view.state = self._state_of[key]
             views.append(view)
@@ -169,6 +179,8 @@ class SequenceCache:
         for group in self.groups:
             if group.k is not None:
                 total += (group.k.numel() + (0 if group.request.shared_values else group.v.numel())) * group.k.element_size()
+            for entry in group.eight or ():
+                total += sum(t.numel() * t.element_size() for t in (entry.k, entry.v, entry.k_scale, entry.v_scale))
         for state in self._state_of.values():
             total += state.numel() * state.element_size()
         return total
@@ -176,6 +188,7 @@ class SequenceCache:
     def token_bytes(self) -> int:
         """Bytes of keys and values one cached token occupies over all full-attention entries."""
         size = torch.empty((), dtype=self.dtype).element_size()
+        # (an 8-bit cache's scales, two of 4 bytes for each page and head, are left out)
         return sum(len(g.owners) * (g.request.kv_heads * g.request.head_dim + (0 if g.request.shared_values else
-                                    (g.request.v_heads or g.request.kv_heads) * (g.request.v_head_dim or g.request.head_dim))) * size
+                                    (g.request.v_heads or g.request.kv_heads) * (g.request.v_head_dim or g.request.head_dim))) * (1 if g.request.eight else size)
                    for g in self.groups)

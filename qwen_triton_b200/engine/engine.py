@@ -52,6 +52,20 @@ def require_gpu(device: torch.device) -> None:
         raise RuntimeError(f"the kernels are built for sm_100a; device {device} is sm_{major}{minor}")
 
 
+def check_formats(spec: ModelSpec, weight_format: str | None, cache_format: str | None) -> dict[str, str]:
+    """What the parts are told of ``weight_format`` and ``cache_format``: None keeps the compute type, "fp8" the weights of attention's and the feed-forward's
+    projections as 8-bit numbers with a scale for each block of 128 x 128 (their rows are brought to 8 bits too), or keys and values with a scale for each
+    page and head.  Models of dense attention and gated feed-forwards take them; parts that do not say so themselves."""
+    formats = {name: given for name, given in (("weight_format", weight_format), ("cache_format", cache_format)) if given is not None}
+    for name, given in formats.items():
+        if given != "fp8":
+            raise ValueError(f"{name}={given!r} is neither None nor 'fp8'")
+        for layer in spec.layers:
+            if layer.block.kind != "pre_norm" or layer.mixer.kind != "attention" or layer.feed_forward is None or layer.feed_forward.kind != "gated_mlp":
+                raise ValueError(f"{name}='fp8' is for models of dense attention and gated feed-forwards; {layer.prefix} of {spec.architecture} is another layer")
+    return formats
+
+
 @dataclass
 class PlannedDecode:
     """A one-token step that has been prepared up to the tokens' values (``Engine.plan_decode``)."""
@@ -68,8 +82,9 @@ class PlannedDecode:
 class Engine:
     def __init__(self, spec: ModelSpec, source, *, dtype=torch.bfloat16, max_tokens: int = 8192,
                  max_seq_len: int | None = None, max_step_tokens: int = 4096, device: str | torch.device = "cuda:0",
-                 page_tokens: int = 64, chunk_tokens: int = 256, options: dict | None = None,
+                 page_tokens: int = 64, chunk_tokens: int = 256, options: dict | None = None, weight_format: str | None = None, cache_format: str | None = None,
                  cuda_graphs: bool = True, max_graph_batch: int = 256, max_graphs: int = 48) -> None:
+        formats = check_formats(spec, weight_format, cache_format)
         self.device = torch.device(device)
         require_gpu(self.device)
         torch.cuda.set_device(self.device)
@@ -82,7 +97,7 @@ class Engine:
         workspace = Workspace(self.device)
         self.runtime = Runtime(device=self.device, dtype=self.dtype, max_step_tokens=self.max_step_tokens,
                                max_positions=self.max_seq_len, workspace=workspace, page_tokens=page_tokens,
-                               options=dict(options or {}))
+                               options={**(options or {}), **formats})
         self.model = CausalLM(spec, self.runtime)
         self.model.load(source)
         self.cache = SequenceCache(self.model.cache_requests(), [c.cache_of for c in spec.schedule],

@@ -1898,9 +1898,11 @@ class Decode8Plan:
         return self.q_shape[0] * self.q_shape[1] * self.ranges * 2 if self.through_memory else 0
 
 
-def decode8_plan(batch: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, max_context: int, sms: int = 148) -> Decode8Plan:
-    """A plan for ``batch`` sequences of up to ``max_context`` keys (a longer one is right too, but slower)."""
-    if batch < 0 or num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or head_dim <= 0 or max_context < 0 or dtype not in _CODES:
+@functools.lru_cache(maxsize=1024)
+def decode8_plan(batch: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, max_context: int, sms: int = 148,
+                 most_ranges: int = 64) -> Decode8Plan:
+    """A plan for ``batch`` sequences of up to ``max_context`` keys (a longer one is right too, but slower) with at most ``most_ranges`` ranges."""
+    if batch < 0 or num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or head_dim <= 0 or max_context < 0 or dtype not in _CODES or most_ranges < 1:
         raise KernelError(f"decode8_plan: {batch} sequences of {num_heads} heads over {num_kv_heads} of {head_dim}, {dtype}, {max_context} keys")
     pages = max(1, -(-max_context // 64))
     walks = max(1, batch * num_kv_heads * -(-(num_heads // num_kv_heads) // 8))
@@ -1909,10 +1911,10 @@ def decode8_plan(batch: int, *, num_heads: int, num_kv_heads: int, head_dim: int
     clusters = True
     if walks >= 128 and pages >= 48:
         # many sequences, seldom of one length: equal portions, so that the longest does not keep a cluster's other blocks (48 of 3,000 to 12,000: 130 us, uncut 153)
-        ranges, clusters = min(_MOST_RANGES, -(-pages // 16)), False
+        ranges, clusters = min(_MOST_RANGES, most_ranges, -(-pages // 16)), False
     else:
         # as many blocks as are resident; at least two pages each, and eight where so many ranges join through memory
-        ranges = max(1, min(slots // walks, -(-pages // 2) if pages > 4 else 1, max(_CLUSTER_RANGES, pages // 8), _MOST_RANGES))
+        ranges = max(1, min(slots // walks, -(-pages // 2) if pages > 4 else 1, max(_CLUSTER_RANGES, pages // 8), _MOST_RANGES, most_ranges))
     range_pages = -(-pages // ranges)
     return Decode8Plan((batch, num_heads, head_dim), num_kv_heads, dtype, -(-pages // range_pages), range_pages, clusters)
 

@@ -142,6 +142,14 @@ class Attention:
         # the mma.sync attention kernels take values as wide as the keys (and compute the distance penalty, given a
         # positive scale); everything else goes to the generic kernels
         self.mma_scores = self.dv == self.d and (not self.penalised or self.scale > 0)
+        # keys and values in 8 bits with a scale for each page and head; the projections' weights in 8 bits
+        self.eight = runtime.options.get("cache_format") == "fp8"
+        eight_weights = runtime.options.get("weight_format") == "fp8"
+        if self.eight and (self.treated or self.own_values or self.window or self.penalised or self.chunk or self.keep_first or self.sink or self.softcap is not None
+                           or not self.own_kv or self.d % 16 or runtime.page_tokens != 64):
+            raise ValueError(f"{prefix}: a cache in 8 bits goes with full attention over keys of the layer's own, heads in steps of 16 and pages of 64 tokens")
+        if eight_weights and (self.own_values or self.treated):
+            raise ValueError(f"{prefix}: weights in 8 bits go with attention whose values are as the projection leaves them")
         proj_rows = self.nq * self.d + ((self.nkv * self.d + self.v_heads * self.dv) if self.own_kv else 0) + self.gate_cols
         self.at_gate = proj_rows - self.gate_cols
         if self.own_values:
@@ -150,10 +158,10 @@ class Attention:
         elif self.treated:
             self.qkv = Linear("attn.qkv.sums", proj_rows, self.hidden, runtime, float_out=True)      # float sums: the bias is added behind it
         else:
-            self.qkv = Linear("attn.qkv" + (".biased" if self.bias else ""), proj_rows, self.hidden, runtime, role="qkv", bias=self.bias)
+            self.qkv = Linear("attn.qkv" + (".biased" if self.bias else ""), proj_rows, self.hidden, runtime, role="qkv", bias=self.bias, eight=eight_weights)
         self.float_out = bool(params.get("float_out", False))
         self.o = Linear("attn.o" + (".biased" if self.o_bias else "") + (".float" if self.float_out else ""), self.hidden,
-                        self.heads_out * self.dv, runtime, role="attn_out", bias=self.o_bias, float_out=self.float_out)
+                        self.heads_out * self.dv, runtime, role="attn_out", bias=self.o_bias, float_out=self.float_out, eight=eight_weights)
         ws = runtime.workspace
         ws.declare("attn.q", runtime.max_step_tokens * self.nq * self.d, runtime.dtype)
         ws.declare("attn.ctx", runtime.max_step_tokens * self.nq * self.dv, runtime.dtype)
@@ -168,7 +176,7 @@ class Attention:
             ws.declare(self.side_name, runtime.max_step_tokens * self.nkv * self.dv, torch.float32)
         # whether a one-token step may read what sequences share once; the engine asks about every kind that does
         self.takes_shared = not (self.window or self.penalised or self.chunk or self.keep_first or self.sink or self.softcap is not None or self.dv != self.d
-                                 or self.v_heads != self.nkv or self.scale <= 0)
+                                 or self.v_heads != self.nkv or self.scale <= 0 or self.eight)
         if self.takes_shared:
             runtime.options.setdefault("shared_attention", set()).add((self.nq, self.nkv, self.d))
         # few tokens: the projection takes rows whose norm factor is still to be applied (``ScaledRows``)
@@ -275,11 +283,13 @@ class Attention:
         if key not in tables:
             tables[key] = self.position.table(self.runtime.max_positions)
         self.cos_sin = tables[key]
+        if self.eight and self.cos_sin is not None and not self.interleaved and self.cos_sin.shape[1] % 16:
+            raise ValueError(f"{self.prefix}: the write into a cache in 8 bits rotates multiples of 16 elements of a head, not {self.cos_sin.shape[1]}")
 
     # ------------------------------------------------------------------ cache
     def cache_request(self) -> KVRequest | None:
         return KVRequest(self.nkv, self.d, None if self.keep_first else self.window, self.dv if self.dv != self.d else None,
-                         self.v_heads if self.v_heads != self.nkv else None)
+                         self.v_heads if self.v_heads != self.nkv else None, eight=self.eight)
 
     # ------------------------------------------------------------------ run
     def _splits(self, ctx, cache) -> tuple[int, int]:
@@ -363,6 +373,8 @@ class Attention:
         write = cache.writable and self.own_kv
         rotary_dim = 0 if self.cos_sin is None else self.cos_sin.shape[1]
         penalty = (self.r1, self.r2) if self.penalised else None
+        if self.eight:
+            return self._forward_eight(x, q, out, table, ctx, cache.eight)
         if self.treated:
             side = ws.view(self.side_name, tokens, self.nkv, self.dv) if self.v_blend is not None else None
             kernels.qkv_treat_write(self.qkv(x), self.qkv_bias, q, cache.k if write else None, cache.v if write else None,
@@ -410,4 +422,20 @@ class Attention:
             kernels.map_difference(out, heads, self.lam, self.head_norm_eps, 1.0 - self.diff)
             out = heads
         out = out.view(tokens, self.heads_out * self.dv)
+        return DeferredProduct(self.o, out) if self.o.fusable(tokens) else self.o(out)
+
+    def _forward_eight(self, x, q, out, table, ctx, cache):
+        """The same over a cache in 8 bits."""
+        tokens = x.shape[0]
+        kernels.qkv_write_cache8(self.qkv(x), q, cache, ctx.seq_start, ctx.seq_past, table, ctx.max_q_len, self.q_weight, self.k_weight, self.eps, self.cos_sin,
+                                 interleaved=self.interleaved)
+        if ctx.is_decode:
+            ws = self.runtime.workspace
+            plan = kernels.decode8_plan(ctx.n_seqs, num_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.d, dtype=self.runtime.dtype, max_context=ctx.max_context,
+                                        sms=self.runtime.sm_count, most_ranges=max(1, _MAX_SPLIT_PAIRS // ctx.n_seqs))
+            kernels.attention_decode_cache8(q, cache, out, table, ctx.seq_len, self.scale, plan, ws.view("attn.part_acc", _MAX_SPLIT_PAIRS * self.nq * self.d),
+                                            ws.view("attn.part_ml", _MAX_SPLIT_PAIRS * self.nq * 2))
+        else:
+            kernels.attention_prefill_cache8(q, cache, out, table, ctx.seq_start, ctx.seq_past, ctx.max_q_len, self.scale)
+        out = out.view(tokens, self.heads_out * self.d)
         return DeferredProduct(self.o, out) if self.o.fusable(tokens) else self.o(out)

@@ -76,7 +76,8 @@ class KVRequest:
     """Keys and values per token: all of them (``window`` None) or the last ``window``.  Values have the keys' head
     size unless ``v_head_dim`` gives their own, and as many heads as the keys unless ``v_heads`` says otherwise
     (several key heads, one per score map, over one set of values).  With ``shared_values`` nothing is stored for
-    the values: they are the cached keys, or the leading elements of them, and the view's ``v`` is its ``k``."""
+    the values: they are the cached keys, or the leading elements of them, and the view's ``v`` is its ``k``.  ``eight``: both
+    are kept as 8-bit numbers with a scale for each page and head (``kernels.Cache8``, the view's ``eight``)."""
 
     kv_heads: int
     head_dim: int
@@ -84,6 +85,7 @@ class KVRequest:
     v_head_dim: int | None = None
     v_heads: int | None = None
     shared_values: bool = False
+    eight: bool = False
 
 
 @dataclass(frozen=True)

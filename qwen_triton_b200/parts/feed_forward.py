@@ -43,10 +43,11 @@ class GatedMLP:
         self.group = kernels.SWIGLU_GROUP if fused else 0
         float_out = bool(params.get("float_out", False))
         key = str(params.get("buffers", "mlp"))           # several such parts in one layer keep their buffers apart
-        self.gate_up = Linear(f"{key}.gate_up", 2 * self.inter, self.hidden, runtime, role="gate" if fused else "")
+        eight = runtime.options.get("weight_format") == "fp8"
+        self.gate_up = Linear(f"{key}.gate_up", 2 * self.inter, self.hidden, runtime, role="gate" if fused else "", eight=eight)
         self.biased = bool(params.get("bias", False))
         self.down = Linear(f"{key}.down" + (".float" if float_out or self.biased else ""), self.hidden, self.inter, runtime,
-                           role="mlp_out", float_out=float_out, bias=self.biased)
+                           role="mlp_out", float_out=float_out, bias=self.biased, eight=eight)
         self.gate_bias: torch.Tensor | None = None        # gate's and up's, in the layout of the fused weight's rows
         self.act_buffer = f"{key}.act"
         runtime.workspace.declare(self.act_buffer, runtime.max_step_tokens * self.inter, runtime.dtype)
@@ -88,6 +89,8 @@ class GatedMLP:
         act = self.runtime.workspace.view(self.act_buffer, tokens, self.inter)
         if self.takes_scaled_rows and self.gate_up.fusable(tokens):
             self.gate_up.into_swiglu(x, act, self.activation, self.limit, self.gate_bias)
+        elif self.gate_up.eight:
+            kernels.swiglu(self.gate_up(x), act, self.group, self.activation, self.limit, self.gate_bias)
         elif self.group and kernels.gemm_uses_pairs(x, self.gate_up.weight):
             kernels.gemm_tc_pair(x, self.gate_up.weight, GemmOut(act.view(1, tokens, self.inter)), swiglu=True, activation=self.activation,
                                  limit=self.limit, bias=self.gate_bias)

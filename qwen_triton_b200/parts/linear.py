@@ -103,7 +103,12 @@ def pick_pair_splits(out_features: int, in_features: int, rows: int, pairs: int)
 
 class Linear:
     def __init__(self, key: str, out_features: int, in_features: int, runtime: Runtime, max_rows: int | None = None,
-                 float_out: bool = False, role: str = "", bias: bool = False) -> None:
+                 float_out: bool = False, role: str = "", bias: bool = False, eight: bool = False) -> None:
+        # eight: the weight is kept as 8-bit numbers with a scale for each block of 128 x 128, and the rows of a product are brought to 8 bits
+        # (``kernels.gemm_fp8``); such a product is one finished plane and has no fused form
+        self.eight = eight
+        self.weight8: kernels.Fp8Weight | None = None
+        self._rows8: dict[int, kernels.Fp8Rows] = {}
         self.key = key
         self.role = role                   # which of the fused products of a decode step this one is, if any
         self.out_features = out_features
@@ -124,7 +129,10 @@ class Linear:
         pairs = max(1, sms // 2)               # pairs of blocks the pair kernel keeps resident (one per TPC)
         self.split_plans: list[tuple[int, int]] = []          # (most rows, splits), fewest rows first
         self.fused_plans: list[tuple[int, int]] = []          # the same for the fused product (its blocks add up in shared memory)
-        if runtime.dtype == torch.bfloat16 and in_features % 8 == 0:
+        if eight:
+            runtime.workspace.declare("fp8.values", self.max_rows * in_features, kernels.E4M3)
+            runtime.workspace.declare("fp8.scales", self.max_rows * -(-in_features // kernels.FP8_GROUP), torch.float32)
+        elif runtime.dtype == torch.bfloat16 and in_features % 8 == 0:
             self.split_plans = [(rows, pick_splits(out_features, in_features, per_sm * sms, rows, sms=sms)) for rows, per_sm in _SPLIT_PLANS]
             self.fused_plans = [(rows, pick_splits(out_features, in_features, (3 if role == "gate" else per_sm) * sms, rows,
                                                    kernels.FUSED_MAX_SPLITS, 1.0, sms=sms))
@@ -146,7 +154,11 @@ class Linear:
     def set_weight(self, weight: torch.Tensor) -> None:
         if tuple(weight.shape) != (self.out_features, self.in_features):
             raise ValueError(f"{self.key}: weight {tuple(weight.shape)} is not [{self.out_features}, {self.in_features}]")
-        self.weight = weight.to(device=self.runtime.device, dtype=self.runtime.dtype).contiguous()
+        weight = weight.to(device=self.runtime.device, dtype=self.runtime.dtype).contiguous()
+        if self.eight:
+            self.weight8 = kernels.quantise_weight_fp8(weight)
+        else:
+            self.weight = weight
 
     def set_bias(self, bias: torch.Tensor) -> None:
         if not self.has_bias or tuple(bias.shape) != (self.out_features,):
@@ -239,8 +251,26 @@ class Linear:
         """The number of K ranges that ``rows`` tokens are cut into by the plain products."""
         return next((n for most, n in self.split_plans if rows <= most), 1)
 
+    def _product8(self, x: torch.Tensor, out: torch.Tensor | None) -> GemmOut:
+        rows = x.shape[0]
+        ws = self.runtime.workspace
+        if out is None:
+            out = ws.view(f"{self.key}.out", rows, self.out_features)
+        scratch = self._rows8.get(rows)
+        if scratch is None:
+            if len(self._rows8) >= 64:
+                self._rows8.clear()
+            scratch = self._rows8[rows] = kernels.Fp8Rows(ws.view("fp8.values", rows, self.in_features),
+                                                          ws.view("fp8.scales", -(-self.in_features // kernels.FP8_GROUP), rows))
+        kernels.gemm_fp8(x, self.weight8, out.view(rows, self.out_features), scratch)
+        if self.has_bias:
+            kernels.add_bias(out.view(rows, self.out_features), self._loaded_bias())
+        return GemmOut(out.view(1, rows, self.out_features))
+
     def __call__(self, x, out: torch.Tensor | None = None) -> GemmOut:
         rows = x.shape[0]
+        if self.eight:
+            return self._product8(x, out)
         if isinstance(x, ScaledRows):
             # rows whose norm factor is still to be applied: the fused product's plain store applies it
             if out is None:

@@ -11,7 +11,8 @@ Added: a model without a folder (``--preset NAME --random-weights``), prompts as
 (``--prompt-ids 1,2,3``, repeatable: a batch of unequal prompts) or random (``--random-prompts 5,9,17``),
 ``--temperature`` (0, or 1 with ``--samples``), ``--seed`` (the seed of everything the run draws: sampling, random weights, random
 prompts; ``--sampling-seed`` and ``--weights-seed`` set one of them apart), ``--stop-ids``,
-``--ignore-eos``, ``--min-p``, ``--samples`` (continuations of every prompt, ranked), ``--max-tokens`` (cache size), ``--max-seq-len``, ``--max-batch-size``.
+``--ignore-eos``, ``--min-p``, ``--samples`` (continuations of every prompt, ranked), ``--weight-format`` and ``--cache-format``
+(8 bits; ``--compare-ref`` compares with the model without them), ``--max-tokens`` (cache size), ``--max-seq-len``, ``--max-batch-size``.
 """
 from __future__ import annotations
 
@@ -45,6 +46,8 @@ def _parse_args(argv=None) -> argparse.Namespace:
     parser.add_argument("--max-tokens", type=int, default=8192, help="cache size in tokens")
     parser.add_argument("--max-seq-len", type=int, default=None, help="longest sequence (prompt and new tokens) the cache holds")
     parser.add_argument("--max-batch-size", type=int, default=None, help="most requests that run as one batch")
+    parser.add_argument("--weight-format", default=None, choices=["fp8"], help="keep the layers' matrices in 8 bits with a scale for each block of 128 x 128")
+    parser.add_argument("--cache-format", default=None, choices=["fp8"], help="keep keys and values in 8 bits with a scale for each page and head")
     parser.add_argument("--compare-ref", action="store_true")
     parser.add_argument("--strict-triton", action="store_true")
     args = parser.parse_args(argv)
@@ -79,11 +82,12 @@ def main(argv=None) -> None:
     options = {"max_tokens": args.max_tokens}
     if args.max_seq_len is not None:
         options["max_seq_len"] = args.max_seq_len
+    formats = {"weight_format": args.weight_format, "cache_format": args.cache_format}
     weights_seed = args.seed if args.weights_seed is None else args.weights_seed
     sampling_seed = args.seed if args.sampling_seed is None else args.sampling_seed
     temperature = args.temperature if args.temperature is not None else 1.0 if args.samples > 1 else 0.0    # several of the likeliest would be one
 
-    def build(dtype: str):
+    def build(dtype: str, **options):
         """The model in ``dtype``; with random weights, always the values a bfloat16 folder of --dtype would hold."""
         if args.random_weights:
             return QwenB200ForCausalLM.from_config(load_preset(args.preset), seed=weights_seed, device=args.device,
@@ -91,7 +95,7 @@ def main(argv=None) -> None:
         return QwenB200ForCausalLM.from_pretrained_hf(args.model_id, backend=args.backend, device=args.device,
                                                       dtype=dtype, **options)
 
-    model = build(args.dtype)
+    model = build(args.dtype, **options, **formats)
     vocab = model.engine.vocab_size
     tokenizer = None
     if args.prompt_ids:
@@ -130,7 +134,7 @@ def main(argv=None) -> None:
         kept = outputs.logits.float().cpu()
         del model, outputs
         torch.cuda.empty_cache()
-        ref_logits = build("fp32").forward(prompts[0], logits_to_keep=1).logits.float().cpu()
+        ref_logits = build("fp32", **options).forward(prompts[0], logits_to_keep=1).logits.float().cpu()
         diff = (kept - ref_logits).abs()
         print(f"logit_max_abs_diff={float(diff.max()):.6f}")
         print(f"logit_mean_abs_diff={float(diff.mean()):.6f}")
