@@ -139,6 +139,27 @@ def test_rows_in_8_bits(m, k, dtype):
     assert torch.equal(rows.values.double().cpu(), values)
 
 
+@pytest.mark.parametrize("power", [-110, -90, -60, -59, -20, 0, 59, 60, 100, 119])
+def test_quotients_next_to_borders(power):
+    """Rows whose quotients lie on, just above and just below the borders of 8-bit numbers, at scales of every size: the division is float32's."""
+    from qwen_triton_b200.ops import kernels
+    g = torch.Generator().manual_seed(power)
+    most = (torch.rand(600, generator=g) + 1) * 2.0 ** power                 # each group's largest number, and its scale
+    scale = (most * plain.PER_TOP).clamp(min=2.0 ** -100)
+    every = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    border = (every[1:] + every[:-1]) / 2
+    pick = border[torch.randint(0, len(border), (600, 127), generator=g)]
+    x = (pick * scale[:, None].double()).float()
+    x = (x.view(torch.int32) + torch.randint(-2, 3, x.shape, generator=g, dtype=torch.int32)).clamp(min=0).view(torch.float32).clamp(max=most[:, None])
+    x = torch.cat((most[:, None], torch.where(torch.rand(x.shape, generator=g) < 0.5, -x, x)), 1)
+    x[:, 5], x[:, 6] = 0.0, -0.0
+    rows = kernels.fp8_rows(600, 128, "cuda")
+    kernels.quantise_rows_fp8(x.cuda(), rows)
+    want = x / rows.scales.cpu().T
+    assert torch.equal(rows.scales.cpu()[0], scale)
+    assert torch.equal(rows.values.cpu().view(torch.uint8), want.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8))
+
+
 @pytest.mark.parametrize("n,k", [(128, 128), (1, 1), (130, 257), (384, 1024)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_a_weight_in_8_bits(n, k, dtype):
