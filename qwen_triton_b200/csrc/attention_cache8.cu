@@ -16,6 +16,7 @@
 #include "cache8_call.h"
 #include "fp8.cuh"
 
+#include <algorithm>
 #include <math.h>
 
 using namespace qt;
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
     int range_pages = p.range_pages;
     if (JOIN == CLUSTER && p.seq_start)                    // prompts: equal ranges of what the tile's last row sees
         range_pages = max(1, (p.seq_past[seq] + (min((tile + 1) * ROWS, (p.seq_start[seq + 1] - p.seq_start[seq]) * group) - 1) / group + PAGE) / PAGE + p.ranges - 1) / p.ranges;
-    const int page_begin = range * range_pages, begin = page_begin * PER_PAGE + warp;
+    const int page_begin = (int)min((long long)range * range_pages, (long long)p.max_blocks), begin = page_begin * PER_PAGE + warp;
     // the first pages are asked for together with the lengths that say whether they are needed
     int first[STAGES];
 #pragma unroll
@@ -503,7 +504,7 @@ extern "C" int qt_attention_decode_cache8(const Cache8Call* call) {
     QT_REQUIRE(c.ranges >= 1 && c.ranges <= MAX_RANGES && c.range_pages >= 1 && (c.ranges == 1 || clusters || (c.part_acc && c.part_ml && (uintptr_t)c.part_ml % 8 == 0)),
                "attention_decode_cache8: %d ranges of %d pages", c.ranges, c.range_pages);
     const Params p{c.q, c.out, (const uint8_t*)c.k, (const uint8_t*)c.v, c.k_scale, c.v_scale, c.block_table, c.max_blocks, c.n_pages, nullptr, nullptr, c.seq_len, c.nq, c.nkv, c.d,
-                   (float)c.scale, c.ranges, c.range_pages, clusters, c.part_acc, c.part_ml};
+                   (float)c.scale, c.ranges, std::min(c.range_pages, c.max_blocks), clusters, c.part_acc, c.part_ml};
     const dim3 grid(c.ranges, c.nkv * tiles, c.n_seqs);
     return c.dtype == QT_F32 ? launch_size<float>(p, grid, (cudaStream_t)c.stream) : launch_size<__nv_bfloat16>(p, grid, (cudaStream_t)c.stream);
 }
@@ -518,7 +519,7 @@ extern "C" int qt_attention_prefill_cache8(const Cache8Call* call) {
     QT_REQUIRE(c.n_seqs > 0 && c.n_seqs <= 65535 && c.nkv <= 65535 && c.max_q_len > 0 && (long long)c.max_q_len * (c.nq / c.nkv) <= 0x7fffffff - ROWS,
                "attention_prefill_cache8: %d sequences of up to %d tokens", c.n_seqs, c.max_q_len);
     const Params p{c.q, c.out, (const uint8_t*)c.k, (const uint8_t*)c.v, c.k_scale, c.v_scale, c.block_table, c.max_blocks, c.n_pages, c.seq_start, c.seq_past, nullptr, c.nq, c.nkv, c.d,
-                   (float)c.scale, c.ranges, 0x7fffffff / PAGE, c.ranges > 1, nullptr, nullptr};
+                   (float)c.scale, c.ranges, c.max_blocks, c.ranges > 1, nullptr, nullptr};
     const long long blocks = (((long long)c.max_q_len * (c.nq / c.nkv) + ROWS - 1) / ROWS) * c.ranges;
     QT_REQUIRE(c.ranges >= 1 && c.ranges <= MAX_CLUSTER && blocks <= 0x7fffffff, "attention_prefill_cache8: %d ranges", c.ranges);
     const dim3 grid((unsigned)blocks, c.nkv, c.n_seqs);

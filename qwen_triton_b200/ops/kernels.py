@@ -1946,7 +1946,7 @@ def attention_decode_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, b
     # one expression for a call that is in order: the host's part of a short step is its time
     if not (q.shape == shape == out.shape and q.dtype is plan.dtype is out.dtype and k.shape[1] == plan.num_kv_heads and k.shape[3] == shape[2] and shape[1] % k.shape[1] == 0
             and block_table.dim() == 2 and block_table.shape[0] == shape[0] and block_table.shape[1] > 0 and seq_len.shape == shape[:1]
-            and block_table.dtype is seq_len.dtype is torch.int32 and 1 <= plan.ranges <= _MOST_RANGES and plan.range_pages >= 1
+            and block_table.dtype is seq_len.dtype is torch.int32 and 1 <= plan.ranges <= _MOST_RANGES and 1 <= plan.range_pages < 1 << 31
             and q.is_contiguous() and out.is_contiguous() and block_table.is_contiguous() and seq_len.is_contiguous()
             and q.get_device() == out.get_device() == k.get_device() == block_table.get_device() == seq_len.get_device() == device
             and (not through_memory or (part_acc is not None and part_ml is not None and part_acc.dtype is part_ml.dtype is torch.float32 and part_acc.is_contiguous()
@@ -1966,7 +1966,7 @@ def _check_decode_cache8(q, cache, out, block_table, seq_len, plan, part_acc, pa
     _need(seq_len, "seq_len", torch.int32, q.shape[:1])
     if tuple(q.shape) != tuple(plan.q_shape) or q.dtype != plan.dtype or cache.kv_heads != plan.num_kv_heads:
         raise KernelError(f"attention_decode_cache8: a plan for {plan.q_shape} over {plan.num_kv_heads} kv heads, {plan.dtype}; queries {tuple(q.shape)} over {cache.kv_heads}, {q.dtype}")
-    if not 1 <= plan.ranges <= _MOST_RANGES or plan.range_pages < 1:
+    if not (1 <= plan.ranges <= _MOST_RANGES and 1 <= plan.range_pages < 1 << 31):
         raise KernelError(f"attention_decode_cache8: {plan.ranges} ranges of {plan.range_pages} pages")
     if plan.through_memory:
         for name, part, need in (("part_acc", part_acc, plan.acc_elements), ("part_ml", part_ml, plan.ml_elements)):
@@ -1987,8 +1987,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
 
     ``impl``: "tc" (tcgen05: bfloat16 heads of 64 or 128 under a positive scale; the default for those, but for few rows) or "mma" (any call; a
     tile of eight rows by a cluster of ``ranges`` blocks, up to eight).  A value
-    that is not a number makes the results of the queries that see it NaN, and on "tc" and "mma" may make those of earlier queries of the call that read its
-    page."""
+    that is not a number makes the results of the queries that see it NaN, and may make those of earlier queries of the call that read its page."""
     n_seqs, device, k = seq_past.shape[0], _current_device(), cache.k
     # one expression for a call that is in order
     if not (q.dim() == 3 and q.shape == out.shape and q.dtype is out.dtype and q.dtype in _CODES and q.shape[2] == k.shape[3] and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0

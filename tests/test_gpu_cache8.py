@@ -130,6 +130,12 @@ def test_what_lies_behind_the_last_key_is_not_looked_at():
             _close(out, *plain.attention(q, *_held(cache), table, [1] * 3, [n - 1 for n in lengths], 0.125, DIGITS[dtype], impl == "tc"))
 
 
+@pytest.mark.parametrize("ranges", [(2, 10 ** 9), (8, 2 ** 31 - 1), (3, 2 ** 30, False), (64, 2 ** 31 - 1, False)])
+def test_ranges_of_more_pages_than_there_are(ranges):
+    """The first range has every key, whatever its size in pages times ranges comes to."""
+    _decode([70, 200, 1], 4, 2, 64, BF16, 3, ranges)
+
+
 def test_a_nan_that_is_seen_is_handed_on():
     from qwen_triton_b200.ops import kernels
     cache = _filled(3, 1, 64, 12)
@@ -477,6 +483,8 @@ def test_refusals():
         decode(q, cache, out, table, lens, 0.1, plan, acc, ml[:-1])
     with pytest.raises(Error, match="65 ranges"):
         decode(q, cache, out, table, lens, 0.1, kernels.Decode8Plan((2, 4, 64), 2, BF16, 65, 1), acc, ml)
+    with pytest.raises(Error, match="9 ranges of"):
+        decode(q, cache, out, table, lens, 0.1, kernels.Decode8Plan((2, 4, 64), 2, BF16, 9, 2 ** 31), acc, ml)
     with pytest.raises(Error, match="plan"):
         decode(q[:1], cache, out[:1], table[:1], lens[:1], 0.1, plan, acc, ml)
     with pytest.raises(Error, match="out must"):
