@@ -199,6 +199,19 @@ __device__ __forceinline__ void umma_fp8(uint32_t tmem_d, uint64_t a_desc, uint6
 __device__ __forceinline__ void commit_one(uint32_t bar, uint32_t one) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one) : "memory");
 }
+// mbar_wait without a call: where warps have different numbers of registers, ptxas finds none for a function that all of them call.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int* status, int code) {
+    unsigned long long since = 0;
+#pragma unroll 1
+    for (uint32_t spins = 1; !mbar_try_wait(bar, parity); ++spins)
+        if ((spins & 0x3ffu) == 0) {
+            if (*(volatile int*)status != 0) return false;
+            const unsigned long long now = global_timer();
+            if (since == 0) since = now;
+            else if (now - since > WAIT_LIMIT_NS) { atomicCAS(status, 0, code); return false; }
+        }
+    return true;
+}
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code)); }
 __device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int c_inner, int c_outer) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c_inner), "r"(c_outer) : "memory");
@@ -240,6 +253,7 @@ struct GemmParams {
     const float* x_scale; const float* w_scale; void* out;
     int rows, n, k, groups;
     int groups_per_split;
+    int first_tile, end_tile;                               // many rows: the tiles of this launch
     int wide;                                               // rows of the output begin at boundaries of 32 bytes (2) or of four numbers (1)
     int* status;
 };
@@ -481,12 +495,16 @@ __global__ void __launch_bounds__(Few<BX, XT>::THREADS) gemm_fp8_few_kernel(cons
 }
 
 // Many rows.  128 rows of x are the instruction's M, 256 weight rows its N; eight warps add up, a row of x and 128 weight rows (of one scale block) a thread.  One
-// block an SM walks tiles.  320 threads: warp 0 copies, warp 1 issues, warps 2 to 9 add up and store.  SPLIT: a cluster a tile, whose blocks take a range of K each and
+// block an SM walks tiles.  384 threads: warp 0 copies, warp 1 issues, warps 4 to 11 add up and store, with most of the registers: 56 + 224 + 224 = 3 * 168 (without
+// the exchange ten warps have 168 each, of which the sums spill some: 24576 features of 4096 x 4096 450 us in the place of 417).  SPLIT: a cluster a tile, whose blocks take a range of K each and
 // add their sums through distributed shared memory, as for few rows.
 constexpr int BN = 256, PARK_ROW = BN + 4;                  // floats from a row of parked sums to the next: 16 bytes of eight neighbouring rows are all the banks
-constexpr int MANY_THREADS = 320, MANY_STAGES = 4, MANY_SLOTS = 512 / BN, MANY_CW = BN / 2;
+constexpr int MANY_THREADS = 384, MANY_STAGES = 4, MANY_SLOTS = 512 / BN, MANY_CW = BN / 2;
 constexpr uint32_t MANY_STAGE_BYTES = A_BYTES + BN * GROUP;
-constexpr size_t MANY_SMEM = (size_t)MANY_STAGES * MANY_STAGE_BYTES + 8 * (2 * MANY_STAGES + 2 * MANY_SLOTS) + 16 + 1024;
+constexpr uint32_t MANY_TURN = MANY_STAGES * MANY_STAGE_BYTES + 8 * (2 * MANY_STAGES + 2 * MANY_SLOTS) + 16;         // 32 rows of 32 columns of each of the eight warps
+constexpr int TURN_ROW = 33, TURN_WARP = 32 * TURN_ROW;
+constexpr size_t MANY_SMEM = MANY_TURN + 8 * TURN_WARP * 4 + 1024;
+static_assert(MANY_SMEM <= 227 * 1024, "shared memory of a block");
 constexpr int RASTER = 8;
 
 __device__ __forceinline__ void tile_of(int t, int w_tiles, int x_tiles, int& w, int& x) {     // groups of RASTER weight tiles, in a group rows of tiles
@@ -506,8 +524,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
     const uint32_t full0 = bars, empty0 = bars + 8 * STAGES, acc_full = empty0 + 8 * STAGES, acc_empty = acc_full + 8 * SLOTS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (acc_empty + 8 * SLOTS - base));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int w_tiles = (p.n + BN - 1) / BN, x_tiles = (p.rows + BM - 1) / BM, tiles = w_tiles * x_tiles;
-    const int splits = SPLIT ? gridDim.x : 1, split = SPLIT ? blockIdx.x : 0, first = SPLIT ? blockIdx.y : blockIdx.x, step = SPLIT ? gridDim.y : gridDim.x;
+    const int w_tiles = (p.n + BN - 1) / BN, x_tiles = (p.rows + BM - 1) / BM, tiles = p.end_tile;
+    const int splits = SPLIT ? gridDim.x : 1, split = SPLIT ? blockIdx.x : 0, first = p.first_tile + (SPLIT ? blockIdx.y : blockIdx.x), step = SPLIT ? gridDim.y : gridDim.x;
     const int g_begin = split * p.groups_per_split, count = min(p.groups, g_begin + p.groups_per_split) - g_begin;
     int* status = p.status;
     if (threadIdx.x == 0) {
@@ -527,46 +545,50 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     pdl_launch_dependents();
-    if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 1;
-            bool ok = true;
-            for (int tile = first; tile < tiles && ok; tile += step) {
-                int w, x;
-                tile_of(tile, w_tiles, x_tiles, w, x);
-                                for (int g = 0; g < count; ++g) {
-                    ok = mbar_wait(empty0 + 8 * s, phase, status, 1);
-                    if (!ok) break;
-                    mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
-                    const uint32_t dst = base + s * STAGE_BYTES;
-                    tma_load_2d(dst, &map_x, full0 + 8 * s, (g_begin + g) * GROUP, x * BM);
-                    tma_load_2d(dst + A_BYTES, &map_w, full0 + 8 * s, (g_begin + g) * GROUP, w * BN);
-                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            if (lane == 0) {
+                int s = 0;
+                uint32_t phase = 1;
+                bool ok = true;
+                for (int tile = first; tile < tiles && ok; tile += step) {
+                    int w, x;
+                    tile_of(tile, w_tiles, x_tiles, w, x);
+                    for (int g = 0; g < count; ++g) {
+                        ok = wait(empty0 + 8 * s, phase, status, 1);
+                        if (!ok) break;
+                        mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
+                        const uint32_t dst = base + s * STAGE_BYTES;
+                        tma_load_2d(dst, &map_x, full0 + 8 * s, (g_begin + g) * GROUP, x * BM);
+                        tma_load_2d(dst + A_BYTES, &map_w, full0 + 8 * s, (g_begin + g) * GROUP, w * BN);
+                        if (++s == STAGES) { s = 0; phase ^= 1u; }
+                    }
                 }
             }
-        }
-    } else if (warp == 1) {
-        const uint64_t a_desc0 = operand_desc(base), b_desc0 = operand_desc(base + A_BYTES);
-        const uint32_t one = elect_one();
-        int s = 0, b = 0;
-        uint32_t phase = 0, acc_phase = 1;
-        bool ok = true;
-        for (int tile = first; tile < tiles && ok; tile += step)
-            for (int g = 0; g < count; ++g) {
-                ok = wait_warp(full0 + 8 * s, phase, status, 2) && wait_warp(acc_empty + 8 * b, acc_phase, status, 2);
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t at = (uint64_t)(s * (STAGE_BYTES >> 4));
+        } else if (warp == 1) {
+            const uint64_t a_desc0 = operand_desc(base), b_desc0 = operand_desc(base + A_BYTES);
+            const uint32_t one = elect_one();
+            int s = 0, b = 0;
+            uint32_t phase = 0, acc_phase = 1;
+            bool ok = true;
+            for (int tile = first; tile < tiles && ok; tile += step)
+                for (int g = 0; g < count; ++g) {
+                    ok = __all_sync(0xffffffffu, wait(full0 + 8 * s, phase, status, 2)) && __all_sync(0xffffffffu, wait(acc_empty + 8 * b, acc_phase, status, 2));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t at = (uint64_t)(s * (STAGE_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < GROUP / 32; ++k) umma_fp8(tmem_base + b * BN, a_desc0 + at + 2 * k, b_desc0 + at + 2 * k, IDESC, k > 0 ? 1u : 0u, one);
-                commit_one(acc_full + 8 * b, one);
-                commit_one(empty0 + 8 * s, one);
-                if (++s == STAGES) { s = 0; phase ^= 1u; }
-                if (++b == SLOTS) { b = 0; acc_phase ^= 1u; }
-            }
+                    for (int k = 0; k < GROUP / 32; ++k) umma_fp8(tmem_base + b * BN, a_desc0 + at + 2 * k, b_desc0 + at + 2 * k, IDESC, k > 0 ? 1u : 0u, one);
+                    commit_one(acc_full + 8 * b, one);
+                    commit_one(empty0 + 8 * s, one);
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                    if (++b == SLOTS) { b = 0; acc_phase ^= 1u; }
+                }
+        }
     } else {
-        const int quarter = warp & 3, part = (warp - 2) >> 2, row = quarter * 32 + lane;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quarter = warp & 3, part = (warp - 4) >> 2, row = quarter * 32 + lane;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * CW);
         int b = 0;
         uint32_t acc_phase = 0;
@@ -594,7 +616,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
                     if (g + 4 < count) fetch(g + 4);
                 }
                 const float now = (g & 2) ? (g & 1) ? by[3] : by[2] : (g & 1) ? by[1] : by[0];
-                ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, acc_phase, status, 3));
+                ok = __all_sync(0xffffffffu, wait(acc_full + 8 * b, acc_phase, status, 3));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t at = lane_addr + (uint32_t)(b * BN);
@@ -616,7 +638,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
                 }
                 if (++b == SLOTS) { b = 0; acc_phase ^= 1u; }
             }
-            TO* dst = (TO*)p.out + (size_t)m * p.n + n0;
             if (SPLIT) {
                 float* park = reinterpret_cast<float*>(smem) + row * PARK_ROW + part * CW;      // over the ring: every product that read it is complete
 #pragma unroll
@@ -624,8 +645,30 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
                     const float2 lo = unpair(acc[c]), hi = unpair(acc[c + 1]);
                     *reinterpret_cast<float4*>(park + 2 * c) = make_float4(lo.x, lo.y, hi.x, hi.y);
                 }
-            } else if (!ok || m >= p.rows) {
-            } else if (p.wide == 2 && n0 + CW <= p.n) {
+            } else if (!ok) {
+            } else if (p.wide != 2 || n0 + CW > p.n) {
+                // rows that do not begin where 32 bytes do, and the last columns: through shared memory, so that a warp writes 32 neighbours of a row at a time
+                // (2795 rows of 2568 x 8576: 85 us, each lane its own row 154)
+                float* turn = reinterpret_cast<float*>(smem + MANY_TURN) + (warp - 4) * TURN_WARP;
+                const int rows = min(32, p.rows - (m - lane));
+#pragma unroll
+                for (int c0 = 0; c0 < CW; c0 += 32) {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const float2 y = unpair(acc[c0 / 2 + c]);
+                        turn[lane * TURN_ROW + 2 * c] = y.x;
+                        turn[lane * TURN_ROW + 2 * c + 1] = y.y;
+                    }
+                    __syncwarp();
+                    const int n = n0 + c0 + lane;
+                    TO* to = (TO*)p.out + (size_t)(m - lane) * p.n + n;
+                    if (n < p.n)
+#pragma unroll 4
+                        for (int r = 0; r < rows; ++r) to[(size_t)r * p.n] = from_float<TO>(turn[r * TURN_ROW + lane]);
+                    __syncwarp();
+                }
+            } else if (m < p.rows) {
+                TO* dst = (TO*)p.out + (size_t)m * p.n + n0;
                 constexpr int PER = 32 / sizeof(TO);       // numbers in 32 bytes
 #pragma unroll
                 for (int c = 0; c < CW; c += PER) {
@@ -644,13 +687,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
                     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c), "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3]), "r"(word[4]),
                                  "r"(word[5]), "r"(word[6]), "r"(word[7]) : "memory");
                 }
-            } else {
-#pragma unroll
-                for (int c = 0; c < CW / 2; ++c) {
-                    const float2 y = unpair(acc[c]);
-                    if (n0 + 2 * c < p.n) dst[2 * c] = from_float<TO>(y.x);
-                    if (n0 + 2 * c + 1 < p.n) dst[2 * c + 1] = from_float<TO>(y.y);
-                }
             }
             __syncwarp();
         }
@@ -667,7 +703,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) gemm_fp8_many_kernel(const __
         // the block of rank r finishes rows r, r + splits, ..., a warp a row, four neighbouring numbers a lane at a time
         int w, x;
         tile_of(first, w_tiles, x_tiles, w, x);
-        for (int i = warp; i * splits + split < BM; i += MANY_THREADS / 32) {
+        for (int i = warp - 4; i >= 0 && i * splits + split < BM; i += 8) {
             const int r = i * splits + split, m = x * BM + r;
             if (m >= p.rows) break;
 #pragma unroll
@@ -738,13 +774,33 @@ template <typename TO> int launch_many(const void* x8, const void* w8, GemmParam
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "gemm_fp8: cannot raise shared memory: %s", cudaGetErrorString(raised));
     const long long tiles = (long long)((p.n + BN - 1) / BN) * ((p.rows + BM - 1) / BM);
     QT_REQUIRE(tiles <= 0x7fffffff / RASTER, "gemm_fp8: %d x %d outputs are too many", p.rows, p.n);
-    p.groups_per_split = (p.groups + splits - 1) / splits;
-    splits = (p.groups + p.groups_per_split - 1) / p.groups_per_split;
+    auto cut = [&p](int ranges) {                           // the ranges that are not empty
+        p.groups_per_split = (p.groups + ranges - 1) / ranges;
+        return (p.groups + p.groups_per_split - 1) / p.groups_per_split;
+    };
+    auto launch_split = [&](int ranges, long long count) {
+        launch_kernel_cluster(gemm_fp8_many_kernel<true, TO>, dim3(ranges, (unsigned)count), dim3(MANY_THREADS), MANY_SMEM, stream, ranges, map_w, map_x, p);
+    };
+    p.first_tile = 0;
+    p.end_tile = (int)tiles;
+    if (splits > 1) splits = cut(splits);
     if (splits > 1) {
         QT_REQUIRE(splits <= 8 && tiles <= 65535, "gemm_fp8: %d ranges of K for %lld tiles", splits, tiles);
-        launch_kernel_cluster(gemm_fp8_many_kernel<true, TO>, dim3(splits, (unsigned)tiles), dim3(MANY_THREADS), MANY_SMEM, stream, splits, map_w, map_x, p);
+        launch_split(splits, tiles);
     } else {
-        launch_kernel(gemm_fp8_many_kernel<false, TO>, dim3((unsigned)std::min<long long>(tiles, sm_count())), dim3(MANY_THREADS), MANY_SMEM, stream, map_w, map_x, p);
+        // A last round of few tiles would leave most SMs idle: its tiles are cut into ranges of K in a launch of their own, where that saves more than the launch and the
+        // join take, some 20 groups' time (1512 rows of 6335 x 6800, 300 tiles, 54 groups: 90 us, uncut 104; 1600 of 4096 x 4096, 208 tiles, 32 groups: 38, uncut 37)
+        const int sms = sm_count(), rest = (int)(tiles % sms), most = tiles > sms && rest ? std::min(std::min(8, 130 * sms / 148 / rest), p.groups / 8) : 1;
+        const int ranges = p.groups * (most - 1) > 20 * most ? most : 1;
+        p.groups_per_split = p.groups;
+        if (ranges > 1) p.end_tile = (int)tiles - rest;
+        launch_kernel(gemm_fp8_many_kernel<false, TO>, dim3((unsigned)std::min<long long>(p.end_tile, sms)), dim3(MANY_THREADS), MANY_SMEM, stream, map_w, map_x, p);
+        if (ranges > 1) {
+            QT_CHECK_LAUNCH("gemm_fp8 many");
+            p.first_tile = p.end_tile;
+            p.end_tile = (int)tiles;
+            launch_split(cut(ranges), rest);
+        }
     }
     QT_CHECK_LAUNCH("gemm_fp8 many");
     return QT_OK;
@@ -810,7 +866,7 @@ extern "C" int qt_gemm_fp8(const Fp8Call* call) {
     QT_REQUIRE(c.status != nullptr && (c.x || !c.fused), "gemm_fp8: a status word is required");
     const int size = c.out_dtype == QT_F32 ? 4 : 2;
     cudaStream_t s = (cudaStream_t)c.stream;
-    const GemmParams p{c.x, c.k % 4 == 0 && (uintptr_t)c.x % 16 == 0, c.x_scale, c.w_scale, c.out, c.rows, c.n, c.k, (c.k + GROUP - 1) / GROUP, 0,
+    const GemmParams p{c.x, c.k % 4 == 0 && (uintptr_t)c.x % 16 == 0, c.x_scale, c.w_scale, c.out, c.rows, c.n, c.k, (c.k + GROUP - 1) / GROUP, 0, 0, 0,
                        (uintptr_t)c.out % 32 == 0 && (size_t)c.n * size % 32 == 0 ? 2 : (uintptr_t)c.out % 16 == 0 && c.n % 4 == 0 ? 1 : 0, c.status};
     const bool aligned = c.k % 16 == 0 && (((uintptr_t)c.x8 | (uintptr_t)c.w8) & 15) == 0;
     const int form = aligned ? c.form : 0;

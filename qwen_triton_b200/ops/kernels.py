@@ -1693,7 +1693,7 @@ def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
 
     Up to 64 rows read the weight once, in ranges that give up to 256 blocks (8 rows of 6144 x 4096 in 4 / 5 / 6 / 8 ranges: 9.6 / 9.4 / 12.3 / 11.8 us; of 4096 x 12288
     in 4 / 8: 16.3 / 14.2).  Beyond, the smaller of two times in us, fitted to 30 shapes of 100 to 768 rows: tiles of 64 rows, two blocks an SM, 0.37 to 0.5 a group of
-    K; of 128 x 256, one block an SM, 0.45 to 0.62, which the L2 cache's 12 TB/s to all SMs bounds.  Clusters of ranges over more than 130 SMs do not fit at once
+    K; of 128 x 256, one block an SM, 0.42 to 0.57, which the L2 cache's 12 TB/s to all SMs bounds.  Clusters of ranges over more than 130 SMs do not fit at once
     (333 rows of 4096 x 12288 in 1 / 2 / 3 ranges: 58 / 39 / 51 us)."""
     groups, blocks_n = -(-k // FP8_GROUP), -(-n // 128)
     if k % 16:
@@ -1709,7 +1709,7 @@ def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
             if form == 64:
                 cost = 6 + 0.4 * (splits - 1) + per_split * (0.37 if blocks <= sms else 0.5 * -(-blocks // (2 * sms)))
             else:
-                cost = 8 + 3 * (splits > 1) + per_split * -(-blocks // sms) * (0.45 + 0.17 * min(1.0, blocks / sms))
+                cost = 8 + 3 * (splits > 1) + per_split * -(-blocks // sms) * (0.42 + 0.15 * min(1.0, blocks / sms))
             if best is None or cost < best[0]:
                 best = (cost, form, splits)
     return best[1:]
