@@ -1,4 +1,4 @@
-// Attention of prompts over a cache held in 8 bits on the fifth-generation tensor cores (bfloat16 queries, heads of 64 or 128, pages of 64).
+// Attention of prompts over a cache held in 8 bits on the fifth-generation tensor cores (bfloat16 queries, heads in steps of 16 up to 128, pages of 64).
 //
 //   S = Q K^T        tcgen05.mma kind::f8f6f4.  The keys are 8-bit numbers as they lie in the cache.  A query row times a power of two is the sum of two such numbers:
 //                    the nearest one and the nearest to what is left, which hold a bfloat16 number's eight digits but for elements below 2^-8 of the row's
@@ -42,7 +42,7 @@ struct TcParams {
     const uint8_t* v; const float* k_scale; const float* v_scale;
     const int* block_table; int max_blocks, n_pages;
     const int* seq_start; const int* seq_past;
-    int nq, nkv;
+    int nq, nkv, d;
     float scale;
     int* status;
 };
@@ -148,9 +148,12 @@ template <int HD> struct Shape {
     static constexpr size_t SMEM = BARS + 8 * N_BARS + 16 + 1024;
 };
 
-template <int HD>
+// HD: the head size, or (not FULL) what it is rounded up to.  Keys and queries have zeros behind d, values anything: their products are columns of O that nobody reads.
+template <int HD, bool FULL>
 __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const __grid_constant__ CUtensorMap map_k, const TcParams p) {
     using S = Shape<HD>;
+    const int d = FULL ? HD : p.d;
+    const uint32_t v_page = FULL ? S::PAGE_BYTES : (uint32_t)(PAGE * p.d);
     constexpr uint32_t IDESC_QK = (1u << 4) | ((uint32_t)(PAGE >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);                      // e4m3, both K-major
     constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);           // halves, V MN-major
     constexpr uint32_t O_COL = TILES * 2 * PAGE;           // S of tile t, buffer b at (2 t + b) * 64; O of tile t behind them
@@ -209,8 +212,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
                     mbar_expect_tx(k_full + 8 * ks, S::PAGE_BYTES);
                     tma_load_2d(base + S::K0 + ks * S::PAGE_BYTES, &map_k, k_full + 8 * ks, 0, (int)(block * PAGE));
                     if (!wait(raw_empty + 8 * rs, ((uint32_t)(j / RAW_STAGES) & 1u) ^ 1u, status, 1)) break;
-                    mbar_expect_tx(raw_full + 8 * rs, S::PAGE_BYTES);
-                    bulk_load(base + S::RAW0 + rs * S::PAGE_BYTES, p.v + block * S::PAGE_BYTES, S::PAGE_BYTES, raw_full + 8 * rs);
+                    mbar_expect_tx(raw_full + 8 * rs, v_page);
+                    bulk_load(base + S::RAW0 + rs * S::PAGE_BYTES, p.v + block * v_page, v_page, raw_full + 8 * rs);
                 }
             }
         } else if (warp == 1) {
@@ -268,7 +271,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
         // 16 bytes of a key's values become 32: two 16-byte pieces of the row's 128 bytes in a block of 64 elements.  Neighbours take the pieces in turns, so that the
         // lanes that write together meet all banks.
         const int thread = threadIdx.x - 128;
-        constexpr int PIECES = HD / 16, EACH = PAGE * PIECES / 128;        // pieces of a key; pieces of a page that a thread converts
+        constexpr int EACH = PAGE * (HD / 16) / 128;       // pieces of a page that a thread converts, at most
+        const int pieces = d / 16;                         // of a key
+        int keys[EACH], columns[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            keys[i] = (thread + i * 128) / pieces;         // PAGE or more: none
+            columns[i] = (thread + i * 128) % pieces;
+        }
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
             const int rs = j % RAW_STAGES, vs = j % V_STAGES;
@@ -277,15 +287,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             uint4 v[EACH];
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                const int piece = thread + i * 128;
-                v[i] = load16(base + S::RAW0 + rs * S::PAGE_BYTES + piece * 16);
-                if (j * PAGE + piece / PIECES >= end) v[i] = make_uint4(0, 0, 0, 0);       // behind the last key lies anything, NaN too
+                if (!FULL && keys[i] >= PAGE) continue;
+                v[i] = load16(base + S::RAW0 + rs * S::PAGE_BYTES + (thread + i * 128) * 16);
+                if (j * PAGE + keys[i] >= end) v[i] = make_uint4(0, 0, 0, 0);       // behind the last key lies anything, NaN too
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(raw_empty + 8 * rs);
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                const int piece = thread + i * 128, key = piece / PIECES, c = piece % PIECES, swap = (c >> 2) & 1;
+                if (!FULL && keys[i] >= PAGE) continue;
+                const int key = keys[i], c = columns[i], swap = (c >> 2) & 1;
                 const uint32_t row = base + S::V0 + vs * S::V_BYTES + (c >> 2) * S::V_BLOCK + key * 128;
                 const uint4 lo = make_uint4(halves(v[i].x), halves(v[i].x >> 16), halves(v[i].y), halves(v[i].y >> 16));
                 const uint4 hi = make_uint4(halves(v[i].z), halves(v[i].z >> 16), halves(v[i].w), halves(v[i].w >> 16));
@@ -307,12 +318,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
         float factor = 0.f;
         if (my_rows) {
             // the row as two 8-bit numbers an element, 2^-shift of it: its largest lies in [2^7, 2^8)
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + ((size_t)token * p.nq + head) * HD);
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + ((size_t)token * p.nq + head) * d);
             uint4 x[HD / 8];
             float most = 0.f;
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
-                x[i] = src[i];
+                x[i] = FULL || 8 * i < d ? src[i] : make_uint4(0, 0, 0, 0);
                 const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
-                for (int c0 = 0; c0 < HD; c0 += 32) {
+                for (int c0 = 0; c0 < d; c0 += 32) {
                     uint32_t o[32];
                     tmem_load32(lane_addr + O_COL + (uint32_t)(t * HD + c0), o);
 #pragma unroll
@@ -428,14 +439,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
         if (last >= 0 && ok && wait_warp(pv_full + 8 * (2 * t + (last & 1)), (uint32_t)(last >> 1) & 1u, status, 3)) {
             tc_fence_after();
             const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-            __nv_bfloat16* dst = p.out + ((size_t)token * p.nq + head) * HD;
+            __nv_bfloat16* dst = p.out + ((size_t)token * p.nq + head) * d;
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 32) {
+            for (int c0 = 0; c0 < d; c0 += 32) {
                 uint32_t o[32];
                 tmem_load32(lane_addr + O_COL + (uint32_t)(t * HD + c0), o);
                 if (r < my_rows) {
 #pragma unroll
                     for (int c = 0; c < 32; c += 8) {
+                        if (!FULL && c0 + c >= d) break;
                         uint4 w;
                         w.x = pack_bf16(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
                         w.y = pack_bf16(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
@@ -457,31 +469,31 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
 }
 
-template <int HD> int launch(const void* k, const TcParams& p, int n_seqs, int max_q_len, cudaStream_t stream) {
+template <int HD, bool FULL> int launch(const void* k, const TcParams& p, int n_seqs, int max_q_len, cudaStream_t stream) {
     EncodeFn encode = encode_fn();
     if (!encode) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8_tc: the driver does not offer cuTensorMapEncodeTiled");
     CUtensorMap map_k;
-    const cuuint64_t dims[2] = {HD, (cuuint64_t)p.n_pages * p.nkv * PAGE}, strides[1] = {HD};
+    const cuuint64_t dims[2] = {(cuuint64_t)p.d, (cuuint64_t)p.n_pages * p.nkv * PAGE}, strides[1] = {(cuuint64_t)p.d};      // zeros behind d
     const cuuint32_t box[2] = {HD, PAGE}, elem[2] = {1, 1};
     const CUresult rc = encode(&map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(k), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8_tc: cuTensorMapEncodeTiled failed with %d", (int)rc);
-    const cudaError_t raised = raise_shared<attention_cache8_tc_kernel<HD>>((int)Shape<HD>::SMEM);
+    const cudaError_t raised = raise_shared<attention_cache8_tc_kernel<HD, FULL>>((int)Shape<HD>::SMEM);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8_tc: cannot raise shared memory: %s", cudaGetErrorString(raised));
     const long long blocks = ((long long)max_q_len * (p.nq / p.nkv) + TILES * BQ - 1) / (TILES * BQ);
     QT_REQUIRE(blocks <= 65535, "attention_cache8_tc: %d tokens of a sequence are too many", max_q_len);
-    launch_kernel(attention_cache8_tc_kernel<HD>, dim3(p.nkv, (unsigned)blocks, n_seqs), dim3(THREADS), Shape<HD>::SMEM, stream, map_k, p);
+    launch_kernel(attention_cache8_tc_kernel<HD, FULL>, dim3(p.nkv, (unsigned)blocks, n_seqs), dim3(THREADS), Shape<HD>::SMEM, stream, map_k, p);
     QT_CHECK_LAUNCH("attention_cache8_tc");
     return QT_OK;
 }
 
 }  // namespace
 
-// Packed bfloat16 queries [n_tokens, nq, d] of sequences whose keys, this call's own among them, are in the cache; causal.  d is 64 or 128.
+// Packed bfloat16 queries [n_tokens, nq, d] of sequences whose keys, this call's own among them, are in the cache; causal.  d is a multiple of 16 up to 128.
 extern "C" int qt_attention_prefill_cache8_tc(const Cache8Call* call) {
     const Cache8Call& c = *call;
     if (c.n_seqs == 0 || c.max_q_len == 0) return QT_OK;
-    QT_REQUIRE(c.dtype == QT_BF16 && (c.d == 64 || c.d == 128), "attention_prefill_cache8_tc: bfloat16 heads of 64 or 128, not %d (type %d)", c.d, c.dtype);
+    QT_REQUIRE(c.dtype == QT_BF16 && c.d > 0 && c.d <= 128 && c.d % 16 == 0, "attention_prefill_cache8_tc: bfloat16 heads in steps of 16 up to 128, not %d (type %d)", c.d, c.dtype);
     QT_REQUIRE(c.nq > 0 && c.nkv > 0 && c.nq % c.nkv == 0 && c.nkv <= 0x7fffffff && c.max_blocks > 0 && c.max_blocks <= 0x7fffffff / PAGE && c.n_pages > 0 && c.n_seqs > 0 &&
                    c.n_seqs <= 65535 && c.max_q_len > 0 && (long long)c.max_q_len * (c.nq / c.nkv) <= 0x7fffffff - TILES * BQ &&
                    (long long)c.n_pages * c.nkv <= 0x7fffffff / PAGE,
@@ -489,8 +501,11 @@ extern "C" int qt_attention_prefill_cache8_tc(const Cache8Call* call) {
     QT_REQUIRE(c.status != nullptr && c.scale > 0., "attention_prefill_cache8_tc: a status word and a positive scale are required");
     QT_REQUIRE((((uintptr_t)c.q | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.out) & 15) == 0, "attention_prefill_cache8_tc: operands must be 16-byte aligned");
     const TcParams p{(const __nv_bfloat16*)c.q, (__nv_bfloat16*)c.out, (const uint8_t*)c.v, c.k_scale, c.v_scale, c.block_table, c.max_blocks, c.n_pages, c.seq_start, c.seq_past,
-                     c.nq, c.nkv, (float)c.scale, c.status};
-    return c.d == 64 ? launch<64>(c.k, p, c.n_seqs, c.max_q_len, (cudaStream_t)c.stream) : launch<128>(c.k, p, c.n_seqs, c.max_q_len, (cudaStream_t)c.stream);
+                     c.nq, c.nkv, c.d, (float)c.scale, c.status};
+    cudaStream_t s = (cudaStream_t)c.stream;
+    if (c.d == 64) return launch<64, true>(c.k, p, c.n_seqs, c.max_q_len, s);
+    if (c.d == 128) return launch<128, true>(c.k, p, c.n_seqs, c.max_q_len, s);
+    return c.d < 64 ? launch<64, false>(c.k, p, c.n_seqs, c.max_q_len, s) : launch<128, false>(c.k, p, c.n_seqs, c.max_q_len, s);
 }
 
 QT_DEFINE_LAST_ERROR(attention_cache8_tc)

@@ -1985,7 +1985,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     """``attention_prefill`` over a cache in 8 bits: packed queries [T, nq, d], sequence i's from ``seq_start[i]`` on (at most ``max_q_len``), behind ``seq_past[i]`` earlier
     tokens; the cache already holds this step's keys; a query sees the keys up to its own.
 
-    ``impl``: "tc" (tcgen05: bfloat16 heads of 64 or 128 under a positive scale; the default for those, but for few rows) or "mma" (any call; a
+    ``impl``: "tc" (tcgen05: bfloat16 heads up to 128 under a positive scale; the default for those, but for few rows) or "mma" (any call; a
     tile of eight rows by a cluster of ``ranges`` blocks, up to eight).  A value
     that is not a number makes the results of the queries that see it NaN, and may make those of earlier queries of the call that read its page."""
     n_seqs, device, k = seq_past.shape[0], _current_device(), cache.k
@@ -1996,11 +1996,11 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
             and q.is_contiguous() and out.is_contiguous() and block_table.is_contiguous() and seq_start.is_contiguous() and seq_past.is_contiguous()
             and q.get_device() == out.get_device() == k.get_device() == block_table.get_device() == seq_start.get_device() == seq_past.get_device() == device):
         _check_prefill_cache8(q, cache, out, block_table, seq_start, seq_past, max_q_len)
-    on_tc = q.dtype is torch.bfloat16 and k.shape[3] in (64, 128) and scale > 0
+    on_tc = q.dtype is torch.bfloat16 and k.shape[3] <= 128 and scale > 0
     if impl not in (None, "tc", "mma") or (impl == "tc" and not on_tc):
         raise KernelError(f"attention_prefill_cache8: impl={impl!r} for {q.dtype}, heads of {k.shape[3]}, a scale of {scale}")
     walks = -(-max_q_len * (q.shape[1] // k.shape[1]) // 8) * k.shape[1] * n_seqs         # tiles of eight rows
-    if impl == "mma" or (impl is None and walks <= _MMA_WALKS[k.shape[3] == 64]):
+    if impl == "mma" or (impl is None and walks <= _MMA_WALKS[k.shape[3] <= 64]):
         on_tc = False
     if ranges is None:
         # as many blocks as are resident

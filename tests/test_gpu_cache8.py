@@ -159,7 +159,7 @@ def _prompt(counts, past, heads, kv_heads, dim, dtype, seed=0, scale=None, sprea
     scale = dim ** -0.5 if scale is None else scale
     starts = [sum(counts[:i]) for i in range(len(counts) + 1)]
     want = {}
-    for form in (impl,) if impl else ("tc", "mma") if dtype == BF16 and dim in (64, 128) and scale > 0 else ("mma",):
+    for form in (impl,) if impl else ("tc", "mma") if dtype == BF16 and dim <= 128 and scale > 0 else ("mma",):
         out = torch.full_like(q, math.nan, device="cuda")
         kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints(starts), _ints(past), max(counts), scale, form, ranges if form == "mma" else None)
         _close(out, *plain.attention(q, *_held(cache), table, counts, past, scale, DIGITS[dtype], form == "tc"))
