@@ -15,6 +15,9 @@
 // scaled by (halves end at 2^16; at 2^8, 2 % slower).  512 threads: warp 0 copies (TMA tiles of keys, bulk copies of values), warp 1 issues, warps 4 to 7 convert values, warps 8 to 11 and 12 to 15 are the
 // softmax of the two tiles, with most of the registers: 88 + 88 + 168 + 168 = 4 * 128.  Every mbarrier wait is bounded and reports through a status word.
 //
+// Few blocks behind many keys: the pages of a block are cut into ranges for a cluster of up to eight, whose sums meet in distributed shared memory, laid over the
+// operands (256 tokens of 32 heads over 8 of 128 behind 8,000: 149 us in one range, 51 in four; 64 tokens 145 and, in eight, 34).
+//
 // What bounds it: the products of scores with a page's 64 keys, whose time is their queries' way from shared memory (66 cycles for 128 x 64 x 32, of which the
 // tensor cores need 32), 1,650 cycles of the 1,900 that a page takes for 256 rows.  Two pages at a time would halve it, but tensor memory then holds one sum
 // per row and the two threads of a row walk in step: 739 us in the place of 712 for 4,096 tokens behind 8,192, 32 heads over 8 of 128 (965 TFLOP/s; the same over a
@@ -35,6 +38,7 @@ constexpr int PAGE = 64;
 constexpr int BQ = 128, TILES = 2;                         // rows of a tile = the instruction's M; tiles of a block
 constexpr int THREADS = 512;
 constexpr int K_STAGES = 3, RAW_STAGES = 3, V_STAGES = 3;
+constexpr int MAX_RANGES = 8, LEAST_PAGES = 4;              // blocks of a cluster; pages that a block walks before another one has any
 constexpr float RESCALE_STEP = 14.f, LOG2E = 1.4426950408889634f;
 
 struct TcParams {
@@ -42,7 +46,7 @@ struct TcParams {
     const uint8_t* v; const float* k_scale; const float* v_scale;
     const int* block_table; int max_blocks, n_pages;
     const int* seq_start; const int* seq_past;
-    int nq, nkv, d;
+    int nq, nkv, d, ranges;
     float scale;
     int* status;
 };
@@ -146,10 +150,15 @@ template <int HD> struct Shape {
     static constexpr uint32_t Q0 = 0, K0 = TILES * Q_TILE, V0 = K0 + K_STAGES * PAGE_BYTES, RAW0 = V0 + V_STAGES * V_BYTES, BARS = RAW0 + RAW_STAGES * PAGE_BYTES;
     static constexpr int N_BARS = TILES + 2 * K_STAGES + 2 * RAW_STAGES + 2 * V_STAGES + 3 * 2 * TILES;
     static constexpr size_t SMEM = BARS + 8 * N_BARS + 16 + 1024;
+    // SPLIT: a block's sums, over everything before the barriers; rows begin four banks apart
+    static constexpr int PARK_ROW = HD + 4;
+    static constexpr uint32_t PARK_ML = TILES * BQ * PARK_ROW * 4;
+    static_assert(PARK_ML + TILES * BQ * 8 <= BARS, "the sums lie over the operands");
 };
 
 // HD: the head size, or (not FULL) what it is rounded up to.  Keys and queries have zeros behind d, values anything: their products are columns of O that nobody reads.
-template <int HD, bool FULL>
+// SPLIT: the pages are walked by a cluster of blocks (along x), a range each, whose sums meet in distributed shared memory.
+template <int HD, bool FULL, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const __grid_constant__ CUtensorMap map_k, const TcParams p) {
     using S = Shape<HD>;
     const int d = FULL ? HD : p.d;
@@ -160,7 +169,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
     extern __shared__ uint8_t smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();                                            // before tensor memory is taken: a block of an earlier kernel never waits for what this one holds
-    const int seq = blockIdx.z, kvh = blockIdx.x, group = p.nq / p.nkv;
+    const int seq = blockIdx.z, ranges = SPLIT ? p.ranges : 1, kvh = SPLIT ? blockIdx.x / ranges : blockIdx.x, range = SPLIT ? blockIdx.x % ranges : 0, group = p.nq / p.nkv;
     const int start = p.seq_start[seq], rows_all = (p.seq_start[seq + 1] - start) * group, past = p.seq_past[seq];
     const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * (TILES * BQ);              // the longest walks first
     if (row0 >= rows_all) return;                          // uniform for the block
@@ -171,10 +180,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
         rows[t] = max(0, min(BQ, rows_all - row0 - t * BQ));
         n_tiles[t] = rows[t] ? (min(past + (row0 + t * BQ + rows[t] - 1) / group + 1, capacity) + PAGE - 1) / PAGE : 0;
     }
+    int page0 = 0;                                         // the block's first page; what follows counts from there
+    if (SPLIT) {
+        const int each = max(LEAST_PAGES, (max(n_tiles[0], n_tiles[1]) + ranges - 1) / ranges);
+        page0 = range * each;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) n_tiles[t] = max(0, min(each, n_tiles[t] - page0));
+    }
     const int n = max(n_tiles[0], n_tiles[1]);
     const int end = min(past + (min(rows_all, row0 + TILES * BQ) - 1) / group + 1, capacity);          // keys that any row sees
     const int* table = p.block_table + (size_t)seq * p.max_blocks;
-    auto block_of = [&](int j) { return (size_t)min(max(table[j], 0), p.n_pages - 1) * p.nkv + kvh; };
+    auto block_of = [&](int j) { return (size_t)min(max(table[page0 + j], 0), p.n_pages - 1) * p.nkv + kvh; };
 
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     const uint32_t bars = base + S::BARS;
@@ -232,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
                                    k_desc0 + (uint64_t)((s * S::PAGE_BYTES + ks * 32) >> 4), IDESC_QK, part + ks > 0 ? 1u : 0u, one);
                 commit_one(s_full + 8 * (2 * t + (j & 1)), one);
             };
-            bool ok = wait_warp(k_full, 0, status, 2);
+            bool ok = n > 0 && wait_warp(k_full, 0, status, 2);
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
                 if (ok && n_tiles[t] > 0) {
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             for (int i = 0; i < EACH; ++i) {
                 if (!FULL && keys[i] >= PAGE) continue;
                 v[i] = load16(base + S::RAW0 + rs * S::PAGE_BYTES + (thread + i * 128) * 16);
-                if (j * PAGE + keys[i] >= end) v[i] = make_uint4(0, 0, 0, 0);       // behind the last key lies anything, NaN too
+                if ((page0 + j) * PAGE + keys[i] >= end) v[i] = make_uint4(0, 0, 0, 0);       // behind the last key lies anything, NaN too
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(raw_empty + 8 * rs);
@@ -377,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             tmem_load32_start(s_addr, v[0]);
             tmem_load32_start(s_addr + 32, v[1]);
             tmem_wait_ld();
-            const int pos0 = j * PAGE;
+            const int pos0 = (page0 + j) * PAGE;
             if (pos0 + PAGE - 1 > first_qpos) {            // some row of the tile does not see the whole page
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
@@ -436,7 +452,28 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             m_run = m_new;
         }
         const int last = my_tiles - 1;
-        if (last >= 0 && ok && wait_warp(pv_full + 8 * (2 * t + (last & 1)), (uint32_t)(last >> 1) & 1u, status, 3)) {
+        const bool done = last >= 0 && ok && wait_warp(pv_full + 8 * (2 * t + (last & 1)), (uint32_t)(last >> 1) & 1u, status, 3);
+        if (SPLIT) asm volatile("bar.sync 1, 256;" ::: "memory");      // both tiles' products are complete: the operands' place is free
+        if (SPLIT) {
+            tc_fence_after();
+            float* park = reinterpret_cast<float*>(smem_raw + (base - raw)) + (t * BQ + r) * S::PARK_ROW;
+            float* ml = reinterpret_cast<float*>(smem_raw + (base - raw) + S::PARK_ML) + 2 * (t * BQ + r);
+            ml[0] = done ? m_run : -INFINITY;
+            ml[1] = done ? l_run : 0.f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                uint32_t o[32];
+                if (done) {
+                    tmem_load32(lane_addr + O_COL + (uint32_t)(t * HD + c0), o);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = 0u;
+                }
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(park + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                __syncwarp();
+            }
+        } else if (done) {
             tc_fence_after();
             const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
             __nv_bfloat16* dst = p.out + ((size_t)token * p.nq + head) * d;
@@ -467,9 +504,44 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
         while (global_timer() - t0 < 2000000ull) __nanosleep(1000);
     }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    if (SPLIT) {
+        cluster_sync_all();
+        // the block of rank i finishes rows i, i + ranges, ...: LANES lanes a row, four columns each
+        constexpr int LANES = HD / 4, AT_ONCE = THREADS / LANES;
+        const int c = threadIdx.x % LANES * 4;
+        for (int i = threadIdx.x / LANES; i * ranges + range < TILES * BQ; i += AT_ONCE) {
+            const int r = i * ranges + range, mine = row0 + r;
+            if (mine >= rows_all) break;
+            float m = -INFINITY, l = 0.f, mk[MAX_RANGES], lk[MAX_RANGES], sum[4] = {};
+            float4 o[MAX_RANGES];
+#pragma unroll
+            for (int k = 0; k < MAX_RANGES; ++k)
+                if (k < ranges) {
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(mk[k]), "=f"(lk[k]) : "r"(map_to_cta(base + S::PARK_ML + 8 * r, k)) : "memory");
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[k].x), "=f"(o[k].y), "=f"(o[k].z), "=f"(o[k].w)
+                                 : "r"(map_to_cta(base + (uint32_t)(r * S::PARK_ROW + c) * 4, k)) : "memory");
+                }
+#pragma unroll
+            for (int k = 0; k < MAX_RANGES; ++k)
+                if (k < ranges) m = fmaxf(m, mk[k]);
+#pragma unroll
+            for (int k = 0; k < MAX_RANGES; ++k)
+                if (k < ranges) {
+                    // a range without keys has nothing; one whose sums are NaN hands that on
+                    const float by = mk[k] == -INFINITY ? 1.f : fast_exp2(mk[k] - m);
+                    l = fmaf(lk[k], by, l);
+                    sum[0] = fmaf(o[k].x, by, sum[0]); sum[1] = fmaf(o[k].y, by, sum[1]); sum[2] = fmaf(o[k].z, by, sum[2]); sum[3] = fmaf(o[k].w, by, sum[3]);
+                }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (FULL || c < d)
+                *reinterpret_cast<uint2*>(p.out + ((size_t)(start + mine / group) * p.nq + kvh * group + mine % group) * d + c) =
+                    make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
+        }
+        cluster_sync_all();                                // nobody leaves while its sums are read
+    }
 }
 
-template <int HD, bool FULL> int launch(const void* k, const TcParams& p, int n_seqs, int max_q_len, cudaStream_t stream) {
+template <int HD, bool FULL, bool SPLIT> int launch(const void* k, const TcParams& p, int n_seqs, int max_q_len, cudaStream_t stream) {
     EncodeFn encode = encode_fn();
     if (!encode) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8_tc: the driver does not offer cuTensorMapEncodeTiled");
     CUtensorMap map_k;
@@ -478,34 +550,41 @@ template <int HD, bool FULL> int launch(const void* k, const TcParams& p, int n_
     const CUresult rc = encode(&map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(k), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8_tc: cuTensorMapEncodeTiled failed with %d", (int)rc);
-    const cudaError_t raised = raise_shared<attention_cache8_tc_kernel<HD, FULL>>((int)Shape<HD>::SMEM);
+    const cudaError_t raised = raise_shared<attention_cache8_tc_kernel<HD, FULL, SPLIT>>((int)Shape<HD>::SMEM);
     if (raised != cudaSuccess) QT_FAIL(QT_ERR_LAUNCH, "attention_cache8_tc: cannot raise shared memory: %s", cudaGetErrorString(raised));
     const long long blocks = ((long long)max_q_len * (p.nq / p.nkv) + TILES * BQ - 1) / (TILES * BQ);
     QT_REQUIRE(blocks <= 65535, "attention_cache8_tc: %d tokens of a sequence are too many", max_q_len);
-    launch_kernel(attention_cache8_tc_kernel<HD, FULL>, dim3(p.nkv, (unsigned)blocks, n_seqs), dim3(THREADS), Shape<HD>::SMEM, stream, map_k, p);
+    const dim3 grid((unsigned)(p.nkv * p.ranges), (unsigned)blocks, n_seqs);
+    if (SPLIT) launch_kernel_cluster(attention_cache8_tc_kernel<HD, FULL, SPLIT>, grid, dim3(THREADS), Shape<HD>::SMEM, stream, (unsigned)p.ranges, map_k, p);
+    else launch_kernel(attention_cache8_tc_kernel<HD, FULL, SPLIT>, grid, dim3(THREADS), Shape<HD>::SMEM, stream, map_k, p);
     QT_CHECK_LAUNCH("attention_cache8_tc");
     return QT_OK;
 }
 
+template <int HD, bool FULL> int launch_ranges(const void* k, const TcParams& p, int n_seqs, int max_q_len, cudaStream_t stream) {
+    return p.ranges > 1 ? launch<HD, FULL, true>(k, p, n_seqs, max_q_len, stream) : launch<HD, FULL, false>(k, p, n_seqs, max_q_len, stream);
+}
+
 }  // namespace
 
-// Packed bfloat16 queries [n_tokens, nq, d] of sequences whose keys, this call's own among them, are in the cache; causal.  d is a multiple of 16 up to 128.
+// Packed bfloat16 queries [n_tokens, nq, d] of sequences whose keys, this call's own among them, are in the cache; causal.  d is a multiple of 16 up to 128.  A block's
+// pages are walked by a cluster of `ranges` blocks.
 extern "C" int qt_attention_prefill_cache8_tc(const Cache8Call* call) {
     const Cache8Call& c = *call;
     if (c.n_seqs == 0 || c.max_q_len == 0) return QT_OK;
     QT_REQUIRE(c.dtype == QT_BF16 && c.d > 0 && c.d <= 128 && c.d % 16 == 0, "attention_prefill_cache8_tc: bfloat16 heads in steps of 16 up to 128, not %d (type %d)", c.d, c.dtype);
-    QT_REQUIRE(c.nq > 0 && c.nkv > 0 && c.nq % c.nkv == 0 && c.nkv <= 0x7fffffff && c.max_blocks > 0 && c.max_blocks <= 0x7fffffff / PAGE && c.n_pages > 0 && c.n_seqs > 0 &&
+    QT_REQUIRE(c.nq > 0 && c.nkv > 0 && c.nq % c.nkv == 0 && c.ranges >= 1 && c.ranges <= MAX_RANGES && c.nkv <= 0x7fffffff / MAX_RANGES && c.max_blocks > 0 && c.max_blocks <= 0x7fffffff / PAGE && c.n_pages > 0 && c.n_seqs > 0 &&
                    c.n_seqs <= 65535 && c.max_q_len > 0 && (long long)c.max_q_len * (c.nq / c.nkv) <= 0x7fffffff - TILES * BQ &&
                    (long long)c.n_pages * c.nkv <= 0x7fffffff / PAGE,
                "attention_prefill_cache8_tc: bad sizes nq=%d nkv=%d, %d pages, %d sequences of up to %d tokens", c.nq, c.nkv, c.n_pages, c.n_seqs, c.max_q_len);
     QT_REQUIRE(c.status != nullptr && c.scale > 0., "attention_prefill_cache8_tc: a status word and a positive scale are required");
     QT_REQUIRE((((uintptr_t)c.q | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.out) & 15) == 0, "attention_prefill_cache8_tc: operands must be 16-byte aligned");
     const TcParams p{(const __nv_bfloat16*)c.q, (__nv_bfloat16*)c.out, (const uint8_t*)c.v, c.k_scale, c.v_scale, c.block_table, c.max_blocks, c.n_pages, c.seq_start, c.seq_past,
-                     c.nq, c.nkv, c.d, (float)c.scale, c.status};
+                     c.nq, c.nkv, c.d, c.ranges, (float)c.scale, c.status};
     cudaStream_t s = (cudaStream_t)c.stream;
-    if (c.d == 64) return launch<64, true>(c.k, p, c.n_seqs, c.max_q_len, s);
-    if (c.d == 128) return launch<128, true>(c.k, p, c.n_seqs, c.max_q_len, s);
-    return c.d < 64 ? launch<64, false>(c.k, p, c.n_seqs, c.max_q_len, s) : launch<128, false>(c.k, p, c.n_seqs, c.max_q_len, s);
+    if (c.d == 64) return launch_ranges<64, true>(c.k, p, c.n_seqs, c.max_q_len, s);
+    if (c.d == 128) return launch_ranges<128, true>(c.k, p, c.n_seqs, c.max_q_len, s);
+    return c.d < 64 ? launch_ranges<64, false>(c.k, p, c.n_seqs, c.max_q_len, s) : launch_ranges<128, false>(c.k, p, c.n_seqs, c.max_q_len, s);
 }
 
 QT_DEFINE_LAST_ERROR(attention_cache8_tc)

@@ -1980,13 +1980,52 @@ def _check_decode_cache8(q, cache, out, block_table, seq_len, plan, part_acc, pa
     raise KernelError("attention_decode_cache8: this call is not in order")
 
 
+@functools.lru_cache(maxsize=1024)
+def prefill8_plan(n_seqs: int, max_q_len: int, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype, max_pages: int, on_tc: bool = True, on_mma: bool = True,
+                  sms: int = 148) -> tuple[str, int]:
+    """(impl, ranges) of ``attention_prefill_cache8`` for ``n_seqs`` sequences of up to ``max_q_len`` tokens that see up to ``max_pages`` pages, the least of a time in us
+    for each number of ranges, fitted to 36 shapes with 1 to 8 ranges on both.
+
+    tcgen05 walks a page for 128 or 256 rows in 0.85 to 1.1 us, one block an SM; clusters of 3 and more do not fill all SMs.  On mma.sync a tile of eight rows takes
+    0.3 to 0.7 us a page by itself and longer beside others.  64 tokens of 32 heads over 8 of 128, mma.sync / tcgen05, each with its best ranges: behind 8,000 tokens 87 / 34 us, behind 500
+    14 / 19; 8 tokens behind 8,000 20 / 23; 256 tokens behind 8,000 on tcgen05 in one range / four 149 / 51."""
+    group, wide, single = num_heads // num_kv_heads, head_dim > 64, dtype == torch.float32
+    on_tc = on_tc and not single and head_dim <= 128
+    best = None
+    blocks = -(-max_q_len * group // 256) * num_kv_heads * n_seqs
+    tiles = -(-max_q_len * group // 8) * num_kv_heads * n_seqs
+    page = (1.1 if wide else 1.0) if max_q_len * group > 128 else (0.9 if wide else 0.85)
+    slots = sms * (2 if head_dim > 128 or (single and wide) else 3 if wide or single else 4)
+    alone, more = (0.7, 0.0012) if single else (0.35, 0.0018) if wide else (0.3, 0.00115)
+    for ranges in range(1, _CLUSTER_RANGES + 1):
+        if ranges > 1 and ranges > max_pages:
+            break
+        if on_tc:
+            rounds = blocks * ranges / ((sms if ranges <= 2 else 135 if ranges <= 4 else 112) * sms / 148)
+            each = 5.5 + (4 + 0.5 * ranges if ranges > 1 else 0)
+            if rounds <= 1:
+                cost = 4 + each + max(-(-max_pages // ranges), min(_LEAST_PAGES, max_pages)) * page
+            else:                                          # short and long walks meet: what counts is their mean
+                cost = 4 + (2 if rounds <= 2 else rounds + 0.5) * (each + max((max_pages - max_q_len / 128) / ranges, min(_LEAST_PAGES, max_pages)) * page)
+            best = min(best or (cost, "tc", ranges), (cost, "tc", ranges))
+        if on_mma or not on_tc:
+            at_once = tiles * ranges
+            cost = 5 + 5 * at_once / slots + (1 + 0.6 * ranges if ranges > 1 else 0) + -(-max_pages // ranges) * max(0.5, alone + more * min(at_once, slots)) * max(1.0, at_once / slots)
+            best = min(best or (cost, "mma", ranges), (cost, "mma", ranges))
+    return best[1:]
+
+
+_LEAST_PAGES = 4         # what a block on tcgen05 walks before another of its cluster has any
+
+
 def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_start: torch.Tensor, seq_past: torch.Tensor,
-                             max_q_len: int, scale: float, impl: str | None = None, ranges: int | None = None) -> None:
+                             max_q_len: int, scale: float, impl: str | None = None, ranges: int | None = None, max_context: int | None = None) -> None:
     """``attention_prefill`` over a cache in 8 bits: packed queries [T, nq, d], sequence i's from ``seq_start[i]`` on (at most ``max_q_len``), behind ``seq_past[i]`` earlier
     tokens; the cache already holds this step's keys; a query sees the keys up to its own.
 
-    ``impl``: "tc" (tcgen05: bfloat16 heads up to 128 under a positive scale; the default for those, but for few rows) or "mma" (any call; a
-    tile of eight rows by a cluster of ``ranges`` blocks, up to eight).  A value
+    ``impl``: "tc" (tcgen05: bfloat16 heads up to 128 under a positive scale, 256 rows a block) or "mma" (any call, eight rows a block), whose keys are walked by a cluster
+    of ``ranges`` blocks, up to eight; the default is ``prefill8_plan``'s choice, by ``max_context``, the most keys that a sequence has (any number gives right
+    results; without it what ``block_table`` has room for).  A value
     that is not a number makes the results of the queries that see it NaN, and may make those of earlier queries of the call that read its page."""
     n_seqs, device, k = seq_past.shape[0], _current_device(), cache.k
     # one expression for a call that is in order
@@ -1999,23 +2038,18 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     on_tc = q.dtype is torch.bfloat16 and k.shape[3] <= 128 and scale > 0
     if impl not in (None, "tc", "mma") or (impl == "tc" and not on_tc):
         raise KernelError(f"attention_prefill_cache8: impl={impl!r} for {q.dtype}, heads of {k.shape[3]}, a scale of {scale}")
-    walks = -(-max_q_len * (q.shape[1] // k.shape[1]) // 8) * k.shape[1] * n_seqs         # tiles of eight rows
-    if impl == "mma" or (impl is None and walks <= _MMA_WALKS[k.shape[3] <= 64]):
-        on_tc = False
-    if ranges is None:
-        # as many blocks as are resident
-        ranges = 1 if on_tc else max(1, min(_CLUSTER_RANGES, 2 * 148 // max(1, walks)))
-    elif on_tc or not 1 <= ranges <= _CLUSTER_RANGES:
+    if ranges is not None and not 1 <= ranges <= _CLUSTER_RANGES:
         raise KernelError(f"attention_prefill_cache8: {ranges} ranges")
+    if ranges is None or impl is None:
+        pages = block_table.shape[1] if max_context is None else max(1, min(block_table.shape[1], -(-max_context // 64)))
+        impl, chosen = prefill8_plan(n_seqs, max_q_len, num_heads=q.shape[1], num_kv_heads=k.shape[1], head_dim=k.shape[3], dtype=q.dtype, max_pages=pages,
+                                     on_tc=on_tc and impl != "mma", on_mma=impl != "tc")
+        ranges = ranges or chosen
+    on_tc = impl == "tc"
     _call(*(("attention_cache8_tc", "qt_attention_prefill_cache8_tc") if on_tc else ("attention_cache8", "qt_attention_prefill_cache8")),
           _CACHE8_CALL.pack(q.data_ptr(), k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(),
                             seq_start.data_ptr(), seq_past.data_ptr(), 0, 0, 0, _status_word(q.device).data_ptr(), _stream(), scale, _CODES[q.dtype], block_table.shape[1],
                             k.shape[0], n_seqs, q.shape[0], max_q_len, q.shape[1], k.shape[1], k.shape[3], ranges, 1, 0))
-
-
-# Tiles of eight query rows (of heads of 128, and of 64) up to which mma.sync takes prompts: their blocks are many, where 256 rows a block would leave most SMs idle
-# (32 heads over 8 of 128 behind 8,000 tokens, mma.sync / tcgen05: 8 tokens 22 / 112 us, 64 108 / 144, 128 154 / 147; behind 500: 15 / 20, 24 / 22).
-_MMA_WALKS = (444, 1184)
 
 
 def _check_prefill_cache8(q, cache, out, block_table, seq_start, seq_past, max_q_len) -> None:

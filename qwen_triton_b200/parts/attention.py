@@ -436,6 +436,6 @@ class Attention:
             kernels.attention_decode_cache8(q, cache, out, table, ctx.seq_len, self.scale, plan, ws.view("attn.part_acc", _MAX_SPLIT_PAIRS * self.nq * self.d),
                                             ws.view("attn.part_ml", _MAX_SPLIT_PAIRS * self.nq * 2))
         else:
-            kernels.attention_prefill_cache8(q, cache, out, table, ctx.seq_start, ctx.seq_past, ctx.max_q_len, self.scale)
+            kernels.attention_prefill_cache8(q, cache, out, table, ctx.seq_start, ctx.seq_past, ctx.max_q_len, self.scale, max_context=ctx.max_context)
         out = out.view(tokens, self.heads_out * self.d)
         return DeferredProduct(self.o, out) if self.o.fusable(tokens) else self.o(out)

@@ -66,3 +66,17 @@ def test_models_that_take_the_formats():
     for preset in ("lederax-tiny-a", "vunepel-tiny-a", "bisodra-tiny-a", "regupel-tiny-a", "misudra-tiny-a", "bizurax-tiny-a"):
         with pytest.raises(ValueError, match="another layer"):
             check_formats(load_preset(preset).model_spec(), None, "fp8")
+
+
+@pytest.mark.parametrize("n_seqs,tokens,heads,kv_heads,dim,dtype", [(1, 1, 16, 8, 128, torch.bfloat16), (3, 900, 32, 8, 128, torch.bfloat16), (64, 4, 64, 8, 64, torch.bfloat16),
+                                                                    (1, 4096, 16, 16, 96, torch.bfloat16), (2, 300, 4, 2, 256, torch.bfloat16), (5, 77, 6, 3, 48, torch.float32)])
+@pytest.mark.parametrize("pages", [1, 2, 9, 300, 5000])
+def test_plans_of_prompts(n_seqs, tokens, heads, kv_heads, dim, dtype, pages):
+    """tcgen05 where it can, as many ranges as a cluster has blocks at most and never more than pages; what is not offered is not chosen."""
+    shape = {"num_heads": heads, "num_kv_heads": kv_heads, "head_dim": dim, "dtype": dtype, "max_pages": pages}
+    impl, ranges = kernels.prefill8_plan(n_seqs, tokens, **shape)
+    assert impl in ("tc", "mma") and 1 <= ranges <= min(8, pages)
+    assert impl == "mma" or (dtype == torch.bfloat16 and dim <= 128)
+    assert kernels.prefill8_plan(n_seqs, tokens, **shape, on_tc=False)[0] == "mma"
+    if dtype == torch.bfloat16 and dim <= 128:
+        assert kernels.prefill8_plan(n_seqs, tokens, **shape, on_mma=False)[0] == "tc"

@@ -161,7 +161,7 @@ def _prompt(counts, past, heads, kv_heads, dim, dtype, seed=0, scale=None, sprea
     want = {}
     for form in (impl,) if impl else ("tc", "mma") if dtype == BF16 and dim <= 128 and scale > 0 else ("mma",):
         out = torch.full_like(q, math.nan, device="cuda")
-        kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints(starts), _ints(past), max(counts), scale, form, ranges if form == "mma" else None)
+        kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints(starts), _ints(past), max(counts), scale, form, ranges)
         _close(out, *plain.attention(q, *_held(cache), table, counts, past, scale, DIGITS[dtype], form == "tc"))
     kernels.check_status()
 
@@ -189,8 +189,10 @@ def test_prompts_of_many_sequences():
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_prompts_in_ranges(ranges, dtype):
     """A tile's keys by clusters of every size, more blocks than pages among them, sequences without tokens."""
-    _prompt([3, 20, 0, 1, 70], [0, 700, 64, 5, 63], 8, 2, 128, dtype, impl="mma", ranges=ranges)
-    _prompt([3, 20, 0, 1, 70], [0, 700, 64, 5, 63], 3, 1, 48, dtype, impl="mma", ranges=ranges)
+    _prompt([3, 20, 0, 1, 70], [0, 700, 64, 5, 63], 8, 2, 128, dtype, ranges=ranges)
+    _prompt([3, 20, 0, 1, 70], [0, 700, 64, 5, 63], 3, 1, 48, dtype, ranges=ranges)
+    _prompt([150, 0, 300], [1500, 64, 0], 6, 2, 64, dtype, ranges=ranges)
+    _prompt([200, 1], [900, 2100], 4, 4, 112, dtype, ranges=ranges)
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 2, 64), (4, 2, 48)])
@@ -507,7 +509,7 @@ def test_refusals():
     for impl, scale in (("other", 0.1), ("tc", -0.1)):
         with pytest.raises(Error, match="impl"):
             prefill(q, cache, out, table, _ints([0, 1, 2]), _ints([0, 0]), 1, scale, impl)
-    for impl, ranges in (("mma", 9), ("mma", 0), ("tc", 2)):
+    for impl, ranges in (("mma", 9), ("mma", 0), ("tc", 9)):
         with pytest.raises(Error, match="ranges"):
             prefill(q, cache, out, table, _ints([0, 1, 2]), _ints([0, 0]), 1, 0.1, impl, ranges)
     with pytest.raises(Error, match="impl"):
