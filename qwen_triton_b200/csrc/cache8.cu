@@ -25,59 +25,105 @@ struct WriteParams {
     int nq, nkv, d;
 };
 
-__device__ __forceinline__ void load8(float (&v)[8], const float* at, bool wide) {
-    if (wide) {
-        const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = at[i];
-    }
+__device__ __forceinline__ void load4(float* v, const float* at) {
+    const float4 f = *reinterpret_cast<const float4*>(at);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
 }
-__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16* at, bool wide) {
-    if (wide) {
-        const uint4 a = *reinterpret_cast<const uint4*>(at);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-            v[2 * i] = f.x; v[2 * i + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_float(at[i]);
-    }
-}
-__device__ __forceinline__ void store8(float* at, const float (&v)[8]) {
-    *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* at, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&two);
-    }
-    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ void store4(float* at, const float* v) { *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16* at, const float* v) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
-// A row of L lanes, eight neighbouring elements a lane (the lanes from d / 8 on have none): normed where there is a weight, rotated where there are angles.
-// Every lane of the warp calls, rows of a warp may be treated differently, and the exchanges are all lanes' together; `there` says whether this lane has elements.
-template <int L, typename TI>
-__device__ __forceinline__ void treated_row(float (&x)[8], const WriteParams& p, size_t at, int position, const float* weight, bool rotate, bool there) {
-    const int e = (threadIdx.x & (L - 1)) * 8;             // the lane's first element
+// The eight elements of a lane of a row, four from `e0` and four from `e1` on: of halves that turn against each other it has both, so that a rotation needs no
+// exchange and half as many angles as with eight neighbours (prompts of 3,600 tokens of 32 + 8 + 8 heads of 128: 31 us, with neighbours 36).
+struct Place { int e0, e1; bool there; };
+template <int L> __device__ __forceinline__ Place place_of(const WriteParams& p) {
+    const int lane = threadIdx.x & (L - 1), half = p.interleaved ? 0 : p.rotary_dim / 2;
+    Place r;
+    r.e0 = lane < half / 4 ? 4 * lane : 8 * lane;          // 2 half + 8 (lane - half / 4)
+    r.e1 = r.e0 + (lane < half / 4 ? half : 4);
+    r.there = lane < p.d / 8;                              // the others have none
+    return r;
+}
+// A lane's elements of the projection, asked for ahead of their use; zeros where it has none.
+template <typename TI> struct Asked {
+    uint2 words[sizeof(TI)];                               // 4 elements are sizeof(TI) / 2 of them
+    __device__ __forceinline__ void ask(const WriteParams& p, size_t at, const Place& place, bool there) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (there) {
-        load8(x, (const TI*)p.qkv + at + e, p.wide);
-        for (int s = 1; s < p.n_splits; ++s) {
-            float more[8];
-            load8(more, (const TI*)p.qkv + at + e + s * p.split_stride, p.wide);
+        for (int i = 0; i < (int)sizeof(TI); ++i) words[i] = make_uint2(0u, 0u);
+        if (!there) return;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] += more[i];
+        for (int h = 0; h < 2; ++h) {
+            const TI* from = (const TI*)p.qkv + at + (h ? place.e1 : place.e0);
+            if (p.wide) {
+                if constexpr (sizeof(TI) == 2) {
+                    words[h] = *reinterpret_cast<const uint2*>(from);
+                } else {
+                    const uint4 w = *reinterpret_cast<const uint4*>(from);
+                    words[2 * h] = make_uint2(w.x, w.y);
+                    words[2 * h + 1] = make_uint2(w.z, w.w);
+                }
+            } else {
+                TI some[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) some[i] = from[i];
+                memcpy(&words[h * sizeof(TI) / 2], some, sizeof(some));
+            }
         }
     }
+    __device__ __forceinline__ void give(float (&x)[8]) const {
+        TI some[8];
+        memcpy(some, words, sizeof(words));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_float(some[i]);
+    }
+};
+
+struct Head { bool query, value; int index; size_t column; };
+__device__ __forceinline__ Head head_of(const WriteParams& p, int h) {     // keys, values, queries
+    Head r;
+    r.query = h >= 2 * p.nkv;
+    r.value = !r.query && h >= p.nkv;
+    r.index = r.query ? h - 2 * p.nkv : r.value ? h - p.nkv : h;
+    r.column = (size_t)(r.query ? r.index : p.nq + h) * p.d;               // values lie behind the keys
+    return r;
+}
+// The lane's part of a head's norm weight; false for a head that has none.
+__device__ __forceinline__ bool weight_of(float (&w)[8], const WriteParams& p, const Head& head, const Place& place) {
+    const float* weight = head.query ? p.q_weight : head.value ? nullptr : p.k_weight;
+    if (!weight) return false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0.f;
+    if (place.there) {
+        load4(w, weight + place.e0);
+        load4(w + 4, weight + place.e1);
+    }
+    return true;
+}
+// A row of L lanes: the sums of its planes, normed where there is a weight, rotated where there are angles.
+// Every lane of the warp calls, rows of a warp may be treated differently, and the exchanges are all lanes' together; `there` says whether this lane has elements.
+template <int L, typename TI>
+__device__ __forceinline__ void treat_row(float (&x)[8], const Asked<TI>& asked, const WriteParams& p, size_t at, const Place& place, int position, const float (&weight)[8], bool normed,
+                                          bool rotate, bool there) {
+    const int half = p.rotary_dim / 2;
+    const float* angles = p.cos_sin + (size_t)min(position, p.max_pos - 1) * p.rotary_dim;
+    const bool turns = there && rotate && !p.interleaved && place.e0 < half;
+    float c[4], s[4];
+    if (turns) {                                           // on their way while the norm's sum is formed
+        load4(c, angles + place.e0);
+        load4(s, angles + half + place.e0);
+    }
+    asked.give(x);
+    if (there)
+        for (int plane = 1; plane < p.n_splits; ++plane) {
+            Asked<TI> more;
+            float y[8];
+            more.ask(p, at + plane * p.split_stride, place, true);
+            more.give(y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] += y[i];
+        }
     if (p.q_weight || p.k_weight) {                        // the same for all lanes, as what follows it
         float sum = 0.f;
 #pragma unroll
@@ -85,38 +131,27 @@ __device__ __forceinline__ void treated_row(float (&x)[8], const WriteParams& p,
 #pragma unroll
         for (int off = L / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         const float factor = rsqrtf(sum / (float)p.d + p.eps);
-        if (there && weight) {
-            float w[8];
-            load8(w, weight + e, true);
+        if (normed) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * factor * w[i];
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * factor * weight[i];
         }
     }
-    if (p.rotary_dim == 0) return;
-    const int half = p.rotary_dim / 2;
-    const float* angles = p.cos_sin + (size_t)min(position, p.max_pos - 1) * p.rotary_dim;
-    if (p.interleaved) {
-        if (there && rotate) {
+    if (turns) {
 #pragma unroll
-            for (int i = 0; i < 8; i += 2)
-                if (e + i < p.rotary_dim) {
-                    const float c = angles[(e + i) / 2], s = angles[half + (e + i) / 2], a = x[i], b = x[i + 1];
-                    x[i] = a * c - b * s;
-                    x[i + 1] = b * c + a * s;
-                }
+        for (int i = 0; i < 4; ++i) {
+            const float a = x[i], b = x[i + 4];
+            x[i] = a * c[i] - b * s[i];
+            x[i + 4] = b * c[i] + a * s[i];
         }
-    } else {
-        // the other halves of the pairs are half / 8 lanes away
-        const bool first = e < half, turned = e < p.rotary_dim;
-        const int lane = threadIdx.x & 31, from = turned ? lane + (first ? half / 8 : -half / 8) : lane;
-        float other[8], c[8], s[8];
+    } else if (p.interleaved && there && rotate) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], from);
-        if (there && rotate && turned) {
-            load8(c, angles + (first ? e : e - half), true);
-            load8(s, angles + half + (first ? e : e - half), true);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = first ? x[i] * c[i] - other[i] * s[i] : x[i] * c[i] + other[i] * s[i];
+        for (int i = 0; i < 8; i += 2) {
+            const int e = place.e0 + i;                    // eight neighbours
+            if (e < p.rotary_dim) {
+                const float c = angles[e / 2], s = angles[half + e / 2], a = x[i], b = x[i + 1];
+                x[i] = a * c - b * s;
+                x[i + 1] = b * c + a * s;
+            }
         }
     }
 }
@@ -130,50 +165,51 @@ __device__ __forceinline__ float hold(float (&x)[8]) {
     }
     return most;
 }
-__device__ __forceinline__ uint2 pack8(const float (&x)[8], float by) {
-    return make_uint2(pack4(x[0] * by, x[1] * by, x[2] * by, x[3] * by), pack4(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
+__device__ __forceinline__ void write8(uint8_t* row, const Place& place, const float (&x)[8], float by) {
+    *reinterpret_cast<uint32_t*>(row + place.e0) = pack4(x[0] * by, x[1] * by, x[2] * by, x[3] * by);
+    *reinterpret_cast<uint32_t*>(row + place.e1) = pack4(x[4] * by, x[5] * by, x[6] * by, x[7] * by);
 }
 // Eight held numbers under a larger scale.
 __device__ __forceinline__ uint2 smaller8(uint2 w, float by) {
     const float2 a = floats(w.x), b = floats(w.x >> 16), c = floats(w.y), d = floats(w.y >> 16);
     return make_uint2(pack4(a.x * by, a.y * by, b.x * by, b.y * by), pack4(c.x * by, c.y * by, d.x * by, d.y * by));
 }
-struct Head { bool query, value; int index; size_t column; };
-__device__ __forceinline__ Head head_of(const WriteParams& p, int h) {     // keys, values, queries
-    Head r;
-    r.query = h >= 2 * p.nkv;
-    r.value = !r.query && h >= p.nkv;
-    r.index = r.query ? h - 2 * p.nkv : r.value ? h - p.nkv : h;
-    r.column = (size_t)(r.query ? r.index : p.nq + h) * p.d;               // values lie behind the keys
-    return r;
-}
-
 // grid: (2 nkv + nq heads, pages that a sequence's tokens touch, sequences).  A row of L lanes a token; what is to be held stays in registers between
-// the page's largest number and the write.
+// the page's largest number and the write.  Bound by latency and instructions (15 an element): all rows' elements are asked for first, and four blocks an SM
+// (some registers spilled) hide more of it than three (3,600 tokens of 32 + 8 + 8 heads of 128 in bfloat16: 28.5 us, 2.9 TB/s, with three blocks 30.2; asked for row by row 43).
 template <int L, typename TI, typename TO>
-__global__ void __launch_bounds__(THREADS) write_pages_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(THREADS, 4) write_pages_kernel(const WriteParams p) {
     constexpr int ROWS = THREADS / L, ITERS = (PAGE + ROWS - 1) / ROWS;
     __shared__ float most[WARPS];
     pdl_launch_dependents();
     pdl_wait();
-    const int seq = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = (threadIdx.x & (L - 1)) * 8;
+    const int seq = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Place place = place_of<L>(p);
     const int start = p.seq_start[seq], count = p.seq_start[seq + 1] - start, past = p.seq_past[seq];
     const int page_at = past / PAGE + blockIdx.y, low = max(past, page_at * PAGE), high = min(past + count, (page_at + 1) * PAGE);
     if (low >= high) return;
     const Head head = head_of(p, blockIdx.x);
     if (!head.query && page_at >= p.max_blocks) return;
-    const float* weight = head.query ? p.q_weight : head.value ? nullptr : p.k_weight;
+    float weight[8];
+    const bool normed = weight_of(weight, p, head, place);
     const size_t width = (size_t)(p.nq + 2 * p.nkv) * p.d;
     float x[ITERS][8], largest = 0.f;
+    Asked<TI> asked[ITERS];
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int pos = low + i * ROWS + threadIdx.x / L;
+        asked[i].ask(p, (start + min(pos, high - 1) - past) * width + head.column, place, pos < high && place.there);
+    }
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
         const int pos = low + i * ROWS + threadIdx.x / L;
         if (low + i * ROWS >= high) break;                 // the same for the block
-        const bool there = pos < high && e < p.d;
+        const bool there = pos < high && place.there;
         const int token = start + min(pos, high - 1) - past;
-        treated_row<L, TI>(x[i], p, token * width + head.column, pos, weight, !head.value, there);
+        treat_row<L>(x[i], asked[i], p, token * width + head.column, place, pos, weight, normed, !head.value, there);
         if (head.query) {
-            if (there) store8((TO*)p.q_out + ((size_t)token * p.nq + head.index) * p.d + e, x[i]);
+            TO* to = (TO*)p.q_out + ((size_t)token * p.nq + head.index) * p.d;
+            if (there) { store4(to + place.e0, x[i]); store4(to + place.e1, x[i] + 4); }
         } else {
             largest = fmaxf(largest, hold(x[i]));          // lanes without elements hold zeros
         }
@@ -199,7 +235,7 @@ __global__ void __launch_bounds__(THREADS) write_pages_kernel(const WriteParams 
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
         const int pos = low + i * ROWS + threadIdx.x / L;
-        if (pos < high && e < p.d) *reinterpret_cast<uint2*>(block + (size_t)(pos - page_at * PAGE) * p.d + e) = pack8(x[i], inverse);
+        if (pos < high && place.there) write8(block + (size_t)(pos - page_at * PAGE) * p.d, place, x[i], inverse);
     }
 }
 
@@ -209,14 +245,22 @@ __global__ void __launch_bounds__(THREADS) write_tokens_kernel(const WriteParams
     pdl_launch_dependents();
     pdl_wait();
     const int heads = p.nq + 2 * p.nkv, e = (threadIdx.x & (L - 1)) * 8;
+    const Place place = place_of<L>(p);
     const long long row = (long long)blockIdx.x * (THREADS / L) + threadIdx.x / L;
     const int seq = (int)min(row / heads, (long long)p.n_seqs - 1);
     const Head head = head_of(p, (int)(row % heads));
     const int token = p.seq_start[seq], pos = p.seq_past[seq], page_at = pos / PAGE;
     const bool live = row < (long long)p.n_seqs * heads && p.seq_start[seq + 1] > token && (head.query || page_at < p.max_blocks), there = live && e < p.d;
-    float x[8];
-    treated_row<L, TI>(x, p, (size_t)token * heads * p.d + head.column, pos, head.query ? p.q_weight : head.value ? nullptr : p.k_weight, !head.value, there);
-    if (head.query && there) store8((TO*)p.q_out + ((size_t)token * p.nq + head.index) * p.d + e, x);
+    float x[8], weight[8];
+    const bool normed = weight_of(weight, p, head, place);
+    Asked<TI> asked;
+    asked.ask(p, (size_t)token * heads * p.d + head.column, place, there);
+    treat_row<L>(x, asked, p, (size_t)token * heads * p.d + head.column, place, pos, weight, normed, !head.value, there);
+    if (head.query && there) {
+        TO* to = (TO*)p.q_out + ((size_t)token * p.nq + head.index) * p.d;
+        store4(to + place.e0, x);
+        store4(to + place.e1, x + 4);
+    }
     float largest = head.query ? 0.f : hold(x);
 #pragma unroll
     for (int off = L / 2; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
@@ -236,7 +280,7 @@ __global__ void __launch_bounds__(THREADS) write_tokens_kernel(const WriteParams
             uint2* words = reinterpret_cast<uint2*>(block + (size_t)i * p.d + e);
             *words = smaller8(*words, was * inverse);
         }
-    *reinterpret_cast<uint2*>(block + (size_t)first * p.d + e) = pack8(x, inverse);
+    write8(block + (size_t)first * p.d, place, x, inverse);
 }
 
 template <int L, typename TI, typename TO> int launch(const WriteParams& p, int max_q_len, cudaStream_t stream) {
