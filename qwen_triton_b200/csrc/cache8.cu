@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(THREADS, 4) write_pages_kernel(const WritePara
     }
 }
 
-// One token a sequence at most: a row of L lanes a (sequence, head).
+// One token a sequence at most: a row of L lanes a (sequence, head).  Bound by one launch's latency (64 sequences of 32 + 8 + 8 heads of 128: 3.1 us).
 template <int L, typename TI, typename TO>
 __global__ void __launch_bounds__(THREADS) write_tokens_kernel(const WriteParams p) {
     pdl_launch_dependents();

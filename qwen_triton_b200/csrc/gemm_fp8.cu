@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256) quantise_rows_kernel(const T* x, uint8_t*
     }
 }
 
-// A block a weight's block of 128 x 128: the same with one scale for all of it.
+// A block a weight's block of 128 x 128: the same with one scale for all of it.  Once a weight is loaded; it reads it twice (24576 x 4096 from bfloat16: 262 us).
 template <typename T>
 __global__ void __launch_bounds__(256) quantise_weight_kernel(const T* w, uint8_t* values, float* scales, int n, int k) {
     __shared__ float most[8];
@@ -138,43 +138,77 @@ __global__ void __launch_bounds__(256) quantise_weight_kernel(const T* w, uint8_
 }
 
 // ----------------------------------------------------------------------------- the product, any sizes
-// 64 x 64 outputs a block, 4 x 4 a thread, a group of K at a time in shared memory as floats.
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_fp8_any_kernel(const uint8_t* x8, const float* x_scale, const uint8_t* w8, const float* w_scale, T* out, int rows,
-                                                           int n, int k, int groups) {
-    __shared__ float xs[32][65], ws[32][65];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float total[4][4] = {};
-    for (int g = 0; g < groups; ++g) {
-        float part[4][4] = {};
-        for (int k0 = g * GROUP; k0 < min(k, (g + 1) * GROUP); k0 += 32) {
-            for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-                const int r = i >> 5, c = i & 31;
-                xs[c][r] = m0 + r < rows && k0 + c < k ? floats(x8[(size_t)(m0 + r) * k + k0 + c]).x : 0.f;
-                ws[c][r] = n0 + r < n && k0 + c < k ? floats(w8[(size_t)(n0 + r) * k + k0 + c]).x : 0.f;
-            }
-            __syncthreads();
-            for (int c = 0; c < 32; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) part[i][j] = fmaf(xs[c][ty + 16 * i], ws[c][tx + 16 * j], part[i][j]);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (m0 + ty + 16 * i < rows && n0 + tx + 16 * j < n)
-                    total[i][j] = fmaf(part[i][j], x_scale[(size_t)g * rows + m0 + ty + 16 * i] * w_scale[(size_t)((n0 + tx + 16 * j) / GROUP) * groups + g], total[i][j]);
-    }
+// For rows that do not begin where 16 bytes do, which no tensor map describes: 64 x 64 outputs a block, a group of K at a time through shared memory, the next one's words
+// on their way meanwhile.  Eight warps of 16 x 32 outputs bring the numbers to halves (exact) for mma.sync; which element of K a place of a fragment is, is free as
+// long as both operands agree, so a lane's four neighbouring bytes are its two pairs.  Bound by the way of a group's words, which a block has one of at a time (333 rows of
+// 5120 x 8200: 260 us, 8 of 4096 x 4100 54, of 4096 x 4101, byte by byte, 109; on the FMA pipe 2,020 and 428).
+constexpr int ANY = 64, ANY_ROW = GROUP + 16;               // bytes from a row to the next: eight rows' words are all the banks
+constexpr int ANY_WORDS = ANY * GROUP / 4 / 256;            // words of an operand's group that a thread carries
+// Four neighbours of a row from column `c` on; zeros behind its end.
+__device__ __forceinline__ uint32_t four_of(const uint8_t* row, int c, int k, bool words) {
+    if (words) return c < k ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+    uint32_t v = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
+        if (c + i < k) v |= (uint32_t)row[c + i] << (8 * i);
+    return v;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) gemm_fp8_any_kernel(const uint8_t* x8, const float* x_scale, const uint8_t* w8, const float* w_scale, T* out, int rows, int n, int k, int groups,
+                                                           int words) {
+    __shared__ __align__(16) uint8_t xs[ANY * ANY_ROW], ws[ANY * ANY_ROW];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int m0 = blockIdx.y * ANY, n0 = blockIdx.x * ANY, warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    const int row0 = warp % 4 * 16 + g, col0 = warp / 4 * 32;                          // rows row0 and row0 + 8, columns col0 + 8 j + 2 t and the next
+    uint32_t xw[ANY_WORDS], ww[ANY_WORDS];
+    auto fetch = [&](int group) {
+#pragma unroll
+        for (int i = 0; i < ANY_WORDS; ++i) {
+            const int at = threadIdx.x + 256 * i, r = at / (GROUP / 4), c = group * GROUP + at % (GROUP / 4) * 4;
+            xw[i] = m0 + r < rows ? four_of(x8 + (size_t)(m0 + r) * k, c, k, words) : 0u;
+            ww[i] = n0 + r < n ? four_of(w8 + (size_t)(n0 + r) * k, c, k, words) : 0u;
+        }
+    };
+    float total[4][4] = {};
+    fetch(0);
+    for (int group = 0; group < groups; ++group) {
+        __syncthreads();                                    // everybody has read the group before
+#pragma unroll
+        for (int i = 0; i < ANY_WORDS; ++i) {
+            const int at = threadIdx.x + 256 * i, to = at / (GROUP / 4) * ANY_ROW + at % (GROUP / 4) * 4;
+            *reinterpret_cast<uint32_t*>(xs + to) = xw[i];
+            *reinterpret_cast<uint32_t*>(ws + to) = ww[i];
+        }
+        __syncthreads();
+        if (group + 1 < groups) fetch(group + 1);
+        float part[4][4] = {};
+#pragma unroll
+        for (int step = 0; step < GROUP / 16; ++step) {
+            const uint32_t a = *reinterpret_cast<const uint32_t*>(xs + row0 * ANY_ROW + step * 16 + 4 * t), b = *reinterpret_cast<const uint32_t*>(xs + (row0 + 8) * ANY_ROW + step * 16 + 4 * t);
+            const uint32_t a0 = halves(a), a1 = halves(b), a2 = halves(a >> 16), a3 = halves(b >> 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(ws + (col0 + 8 * j + g) * ANY_ROW + step * 16 + 4 * t);
+                asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                             : "+f"(part[j][0]), "+f"(part[j][1]), "+f"(part[j][2]), "+f"(part[j][3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(halves(w)), "r"(halves(w >> 16)));
+            }
+        }
+        const float* scales = x_scale + (size_t)group * rows;
+        const float s0 = m0 + row0 < rows ? scales[m0 + row0] : 0.f, s1 = m0 + row0 + 8 < rows ? scales[m0 + row0 + 8] : 0.f;
+        const float by = w_scale[(size_t)(n0 / GROUP) * groups + group];               // a block's columns are of one scale block
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (m0 + ty + 16 * i < rows && n0 + tx + 16 * j < n) out[(size_t)(m0 + ty + 16 * i) * n + n0 + tx + 16 * j] = from_float<T>(total[i][j]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[j][i] = fmaf(part[j][i], (i < 2 ? s0 : s1) * by, total[j][i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = m0 + row0 + 8 * (i >> 1), c = n0 + col0 + 8 * j + 2 * t + (i & 1);
+            if (m < rows && c < n) out[(size_t)m * n + c] = from_float<T>(total[j][i]);
+        }
 }
 
 // ----------------------------------------------------------------------------- the product on tcgen05
@@ -261,7 +295,8 @@ struct GemmParams {
 // Few rows.  The weight's rows are the instruction's M (a tile is one row of scale blocks), BX rows of x its N; a cluster's blocks take a range of K each and add
 // their sums through distributed shared memory in the order of their ranks.  Warp 0 copies, warp 1 issues, the others add up, a weight row and CW rows of x a
 // thread.  Four accumulators: from the last product of a group to the slot's next one (a commit, two waits, the read) it takes about 1,000 cycles, and a group's
-// products 300.
+// products 300.  Bound by the weight's way from memory and, where it is small, by the latencies of a launch, a ring and a join (8 rows of 4096 x 12288: 14 us, 3.6 TB/s; of
+// 51200 x 5120 50, 5.2 TB/s; one row of 1024 x 2048 4.1).
 // XT: the type of rows that the summing warps bring to 8 bits themselves, straight into shared memory, ahead of their sums (few of them, in up to FUSED_GROUPS groups a
 // block: saves the launch); uint8_t: rows in 8 bits already.
 constexpr int PREFETCH = 16;                                // weight tiles asked into the L2 cache ahead of the wait
@@ -496,8 +531,12 @@ __global__ void __launch_bounds__(Few<BX, XT>::THREADS) gemm_fp8_few_kernel(cons
 
 // Many rows.  128 rows of x are the instruction's M, 256 weight rows its N; eight warps add up, a row of x and 128 weight rows (of one scale block) a thread.  One
 // block an SM walks tiles.  384 threads: warp 0 copies, warp 1 issues, warps 4 to 11 add up and store, with most of the registers: 56 + 224 + 224 = 3 * 168 (without
-// the exchange ten warps have 168 each, of which the sums spill some: 24576 features of 4096 x 4096 450 us in the place of 417).  SPLIT: a cluster a tile, whose blocks take a range of K each and
-// add their sums through distributed shared memory, as for few rows.
+// the exchange ten warps have 168 each, of which the sums spill some: 4096 rows of 24576 x 4096 450 us in the place of 417).  SPLIT: a cluster a tile, whose blocks take
+// a range of K each and add their sums through distributed shared memory, as for few rows.
+//
+// Bound by the operands' way from the L2 cache: a group of a tile is 48 KB for 520 cycles of products and takes 0.57 us, 12.5 TB/s to all SMs (4096 rows of 51200 x 5120:
+// 1,150 us, 1.87 PFLOP/s).  With fewer blocks it takes 0.42 us, the way round of one of the two accumulators: products, commit, eight reads of 16 columns, release.  Tiles of
+// 256 x 256 by pairs of blocks (a third less to fetch) were no faster, their two SMs waiting for each other; reads of 32 columns spill.
 constexpr int BN = 256, PARK_ROW = BN + 4;                  // floats from a row of parked sums to the next: 16 bytes of eight neighbouring rows are all the banks
 constexpr int MANY_THREADS = 384, MANY_STAGES = 4, MANY_SLOTS = 512 / BN, MANY_CW = BN / 2;
 constexpr uint32_t MANY_STAGE_BYTES = A_BYTES + BN * GROUP;
@@ -887,7 +926,7 @@ extern "C" int qt_gemm_fp8(const Fp8Call* call) {
         if (form == 64) return launch_few<64, uint8_t, T>(c.x8, c.w8, p, c.splits, s);
         if (form == 256) return launch_many<T>(c.x8, c.w8, p, c.splits, s);
         launch_kernel(gemm_fp8_any_kernel<T>, dim3((c.n + 63) / 64, (c.rows + 63) / 64), dim3(256), 0, s, (const uint8_t*)c.x8, c.x_scale, (const uint8_t*)c.w8, c.w_scale, (T*)c.out,
-                      c.rows, c.n, c.k, p.groups);
+                      c.rows, c.n, c.k, p.groups, c.k % 4 == 0 && (((uintptr_t)c.x8 | (uintptr_t)c.w8) & 3) == 0);
         QT_CHECK_LAUNCH("gemm_fp8");
         return QT_OK;
     });
