@@ -459,6 +459,64 @@ def test_on_another_stream():
     stream.synchronize()
 
 
+def test_pages_beyond_32_bits():
+    """Pages that begin more than 2^31 and 2^32 bytes into a cache, listed also twice: the results are those of the same contents in a small cache, bit by bit."""
+    from qwen_triton_b200.ops import kernels
+    heads, kv_heads, dim = 16, 8, 128
+    far = 66000                                            # pages of 64 KB: 4.3 GB each of keys and values
+    places = [far - 1, 33000, 3, 65536, 32768]             # of the small cache's pages
+    small, large = kernels.cache8(5, kv_heads, dim, "cuda"), kernels.cache8(far, kv_heads, dim, "cuda")
+    table = torch.tensor([[0, 1, 2, 0], [3, 4, 4, 4]], dtype=torch.int32)
+    moved = torch.tensor(places, dtype=torch.int32)[table.long()]
+    gen = torch.Generator().manual_seed(5)
+    qkv = torch.randn((1, 300, (heads + 2 * kv_heads) * dim), generator=gen).to(BF16).cuda()
+    starts, none = _ints([0, 180, 300]), _ints([0, 0])
+    got = []
+    for cache, pages in ((small, table.cuda()), (large, moved.cuda())):
+        q = torch.empty((300, heads, dim), dtype=BF16, device="cuda")
+        kernels.qkv_write_cache8(kernels.GemmOut(qkv), q, cache, starts, none, pages, 180, None, None, 1e-6, None)
+        one = kernels.GemmOut(qkv[:, :2].contiguous())
+        kernels.qkv_write_cache8(one, q[:2], cache, _ints([0, 1, 2]), _ints([180, 120]), pages, 1, None, None, 1e-6, None)
+        outs = [q]
+        for impl, ranges in (("tc", 1), ("tc", 2), ("mma", 1), ("mma", 3)):
+            outs.append(torch.empty_like(q))
+            kernels.attention_prefill_cache8(q, cache, outs[-1], pages, starts, _ints([70, 100]), 180, 0.1, impl, ranges)
+        for ranges in ((1, 4), (4, 1), (2, 2, False)):
+            plan = kernels.Decode8Plan((2, heads, dim), kv_heads, BF16, *ranges)
+            scratch = [torch.empty(n, device="cuda") for n in (plan.acc_elements, plan.ml_elements)]
+            outs.append(torch.empty((2, heads, dim), dtype=BF16, device="cuda"))
+            kernels.attention_decode_cache8(q[:2].contiguous(), cache, outs[-1], pages, _ints([250, 256]), 0.1, plan, *scratch)
+        got.append(outs)
+    for a, b in zip(*got):
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
+    index = torch.tensor(places, device="cuda")
+    for a, b in ((small.k, large.k), (small.v, large.v)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)[index])
+    assert torch.equal(small.k_scale, large.k_scale[index]) and torch.equal(small.v_scale, large.v_scale[index])
+
+
+def test_two_graphs_that_share_scratch():
+    """Captured calls of other lengths over one cache and one scratch, replayed in turns: each replay's results are its launched call's."""
+    from qwen_triton_b200.ops import kernels
+    cache = _filled(20, 2, 64, 6)
+    tables, lengths = _table([9, 7], 20, 1).cuda(), ([560, 430], [3, 448])
+    q = torch.randn((2, 4, 64), generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+    plan = kernels.Decode8Plan((2, 4, 64), 2, BF16, 9, 1)
+    scratch = [torch.empty(n, device="cuda") for n in (plan.acc_elements, plan.ml_elements)]
+    lens, outs, wants, graphs = [_ints(n) for n in lengths], [], [], []
+    for n in lens:
+        want, out, graph = torch.empty_like(q), torch.empty_like(q), torch.cuda.CUDAGraph()
+        kernels.attention_decode_cache8(q, cache, want, tables, n, 0.1, plan, *scratch)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            kernels.attention_decode_cache8(q, cache, out, tables, n, 0.1, plan, *scratch)
+        outs.append(out), wants.append(want), graphs.append(graph)
+    for turn in range(6):
+        outs[turn % 2].fill_(math.nan)
+        graphs[turn % 2].replay()
+        assert torch.equal(outs[turn % 2], wants[turn % 2])
+
+
 def test_refusals():
     from qwen_triton_b200.ops import kernels
     Error = kernels.KernelError
