@@ -198,6 +198,22 @@ def test_captured_and_on_another_stream():
         assert torch.equal(second, out)
 
 
+@pytest.mark.parametrize("m,n,k", [(600_000, 128, 4096), (45_000, 51_200, 128)])
+def test_offsets_beyond_32_bits(m, n, k):
+    """Rows, and results, of more than 2^31 numbers: those of rows from all over are what these rows give by themselves."""
+    from qwen_triton_b200.ops import kernels
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn((m, k), generator=gen, device="cuda", dtype=torch.bfloat16)
+    weight = kernels.quantise_weight_fp8(torch.randn((n, k), generator=gen, device="cuda", dtype=torch.bfloat16))
+    out, rows = torch.empty((m, n), dtype=torch.bfloat16, device="cuda"), kernels.fp8_rows(m, k, "cuda")
+    kernels.gemm_fp8(x, weight, out, rows, (256, 1))
+    pick = torch.cat((torch.arange(5), torch.tensor([m // 2, 2 ** 31 // max(n, k) - 1, 2 ** 31 // max(n, k) + 1]), torch.arange(m - 60, m))).cuda()
+    few, want = kernels.fp8_rows(len(pick), k, "cuda"), torch.empty((len(pick), n), dtype=torch.bfloat16, device="cuda")
+    kernels.gemm_fp8(x[pick], weight, want, few, (256, 1))
+    assert torch.equal(out[pick], want) and bool(want.isfinite().all())
+    assert torch.equal(rows.values.view(torch.uint8)[pick], few.values.view(torch.uint8)) and torch.equal(rows.scales[:, pick], few.scales)
+
+
 def test_refusals():
     from qwen_triton_b200.ops import kernels
     Error = kernels.KernelError
