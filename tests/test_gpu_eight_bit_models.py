@@ -118,6 +118,23 @@ def test_logits_are_those_of_the_model_in_8_bits(preset, formats):
     assert off(plain_logits8(preset, "fp32", tokens, {}), want) > 1e-3
 
 
+@pytest.mark.parametrize("formats", FORMATS, ids=_names)
+@pytest.mark.parametrize("preset", ["tiny-a", "tiny-b", "tiny-d"])
+def test_logits_in_bfloat16(preset, formats):
+    """Prompts and single tokens.  Here a weight's rows lie otherwise (gate and up in turns), so that its blocks' scales are others: four more roundings a layer,
+    independent of the statement's; and bfloat16 itself, some ten roundings of 2^-9 a layer."""
+    layers = load_preset(preset).num_hidden_layers
+    close = (layers * 11 * 2 * 0.026 ** 2) ** 0.5 + (10 * layers) ** 0.5 * 2 ** -9
+    tokens = random_tokens(preset, 80, 1)
+    want = plain_logits8(preset, "bf16", tokens, formats)
+    engine = engine8(preset, "bf16", formats)
+    assert off(run_whole(engine, tokens), want) < close
+    slot = engine.new_sequence()
+    got = [engine.step([StepEntry(slot, tokens[:60], list(range(60)))]).cpu()]
+    got += [engine.step([StepEntry(slot, [t], [0])]).cpu() for t in tokens[60:]]
+    assert off(torch.cat(got), want) < close
+
+
 @pytest.mark.parametrize("preset", ["tiny-a", "tiny-b", "tiny-d"])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_steps_give_the_logits_of_whole_prompts(preset, dtype):
