@@ -52,23 +52,14 @@ struct Divisor {
         return __fmaf_rn(__fmaf_rn(q, s, -x), -r, q);
     }
 };
-// Rows in 8 bits, scales as [group, row], bound by memory where there are many: a lane 16 columns, eight lanes a group, a warp 512 columns of a row, a block eight
-// rows, whose scales lie side by side.  4096 rows of 12288 in bfloat16: 33 us (4.6 TB/s), where four columns a lane, a warp a group and CUDA's division took 76; 333 of
-// 8192: 3.1 (5.1); 8 of 4096: 1.8 (1.6).
-template <typename T>
-__global__ void __launch_bounds__(256) quantise_rows_wide_kernel(const T* x, uint8_t* values, float* scales, int rows, int k, int groups) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, m = blockIdx.y * 8 + (threadIdx.x >> 5), c0 = blockIdx.x * 512 + lane * 16;
-    if (m >= rows) return;
-    const bool inside = c0 < k;
-    float v[16];
-    const uint4* from = reinterpret_cast<const uint4*>(x + (size_t)m * k + c0);
-    uint4 raw[sizeof(T)];
+// N neighbours that begin at a boundary of 16 bytes.
+template <int N, typename T> __device__ __forceinline__ void load_neighbours(float (&v)[N], const T* at) {
+    constexpr int PIECES = N * (int)sizeof(T) / 16;
+    uint4 raw[PIECES];
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) raw[i] = inside ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < PIECES; ++i) raw[i] = reinterpret_cast<const uint4*>(at)[i];
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) {
+    for (int i = 0; i < PIECES; ++i) {
         const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -80,19 +71,57 @@ __global__ void __launch_bounds__(256) quantise_rows_wide_kernel(const T* x, uin
             }
         }
     }
+}
+// A lane's N columns from c0 on of row m (zeros and not `inside` behind the row's end), GROUP / N lanes a group: every lane of the warp calls.
+template <int N> __device__ __forceinline__ void quantise_neighbours(const float (&v)[N], uint8_t* values, float* scales, int rows, int k, int m, int c0, bool inside) {
     float largest = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) largest = fmaxf(largest, fabsf(v[i]));
+    for (int i = 0; i < N; ++i) largest = fmaxf(largest, fabsf(v[i]));
 #pragma unroll
-    for (int d = 1; d < 8; d *= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, d));
+    for (int d = 1; d < GROUP / N; d *= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, d));
     const float scale = fmaxf(__fmul_rn(largest, PER_TOP), LEAST_SCALE);
     const Divisor over{scale, __frcp_rn(scale), scale > 0x1p-60f && scale < 0x1p60f};
     if (!inside) return;
-    if ((lane & 7) == 0) scales[(size_t)(c0 / GROUP) * rows + m] = scale;
-    uint32_t out[4];
+    if (c0 % GROUP == 0) scales[(size_t)(c0 / GROUP) * rows + m] = scale;
+    uint32_t out[N / 4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = pack4(over(v[4 * i]), over(v[4 * i + 1]), over(v[4 * i + 2]), over(v[4 * i + 3]));
-    *reinterpret_cast<uint4*>(values + (size_t)m * k + c0) = make_uint4(out[0], out[1], out[2], out[3]);
+    for (int i = 0; i < N / 4; ++i) out[i] = pack4(over(v[4 * i]), over(v[4 * i + 1]), over(v[4 * i + 2]), over(v[4 * i + 3]));
+    uint8_t* to = values + (size_t)m * k + c0;
+    if constexpr (N == 16) *reinterpret_cast<uint4*>(to) = make_uint4(out[0], out[1], out[2], out[3]);
+    else *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
+}
+// Rows in 8 bits, scales as [group, row], bound by memory where there are many: a lane 16 columns, eight lanes a group, a warp 512 columns of a row, a block eight
+// rows, whose scales lie side by side.  4096 rows of 12288 in bfloat16: 33 us (4.6 TB/s), where four columns a lane, a warp a group and CUDA's division took 76; 333 of
+// 8192: 3.1 (5.1); 8 of 4096: 1.8 (1.6); with eight columns a lane 41, 3.3 and 1.6.
+template <typename T>
+__global__ void __launch_bounds__(256) quantise_rows_wide_kernel(const T* x, uint8_t* values, float* scales, int rows, int k) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int m = blockIdx.y * 8 + (threadIdx.x >> 5), c0 = blockIdx.x * 512 + (threadIdx.x & 31) * 16;
+    if (m >= rows) return;
+    float v[16] = {};
+    if (c0 < k) load_neighbours(v, x + (size_t)m * k + c0);
+    quantise_neighbours(v, values, scales, rows, k, m, c0, c0 < k);
+}
+// The same of act(gate) * up, rounded to T first as the activation by itself leaves it: of a row of 2 k numbers, gate then up (group 0) or `group` of each in turns.
+// Eight columns a lane: its instructions and exponentials bound it as much as memory (4096 rows of 2 * 12288 in bfloat16 71 us, 3.6 TB/s, where the activation and the rows to
+// 8 bits take 97 in two launches; 8 rows 2.6 and 3.7; with 16 columns a lane 88 and 4.7).
+template <typename T>
+__global__ void __launch_bounds__(256) gated_rows_kernel(const T* gate_up, uint8_t* values, float* scales, int rows, int k, int group, int act, float limit) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int m = blockIdx.y * 8 + (threadIdx.x >> 5), c0 = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
+    if (m >= rows) return;
+    float v[8] = {};
+    if (c0 < k) {
+        float up[8];
+        const T* gate = gate_up + (size_t)m * 2 * k + (group ? (size_t)(c0 / group) * 2 * group + c0 % group : (size_t)c0);
+        load_neighbours(v, gate);
+        load_neighbours(up, gate + (group ? group : k));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_float(from_float<T>(gated_value<sizeof(T) == 2>(v[i], up[i], act, limit)));
+    }
+    quantise_neighbours(v, values, scales, rows, k, m, c0, c0 < k);
 }
 // The same for columns that are no multiple of 16 or rows off 16 bytes: a warp a row and 128 columns.
 template <typename T>
@@ -850,8 +879,7 @@ int quantise_rows(const void* x, int dtype, void* values, float* scales, int row
     const long long blocks = ((long long)rows * groups + 7) / 8;
     if (k % 16 == 0 && (((uintptr_t)x | (uintptr_t)values) & 15) == 0 && rows <= 65535 * 8) {
         return QT_DISPATCH_DTYPE(dtype, "quantise_rows", {
-            launch_kernel(quantise_rows_wide_kernel<T>, dim3((k + 511) / 512, (rows + 7) / 8), dim3(256), 0, stream, (const T*)x, (uint8_t*)values, scales, rows, k,
-                          groups);
+            launch_kernel(quantise_rows_wide_kernel<T>, dim3((k + 511) / 512, (rows + 7) / 8), dim3(256), 0, stream, (const T*)x, (uint8_t*)values, scales, rows, k);
             QT_CHECK_LAUNCH("quantise_rows");
             return QT_OK;
         });
@@ -882,6 +910,20 @@ static_assert(sizeof(Fp8Call) == 8 * 8 + 8 * 4, "8 addresses and 8 numbers of 32
 extern "C" int qt_quantise_rows(const void* x, int dtype, void* values, float* scales, int rows, int k, void* stream) {
     QT_REQUIRE(rows >= 0 && k > 0, "quantise_rows: bad sizes %d x %d", rows, k);
     return rows == 0 ? QT_OK : quantise_rows(x, dtype, values, scales, rows, k, (cudaStream_t)stream);
+}
+
+// gate_up [rows, 2 k] -> act(gate) * up as values [rows, k] e4m3, scales [ceil(k / 128), rows].  `group`: 0, or how many numbers of gate and of up alternate.
+extern "C" int qt_gated_rows(const void* gate_up, int dtype, void* values, float* scales, int rows, int k, int group, int act, float limit, void* stream) {
+    QT_REQUIRE(rows >= 0 && k > 0 && k % 16 == 0 && rows <= 65535 * 8, "gated_rows: %d x %d (columns in steps of 16)", rows, k);
+    QT_REQUIRE(group >= 0 && group % 16 == 0 && (group == 0 || k % group == 0) && ((act >= 0 && act < QT_ACT_COUNT) || act == QT_ACT_CAPPED), "gated_rows: groups of %d of %d, activation %d", group, k, act);
+    QT_REQUIRE((((uintptr_t)gate_up | (uintptr_t)values) & 15) == 0, "gated_rows: operands must be 16-byte aligned");
+    if (rows == 0) return QT_OK;
+    return QT_DISPATCH_DTYPE(dtype, "gated_rows", {
+        launch_kernel(gated_rows_kernel<T>, dim3((k + 255) / 256, (rows + 7) / 8), dim3(256), 0, (cudaStream_t)stream, (const T*)gate_up, (uint8_t*)values, scales, rows, k, group, act,
+                      limit);
+        QT_CHECK_LAUNCH("gated_rows");
+        return QT_OK;
+    });
 }
 
 // w [n, k] -> values [n, k] e4m3, scales [ceil(n / 128), ceil(k / 128)].

@@ -143,6 +143,8 @@ _SIGNATURES = {
     "gemm_fp8": {
         # x, dtype, values, scales, rows, k, stream
         "qt_quantise_rows": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
+        # gate_up, dtype, values, scales, rows, k, group, act, limit, stream
+        "qt_gated_rows": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, ctypes.c_float, _c_ptr],
         "qt_quantise_weight": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
         "qt_gemm_fp8": [ctypes.c_char_p],                     # an Fp8Call (_FP8_CALL)
     },
@@ -1666,6 +1668,20 @@ def quantise_rows_fp8(x: torch.Tensor, rows: Fp8Rows) -> None:
     _need(x, "x", shape=rows.shape)
     _same_device("quantise_rows_fp8", x, rows.values)
     _call("gemm_fp8", "qt_quantise_rows", _ptr(x), _code(x, "x"), _ptr(rows.values), _ptr(rows.scales), *x.shape, _stream())
+
+
+def swiglu_fp8(gate_up: GemmOut, rows: Fp8Rows, group: int = 0, activation: str = "silu", limit: float = 0.0) -> None:
+    """``swiglu`` of one finished plane [1, M, 2 K] (bfloat16 or float32, K a multiple of 16), brought to 8 bits in the same pass: ``rows`` [M, K] get, bit by bit, what
+    ``swiglu`` into a tensor of gate_up's type and ``quantise_rows_fp8`` of that leave."""
+    x = gate_up.tensor
+    m, k = rows.shape
+    if (gate_up.n_splits, gate_up.rows, gate_up.cols) != (1, m, 2 * k):
+        raise KernelError(f"swiglu_fp8: {tuple(x.shape)} for {m} x {k} rows in 8 bits")
+    if k % 16 or group < 0 or group % 16 or (group and k % group):
+        raise KernelError(f"swiglu_fp8: {k} columns in turns of {group}: multiples of 16, and of one another, are required")
+    _same_device("swiglu_fp8", x, rows.values)
+    _call("gemm_fp8", "qt_gated_rows", _ptr(x), _code(x, "gate_up"), _ptr(rows.values), _ptr(rows.scales), m, k, int(group), activation_code(activation, True), float(limit),
+          _stream())
 
 
 def quantise_weight_fp8(weight: torch.Tensor) -> Fp8Weight:

@@ -89,6 +89,9 @@ class GatedMLP:
         act = self.runtime.workspace.view(self.act_buffer, tokens, self.inter)
         if self.takes_scaled_rows and self.gate_up.fusable(tokens):
             self.gate_up.into_swiglu(x, act, self.activation, self.limit, self.gate_bias)
+        elif self.gate_up.eight and not self.biased and self.inter % 16 == 0:
+            act = self.down.rows8(tokens)                 # (the rows of x have been read by then)
+            kernels.swiglu_fp8(self.gate_up(x), act, self.group, self.activation, self.limit)
         elif self.gate_up.eight:
             kernels.swiglu(self.gate_up(x), act, self.group, self.activation, self.limit, self.gate_bias)
         elif self.group and kernels.gemm_uses_pairs(x, self.gate_up.weight):

@@ -251,18 +251,21 @@ class Linear:
         """The number of K ranges that ``rows`` tokens are cut into by the plain products."""
         return next((n for most, n in self.split_plans if rows <= most), 1)
 
-    def _product8(self, x: torch.Tensor, out: torch.Tensor | None) -> GemmOut:
-        rows = x.shape[0]
-        ws = self.runtime.workspace
-        if out is None:
-            out = ws.view(f"{self.key}.out", rows, self.out_features)
-        scratch = self._rows8.get(rows)
-        if scratch is None:
+    def rows8(self, rows: int) -> kernels.Fp8Rows:
+        """Where ``rows`` rows for this product are brought to 8 bits (all products share the place)."""
+        found = self._rows8.get(rows)
+        if found is None:
             if len(self._rows8) >= 64:
                 self._rows8.clear()
-            scratch = self._rows8[rows] = kernels.Fp8Rows(ws.view("fp8.values", rows, self.in_features),
-                                                          ws.view("fp8.scales", -(-self.in_features // kernels.FP8_GROUP), rows))
-        kernels.gemm_fp8(x, self.weight8, out.view(rows, self.out_features), scratch)
+            ws = self.runtime.workspace
+            found = self._rows8[rows] = kernels.Fp8Rows(ws.view("fp8.values", rows, self.in_features), ws.view("fp8.scales", -(-self.in_features // kernels.FP8_GROUP), rows))
+        return found
+
+    def _product8(self, x: "torch.Tensor | kernels.Fp8Rows", out: torch.Tensor | None) -> GemmOut:
+        rows = x.shape[0]
+        if out is None:
+            out = self.runtime.workspace.view(f"{self.key}.out", rows, self.out_features)
+        kernels.gemm_fp8(x, self.weight8, out.view(rows, self.out_features), self.rows8(rows))
         if self.has_bias:
             kernels.add_bias(out.view(rows, self.out_features), self._loaded_bias())
         return GemmOut(out.view(1, rows, self.out_features))

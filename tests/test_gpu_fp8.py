@@ -160,6 +160,38 @@ def test_quotients_next_to_borders(power):
     assert torch.equal(rows.values.cpu().view(torch.uint8), want.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8))
 
 
+@pytest.mark.parametrize("m,k,group", [(1, 16, 0), (3, 160, 16), (9, 512, 16), (130, 528, 0), (17, 1536, 32), (8, 12288, 16)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("activation,limit", [("silu", 0.0), ("capped", 1.5)])
+def test_gated_rows_in_8_bits(m, k, group, dtype, activation, limit):
+    """Bit by bit what the activation and the rows to 8 bits give one after the other; infinities and NaN among them."""
+    from qwen_triton_b200.ops import kernels
+    activation = kernels.CAPPED_GATE if activation == "capped" else activation
+    x = _rows(m, 2 * k, dtype, k + m).cuda() * 3
+    if m > 2:
+        x[1, 5], x[2, k] = math.inf, math.nan
+    gate_up = kernels.GemmOut(x[None])
+    act, want, got = torch.empty((m, k), dtype=dtype, device="cuda"), kernels.fp8_rows(m, k, "cuda"), kernels.fp8_rows(m, k, "cuda")
+    kernels.swiglu(gate_up, act, group, activation, limit)
+    kernels.quantise_rows_fp8(act, want)
+    kernels.swiglu_fp8(gate_up, got, group, activation, limit)
+    assert torch.equal(got.scales.view(torch.int32), want.scales.view(torch.int32))
+    assert torch.equal(got.values.view(torch.uint8), want.values.view(torch.uint8))
+
+
+def test_gated_rows_refusals():
+    from qwen_triton_b200.ops import kernels
+    plane = kernels.GemmOut(torch.zeros((1, 4, 64), dtype=torch.bfloat16, device="cuda"))
+    for rows, group, match in ((kernels.fp8_rows(4, 32, "cuda"), 24, "turns"), (kernels.fp8_rows(4, 48, "cuda"), 0, "for 4 x 48"), (kernels.fp8_rows(3, 32, "cuda"), 0, "for 3 x 32"),
+                               (kernels.fp8_rows(4, 32, "cuda"), -16, "turns")):
+        with pytest.raises(kernels.KernelError, match=match):
+            kernels.swiglu_fp8(plane, rows, group)
+    with pytest.raises(kernels.KernelError):
+        kernels.swiglu_fp8(kernels.GemmOut(torch.zeros((1, 4, 36), dtype=torch.bfloat16, device="cuda")), kernels.fp8_rows(4, 18, "cuda"))
+    with pytest.raises(kernels.KernelError):
+        kernels.swiglu_fp8(kernels.GemmOut(torch.zeros((1, 4, 64), dtype=torch.float16, device="cuda")), kernels.fp8_rows(4, 32, "cuda"))
+
+
 @pytest.mark.parametrize("n,k", [(128, 128), (1, 1), (130, 257), (384, 1024)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_a_weight_in_8_bits(n, k, dtype):
