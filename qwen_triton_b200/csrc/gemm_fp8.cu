@@ -276,9 +276,6 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int* status,
     return true;
 }
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code)); }
-__device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int c_inner, int c_outer) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c_inner), "r"(c_outer) : "memory");
-}
 // float accumulator, e4m3 operands, both K-major
 template <int N> constexpr uint32_t FP8_IDESC = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 
@@ -324,11 +321,10 @@ struct GemmParams {
 // Few rows.  The weight's rows are the instruction's M (a tile is one row of scale blocks), BX rows of x its N; a cluster's blocks take a range of K each and add
 // their sums through distributed shared memory in the order of their ranks.  Warp 0 copies, warp 1 issues, the others add up, a weight row and CW rows of x a
 // thread.  Four accumulators: from the last product of a group to the slot's next one (a commit, two waits, the read) it takes about 1,000 cycles, and a group's
-// products 300.  Bound by the weight's way from memory and, where it is small, by the latencies of a launch, a ring and a join (8 rows of 4096 x 12288: 14 us, 3.6 TB/s; of
-// 51200 x 5120 50, 5.2 TB/s; one row of 1024 x 2048 4.1).
+// products 300.  Bound by the weight's way from memory and, where it is small, by the latencies of a launch, a ring and a join (8 rows of 4096 x 12288: 13.4 us, 3.8 TB/s; of
+// 51200 x 5120 49, 5.3 TB/s; one row of 1024 x 2048 4.1).  The weight asked into the L2 cache ahead of the wait for the kernels before only costs (14.2, 50.5 us).
 // XT: the type of rows that the summing warps bring to 8 bits themselves, straight into shared memory, ahead of their sums (few of them, in up to FUSED_GROUPS groups a
 // block: saves the launch); uint8_t: rows in 8 bits already.
-constexpr int PREFETCH = 16;                                // weight tiles asked into the L2 cache ahead of the wait
 constexpr int CHUNK = 16;                                   // groups whose scales are in shared memory at a time, twice
 constexpr int FEW_SLOTS = 4, FUSED_GROUPS = 2 * CHUNK;
 template <int BX, typename XT> struct Few {
@@ -394,8 +390,6 @@ __global__ void __launch_bounds__(Few<BX, XT>::THREADS) gemm_fp8_few_kernel(cons
 
     if (warp == 0) {
         if (lane == 0) {
-            // while the kernels before this one run, the weight comes as far as the L2 cache (where they may still write it)
-            for (int i = 0; i < min(count, PREFETCH); ++i) prefetch_2d(&map_w, (g_begin + i) * GROUP, w0);
             pdl_wait();
             for (int i = 0; i < count; ++i) {
                 const int s = i % stages;

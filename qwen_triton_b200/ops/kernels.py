@@ -1707,10 +1707,10 @@ FP8_FUSED_UNITS = 16       # most rows times groups a block that a product bring
 def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
     """(form, ranges of K) of the product of ``m`` rows and a weight [n, k]: form 0 takes any sizes, 16 to 64 few rows in tiles of so many, 256 many rows.
 
-    Up to 64 rows read the weight once, in ranges that give up to 256 blocks (8 rows of 6144 x 4096 in 4 / 5 / 6 / 8 ranges: 9.6 / 9.4 / 12.3 / 11.8 us; of 4096 x 12288
-    in 4 / 8: 16.3 / 14.2).  Beyond, the smaller of two times in us, fitted to 30 shapes of 100 to 768 rows: tiles of 64 rows, two blocks an SM, 0.37 to 0.5 a group of
+    Up to 64 rows read the weight once, in ranges that give up to 256 blocks (8 rows of 6144 x 4096 in 4 / 5 / 6 / 8 ranges: 9.3 / 9.4 / 13.5 / 12.3 us; of 4096 x 12288
+    in 4 / 8: 14.3 / 13.4).  Beyond, the smaller of two times in us, fitted to shapes of 77 to 4,096 rows: tiles of 64 rows, two blocks an SM, 0.37 to 0.5 a group of
     K; of 128 x 256, one block an SM, 0.42 to 0.57, which the L2 cache's 12 TB/s to all SMs bounds.  Clusters of ranges over more than 130 SMs do not fit at once
-    (333 rows of 4096 x 12288 in 1 / 2 / 3 ranges: 58 / 39 / 51 us)."""
+    (333 rows of 4096 x 12288 in 1 / 2 / 3 ranges: 51 / 35 / 46 us)."""
     groups, blocks_n = -(-k // FP8_GROUP), -(-n // 128)
     if k % 16:
         return 0, 1
