@@ -36,7 +36,8 @@ class QwenB200ForCausalLM:
     def from_pretrained_hf(cls, model_id: str | Path, backend: str = "b200", device: str | torch.device = "cuda:0",
                            dtype: torch.dtype | str | None = None, **engine_options: Any) -> "QwenB200ForCausalLM":
         """``model_id`` is a local model folder (config.json + safetensors); nothing is downloaded.
-        ``backend`` exists for the reference's signature; the only backend is the sm_100a kernels."""
+        ``backend`` exists for the reference's signature; the only backend is the sm_100a kernels.  ``engine_options``: ``Engine``'s, among them ``max_tokens`` (cache size),
+        ``weight_format="fp8"`` and ``cache_format="fp8"`` (the layers' matrices, keys and values in 8 bits)."""
         if backend not in ("b200", "cuda"):
             raise ValueError(f"backend {backend!r} is not built; this library has one backend, 'b200'")
         if not Path(model_id).exists():

@@ -145,6 +145,8 @@ _SIGNATURES = {
         "qt_quantise_rows": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
         # gate_up, dtype, values, scales, rows, k, group, act, limit, stream
         "qt_gated_rows": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, ctypes.c_float, _c_ptr],
+        # stream_rows, delta, delta_dtype, planes, plane_stride, weight, eps, dtype, values, scales, rows, k, stream
+        "qt_norm_rows": [_c_ptr, _c_ptr, _c_int, _c_int, _c_ll, _c_ptr, ctypes.c_float, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
         "qt_quantise_weight": [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr],
         "qt_gemm_fp8": [ctypes.c_char_p],                     # an Fp8Call (_FP8_CALL)
     },
@@ -1682,6 +1684,26 @@ def swiglu_fp8(gate_up: GemmOut, rows: Fp8Rows, group: int = 0, activation: str 
     _same_device("swiglu_fp8", x, rows.values)
     _call("gemm_fp8", "qt_gated_rows", _ptr(x), _code(x, "gate_up"), _ptr(rows.values), _ptr(rows.scales), m, k, int(group), activation_code(activation, True), float(limit),
           _stream())
+
+
+NORM_ROWS_MOST = 16384        # columns that ``add_rmsnorm_fp8`` takes
+
+
+def add_rmsnorm_fp8(residual: torch.Tensor, delta: GemmOut | None, weight: torch.Tensor, eps: float, rows: Fp8Rows, dtype: torch.dtype = torch.bfloat16) -> None:
+    """``add_rmsnorm`` of every row (stream += delta in place), brought to 8 bits in the same pass: ``rows`` [T, H] are the normed rows, rounded to ``dtype``, as
+    ``quantise_rows_fp8`` defines them.  H is a multiple of 16 up to 16384."""
+    hidden = residual.shape[1]
+    _need(residual, "residual", torch.float32, rows.shape)
+    _need(weight, "weight", torch.float32, (hidden,))
+    if hidden % 16 or hidden > NORM_ROWS_MOST or dtype not in _CODES:
+        raise KernelError(f"add_rmsnorm_fp8: {hidden} columns (in steps of 16 up to {NORM_ROWS_MOST}), {dtype}")
+    if delta is not None:
+        if (delta.rows, delta.cols) != tuple(residual.shape):
+            raise KernelError(f"add_rmsnorm_fp8: delta {tuple(delta.tensor.shape)} does not match the stream {tuple(residual.shape)}")
+        _same_device("add_rmsnorm_fp8", delta.tensor)
+    _same_device("add_rmsnorm_fp8", residual, weight, rows.values)
+    _call("gemm_fp8", "qt_norm_rows", _ptr(residual), _ptr(delta.tensor) if delta else None, _code(delta.tensor, "delta") if delta else F32, delta.n_splits if delta else 0,
+          delta.split_stride if delta else 0, _ptr(weight), float(eps), _CODES[dtype], _ptr(rows.values), _ptr(rows.scales), *residual.shape, _stream())
 
 
 def quantise_weight_fp8(weight: torch.Tensor) -> Fp8Weight:

@@ -181,6 +181,7 @@ class Attention:
             runtime.options.setdefault("shared_attention", set()).add((self.nq, self.nkv, self.d))
         # few tokens: the projection takes rows whose norm factor is still to be applied (``ScaledRows``)
         self.takes_scaled_rows = self.qkv.fused_capable and not self.own_values
+        self.takes_rows8, self.rows8 = eight_weights, self.qkv.rows8
 
     # ------------------------------------------------------------------ weights
     @staticmethod

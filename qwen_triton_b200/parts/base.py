@@ -10,7 +10,8 @@ Interfaces (what a new part must offer):
 * norm:        ``apply(stream, rows=None) -> Tensor``: folds the pending delta into the
   residual stream and returns the normed rows in the activation dtype.  A norm that sets
   ``offers_scaled_rows`` also takes ``lazy=True`` and may then hand on ``ScaledRows`` (the rows times its
-  weight, the rows' factor left to the consumer's product) to a consumer that sets ``takes_scaled_rows``.
+  weight, the rows' factor left to the consumer's product) to a consumer that sets ``takes_scaled_rows``.  A norm that sets ``offers_rows8`` may be
+  called with ``rows8=`` (where to) and hands on rows in 8 bits to a consumer that sets ``takes_rows8``.
 * position:    ``__init__(params, runtime)``, ``table(max_positions) -> float32 [P, rotary_dim]`` (cos | sin) or ``None``
   for no encoding, and ``key() -> tuple`` that names the table's content (equal keys share one table).  Column i
   and rotary_dim / 2 + i of a row are the cos and sin of the angle of rotation pair i; the pair is elements

@@ -74,7 +74,9 @@ class PreNormBlock:
 
     @staticmethod
     def _normed(norm, stream: ResidualStream, consumer):
-        """The consumer's input: ``ScaledRows`` where the norm offers them and the consumer takes them."""
+        """The consumer's input: ``ScaledRows``, or rows in 8 bits, where the norm offers them and the consumer takes them."""
+        if getattr(norm, "offers_rows8", False) and getattr(consumer, "takes_rows8", False):
+            return norm.apply(stream, rows8=consumer.rows8)
         if getattr(norm, "offers_scaled_rows", False) and getattr(consumer, "takes_scaled_rows", False):
             return norm.apply(stream, lazy=True)
         return norm.apply(stream)

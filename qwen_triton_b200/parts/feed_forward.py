@@ -54,6 +54,7 @@ class GatedMLP:
         # few tokens: the gate in the epilogue of the gate/up product, which then also applies the factor of the norm
         # in front of it (``ScaledRows``)
         self.takes_scaled_rows = bool(self.group) and self.gate_up.fused_capable
+        self.takes_rows8, self.rows8 = eight, self.gate_up.rows8
 
     @classmethod
     def expected_tensors(cls, params, prefix: str) -> dict[str, TensorSpec]:

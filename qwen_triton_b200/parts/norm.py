@@ -29,6 +29,7 @@ class RMSNorm:
             raise ValueError(f"{name}: {self.groups} groups do not divide a width of {self.size}")
         # apply(..., lazy=True) may hand on ScaledRows: one factor per row, so only where the row is one group
         self.offers_scaled_rows = self.groups == 1
+        self.offers_rows8 = self.groups == 1 and self.size % 16 == 0 and self.size <= kernels.NORM_ROWS_MOST
         self.tensor = name + str(params.get("suffix", ".weight"))
         self.name = name
         self.runtime = runtime
@@ -60,7 +61,7 @@ class RMSNorm:
             stream.pending = stream.write = None
         return out
 
-    def apply(self, stream: ResidualStream, rows: torch.Tensor | None = None, lazy: bool = False, read: torch.Tensor | None = None):
+    def apply(self, stream: ResidualStream, rows: torch.Tensor | None = None, lazy: bool = False, read: torch.Tensor | None = None, rows8=None):
         """Fold the pending delta into the stream and return the normed rows.
 
         With ``rows`` (int32 row numbers) only those rows are produced and the stream stays as it is.
@@ -70,6 +71,8 @@ class RMSNorm:
         a product that takes ``ScaledRows``) the same launch also prepares this norm: it writes the stream times
         the norm's weight and the rows' sums of squares, and the rows' factor is applied by the consumer's
         epilogue; no norm kernel runs.
+
+        With ``rows8`` (a function of the number of rows; the consumer is a product of rows in 8 bits) the rows are brought to 8 bits in the same launch, where it says.
         """
         ws = self.runtime.workspace
         if stream.more:
@@ -90,6 +93,11 @@ class RMSNorm:
             else:
                 deferred.linear.into_residual(deferred.x, stream.residual)
         count = stream.residual.shape[0] if rows is None else rows.shape[0]
+        if rows8 is not None and rows is None:
+            out = rows8(count)
+            kernels.add_rmsnorm_fp8(stream.residual, stream.pending, self.weight, self.eps, out, self.runtime.dtype)
+            stream.pending = None
+            return out
         out = ws.view("normed", count, self.size)
         kernels.add_rmsnorm(stream.residual, stream.pending, self.weight, self.eps, out, rows, self.groups)
         if rows is None:

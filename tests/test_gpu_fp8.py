@@ -179,6 +179,50 @@ def test_gated_rows_in_8_bits(m, k, group, dtype, activation, limit):
     assert torch.equal(got.values.view(torch.uint8), want.values.view(torch.uint8))
 
 
+@pytest.mark.parametrize("m,k,planes", [(1, 16, 1), (3, 144, 0), (9, 1024, 3), (130, 4096, 1), (5, 8208, 2), (2, 16384, 1), (700, 512, 1)])
+@pytest.mark.parametrize("dtype,delta_type", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32), (torch.float32, torch.bfloat16)])
+def test_normed_rows_in_8_bits(m, k, planes, dtype, delta_type):
+    """The stream with its addition, bit by bit; the rows within their roundings: e4m3's half step, the type's, and float32's in the row's factor (a sum of k squares in
+    a tree: a few 2^-24, counted as 2^-20)."""
+    from qwen_triton_b200.ops import kernels
+    gen = torch.Generator().manual_seed(m + k)
+    stream, weight = torch.randn((m, k), generator=gen) * torch.exp2(torch.randint(-3, 4, (m, 1), generator=gen).float()), 1 + 0.3 * torch.randn(k, generator=gen)
+    delta = torch.randn((planes, m, k), generator=gen).to(delta_type) if planes else None
+    rows, held = kernels.fp8_rows(m, k, "cuda"), stream.cuda()
+    kernels.add_rmsnorm_fp8(held, kernels.GemmOut(delta.cuda()) if planes else None, weight.cuda(), 1e-6, rows, dtype)
+    if planes:
+        total = delta[0].float()
+        for plane in delta[1:]:
+            total = total + plane.float()
+        stream = stream + total
+    assert torch.equal(held.cpu(), stream)
+    x = stream.double()
+    want = x * torch.rsqrt((x * x).mean(1, keepdim=True) + 1e-6) * weight.double()
+    groups = -(-k // 128)
+    most = torch.stack([want[:, g * 128:(g + 1) * 128].abs().amax(1) for g in range(groups)])
+    scales = rows.scales.cpu().double()
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((scales - most / 448).abs() <= most / 448 * (half + 2.0 ** -20)).all())
+    wide = scales.repeat_interleave(128, 0)[:k].T
+    got = rows.values.cpu().view(torch.uint8).view(torch.float8_e4m3fn).double() * wide
+    assert bool(((got - want).abs() <= want.abs() * (2.0 ** -4 + half + 2.0 ** -20) * (1 + 2.0 ** -8) + wide * 2.0 ** -10).all())
+
+
+def test_normed_rows_refusals():
+    from qwen_triton_b200.ops import kernels
+    stream, weight = torch.zeros((4, 32), device="cuda"), torch.ones(32, device="cuda")
+    rows = kernels.fp8_rows(4, 32, "cuda")
+    kernels.add_rmsnorm_fp8(stream, None, weight, 1e-6, rows)
+    assert int(rows.values.view(torch.uint8).max()) == 0
+    for bad in ({"residual": stream[:3]}, {"residual": stream.bfloat16()}, {"weight": weight[:16].contiguous()}, {"delta": kernels.GemmOut(torch.zeros((1, 3, 32), device="cuda"))},
+                {"dtype": torch.float16}, {"rows": kernels.fp8_rows(4, 48, "cuda")}):
+        given = {"residual": stream, "delta": None, "weight": weight, "eps": 1e-6, "rows": rows, **bad}
+        with pytest.raises(kernels.KernelError):
+            kernels.add_rmsnorm_fp8(**given)
+    with pytest.raises(kernels.KernelError, match="24 columns"):
+        kernels.add_rmsnorm_fp8(torch.zeros((4, 24), device="cuda"), None, torch.ones(24, device="cuda"), 1e-6, kernels.fp8_rows(4, 24, "cuda"))
+
+
 def test_gated_rows_refusals():
     from qwen_triton_b200.ops import kernels
     plane = kernels.GemmOut(torch.zeros((1, 4, 64), dtype=torch.bfloat16, device="cuda"))
