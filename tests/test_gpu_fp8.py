@@ -179,7 +179,7 @@ def test_gated_rows_in_8_bits(m, k, group, dtype, activation, limit):
     assert torch.equal(got.values.view(torch.uint8), want.values.view(torch.uint8))
 
 
-@pytest.mark.parametrize("m,k,planes", [(1, 16, 1), (3, 144, 0), (9, 1024, 3), (130, 4096, 1), (5, 8208, 2), (2, 16384, 1), (700, 512, 1)])
+@pytest.mark.parametrize("m,k,planes", [(1, 16, 1), (3, 144, 0), (9, 1024, 3), (130, 4096, 1), (5, 8208, 2), (2, 16384, 1), (700, 512, 1), (600, 2064, 1)])
 @pytest.mark.parametrize("dtype,delta_type", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32), (torch.float32, torch.bfloat16)])
 def test_normed_rows_in_8_bits(m, k, planes, dtype, delta_type):
     """The stream with its addition, bit by bit; the rows within their roundings: e4m3's half step, the type's, and float32's in the row's factor (a sum of k squares in
