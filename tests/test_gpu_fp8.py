@@ -236,7 +236,7 @@ def test_gated_rows_refusals():
         kernels.swiglu_fp8(kernels.GemmOut(torch.zeros((1, 4, 64), dtype=torch.float16, device="cuda")), kernels.fp8_rows(4, 32, "cuda"))
 
 
-@pytest.mark.parametrize("n,k", [(128, 128), (1, 1), (130, 257), (384, 1024)])
+@pytest.mark.parametrize("n,k", [(128, 128), (1, 1), (130, 257), (384, 1024), (1000, 144), (33, 2832)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_a_weight_in_8_bits(n, k, dtype):
     from qwen_triton_b200.ops import kernels
