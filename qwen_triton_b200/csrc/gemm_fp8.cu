@@ -904,7 +904,7 @@ int launch_few(const void* x8, const void* w8, GemmParams p, int splits, cudaStr
     return QT_OK;
 }
 
-template <typename TO> int launch_many(const void* x8, const void* w8, GemmParams p, int splits, cudaStream_t stream) {
+template <typename TO> int launch_many(const void* x8, const void* w8, GemmParams p, int splits, int last, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
     int rc = byte_map(&map_w, w8, p.n, p.k, BN);
     if (rc) return rc;
@@ -929,10 +929,8 @@ template <typename TO> int launch_many(const void* x8, const void* w8, GemmParam
         QT_REQUIRE(splits <= 8 && tiles <= 65535, "gemm_fp8: %d ranges of K for %lld tiles", splits, tiles);
         launch_split(splits, tiles);
     } else {
-        // A last round of few tiles would leave most SMs idle: its tiles are cut into ranges of K in a launch of their own, where that saves more than the launch and the
-        // join take, some 20 groups' time (1512 rows of 6335 x 6800, 300 tiles, 54 groups: 90 us, uncut 104; 1600 of 4096 x 4096, 208 tiles, 32 groups: 38, uncut 37)
-        const int sms = sm_count(), rest = (int)(tiles % sms), most = tiles > sms && rest ? std::min(std::min(8, 130 * sms / 148 / rest), p.groups / 8) : 1;
-        const int ranges = p.groups * (most - 1) > 20 * most ? most : 1;
+        const int sms = sm_count(), rest = (int)(tiles % sms), ranges = tiles > sms && rest ? last : 1;
+        QT_REQUIRE(last >= 1 && last <= 8, "gemm_fp8: %d ranges of K for the last round", last);
         p.groups_per_split = p.groups;
         if (ranges > 1) p.end_tile = (int)tiles - rest;
         launch_kernel(gemm_fp8_many_kernel<false, TO>, dim3((unsigned)std::min<long long>(p.end_tile, sms)), dim3(MANY_THREADS), MANY_SMEM, stream, map_w, map_x, p);
@@ -975,9 +973,9 @@ template <typename XT, typename TO> int launch_fused(const GemmParams& p, const 
 // The arguments of qt_gemm_fp8 as one structure: rows in 8 bits (x8, x_scale), which are made from x first where it is given.
 struct Fp8Call {
     const void* x; void* x8; float* x_scale; const void* w8; const float* w_scale; void* out; int* status; void* stream;
-    int x_dtype, out_dtype, rows, n, k, form, splits, fused;
+    int x_dtype, out_dtype, rows, n, k, form, splits, fused, last, unused;
 };
-static_assert(sizeof(Fp8Call) == 8 * 8 + 8 * 4, "8 addresses and 8 numbers of 32 bits, without gaps");
+static_assert(sizeof(Fp8Call) == 8 * 8 + 10 * 4, "8 addresses and 10 numbers of 32 bits, without gaps");
 
 // x [rows, k] -> values [rows, k] e4m3, scales [ceil(k / 128), rows].
 extern "C" int qt_quantise_rows(const void* x, int dtype, void* values, float* scales, int rows, int k, void* stream) {
@@ -1033,7 +1031,7 @@ extern "C" int qt_quantise_weight(const void* w, int dtype, void* values, float*
 }
 
 // x [rows, k] or null, x8 [rows, k], x_scale [groups, rows], w8 [n, k], w_scale [ceil(n / 128), groups], out [rows, n].  `form`: 0 any sizes; 16, 32, 64: few rows in
-// tiles of so many, 256: many rows, with `splits` ranges of K.  `fused` (form 16, at most 16 rows and 32 groups a range): x is brought to 8 bits on the way, and x8
+// tiles of so many, 256: many rows, with `splits` ranges of K, or, in one range, `last` of them for the tiles of a last round that leaves most SMs idle.  `fused` (form 16, at most 16 rows and 32 groups a range): x is brought to 8 bits on the way, and x8
 // and x_scale stay as they are.
 extern "C" int qt_gemm_fp8(const Fp8Call* call) {
     const Fp8Call& c = *call;
@@ -1061,7 +1059,7 @@ extern "C" int qt_gemm_fp8(const Fp8Call* call) {
         if (form == 16) return launch_few<16, uint8_t, T>(c.x8, c.w8, p, c.splits, s);
         if (form == 32) return launch_few<32, uint8_t, T>(c.x8, c.w8, p, c.splits, s);
         if (form == 64) return launch_few<64, uint8_t, T>(c.x8, c.w8, p, c.splits, s);
-        if (form == 256) return launch_many<T>(c.x8, c.w8, p, c.splits, s);
+        if (form == 256) return launch_many<T>(c.x8, c.w8, p, c.splits, c.last, s);
         launch_kernel(gemm_fp8_any_kernel<T>, dim3((c.n + 63) / 64, (c.rows + 63) / 64), dim3(256), 0, s, (const uint8_t*)c.x8, c.x_scale, (const uint8_t*)c.w8, c.w_scale, (T*)c.out,
                       c.rows, c.n, c.k, p.groups, c.k % 4 == 0 && (((uintptr_t)c.x8 | (uintptr_t)c.w8) & 3) == 0);
         QT_CHECK_LAUNCH("gemm_fp8");

@@ -1753,8 +1753,19 @@ def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
     return best[1:]
 
 
-# x, x8, x_scale, w8, w_scale, out, status, stream, x_dtype, out_dtype, rows, n, k, form, splits, fused: a structure costs the host less than as many arguments
-_FP8_CALL = struct.Struct("@8P8i")
+@functools.lru_cache(maxsize=1024)
+def fp8_last_round(m: int, n: int, k: int, sms: int = 148) -> int:
+    """How many ranges of K the last round of a product in form 256 is cut into, in a launch of its own: a last round of few tiles would leave most SMs idle.  Where that
+    saves more than the launch and the join take, some 20 groups' time (1512 rows of 6335 x 6800, 300 tiles, 54 groups: 90 us, uncut 104; 1600 of 4096 x 4096, 208 tiles,
+    32 groups: 38, uncut 37)."""
+    groups, tiles = -(-k // FP8_GROUP), -(-n // 256) * -(-m // 128)
+    rest = tiles % sms
+    most = min(8, 130 * sms // 148 // rest, groups // 8) if tiles > sms and rest else 1
+    return most if most > 1 and groups * (most - 1) > 20 * most else 1
+
+
+# x, x8, x_scale, w8, w_scale, out, status, stream, x_dtype, out_dtype, rows, n, k, form, splits, fused, last, unused: a structure costs the host less than as many arguments
+_FP8_CALL = struct.Struct("@8P10i")
 
 
 def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None = None, plan: tuple[int, int] | None = None) -> None:
@@ -1777,10 +1788,11 @@ def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, 
     if form not in FP8_FORMS or not 1 <= splits <= 8:
         raise KernelError(f"gemm_fp8: a plan {plan}")
     fused = not given and form == 16 and k % 16 == 0 and m * -(-(-(-k // FP8_GROUP)) // splits) <= FP8_FUSED_UNITS
+    last = fp8_last_round(m, n, k) if form == 256 and splits == 1 else 1
     _call("gemm_fp8", "qt_gemm_fp8",
           _FP8_CALL.pack(0 if given else x.data_ptr(), rows.values.data_ptr(), rows.scales.data_ptr(), w.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
-                         _status_word(out.device).data_ptr(), _stream(), 0 if given else _CODES[x.dtype], _CODES[out.dtype], m, n, k, form, splits, fused),
-          launches=1 if given or fused else 2)
+                         _status_word(out.device).data_ptr(), _stream(), 0 if given else _CODES[x.dtype], _CODES[out.dtype], m, n, k, form, splits, fused, last, 0),
+          launches=(1 if given or fused else 2) + (last > 1))
 
 
 def _check_gemm_fp8(x, weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None, given: bool) -> None:

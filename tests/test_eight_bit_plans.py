@@ -80,3 +80,13 @@ def test_plans_of_prompts(n_seqs, tokens, heads, kv_heads, dim, dtype, pages):
     assert kernels.prefill8_plan(n_seqs, tokens, **shape, on_tc=False)[0] == "mma"
     if dtype == torch.bfloat16 and dim <= 128:
         assert kernels.prefill8_plan(n_seqs, tokens, **shape, on_mma=False)[0] == "tc"
+
+
+@pytest.mark.parametrize("m", [1, 128, 333, 1512, 1600, 4096, 100_000])
+@pytest.mark.parametrize("n,k", [(6335, 6800), (4096, 4096), (51200, 5120), (256, 128), (2568, 1024)])
+def test_last_rounds(m, n, k):
+    """A last round is cut only where there is one behind a full one, into ranges that fit at once."""
+    ranges, tiles = kernels.fp8_last_round(m, n, k), -(-n // 256) * -(-m // 128)
+    assert 1 <= ranges <= 8
+    if ranges > 1:
+        assert tiles > 148 and 0 < tiles % 148 * ranges <= 130 and -(-k // 128) // ranges >= 8

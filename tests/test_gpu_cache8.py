@@ -517,6 +517,23 @@ def test_two_graphs_that_share_scratch():
         assert torch.equal(outs[turn % 2], wants[turn % 2])
 
 
+def test_launches_are_counted():
+    from qwen_triton_b200.ops import kernels
+    from test_gpu_launch_counts import kernels_of
+    cache, table = kernels.cache8(20, 2, 64, "cuda"), _table([9, 7], 20, 1).cuda()
+    q = torch.ones((2, 4, 64), dtype=BF16, device="cuda")
+    out, lens, starts, past = torch.empty_like(q), _ints([500, 400]), _ints([0, 1, 2]), _ints([499, 399])
+    for ranges, launches in (((1, 9), 1), ((4, 3), 1), ((4, 3, False), 2), ((9, 1), 2)):
+        plan = kernels.Decode8Plan((2, 4, 64), 2, BF16, *ranges)
+        scratch = [torch.empty(n, device="cuda") for n in (plan.acc_elements, plan.ml_elements)]
+        assert kernels_of(lambda: kernels.attention_decode_cache8(q, cache, out, table, lens, 0.1, plan, *scratch)) == (launches, launches)
+    for impl, ranges in (("tc", 1), ("tc", 3), ("mma", 1), ("mma", 3)):
+        assert kernels_of(lambda: kernels.attention_prefill_cache8(q, cache, out, table, starts, past, 1, 0.1, impl, ranges)) == (1, 1)
+    qkv = kernels.GemmOut(torch.ones((1, 2, 512), dtype=BF16, device="cuda"))
+    for most in (1, 2):
+        assert kernels_of(lambda: kernels.qkv_write_cache8(qkv, q, cache, starts, past, table, most, None, None, 1e-6, None)) == (1, 1)
+
+
 def test_refusals():
     from qwen_triton_b200.ops import kernels
     Error = kernels.KernelError

@@ -290,6 +290,17 @@ def test_offsets_beyond_32_bits(m, n, k):
     assert torch.equal(rows.values.view(torch.uint8)[pick], few.values.view(torch.uint8)) and torch.equal(rows.scales[:, pick], few.scales)
 
 
+@pytest.mark.parametrize("m,n,k,launches", [(1, 512, 1024, 1), (8, 512, 12288, 2), (333, 512, 1024, 2), (1512, 6335, 6800, 3), (1600, 4096, 4096, 2), (5, 64, 100, 2)])
+def test_launches_are_counted(m, n, k, launches):
+    """Rows brought to 8 bits on the way, by a launch of their own, and the last round of a large product."""
+    from qwen_triton_b200.ops import kernels
+    from test_gpu_launch_counts import kernels_of
+    x, weight = torch.ones((m, k), dtype=torch.bfloat16, device="cuda"), kernels.quantise_weight_fp8(torch.ones((n, k), dtype=torch.bfloat16, device="cuda"))
+    out, rows = torch.empty((m, n), dtype=torch.bfloat16, device="cuda"), kernels.fp8_rows(m, k, "cuda")
+    assert kernels_of(lambda: kernels.gemm_fp8(x, weight, out, rows)) == (launches, launches)
+    assert bool((out.float() - k).abs().max() <= k * 2.0 ** -8)            # 1 / s and s may each be rounded
+
+
 def test_refusals():
     from qwen_triton_b200.ops import kernels
     Error = kernels.KernelError
