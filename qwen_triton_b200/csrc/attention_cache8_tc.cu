@@ -18,10 +18,11 @@
 // Few blocks behind many keys: the pages of a block are cut into ranges for a cluster of up to eight, whose sums meet in distributed shared memory, laid over the
 // operands (256 tokens of 32 heads over 8 of 128 behind 8,000: 149 us in one range, 51 in four; 64 tokens 145 and, in eight, 34).
 //
-// What bounds it: the products of scores with a page's 64 keys, whose time is their queries' way from shared memory (66 cycles for 128 x 64 x 32, of which the
-// tensor cores need 32), 1,650 cycles of the 1,900 that a page takes for 256 rows.  Two pages at a time would halve it, but tensor memory then holds one sum
-// per row and the two threads of a row walk in step: 739 us in the place of 712 for 4,096 tokens behind 8,192, 32 heads over 8 of 128 (965 TFLOP/s; the same over a
-// 16-bit cache, attention_tc.cu, 734).
+// What bounds it: a page of a block takes 1,900 cycles, of which the tensor cores are asked for 1,600: the products of scores run at half their rate, their queries on the way
+// from shared memory (66 cycles for 128 x 64 x 32, of which the tensor cores need 32).  4,096 tokens behind 8,192, 32 heads over 8 of 128: 712-770 us as clocks are, 965-890
+// TFLOP/s; the same over a 16-bit cache, attention_tc.cu, 734.  What was tried on it: two pages at a time, which halve the queries' way, but leave room for one sum a row, so
+// that the two threads of a row walk in step (739 in the place of 712); half of the queries in tensor memory, with scores buffered once (810 in the place of 729, and with
+// heads of 64 695 in the place of 620); an eighth of the exponentials on the FMA pipe (no change, more of them slower).
 #include "cache8_call.h"
 #include "fp8.cuh"
 #include "tc_common.cuh"
