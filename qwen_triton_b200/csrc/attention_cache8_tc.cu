@@ -22,7 +22,8 @@
 // from shared memory (66 cycles for 128 x 64 x 32, of which the tensor cores need 32).  4,096 tokens behind 8,192, 32 heads over 8 of 128: 712-770 us as clocks are, 965-890
 // TFLOP/s; the same over a 16-bit cache, attention_tc.cu, 734.  What was tried on it: two pages at a time, which halve the queries' way, but leave room for one sum a row, so
 // that the two threads of a row walk in step (739 in the place of 712); half of the queries in tensor memory, with scores buffered once (810 in the place of 729, and with
-// heads of 64 695 in the place of 620); an eighth of the exponentials on the FMA pipe (no change, more of them slower).
+// heads of 64 695 in the place of 620); an eighth of the exponentials on the FMA pipe (no change, more of them slower); other orders of the products than a tile's next
+// scores, then its values, tile by tile (both tiles' scores first 785, values first 850, whatever is ready 758).
 #include "cache8_call.h"
 #include "fp8.cuh"
 #include "tc_common.cuh"
