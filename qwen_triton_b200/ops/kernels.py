@@ -1731,8 +1731,8 @@ def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
 
     Up to 64 rows read the weight once, in ranges that give up to 256 blocks (8 rows of 6144 x 4096 in 4 / 5 / 6 / 8 ranges: 9.3 / 9.4 / 13.5 / 12.3 us; of 4096 x 12288
     in 4 / 8: 14.3 / 13.4).  Beyond, the smaller of two times in us, fitted to shapes of 77 to 4,096 rows: tiles of 64 rows, two blocks an SM, 0.37 to 0.5 a group of
-    K; of 128 x 256, one block an SM, 0.42 to 0.57, which the L2 cache's 12 TB/s to all SMs bounds.  Clusters of ranges over more than 130 SMs do not fit at once
-    (333 rows of 4096 x 12288 in 1 / 2 / 3 ranges: 51 / 35 / 46 us)."""
+    K; of 128 x 256, one block an SM, 0.42 to 0.57, which the L2 cache's 12 TB/s to all SMs bounds.  Clusters of three and more over more than 130 SMs do not fit at once
+    (333 rows of 4096 x 12288 in 1 / 2 / 3 ranges, 48 tiles: 51 / 35 / 46 us)."""
     groups, blocks_n = -(-k // FP8_GROUP), -(-n // 128)
     if k % 16:
         return 0, 1
@@ -1740,9 +1740,9 @@ def fp8_plan(m: int, n: int, k: int, sms: int = 148) -> tuple[int, int]:
         return next(t for t in (16, 32, 64) if m <= t), max(1, min(8, groups // 2, 256 * sms // 148 // blocks_n))
     best = None
     for form, tiles in ((64, blocks_n * -(-m // 64)), (256, -(-n // 256) * -(-m // 128))):
-        for splits in range(1, 6 if form == 64 else 7):
+        for splits in range(1, 9):
             blocks, per_split = tiles * splits, -(-groups // splits)
-            if splits > 1 and (blocks > (256 if form == 64 else 130) * sms // 148 or per_split < 2):
+            if splits > 1 and (blocks > (256 if form == 64 else 148 if splits == 2 else 130) * sms // 148 or per_split < 2):
                 break
             if form == 64:
                 cost = 6 + 0.4 * (splits - 1) + per_split * (0.37 if blocks <= sms else 0.5 * -(-blocks // (2 * sms)))
