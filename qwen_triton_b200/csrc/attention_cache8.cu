@@ -11,6 +11,8 @@
 // Every e4m3 number is a half.  Queries are brought to halves with a power of two for each row (its largest element lies in [2^14, 2^15), so no digit
 // of it is lost but below 2^-38 of that); FLOAT queries are two halves, and so is P then.  A weight is p_j s_v[j] relative to the largest such: the running
 // maximum is that of the score plus log2 s_v, so that halves hold the weights whatever scales the pages have; the sum of the p_j takes the scale back out.
+// Weights are held times 2^11, at most 2^15, so that one down to 2^-25 of the largest keeps a half's eleven digits, and what is smaller is off by at most 2^-36 of the
+// largest.  FLOAT: the second half is what the first one leaves, times 2^11 and with sums of its own, so that it too has its digits: 2^-24 of a weight, or 2^-47 of the largest.
 //
 // Ranges of a sequence join in the cluster that they form (up to eight), or through memory and a second launch.
 //
@@ -33,7 +35,9 @@ constexpr int WARPS = 4;
 constexpr int ROWS = 8;                                    // query rows of a block
 constexpr int MAX_CLUSTER = 8, MAX_RANGES = 64;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float RESCALE_STEP = 8.f;                        // a row's maximum moves when the true one is more than 2^8 above it
+constexpr float RESCALE_STEP = 4.f;                        // a row's maximum moves when the true one is more than 2^4 above it
+constexpr float LIFT = 11.f;                               // weights are held times 2^11: halves end at 2^16
+constexpr float REST = 2048.f;                             // FLOAT: and what a half leaves of one times 2^11 again
 
 struct Params {
     const void* q; void* out;
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
     const int limit1 = row0 + 2 * t + 1 <= last_row ? past + (row0 + 2 * t + 1) / group + 1 : 0;
     const int least = past + row0 / group + 1;             // keys below are seen by every row that is there
 
-    float acc[STEPS][4] = {};
+    float acc[STEPS][4] = {}, rest[FLOAT ? STEPS : 1][4] = {};
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     int s_at = 0;
     for (int u = begin; u < stop; u += WARPS) {
@@ -286,10 +290,13 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
             const float a0 = n0 == -INFINITY ? 1.f : fast_exp2(m0 - n0), a1 = n1 == -INFINITY ? 1.f : fast_exp2(m1 - n1);
             l0 *= a0; l1 *= a1;
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) { acc[i][0] *= a0; acc[i][1] *= a1; acc[i][2] *= a0; acc[i][3] *= a1; }
+            for (int i = 0; i < STEPS; ++i) {
+                acc[i][0] *= a0; acc[i][1] *= a1; acc[i][2] *= a0; acc[i][3] *= a1;
+                if (FLOAT) { float (&r)[4] = rest[FLOAT ? i : 0]; r[0] *= a0; r[1] *= a1; r[2] *= a0; r[3] *= a1; }
+            }
             m0 = n0; m1 = n1;
         }
-        const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+        const float u0 = m0 == -INFINITY ? 0.f : m0 - LIFT, u1 = m1 == -INFINITY ? 0.f : m1 - LIFT;
 #pragma unroll
         for (int v = 0; v < SUBS; ++v) {
             const float w0 = fast_exp2(s[v][0] - u0), w1 = fast_exp2(s[v][1] - u1), w2 = fast_exp2(s[v][2] - u0), w3 = fast_exp2(s[v][3] - u1);
@@ -300,8 +307,8 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
             uint32_t r0 = 0, r1 = 0;
             if (FLOAT) {
                 const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h0)), y = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                r0 = transposed(pack_half(w0 - x.x, w1 - x.y));
-                r1 = transposed(pack_half(w2 - y.x, w3 - y.y));
+                r0 = transposed(pack_half((w0 - x.x) * REST, (w1 - x.y) * REST));
+                r1 = transposed(pack_half((w2 - y.x) * REST, (w3 - y.y) * REST));
             }
             const uint8_t* values = stage + R::HALF;
 #pragma unroll
@@ -323,8 +330,8 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
                     mma(acc[8 * c + 2 * w], x0, x1, x2, x3, b0, b1);
                     mma(acc[8 * c + 2 * w + 1], y0, y1, y2, y3, b0, b1);
                     if (FLOAT) {
-                        mma(acc[8 * c + 2 * w], x0, x1, x2, x3, r0, r1);
-                        mma(acc[8 * c + 2 * w + 1], y0, y1, y2, y3, r0, r1);
+                        mma(rest[FLOAT ? 8 * c + 2 * w : 0], x0, x1, x2, x3, r0, r1);
+                        mma(rest[FLOAT ? 8 * c + 2 * w + 1 : 0], y0, y1, y2, y3, r0, r1);
                     }
                 }
             }
@@ -350,6 +357,10 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
     float* own = parts + warp * ROWS * D + g * VBYTES;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {                      // elements 2 i and 2 i + 1 of the lane's
+        if (FLOAT) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(rest[FLOAT ? i : 0][j], 1.f / REST, acc[i][j]);
+        }
         *reinterpret_cast<float2*>(own + (2 * t) * D + 2 * i) = make_float2(acc[i][0], acc[i][2]);
         *reinterpret_cast<float2*>(own + (2 * t + 1) * D + 2 * i) = make_float2(acc[i][1], acc[i][3]);
     }

@@ -8,11 +8,13 @@
 //                    from one shared-memory tile to another, once for the block's 256 rows.  (Both as 8-bit numbers, P in two, would need no conversion of
 //                    values, but P's small weights would end at 2^-18 of the largest, and the conversions of P are more.)
 //
-// A weight is p_j s_v[j] relative to the largest such, as in attention_cache8.cu: the maximum is that of the score plus log2 s_v, and the row's sum takes the scale out.
+// A weight is p_j s_v[j] relative to the largest such, as in attention_cache8.cu: the maximum is that of the score plus log2 s_v, and the row's sum takes the scale out.  Weights are
+// held times 2^11, at most 2^15: one down to 2^-25 of the largest keeps a half's eleven digits, and what is smaller is off by at most 2^-36 of the largest.
 //
 // A block takes 256 rows (query token, head of a kv head's group; a token's heads are neighbours) as two tiles of 128 and walks the keys page by page.  S of a
-// page is double buffered, P lies over the scores it came from, O stays in tensor memory and is scaled only where a row's maximum runs 2^14 ahead of the one it is
-// scaled by (halves end at 2^16; at 2^8, 2 % slower).  512 threads: warp 0 copies (TMA tiles of keys, bulk copies of values), warp 1 issues, warps 4 to 7 convert values, warps 8 to 11 and 12 to 15 are the
+// page is double buffered, P lies over the scores it came from, O stays in tensor memory and is scaled only where a row's maximum runs 2^4 ahead of the one it is
+// scaled by (at 2^14, which leaves the weights no room to be lifted, 758 us in the place of 779 and with heads of 64 153 in the place of 161; but all below 2^-25 of the largest are
+// lost then, however many).  512 threads: warp 0 copies (TMA tiles of keys, bulk copies of values), warp 1 issues, warps 4 to 7 convert values, warps 8 to 11 and 12 to 15 are the
 // softmax of the two tiles, with most of the registers: 88 + 88 + 168 + 168 = 4 * 128.  Every mbarrier wait is bounded and reports through a status word.
 //
 // Few blocks behind many keys: the pages of a block are cut into ranges for a cluster of up to eight, whose sums meet in distributed shared memory, laid over the
@@ -41,7 +43,7 @@ constexpr int BQ = 128, TILES = 2;                         // rows of a tile = t
 constexpr int THREADS = 512;
 constexpr int K_STAGES = 3, RAW_STAGES = 3, V_STAGES = 3;
 constexpr int MAX_RANGES = 8, LEAST_PAGES = 4;              // blocks of a cluster; pages that a block walks before another one has any
-constexpr float RESCALE_STEP = 14.f, LOG2E = 1.4426950408889634f;
+constexpr float RESCALE_STEP = 4.f, LIFT = 11.f, LOG2E = 1.4426950408889634f;       // weights are held times 2^LIFT: 2^15 at most, halves end at 2^16
 
 struct TcParams {
     const __nv_bfloat16* q; __nv_bfloat16* out;
@@ -430,7 +432,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             }
             // P as halves, two keys to a column, over this row's scores (they are in registers)
             uint64_t sum2[2] = {0ull, 0ull};
-            const uint64_t below2 = pair_f32(lift - m_use, lift - m_use);
+            const float below = lift - m_use + LIFT;
+            const uint64_t below2 = pair_f32(below, below);
             uint32_t packed[32];
 #pragma unroll
             for (int q = 0; q < 2; ++q)

@@ -1,0 +1,98 @@
+"""Attention over an 8-bit cache where single numbers decide: weights far below the largest one, and values that are not numbers."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+PAGE = 64
+BF16, F32 = torch.bfloat16, torch.float32
+# What a weight may be off by, relative to itself, and relative to the largest of p_j s_v[j].  A half has 11 binary digits, 2^-12 at most; it ends at 2^-24, off by 2^-25 at
+# most, and weights are held times 2^11 (the largest, whose reference may lag by 2^4, at most 2^15).  Float calls hold the remainder times 2^11 as another half: 2^-24, and 2^-11 of that.
+OF_ITSELF, OF_LARGEST = {BF16: 2.0 ** -12, F32: 2.0 ** -23}, {BF16: 2.0 ** -36, F32: 2.0 ** -47}
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _cache(k8, v8, k_scale, v_scale):
+    """Numbers [tokens, d] of one kv head, a multiple of 64 of them, as pages in order."""
+    from qwen_triton_b200.ops import kernels
+    k8, v8 = (t.float().to(E4M3).view(-1, 1, PAGE, t.shape[1]).cuda() for t in (k8, v8))
+    return kernels.Cache8(k8, v8, k_scale.float().view(-1, 1).cuda(), v_scale.float().view(-1, 1).cuda())
+
+
+def _expected(score, v8, v_scale, dtype):
+    """(out, bound) of one query with these scores.  Here a query has one element that is not zero, so that a score's sum is exact; its scaling and the exponential are off by
+    2^-21 of the score and 2^-21, which meet a result twice; sums over the keys by 2^-23 an addition, at most 200 in turn for a range and the joins, the others within an
+    instruction of eight keys."""
+    p = torch.softmax(score, 0)
+    scale = v_scale.double().repeat_interleave(PAGE)[:, None]
+    sizes = (v8.double() * scale).abs()
+    relative = OF_ITSELF[dtype] + 2 * (float(score[score.isfinite()].abs().max()) + 1) * 2.0 ** -21 + (200 + len(score) / 8) * 2.0 ** -23
+    lost = OF_LARGEST[dtype] * float((p[:, None] * scale).max()) * v8.double().abs().sum(0)
+    out = p @ (v8.double() * scale)
+    return out, relative * (p @ sizes) + lost + out.abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -8)
+
+
+def _far_below(length, dim, at, seed):
+    """One key 18 nats above all others, whose value is 0 in every other element: these are sums of weights between e^-17 and e^-19."""
+    gen = torch.Generator().manual_seed(seed)
+    k8 = torch.randint(-8, 9, (length, dim), generator=gen).double()
+    k8[:, 0] = torch.randint(-8, 9, (length,), generator=gen)
+    k8[at, 0] = 288                                        # 18 under a scale of 2^-4
+    v8 = torch.randint(8, 16, (length, dim), generator=gen).double() * 16
+    v8[at, ::2] = 0
+    pages = length // PAGE
+    return k8, v8, torch.full((pages,), 2.0 ** -4), torch.exp2(torch.randint(-9, -6, (pages,), generator=gen).float())
+
+
+def _beside_large_scale(length, dim, at, seed):
+    """One page whose values are under a scale 2^20 times the others', and 0 in every other element: there the others alone are left."""
+    k8, v8, k_scale, v_scale = _far_below(length, dim, at, seed)
+    k8[at, 0] = 0
+    v8[at // PAGE * PAGE:(at // PAGE + 1) * PAGE, ::2] = 0
+    v_scale[:] = 2.0 ** -8
+    v_scale[at // PAGE] = 2.0 ** 12
+    return k8, v8, k_scale, v_scale
+
+
+@pytest.mark.parametrize("kind", [_far_below, _beside_large_scale])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,ranges", [(128, (1, 1000)), (64, (4, 32)), (128, (16, 8, False)), (256, (2, 64))])
+@pytest.mark.parametrize("at", [3, 4000, 8190])
+def test_decode_of_small_weights(kind, dtype, dim, ranges, at):
+    from qwen_triton_b200.ops import kernels
+    k8, v8, k_scale, v_scale = kind(8192, dim, at, dim + at)
+    cache = _cache(k8, v8, k_scale, v_scale)
+    q = torch.zeros((1, 2, dim), dtype=dtype)
+    q[..., 0] = 1
+    plan = kernels.Decode8Plan((1, 2, dim), 1, dtype, *ranges)
+    out = torch.full_like(q, math.nan, device="cuda")
+    scratch = [torch.full((n,), math.nan, device="cuda") for n in (plan.acc_elements, plan.ml_elements)]
+    kernels.attention_decode_cache8(q.cuda(), cache, out, torch.arange(128, dtype=torch.int32)[None].cuda(), _ints([8192]), 1.0, plan, *scratch)
+    want, bound = _expected(k8[:, 0] / 16, v8, v_scale, dtype)
+    off = (out.double().cpu() - want).abs()
+    assert bool((off <= bound).all()), f"{float((off / bound).max())} of the bound"
+
+
+@pytest.mark.parametrize("kind", [_far_below, _beside_large_scale])
+@pytest.mark.parametrize("impl,dtype,dim", [("mma", BF16, 128), ("mma", F32, 128), ("mma", F32, 256), ("mma", F32, 48), ("tc", BF16, 128), ("tc", BF16, 64), ("tc", BF16, 80)])
+@pytest.mark.parametrize("at,ranges", [(3, 1), (4000, 1), (4000, 4), (8100, 3)])
+def test_prompt_of_small_weights(kind, impl, dtype, dim, at, ranges):
+    from qwen_triton_b200.ops import kernels
+    k8, v8, k_scale, v_scale = kind(8192, dim, at, dim + at)
+    cache = _cache(k8, v8, k_scale, v_scale)
+    count = 50
+    q = torch.zeros((count, 2, dim), dtype=dtype)
+    q[..., 0] = 1
+    out = torch.full_like(q, math.nan, device="cuda")
+    kernels.attention_prefill_cache8(q.cuda(), cache, out, torch.arange(128, dtype=torch.int32)[None].cuda(), _ints([0, count]), _ints([8192 - count]), count, 1.0, impl, ranges)
+    kernels.check_status()
+    for i in range(count):
+        seen = torch.arange(8192) <= 8192 - count + i
+        want, bound = _expected((k8[:, 0] / 16).masked_fill(~seen, -math.inf), v8, v_scale, dtype)
+        off = (out[i].double().cpu() - want).abs()
+        assert bool((off <= bound).all()), f"query {i}: {float((off / bound).max())} of the bound"
