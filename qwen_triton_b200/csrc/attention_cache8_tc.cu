@@ -17,6 +17,9 @@
 // lost then, however many).  512 threads: warp 0 copies (TMA tiles of keys, bulk copies of values), warp 1 issues, warps 4 to 7 convert values, warps 8 to 11 and 12 to 15 are the
 // softmax of the two tiles, with most of the registers: 88 + 88 + 168 + 168 = 4 * 128.  Every mbarrier wait is bounded and reports through a status word.
 //
+// A value that is not a number, in a page that not every row sees, becomes zero as it is converted, and the first key of each element is noted: that element is NaN in the rows
+// that see it, and in no other.
+//
 // Few blocks behind many keys: the pages of a block are cut into ranges for a cluster of up to eight, whose sums meet in distributed shared memory, laid over the
 // operands (256 tokens of 32 heads over 8 of 128 behind 8,000: 149 us in one range, 51 in four; 64 tokens 145 and, in eight, 34).
 //
@@ -146,6 +149,28 @@ __device__ __forceinline__ uint4 load16(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
+// Sixteen values of a key, in shared memory or in registers: NaN become zeros, and the first key of each element is noted.  (Not functions that are called: see `wait`.)
+__device__ __forceinline__ void take_out_nan(uint32_t addr, int* first_nan, int key) {
+#pragma unroll 1
+    for (int b = 0; b < 16; ++b) {
+        uint32_t byte;
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(addr + b) : "memory");
+        if ((byte & 0x7f) != 0x7f) continue;
+        asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr + b), "r"(0) : "memory");
+        atomicMin(first_nan + b, key);
+    }
+}
+__device__ __forceinline__ void take_out_nan(uint4& v, int* first_nan, int key) {
+    uint32_t* words[4] = {&v.x, &v.y, &v.z, &v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll 1
+        for (int b = 0; b < 32; b += 8)
+            if ((*words[k] >> b & 0x7f) == 0x7f) {
+                *words[k] &= ~(0xffu << b);
+                atomicMin(first_nan + 4 * k + b / 8, key);
+            }
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <int HD> struct Shape {
@@ -153,7 +178,8 @@ template <int HD> struct Shape {
     static constexpr uint32_t PAGE_BYTES = PAGE * HD, V_BYTES = 2 * PAGE_BYTES, V_BLOCK = PAGE * 128;
     static constexpr uint32_t Q0 = 0, K0 = TILES * Q_TILE, V0 = K0 + K_STAGES * PAGE_BYTES, RAW0 = V0 + V_STAGES * V_BYTES, BARS = RAW0 + RAW_STAGES * PAGE_BYTES;
     static constexpr int N_BARS = TILES + 2 * K_STAGES + 2 * RAW_STAGES + 2 * V_STAGES + 3 * 2 * TILES;
-    static constexpr size_t SMEM = BARS + 8 * N_BARS + 16 + 1024;
+    static constexpr uint32_t NANS = BARS + 8 * N_BARS + 16;          // of each element, the first key taken out; whether there is one at all
+    static constexpr size_t SMEM = NANS + 4 * HD + 16 + 1024;
     // SPLIT: a block's sums, over everything before the barriers; rows begin four banks apart
     static constexpr int PARK_ROW = HD + 4;
     static constexpr uint32_t PARK_ML = TILES * BQ * PARK_ROW * 4;
@@ -201,6 +227,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
     const uint32_t q_full = bars, k_full = q_full + 8 * TILES, k_empty = k_full + 8 * K_STAGES, raw_full = k_empty + 8 * K_STAGES, raw_empty = raw_full + 8 * RAW_STAGES;
     const uint32_t v_full = raw_empty + 8 * RAW_STAGES, v_empty = v_full + 8 * V_STAGES, s_full = v_empty + 8 * V_STAGES, p_full = s_full + 16 * TILES, pv_full = p_full + 16 * TILES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (base - raw) + S::BARS + 8 * S::N_BARS);
+    int* first_nan = reinterpret_cast<int*>(smem_raw + (base - raw) + S::NANS);
+    volatile int* some_nan = first_nan + HD;
+    for (int i = threadIdx.x; i <= HD; i += THREADS) first_nan[i] = i < HD ? 0x7fffffff : 0;
     int* status = p.status;
     if (threadIdx.x == 0) {
         prefetch_tensor_map(&map_k);
@@ -299,6 +328,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             keys[i] = (thread + i * 128) / pieces;         // PAGE or more: none
             columns[i] = (thread + i * 128) % pieces;
         }
+        const int all_see = past + row0 / group + 1;       // keys that every row sees
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
             const int rs = j % RAW_STAGES, vs = j % V_STAGES;
@@ -307,9 +337,31 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             uint4 v[EACH];
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
+                if (!FULL) v[i] = make_uint4(0, 0, 0, 0);
                 if (!FULL && keys[i] >= PAGE) continue;
                 v[i] = load16(base + S::RAW0 + rs * S::PAGE_BYTES + (thread + i * 128) * 16);
                 if ((page0 + j) * PAGE + keys[i] >= end) v[i] = make_uint4(0, 0, 0, 0);       // behind the last key lies anything, NaN too
+            }
+            if ((page0 + j) * PAGE + PAGE > all_see) {
+                // FULL: piece by piece, through shared memory; the others: all at once, in registers.  What never runs decides how the rest is scheduled: 4,096 tokens of heads of
+                // 128 take 752 us so, the other way 821; 2 x 2,000 of heads of 96 take 94 us, the other way 107.
+                uint32_t some = 0;
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) {
+                    const uint32_t here = any_nan(v[i].x) | any_nan(v[i].y) | any_nan(v[i].z) | any_nan(v[i].w);
+                    some |= here;
+                    if (FULL && here) {
+                        const uint32_t at = base + S::RAW0 + rs * S::PAGE_BYTES + (thread + i * 128) * 16;
+                        take_out_nan(at, first_nan + 16 * columns[i], (page0 + j) * PAGE + keys[i]);
+                        v[i] = load16(at);
+                        *some_nan = 1;
+                    }
+                }
+                if (!FULL && some) {
+#pragma unroll
+                    for (int i = 0; i < EACH; ++i) take_out_nan(v[i], first_nan + 16 * columns[i], (page0 + j) * PAGE + keys[i]);
+                    *some_nan = 1;
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(raw_empty + 8 * rs);
@@ -457,6 +509,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             m_run = m_new;
         }
         const int last = my_tiles - 1;
+        // the elements of this row that a value which is no number reaches
+        auto hand_on_nan = [&](uint32_t (&o)[32], int c0) {
+            if (*some_nan)
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    if (first_nan[c0 + c] <= qpos) o[c] = 0x7fffffffu;
+        };
         const bool done = last >= 0 && ok && wait_warp(pv_full + 8 * (2 * t + (last & 1)), (uint32_t)(last >> 1) & 1u, status, 3);
         if (SPLIT) asm volatile("bar.sync 1, 256;" ::: "memory");      // both tiles' products are complete: the operands' place is free
         if (SPLIT) {
@@ -470,6 +529,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
                 uint32_t o[32];
                 if (done) {
                     tmem_load32(lane_addr + O_COL + (uint32_t)(t * HD + c0), o);
+                    hand_on_nan(o, c0);
                 } else {
 #pragma unroll
                     for (int c = 0; c < 32; ++c) o[c] = 0u;
@@ -486,6 +546,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_cache8_tc_kernel(const _
             for (int c0 = 0; c0 < d; c0 += 32) {
                 uint32_t o[32];
                 tmem_load32(lane_addr + O_COL + (uint32_t)(t * HD + c0), o);
+                hand_on_nan(o, c0);
                 if (r < my_rows) {
 #pragma unroll
                     for (int c = 0; c < 32; c += 8) {

@@ -27,6 +27,8 @@ __device__ __forceinline__ float2 floats(uint32_t two) {
     const uint32_t v = halves(two);
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
+// Whether one of four numbers is NaN: all bits but the sign are set.
+__device__ __forceinline__ uint32_t any_nan(uint32_t four) { return ((four & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 // An infinity is held as NaN: 448 would be a number.
 __device__ __forceinline__ float nan_if_infinite(float v) { return fabsf(v) < INFINITY ? v : __int_as_float(0x7fffffff); }
 

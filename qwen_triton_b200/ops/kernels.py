@@ -2076,7 +2076,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     ``impl``: "tc" (tcgen05: bfloat16 heads up to 128 under a positive scale, 256 rows a block) or "mma" (any call, eight rows a block), whose keys are walked by a cluster
     of ``ranges`` blocks, up to eight; the default is ``prefill8_plan``'s choice, by ``max_context``, the most keys that a sequence has (any number gives right
     results; without it what ``block_table`` has room for).  A value
-    that is not a number makes the results of the queries that see it NaN, and may make those of earlier queries of the call that read its page."""
+    that is not a number makes its element NaN in the results of the queries that see it, a key that is not one all their elements; earlier queries of the call are as without."""
     n_seqs, device, k = seq_past.shape[0], _current_device(), cache.k
     # one expression for a call that is in order
     if not (q.dim() == 3 and q.shape == out.shape and q.dtype is out.dtype and q.dtype in _CODES and q.shape[2] == k.shape[3] and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0

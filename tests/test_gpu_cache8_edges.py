@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+import plain_8bit as plain
+
 pytestmark = pytest.mark.gpu
 E4M3 = torch.float8_e4m3fn
 PAGE = 64
@@ -96,3 +98,58 @@ def test_prompt_of_small_weights(kind, impl, dtype, dim, at, ranges):
         want, bound = _expected((k8[:, 0] / 16).masked_fill(~seen, -math.inf), v8, v_scale, dtype)
         off = (out[i].double().cpu() - want).abs()
         assert bool((off <= bound).all()), f"query {i}: {float((off / bound).max())} of the bound"
+
+
+# (key, element) of the values that are not numbers, in a prompt of 150 tokens behind 100: in the earlier tokens, at a page's first and last place, several in one element, the last
+# token's; and what lies behind the last token
+NANS = [[(40, 3)], [(100, 0), (100, 17)], [(127, 5), (128, 6)], [(249, 15)], [(130, 2), (200, 2), (201, 9)], [(250, 1), (255, 8)], []]
+
+
+@pytest.mark.parametrize("impl,dtype,dim,heads", [("tc", BF16, 128, 4), ("tc", BF16, 64, 2), ("tc", BF16, 48, 6), ("mma", BF16, 128, 4), ("mma", BF16, 64, 6), ("mma", F32, 128, 2),
+                                                  ("mma", F32, 256, 2), ("mma", BF16, 16, 16)])
+@pytest.mark.parametrize("ranges", [1, 2, 3])
+@pytest.mark.parametrize("sign", [0x7f, 0xff])
+def test_a_value_that_is_no_number_reaches_its_element_of_the_queries_that_see_it(impl, dtype, dim, heads, ranges, sign):
+    """One sequence for each of NANS, in one call; kv head 1 of two has the NaN."""
+    from qwen_triton_b200.ops import kernels
+    count, past, pages = 150, 100, 4
+    gen = torch.Generator().manual_seed(dim)
+    n = len(NANS)
+    k8, v8 = ((torch.randn((n * pages, 2, PAGE, dim), generator=gen) * 90).clamp(-448, 448).to(E4M3).cuda() for _ in range(2))
+    held = [t.view(torch.uint8).cpu().view(E4M3).double() * 2.0 ** -7 for t in (k8, v8)]
+    for i, places in enumerate(NANS):
+        for key, element in places:
+            v8.view(torch.uint8)[i * pages + key // PAGE, 1, key % PAGE, element % dim] = sign
+    cache = kernels.Cache8(k8, v8, *(torch.full((n * pages, 2), 2.0 ** -7, device="cuda") for _ in range(2)))
+    table = torch.arange(n * pages, dtype=torch.int32).view(n, pages)
+    q = torch.randn((n * count, heads, dim), generator=gen).to(dtype)
+    out = torch.zeros_like(q, device="cuda")
+    kernels.attention_prefill_cache8(q.cuda(), cache, out, table.cuda(), _ints([count * i for i in range(n + 1)]), _ints([past] * n), count, dim ** -0.5, impl, ranges)
+    kernels.check_status()
+    want, bound = plain.attention(q, *held, table, [count] * n, [past] * n, dim ** -0.5, 11 if dtype == BF16 else 20, impl == "tc")
+    bound = bound + want.abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -8) + 1e-30
+    nan = torch.zeros_like(want, dtype=torch.bool).view(n, count, heads, dim)
+    for i, places in enumerate(NANS):
+        for key, element in places:
+            nan[i, max(0, key - past):, heads // 2:, element % dim] = True
+    nan = nan.view_as(want)
+    out = out.double().cpu()
+    assert torch.equal(out.isnan(), nan)
+    off = (out - want).abs()[~nan]
+    assert bool((off <= bound[~nan]).all()), f"{float((off / bound[~nan]).max())} of the bound"
+
+
+@pytest.mark.parametrize("impl,dtype", [("tc", BF16), ("mma", BF16), ("mma", F32)])
+def test_a_key_that_is_no_number_reaches_the_queries_that_see_it(impl, dtype):
+    from qwen_triton_b200.ops import kernels
+    count, past = 100, 30
+    gen = torch.Generator().manual_seed(1)
+    k8, v8 = ((torch.randn((3, 1, PAGE, 64), generator=gen) * 90).clamp(-448, 448).to(E4M3).cuda() for _ in range(2))
+    cache = kernels.Cache8(k8, v8, *(torch.full((3, 1), 2.0 ** -7, device="cuda") for _ in range(2)))
+    q = torch.randn((count, 2, 64), generator=gen).to(dtype).cuda()
+    args = (_ints([[0, 1, 2]]), _ints([0, count]), _ints([past]), count, 0.125, impl)
+    without, out = torch.empty_like(q), torch.empty_like(q)
+    kernels.attention_prefill_cache8(q, cache, without, *args)
+    k8.view(torch.uint8)[1, 0, 16, 5] = 0x7f               # key 80, token 50
+    kernels.attention_prefill_cache8(q, cache, out, *args)
+    assert torch.equal(out[:50], without[:50]) and bool(out[50:].isnan().all()) and bool(without.isfinite().all())
