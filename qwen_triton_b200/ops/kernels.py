@@ -2066,6 +2066,13 @@ def prefill8_plan(n_seqs: int, max_q_len: int, *, num_heads: int, num_kv_heads: 
 
 
 _LEAST_PAGES = 4         # what a block on tcgen05 walks before another of its cluster has any
+_TC_PAGE_HEADS, _TC_ROW_BLOCKS = (2 ** 31 - 1) // 64, 65535        # rows of keys that a tensor map's coordinate reaches; blocks of 256 rows along a grid's second axis
+
+
+def prefill8_tc_takes(dtype: torch.dtype, head_dim: int, scale: float, page_heads: int, rows: int) -> bool:
+    """Whether ``attention_prefill_cache8`` can run on tcgen05: bfloat16 heads up to 128 under a positive scale, ``page_heads`` pages times kv heads in the cache, and up to
+    ``rows`` tokens times heads of a kv head in a sequence."""
+    return dtype is torch.bfloat16 and head_dim <= 128 and scale > 0 and page_heads <= _TC_PAGE_HEADS and -(-rows // 256) <= _TC_ROW_BLOCKS
 
 
 def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, block_table: torch.Tensor, seq_start: torch.Tensor, seq_past: torch.Tensor,
@@ -2073,7 +2080,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     """``attention_prefill`` over a cache in 8 bits: packed queries [T, nq, d], sequence i's from ``seq_start[i]`` on (at most ``max_q_len``), behind ``seq_past[i]`` earlier
     tokens; the cache already holds this step's keys; a query sees the keys up to its own.
 
-    ``impl``: "tc" (tcgen05: bfloat16 heads up to 128 under a positive scale, 256 rows a block) or "mma" (any call, eight rows a block), whose keys are walked by a cluster
+    ``impl``: "tc" (tcgen05: bfloat16 heads up to 128 under a positive scale, sizes up to ``prefill8_tc_takes``', 256 rows a block) or "mma" (any call, eight rows a block), whose keys are walked by a cluster
     of ``ranges`` blocks, up to eight; the default is ``prefill8_plan``'s choice, by ``max_context``, the most keys that a sequence has (any number gives right
     results; without it what ``block_table`` has room for).  A value
     that is not a number makes its element NaN in the results of the queries that see it, a key that is not one all their elements; earlier queries of the call are as without."""
@@ -2085,9 +2092,10 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
             and q.is_contiguous() and out.is_contiguous() and block_table.is_contiguous() and seq_start.is_contiguous() and seq_past.is_contiguous()
             and q.get_device() == out.get_device() == k.get_device() == block_table.get_device() == seq_start.get_device() == seq_past.get_device() == device):
         _check_prefill_cache8(q, cache, out, block_table, seq_start, seq_past, max_q_len)
-    on_tc = q.dtype is torch.bfloat16 and k.shape[3] <= 128 and scale > 0
+    on_tc = prefill8_tc_takes(q.dtype, k.shape[3], scale, k.shape[0] * k.shape[1], max_q_len * (q.shape[1] // k.shape[1]))
     if impl not in (None, "tc", "mma") or (impl == "tc" and not on_tc):
-        raise KernelError(f"attention_prefill_cache8: impl={impl!r} for {q.dtype}, heads of {k.shape[3]}, a scale of {scale}")
+        raise KernelError(f"attention_prefill_cache8: impl={impl!r} for {q.dtype}, heads of {k.shape[3]}, a scale of {scale}, {k.shape[0]} pages of {k.shape[1]} heads, "
+                          f"{max_q_len} tokens of {q.shape[1]} heads")
     if ranges is not None and not 1 <= ranges <= _CLUSTER_RANGES:
         raise KernelError(f"attention_prefill_cache8: {ranges} ranges")
     if ranges is None or impl is None:

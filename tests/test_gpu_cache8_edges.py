@@ -153,3 +153,29 @@ def test_a_key_that_is_no_number_reaches_the_queries_that_see_it(impl, dtype):
     k8.view(torch.uint8)[1, 0, 16, 5] = 0x7f               # key 80, token 50
     kernels.attention_prefill_cache8(q, cache, out, *args)
     assert torch.equal(out[:50], without[:50]) and bool(out[50:].isnan().all()) and bool(without.isfinite().all())
+
+
+def test_sizes_beyond_what_tcgen05_takes_go_to_the_other_form(monkeypatch):
+    """The limits made small: the default takes the form that has none, and a call that asks for tcgen05 is refused."""
+    from qwen_triton_b200.ops import kernels
+    gen = torch.Generator().manual_seed(2)
+    k8, v8 = ((torch.randn((5, 2, PAGE, 64), generator=gen) * 90).clamp(-448, 448).to(E4M3).cuda() for _ in range(2))
+    cache = kernels.Cache8(k8, v8, *(torch.full((5, 2), 2.0 ** -7, device="cuda") for _ in range(2)))
+    q = torch.randn((300, 4, 64), generator=gen).to(BF16).cuda()
+    args = (_ints([[0, 1, 2, 3, 4]]), _ints([0, 300]), _ints([20]), 300, 0.125)
+
+    def call(impl):
+        out = torch.empty_like(q)
+        kernels.attention_prefill_cache8(q, cache, out, *args, impl)
+        return out
+
+    want, tc = call("mma"), call("tc")
+    assert not torch.equal(want, tc)                       # what follows tells the forms apart
+    monkeypatch.setattr(kernels, "prefill8_plan", lambda *a, on_tc, on_mma, **sizes: ("tc", 1) if on_tc else ("mma", 1))
+    assert torch.equal(call(None), tc)
+    for name, limit in (("_TC_PAGE_HEADS", 9), ("_TC_ROW_BLOCKS", 2)):
+        with monkeypatch.context() as limits:
+            limits.setattr(kernels, name, limit)
+            assert torch.equal(call(None), want)
+            with pytest.raises(kernels.KernelError, match="impl='tc'"):
+                call("tc")
