@@ -1784,11 +1784,12 @@ def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, 
             and rows.values.shape[1] == k and rows.values.shape[0] >= m and (given or (x.dtype in _CODES and x.is_contiguous()))
             and values.get_device() == out.get_device() == w.get_device() == rows.values.get_device() == device):
         _check_gemm_fp8(x, weight, out, scratch, given)
-    form, splits = plan or fp8_plan(m, n, k)
+    sms = _SM_COUNTS.get(device) or sm_count()
+    form, splits = plan or fp8_plan(m, n, k, sms)
     if form not in FP8_FORMS or not 1 <= splits <= 8:
         raise KernelError(f"gemm_fp8: a plan {plan}")
     fused = not given and form == 16 and k % 16 == 0 and m * -(-(-(-k // FP8_GROUP)) // splits) <= FP8_FUSED_UNITS
-    last = fp8_last_round(m, n, k) if form == 256 and splits == 1 else 1
+    last = fp8_last_round(m, n, k, sms) if form == 256 and splits == 1 else 1
     _call("gemm_fp8", "qt_gemm_fp8",
           _FP8_CALL.pack(0 if given else x.data_ptr(), rows.values.data_ptr(), rows.scales.data_ptr(), w.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
                          _status_word(out.device).data_ptr(), _stream(), 0 if given else _CODES[x.dtype], _CODES[out.dtype], m, n, k, form, splits, fused, last, 0),
@@ -2101,7 +2102,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     if ranges is None or impl is None:
         pages = block_table.shape[1] if max_context is None else max(1, min(block_table.shape[1], -(-max_context // 64)))
         impl, chosen = prefill8_plan(n_seqs, max_q_len, num_heads=q.shape[1], num_kv_heads=k.shape[1], head_dim=k.shape[3], dtype=q.dtype, max_pages=pages,
-                                     on_tc=on_tc and impl != "mma", on_mma=impl != "tc")
+                                     on_tc=on_tc and impl != "mma", on_mma=impl != "tc", sms=_SM_COUNTS.get(device) or sm_count())
         ranges = ranges or chosen
     on_tc = impl == "tc"
     _call(*(("attention_cache8_tc", "qt_attention_prefill_cache8_tc") if on_tc else ("attention_cache8", "qt_attention_prefill_cache8")),
