@@ -63,6 +63,8 @@ def check_formats(spec: ModelSpec, weight_format: str | None, cache_format: str 
         for layer in spec.layers:
             if layer.block.kind != "pre_norm" or layer.mixer.kind != "attention" or layer.feed_forward is None or layer.feed_forward.kind != "gated_mlp":
                 raise ValueError(f"{name}='fp8' is for models of dense attention and gated feed-forwards; {layer.prefix} of {spec.architecture} is another layer")
+    if cache_format is not None and any(call.cache_of is not None for call in spec.schedule):
+        raise ValueError("cache_format='fp8' is for models whose every layer call writes keys and values of its own; a call of this one reads another's")
     return formats
 
 
