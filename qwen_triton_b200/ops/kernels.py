@@ -1778,7 +1778,7 @@ def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, 
     n, k = w.shape
     rows = x if given else scratch
     values = x.values if given else x
-    m, device = values.shape[0], _current_device()
+    m, device = values.shape[0] if values.dim() else 0, _current_device()
     # one expression for a call that is in order: the host's part of a short product is its time
     if not (values.dim() == 2 and values.shape[1] == k and out.shape == (m, n) and out.is_contiguous() and out.dtype in _CODES and rows is not None
             and rows.values.shape[1] == k and rows.values.shape[0] >= m and (given or (x.dtype in _CODES and x.is_contiguous()))
@@ -1799,7 +1799,7 @@ def gemm_fp8(x: "torch.Tensor | Fp8Rows", weight: Fp8Weight, out: torch.Tensor, 
 def _check_gemm_fp8(x, weight: Fp8Weight, out: torch.Tensor, scratch: Fp8Rows | None, given: bool) -> None:
     """The refusal of a call that is not in order."""
     n, k = weight.shape
-    m = x.shape[0]
+    m = x.shape[0] if given or x.dim() else 0
     if given:
         if x.shape[1] != k:
             raise KernelError(f"gemm_fp8: rows {tuple(x.shape)} for a weight {tuple(weight.shape)}")
@@ -1868,8 +1868,8 @@ def qkv_write_cache8(qkv: GemmOut, q_out: torch.Tensor, cache: Cache8, seq_start
     once, and beyond 448 * 2^40 end there.  e starts with the write of a page's first place and then only grows: what the page's earlier places hold is then brought
     under the larger scale (exact but for numbers below 2^-6 of it).  Infinities are held as NaN.  Places behind a sequence's last token stay as they were."""
     proj, device = qkv.tensor, _current_device()
-    n_seqs, tokens = seq_past.shape[0], proj.shape[1]
-    num_heads = q_out.shape[1]
+    n_seqs, tokens = seq_past.numel(), proj.shape[1]
+    num_heads = q_out.shape[1] if q_out.dim() == 3 else 0
     k = cache.k
     _, kv_heads, _, head_dim = k.shape
     # one expression for a call that is in order: the host's part of a short step is its time
@@ -1896,8 +1896,10 @@ _WRITE8_CALL = struct.Struct("@Pq12Pd14i")
 
 def _check_write_cache8(qkv, q_out, cache, seq_start, seq_past, block_table, max_q_len, q_weight, k_weight, cos_sin) -> None:
     """The refusal of a call that is not in order."""
+    if q_out.dim() != 3 or block_table.dim() != 2:
+        raise KernelError(f"qkv_write_cache8: q_out {tuple(q_out.shape)}, a block table {tuple(block_table.shape)}")
     tokens, num_heads, head_dim = q_out.shape
-    n_seqs = seq_past.shape[0]
+    n_seqs = seq_past.numel()
     _need(q_out, "q_out", shape=(tokens, num_heads, cache.head_dim))
     _code(q_out, "q_out")
     _code(qkv.tensor, "qkv")
@@ -2013,7 +2015,7 @@ def attention_decode_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, b
 
 def _check_decode_cache8(q, cache, out, block_table, seq_len, plan, part_acc, part_ml) -> None:
     """The refusal of a call that is not in order."""
-    _check_cache8("attention_decode_cache8", q, cache, out, block_table, q.shape[0])
+    _check_cache8("attention_decode_cache8", q, cache, out, block_table, q.shape[0] if q.dim() else 0)
     _need(seq_len, "seq_len", torch.int32, q.shape[:1])
     if tuple(q.shape) != tuple(plan.q_shape) or q.dtype != plan.dtype or cache.kv_heads != plan.num_kv_heads:
         raise KernelError(f"attention_decode_cache8: a plan for {plan.q_shape} over {plan.num_kv_heads} kv heads, {plan.dtype}; queries {tuple(q.shape)} over {cache.kv_heads}, {q.dtype}")
@@ -2085,7 +2087,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
     of ``ranges`` blocks, up to eight; the default is ``prefill8_plan``'s choice, by ``max_context``, the most keys that a sequence has (any number gives right
     results; without it what ``block_table`` has room for).  A value
     that is not a number makes its element NaN in the results of the queries that see it, a key that is not one all their elements; earlier queries of the call are as without."""
-    n_seqs, device, k = seq_past.shape[0], _current_device(), cache.k
+    n_seqs, device, k = seq_past.numel(), _current_device(), cache.k
     # one expression for a call that is in order
     if not (q.dim() == 3 and q.shape == out.shape and q.dtype is out.dtype and q.dtype in _CODES and q.shape[2] == k.shape[3] and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0
             and block_table.dim() == 2 and block_table.shape[0] == n_seqs and block_table.shape[1] > 0 and seq_past.dim() == 1 and seq_start.shape == (n_seqs + 1,)
@@ -2113,7 +2115,7 @@ def attention_prefill_cache8(q: torch.Tensor, cache: Cache8, out: torch.Tensor, 
 
 def _check_prefill_cache8(q, cache, out, block_table, seq_start, seq_past, max_q_len) -> None:
     """The refusal of a call that is not in order."""
-    n_seqs = seq_past.shape[0]
+    n_seqs = seq_past.numel()
     _check_cache8("attention_prefill_cache8", q, cache, out, block_table, n_seqs)
     _need(seq_past, "seq_past", torch.int32, (n_seqs,))
     _need(seq_start, "seq_start", torch.int32, (n_seqs + 1,))

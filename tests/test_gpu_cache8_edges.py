@@ -179,3 +179,27 @@ def test_sizes_beyond_what_tcgen05_takes_go_to_the_other_form(monkeypatch):
             assert torch.equal(call(None), want)
             with pytest.raises(kernels.KernelError, match="impl='tc'"):
                 call("tc")
+
+
+def test_operands_of_another_rank_are_refused():
+    """As every other call that is not in order: with a KernelError, before anything is launched."""
+    from qwen_triton_b200.ops import kernels
+    cache = kernels.cache8(2, 1, 64, "cuda")
+    q, out = (torch.zeros((2, 1, 64), device="cuda") for _ in range(2))
+    qkv, table, start, past = kernels.GemmOut(torch.zeros((1, 2, 192), device="cuda")), _ints([[0], [1]]), _ints([0, 1, 2]), _ints([0, 0])
+    plan = kernels.decode8_plan(2, num_heads=1, num_kv_heads=1, head_dim=64, dtype=F32, max_context=64)
+    weight, rows, x, y = kernels.quantise_weight_fp8(torch.zeros((64, 32), device="cuda")), kernels.fp8_rows(2, 32, "cuda"), torch.zeros((2, 32), device="cuda"), torch.zeros((2, 64), device="cuda")
+    calls = [(lambda *a: kernels.qkv_write_cache8(qkv, a[0], cache, *a[1:], 1, None, None, 1e-6, None), (q, start, past, table)),
+             (lambda *a: kernels.attention_prefill_cache8(a[0], cache, *a[1:], 1, 0.1), (q, out, table, start, past)),
+             (lambda *a: kernels.attention_decode_cache8(a[0], cache, *a[1:], 0.1, plan), (q, out, table, past)),
+             (lambda *a: kernels.gemm_fp8(a[0], weight, a[1], rows), (x, y))]
+    before = kernels.launch_count()
+    for call, operands in calls:
+        for i, operand in enumerate(operands):
+            for other in (operand[None], operand.reshape(-1), operand.reshape(-1)[0]):
+                if other.shape != operand.shape:
+                    with pytest.raises(kernels.KernelError):
+                        call(*operands[:i], other, *operands[i + 1:])
+    assert kernels.launch_count() == before
+    for call, operands in calls:
+        call(*operands)
