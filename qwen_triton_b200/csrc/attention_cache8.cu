@@ -14,7 +14,7 @@
 // Weights are held times 2^11, at most 2^15, so that one down to 2^-25 of the largest keeps a half's eleven digits, and what is smaller is off by at most 2^-36 of the
 // largest.  FLOAT: the second half is what the first one leaves, times 2^11 and with sums of its own, so that it too has its digits: 2^-24 of a weight, or 2^-47 of the largest.
 //
-// A value that is not a number, in a portion that not every row sees, is taken out and noted: its element becomes NaN in the rows that see it, and in no other.
+// A value that is not a number, of a key that not every row sees, is taken out and noted: its element becomes NaN in the rows that see it, and in no other.
 //
 // Ranges of a sequence join in the cluster that they form (up to eight), or through memory and a second launch.
 //
@@ -103,11 +103,10 @@ template <int D> struct Ring {
     __device__ static int at(int r, int c) { return r * D + ((D == 64 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 4); }
 };
 
-// A warp's values of a portion from key `key0` on: NaN become zeros, and the first key of each element is noted.
-template <int D> __device__ __forceinline__ void take_out_nan(uint8_t* values, int key0, int* first_nan) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll 2
-    for (int i = lane; i < Ring<D>::HALF / 16; i += 32) {
+// Of a warp's values of a portion from key `key0` on, rows `from` to `to`: NaN become zeros, and the first key of each element is noted.
+template <int D> __device__ __forceinline__ void take_out_nan(uint8_t* values, int from, int to, int key0, int* first_nan) {
+#pragma unroll 1
+    for (int i = from * Ring<D>::PIECES + (threadIdx.x & 31); i < to * Ring<D>::PIECES; i += 32) {
         uint32_t* words = reinterpret_cast<uint32_t*>(values + Ring<D>::at(i / Ring<D>::PIECES, i % Ring<D>::PIECES));
         const uint4 w = *reinterpret_cast<const uint4*>(words);
         if (!(any_nan(w.x) | any_nan(w.y) | any_nan(w.z) | any_nan(w.w))) continue;
@@ -116,6 +115,7 @@ template <int D> __device__ __forceinline__ void take_out_nan(uint8_t* values, i
             const uint32_t word = words[b >> 2];
             if ((word >> (8 * (b & 3)) & 0x7f) != 0x7f) continue;
             words[b >> 2] = word & ~(0xffu << (8 * (b & 3)));
+            first_nan[D] = 1;
             atomicMin(first_nan + i % Ring<D>::PIECES * 16 + b, key0 + i / Ring<D>::PIECES);
         }
     }
@@ -133,10 +133,10 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
     constexpr int KPIECES = D / 64;                        // of a key row, a lane's pieces: KPIECES t + c (of 64 elements: t)
     constexpr int VBYTES = D / 8;                          // of a value row, a lane's neighbouring elements
     extern __shared__ __align__(128) uint8_t shared[];
-    __shared__ int first_nan[D];                           // prompts: of each element, the first key taken out
+    __shared__ int first_nan[D + 1];                       // prompts: of each element, the first key taken out; whether there is one
     pdl_launch_dependents();
     if (p.seq_start) {
-        for (int i = threadIdx.x; i < D; i += 32 * WARPS) first_nan[i] = 0x7fffffff;
+        for (int i = threadIdx.x; i <= D; i += 32 * WARPS) first_nan[i] = i < D ? 0x7fffffff : 0;
         __syncthreads();
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -270,10 +270,10 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
         copies_wait<STAGES - 1>();
         __syncwarp();
         const uint8_t* stage = ring + s_at * R::STAGE;
+        const int key0 = u * KEYS;
         s_at = s_at == STAGES - 1 ? 0 : s_at + 1;
         const float2 scales = *reinterpret_cast<const float2*>(stage + 2 * R::HALF);
         const float f0 = factor0 * scales.x, f1 = factor1 * scales.x, lift = log2f(scales.y), out_of = 1.f / scales.y;
-        const int key0 = u * KEYS;
         float s[SUBS][4];
 #pragma unroll
         for (int v = 0; v < SUBS; ++v) {
@@ -299,7 +299,8 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (key0 + 16 * v + g + 8 * (i >> 1) >= ((i & 1) ? limit1 : limit0)) s[v][i] = -INFINITY;
-            if (p.seq_start && key0 + KEYS > least) take_out_nan<D>(const_cast<uint8_t*>(stage) + R::HALF, key0, first_nan);
+            if (p.seq_start && key0 + KEYS > least)         // (a value that every row sees makes its element NaN in all of them by itself)
+                take_out_nan<D>(const_cast<uint8_t*>(stage) + R::HALF, max(least - key0, 0), min(end - key0, KEYS), key0, first_nan);
         }
         float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
@@ -392,6 +393,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
         *reinterpret_cast<float2*>(own + (2 * t + 1) * D + 2 * i) = make_float2(acc[i][1], acc[i][3]);
     }
     __syncthreads();
+    const bool some_nan = p.seq_start && first_nan[D];
     for (int i = threadIdx.x; i < ROWS * p.d; i += 32 * WARPS) {
         const int r = i / p.d, c = i % p.d, row = row0 + r;
         if (row > last_row) break;
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 || D > 128 ? 2 : 3)
             a = fmaf(parts[(w * ROWS + r) * D + c], by, a);
         }
         const int head = kvh * group + row % group;
-        if (p.seq_start && first_nan[c] <= past + row / group) a = NAN;
+        if (some_nan && first_nan[c] <= past + row / group) a = NAN;
         if (JOIN == ALONE) {
             ((T*)p.out)[((size_t)(token0 + row / group) * p.nq + head) * p.d + c] = from_float<T>(l == 0.f ? 0.f : a / l);
         } else if (JOIN == MEMORY) {
