@@ -19,8 +19,10 @@
 // Ranges of a sequence join in the cluster that they form (up to eight), or through memory and a second launch.
 //
 // Bound by the cache's way from memory for many keys (128 sequences of 4,096 tokens, 32 heads over 8 of 128: 181 us, 5.9 TB/s; 48 of 3,000 to 12,000: 130 us, 5.6 TB/s), by the
-// latency of a warp's ring and the join for few (one sequence of 700 tokens, 16 heads over 8: 5.2 us; 8 of 2,048: 13, 5 of them the bytes); in float32, twice the products, by these
-// (5 sequences of 1,500, 16 heads of 96: 12.8 us).
+// latency of a warp's ring and the join for few (one sequence of 700 tokens, 16 heads over 8: 5.1 us; 8 of 2,048: 13, 5 of them the bytes); in float32, twice the products, by these
+// (5 sequences of 1,500, 16 heads of 96: 12.4 us).  Prompts, eight rows a block, walk all keys again for every eight rows: 1,000 tokens behind 2,000, 16 heads over 4, take 404 us with
+// heads of 256 (24 are the products at the rate of 16-bit ones), in float32 232 with heads of 128 and 534 with heads of 256, where a few registers spill (on tcgen05 heads of 128 take
+// 46 in bfloat16).
 #include "cache8_call.h"
 #include "fp8.cuh"
 

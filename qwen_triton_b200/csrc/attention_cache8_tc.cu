@@ -2,7 +2,7 @@
 //
 //   S = Q K^T        tcgen05.mma kind::f8f6f4.  The keys are 8-bit numbers as they lie in the cache.  A query row times a power of two is the sum of two such numbers:
 //                    the nearest one and the nearest to what is left, which hold a bfloat16 number's eight digits but for elements below 2^-8 of the row's
-//                    largest (these are off by at most 2^-18 of it).  Twice the products at twice the rate of 16-bit ones, and no key is converted.
+//                    largest (these are off by at most 2^-17 of it: the largest lies from 2^7 on, the second number ends at 2^-9 and may be off by 2^-10).  Twice the products at twice the rate of 16-bit ones, and no key is converted.
 //   P = softmax(S)   a thread a row, in registers; the powers of two and the page's scales are factors on the scores
 //   O += P V         tcgen05.mma kind::f16.  P is halves in tensor memory; the values are brought to halves, which hold every 8-bit number, by four warps on their way
 //                    from one shared-memory tile to another, once for the block's 256 rows.  (Both as 8-bit numbers, P in two, would need no conversion of
@@ -21,11 +21,11 @@
 // that see it, and in no other.
 //
 // Few blocks behind many keys: the pages of a block are cut into ranges for a cluster of up to eight, whose sums meet in distributed shared memory, laid over the
-// operands (256 tokens of 32 heads over 8 of 128 behind 8,000: 149 us in one range, 51 in four; 64 tokens 145 and, in eight, 34).
+// operands (256 tokens of 32 heads over 8 of 128 behind 8,000: 158 us in one range, 56 in four; 64 tokens 154 and, in eight, 37).
 //
-// What bounds it: a page of a block takes 1,900 cycles, of which the tensor cores are asked for 1,600: the products of scores run at half their rate, their queries on the way
-// from shared memory (66 cycles for 128 x 64 x 32, of which the tensor cores need 32).  4,096 tokens behind 8,192, 32 heads over 8 of 128: 712-770 us as clocks are, 965-890
-// TFLOP/s; the same over a 16-bit cache, attention_tc.cu, 734.  What was tried on it: two pages at a time, which halve the queries' way, but leave room for one sum a row, so
+// What bounds it: a page of a block takes some 1,950 cycles, of which the tensor cores are asked for 1,600: the products of scores run at half their rate, their queries on the way
+// from shared memory (66 cycles for 128 x 64 x 32, of which the tensor cores need 32).  4,096 tokens behind 8,192, 32 heads over 8 of 128: 744-791 us as clocks are, 925-870
+// TFLOP/s; the same over a 16-bit cache, attention_tc.cu, 734.  What was tried on it (figures of before the weights were lifted): two pages at a time, which halve the queries' way, but leave room for one sum a row, so
 // that the two threads of a row walk in step (739 in the place of 712); half of the queries in tensor memory, with scores buffered once (810 in the place of 729, and with
 // heads of 64 695 in the place of 620); an eighth of the exponentials on the FMA pipe (no change, more of them slower); other orders of the products than a tile's next
 // scores, then its values, tile by tile (both tiles' scores first 785, values first 850, whatever is ready 758).

@@ -176,7 +176,9 @@ __device__ __forceinline__ uint2 smaller8(uint2 w, float by) {
 }
 // grid: (2 nkv + nq heads, pages that a sequence's tokens touch, sequences).  A row of L lanes a token; what is to be held stays in registers between
 // the page's largest number and the write.  Bound by latency and instructions (15 an element): all rows' elements are asked for first, and four blocks an SM
-// (some registers spilled) hide more of it than three (3,600 tokens of 32 + 8 + 8 heads of 128 in bfloat16: 28.5 us, 2.9 TB/s, with three blocks 30.2; asked for row by row 43).
+// hide more of it than three (3,600 tokens of 32 + 8 + 8 heads of 128 in bfloat16: 28.5 us, 2.9 TB/s, with three blocks 30.2; asked for row by row 43).  Four blocks leave 64 registers a
+// thread: heads of 65 to 128 spill 56 bytes of them at most, heads of 129 to 256, whose rows are whole warps', 1.1 to 1.2 KB, which they pay for (heads of 256: 88 us for twice the
+// bytes of 33, in float32 125).
 template <int L, typename TI, typename TO>
 __global__ void __launch_bounds__(THREADS, 4) write_pages_kernel(const WriteParams p) {
     constexpr int ROWS = THREADS / L, ITERS = (PAGE + ROWS - 1) / ROWS;
@@ -239,7 +241,9 @@ __global__ void __launch_bounds__(THREADS, 4) write_pages_kernel(const WritePara
     }
 }
 
-// One token a sequence at most: a row of L lanes a (sequence, head).  Bound by one launch's latency (64 sequences of 32 + 8 + 8 heads of 128: 3.1 us).
+// One token a sequence at most: a row of L lanes a (sequence, head).  Bound by one launch's latency where no scale grows (64 sequences of 32 + 8 + 8 heads of 128: 3.1 us).  Where one does,
+// its lanes bring the page's earlier rows under it one after the other, 0.6 us a row, and the launch takes as long as its longest page: 18 us more with 32 earlier rows, 37 with 63,
+// for one sequence as for 64.
 template <int L, typename TI, typename TO>
 __global__ void __launch_bounds__(THREADS) write_tokens_kernel(const WriteParams p) {
     pdl_launch_dependents();

@@ -90,7 +90,7 @@ template <int N> __device__ __forceinline__ void quantise_neighbours(const float
     if constexpr (N == 16) *reinterpret_cast<uint4*>(to) = make_uint4(out[0], out[1], out[2], out[3]);
     else *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
 }
-// Rows in 8 bits, scales as [group, row], bound by memory where there are many: a lane 16 columns, eight lanes a group, a warp 512 columns of a row, a block eight
+// Rows in 8 bits, scales as [group, row], bound by instructions (73 % of the issue slots) where there are many: a lane 16 columns, eight lanes a group, a warp 512 columns of a row, a block eight
 // rows, whose scales lie side by side.  4096 rows of 12288 in bfloat16: 33 us (4.6 TB/s), where four columns a lane, a warp a group and CUDA's division took 76; 333 of
 // 8192: 3.1 (5.1); 8 of 4096: 1.8 (1.6); with eight columns a lane 41, 3.3 and 1.6.
 template <typename T>
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) quantise_rows_wide_kernel(const T* x, uin
     quantise_neighbours(v, values, scales, rows, k, m, c0, c0 < k);
 }
 // The same of act(gate) * up, rounded to T first as the activation by itself leaves it: of a row of 2 k numbers, gate then up (group 0) or `group` of each in turns.
-// Eight columns a lane: its instructions and exponentials bound it as much as memory (4096 rows of 2 * 12288 in bfloat16 71 us, 3.6 TB/s, where the activation and the rows to
+// Eight columns a lane: its instructions (76 % of the issue slots) and exponentials (55 % of their pipe) bound it more than memory (4096 rows of 2 * 12288 in bfloat16 71 us, 3.6 TB/s, where the activation and the rows to
 // 8 bits take 97 in two launches; 8 rows 2.6 and 3.7; with 16 columns a lane 88 and 4.7).
 template <typename T>
 __global__ void __launch_bounds__(256) gated_rows_kernel(const T* gate_up, uint8_t* values, float* scales, int rows, int k, int group, int act, float limit) {
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(256) quantise_rows_kernel(const T* x, uint8_t*
 }
 
 // A weight's block of 128 x 128, one scale for all of it, by a block of eight warps: a lane 16 neighbours of four rows, which stay in registers between the block's
-// largest number and the write.  Bound by memory (24576 x 4096 from bfloat16: 127 us, read twice and divided element by element 262).
+// largest number and the write.  Bound by latency: 127 registers leave two blocks an SM, 24 % of its warps, and each waits for all of its reads before its first write (24576 x 4096 from
+// bfloat16: 127 us, 2.4 TB/s; read twice and divided element by element 262).
 __device__ __forceinline__ float block_scale(float largest, float* most) {
     largest = warp_max(largest);
     if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = largest;
@@ -638,7 +639,7 @@ __global__ void __launch_bounds__(Few<BX, XT>::THREADS) gemm_fp8_few_kernel(cons
 //
 // Bound by the operands' way from the L2 cache: a group of a tile is 48 KB for 520 cycles of products and takes 0.57 us, 12.5 TB/s to all SMs (4096 rows of 51200 x 5120:
 // 1,150 us, 1.87 PFLOP/s).  With fewer blocks it takes 0.42 us, the way round of one of the two accumulators: products, commit, eight reads of 16 columns, release.  Tiles of
-// 256 x 256 by pairs of blocks (a third less to fetch) were no faster, their two SMs waiting for each other; reads of 32 columns spill.
+// 256 x 256 by pairs of blocks (a third less to fetch) were tried only while the sums still spilled: 2,048 rows 210 us, these tiles then 220, more rows slower.  Reads of 32 columns spill.
 constexpr int BN = 256, PARK_ROW = BN + 4;                  // floats from a row of parked sums to the next: 16 bytes of eight neighbouring rows are all the banks
 constexpr int MANY_THREADS = 384, MANY_STAGES = 4, MANY_SLOTS = 512 / BN, MANY_CW = BN / 2;
 constexpr uint32_t MANY_STAGE_BYTES = A_BYTES + BN * GROUP;

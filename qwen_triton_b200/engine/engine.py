@@ -55,7 +55,8 @@ def require_gpu(device: torch.device) -> None:
 def check_formats(spec: ModelSpec, weight_format: str | None, cache_format: str | None) -> dict[str, str]:
     """What the parts are told of ``weight_format`` and ``cache_format``: None keeps the compute type, "fp8" the weights of attention's and the feed-forward's
     projections as 8-bit numbers with a scale for each block of 128 x 128 (their rows are brought to 8 bits too), or keys and values with a scale for each
-    page and head.  Models of dense attention and gated feed-forwards take them; parts that do not say so themselves."""
+    page and head (half the memory; steps of few sequences take as long as over a 16-bit cache or a little longer, the fused write being the latter's).  Models of dense
+    attention and gated feed-forwards take them; parts that do not say so themselves.  ``cache_format`` also wants every layer call to have a cache entry of its own."""
     formats = {name: given for name, given in (("weight_format", weight_format), ("cache_format", cache_format)) if given is not None}
     for name, given in formats.items():
         if given != "fp8":

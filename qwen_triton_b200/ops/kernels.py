@@ -1606,7 +1606,8 @@ E4M3 = torch.float8_e4m3fn
 @dataclass(frozen=True)
 class Fp8Weight:
     """A weight [N, K] of 8-bit numbers: ``values`` (e4m3) times ``scales`` [ceil(N / 128), ceil(K / 128)] (float), one for each block of 128 x 128.
-    ``quantise_weight_fp8`` makes one; a checkpoint's values and scales of that form are taken as they are."""
+    ``quantise_weight_fp8`` makes one; a caller's own values and scales of that form are taken as they are.  (Models quantise what they load: no loader reads 8-bit weights from
+    a file, and the layers lay q, k, v and gate, up into one weight each, whose blocks are not a file's.)"""
 
     values: torch.Tensor
     scales: torch.Tensor
@@ -2040,8 +2041,8 @@ def prefill8_plan(n_seqs: int, max_q_len: int, *, num_heads: int, num_kv_heads: 
     for each number of ranges, fitted to 57 shapes with 1 to 8 ranges on both (its choice is within 8 % of their best for all but nine, at worst 25 %).
 
     tcgen05 walks a page for 128 or 256 rows in 0.85 to 1.1 us, one block an SM; clusters of 3 and more do not fill all SMs.  On mma.sync a tile of eight rows takes
-    0.3 to 0.7 us a page by itself and longer beside others.  64 tokens of 32 heads over 8 of 128, mma.sync / tcgen05, each with its best ranges: behind 8,000 tokens 87 / 34 us, behind 500
-    14 / 19; 8 tokens behind 8,000 20 / 23; 256 tokens behind 8,000 on tcgen05 in one range / four 149 / 51."""
+    0.3 to 0.7 us a page by itself and longer beside others.  64 tokens of 32 heads over 8 of 128, mma.sync / tcgen05, each with its best ranges: behind 8,000 tokens 90 / 37 us, behind 500
+    15 / 22; 8 tokens behind 8,000 21 / 24; 256 tokens behind 8,000 on tcgen05 in one range / four 158 / 56."""
     group, wide, single = num_heads // num_kv_heads, head_dim > 64, dtype == torch.float32
     on_tc = on_tc and not single and head_dim <= 128
     best = None
